@@ -538,6 +538,104 @@ int lg_ep_advance(void* arena, void* stream);
 /* Status word of an arena (0 = ok). Synchronous; reset != 0 clears it. */
 int lg_ep_status(const void* arena, int reset, int* status);
 
+/* ---------------------------------------------------------------------------------------
+ * Paged K/V cache: pages of R rows that streams name through a table, the operations on the
+ * pages, and the attention that reads them. No counterpart in the reference, whose caches hold
+ * one sequence each in one buffer (laguna_mlx/cache.py:66-157).
+ *
+ * A pool holds `planes` planes (one layer's K or V each) of P pages [H, R, row_bytes]. Page p of
+ * every plane belongs together: row j of stream s lies in row j % R of page table[s, j / R] of
+ * every plane. State on the device: table int32 [S, M] (page ids from column 0 on, -1 past them),
+ * lens int32 [S] (rows held), refs int32 [P] (how many streams name the page; 0: free).
+ * Calls that change one state must be ordered by the caller (one stream).
+ *
+ * Each operation checks its lists on the device; one whose check fails changes nothing.
+ * status int32 [2]: {LG_PAGES_*, count} with the count of pages taken (reserve, fork), streams
+ * freed, or pages moved. Pages are taken lowest id first in the order of the call's list.
+ * Workspace: lg_pages_workspace_bytes(P, n) for a list of n (compact: n = 0).
+ * ------------------------------------------------------------------------------------- */
+enum {
+  LG_PAGES_OK = 0,
+  LG_PAGES_NONE_FREE = 1,  /* not enough free pages */
+  LG_PAGES_BAD_STREAM = 2, /* a stream outside [0, S), listed twice, or a fork's child that holds
+                              pages or is a source too */
+  LG_PAGES_TABLE_FULL = 3, /* more rows than a table row's M pages hold */
+  LG_PAGES_BAD_PAGE = 4    /* a page id outside [0, P) or a negative count */
+};
+
+size_t lg_pages_workspace_bytes(int P, int n);
+
+/* Each stream ids[i] (device int32 [n], distinct) gets pages for rows[i] rows in all; those it has
+ * stay. */
+int lg_pages_reserve(int32_t* table, int32_t* refs, int S, int M, int P, int R,
+                     const int32_t* ids, const int32_t* rows, int n, int32_t* status,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* The streams ids[i] give their pages back: refs - 1, table row -1, length 0. */
+int lg_pages_free(int32_t* table, int32_t* lens, int32_t* refs, int S, int M, int P,
+                  const int32_t* ids, int n, int32_t* status, void* stream);
+
+/* Child dst[i] (an empty stream) becomes a copy of stream src[i]: it shares the whole pages
+ * (refs + 1) and gets a page of its own for a part-filled last one, whose rows below the length
+ * are copied in every plane. Pages that the source holds beyond its length are not shared.
+ * row_bytes a multiple of 16; the pool 16-byte aligned, [planes, P, H, R, row_bytes]. */
+int lg_pages_fork(void* pool, int planes, int H, int R, int row_bytes, int32_t* table,
+                  int32_t* lens, int32_t* refs, int S, int M, int P, const int32_t* src,
+                  const int32_t* dst, int n, int32_t* status, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
+/* Live pages move to the lowest ids: with n live pages, those with id >= n go, in ascending order,
+ * to the free ids below n, whole, in every plane; table and refs name them anew. */
+int lg_pages_compact(void* pool, int planes, int H, int R, int row_bytes, int32_t* table,
+                     int32_t* refs, int S, int M, int P, int32_t* status, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/*
+ * Plans: how a batch's attention work is divided over the GPU, computed on the device from the
+ * lengths. A plan serves every layer with the same heads, page rows and window; it also holds the
+ * partial results of a call, so two calls that can overlap on the GPU need a plan each.
+ * The buffer: 256-byte aligned, lg_prompt_plan_bytes / lg_stream_plan_bytes of the current device.
+ */
+size_t lg_prompt_plan_bytes(int T, int B, int Hq, int Hkv);
+size_t lg_stream_plan_bytes(int B, int Hq, int Hkv);
+
+/* B sequences' new tokens, packed: tokens [cu_q[b], cu_q[b + 1]) (device int32 [B + 1], ascending,
+ * at most T) are the newest of the kv_len[b] rows (device int32 [B]) that sequence b holds, its
+ * newest row included. window > 0: a token sees its own and the window - 1 rows before. */
+int lg_prompt_plan(const int32_t* cu_q, const int32_t* kv_len, int B, int T, int Hq, int Hkv,
+                   int page_rows, int window, void* plan, size_t plan_bytes, void* stream);
+
+/* One token of each of B streams, the newest of its kv_len[b] rows. Rows [0, prefix) are the same
+ * for every stream that has them (the same pages, or copies): they are read once for all. A
+ * stream with kv_len[b] == 0 sees no key. */
+int lg_stream_plan(const int32_t* kv_len, int B, int Hq, int Hkv, int page_rows, int prefix,
+                   int window, void* plan, size_t plan_bytes, void* stream);
+
+/*
+ * Causal attention of packed prompts (the SDPA branch of Attention.__call__, laguna.py:102-107,
+ * for several sequences at once): token t at position p, head h, kv head h / (Hq / Hkv):
+ *   out = bf16(bf16(sum_j softmax_j(scale q . k_j) v_j) * gate),  max(0, p - window + 1) <= j <= p
+ * and 0 for a token without keys. q bf16 [T, Hq, 128] with element strides q_tok, q_head; k_pages,
+ * v_pages bf16 [P, Hkv, R, 128] with one set of element strides; table int32 [B, M]; gate bf16
+ * [T, Hq] or NULL; out bf16 [T, Hq, 128], whose rows outside [cu_q[0], cu_q[B]) stay as they were.
+ * R in {16, 32, 64, 128}; Hq % Hkv == 0, Hq / Hkv <= 16; scale > 0; pointers 16-byte aligned,
+ * strides multiples of 8 elements. Rows of a sequence below its length are finite; what lies in
+ * its pages past the length does not matter. A sequence whose table names no page of the pool
+ * for a row it needs gives NaN.
+ */
+int lg_prompt_attention(const void* q, long long q_tok, long long q_head, int T, int Hq, int Hkv,
+                        int D, const void* k_pages, const void* v_pages, int P, int R,
+                        long long page_stride, long long head_stride, long long row_stride,
+                        const int32_t* table, int B, int M, float scale, const void* gate,
+                        void* out, void* plan, size_t plan_bytes, void* stream);
+
+/* The same for one token of each of B streams (q [B, Hq, 128], table [B, M]). */
+int lg_stream_attention(const void* q, long long q_tok, long long q_head, int B, int Hq, int Hkv,
+                        int D, const void* k_pages, const void* v_pages, int P, int R,
+                        long long page_stride, long long head_stride, long long row_stride,
+                        const int32_t* table, int M, float scale, const void* gate, void* out,
+                        void* plan, size_t plan_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,8 @@ LG_OK, LG_ERR_INVALID, LG_ERR_UNSUPPORTED, LG_ERR_CUDA, LG_ERR_WORKSPACE = range
 LG_SCORE_SIGMOID, LG_SCORE_SOFTMAX = 0, 1
 LG_PATH_AUTO, LG_PATH_GEMV, LG_PATH_TENSOR = 0, 1, 2
 LG_MOE_GEMV_MAX_ROWS = 768
+(LG_PAGES_OK, LG_PAGES_NONE_FREE, LG_PAGES_BAD_STREAM, LG_PAGES_TABLE_FULL,
+ LG_PAGES_BAD_PAGE) = range(5)
 
 P = c_void_p
 I = c_int
@@ -91,6 +93,20 @@ SIGNATURES = {
     "lg_ep_advance": (c_int, [P, P]),
     "lg_moe_decode": (c_int, [P, P, P, I, I, I, I, c_float, P, P, P, P, P, P, P, P, P, I,
                               P, P, P, P, P, P, P, P, P, P, P, P, c_size_t, P]),
+    "lg_pages_workspace_bytes": (c_size_t, [I, I]),
+    "lg_pages_reserve": (c_int, [P, P, I, I, I, I, P, P, I, P, P, c_size_t, P]),
+    "lg_pages_free": (c_int, [P, P, P, I, I, I, P, I, P, P]),
+    "lg_pages_fork": (c_int, [P, I, I, I, I, P, P, P, I, I, I, P, P, I, P, P, c_size_t, P]),
+    "lg_pages_compact": (c_int, [P, I, I, I, I, P, P, I, I, I, P, P, c_size_t, P]),
+    "lg_prompt_plan_bytes": (c_size_t, [I, I, I, I]),
+    "lg_stream_plan_bytes": (c_size_t, [I, I, I]),
+    "lg_prompt_plan": (c_int, [P, P, I, I, I, I, I, I, P, c_size_t, P]),
+    "lg_stream_plan": (c_int, [P, I, I, I, I, I, I, P, c_size_t, P]),
+    "lg_prompt_attention": (c_int, [P, c_longlong, c_longlong, I, I, I, I, P, P, I, I, c_longlong,
+                                    c_longlong, c_longlong, P, I, I, c_float, P, P, P, c_size_t,
+                                    P]),
+    "lg_stream_attention": (c_int, [P, c_longlong, c_longlong, I, I, I, I, P, P, I, I, c_longlong,
+                                    c_longlong, c_longlong, P, I, c_float, P, P, P, c_size_t, P]),
 }
 
 _lib = None

@@ -617,3 +617,229 @@ def argmax(logits, ids=None, pos=None, inc=1):
     _lib.call("lg_argmax", _p(l2), l2.shape[0], V, _p(ids), _p(pos), int(inc),
               _stream(logits.device))
     return ids
+
+
+# ---------------------------------------------------------------------------------------
+# Paged K/V cache: page operations, plans and attention (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------
+
+PAGES_ERRORS = {
+    _lib.LG_PAGES_NONE_FREE: "not enough free pages",
+    _lib.LG_PAGES_BAD_STREAM: "a stream out of range, listed twice, or a fork's child that holds "
+                              "pages or is a source too",
+    _lib.LG_PAGES_TABLE_FULL: "more rows than a stream's table row holds",
+    _lib.LG_PAGES_BAD_PAGE: "a page outside the pool",
+}
+
+
+def _call_on(device, name, *args):
+    """``_lib.call`` with ``device`` current (kernels launch on the current device)."""
+    if torch.cuda.current_device() == device.index:
+        return _lib.call(name, *args)
+    with torch.cuda.device(device):
+        return _lib.call(name, *args)
+
+
+def _i32(t, name, dims, device):
+    """A contiguous int32 tensor of ``dims`` dimensions on ``device``, updated in place by the
+    page operations, so never copied."""
+    if _dev(t) != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {dims} dimension(s)")
+    return t
+
+
+def _state(table, refs, lens=None):
+    dev = _dev(table)
+    S, M = _i32(table, "table", 2, dev).shape
+    P = _i32(refs, "refs", 1, dev).shape[0]
+    if lens is not None and _i32(lens, "lens", 1, dev).shape[0] != S:
+        raise ValueError(f"lens holds {lens.shape[0]} streams, table {S}")
+    return dev, S, M, P
+
+
+def _pool(pool, dev, P):
+    """(planes, heads, rows, row bytes) of a page pool [..., P, H, R, D]."""
+    if _dev(pool) != dev:
+        raise ValueError(f"the pool is on {pool.device}, not on {dev}")
+    if pool.dim() < 4 or not pool.is_contiguous():
+        raise ValueError("the pool must be a contiguous tensor [..., pages, heads, rows, dim]")
+    p, h, r, d = pool.shape[-4:]
+    if p != P:
+        raise ValueError(f"the pool holds {p} pages, refs {P}")
+    return pool.numel() // max(p * h * r * d, 1), h, r, d * pool.element_size()
+
+
+def _ids(ids, name, dev):
+    ids = _i32(ids if ids.is_contiguous() else ids.contiguous(), name, 1, dev)
+    return ids, ids.shape[0]
+
+
+def _pages_ws(dev, P, n):
+    """A workspace of this call's own: an operation's list of moves must not be another's."""
+    nb = _lib.lib().lg_pages_workspace_bytes(P, n)
+    return torch.empty(nb, dtype=torch.uint8, device=dev), nb
+
+
+def pages_reserve(table, refs, ids, rows, page_rows):
+    """Pages for ``rows[i]`` rows in all of each stream ``ids[i]`` (device int32 [n], distinct),
+    lowest free ids first; pages a stream has stay. ``table`` int32 [S, M] and ``refs`` int32 [P]
+    are updated in place. Returns status int32 [2] on the device: (0 or a key of
+    ``PAGES_ERRORS``, pages taken); on an error nothing has changed."""
+    dev, S, M, P = _state(table, refs)
+    (ids, n), (rows, m) = _ids(ids, "ids", dev), _ids(rows, "rows", dev)
+    if n != m:
+        raise ValueError(f"{n} streams, {m} row counts")
+    status = torch.empty(2, dtype=torch.int32, device=dev)
+    ws, nb = _pages_ws(dev, P, n)
+    _call_on(dev, "lg_pages_reserve", _p(table), _p(refs), S, M, P, int(page_rows), _p(ids),
+             _p(rows), n, _p(status), _p(ws), nb, _stream(dev))
+    return status
+
+
+def pages_free(table, lens, refs, ids):
+    """The streams ``ids`` give their pages back (counts - 1, table rows -1, lengths 0). Returns
+    status int32 [2]: (0 or a key of ``PAGES_ERRORS``, streams freed)."""
+    dev, S, M, P = _state(table, refs, lens)
+    ids, n = _ids(ids, "ids", dev)
+    status = torch.empty(2, dtype=torch.int32, device=dev)
+    _call_on(dev, "lg_pages_free", _p(table), _p(lens), _p(refs), S, M, P, _p(ids), n, _p(status),
+             _stream(dev))
+    return status
+
+
+def pages_fork(pool, table, lens, refs, src, dst):
+    """Stream ``dst[i]`` (empty) becomes a copy of stream ``src[i]``: whole pages are shared, a
+    part-filled last page is copied into a page of the child's own in every plane of ``pool``
+    [..., P, H, R, D]. Returns status int32 [2]: (0 or a key of ``PAGES_ERRORS``, pages taken)."""
+    dev, S, M, P = _state(table, refs, lens)
+    planes, H, R, rb = _pool(pool, dev, P)
+    (src, n), (dst, m) = _ids(src, "src", dev), _ids(dst, "dst", dev)
+    if n != m:
+        raise ValueError(f"{n} sources, {m} children")
+    status = torch.empty(2, dtype=torch.int32, device=dev)
+    ws, nb = _pages_ws(dev, P, n)
+    _call_on(dev, "lg_pages_fork", _p(pool), planes, H, R, rb, _p(table), _p(lens), _p(refs), S, M,
+             P, _p(src), _p(dst), n, _p(status), _p(ws), nb, _stream(dev))
+    return status
+
+
+def pages_compact(pool, table, refs):
+    """Live pages move to the lowest ids of ``pool`` [..., P, H, R, D] (with n live pages those
+    with id >= n go, ascending, to the free ids below n); ``table`` and ``refs`` name them anew.
+    Returns status int32 [2]: (0 or a key of ``PAGES_ERRORS``, pages moved)."""
+    dev, S, M, P = _state(table, refs)
+    planes, H, R, rb = _pool(pool, dev, P)
+    status = torch.empty(2, dtype=torch.int32, device=dev)
+    ws, nb = _pages_ws(dev, P, 0)
+    _call_on(dev, "lg_pages_compact", _p(pool), planes, H, R, rb, _p(table), _p(refs), S, M, P,
+             _p(status), _p(ws), nb, _stream(dev))
+    return status
+
+
+class AttentionPlan:
+    """The division of a batch's paged attention over the GPU (``prompt_plan``, ``stream_plan``).
+    It serves every layer with the same heads, page rows and window, and holds a call's partial
+    results: calls that may overlap on the GPU (another stream, another captured graph) need a
+    plan each. ``update()`` divides anew for the lengths that its tensors hold by then."""
+
+    def __init__(self, kind, cu_q, kv_len, T, Hq, Hkv, page_rows, prefix, window):
+        dev = _dev(kv_len)
+        self.kind, self.T, self.Hq, self.Hkv = kind, int(T), int(Hq), int(Hkv)
+        self.page_rows, self.prefix, self.window = int(page_rows), int(prefix), int(window)
+        self.device = dev
+        self.kv_len = _i32(kv_len, "kv_len", 1, dev)
+        self.B = kv_len.shape[0]
+        self.cu_q = cu_q
+        if kind == "prompt" and _i32(cu_q, "cu_q", 1, dev).shape[0] != self.B + 1:
+            raise ValueError(f"cu_q holds {cu_q.shape[0]} offsets for {self.B} sequences")
+        with torch.cuda.device(dev):
+            self.nbytes = (_lib.lib().lg_prompt_plan_bytes(self.T, self.B, self.Hq, self.Hkv)
+                           if kind == "prompt" else
+                           _lib.lib().lg_stream_plan_bytes(self.B, self.Hq, self.Hkv))
+        self.buf = torch.empty(max(self.nbytes, 256), dtype=torch.uint8, device=dev)
+        self.update()
+
+    def update(self):
+        st = _stream(self.device)
+        if self.kind == "prompt":
+            _call_on(self.device, "lg_prompt_plan", _p(self.cu_q), _p(self.kv_len), self.B, self.T,
+                     self.Hq, self.Hkv, self.page_rows, self.window, _p(self.buf), self.nbytes, st)
+        else:
+            _call_on(self.device, "lg_stream_plan", _p(self.kv_len), self.B, self.Hq, self.Hkv,
+                     self.page_rows, self.prefix, self.window, _p(self.buf), self.nbytes, st)
+        return self
+
+
+def prompt_plan(cu_q, kv_len, T, Hq, Hkv, page_rows, window=0):
+    """A plan for ``prompt_attention``: sequence b's new tokens are rows [cu_q[b], cu_q[b + 1])
+    (device int32 [B + 1]) of T packed ones and the newest of the kv_len[b] rows (device int32
+    [B]) it holds. ``window`` > 0: a token sees its own and the window - 1 rows before."""
+    return AttentionPlan("prompt", cu_q, kv_len, T, Hq, Hkv, page_rows, 0, window)
+
+
+def stream_plan(kv_len, Hq, Hkv, page_rows, prefix=0, window=0):
+    """A plan for ``stream_attention``: one token of each of B streams, the newest of its
+    kv_len[b] rows (device int32 [B]). Rows [0, prefix) are the same for every stream that has
+    them and are read once for all."""
+    return AttentionPlan("stream", None, kv_len, kv_len.shape[0], Hq, Hkv, page_rows, prefix, window)
+
+
+def _paged_attention(kind, q, k_pages, v_pages, table, plan, scale, gate, out):
+    dev = _dev(q)
+    if q.dtype != torch.bfloat16 or k_pages.dtype != torch.bfloat16 or \
+            v_pages.dtype != torch.bfloat16:
+        raise ValueError("q, k_pages and v_pages must be bf16")
+    T, Hq, D = q.shape
+    P, Hkv, R, _ = k_pages.shape
+    if (plan.kind, plan.T, plan.Hq, plan.Hkv, plan.page_rows, plan.device) != \
+            (kind, T, Hq, Hkv, R, dev):
+        raise ValueError(f"the plan is for {plan.kind} attention of {plan.T} tokens, heads "
+                         f"{plan.Hq}/{plan.Hkv}, pages of {plan.page_rows} rows on {plan.device}")
+    ks = k_pages.stride()
+    if k_pages.shape != v_pages.shape or ks != v_pages.stride() or ks[3] != 1 or \
+            k_pages.shape[3] != D:
+        raise ValueError("k_pages and v_pages must have one shape [P, Hkv, R, head_dim] and one "
+                         "set of strides, unit along head_dim")
+    if k_pages.device != dev or v_pages.device != dev:
+        raise ValueError(f"the pages are not on {dev}")
+    B, M = _i32(table, "table", 2, dev).shape
+    if B != plan.B:
+        raise ValueError(f"the table has {B} rows, the plan {plan.B} sequences")
+    qs = q.stride()
+    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or q.data_ptr() % 16:
+        q = q.contiguous().clone() if q.is_contiguous() else q.contiguous()
+        qs = q.stride()
+    if gate is not None:
+        if gate.shape != (T, Hq) or gate.dtype != torch.bfloat16 or _dev(gate) != dev:
+            raise ValueError(f"the gate must be bf16 [{T}, {Hq}] on {dev}")
+        gate = _c(gate)
+    if out is None:
+        out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=dev)
+    elif out.shape != (T, Hq, D) or out.dtype != torch.bfloat16 or _dev(out) != dev or \
+            not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous bf16 tensor [{T}, {Hq}, {D}] on {dev}")
+    a = (_p(q), qs[0], qs[1], T, Hq, Hkv, D, _p(k_pages), _p(v_pages), P, R, ks[0], ks[1], ks[2],
+         _p(table))
+    b = (M, float(scale), _p(gate), _p(out), _p(plan.buf), plan.nbytes, _stream(dev))
+    if kind == "prompt":
+        _call_on(dev, "lg_prompt_attention", *a, B, *b)
+    else:
+        _call_on(dev, "lg_stream_attention", *a, *b)
+    return out
+
+
+def prompt_attention(q, k_pages, v_pages, table, plan, scale, gate=None, out=None):
+    """Causal attention of packed prompts over cache pages. q bf16 [T, Hq, 128]; k_pages, v_pages
+    bf16 [P, Hkv, R, 128] (one layer of a pool) that hold the new tokens' rows already; table int32
+    [B, M]; ``plan`` from ``prompt_plan``; gate bf16 [T, Hq] or None. Returns bf16 [T, Hq, 128]:
+    bf16(attention) * gate per token and head, 0 for a token without keys; with ``out`` given, rows
+    of no sequence stay as they were."""
+    return _paged_attention("prompt", q, k_pages, v_pages, table, plan, scale, gate, out)
+
+
+def stream_attention(q, k_pages, v_pages, table, plan, scale, gate=None, out=None):
+    """``prompt_attention`` for one token of each of B streams (q bf16 [B, Hq, 128], ``plan`` from
+    ``stream_plan``); the plan's shared prefix is read once for all streams."""
+    return _paged_attention("stream", q, k_pages, v_pages, table, plan, scale, gate, out)
