@@ -599,6 +599,10 @@ int lg_pages_compact(void* pool, int planes, int H, int R, int row_bytes, int32_
 size_t lg_prompt_plan_bytes(int T, int B, int Hq, int Hkv);
 size_t lg_stream_plan_bytes(int B, int Hq, int Hkv);
 
+/* 0, or the code of a wait that ran out in a call with this plan (the call then ended with wrong
+ * rows instead of hanging). Synchronous (copies the plan's head to the host). */
+int lg_plan_status(const void* plan, int* status);
+
 /* B sequences' new tokens, packed: tokens [cu_q[b], cu_q[b + 1]) (device int32 [B + 1], ascending,
  * at most T) are the newest of the kv_len[b] rows (device int32 [B]) that sequence b holds, its
  * newest row included. window > 0: a token sees its own and the window - 1 rows before. */

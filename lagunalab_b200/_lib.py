@@ -100,6 +100,7 @@ SIGNATURES = {
     "lg_pages_compact": (c_int, [P, I, I, I, I, P, P, I, I, I, P, P, c_size_t, P]),
     "lg_prompt_plan_bytes": (c_size_t, [I, I, I, I]),
     "lg_stream_plan_bytes": (c_size_t, [I, I, I]),
+    "lg_plan_status": (c_int, [P, ctypes.POINTER(c_int)]),
     "lg_prompt_plan": (c_int, [P, P, I, I, I, I, I, I, P, c_size_t, P]),
     "lg_stream_plan": (c_int, [P, I, I, I, I, I, I, P, c_size_t, P]),
     "lg_prompt_attention": (c_int, [P, c_longlong, c_longlong, I, I, I, I, P, P, I, I, c_longlong,

@@ -3,8 +3,8 @@
 // Work is a list of segments: a row tile of queries (tokens x the G query heads of one kv head)
 // against a range of 128-key tiles. A plan lists the row tiles (each stands for Hkv segments, one
 // per kv head) with the cost that lies before each, and gives every CTA an equal share of the
-// summed cost: CTA c takes the key tiles that start in [c, c + 1) * chunk. A CTA's share may begin
-// and end inside a segment; the parts of a split segment leave partial results that a second
+// summed cost: CTA c takes the key tiles whose cost begins in [c, c + 1) * chunk. A CTA's share may
+// begin and end inside a segment; the parts of a split segment leave partial results that a second
 // kernel joins.
 #pragma once
 
@@ -24,12 +24,24 @@ struct PaTile {
   int pos0;     // PA_PROMPT: position of token q0
   int key0;     // first key, a multiple of the page rows
   int key_end;  // one past the last key that any row sees
-  int ntile;    // ceil((key_end - key0) / 128), at least 1
+  int ntile;    // key tiles: ceil((key_end - key0) / 128), at least 1
+  int ntile0;   // pair: key tiles of the first row tile (at most ntile)
   int kind;
-  int pair;     // 1: two row tiles (2 * tq tokens) share each key tile; 0: one row tile
-  int cost;     // of one segment (one kv head)
+  int pair;  // 1: two row tiles (2 * tq tokens) share each key tile; 0: one row tile
+  int w;     // cost of a key tile
+  int pad;
   long long before;  // cost of all segments before this tile's first
 };
+
+// Costs: half a row tile's worth of tensor-core time on one key tile is 1, so a pair's key tile
+// is 4 and a lone row tile's 2; a stream's own key tile waits for HBM rather than the tensor
+// cores. Every segment costs PA_SEG more (Q load, first score, output).
+constexpr int PA_W_PAIR = 4, PA_W_ONE = 2, PA_W_OWN = 3, PA_SEG = 2;
+constexpr int PA_MIN_CHUNK = 8;  // at least the largest PA_SEG + w: no CTA below the last is idle
+
+__host__ __device__ inline long long pa_cost(int ntile, int w) {
+  return PA_SEG + (long long)ntile * w;
+}
 
 struct PaStart {
   int tile, head, t;  // a CTA's first segment and key tile
@@ -37,8 +49,9 @@ struct PaStart {
 
 struct PaHead {
   long long total, chunk;
-  int ntile_rows, nprefix;  // row tiles, and how many of them are PA_PREFIX
+  int ntiles, nprefix;  // row tiles, and how many of them (the first ones) are PA_PREFIX
   int kind, B, T, Hq, Hkv, R, prefix, window;
+  int err;  // a wait that ran out (its code), else 0
 };
 
 // The parts of a plan buffer.
@@ -48,10 +61,19 @@ struct PaPlan {
   int* kv;         // [B] rows of each sequence
   int* off;        // [B + 1] first row tile of each sequence (prompts)
   PaTile* tiles;   // [max_tiles]
-  char* parts;     // partial results
+  // partial results: per slot, {m, l} of every row, then o as [32 column quads][rows][4]
+  float* wide;  // slots of 2 * PA_ROWS rows (prompts, prefixes)
+  float* own;   // slots of G rows (streams' own keys)
   int ncta, max_tiles;
   size_t bytes;
 };
+
+constexpr int PA_WIDE_ROWS = 2 * PA_ROWS;
+
+__host__ __device__ inline size_t pa_slot_floats(int rows) { return (size_t)rows * (2 + PA_D); }
+
+// Rows of a slot for a stream's own keys: G, even, so that slots stay 16-byte aligned.
+__host__ __device__ inline int pa_own_rows(int Hq, int Hkv) { return (Hq / Hkv + 1) & ~1; }
 
 __host__ __device__ inline int pa_tq(int Hq, int Hkv) { return PA_ROWS / (Hq / Hkv); }
 

@@ -3,16 +3,42 @@
 //
 // For a query q at position p of a sequence (token and head), S = {j : max(0, p - W + 1) <= j <= p}:
 //   out = sum_{j in S} softmax_S(scale q . k_j) v_j      (0 where S is empty)
-// with one pass over the keys: a running maximum m, l = sum exp(s_j - m), o = sum exp(s_j - m) v_j,
+// with one pass over the keys: a running reference m, l = sum exp(s_j - m), o = sum exp(s_j - m) v_j,
 // all in fp32; out = bf16(o / l), then bf16(out * gate) with a gate per (token, head).
+//
+// One kernel serves all of it. A row tile is 128 query rows of one kv head: the G query heads of
+// 128 / G tokens (or streams) beside each other, so that grouped heads share every key they read
+// and the causal edge costs at most 128 / G keys a tile. Per 128-key tile two products run on the
+// tensor cores, S = Q K^T (both operands in shared memory) and O += P V (P from TMEM, where the
+// softmax warps put it in bf16 over the scores; V as it lies, keys by head dim).
+//   warps 0-3, 4-7  softmax of row tile 0 / 1, a row a thread: scores from TMEM, mask, exponentials,
+//                   P into TMEM, and the output at the end
+//   warp 8          issues the products
+//   warp 9          TMA: Q, and the pages' rows into a ring of five 32 KB tiles
+// Two row tiles (a pair) take each key tile in turn, so one's softmax runs under the other's
+// products. A lone row tile (streams, short prompts) takes the key tiles in turn as two halves,
+// even and odd ones, whose results are joined at the end: the same overlap, and 160 KB of loads in
+// flight for a cache that is read once.
+//
+// The reference m of a row follows the maximum only when that moves by more than 2^8 (the rows'
+// sums and O are then rescaled): exponentials up to 2^8 lose nothing in fp32 or bf16, and the
+// common tile touches O only through the tensor cores.
+//
+// P is rounded to bf16 (relative 2^-8 a weight, averaged over the keys) because the tensor cores
+// take it so; l sums the unrounded weights, and O, m and l stay in fp32 through the join.
 #include "paged.cuh"
+#include "tc_ptx.cuh"
+#include "tmap.cuh"
 
 namespace lg {
 
+using namespace tc;
+
+// ---- plan ---------------------------------------------------------------------------------
+
 static int pa_max_tiles(int kind, int T, int B, int Hq, int Hkv) {
-  (void)Hq;
-  (void)Hkv;
-  return kind == PA_PROMPT ? T / (2 * pa_tq(Hq, Hkv)) + B : B;
+  const int tq2 = 2 * pa_tq(Hq, Hkv);
+  return kind == PA_PROMPT ? T / tq2 + B : B + (B + tq2 - 1) / tq2;
 }
 
 static PaPlan pa_layout(void* buf, int kind, int T, int B, int Hq, int Hkv) {
@@ -25,19 +51,59 @@ static PaPlan pa_layout(void* buf, int kind, int T, int B, int Hq, int Hkv) {
   p.kv = c.take<int>(B);
   p.off = c.take<int>(B + 1);
   p.tiles = c.take<PaTile>(p.max_tiles);
-  p.parts = c.take<char>(0);
+  // prompts: two slots a CTA (a part that begins its segment, one that does not); streams: the
+  // parts in order, segment + CTA
+  const size_t wide = kind == PA_PROMPT
+                          ? 2 * (size_t)p.ncta
+                          : (size_t)(p.max_tiles - B) * Hkv + p.ncta;
+  const size_t own = kind == PA_PROMPT ? 0 : (size_t)B * Hkv + p.ncta;
+  p.wide = c.take<float>(wide * pa_slot_floats(PA_WIDE_ROWS));
+  p.own = c.take<float>(own * pa_slot_floats(pa_own_rows(Hq, Hkv)));
   p.bytes = align_up(c.used, 256);
   return p;
 }
 
 constexpr int PLAN_THREADS = 1024;
 
+__device__ __forceinline__ PaTile pa_stream_tile(const PaHead& h, const PaPlan& p, int i, int np,
+                                                 int tq) {
+  PaTile t = {};
+  if (i >= np) {  // stream i - np: its own keys
+    const int b = i - np, kv = p.kv[b];
+    t.row = t.q0 = b;
+    t.nq = 1;
+    t.kind = PA_OWN;
+    t.key_end = kv;
+    t.key0 = min(max(h.prefix, h.window ? kv - h.window : 0), kv);
+    t.w = PA_W_OWN;
+  } else {  // 2 tq streams against the shared prefix
+    t.q0 = i * 2 * tq;
+    t.nq = min(2 * tq, h.B - t.q0);
+    t.row = t.q0;
+    t.kind = PA_PREFIX;
+    t.pair = t.nq > tq;
+    int lo = h.prefix, most = -1;
+    for (int b = t.q0; b < t.q0 + t.nq; ++b) {
+      const int kv = p.kv[b];
+      if (kv > most) most = kv, t.row = b;  // the longest stream names the pages
+      if (kv > 0) lo = min(lo, h.window ? max(0, kv - h.window) : 0);
+    }
+    t.key_end = min(h.prefix, max(most, 0));
+    t.key0 = min(lo, t.key_end);
+    t.w = t.pair ? PA_W_PAIR : PA_W_ONE;
+  }
+  return t;
+}
+
+// Row tiles, their costs summed, and each CTA's start: one CTA; a few microseconds, once for all
+// layers of a step.
 __global__ void __launch_bounds__(PLAN_THREADS)
     pa_plan_kernel(const int* cu, const int* kv_len, PaHead h, PaPlan p) {
   __shared__ int wt[32], tot;
-  const int tid = threadIdx.x;
-  const int tq2 = 2 * pa_tq(h.Hq, h.Hkv);
-  int n = 0;
+  __shared__ long long wsum[32], carry;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tq = pa_tq(h.Hq, h.Hkv), tq2 = 2 * tq;
+  int n = 0, np = 0;
   for (int b0 = 0; b0 < h.B; b0 += PLAN_THREADS) {
     const int b = b0 + tid;
     int v = 0;
@@ -46,97 +112,734 @@ __global__ void __launch_bounds__(PLAN_THREADS)
       if (h.kind == PA_PROMPT) {
         const int t0 = min(max(cu[b], 0), h.T), t1 = min(max(cu[b + 1], t0), h.T);
         v = (t1 - t0 + tq2 - 1) / tq2;
-      } else {
-        v = 1;
       }
     }
-    const int at = n + block_excl_scan(v, wt, &tot);
-    if (b < h.B) p.off[b] = at;
-    n += tot;
+    if (h.kind == PA_PROMPT) {
+      const int at = n + block_excl_scan(v, wt, &tot);
+      if (b < h.B) p.off[b] = at;
+      n += tot;
+    }
     __syncthreads();
   }
+  if (h.kind != PA_PROMPT) {
+    np = h.prefix > 0 ? (h.B + tq2 - 1) / tq2 : 0;
+    n = np + h.B;
+  }
   n = min(n, p.max_tiles);  // offsets that do not ascend could ask for more
-  if (tid == 0) p.off[h.B] = n;
+  if (tid == 0) carry = 0;
   __syncthreads();
-  for (int i = tid; i < n; i += PLAN_THREADS) {
-    int lo = 0, hi = h.B - 1;  // the last sequence whose tiles start at or before i
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (p.off[mid] <= i) lo = mid;
-      else hi = mid - 1;
-    }
-    const int b = lo;
+  for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
+    const int i = i0 + tid;
     PaTile t = {};
-    t.row = b;
-    if (h.kind == PA_PROMPT) {
-      const int t0 = min(max(cu[b], 0), h.T), t1 = min(max(cu[b + 1], t0), h.T);
-      const int first = (i - p.off[b]) * tq2;
-      t.q0 = t0 + first;
-      t.nq = min(tq2, t1 - t0 - first);
-      t.pos0 = p.kv[b] - (t1 - t0) + first;
-      t.kind = PA_PROMPT;
-    } else {
-      t.q0 = b;
-      t.nq = 1;
-      t.pos0 = p.kv[b] - 1;
-      t.kind = PA_OWN;
+    long long cost = 0;
+    if (i < n) {
+      if (h.kind == PA_PROMPT) {
+        int lo = 0, hi = h.B - 1;  // the last sequence whose tiles start at or before i
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (p.off[mid] <= i) lo = mid;
+          else hi = mid - 1;
+        }
+        const int t0 = min(max(cu[lo], 0), h.T), t1 = min(max(cu[lo + 1], t0), h.T);
+        const int first = (i - p.off[lo]) * tq2;
+        t.row = lo;
+        t.q0 = t0 + first;
+        t.nq = min(tq2, t1 - t0 - first);
+        t.pos0 = p.kv[lo] - (t1 - t0) + first;
+        t.kind = PA_PROMPT;
+        t.pair = t.nq > tq;
+        t.key_end = max(0, t.pos0 + t.nq);
+        t.key0 = min(h.window ? max(0, t.pos0 - h.window + 1) : 0, t.key_end);
+        t.w = t.pair ? PA_W_PAIR : PA_W_ONE;
+      } else {
+        t = pa_stream_tile(h, p, i, np, tq);
+      }
+      t.key0 = t.key0 / h.R * h.R;
+      t.ntile = t.ntile0 = max(1, (t.key_end - t.key0 + PA_KEYS - 1) / PA_KEYS);
+      if (t.kind == PA_PROMPT && t.pair)  // the first row tile's tokens see fewer keys
+        t.ntile0 = max(1, (max(0, t.pos0 + tq) - t.key0 + PA_KEYS - 1) / PA_KEYS);
+      cost = pa_cost(t.ntile, t.w) * h.Hkv;
     }
-    t.key_end = max(0, t.pos0 + t.nq);
-    const int low = h.window ? max(0, t.pos0 - h.window + 1) : 0;
-    t.key0 = min(low, t.key_end) / h.R * h.R;
-    t.ntile = max(1, (t.key_end - t.key0 + PA_KEYS - 1) / PA_KEYS);
-    p.tiles[i] = t;
+    long long inc = cost;  // sum of the costs up to this tile's
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    long long base = carry;
+    for (int w = 0; w < warp; ++w) base += wsum[w];
+    t.before = base + inc - cost;
+    if (i < n) p.tiles[i] = t;
+    __syncthreads();
+    if (tid == PLAN_THREADS - 1) carry = base + inc;
+    __syncthreads();
+  }
+  const long long total = carry;
+  const long long chunk = max((long long)PA_MIN_CHUNK, (total + p.ncta - 1) / p.ncta);
+  for (int c = tid; c <= p.ncta; c += PLAN_THREADS) {
+    PaStart s = {n, 0, 0};
+    const long long u = c * chunk;
+    if (u < total) {
+      int lo = 0, hi = n - 1;  // the last tile whose cost begins at or before u
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.tiles[mid].before <= u) lo = mid;
+        else hi = mid - 1;
+      }
+      const PaTile t = p.tiles[lo];
+      const long long seg = pa_cost(t.ntile, t.w), r = u - t.before;
+      const long long in = r % seg - PA_SEG;  // key tile k begins at PA_SEG + k w of its segment
+      s.tile = lo;
+      s.head = (int)(r / seg);
+      s.t = in <= 0 ? 0 : (int)((in + t.w - 1) / t.w);
+      if (s.t >= t.ntile) {
+        s.t = 0;
+        if (++s.head == h.Hkv) s.head = 0, ++s.tile;
+      }
+    }
+    p.start[c] = s;
   }
   if (tid == 0) {
-    h.ntile_rows = n;
+    h.total = total;
+    h.chunk = chunk;
+    h.ntiles = n;
+    h.nprefix = np;
+    h.err = 0;
     *p.head = h;
   }
 }
 
+// ---- attention ----------------------------------------------------------------------------
+
 struct PaArgs {
-  const __nv_bfloat16 *q, *k, *v, *gate;
+  const __nv_bfloat16* gate;
   __nv_bfloat16* out;
   const int* table;
-  long long q_tok, q_head, pg, hd, rw;  // element strides
   int P, R, M, Hq, Hkv;
-  float scale;
+  float scale_log2;  // scale * log2(e): exponentials are powers of two
   PaPlan plan;
 };
 
-// The plain form: one warp per (token, head), four dims a lane, one key at a time.
-__global__ void __launch_bounds__(256) pa_simple_kernel(PaArgs a) {
-  const PaHead h = *a.plan.head;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.Hq / a.Hkv;
-  if ((int)blockIdx.x >= h.ntile_rows) return;
-  const PaTile t = a.plan.tiles[blockIdx.x];
-  for (int r = warp; r < t.nq * G; r += 8) {
-    const int tok = t.q0 + r / G, head = blockIdx.y * G + r % G, pos = t.pos0 + r / G;
-    const int lo = h.window ? max(0, pos - h.window + 1) : 0;
-    float q[4], o[4] = {}, m = -INFINITY, l = 0.f;
-    const __nv_bfloat16* qp = a.q + tok * a.q_tok + head * a.q_head + lane * 4;
-    for (int d = 0; d < 4; ++d) q[d] = bf2f(qp[d]) * a.scale;
-    for (int j = lo; j <= pos; ++j) {
-      const int c = j / a.R, pg = c < a.M ? a.table[(long long)t.row * a.M + c] : -1;
-      if (pg < 0 || pg >= a.P) {
-        l = NAN;
-        break;
-      }
-      const long long at = pg * a.pg + blockIdx.y * a.hd + (j % a.R) * a.rw + lane * 4;
-      float s = 0.f;
-      for (int d = 0; d < 4; ++d) s += q[d] * bf2f(a.k[at + d]);
-      s = warp_sum(s);
-      const float mn = fmaxf(m, s), f = __expf(m - mn), e = __expf(s - mn);
-      l = l * f + e;
-      for (int d = 0; d < 4; ++d) o[d] = o[d] * f + e * bf2f(a.v[at + d]);
-      m = mn;
+constexpr int PA_THREADS = 384;  // two softmax warpgroups, and one of which two warps work
+// Registers a thread: 168 at launch (65,536 over 384 threads); 2 * 216 + 72 = 3 * 168.
+constexpr int PA_REGS_SOFTMAX = 216, PA_REGS_OTHER = 72;
+constexpr int PA_TILE_BYTES = PA_KEYS * PA_D * 2;  // 32 KB: two halves of 64 dims, 128-byte rows
+constexpr int PA_HALF = PA_TILE_BYTES / 2;
+constexpr int PA_RING = 5;
+constexpr int PA_NBAD = 8;
+constexpr size_t PA_SMEM = (2 + PA_RING) * PA_TILE_BYTES + 512 + 2 * PA_ROWS * 8;
+
+// The segments of a CTA's share, in order; every warp walks them by itself.
+struct PaWalk {
+  PaStart at, end;
+  int t0, t1;
+  PaTile rec;
+  __device__ PaWalk(const PaPlan& p) : at(p.start[blockIdx.x]), end(p.start[blockIdx.x + 1]) {}
+  __device__ bool next(const PaPlan& p) {
+    const bool same = at.tile == end.tile && at.head == end.head;
+    if (at.tile > end.tile || (at.tile == end.tile && at.head > end.head) ||
+        (same && at.t >= end.t))
+      return false;
+    rec = p.tiles[at.tile];
+    t0 = at.t;
+    t1 = same ? end.t : rec.ntile;
+    return true;
+  }
+  __device__ void step(int Hkv) {
+    at.t = 0;
+    if (++at.head == Hkv) at.head = 0, ++at.tile;
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A bounded wait with one verdict for the whole warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
+
+// Both softmax warpgroups (named barrier 1): false for all if it is for one.
+__device__ __forceinline__ bool softmax_sync(bool ok) {
+  tc_fence_before();
+  ok = bar_and_n<1, 256>(ok);
+  tc_fence_after();
+  return ok;
+}
+
+__global__ void __launch_bounds__(PA_THREADS, 1)
+    pa_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+              const __grid_constant__ CUtensorMap tm_v, const PaArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem[];  // 1,024: the swizzle's period
+  uint8_t* sQ = smem;                       // two row tiles
+  uint8_t* sKV = sQ + 2 * PA_TILE_BYTES;    // ring
+  uint64_t* full = reinterpret_cast<uint64_t*>(sKV + PA_RING * PA_TILE_BYTES);
+  uint64_t* empty = full + PA_RING;
+  uint64_t* q_full = empty + PA_RING;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;   // [2] scores of row tile (or half) w
+  uint64_t* p_ready = s_full + 2;   // [2] its weights are in TMEM
+  uint64_t* o_full = p_ready + 2;   // [2] its output is complete
+  uint64_t* done = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* bad = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [PA_NBAD] per segment
+  float2* ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(full) + 512);  // [2][128]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  PaHead* const head = a.plan.head;
+  int* const err = &head->err;
+  const int G = a.Hq / a.Hkv, tq = PA_ROWS / G;
+  PaWalk walk(a.plan);
+  if (smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0) *err = 9;
+    return;
+  }
+  {
+    PaWalk w = walk;
+    if (!w.next(a.plan)) return;  // nothing for this CTA
+  }
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < PA_RING; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
     }
-    for (int d = 0; d < 4; ++d) {
-      float x = l == 0.f ? 0.f : o[d] / l;
-      if (a.gate) x = round_bf16(x) * bf2f(a.gate[(long long)tok * a.Hq + head]);
-      a.out[((long long)tok * a.Hq + head) * PA_D + lane * 4 + d] = __float2bfloat16_rn(x);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(s_full + w, 1);
+      mbar_init(p_ready + w, 128);
+      mbar_init(o_full + w, 1);
+    }
+    mbar_init(done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) {  // one setmaxnreg for the whole warpgroup
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_OTHER));
+  if (warp == 9) {
+    // ---- loads: per segment the first key tiles, Q, then V and K in the order of use ----
+    int rc = 0, seg = 0, nq = 0;  // ring tiles, segments and Q tiles so far
+    bool ok = true;
+    const int boxes = PA_KEYS / a.R;  // pages a tile; lanes [0, 2 boxes): (page, half)
+    const bool mine = lane < 2 * boxes;
+    const int half = lane & 1, box = lane >> 1;
+    for (; ok && walk.next(a.plan); walk.step(a.Hkv), ++seg) {
+      const PaTile r = walk.rec;
+      const int lead = r.pair ? 1 : 2, n = walk.t1 - walk.t0;
+      if (lane == 0) bad[seg % PA_NBAD] = 0;
+      __syncwarp();
+      const int npage = (r.key_end + a.R - 1) / a.R;  // pages the rows need
+      const int* row = a.table + (long long)r.row * a.M;
+      // this lane's page of key tile i: the pool's page count (it reads as zeros) past the end
+      auto page_of = [&](int i) {
+        const int c = (r.key0 + (walk.t0 + i) * PA_KEYS) / a.R + box;
+        if (!mine || i >= n || c >= npage) return a.P;
+        const int p = c < a.M ? __ldg(row + c) : -1;
+        if (p >= 0 && p < a.P) return p;
+        bad[seg % PA_NBAD] = 1;
+        return a.P;
+      };
+      auto load = [&](const CUtensorMap* m, int page) {
+        const int s = rc % PA_RING;
+        if (!warp_wait(empty + s, ((rc / PA_RING) & 1) ^ 1, err, 1)) return false;
+        if (lane == 0) mbar_arrive_expect_tx(full + s, PA_TILE_BYTES);
+        __syncwarp();
+        if (mine)
+          tma_load_4d(sKV + s * PA_TILE_BYTES + half * PA_HALF + box * a.R * 128, m, full + s,
+                      half * 64, 0, walk.at.head, page);
+        ++rc;
+        return true;
+      };
+      int p0 = page_of(0), p1 = page_of(1), p2 = page_of(2);
+      ok = load(&tm_k, p0);
+      if (ok && lead == 2 && n > 1) ok = load(&tm_k, p1);
+      if (ok) ok = warp_wait(q_empty, (seg & 1) ^ 1, err, 2);
+      nq += ok;
+      if (ok && lane == 0) {
+        const uint32_t bytes = 128 * G * tq;
+        mbar_arrive_expect_tx(q_full, (r.pair ? 4 : 2) * bytes);
+        for (int w = 0; w <= r.pair; ++w)
+          for (int f = 0; f < 2; ++f)
+            tma_load_3d(sQ + w * PA_TILE_BYTES + f * PA_HALF, &tm_q, q_full, f * 64,
+                        walk.at.head * G, r.q0 + w * tq);
+      }
+      __syncwarp();
+      for (int i = 0; ok && i < n; ++i) {
+        const int p3 = page_of(i + 3);
+        ok = load(&tm_v, p0);
+        if (ok && i + lead < n) ok = load(&tm_k, lead == 1 ? p1 : p2);
+        p0 = p1;
+        p1 = p2;
+        p2 = p3;
+      }
+    }
+    // every copy issued has landed before the CTA ends (bounded, also after a failed wait)
+    const long long t0 = clock64();
+    for (int i = max(0, rc - PA_RING); i < rc; ++i)
+      while (!mbar_try_wait(full + i % PA_RING, (i / PA_RING) & 1) &&
+             clock64() - t0 < 4000000000LL) {
+      }
+    while (nq > 0 && !mbar_try_wait(q_full, (nq - 1) & 1) && clock64() - t0 < 4000000000LL) {
+    }
+  } else if (warp == 8) {
+    // ---- products ----
+    int rc = 0, seg = 0;
+    bool ok = true;
+    uint32_t p_phase[2] = {0, 0};
+    const uint32_t id_qk = idesc_bf16(PA_ROWS, PA_KEYS);
+    const uint32_t id_pv = idesc_bf16(PA_ROWS, PA_D) | IDESC_B_MN;
+    const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
+    for (; ok && walk.next(a.plan); walk.step(a.Hkv), ++seg) {
+      const PaTile r = walk.rec;
+      const int n = walk.t1 - walk.t0;
+      // key tiles of this part that half w takes: [0, lim[w]) (pair), or every second one
+      const int lim0 = r.pair ? min(n, max(0, r.ntile0 - walk.t0)) : n;
+      auto wait_full = [&]() {
+        const bool got = warp_wait(full + rc % PA_RING, (rc / PA_RING) & 1, err, 3);
+        tc_fence_after();
+        return got;
+      };
+      auto qk = [&](int w, int slot) {
+        if (lane == 0) {
+          // opaque: or the 16 descriptors of every call site are kept in registers throughout
+          uint32_t q = q_addr + (r.pair ? w * PA_TILE_BYTES : 0);
+          uint32_t k = kv_addr + slot * PA_TILE_BYTES;
+          asm volatile("" : "+r"(q), "+r"(k));
+#pragma unroll
+          for (int s = 0; s < PA_D / 16; ++s) {
+            const uint32_t off = (s >> 2) * PA_HALF + (s & 3) * 32;
+            umma_bf16(tmem + w * 128, sw128_desc(q + off), sw128_desc(k + off), id_qk, s > 0);
+          }
+          umma_commit(s_full + w);
+        }
+        __syncwarp();
+      };
+      auto pv = [&](int w, int slot, bool first) {
+        if (lane == 0) {
+          uint32_t v = kv_addr + slot * PA_TILE_BYTES;
+          asm volatile("" : "+r"(v));
+#pragma unroll
+          for (int s = 0; s < PA_KEYS / 16; ++s)
+            umma_bf16_ts(tmem + 256 + w * 128, tmem + w * 128 + s * 8,
+                         sw128_desc_mn(v + s * 2048, PA_HALF), id_pv, !(first && s == 0));
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* b) {
+        if (lane == 0) umma_commit(b);
+        __syncwarp();
+      };
+      auto wait_p = [&](int w) {
+        const bool got = warp_wait(p_ready + w, p_phase[w], err, 4);
+        p_phase[w] ^= 1;
+        tc_fence_after();
+        return got;
+      };
+      // rows of V past the last key hold anything (also NaN): their weights are 0, they become 0
+      auto clear_tail = [&](int i, int slot) {
+        const int keep = r.key_end - (r.key0 + (walk.t0 + i) * PA_KEYS);
+        if (keep >= PA_KEYS) return;
+        uint8_t* v = sKV + slot * PA_TILE_BYTES;
+        for (int x = max(keep, 0) * 8 + lane; x < PA_KEYS * 8; x += 32) {
+          *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(v + PA_HALF + x * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      };
+      ok = warp_wait(q_full, seg & 1, err, 5);
+      if (!ok) break;
+      if (r.pair) {
+        if (!(ok = wait_full())) break;
+        if (lim0 > 0) qk(0, rc % PA_RING);
+        qk(1, rc % PA_RING);
+        commit(empty + rc % PA_RING);
+        if (n == 1) commit(q_empty);
+        ++rc;
+        for (int i = 0; ok && i < n; ++i) {
+          if (!(ok = wait_full())) break;
+          const int vs = rc % PA_RING;
+          clear_tail(i, vs);
+          ++rc;
+          const bool more = i + 1 < n;
+          const int ks = rc % PA_RING;
+          if (i < lim0) {
+            if (!(ok = wait_p(0))) break;
+            pv(0, vs, i == 0);
+            if (i + 1 == lim0) commit(o_full);
+          }
+          if (more && !(ok = wait_full())) break;
+          if (i + 1 < lim0) qk(0, ks);
+          if (!(ok = wait_p(1))) break;
+          pv(1, vs, i == 0);
+          commit(empty + vs);
+          if (!more) commit(o_full + 1);
+          if (more) {
+            qk(1, ks);
+            commit(empty + ks);
+            if (i + 2 == n) commit(q_empty);
+            ++rc;
+          }
+        }
+      } else {
+        for (int w = 0; ok && w < 2 && w < n; ++w) {
+          if (!(ok = wait_full())) break;
+          qk(w, rc % PA_RING);
+          commit(empty + rc % PA_RING);
+          if (w + 1 == n) commit(q_empty);
+          ++rc;
+        }
+        for (int i = 0; ok && i < n; ++i) {
+          const int w = i & 1;
+          if (!(ok = wait_full())) break;
+          const int vs = rc % PA_RING;
+          clear_tail(i, vs);
+          ++rc;
+          if (!(ok = wait_p(w))) break;
+          pv(w, vs, i < 2);
+          commit(empty + vs);
+          if (i + 2 >= n) commit(o_full + w);
+          if (i + 2 < n) {
+            if (!(ok = wait_full())) break;
+            qk(w, rc % PA_RING);
+            commit(empty + rc % PA_RING);
+            if (i + 3 == n) commit(q_empty);
+            ++rc;
+          }
+        }
+      }
+    }
+    if (lane == 0) umma_commit(done);
+    __syncwarp();
+    const long long t0 = clock64();
+    while (!mbar_try_wait(done, 0) && clock64() - t0 < 4000000000LL) {
     }
   }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_REGS_SOFTMAX));
+    // ---- softmax: warpgroup w, thread = row ----
+    const int w = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t quarter = (uint32_t)(warp & 3) << 21;  // lane field: 32 (warp & 3) << 16
+    const uint32_t tS = tmem + w * 128 + quarter, tO = tmem + 256 + quarter;
+    const float c = a.scale_log2;
+    const int prefix = head->prefix, window = head->window;
+    uint32_t s_phase = 0, o_phase = 0;
+    int seg = 0;
+    bool ok = true;
+    // after a failed wait the group only meets the other one at its barriers
+    for (; walk.next(a.plan); walk.step(a.Hkv), ++seg) {
+      const PaTile r = walk.rec;
+      const int n = walk.t1 - walk.t0;
+      const int lim0 = r.pair ? min(n, max(0, r.ntile0 - walk.t0)) : n;
+      // this row's token and the keys [lo, hi) it sees
+      const int i0 = r.pair ? w * tq : 0, i = i0 + row / G;
+      const bool valid = row < tq * G && i < r.nq;
+      int lo = 0, hi = 1 << 30;
+      if (valid) {
+        const int kv = r.kind == PA_PROMPT ? r.pos0 + i + 1 : a.plan.kv[r.q0 + i];
+        hi = r.kind == PA_PREFIX ? min(prefix, kv) : kv;
+        lo = window ? max(0, kv - window) : 0;
+        if (r.kind == PA_OWN) lo = max(lo, prefix);
+      }
+      const bool active = __any_sync(0xffffffffu, valid);
+      float m = -INFINITY, l = 0.f;
+      const int first = r.pair ? 0 : w, stride = r.pair ? 1 : 2;
+      const int last = r.pair && w == 0 ? lim0 : n;
+      bool any = false;  // this half has a key tile
+      for (int t = first; ok && t < last; t += stride) {
+        if (!(ok = warp_wait(s_full + w, s_phase, err, 6))) break;
+        s_phase ^= 1;
+        tc_fence_after();
+        if (active) {
+          const int kb = r.key0 + (walk.t0 + t) * PA_KEYS;
+          float s[4][32];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tmem_ld32(tS + 32 * j, s[j]);
+          tmem_ld_wait_all();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) keep32(s[j]);
+          if (__any_sync(0xffffffffu, valid && (kb < lo || kb + PA_KEYS > hi))) {
+#pragma unroll
+            for (int j = 0; j < 128; ++j)
+              if (kb + j < lo || kb + j >= hi) s[j >> 5][j & 31] = -INFINITY;
+          }
+          float mx[4] = {s[0][0], s[1][0], s[2][0], s[3][0]};
+#pragma unroll
+          for (int j = 1; j < 32; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) mx[x] = fmaxf(mx[x], s[x][j]);
+          const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const bool move = tm > m && (tm - m) * c > 8.f;  // also from m = -inf
+          if (!any) {
+            m = tm;
+          } else if (__any_sync(0xffffffffu, move)) {
+            const float f = move ? (m == -INFINITY ? 0.f : ex2((m - tm) * c)) : 1.f;
+            if (move) m = tm;
+            l *= f;
+#pragma unroll 1
+            for (int j = 0; j < PA_D; j += 16) {
+              uint32_t o[16];
+              tmem_ld16(tO + w * 128 + j, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st16(tO + w * 128 + j, o);
+            }
+          }
+          const float mc = m == -INFINITY ? 0.f : m * c;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t p[32];
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              const float e0 = ex2(fmaf(s[2 * j + (x >> 4)][2 * x & 31], c, -mc));
+              const float e1 = ex2(fmaf(s[2 * j + (x >> 4)][(2 * x & 31) + 1], c, -mc));
+              sum[x & 3] += e0 + e1;
+              p[x] = pack2(e0, e1);
+            }
+            tmem_st32(tS + 32 * j, p);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st_wait();
+        }
+        any = true;
+        tc_fence_before();
+        mbar_arrive(p_ready + w);
+      }
+      // ---- output ----
+      if (ok && any) {
+        ok = warp_wait(o_full + w, o_phase, err, 7);
+        o_phase ^= 1;
+        tc_fence_after();
+      }
+      if (r.pair && !ok) continue;
+      if (bad[seg % PA_NBAD]) l = NAN;
+      const bool whole = walk.t0 == 0 && walk.t1 == r.ntile && (r.kind == PA_PROMPT || prefix == 0);
+      // a pair: all columns of the own row tile; else columns [64 w, 64 w + 64) of both halves
+      float f0 = 1.f, f1 = 0.f;
+      bool has0 = any, has1 = false;
+      if (!r.pair) {
+        ml[w * PA_ROWS + row] = make_float2(m, l);
+        if (!(ok = softmax_sync(ok))) continue;
+        const float2 x0 = ml[row], x1 = ml[PA_ROWS + row];
+        m = fmaxf(x0.x, x1.x);
+        f0 = x0.x == -INFINITY ? 0.f : ex2((x0.x - m) * c);
+        f1 = x1.x == -INFINITY ? 0.f : ex2((x1.x - m) * c);
+        l = x0.y * f0 + x1.y * f1;
+        if (bad[seg % PA_NBAD]) l = NAN;
+        has0 = true;
+        has1 = n > 1;
+      }
+      if (active) {
+        const int rr = (r.pair ? w * PA_ROWS : 0) + row;
+        float* slot = nullptr;
+        int rows = PA_WIDE_ROWS;
+        if (!whole) {
+          if (r.kind == PA_PROMPT) {
+            slot = a.plan.wide + (2 * blockIdx.x + (walk.t0 == 0)) * pa_slot_floats(rows);
+          } else if (r.kind == PA_PREFIX) {
+            slot = a.plan.wide +
+                   ((size_t)walk.at.tile * a.Hkv + walk.at.head + blockIdx.x) * pa_slot_floats(rows);
+          } else {
+            rows = pa_own_rows(a.Hq, a.Hkv);
+            slot = a.plan.own + ((size_t)(walk.at.tile - head->nprefix) * a.Hkv + walk.at.head +
+                                 blockIdx.x) * pa_slot_floats(rows);
+          }
+          if (valid && (r.pair || w == 0))
+            reinterpret_cast<float2*>(slot)[rr] = make_float2(m, l);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int tok = r.q0 + i, qh = walk.at.head * G + row % G;
+        const float g = valid && whole && a.gate ? bf2f(a.gate[(long long)tok * a.Hq + qh]) : 1.f;
+        const int j0 = r.pair ? 0 : 2 * w, j1 = r.pair ? 4 : 2 * w + 2;
+        for (int j = j0; j < j1; ++j) {
+          float x0[32], x1[32];
+          if (has0) tmem_ld32(tO + (r.pair ? w * 128 : 0) + 32 * j, x0);
+          if (has1) tmem_ld32(tO + 128 + 32 * j, x1);
+          tmem_ld_wait_all();
+          keep32(x0);
+          keep32(x1);
+          float o[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            o[x] = has0 ? x0[x] * f0 : 0.f;
+            if (has1) o[x] = fmaf(x1[x], f1, o[x]);
+          }
+          if (!valid) continue;
+          if (whole) {
+            uint4* dst = reinterpret_cast<uint4*>(a.out + ((long long)tok * a.Hq + qh) * PA_D + 32 * j);
+            uint32_t y[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              float u = o[2 * x] * inv, v = o[2 * x + 1] * inv;
+              if (l == 0.f) u = v = 0.f;
+              if (a.gate) u = round_bf16(u) * g, v = round_bf16(v) * g;
+              y[x] = pack2(u, v);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) dst[x] = make_uint4(y[4 * x], y[4 * x + 1], y[4 * x + 2], y[4 * x + 3]);
+          } else {
+            float4* po = reinterpret_cast<float4*>(slot + 2 * rows);
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              po[(8 * j + x) * rows + rr] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+          }
+        }
+      }
+      // neither half's O or ml is overwritten before both groups have read it
+      if (!r.pair) ok = softmax_sync(ok);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, 512);
 }
+
+// The CTAs [c0, c1] whose shares hold key tiles of the segment (tile t, head).
+__device__ __forceinline__ void pa_parts(const PaHead& h, const PaTile& t, int head, int* c0,
+                                         int* c1) {
+  const long long s = t.before + head * pa_cost(t.ntile, t.w) + PA_SEG;
+  *c0 = (int)(s / h.chunk);
+  *c1 = (int)((s + (long long)(t.ntile - 1) * t.w) / h.chunk);
+}
+
+// Joins the parts of prompts' split segments: block x looks at the segment that CTA x + 1 begins
+// inside of, if CTA x began it; block y takes 32 of its rows (lane = row, so a slot's column quads
+// are read 512 bytes at a time), and the rows leave through shared memory, 256 bytes each.
+constexpr int JP_ROWS = 32;
+__global__ void __launch_bounds__(256) pa_join_prompt_kernel(const PaArgs a) {
+  __shared__ uint2 rows[JP_ROWS][33];
+  const PaHead h = *a.plan.head;
+  const int c = blockIdx.x;
+  const PaStart st = a.plan.start[c + 1];
+  if (st.tile >= h.ntiles || st.t == 0) return;
+  const PaTile t = a.plan.tiles[st.tile];
+  int c0, c1;
+  pa_parts(h, t, st.head, &c0, &c1);
+  if (c0 != c) return;
+  const int G = a.Hq / a.Hkv, tq = PA_ROWS / G;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rr = blockIdx.y * JP_ROWS + lane, w = rr / PA_ROWS, row = rr % PA_ROWS;
+  const int i = w * tq + row / G;
+  const bool valid = row < tq * G && i < t.nq && w <= t.pair;
+  const size_t slot = pa_slot_floats(PA_WIDE_ROWS);
+  if (!__syncthreads_or(valid)) return;
+  if (valid) {
+    float m = -INFINITY;
+    for (int x = c0; x <= c1; ++x) {
+      const float* p = a.plan.wide + (2 * x + (x == c0)) * slot;
+      m = fmaxf(m, reinterpret_cast<const float2*>(p)[rr].x);
+    }
+    float l = 0.f;
+    float4 o[4] = {};
+    for (int x = c0; x <= c1; ++x) {
+      const float* p = a.plan.wide + (2 * x + (x == c0)) * slot;
+      const float2 ml = reinterpret_cast<const float2*>(p)[rr];
+      const float f = ml.x == -INFINITY ? 0.f : ex2((ml.x - m) * a.scale_log2);
+      l += ml.y * f;
+      const float4* po = reinterpret_cast<const float4*>(p + 2 * PA_WIDE_ROWS);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 v = po[(4 * warp + j) * PA_WIDE_ROWS + rr];
+        o[j].x = fmaf(v.x, f, o[j].x);
+        o[j].y = fmaf(v.y, f, o[j].y);
+        o[j].z = fmaf(v.z, f, o[j].z);
+        o[j].w = fmaf(v.w, f, o[j].w);
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float g = a.gate ? bf2f(a.gate[(long long)(t.q0 + i) * a.Hq + st.head * G + row % G]) : 1.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float4 v = make_float4(o[j].x * inv, o[j].y * inv, o[j].z * inv, o[j].w * inv);
+      if (a.gate)
+        v = make_float4(round_bf16(v.x) * g, round_bf16(v.y) * g, round_bf16(v.z) * g,
+                        round_bf16(v.w) * g);
+      rows[lane][4 * warp + j] = make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
+    }
+  }
+  __syncthreads();
+  for (int x = warp; x < JP_ROWS; x += 8) {
+    const int r2 = blockIdx.y * JP_ROWS + x, w2 = r2 / PA_ROWS, row2 = r2 % PA_ROWS;
+    const int i2 = w2 * tq + row2 / G;
+    if (row2 >= tq * G || i2 >= t.nq || w2 > t.pair) continue;
+    reinterpret_cast<uint2*>(a.out + ((long long)(t.q0 + i2) * a.Hq + st.head * G + row2 % G) *
+                                         PA_D)[lane] = rows[x][lane];
+  }
+}
+
+// Joins a stream's parts for one kv head: its share of the prefix's and its own keys'.
+__global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
+  const PaHead h = *a.plan.head;
+  const int b = blockIdx.x, head = blockIdx.y, G = a.Hq / a.Hkv, tq = PA_ROWS / G;
+  const PaTile own = a.plan.tiles[h.nprefix + b];
+  int c0, c1, p0 = 0, p1 = -1, rr = 0;
+  pa_parts(h, own, head, &c0, &c1);
+  if (h.nprefix == 0 && c0 == c1) return;  // written by the CTA that had it whole
+  const int rows = pa_own_rows(a.Hq, a.Hkv), pi = b / (2 * tq);
+  if (h.nprefix) {
+    const PaTile pre = a.plan.tiles[pi];
+    pa_parts(h, pre, head, &p0, &p1);
+    const int i = b - pre.q0, w = i / tq;
+    rr = w * PA_ROWS + (i - w * tq) * G;
+  }
+  const float* wide = a.plan.wide + ((size_t)pi * a.Hkv + head) * pa_slot_floats(PA_WIDE_ROWS);
+  const float* ow = a.plan.own + ((size_t)b * a.Hkv + head) * pa_slot_floats(rows);
+  for (int e = threadIdx.x; e < G * 32; e += 128) {
+    const int g = e % G, q = e / G;  // neighbours take neighbouring rows of one column quad
+    float m = -INFINITY;
+    for (int x = p0; x <= p1; ++x)
+      m = fmaxf(m, reinterpret_cast<const float2*>(wide + x * pa_slot_floats(PA_WIDE_ROWS))[rr + g].x);
+    for (int x = c0; x <= c1; ++x)
+      m = fmaxf(m, reinterpret_cast<const float2*>(ow + x * pa_slot_floats(rows))[g].x);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float* p, int n, int r) {
+      const float2 ml = reinterpret_cast<const float2*>(p)[r];
+      const float f = ml.x == -INFINITY ? 0.f : ex2((ml.x - m) * a.scale_log2);
+      const float4 v = reinterpret_cast<const float4*>(p + 2 * n)[q * n + r];
+      l += ml.y * f;
+      o.x = fmaf(v.x, f, o.x);
+      o.y = fmaf(v.y, f, o.y);
+      o.z = fmaf(v.z, f, o.z);
+      o.w = fmaf(v.w, f, o.w);
+    };
+    for (int x = p0; x <= p1; ++x) add(wide + x * pa_slot_floats(PA_WIDE_ROWS), PA_WIDE_ROWS, rr + g);
+    for (int x = c0; x <= c1; ++x) add(ow + x * pa_slot_floats(rows), rows, g);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float4 v = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    const long long at = (long long)b * a.Hq + head * G + g;
+    if (a.gate) {
+      const float s = bf2f(a.gate[at]);
+      v = make_float4(round_bf16(v.x) * s, round_bf16(v.y) * s, round_bf16(v.z) * s,
+                      round_bf16(v.w) * s);
+    }
+    reinterpret_cast<uint2*>(a.out + at * PA_D)[q] = make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
+  }
+}
+
+// ---- entry points -------------------------------------------------------------------------
 
 static int plan_check(const char* who, int T, int B, int Hq, int Hkv, int R, int window) {
   LG_CHECK_ARG(T >= 0 && B > 0 && B <= (1 << 20) && T <= (1 << 26), "%s: %d tokens of %d sequences",
@@ -186,27 +889,43 @@ static int attn_run(const char* who, int kind, const void* q, long long q_tok, l
   const PaPlan p = pa_layout(plan, kind, T, B, Hq, Hkv);
   if (!plan || !aligned(plan, 256) || bytes < p.bytes)
     return fail(LG_ERR_WORKSPACE, "%s: the plan buffer needs %zu bytes", who, p.bytes);
+  // a dimension of one element has no stride to speak of
+  if (T == 1) q_tok = D;
+  if (Hq == 1) q_head = D;
+  if (P == 1) pg = D;
+  if (Hkv == 1) hd = D;
+  const int G = Hq / Hkv;
+  CUtensorMap tm_q, tm_k, tm_v;
+  const uint64_t qd[3] = {(uint64_t)D, (uint64_t)Hq, (uint64_t)T};
+  const uint64_t qst[2] = {(uint64_t)q_head * 2, (uint64_t)q_tok * 2};
+  const uint32_t qb[3] = {64, (uint32_t)G, (uint32_t)pa_tq(Hq, Hkv)};
+  const uint64_t kd[4] = {(uint64_t)D, (uint64_t)R, (uint64_t)Hkv, (uint64_t)P};
+  const uint64_t kst[3] = {(uint64_t)rw * 2, (uint64_t)hd * 2, (uint64_t)pg * 2};
+  const uint32_t kb[4] = {64, (uint32_t)R, 1, 1};
+  if (int rc = make_map_nd(&tm_q, q, 3, qd, qst, qb)) return rc;
+  if (int rc = make_map_nd(&tm_k, k, 4, kd, kst, kb)) return rc;
+  if (int rc = make_map_nd(&tm_v, v, 4, kd, kst, kb)) return rc;
   PaArgs a;
-  a.q = static_cast<const __nv_bfloat16*>(q);
-  a.k = static_cast<const __nv_bfloat16*>(k);
-  a.v = static_cast<const __nv_bfloat16*>(v);
   a.gate = static_cast<const __nv_bfloat16*>(gate);
   a.out = static_cast<__nv_bfloat16*>(out);
   a.table = table;
-  a.q_tok = q_tok;
-  a.q_head = q_head;
-  a.pg = pg;
-  a.hd = hd;
-  a.rw = rw;
   a.P = P;
   a.R = R;
   a.M = M;
   a.Hq = Hq;
   a.Hkv = Hkv;
-  a.scale = scale;
+  a.scale_log2 = scale * 1.4426950408889634f;
   a.plan = p;
-  pa_simple_kernel<<<dim3(p.max_tiles, Hkv), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  LG_CUDA_TRY(cudaFuncSetAttribute(pa_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)PA_SMEM));
+  pa_kernel<<<p.ncta, PA_THREADS, PA_SMEM, st>>>(tm_q, tm_k, tm_v, a);
   LG_LAUNCH_CHECK(who);
+  if (kind == PA_PROMPT)
+    pa_join_prompt_kernel<<<dim3(p.ncta, PA_WIDE_ROWS / JP_ROWS), 256, 0, st>>>(a);
+  else
+    pa_join_stream_kernel<<<dim3(B, Hkv), 128, 0, st>>>(a);
+  LG_LAUNCH_CHECK("paged_join");
   return LG_OK;
 }
 
@@ -222,6 +941,14 @@ extern "C" size_t lg_prompt_plan_bytes(int T, int B, int Hq, int Hkv) {
 extern "C" size_t lg_stream_plan_bytes(int B, int Hq, int Hkv) {
   if (plan_check("stream_plan_bytes", B, B, Hq, Hkv, 16, 0)) return 0;
   return pa_layout(nullptr, PA_OWN, B, B, Hq, Hkv).bytes;
+}
+
+extern "C" int lg_plan_status(const void* plan, int* status) {
+  LG_CHECK_ARG(plan && status, "plan_status: NULL pointer");
+  PaHead h;
+  LG_CUDA_TRY(cudaMemcpy(&h, plan, sizeof(h), cudaMemcpyDeviceToHost));
+  *status = h.err;
+  return LG_OK;
 }
 
 extern "C" int lg_prompt_plan(const int32_t* cu_q, const int32_t* kv_len, int B, int T, int Hq,

@@ -43,4 +43,26 @@ inline int make_map_2d(CUtensorMap* m, const void* base, bool bf16, uint64_t inn
   return LG_OK;
 }
 
+// bf16 map of up to 4 dimensions, innermost first (dims[0] contiguous), 128-byte swizzle;
+// strides[i] bytes between steps of dims[i + 1]. Coordinates past a dimension read as zeros.
+inline int make_map_nd(CUtensorMap* m, const void* base, int n, const uint64_t* dims,
+                       const uint64_t* strides, const uint32_t* box) {
+  auto fn = tmap_encode_fn();
+  if (!fn) return fail(LG_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4], e[4];
+  for (int i = 0; i < n; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    e[i] = 1;
+    if (i) s[i - 1] = strides[i - 1];
+  }
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, n, const_cast<void*>(base), d, s, b, e,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(LG_ERR_INVALID, "cuTensorMapEncodeTiled refused the strides (%d)", (int)r);
+  return LG_OK;
+}
+
 }  // namespace lg
