@@ -36,8 +36,8 @@ struct PaTile {
 // Costs: half a row tile's worth of tensor-core time on one key tile is 1, so a pair's key tile
 // is 4 and a lone row tile's 2; a stream's own key tile waits for HBM rather than the tensor
 // cores. Every segment costs PA_SEG more (Q load, first score, output).
-constexpr int PA_W_PAIR = 4, PA_W_ONE = 2, PA_W_OWN = 3, PA_SEG = 2;
-constexpr int PA_MIN_CHUNK = 8;  // at least the largest PA_SEG + w: no CTA below the last is idle
+constexpr int PA_W_PAIR = 4, PA_W_ONE = 2, PA_W_OWN = 3, PA_SEG = 8;
+constexpr int PA_MIN_CHUNK = 12;  // at least the largest PA_SEG + w: no CTA below the last is idle
 
 __host__ __device__ inline long long pa_cost(int ntile, int w) {
   return PA_SEG + (long long)ntile * w;

@@ -13,11 +13,12 @@
 // softmax warps put it in bf16 over the scores; V as it lies, keys by head dim).
 //   warps 0-3, 4-7  softmax of row tile 0 / 1, a row a thread: scores from TMEM, mask, exponentials,
 //                   P into TMEM, and the output at the end
-//   warp 8          issues the products
-//   warp 9          TMA: Q, and the pages' rows into a ring of five 32 KB tiles
+//   warps 8, 11     issue the products of row tile 0 / 1
+//   warp 10         clears what a last V tile holds past the last key
+//   warp 9          TMA: Q, and the pages' rows into a ring of four 32 KB tiles
 // Two row tiles (a pair) take each key tile in turn, so one's softmax runs under the other's
 // products. A lone row tile (streams, short prompts) takes the key tiles in turn as two halves,
-// even and odd ones, whose results are joined at the end: the same overlap, and 160 KB of loads in
+// even and odd ones, whose results are joined at the end: the same overlap, and 128 KB of loads in
 // flight for a cache that is read once.
 //
 // The reference m of a row follows the maximum only when that moves by more than 2^8 (the rows'
@@ -222,34 +223,44 @@ struct PaArgs {
   PaPlan plan;
 };
 
-constexpr int PA_THREADS = 384;  // two softmax warpgroups, and one of which two warps work
+constexpr int PA_THREADS = 384;  // two softmax warpgroups, and one of four single workers
 // Registers a thread: 168 at launch (65,536 over 384 threads); 2 * 216 + 72 = 3 * 168.
 constexpr int PA_REGS_SOFTMAX = 216, PA_REGS_OTHER = 72;
 constexpr int PA_TILE_BYTES = PA_KEYS * PA_D * 2;  // 32 KB: two halves of 64 dims, 128-byte rows
 constexpr int PA_HALF = PA_TILE_BYTES / 2;
-constexpr int PA_RING = 5;
+constexpr int PA_RING = 4;
+constexpr int PA_STAGE = 4096;  // output staging of a softmax warp: 32 rows of 128 bytes
 constexpr int PA_NBAD = 8;
-constexpr size_t PA_SMEM = (2 + PA_RING) * PA_TILE_BYTES + 512 + 2 * PA_ROWS * 8;
+constexpr size_t PA_SMEM = (2 + PA_RING) * PA_TILE_BYTES + 8 * PA_STAGE + 512 + 2 * PA_ROWS * 8;
 
 // The segments of a CTA's share, in order; every warp walks them by itself.
 struct PaWalk {
+  const PaTile* tiles;
   PaStart at, end;
   int t0, t1;
   PaTile rec;
-  __device__ PaWalk(const PaPlan& p) : at(p.start[blockIdx.x]), end(p.start[blockIdx.x + 1]) {}
-  __device__ bool next(const PaPlan& p) {
-    const bool same = at.tile == end.tile && at.head == end.head;
-    if (at.tile > end.tile || (at.tile == end.tile && at.head > end.head) ||
-        (same && at.t >= end.t))
-      return false;
-    rec = p.tiles[at.tile];
+  __device__ explicit PaWalk(const PaPlan& p)
+      : tiles(p.tiles), at(p.start[blockIdx.x]), end(p.start[blockIdx.x + 1]) {
+    if (more()) rec = tiles[at.tile];
+  }
+  __device__ bool more() const {
+    if (at.tile != end.tile) return at.tile < end.tile;
+    return at.head != end.head ? at.head < end.head : at.t < end.t;
+  }
+  __device__ bool next() {
+    if (!more()) return false;
     t0 = at.t;
-    t1 = same ? end.t : rec.ntile;
+    t1 = at.tile == end.tile && at.head == end.head ? end.t : rec.ntile;
     return true;
   }
-  __device__ void step(int Hkv) {
+  // The record of the segment after this one: fetched early, for step().
+  __device__ PaTile ahead(int Hkv) const {
+    return at.head + 1 == Hkv && at.tile < end.tile ? tiles[at.tile + 1] : rec;
+  }
+  __device__ void step(int Hkv, const PaTile& then) {
     at.t = 0;
     if (++at.head == Hkv) at.head = 0, ++at.tile;
+    rec = then;
   }
 };
 
@@ -259,39 +270,121 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The order of a part's n K and n V tiles in the ring, by place: K0 V0 K1 V1 ... (pair), or
+// K0 K1 V0 K2 V1 K3 ...: V tile t as 2 t + 1, K tile t as 2 t.
+__device__ __forceinline__ int pa_ring(int place, int n, bool pair) {
+  if (pair) return place;
+  if (place < 2) return place == 0 ? 0 : n > 1 ? 2 : 1;
+  if (place >= 2 * n - 2) return 2 * (place - n) + 1;  // the last two V
+  return place & 1 ? place + 1 : place - 1;            // K tile (place + 1) / 2, V tile place / 2 - 1
+}
+
+// Whether the part that ends with key tile t1 has keys past the segment's end in its last tile.
+__device__ __forceinline__ bool pa_tail(const PaTile& r, int t1) {
+  return r.key0 + t1 * PA_KEYS > r.key_end;
+}
+
+// Two fp32 values in one 64-bit register: the packed operations issue two lanes' work at once.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void f2_get(F2 a, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v));
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+// Bits [lo, hi) of a word.
+__device__ __forceinline__ uint32_t key_bits(int lo, int hi) {
+  const uint32_t from = lo <= 0 ? ~0u : lo >= 32 ? 0u : ~0u << lo;
+  const uint32_t to = hi <= 0 ? 0u : hi >= 32 ? ~0u : ~(~0u << hi);
+  return from & to;
+}
+
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// A bounded wait with one verdict for the whole warp.
+// The weights of 32 keys: p = bf16 pairs of 2^(s c - mc), their sum added to sum.
+__device__ __forceinline__ void weights32(const float* s, F2 c, F2 mc, uint32_t (&p)[16],
+                                          F2 (&sum)[2]) {
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    float e0, e1;
+    f2_get(fma2(f2(s[2 * x], s[2 * x + 1]), c, mc), e0, e1);
+    e0 = ex2(e0);
+    e1 = ex2(e1);
+    sum[x & 1] = add2(sum[x & 1], f2(e0, e1));
+    p[x] = pack2(e0, e1);
+  }
+}
+
+// A bounded wait (about two seconds) with one verdict for the whole warp; a failure's code goes to
+// *err, which ends the others' waits. Short: a wait stands in many places of the kernel, whose code
+// has to stay in the instruction cache.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+  bool got = mbar_try_wait(bar, parity);
+  if (!got) {
+    const long long t0 = clock64();
+#pragma unroll 1
+    for (uint32_t n = 1; !got; ++n) {
+      got = mbar_try_wait(bar, parity);
+      if (!got && (n & 255) == 0 &&
+          (*reinterpret_cast<volatile int*>(err) != 0 || clock64() - t0 > 4000000000LL)) {
+        atomicCAS(err, 0, code);
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, got);
 }
 
-// Both softmax warpgroups (named barrier 1): false for all if it is for one.
-__device__ __forceinline__ bool softmax_sync(bool ok) {
+// A warp's one arrival, after its TMEM accesses. (32 lanes that arrive by themselves are 32 updates
+// of one word, one after the other.)
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   tc_fence_before();
-  ok = bar_and_n<1, 256>(ok);
-  tc_fence_after();
-  return ok;
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
+// Named barriers of `n` threads (whole warps). The TMEM accesses before it are ordered before
+// those after it.
+__device__ __forceinline__ void bar_sync(int id, int n) {
+  tc_fence_before();
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
+  tc_fence_after();
+}
 __global__ void __launch_bounds__(PA_THREADS, 1)
     pa_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, const PaArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];  // 1,024: the swizzle's period
   uint8_t* sQ = smem;                       // two row tiles
   uint8_t* sKV = sQ + 2 * PA_TILE_BYTES;    // ring
-  uint64_t* full = reinterpret_cast<uint64_t*>(sKV + PA_RING * PA_TILE_BYTES);
+  uint8_t* sOut = sKV + PA_RING * PA_TILE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + 8 * PA_STAGE);
   uint64_t* empty = full + PA_RING;
   uint64_t* q_full = empty + PA_RING;
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;   // [2] scores of row tile (or half) w
-  uint64_t* p_ready = s_full + 2;   // [2] its weights are in TMEM
-  uint64_t* o_full = p_ready + 2;   // [2] its output is complete
-  uint64_t* done = o_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* p_ready = s_full + 2;   // [2][2] the weights of its key tile's halves are in TMEM
+  uint64_t* o_full = p_ready + 4;   // [2] its output is complete
+  uint64_t* tail = o_full + 2;      // [ring] a last V tile with rows to clear has landed
+  uint64_t* done = tail + PA_RING;  // [2]
+  uint64_t* turn = done + 2;        // [2] the tensor cores are w's
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
   volatile int* bad = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [PA_NBAD] per segment
   float2* ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(full) + 512);  // [2][128]
 
@@ -304,24 +397,25 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     if (threadIdx.x == 0) *err = 9;
     return;
   }
-  {
-    PaWalk w = walk;
-    if (!w.next(a.plan)) return;  // nothing for this CTA
-  }
+  if (!walk.more()) return;  // nothing for this CTA
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < PA_RING; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, 1);
+      mbar_init(empty + i, 2);  // one arrival of each w's
+      mbar_init(tail + i, 1);
     }
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);
     for (int w = 0; w < 2; ++w) {
       mbar_init(s_full + w, 1);
-      mbar_init(p_ready + w, 128);
+      mbar_init(p_ready + 2 * w, 4);  // one arrival a warp
+      mbar_init(p_ready + 2 * w + 1, 4);
       mbar_init(o_full + w, 1);
+      mbar_init(done + w, 1);
+      mbar_init(turn + w, 1);
     }
-    mbar_init(done, 1);
+    mbar_arrive(turn);  // row tile 0 is first
     fence_mbar_init();
   }
   if (warp == 8) {
@@ -336,61 +430,66 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   if (warp >= 8) {  // one setmaxnreg for the whole warpgroup
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_OTHER));
   if (warp == 9) {
-    // ---- loads: per segment the first key tiles, Q, then V and K in the order of use ----
+    // ---- loads: per segment Q, and K and V tiles in the order of use ----
     int rc = 0, seg = 0, nq = 0;  // ring tiles, segments and Q tiles so far
     bool ok = true;
     const int boxes = PA_KEYS / a.R;  // pages a tile; lanes [0, 2 boxes): (page, half)
     const bool mine = lane < 2 * boxes;
     const int half = lane & 1, box = lane >> 1;
-    for (; ok && walk.next(a.plan); walk.step(a.Hkv), ++seg) {
-      const PaTile r = walk.rec;
-      const int lead = r.pair ? 1 : 2, n = walk.t1 - walk.t0;
+    for (; ok && walk.next(); ++seg) {
+      const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
+      const int n = walk.t1 - walk.t0;
+      const bool clear = pa_tail(r, walk.t1);
       if (lane == 0) bad[seg % PA_NBAD] = 0;
       __syncwarp();
       const int npage = (r.key_end + a.R - 1) / a.R;  // pages the rows need
       const int* row = a.table + (long long)r.row * a.M;
-      // this lane's page of key tile i: the pool's page count (it reads as zeros) past the end
-      auto page_of = [&](int i) {
-        const int c = (r.key0 + (walk.t0 + i) * PA_KEYS) / a.R + box;
-        if (!mine || i >= n || c >= npage) return a.P;
-        const int p = c < a.M ? __ldg(row + c) : -1;
-        if (p >= 0 && p < a.P) return p;
-        bad[seg % PA_NBAD] = 1;
-        return a.P;
+      // this lane's column of the table at a place of the ring, and its entry, fetched three
+      // places ahead and looked at only when its copy goes out
+      auto column = [&](int place) {
+        const int t = walk.t0 + (pa_ring(place, n, r.pair) >> 1);
+        return (r.key0 + t * PA_KEYS) / a.R + box;
       };
-      auto load = [&](const CUtensorMap* m, int page) {
-        const int s = rc % PA_RING;
-        if (!warp_wait(empty + s, ((rc / PA_RING) & 1) ^ 1, err, 1)) return false;
-        if (lane == 0) mbar_arrive_expect_tx(full + s, PA_TILE_BYTES);
+      auto entry = [&](int place) {
+        const int c = place < 2 * n ? column(place) : npage;
+        return mine && c < npage && c < a.M ? __ldg(row + c) : -1;
+      };
+      int e0 = entry(0), e1 = entry(1), e2 = entry(2);
+#pragma unroll 1
+      for (int place = 0; place < 2 * n; ++place, ++rc) {
+        const int slot = rc % PA_RING, x = pa_ring(place, n, r.pair);
+        const int e3 = entry(place + 3);
+        if (!(ok = warp_wait(empty + slot, ((rc / PA_RING) & 1) ^ 1, err, 1))) break;
+        uint64_t* const bar = (clear && place + 1 == 2 * n ? tail : full) + slot;
+        if (lane == 0) mbar_arrive_expect_tx(bar, PA_TILE_BYTES);
+        int page = e0;
+        if ((unsigned)page >= (unsigned)a.P) {
+          page = a.P;  // outside the pool: reads as zeros
+          if (mine && column(place) < npage) bad[seg % PA_NBAD] = 1;
+        }
         __syncwarp();
         if (mine)
-          tma_load_4d(sKV + s * PA_TILE_BYTES + half * PA_HALF + box * a.R * 128, m, full + s,
-                      half * 64, 0, walk.at.head, page);
-        ++rc;
-        return true;
-      };
-      int p0 = page_of(0), p1 = page_of(1), p2 = page_of(2);
-      ok = load(&tm_k, p0);
-      if (ok && lead == 2 && n > 1) ok = load(&tm_k, p1);
-      if (ok) ok = warp_wait(q_empty, (seg & 1) ^ 1, err, 2);
-      nq += ok;
-      if (ok && lane == 0) {
-        const uint32_t bytes = 128 * G * tq;
-        mbar_arrive_expect_tx(q_full, (r.pair ? 4 : 2) * bytes);
-        for (int w = 0; w <= r.pair; ++w)
-          for (int f = 0; f < 2; ++f)
-            tma_load_3d(sQ + w * PA_TILE_BYTES + f * PA_HALF, &tm_q, q_full, f * 64,
-                        walk.at.head * G, r.q0 + w * tq);
+          tma_load_4d(sKV + slot * PA_TILE_BYTES + half * PA_HALF + box * a.R * 128,
+                      x & 1 ? &tm_v : &tm_k, bar, half * 64, 0, walk.at.head, page);
+        e0 = e1;
+        e1 = e2;
+        e2 = e3;
+        if (place == 0) {
+          if (!(ok = warp_wait(q_empty, (seg & 1) ^ 1, err, 2))) {
+            ++rc;
+            break;
+          }
+          ++nq;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(q_full, (r.pair ? 4 : 2) * 128 * G * tq);
+            for (int f = 0; f < (r.pair ? 4 : 2); ++f)
+              tma_load_3d(sQ + f * PA_HALF, &tm_q, q_full, (f & 1) * 64, walk.at.head * G,
+                          r.q0 + (f >> 1) * tq);
+          }
+          __syncwarp();
+        }
       }
-      __syncwarp();
-      for (int i = 0; ok && i < n; ++i) {
-        const int p3 = page_of(i + 3);
-        ok = load(&tm_v, p0);
-        if (ok && i + lead < n) ok = load(&tm_k, lead == 1 ? p1 : p2);
-        p0 = p1;
-        p1 = p2;
-        p2 = p3;
-      }
+      walk.step(a.Hkv, then);
     }
     // every copy issued has landed before the CTA ends (bounded, also after a failed wait)
     const long long t0 = clock64();
@@ -400,193 +499,190 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
     while (nq > 0 && !mbar_try_wait(q_full, (nq - 1) & 1) && clock64() - t0 < 4000000000LL) {
     }
-  } else if (warp == 8) {
-    // ---- products ----
+  } else if (warp == 8 || warp == 11) {
+    // ---- products of row tile (or half of the keys) w: lane 0 issues, the warp stays together so
+    // that all operands are uniform. The tensor cores hold only two or three products ahead, an
+    // issue waits for room and every wait costs 115 cycles or more, so each w has a warp of its
+    // own: one's waits pass under the other's products. Both see every tile of the ring go by (a
+    // skipped phase of a barrier could not be told from the next); one that w does not use it
+    // gives back at once, the others its softmax warps do. ----
+    const int w = warp == 11;
     int rc = 0, seg = 0;
     bool ok = true;
-    uint32_t p_phase[2] = {0, 0};
+    uint32_t p_phase = 0, turn_phase = 0;
+    const uint32_t one = lane == 0;
     const uint32_t id_qk = idesc_bf16(PA_ROWS, PA_KEYS);
     const uint32_t id_pv = idesc_bf16(PA_ROWS, PA_D) | IDESC_B_MN;
-    const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
-    for (; ok && walk.next(a.plan); walk.step(a.Hkv), ++seg) {
-      const PaTile r = walk.rec;
+    const uint32_t q_lo = sw128_lo(smem_u32(sQ)), k_lo = sw128_lo(smem_u32(sKV));
+    const uint32_t v_lo = sw128_lo_mn(smem_u32(sKV), PA_HALF);
+    const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
+    for (; ok && walk.next(); ++seg) {
+      const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
       const int n = walk.t1 - walk.t0;
-      // key tiles of this part that half w takes: [0, lim[w]) (pair), or every second one
-      const int lim0 = r.pair ? min(n, max(0, r.ntile0 - walk.t0)) : n;
-      auto wait_full = [&]() {
-        const bool got = warp_wait(full + rc % PA_RING, (rc / PA_RING) & 1, err, 3);
-        tc_fence_after();
-        return got;
-      };
-      auto qk = [&](int w, int slot) {
-        if (lane == 0) {
-          // opaque: or the 16 descriptors of every call site are kept in registers throughout
-          uint32_t q = q_addr + (r.pair ? w * PA_TILE_BYTES : 0);
-          uint32_t k = kv_addr + slot * PA_TILE_BYTES;
-          asm volatile("" : "+r"(q), "+r"(k));
+      const int lim = r.pair && w == 0 ? min(n, max(0, r.ntile0 - walk.t0)) : n;
+      const int step = r.pair ? 1 : 2, first = r.pair ? 0 : w;
+      uint32_t slot = 0;  // the tile at hand, in 16-byte units
+      auto qk = [&](int t) {
+        const uint32_t q = q_lo + (r.pair ? w * (PA_TILE_BYTES >> 4) : 0), k = k_lo + slot;
 #pragma unroll
-          for (int s = 0; s < PA_D / 16; ++s) {
-            const uint32_t off = (s >> 2) * PA_HALF + (s & 3) * 32;
-            umma_bf16(tmem + w * 128, sw128_desc(q + off), sw128_desc(k + off), id_qk, s > 0);
-          }
-          umma_commit(s_full + w);
+        for (int s = 0; s < PA_D / 16; ++s) {
+          const uint32_t off = ((s >> 2) * PA_HALF + (s & 3) * 32) >> 4;
+          umma_bf16_warp(one, tS, q + off, k + off, SW128_HI, id_qk, s > 0);
         }
-        __syncwarp();
+        umma_commit_warp(one, s_full + w);
+        if (t + step >= lim) umma_commit_warp(one, q_empty);  // the last use of Q
       };
-      auto pv = [&](int w, int slot, bool first) {
-        if (lane == 0) {
-          uint32_t v = kv_addr + slot * PA_TILE_BYTES;
-          asm volatile("" : "+r"(v));
+      // The two warps take turns, each with a weights' and a score product: left alone they fall
+      // into step, both row tiles' products at once and then both softmaxes.
+      auto turn_wait = [&]() {
+        ok = ok && warp_wait(turn + w, turn_phase, err, 9);
+        turn_phase ^= 1;
+      };
+      auto turn_pass = [&]() {
+        if (ok && lane == 0) mbar_arrive(turn + 1 - w);
+      };
+      // O += P V, as soon as each half of the weights is there
+      auto pv = [&](int t) {
+        const uint32_t v = v_lo + slot;
 #pragma unroll
-          for (int s = 0; s < PA_KEYS / 16; ++s)
-            umma_bf16_ts(tmem + 256 + w * 128, tmem + w * 128 + s * 8,
-                         sw128_desc_mn(v + s * 2048, PA_HALF), id_pv, !(first && s == 0));
+        for (int half = 0; half < 2; ++half) {
+          ok = ok && warp_wait(p_ready + 2 * w + half, p_phase, err, 4);
+          if (half == 0) turn_wait();
+          if (!ok) return;
+          tc_fence_after();
+#pragma unroll
+          for (int s = 4 * half; s < 4 * half + 4; ++s)
+            umma_bf16_ts_warp(one, tO, tS + s * 8, v + s * (2048 >> 4), SW128_HI, id_pv,
+                              s > 0 || t != first);
         }
-        __syncwarp();
+        p_phase ^= 1;
+        if (t + step >= lim) umma_commit_warp(one, o_full + w);
       };
-      auto commit = [&](uint64_t* b) {
-        if (lane == 0) umma_commit(b);
-        __syncwarp();
-      };
-      auto wait_p = [&](int w) {
-        const bool got = warp_wait(p_ready + w, p_phase[w], err, 4);
-        p_phase[w] ^= 1;
-        tc_fence_after();
-        return got;
-      };
-      // rows of V past the last key hold anything (also NaN): their weights are 0, they become 0
-      auto clear_tail = [&](int i, int slot) {
-        const int keep = r.key_end - (r.key0 + (walk.t0 + i) * PA_KEYS);
-        if (keep >= PA_KEYS) return;
+      ok = warp_wait(q_full, seg & 1, err, 5);
+      tc_fence_after();
+      if (ok && first >= lim && lane == 0) mbar_arrive(q_empty);
+      const int lead = r.pair ? 1 : 2;
+#pragma unroll 1
+      for (int place = 0; ok && place < 2 * n; ++place, ++rc) {
+        const int x = pa_ring(place, n, r.pair), t = x >> 1, s = rc % PA_RING;
+        const bool own = r.pair || (t & 1) == w;
+        const bool use = own && t < lim;
+        if (!(ok = warp_wait(full + s, (rc / PA_RING) & 1, err, 3))) break;
+        if (!use && lane == 0) mbar_arrive(empty + s);
+        slot = __shfl_sync(0xffffffffu, (uint32_t)s * (PA_TILE_BYTES >> 4), 0);
+        if (x & 1) {
+          if (use) pv(t);
+          else if (own) turn_wait();
+          if (own && t + lead >= n) turn_pass();
+        } else {
+          if (use) qk(t);
+          if (own && t >= lead) turn_pass();
+        }
+      }
+      if (!r.pair && (n & 1) && w == 1) {  // as many turns for both
+        turn_wait();
+        turn_pass();
+      }
+      walk.step(a.Hkv, then);
+    }
+    umma_commit_warp(one, done + w);
+    const long long t0 = clock64();
+    while (!mbar_try_wait(done + w, 0) && clock64() - t0 < 4000000000LL) {
+    }
+  } else if (warp == 10) {
+    // ---- rows of V past the last key hold anything (also NaN): their weights are 0, they become
+    // 0 too. The last V tile of such a segment lands here first and is passed on when clear. ----
+    // A barrier a slot: a second such tile may be under way before the first has landed.
+    int rc = 0;
+    uint32_t phases = 0;
+    bool ok = true;
+    for (; ok && walk.next();) {
+      const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
+      rc += 2 * (walk.t1 - walk.t0);
+      if (pa_tail(r, walk.t1)) {
+        const int slot = (rc - 1) % PA_RING;  // a part's last tile in the ring is its last V
+        ok = warp_wait(tail + slot, phases >> slot & 1, err, 8);
+        phases ^= 1u << slot;
         uint8_t* v = sKV + slot * PA_TILE_BYTES;
-        for (int x = max(keep, 0) * 8 + lane; x < PA_KEYS * 8; x += 32) {
+        const int keep = max(0, r.key_end - (r.key0 + (walk.t1 - 1) * PA_KEYS));
+        for (int x = keep * 8 + lane; ok && x < PA_KEYS * 8; x += 32) {
           *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0, 0, 0, 0);
           *reinterpret_cast<uint4*>(v + PA_HALF + x * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         __syncwarp();
-      };
-      ok = warp_wait(q_full, seg & 1, err, 5);
-      if (!ok) break;
-      if (r.pair) {
-        if (!(ok = wait_full())) break;
-        if (lim0 > 0) qk(0, rc % PA_RING);
-        qk(1, rc % PA_RING);
-        commit(empty + rc % PA_RING);
-        if (n == 1) commit(q_empty);
-        ++rc;
-        for (int i = 0; ok && i < n; ++i) {
-          if (!(ok = wait_full())) break;
-          const int vs = rc % PA_RING;
-          clear_tail(i, vs);
-          ++rc;
-          const bool more = i + 1 < n;
-          const int ks = rc % PA_RING;
-          if (i < lim0) {
-            if (!(ok = wait_p(0))) break;
-            pv(0, vs, i == 0);
-            if (i + 1 == lim0) commit(o_full);
-          }
-          if (more && !(ok = wait_full())) break;
-          if (i + 1 < lim0) qk(0, ks);
-          if (!(ok = wait_p(1))) break;
-          pv(1, vs, i == 0);
-          commit(empty + vs);
-          if (!more) commit(o_full + 1);
-          if (more) {
-            qk(1, ks);
-            commit(empty + ks);
-            if (i + 2 == n) commit(q_empty);
-            ++rc;
-          }
-        }
-      } else {
-        for (int w = 0; ok && w < 2 && w < n; ++w) {
-          if (!(ok = wait_full())) break;
-          qk(w, rc % PA_RING);
-          commit(empty + rc % PA_RING);
-          if (w + 1 == n) commit(q_empty);
-          ++rc;
-        }
-        for (int i = 0; ok && i < n; ++i) {
-          const int w = i & 1;
-          if (!(ok = wait_full())) break;
-          const int vs = rc % PA_RING;
-          clear_tail(i, vs);
-          ++rc;
-          if (!(ok = wait_p(w))) break;
-          pv(w, vs, i < 2);
-          commit(empty + vs);
-          if (i + 2 >= n) commit(o_full + w);
-          if (i + 2 < n) {
-            if (!(ok = wait_full())) break;
-            qk(w, rc % PA_RING);
-            commit(empty + rc % PA_RING);
-            if (i + 3 == n) commit(q_empty);
-            ++rc;
-          }
-        }
+        if (ok && lane == 0) mbar_arrive(full + slot);
       }
-    }
-    if (lane == 0) umma_commit(done);
-    __syncwarp();
-    const long long t0 = clock64();
-    while (!mbar_try_wait(done, 0) && clock64() - t0 < 4000000000LL) {
+      walk.step(a.Hkv, then);
     }
   }
+  __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_REGS_SOFTMAX));
-    // ---- softmax: warpgroup w, thread = row ----
+    // ---- softmax: warpgroup w, a row a thread ----
     const int w = warp >> 2, row = threadIdx.x & 127;
+    const int quad_bar = 1 + (warp & 3);  // the two warps of the same 32 rows
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;  // lane field: 32 (warp & 3) << 16
     const uint32_t tS = tmem + w * 128 + quarter, tO = tmem + 256 + quarter;
     const float c = a.scale_log2;
-    const int prefix = head->prefix, window = head->window;
+    const int prefix = head->prefix, window = head->window, nprefix = head->nprefix;
     uint32_t s_phase = 0, o_phase = 0;
-    int seg = 0;
+    int seg = 0, rc = 0;
+    // After a failed wait a warp arrives at no mbarrier any more (each role has then done a prefix
+    // of what it does otherwise, and the others' waits end too); the softmax warps still meet at
+    // their named barriers.
     bool ok = true;
-    // after a failed wait the group only meets the other one at its barriers
-    for (; walk.next(a.plan); walk.step(a.Hkv), ++seg) {
-      const PaTile r = walk.rec;
+    for (; walk.next(); ++seg) {
+      const PaTile& r = walk.rec;
       const int n = walk.t1 - walk.t0;
-      const int lim0 = r.pair ? min(n, max(0, r.ntile0 - walk.t0)) : n;
       // this row's token and the keys [lo, hi) it sees
-      const int i0 = r.pair ? w * tq : 0, i = i0 + row / G;
+      const int i = (r.pair ? w * tq : 0) + row / G;
       const bool valid = row < tq * G && i < r.nq;
       int lo = 0, hi = 1 << 30;
       if (valid) {
-        const int kv = r.kind == PA_PROMPT ? r.pos0 + i + 1 : a.plan.kv[r.q0 + i];
+        const int kv = r.kind == PA_PROMPT ? r.pos0 + i + 1
+                       : r.kind == PA_OWN  ? r.key_end
+                                           : a.plan.kv[r.q0 + i];
         hi = r.kind == PA_PREFIX ? min(prefix, kv) : kv;
         lo = window ? max(0, kv - window) : 0;
         if (r.kind == PA_OWN) lo = max(lo, prefix);
       }
       const bool active = __any_sync(0xffffffffu, valid);
+      const bool whole = walk.t0 == 0 && walk.t1 == r.ntile && (r.kind == PA_PROMPT || prefix == 0);
+      const long long at = (long long)(r.q0 + i) * a.Hq + walk.at.head * G + row % G;
+      // fetched now, looked at at the end
+      const __nv_bfloat16 gb = valid && whole && a.gate ? a.gate[at] : __nv_bfloat16();
       float m = -INFINITY, l = 0.f;
-      const int first = r.pair ? 0 : w, stride = r.pair ? 1 : 2;
-      const int last = r.pair && w == 0 ? lim0 : n;
-      bool any = false;  // this half has a key tile
-      for (int t = first; ok && t < last; t += stride) {
-        if (!(ok = warp_wait(s_full + w, s_phase, err, 6))) break;
+      const int stride = r.pair ? 1 : 2;
+      const int last = r.pair && w == 0 ? min(n, max(0, r.ntile0 - walk.t0)) : n;
+      bool any = false;  // this row tile (or half of the keys) has a key tile
+      const int last_t = n - 1 - (n - 1 - w & 1);  // half w's last key tile
+      int kb = r.key0 + (walk.t0 + (r.pair ? 0 : w)) * PA_KEYS;
+      for (int t = r.pair ? 0 : w; t < last; t += stride, kb += stride * PA_KEYS) {
+        ok = ok && warp_wait(s_full + w, s_phase, err, 6);
         s_phase ^= 1;
         tc_fence_after();
-        if (active) {
-          const int kb = r.key0 + (walk.t0 + t) * PA_KEYS;
-          float s[4][32];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) tmem_ld32(tS + 32 * j, s[j]);
-          tmem_ld_wait_all();
-#pragma unroll
-          for (int j = 0; j < 4; ++j) keep32(s[j]);
+        // these scores are there: so the products are through with their K tile and with the V
+        // tile of the weights before
+        if (ok && (threadIdx.x & 127) == 0) {
+          mbar_arrive(empty + (rc + (r.pair ? 2 * t : t < 2 ? t : 2 * t - 1)) % PA_RING);
+          if (any) mbar_arrive(empty + (rc + (r.pair ? 2 * t - 1 : 2 * t - 2)) % PA_RING);
+        }
+        if (active && ok) {
+          float s[128];
+          tmem_ld128_wait(tS, s);
           if (__any_sync(0xffffffffu, valid && (kb < lo || kb + PA_KEYS > hi))) {
 #pragma unroll
-            for (int j = 0; j < 128; ++j)
-              if (kb + j < lo || kb + j >= hi) s[j >> 5][j & 31] = -INFINITY;
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t seen = key_bits(lo - kb - 32 * j, hi - kb - 32 * j);
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                if (!(seen >> x & 1)) s[32 * j + x] = -INFINITY;
+            }
           }
-          float mx[4] = {s[0][0], s[1][0], s[2][0], s[3][0]};
+          float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int j = 1; j < 32; ++j)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) mx[x] = fmaxf(mx[x], s[x][j]);
+          for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
           const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           const bool move = tm > m && (tm - m) * c > 8.f;  // also from m = -inf
           if (!any) {
@@ -597,60 +693,61 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             l *= f;
 #pragma unroll 1
             for (int j = 0; j < PA_D; j += 16) {
-              uint32_t o[16];
-              tmem_ld16(tO + w * 128 + j, o);
-              tmem_ld_wait(o);
+              float o[16];
+              uint32_t y[16];
+              tmem_ld16_wait(tO + w * 128 + j, o);
 #pragma unroll
-              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-              tmem_st16(tO + w * 128 + j, o);
+              for (int x = 0; x < 16; ++x) y[x] = __float_as_uint(o[x] * f);
+              tmem_st16(tO + w * 128 + j, y);
             }
           }
           const float mc = m == -INFINITY ? 0.f : m * c;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const F2 c2 = f2(c, c), mc2 = f2(-mc, -mc);
+          F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t p[32];
-#pragma unroll
-            for (int x = 0; x < 32; ++x) {
-              const float e0 = ex2(fmaf(s[2 * j + (x >> 4)][2 * x & 31], c, -mc));
-              const float e1 = ex2(fmaf(s[2 * j + (x >> 4)][(2 * x & 31) + 1], c, -mc));
-              sum[x & 3] += e0 + e1;
-              p[x] = pack2(e0, e1);
+          for (int j = 0; j < 4; ++j) {
+            uint32_t p[16];
+            weights32(s + 32 * j, c2, mc2, p, sum);
+            tmem_st16(tS + 16 * j, p);
+            if (j & 1) {
+              tmem_st_wait();
+              warp_arrive(p_ready + 2 * w + (j >> 1));
             }
-            tmem_st32(tS + 32 * j, p);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_st_wait();
+          float l0, l1;
+          f2_get(add2(sum[0], sum[1]), l0, l1);
+          l += l0 + l1;
+        } else if (ok) {
+          warp_arrive(p_ready + 2 * w);
+          warp_arrive(p_ready + 2 * w + 1);
         }
         any = true;
-        tc_fence_before();
-        mbar_arrive(p_ready + w);
       }
-      // ---- output ----
-      if (ok && any) {
-        ok = warp_wait(o_full + w, o_phase, err, 7);
+      const PaTile then = walk.ahead(a.Hkv);
+      // ---- output: a pair's row tile, else both halves' sum, 64 columns a thread ----
+      if (any) {
+        ok = ok && warp_wait(o_full + w, o_phase, err, 7);
         o_phase ^= 1;
         tc_fence_after();
+        if (ok && (threadIdx.x & 127) == 0)  // the last V
+          mbar_arrive(empty + (rc + (r.pair ? 2 * last - 1 : min(2 * last_t + 2, n + last_t))) %
+                                  PA_RING);
       }
-      if (r.pair && !ok) continue;
-      if (bad[seg % PA_NBAD]) l = NAN;
-      const bool whole = walk.t0 == 0 && walk.t1 == r.ntile && (r.kind == PA_PROMPT || prefix == 0);
-      // a pair: all columns of the own row tile; else columns [64 w, 64 w + 64) of both halves
-      float f0 = 1.f, f1 = 0.f;
-      bool has0 = any, has1 = false;
-      if (!r.pair) {
-        ml[w * PA_ROWS + row] = make_float2(m, l);
-        if (!(ok = softmax_sync(ok))) continue;
-        const float2 x0 = ml[row], x1 = ml[PA_ROWS + row];
-        m = fmaxf(x0.x, x1.x);
-        f0 = x0.x == -INFINITY ? 0.f : ex2((x0.x - m) * c);
-        f1 = x1.x == -INFINITY ? 0.f : ex2((x1.x - m) * c);
-        l = x0.y * f0 + x1.y * f1;
-        if (bad[seg % PA_NBAD]) l = NAN;
-        has0 = true;
-        has1 = n > 1;
-      }
+      rc += 2 * n;
       if (active) {
+        if (bad[seg % PA_NBAD] || !ok) l = NAN;
+        float f0 = any ? 1.f : 0.f, f1 = 0.f;
+        if (!r.pair) {
+          ml[w * PA_ROWS + row] = make_float2(m, l);
+          bar_sync(quad_bar, 64);
+          const float2 x0 = ml[row], x1 = ml[PA_ROWS + row];
+          m = fmaxf(x0.x, x1.x);
+          f0 = x0.x == -INFINITY ? 0.f : ex2((x0.x - m) * c);
+          f1 = x1.x == -INFINITY ? 0.f : ex2((x1.x - m) * c);
+          l = x0.y * f0 + (n > 1 ? x1.y * f1 : 0.f);
+          if (bad[seg % PA_NBAD] || !ok) l = NAN;
+        }
+        const bool has0 = any || !r.pair, has1 = !r.pair && n > 1;
         const int rr = (r.pair ? w * PA_ROWS : 0) + row;
         float* slot = nullptr;
         int rows = PA_WIDE_ROWS;
@@ -662,52 +759,74 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                    ((size_t)walk.at.tile * a.Hkv + walk.at.head + blockIdx.x) * pa_slot_floats(rows);
           } else {
             rows = pa_own_rows(a.Hq, a.Hkv);
-            slot = a.plan.own + ((size_t)(walk.at.tile - head->nprefix) * a.Hkv + walk.at.head +
+            slot = a.plan.own + ((size_t)(walk.at.tile - nprefix) * a.Hkv + walk.at.head +
                                  blockIdx.x) * pa_slot_floats(rows);
           }
           if (valid && (r.pair || w == 0))
             reinterpret_cast<float2*>(slot)[rr] = make_float2(m, l);
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int tok = r.q0 + i, qh = walk.at.head * G + row % G;
-        const float g = valid && whole && a.gate ? bf2f(a.gate[(long long)tok * a.Hq + qh]) : 1.f;
-        const int j0 = r.pair ? 0 : 2 * w, j1 = r.pair ? 4 : 2 * w + 2;
-        for (int j = j0; j < j1; ++j) {
-          float x0[32], x1[32];
-          if (has0) tmem_ld32(tO + (r.pair ? w * 128 : 0) + 32 * j, x0);
-          if (has1) tmem_ld32(tO + 128 + 32 * j, x1);
-          tmem_ld_wait_all();
-          keep32(x0);
-          keep32(x1);
-          float o[32];
+        const float g = bf2f(gb);
+        if (whole) {  // the sum's reciprocal; a row without a key is 0
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          f0 *= inv;
+          f1 *= inv;
+        }
+        uint8_t* const stage = sOut + warp * PA_STAGE;
+#pragma unroll 1
+        for (int hc = r.pair ? 0 : w; hc < (r.pair ? 2 : w + 1); ++hc) {  // 64 columns at a time
+#pragma unroll 1
+          for (int j = 2 * hc; j < 2 * hc + 2; ++j) {
+            float o[32];
+            tmem_ld32_wait(tO + (r.pair ? w * 128 : 0) + 32 * j, o);
 #pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            o[x] = has0 ? x0[x] * f0 : 0.f;
-            if (has1) o[x] = fmaf(x1[x], f1, o[x]);
-          }
-          if (!valid) continue;
-          if (whole) {
-            uint4* dst = reinterpret_cast<uint4*>(a.out + ((long long)tok * a.Hq + qh) * PA_D + 32 * j);
-            uint32_t y[16];
+            for (int x = 0; x < 32; ++x) o[x] = has0 ? o[x] * f0 : 0.f;
+            if (has1) {
+              float o1[32];
+              tmem_ld32_wait(tO + 128 + 32 * j, o1);
 #pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              float u = o[2 * x] * inv, v = o[2 * x + 1] * inv;
-              if (l == 0.f) u = v = 0.f;
-              if (a.gate) u = round_bf16(u) * g, v = round_bf16(v) * g;
-              y[x] = pack2(u, v);
+              for (int x = 0; x < 32; ++x) o[x] = fmaf(o1[x], f1, o[x]);
             }
+            if (whole) {
+              // 16-byte chunk k of row `lane` at k ^ (lane & 7): no bank conflicts either way
 #pragma unroll
-            for (int x = 0; x < 4; ++x) dst[x] = make_uint4(y[4 * x], y[4 * x + 1], y[4 * x + 2], y[4 * x + 3]);
-          } else {
-            float4* po = reinterpret_cast<float4*>(slot + 2 * rows);
+              for (int k = 0; k < 4; ++k) {
+                uint32_t y[4];
 #pragma unroll
-            for (int x = 0; x < 8; ++x)
-              po[(8 * j + x) * rows + rr] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                for (int x = 0; x < 4; ++x) {
+                  float u = o[8 * k + 2 * x], v = o[8 * k + 2 * x + 1];
+                  if (a.gate) u = round_bf16(u) * g, v = round_bf16(v) * g;
+                  y[x] = pack2(u, v);
+                }
+                *reinterpret_cast<uint4*>(stage + lane * 128 +
+                                          ((4 * (j & 1) + k) ^ (lane & 7)) * 16) =
+                    make_uint4(y[0], y[1], y[2], y[3]);
+              }
+            } else if (valid) {
+              float4* po = reinterpret_cast<float4*>(slot + 2 * rows);
+#pragma unroll
+              for (int x = 0; x < 8; ++x)
+                po[(8 * j + x) * rows + rr] =
+                    make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+            }
+            __syncwarp();
+          }
+          if (whole) {  // whole 128-byte lines: 8 lanes a row
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int src = 4 * k + (lane >> 3);
+              const long long to = __shfl_sync(0xffffffffu, valid ? at : -1LL, src);
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + src * 128 +
+                                                              ((lane & 7) ^ (src & 7)) * 16);
+              if (to >= 0)
+                *reinterpret_cast<uint4*>(a.out + to * PA_D + 64 * hc + (lane & 7) * 8) = v;
+            }
+            __syncwarp();
           }
         }
+        // neither half's O or ml is overwritten before both have read it
+        if (!r.pair) bar_sync(quad_bar, 64);
       }
-      // neither half's O or ml is overwritten before both groups have read it
-      if (!r.pair) ok = softmax_sync(ok);
+      walk.step(a.Hkv, then);
     }
   }
   tc_fence_before();

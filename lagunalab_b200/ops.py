@@ -6,6 +6,8 @@ Packed MLX words are carried as ``torch.int32`` tensors holding the uint32 bit p
 (``torch.uint32`` has too few kernels to be practical); ``torch.uint32`` inputs are viewed
 as int32.
 """
+import ctypes
+
 import torch
 
 from . import _lib
@@ -770,6 +772,14 @@ class AttentionPlan:
             _call_on(self.device, "lg_stream_plan", _p(self.kv_len), self.B, self.Hq, self.Hkv,
                      self.page_rows, self.prefix, self.window, _p(self.buf), self.nbytes, st)
         return self
+
+
+    def status(self):
+        """0, or the code of a wait that ran out in a call with this plan. Waits for the device."""
+        st = ctypes.c_int(0)
+        torch.cuda.synchronize(self.device)
+        _call_on(self.device, "lg_plan_status", _p(self.buf), ctypes.byref(st))
+        return st.value
 
 
 def prompt_plan(cu_q, kv_len, T, Hq, Hkv, page_rows, window=0):

@@ -269,3 +269,18 @@ def test_streams_of_their_own():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_runs_of_one_tile_segments():
+    """Many row tiles a CTA, each with one key tile that ends inside a page: the next one's loads
+    are under way while this one's rows are cleared."""
+    from lagunalab_b200 import ops
+    r = random.Random(2)
+    kv = [r.randint(1, 127) for _ in range(2500)]
+    q, k, v, table, cu, kvt, _ = _case([1] * len(kv), kv, 4, 4, 128, seed=8)
+    plan = ops.prompt_plan(cu, kvt, q.shape[0], 4, 4, 128)
+    for _ in range(5):
+        got = ops.prompt_attention(q, k, v, table, plan, 0.1)
+    out, A = _exact(q, k, v, table, [1] * len(kv), kv, 0.1, None, 0)
+    _near(got, out, A, len(kv))
+    assert plan.status() == 0
