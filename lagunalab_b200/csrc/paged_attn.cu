@@ -454,11 +454,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const int c = place < 2 * n ? column(place) : npage;
         return mine && c < npage && c < a.M ? __ldg(row + c) : -1;
       };
-      int e0 = entry(0), e1 = entry(1), e2 = entry(2);
+      int e0 = -1, e1 = -1, e2 = -1, e3 = -1;
 #pragma unroll 1
-      for (int place = 0; place < 2 * n; ++place, ++rc) {
+      for (int place = -3; place < 2 * n; ++place) {
+        e0 = e1;
+        e1 = e2;
+        e2 = e3;
+        e3 = entry(place + 3);
+        if (place < 0) continue;
         const int slot = rc % PA_RING, x = pa_ring(place, n, r.pair);
-        const int e3 = entry(place + 3);
         if (!(ok = warp_wait(empty + slot, ((rc / PA_RING) & 1) ^ 1, err, 1))) break;
         uint64_t* const bar = (clear && place + 1 == 2 * n ? tail : full) + slot;
         if (lane == 0) mbar_arrive_expect_tx(bar, PA_TILE_BYTES);
@@ -471,14 +475,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         if (mine)
           tma_load_4d(sKV + slot * PA_TILE_BYTES + half * PA_HALF + box * a.R * 128,
                       x & 1 ? &tm_v : &tm_k, bar, half * 64, 0, walk.at.head, page);
-        e0 = e1;
-        e1 = e2;
-        e2 = e3;
+        ++rc;
         if (place == 0) {
-          if (!(ok = warp_wait(q_empty, (seg & 1) ^ 1, err, 2))) {
-            ++rc;
-            break;
-          }
+          if (!(ok = warp_wait(q_empty, (seg & 1) ^ 1, err, 2))) break;
           ++nq;
           if (lane == 0) {
             mbar_arrive_expect_tx(q_full, (r.pair ? 4 : 2) * 128 * G * tq);
@@ -651,7 +650,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const bool whole = walk.t0 == 0 && walk.t1 == r.ntile && (r.kind == PA_PROMPT || prefix == 0);
       const long long at = (long long)(r.q0 + i) * a.Hq + walk.at.head * G + row % G;
       // fetched now, looked at at the end
-      const __nv_bfloat16 gb = valid && whole && a.gate ? a.gate[at] : __nv_bfloat16();
+      const __nv_bfloat16 gb = valid && whole && a.gate ? a.gate[at] : __float2bfloat16_rn(1.f);
       float m = -INFINITY, l = 0.f;
       const int stride = r.pair ? 1 : 2;
       const int last = r.pair && w == 0 ? min(n, max(0, r.ntile0 - walk.t0)) : n;
@@ -736,18 +735,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       rc += 2 * n;
       if (active) {
         if (bad[seg % PA_NBAD] || !ok) l = NAN;
-        float f0 = any ? 1.f : 0.f, f1 = 0.f;
+        float f0 = 1.f, f1 = 0.f;
         if (!r.pair) {
           ml[w * PA_ROWS + row] = make_float2(m, l);
           bar_sync(quad_bar, 64);
           const float2 x0 = ml[row], x1 = ml[PA_ROWS + row];
           m = fmaxf(x0.x, x1.x);
           f0 = x0.x == -INFINITY ? 0.f : ex2((x0.x - m) * c);
-          f1 = x1.x == -INFINITY ? 0.f : ex2((x1.x - m) * c);
-          l = x0.y * f0 + (n > 1 ? x1.y * f1 : 0.f);
+          f1 = n < 2 || x1.x == -INFINITY ? 0.f : ex2((x1.x - m) * c);
+          l = x0.y * f0 + x1.y * f1;
           if (bad[seg % PA_NBAD] || !ok) l = NAN;
         }
-        const bool has0 = any || !r.pair, has1 = !r.pair && n > 1;
         const int rr = (r.pair ? w * PA_ROWS : 0) + row;
         float* slot = nullptr;
         int rows = PA_WIDE_ROWS;
@@ -772,45 +770,45 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           f1 *= inv;
         }
         uint8_t* const stage = sOut + warp * PA_STAGE;
+        // Four or two times 32 columns; `part` is opaque so that the loop is not written out for
+        // each kind of output (code that is not in the instruction cache took 3 us here). Without a
+        // key tile (a pair's first row tile in a late part) there is no O: m = -inf says so.
+        int part = !whole;
 #pragma unroll 1
-        for (int hc = r.pair ? 0 : w; hc < (r.pair ? 2 : w + 1); ++hc) {  // 64 columns at a time
-#pragma unroll 1
-          for (int j = 2 * hc; j < 2 * hc + 2; ++j) {
-            float o[32];
-            tmem_ld32_wait(tO + (r.pair ? w * 128 : 0) + 32 * j, o);
+        for (int j = r.pair ? 0 : 2 * w; j < (r.pair ? (any ? 4 : 0) : 2 * w + 2); ++j) {
+          asm volatile("" : "+r"(part));
+          float o[32];
+          tmem_ld32_wait(tO + (r.pair ? w * 128 : 0) + 32 * j, o);
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = has0 ? o[x] * f0 : 0.f;
-            if (has1) {
-              float o1[32];
-              tmem_ld32_wait(tO + 128 + 32 * j, o1);
+          for (int x = 0; x < 32; ++x) o[x] *= f0;
+          if (!r.pair) {
+            float o1[32];
+            tmem_ld32_wait(tO + (n > 1 ? 128 : 0) + 32 * j, o1);  // f1 = 0 without a second half
 #pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = fmaf(o1[x], f1, o[x]);
-            }
-            if (whole) {
-              // 16-byte chunk k of row `lane` at k ^ (lane & 7): no bank conflicts either way
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                uint32_t y[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                  float u = o[8 * k + 2 * x], v = o[8 * k + 2 * x + 1];
-                  if (a.gate) u = round_bf16(u) * g, v = round_bf16(v) * g;
-                  y[x] = pack2(u, v);
-                }
-                *reinterpret_cast<uint4*>(stage + lane * 128 +
-                                          ((4 * (j & 1) + k) ^ (lane & 7)) * 16) =
-                    make_uint4(y[0], y[1], y[2], y[3]);
-              }
-            } else if (valid) {
-              float4* po = reinterpret_cast<float4*>(slot + 2 * rows);
+            for (int x = 0; x < 32; ++x) o[x] = fmaf(o1[x], f1, o[x]);
+          }
+          if (part) {
+            float4* po = reinterpret_cast<float4*>(slot + 2 * rows);
+            if (valid)
 #pragma unroll
               for (int x = 0; x < 8; ++x)
                 po[(8 * j + x) * rows + rr] =
                     make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
-            }
             __syncwarp();
+            continue;
           }
-          if (whole) {  // whole 128-byte lines: 8 lanes a row
+          // 16-byte chunk k of row `lane` at k ^ (lane & 7): no bank conflicts either way
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t y[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              y[x] = pack2(round_bf16(o[8 * k + 2 * x]) * g, round_bf16(o[8 * k + 2 * x + 1]) * g);
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((4 * (j & 1) + k) ^ (lane & 7)) * 16) =
+                make_uint4(y[0], y[1], y[2], y[3]);
+          }
+          __syncwarp();
+          if (j & 1) {  // 64 columns are there: whole 128-byte lines, 8 lanes a row
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const int src = 4 * k + (lane >> 3);
@@ -818,7 +816,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
               const uint4 v = *reinterpret_cast<const uint4*>(stage + src * 128 +
                                                               ((lane & 7) ^ (src & 7)) * 16);
               if (to >= 0)
-                *reinterpret_cast<uint4*>(a.out + to * PA_D + 64 * hc + (lane & 7) * 8) = v;
+                *reinterpret_cast<uint4*>(a.out + to * PA_D + 32 * (j - 1) + (lane & 7) * 8) = v;
             }
             __syncwarp();
           }
@@ -875,7 +873,11 @@ __global__ void __launch_bounds__(256) pa_join_prompt_kernel(const PaArgs a) {
     for (int x = c0; x <= c1; ++x) {
       const float* p = a.plan.wide + (2 * x + (x == c0)) * slot;
       const float2 ml = reinterpret_cast<const float2*>(p)[rr];
-      const float f = ml.x == -INFINITY ? 0.f : ex2((ml.x - m) * a.scale_log2);
+      if (ml.x == -INFINITY) {  // no key, and maybe no O; a NaN l stays one
+        l += ml.y;
+        continue;
+      }
+      const float f = ex2((ml.x - m) * a.scale_log2);
       l += ml.y * f;
       const float4* po = reinterpret_cast<const float4*>(p + 2 * PA_WIDE_ROWS);
 #pragma unroll
@@ -928,8 +930,10 @@ __global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
   for (int e = threadIdx.x; e < G * 32; e += 128) {
     const int g = e % G, q = e / G;  // neighbours take neighbouring rows of one column quad
     float m = -INFINITY;
+#pragma unroll 2
     for (int x = p0; x <= p1; ++x)
       m = fmaxf(m, reinterpret_cast<const float2*>(wide + x * pa_slot_floats(PA_WIDE_ROWS))[rr + g].x);
+#pragma unroll 2
     for (int x = c0; x <= c1; ++x)
       m = fmaxf(m, reinterpret_cast<const float2*>(ow + x * pa_slot_floats(rows))[g].x);
     float l = 0.f;
@@ -938,13 +942,15 @@ __global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
       const float2 ml = reinterpret_cast<const float2*>(p)[r];
       const float f = ml.x == -INFINITY ? 0.f : ex2((ml.x - m) * a.scale_log2);
       const float4 v = reinterpret_cast<const float4*>(p + 2 * n)[q * n + r];
-      l += ml.y * f;
+      l += ml.x == -INFINITY ? ml.y : ml.y * f;
       o.x = fmaf(v.x, f, o.x);
       o.y = fmaf(v.y, f, o.y);
       o.z = fmaf(v.z, f, o.z);
       o.w = fmaf(v.w, f, o.w);
     };
+#pragma unroll 2
     for (int x = p0; x <= p1; ++x) add(wide + x * pa_slot_floats(PA_WIDE_ROWS), PA_WIDE_ROWS, rr + g);
+#pragma unroll 2
     for (int x = c0; x <= c1; ++x) add(ow + x * pa_slot_floats(rows), rows, g);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     float4 v = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
