@@ -149,8 +149,15 @@ def call(name, *args):
     """Call an entry point; raise ValueError for invalid arguments, LagunaError otherwise."""
     rc = getattr(lib(), name)(*args)
     if rc != LG_OK:
-        msg = lib().lg_last_error().decode(errors="replace")
-        if rc == LG_ERR_INVALID:
-            raise ValueError(msg)
-        raise LagunaError(rc, f"{name}: {msg} (status {rc})")
+        check(name, rc)
     return rc
+
+
+def check(name, rc):
+    """Raise for an entry point's error status (with the message of the thread's last call)."""
+    if rc == LG_OK:
+        return
+    msg = lib().lg_last_error().decode(errors="replace")
+    if rc == LG_ERR_INVALID:
+        raise ValueError(msg)
+    raise LagunaError(rc, f"{name}: {msg} (status {rc})")

@@ -27,6 +27,8 @@
 //
 // P is rounded to bf16 (relative 2^-8 a weight, averaged over the keys) because the tensor cores
 // take it so; l sums the unrounded weights, and O, m and l stay in fp32 through the join.
+#include <atomic>
+
 #include "paged.cuh"
 #include "tc_ptx.cuh"
 #include "tmap.cuh"
@@ -997,6 +999,18 @@ static int plan_run(const char* who, int kind, const int* cu, const int* kv, int
   return LG_OK;
 }
 
+// The kernel's shared memory limit, raised once per device.
+static int pa_smem_once() {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  LG_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 64 && done[dev].load(std::memory_order_relaxed)) return LG_OK;
+  LG_CUDA_TRY(cudaFuncSetAttribute(pa_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)PA_SMEM));
+  if (dev < 64) done[dev].store(true, std::memory_order_relaxed);
+  return LG_OK;
+}
+
 static int attn_run(const char* who, int kind, const void* q, long long q_tok, long long q_head,
                     int T, int Hq, int Hkv, int D, const void* k, const void* v, int P, int R,
                     long long pg, long long hd, long long rw, const int32_t* table, int B, int M,
@@ -1042,8 +1056,7 @@ static int attn_run(const char* who, int kind, const void* q, long long q_tok, l
   a.scale_log2 = scale * 1.4426950408889634f;
   a.plan = p;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  LG_CUDA_TRY(cudaFuncSetAttribute(pa_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   (int)PA_SMEM));
+  if (int rc = pa_smem_once()) return rc;
   pa_kernel<<<p.ncta, PA_THREADS, PA_SMEM, st>>>(tm_q, tm_k, tm_v, a);
   LG_LAUNCH_CHECK(who);
   if (kind == PA_PROMPT)

@@ -7,6 +7,7 @@ Packed MLX words are carried as ``torch.int32`` tensors holding the uint32 bit p
 as int32.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -634,37 +635,45 @@ PAGES_ERRORS = {
 }
 
 
-def _call_on(device, name, *args):
-    """``_lib.call`` with ``device`` current (kernels launch on the current device)."""
-    if torch.cuda.current_device() == device.index:
-        return _lib.call(name, *args)
-    with torch.cuda.device(device):
-        return _lib.call(name, *args)
+_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_BF16, _I32 = torch.bfloat16, torch.int32
 
 
-def _i32(t, name, dims, device):
-    """A contiguous int32 tensor of ``dims`` dimensions on ``device``, updated in place by the
-    page operations, so never copied."""
-    if _dev(t) != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous():
+def _call_on(index, fn, *args):
+    """A C call with device ``index`` current (kernels launch on the current device) on that
+    device's current stream (the call's last argument)."""
+    if _current() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(fn.__name__, rc)
+
+
+def _i32(t, name, dims, index):
+    """The shape of a contiguous int32 tensor of ``dims`` dimensions on device ``index``."""
+    if t.dtype is not _I32 or t.dim() != dims or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of {dims} dimension(s)")
-    return t
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
+    return t.shape
 
 
 def _state(table, refs, lens=None):
-    dev = _dev(table)
-    S, M = _i32(table, "table", 2, dev).shape
-    P = _i32(refs, "refs", 1, dev).shape[0]
-    if lens is not None and _i32(lens, "lens", 1, dev).shape[0] != S:
+    _dev(table)
+    index = table.get_device()
+    S, M = _i32(table, "table", 2, index)
+    P, = _i32(refs, "refs", 1, index)
+    if lens is not None and _i32(lens, "lens", 1, index)[0] != S:
         raise ValueError(f"lens holds {lens.shape[0]} streams, table {S}")
-    return dev, S, M, P
+    return index, S, M, P
 
 
-def _pool(pool, dev, P):
+def _pool(pool, index, P):
     """(planes, heads, rows, row bytes) of a page pool [..., P, H, R, D]."""
-    if _dev(pool) != dev:
-        raise ValueError(f"the pool is on {pool.device}, not on {dev}")
+    if pool.get_device() != index:
+        raise ValueError(f"the pool is on {pool.device}, not on cuda:{index}")
     if pool.dim() < 4 or not pool.is_contiguous():
         raise ValueError("the pool must be a contiguous tensor [..., pages, heads, rows, dim]")
     p, h, r, d = pool.shape[-4:]
@@ -673,15 +682,24 @@ def _pool(pool, dev, P):
     return pool.numel() // max(p * h * r * d, 1), h, r, d * pool.element_size()
 
 
-def _ids(ids, name, dev):
-    ids = _i32(ids if ids.is_contiguous() else ids.contiguous(), name, 1, dev)
-    return ids, ids.shape[0]
+def _pair(a, b, names, index):
+    n, = _i32(a, names[0], 1, index)
+    if _i32(b, names[1], 1, index)[0] != n:
+        raise ValueError(f"{n} {names[0]}, {b.shape[0]} {names[1]}")
+    return n
 
 
-def _pages_ws(dev, P, n):
-    """A workspace of this call's own: an operation's list of moves must not be another's."""
-    nb = _lib.lib().lg_pages_workspace_bytes(P, n)
-    return torch.empty(nb, dtype=torch.uint8, device=dev), nb
+@functools.lru_cache(maxsize=256)
+def _pages_words(P, n):
+    return 64 + _lib.lib().lg_pages_workspace_bytes(P, n) // 4
+
+
+def _pages_ws(table, P, n):
+    """(status, workspace pointer, bytes): memory of this call's own, since an operation's list of
+    moves must not be another's."""
+    words = _pages_words(P, n)
+    ws = torch.empty(words, dtype=_I32, device=table.device)
+    return ws[:2], ws.data_ptr() + 256, 4 * words - 256
 
 
 def pages_reserve(table, refs, ids, rows, page_rows):
@@ -689,25 +707,22 @@ def pages_reserve(table, refs, ids, rows, page_rows):
     lowest free ids first; pages a stream has stay. ``table`` int32 [S, M] and ``refs`` int32 [P]
     are updated in place. Returns status int32 [2] on the device: (0 or a key of
     ``PAGES_ERRORS``, pages taken); on an error nothing has changed."""
-    dev, S, M, P = _state(table, refs)
-    (ids, n), (rows, m) = _ids(ids, "ids", dev), _ids(rows, "rows", dev)
-    if n != m:
-        raise ValueError(f"{n} streams, {m} row counts")
-    status = torch.empty(2, dtype=torch.int32, device=dev)
-    ws, nb = _pages_ws(dev, P, n)
-    _call_on(dev, "lg_pages_reserve", _p(table), _p(refs), S, M, P, int(page_rows), _p(ids),
-             _p(rows), n, _p(status), _p(ws), nb, _stream(dev))
+    index, S, M, P = _state(table, refs)
+    n = _pair(ids, rows, ("ids", "rows"), index)
+    status, ws, nb = _pages_ws(table, P, n)
+    _call_on(index, _lib.lib().lg_pages_reserve, table.data_ptr(), refs.data_ptr(), S, M, P,
+             int(page_rows), ids.data_ptr(), rows.data_ptr(), n, status.data_ptr(), ws, nb)
     return status
 
 
 def pages_free(table, lens, refs, ids):
     """The streams ``ids`` give their pages back (counts - 1, table rows -1, lengths 0). Returns
     status int32 [2]: (0 or a key of ``PAGES_ERRORS``, streams freed)."""
-    dev, S, M, P = _state(table, refs, lens)
-    ids, n = _ids(ids, "ids", dev)
-    status = torch.empty(2, dtype=torch.int32, device=dev)
-    _call_on(dev, "lg_pages_free", _p(table), _p(lens), _p(refs), S, M, P, _p(ids), n, _p(status),
-             _stream(dev))
+    index, S, M, P = _state(table, refs, lens)
+    n, = _i32(ids, "ids", 1, index)
+    status = torch.empty(2, dtype=_I32, device=table.device)
+    _call_on(index, _lib.lib().lg_pages_free, table.data_ptr(), lens.data_ptr(), refs.data_ptr(), S,
+             M, P, ids.data_ptr(), n, status.data_ptr())
     return status
 
 
@@ -715,15 +730,13 @@ def pages_fork(pool, table, lens, refs, src, dst):
     """Stream ``dst[i]`` (empty) becomes a copy of stream ``src[i]``: whole pages are shared, a
     part-filled last page is copied into a page of the child's own in every plane of ``pool``
     [..., P, H, R, D]. Returns status int32 [2]: (0 or a key of ``PAGES_ERRORS``, pages taken)."""
-    dev, S, M, P = _state(table, refs, lens)
-    planes, H, R, rb = _pool(pool, dev, P)
-    (src, n), (dst, m) = _ids(src, "src", dev), _ids(dst, "dst", dev)
-    if n != m:
-        raise ValueError(f"{n} sources, {m} children")
-    status = torch.empty(2, dtype=torch.int32, device=dev)
-    ws, nb = _pages_ws(dev, P, n)
-    _call_on(dev, "lg_pages_fork", _p(pool), planes, H, R, rb, _p(table), _p(lens), _p(refs), S, M,
-             P, _p(src), _p(dst), n, _p(status), _p(ws), nb, _stream(dev))
+    index, S, M, P = _state(table, refs, lens)
+    planes, H, R, rb = _pool(pool, index, P)
+    n = _pair(src, dst, ("src", "dst"), index)
+    status, ws, nb = _pages_ws(table, P, n)
+    _call_on(index, _lib.lib().lg_pages_fork, pool.data_ptr(), planes, H, R, rb, table.data_ptr(),
+             lens.data_ptr(), refs.data_ptr(), S, M, P, src.data_ptr(), dst.data_ptr(), n,
+             status.data_ptr(), ws, nb)
     return status
 
 
@@ -731,12 +744,11 @@ def pages_compact(pool, table, refs):
     """Live pages move to the lowest ids of ``pool`` [..., P, H, R, D] (with n live pages those
     with id >= n go, ascending, to the free ids below n); ``table`` and ``refs`` name them anew.
     Returns status int32 [2]: (0 or a key of ``PAGES_ERRORS``, pages moved)."""
-    dev, S, M, P = _state(table, refs)
-    planes, H, R, rb = _pool(pool, dev, P)
-    status = torch.empty(2, dtype=torch.int32, device=dev)
-    ws, nb = _pages_ws(dev, P, 0)
-    _call_on(dev, "lg_pages_compact", _p(pool), planes, H, R, rb, _p(table), _p(refs), S, M, P,
-             _p(status), _p(ws), nb, _stream(dev))
+    index, S, M, P = _state(table, refs)
+    planes, H, R, rb = _pool(pool, index, P)
+    status, ws, nb = _pages_ws(table, P, 0)
+    _call_on(index, _lib.lib().lg_pages_compact, pool.data_ptr(), planes, H, R, rb,
+             table.data_ptr(), refs.data_ptr(), S, M, P, status.data_ptr(), ws, nb)
     return status
 
 
@@ -747,38 +759,37 @@ class AttentionPlan:
     plan each. ``update()`` divides anew for the lengths that its tensors hold by then."""
 
     def __init__(self, kind, cu_q, kv_len, T, Hq, Hkv, page_rows, prefix, window):
-        dev = _dev(kv_len)
+        self.device, self.index = _dev(kv_len), kv_len.get_device()
         self.kind, self.T, self.Hq, self.Hkv = kind, int(T), int(Hq), int(Hkv)
         self.page_rows, self.prefix, self.window = int(page_rows), int(prefix), int(window)
-        self.device = dev
-        self.kv_len = _i32(kv_len, "kv_len", 1, dev)
-        self.B = kv_len.shape[0]
-        self.cu_q = cu_q
-        if kind == "prompt" and _i32(cu_q, "cu_q", 1, dev).shape[0] != self.B + 1:
+        self.B, = _i32(kv_len, "kv_len", 1, self.index)
+        self.cu_q, self.kv_len = cu_q, kv_len
+        if kind == "prompt" and _i32(cu_q, "cu_q", 1, self.index)[0] != self.B + 1:
             raise ValueError(f"cu_q holds {cu_q.shape[0]} offsets for {self.B} sequences")
-        with torch.cuda.device(dev):
+        with torch.cuda.device(self.index):
             self.nbytes = (_lib.lib().lg_prompt_plan_bytes(self.T, self.B, self.Hq, self.Hkv)
                            if kind == "prompt" else
                            _lib.lib().lg_stream_plan_bytes(self.B, self.Hq, self.Hkv))
-        self.buf = torch.empty(max(self.nbytes, 256), dtype=torch.uint8, device=dev)
+        self.buf = torch.empty(max(self.nbytes, 256), dtype=torch.uint8, device=self.device)
+        self.ptr = self.buf.data_ptr()
         self.update()
 
     def update(self):
-        st = _stream(self.device)
         if self.kind == "prompt":
-            _call_on(self.device, "lg_prompt_plan", _p(self.cu_q), _p(self.kv_len), self.B, self.T,
-                     self.Hq, self.Hkv, self.page_rows, self.window, _p(self.buf), self.nbytes, st)
+            _call_on(self.index, _lib.lib().lg_prompt_plan, self.cu_q.data_ptr(),
+                     self.kv_len.data_ptr(), self.B, self.T, self.Hq, self.Hkv, self.page_rows,
+                     self.window, self.ptr, self.nbytes)
         else:
-            _call_on(self.device, "lg_stream_plan", _p(self.kv_len), self.B, self.Hq, self.Hkv,
-                     self.page_rows, self.prefix, self.window, _p(self.buf), self.nbytes, st)
+            _call_on(self.index, _lib.lib().lg_stream_plan, self.kv_len.data_ptr(), self.B, self.Hq,
+                     self.Hkv, self.page_rows, self.prefix, self.window, self.ptr, self.nbytes)
         return self
-
 
     def status(self):
         """0, or the code of a wait that ran out in a call with this plan. Waits for the device."""
         st = ctypes.c_int(0)
-        torch.cuda.synchronize(self.device)
-        _call_on(self.device, "lg_plan_status", _p(self.buf), ctypes.byref(st))
+        torch.cuda.synchronize(self.index)
+        with torch.cuda.device(self.index):
+            _lib.call("lg_plan_status", self.ptr, ctypes.byref(st))
         return st.value
 
 
@@ -797,46 +808,47 @@ def stream_plan(kv_len, Hq, Hkv, page_rows, prefix=0, window=0):
 
 
 def _paged_attention(kind, q, k_pages, v_pages, table, plan, scale, gate, out):
-    dev = _dev(q)
-    if q.dtype != torch.bfloat16 or k_pages.dtype != torch.bfloat16 or \
-            v_pages.dtype != torch.bfloat16:
-        raise ValueError("q, k_pages and v_pages must be bf16")
     T, Hq, D = q.shape
-    P, Hkv, R, _ = k_pages.shape
-    if (plan.kind, plan.T, plan.Hq, plan.Hkv, plan.page_rows, plan.device) != \
-            (kind, T, Hq, Hkv, R, dev):
+    P, Hkv, R, _ = shape = k_pages.shape
+    ks, index = k_pages.stride(), plan.index
+    if plan.kind != kind or T != plan.T or Hq != plan.Hq or Hkv != plan.Hkv or R != plan.page_rows:
         raise ValueError(f"the plan is for {plan.kind} attention of {plan.T} tokens, heads "
-                         f"{plan.Hq}/{plan.Hkv}, pages of {plan.page_rows} rows on {plan.device}")
-    ks = k_pages.stride()
-    if k_pages.shape != v_pages.shape or ks != v_pages.stride() or ks[3] != 1 or \
-            k_pages.shape[3] != D:
+                         f"{plan.Hq}/{plan.Hkv}, pages of {plan.page_rows} rows")
+    if not (q.dtype is _BF16 and k_pages.dtype is _BF16 and v_pages.dtype is _BF16):
+        raise ValueError("q, k_pages and v_pages must be bf16")
+    if shape != v_pages.shape or ks != v_pages.stride() or ks[3] != 1 or shape[3] != D:
         raise ValueError("k_pages and v_pages must have one shape [P, Hkv, R, head_dim] and one "
                          "set of strides, unit along head_dim")
-    if k_pages.device != dev or v_pages.device != dev:
-        raise ValueError(f"the pages are not on {dev}")
-    B, M = _i32(table, "table", 2, dev).shape
+    if q.get_device() != index or k_pages.get_device() != index or v_pages.get_device() != index:
+        raise ValueError(f"q and the pages must be on the plan's device, {plan.device}")
+    B, M = _i32(table, "table", 2, index)
     if B != plan.B:
         raise ValueError(f"the table has {B} rows, the plan {plan.B} sequences")
     qs = q.stride()
     if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or q.data_ptr() % 16:
-        q = q.contiguous().clone() if q.is_contiguous() else q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)
         qs = q.stride()
-    if gate is not None:
-        if gate.shape != (T, Hq) or gate.dtype != torch.bfloat16 or _dev(gate) != dev:
-            raise ValueError(f"the gate must be bf16 [{T}, {Hq}] on {dev}")
-        gate = _c(gate)
-    if out is None:
-        out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=dev)
-    elif out.shape != (T, Hq, D) or out.dtype != torch.bfloat16 or _dev(out) != dev or \
-            not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous bf16 tensor [{T}, {Hq}, {D}] on {dev}")
-    a = (_p(q), qs[0], qs[1], T, Hq, Hkv, D, _p(k_pages), _p(v_pages), P, R, ks[0], ks[1], ks[2],
-         _p(table))
-    b = (M, float(scale), _p(gate), _p(out), _p(plan.buf), plan.nbytes, _stream(dev))
-    if kind == "prompt":
-        _call_on(dev, "lg_prompt_attention", *a, B, *b)
+    if gate is None:
+        gp = None
     else:
-        _call_on(dev, "lg_stream_attention", *a, *b)
+        if gate.shape != (T, Hq) or gate.dtype is not _BF16 or gate.get_device() != index:
+            raise ValueError(f"the gate must be bf16 [{T}, {Hq}] on {plan.device}")
+        if not gate.is_contiguous():
+            gate = gate.contiguous()
+        gp = gate.data_ptr()
+    if out is None:
+        out = torch.empty(T, Hq, D, dtype=_BF16, device=plan.device)
+    elif out.shape != (T, Hq, D) or out.dtype is not _BF16 or out.get_device() != index or \
+            not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous bf16 tensor [{T}, {Hq}, {D}] on {plan.device}")
+    if kind == "prompt":
+        _call_on(index, _lib.lib().lg_prompt_attention, q.data_ptr(), qs[0], qs[1], T, Hq, Hkv, D,
+                 k_pages.data_ptr(), v_pages.data_ptr(), P, R, ks[0], ks[1], ks[2],
+                 table.data_ptr(), B, M, scale, gp, out.data_ptr(), plan.ptr, plan.nbytes)
+    else:
+        _call_on(index, _lib.lib().lg_stream_attention, q.data_ptr(), qs[0], qs[1], T, Hq, Hkv, D,
+                 k_pages.data_ptr(), v_pages.data_ptr(), P, R, ks[0], ks[1], ks[2],
+                 table.data_ptr(), M, scale, gp, out.data_ptr(), plan.ptr, plan.nbytes)
     return out
 
 
