@@ -45,6 +45,8 @@ __host__ __device__ inline long long pa_cost(int ntile, int w) {
 
 struct PaStart {
   int tile, head, t;  // a CTA's first segment and key tile
+  int pad;
+  PaTile rec;  // that tile's record, so that a CTA has it with the first load
 };
 
 struct PaHead {

@@ -182,7 +182,8 @@ __global__ void __launch_bounds__(PLAN_THREADS)
   const long long total = carry;
   const long long chunk = max((long long)PA_MIN_CHUNK, (total + p.ncta - 1) / p.ncta);
   for (int c = tid; c <= p.ncta; c += PLAN_THREADS) {
-    PaStart s = {n, 0, 0};
+    PaStart s = {};
+    s.tile = n;
     const long long u = c * chunk;
     if (u < total) {
       int lo = 0, hi = n - 1;  // the last tile whose cost begins at or before u
@@ -201,6 +202,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         s.t = 0;
         if (++s.head == h.Hkv) s.head = 0, ++s.tile;
       }
+      if (s.tile < n) s.rec = p.tiles[s.tile];
     }
     p.start[c] = s;
   }
@@ -238,12 +240,17 @@ constexpr size_t PA_SMEM = (2 + PA_RING) * PA_TILE_BYTES + 8 * PA_STAGE + 512 + 
 // The segments of a CTA's share, in order; every warp walks them by itself.
 struct PaWalk {
   const PaTile* tiles;
-  PaStart at, end;
+  struct Place {
+    int tile, head, t;
+  } at, end;
   int t0, t1;
   PaTile rec;
-  __device__ explicit PaWalk(const PaPlan& p)
-      : tiles(p.tiles), at(p.start[blockIdx.x]), end(p.start[blockIdx.x + 1]) {
-    if (more()) rec = tiles[at.tile];
+  __device__ explicit PaWalk(const PaPlan& p) : tiles(p.tiles) {
+    const PaStart& s = p.start[blockIdx.x];
+    const PaStart& e = p.start[blockIdx.x + 1];
+    at = {s.tile, s.head, s.t};
+    end = {e.tile, e.head, e.t};
+    rec = s.rec;
   }
   __device__ bool more() const {
     if (at.tile != end.tile) return at.tile < end.tile;
@@ -394,12 +401,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   PaHead* const head = a.plan.head;
   int* const err = &head->err;
   const int G = a.Hq / a.Hkv, tq = PA_ROWS / G;
+  pdl_trigger();  // the joining kernel waits for this one itself
   PaWalk walk(a.plan);
   if (smem_u32(smem) & 1023) {
     if (threadIdx.x == 0) *err = 9;
     return;
   }
-  if (!walk.more()) return;  // nothing for this CTA
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < PA_RING; ++i) {
@@ -852,6 +859,8 @@ __global__ void __launch_bounds__(256) pa_join_prompt_kernel(const PaArgs a) {
   const PaHead h = *a.plan.head;
   const int c = blockIdx.x;
   const PaStart st = a.plan.start[c + 1];
+  pdl_wait();  // so far the plan was read, now the parts; a CTA without work waits too, or this
+               // kernel, and with it what follows, could come before the attention's end
   if (st.tile >= h.ntiles || st.t == 0) return;
   const PaTile t = a.plan.tiles[st.tile];
   int c0, c1;
@@ -919,6 +928,7 @@ __global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
   const PaTile own = a.plan.tiles[h.nprefix + b];
   int c0, c1, p0 = 0, p1 = -1, rr = 0;
   pa_parts(h, own, head, &c0, &c1);
+  pdl_wait();  // as above
   if (h.nprefix == 0 && c0 == c1) return;  // written by the CTA that had it whole
   const int rows = pa_own_rows(a.Hq, a.Hkv), pi = b / (2 * tq);
   if (h.nprefix) {
@@ -1059,10 +1069,23 @@ static int attn_run(const char* who, int kind, const void* q, long long q_tok, l
   if (int rc = pa_smem_once()) return rc;
   pa_kernel<<<p.ncta, PA_THREADS, PA_SMEM, st>>>(tm_q, tm_k, tm_v, a);
   LG_LAUNCH_CHECK(who);
-  if (kind == PA_PROMPT)
-    pa_join_prompt_kernel<<<dim3(p.ncta, PA_WIDE_ROWS / JP_ROWS), 256, 0, st>>>(a);
-  else
-    pa_join_stream_kernel<<<dim3(B, Hkv), 128, 0, st>>>(a);
+  // launched early: its CTAs read the plan and wait for the attention's end on the GPU
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (kind == PA_PROMPT) {
+    cfg.gridDim = dim3(p.ncta, PA_WIDE_ROWS / JP_ROWS);
+    cfg.blockDim = dim3(256);
+    LG_CUDA_TRY(cudaLaunchKernelEx(&cfg, pa_join_prompt_kernel, a));
+  } else {
+    cfg.gridDim = dim3(B, Hkv);
+    cfg.blockDim = dim3(128);
+    LG_CUDA_TRY(cudaLaunchKernelEx(&cfg, pa_join_stream_kernel, a));
+  }
   LG_LAUNCH_CHECK("paged_join");
   return LG_OK;
 }
