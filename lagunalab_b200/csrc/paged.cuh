@@ -27,21 +27,25 @@ struct PaTile {
   int ntile;    // key tiles: ceil((key_end - key0) / 128), at least 1
   int ntile0;   // pair: key tiles of the first row tile (at most ntile)
   int kind;
-  int pair;  // 1: two row tiles (2 * tq tokens) share each key tile; 0: one row tile
-  int w;     // cost of a key tile
-  int pad;
+  int pair;  // 1: two row tiles (2 * tq tokens) share each key tile
+  int duo;   // 1: the same tokens' row tiles of two neighbouring kv heads, with their own key tiles;
+             // neither (an odd number of kv heads): one row tile, its key tiles in two halves
+  int w;     // cost of a key tile (of both heads')
   long long before;  // cost of all segments before this tile's first
 };
 
-// Costs: half a row tile's worth of tensor-core time on one key tile is 1, so a pair's key tile
-// is 4 and a lone row tile's 2; a stream's own key tile waits for HBM rather than the tensor
-// cores. Every segment costs PA_SEG more (Q load, first score, output).
-constexpr int PA_W_PAIR = 4, PA_W_ONE = 2, PA_W_OWN = 3, PA_SEG = 8;
-constexpr int PA_MIN_CHUNK = 12;  // at least the largest PA_SEG + w: no CTA below the last is idle
+// Costs: half a row tile's worth of tensor-core time on one key tile is 1, so a key tile of two row
+// tiles is 4 and of one 2; a stream's own key tile waits for HBM rather than the tensor cores.
+// Every segment costs PA_SEG more (Q load, first score, output).
+constexpr int PA_W_TWO = 4, PA_W_ONE = 2, PA_W_OWN = 3, PA_SEG = 8;
+constexpr int PA_MIN_CHUNK = 14;  // at least the largest PA_SEG + w: no CTA below the last is idle
 
 __host__ __device__ inline long long pa_cost(int ntile, int w) {
   return PA_SEG + (long long)ntile * w;
 }
+
+// A row tile stands for Hkv segments, or Hkv / 2 of two heads; head: a segment's first.
+__host__ __device__ inline int pa_segments(const PaTile& t, int Hkv) { return Hkv >> t.duo; }
 
 struct PaStart {
   int tile, head, t;  // a CTA's first segment and key tile
@@ -76,6 +80,13 @@ __host__ __device__ inline size_t pa_slot_floats(int rows) { return (size_t)rows
 
 // Rows of a slot for a stream's own keys: G, even, so that slots stay 16-byte aligned.
 __host__ __device__ inline int pa_own_rows(int Hq, int Hkv) { return (Hq / Hkv + 1) & ~1; }
+
+// The slot of a stream's own keys for one head in the part of CTA c: parts in order, segment + CTA,
+// with two slots a part when its segments have two heads.
+__host__ __device__ inline size_t pa_own_slot(int b, int head, int c, int Hkv) {
+  return Hkv & 1 ? (size_t)b * Hkv + head + c
+                 : ((size_t)b * (Hkv >> 1) + (head >> 1) + c) * 2 + (head & 1);
+}
 
 __host__ __device__ inline int pa_tq(int Hq, int Hkv) { return PA_ROWS / (Hq / Hkv); }
 

@@ -59,7 +59,7 @@ static PaPlan pa_layout(void* buf, int kind, int T, int B, int Hq, int Hkv) {
   const size_t wide = kind == PA_PROMPT
                           ? 2 * (size_t)p.ncta
                           : (size_t)(p.max_tiles - B) * Hkv + p.ncta;
-  const size_t own = kind == PA_PROMPT ? 0 : (size_t)B * Hkv + p.ncta;
+  const size_t own = kind == PA_PROMPT ? 0 : (size_t)B * Hkv + 2 * (size_t)p.ncta;
   p.wide = c.take<float>(wide * pa_slot_floats(PA_WIDE_ROWS));
   p.own = c.take<float>(own * pa_slot_floats(pa_own_rows(Hq, Hkv)));
   p.bytes = align_up(c.used, 256);
@@ -78,13 +78,15 @@ __device__ __forceinline__ PaTile pa_stream_tile(const PaHead& h, const PaPlan& 
     t.kind = PA_OWN;
     t.key_end = kv;
     t.key0 = min(max(h.prefix, h.window ? kv - h.window : 0), kv);
-    t.w = PA_W_OWN;
+    t.duo = !(h.Hkv & 1);
+    t.w = PA_W_OWN << t.duo;
   } else {  // 2 tq streams against the shared prefix
     t.q0 = i * 2 * tq;
     t.nq = min(2 * tq, h.B - t.q0);
     t.row = t.q0;
     t.kind = PA_PREFIX;
     t.pair = t.nq > tq;
+    t.duo = !t.pair && !(h.Hkv & 1);
     int lo = h.prefix, most = -1;
     for (int b = t.q0; b < t.q0 + t.nq; ++b) {
       const int kv = p.kv[b];
@@ -93,7 +95,7 @@ __device__ __forceinline__ PaTile pa_stream_tile(const PaHead& h, const PaPlan& 
     }
     t.key_end = min(h.prefix, max(most, 0));
     t.key0 = min(lo, t.key_end);
-    t.w = t.pair ? PA_W_PAIR : PA_W_ONE;
+    t.w = t.pair || t.duo ? PA_W_TWO : PA_W_ONE;
   }
   return t;
 }
@@ -151,9 +153,10 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         t.pos0 = p.kv[lo] - (t1 - t0) + first;
         t.kind = PA_PROMPT;
         t.pair = t.nq > tq;
+        t.duo = !t.pair && !(h.Hkv & 1);
         t.key_end = max(0, t.pos0 + t.nq);
         t.key0 = min(h.window ? max(0, t.pos0 - h.window + 1) : 0, t.key_end);
-        t.w = t.pair ? PA_W_PAIR : PA_W_ONE;
+        t.w = t.pair || t.duo ? PA_W_TWO : PA_W_ONE;
       } else {
         t = pa_stream_tile(h, p, i, np, tq);
       }
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
       t.ntile = t.ntile0 = max(1, (t.key_end - t.key0 + PA_KEYS - 1) / PA_KEYS);
       if (t.kind == PA_PROMPT && t.pair)  // the first row tile's tokens see fewer keys
         t.ntile0 = max(1, (max(0, t.pos0 + tq) - t.key0 + PA_KEYS - 1) / PA_KEYS);
-      cost = pa_cost(t.ntile, t.w) * h.Hkv;
+      cost = pa_cost(t.ntile, t.w) * pa_segments(t, h.Hkv);
     }
     long long inc = cost;  // sum of the costs up to this tile's
 #pragma unroll
@@ -196,11 +199,12 @@ __global__ void __launch_bounds__(PLAN_THREADS)
       const long long seg = pa_cost(t.ntile, t.w), r = u - t.before;
       const long long in = r % seg - PA_SEG;  // key tile k begins at PA_SEG + k w of its segment
       s.tile = lo;
-      s.head = (int)(r / seg);
+      s.head = (int)(r / seg) << t.duo;
       s.t = in <= 0 ? 0 : (int)((in + t.w - 1) / t.w);
       if (s.t >= t.ntile) {
         s.t = 0;
-        if (++s.head == h.Hkv) s.head = 0, ++s.tile;
+        s.head += 1 << t.duo;
+        if (s.head == h.Hkv) s.head = 0, ++s.tile;
       }
       if (s.tile < n) s.rec = p.tiles[s.tile];
     }
@@ -264,11 +268,12 @@ struct PaWalk {
   }
   // The record of the segment after this one: fetched early, for step().
   __device__ PaTile ahead(int Hkv) const {
-    return at.head + 1 == Hkv && at.tile < end.tile ? tiles[at.tile + 1] : rec;
+    return at.head + (1 << rec.duo) == Hkv && at.tile < end.tile ? tiles[at.tile + 1] : rec;
   }
   __device__ void step(int Hkv, const PaTile& then) {
     at.t = 0;
-    if (++at.head == Hkv) at.head = 0, ++at.tile;
+    at.head += 1 << rec.duo;
+    if (at.head == Hkv) at.head = 0, ++at.tile;
     rec = then;
   }
 };
@@ -447,52 +452,50 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const int half = lane & 1, box = lane >> 1;
     for (; ok && walk.next(); ++seg) {
       const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
-      const int n = walk.t1 - walk.t0;
+      const int n = (walk.t1 - walk.t0) << r.duo;
       const bool clear = pa_tail(r, walk.t1);
       if (lane == 0) bad[seg % PA_NBAD] = 0;
       __syncwarp();
       const int npage = (r.key_end + a.R - 1) / a.R;  // pages the rows need
       const int* row = a.table + (long long)r.row * a.M;
-      // this lane's column of the table at a place of the ring, and its entry, fetched three
-      // places ahead and looked at only when its copy goes out
-      auto column = [&](int place) {
-        const int t = walk.t0 + (pa_ring(place, n, r.pair) >> 1);
-        return (r.key0 + t * PA_KEYS) / a.R + box;
-      };
-      auto entry = [&](int place) {
-        const int c = place < 2 * n ? column(place) : npage;
-        return mine && c < npage && c < a.M ? __ldg(row + c) : -1;
-      };
-      int e0 = -1, e1 = -1, e2 = -1, e3 = -1;
+      // The table 32 columns at a time, a column a lane, the next 32 fetched ahead: a key tile's
+      // entries lie within one such group or the next.
+      const int c0 = r.key0 / a.R + walk.t0 * boxes;
+      auto entries = [&](int c) { return c + lane < min(npage, a.M) ? __ldg(row + c + lane) : -1; };
+      int group = 0, cur = entries(c0), nxt = entries(c0 + 32);
 #pragma unroll 1
-      for (int place = -3; place < 2 * n; ++place) {
-        e0 = e1;
-        e1 = e2;
-        e2 = e3;
-        e3 = entry(place + 3);
-        if (place < 0) continue;
-        const int slot = rc % PA_RING, x = pa_ring(place, n, r.pair);
+      for (int place = 0; place < 2 * n; ++place) {
+        const int slot = rc % PA_RING, x = pa_ring(place, n, r.pair), t = x >> 1 >> r.duo;
+        const int col = t * boxes - group + box;  // V tiles trail K tiles by two at most
+        const int in_cur = __shfl_sync(0xffffffffu, cur, col & 31);
+        const int in_nxt = __shfl_sync(0xffffffffu, nxt, col & 31);
+        int page = col < 32 ? in_cur : in_nxt;
+        if ((x & 1) && t * boxes - group >= 32) {  // the last use of the older group has gone
+          group += 32;
+          cur = nxt;
+          nxt = entries(c0 + group + 32);
+        }
         if (!(ok = warp_wait(empty + slot, ((rc / PA_RING) & 1) ^ 1, err, 1))) break;
-        uint64_t* const bar = (clear && place + 1 == 2 * n ? tail : full) + slot;
+        uint64_t* const bar = (clear && place + 1 + r.duo >= 2 * n ? tail : full) + slot;
         if (lane == 0) mbar_arrive_expect_tx(bar, PA_TILE_BYTES);
-        int page = e0;
         if ((unsigned)page >= (unsigned)a.P) {
           page = a.P;  // outside the pool: reads as zeros
-          if (mine && column(place) < npage) bad[seg % PA_NBAD] = 1;
+          if (mine && c0 + t * boxes + box < npage) bad[seg % PA_NBAD] = 1;
         }
         __syncwarp();
         if (mine)
           tma_load_4d(sKV + slot * PA_TILE_BYTES + half * PA_HALF + box * a.R * 128,
-                      x & 1 ? &tm_v : &tm_k, bar, half * 64, 0, walk.at.head, page);
+                      x & 1 ? &tm_v : &tm_k, bar, half * 64, 0, walk.at.head + (x >> 1 & r.duo), page);
         ++rc;
         if (place == 0) {
           if (!(ok = warp_wait(q_empty, (seg & 1) ^ 1, err, 2))) break;
           ++nq;
           if (lane == 0) {
-            mbar_arrive_expect_tx(q_full, (r.pair ? 4 : 2) * 128 * G * tq);
-            for (int f = 0; f < (r.pair ? 4 : 2); ++f)
-              tma_load_3d(sQ + f * PA_HALF, &tm_q, q_full, (f & 1) * 64, walk.at.head * G,
-                          r.q0 + (f >> 1) * tq);
+            const int halves = r.pair || r.duo ? 4 : 2;
+            mbar_arrive_expect_tx(q_full, halves * 128 * G * tq);
+            for (int f = 0; f < halves; ++f)
+              tma_load_3d(sQ + f * PA_HALF, &tm_q, q_full, (f & 1) * 64,
+                          (walk.at.head + (f >> 1 & r.duo)) * G, r.q0 + (f >> 1) * r.pair * tq);
           }
           __syncwarp();
         }
@@ -526,12 +529,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
     for (; ok && walk.next(); ++seg) {
       const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
-      const int n = walk.t1 - walk.t0;
+      const int n = (walk.t1 - walk.t0) << r.duo;
       const int lim = r.pair && w == 0 ? min(n, max(0, r.ntile0 - walk.t0)) : n;
       const int step = r.pair ? 1 : 2, first = r.pair ? 0 : w;
       uint32_t slot = 0;  // the tile at hand, in 16-byte units
       auto qk = [&](int t) {
-        const uint32_t q = q_lo + (r.pair ? w * (PA_TILE_BYTES >> 4) : 0), k = k_lo + slot;
+        const uint32_t q = q_lo + (r.pair || r.duo ? w * (PA_TILE_BYTES >> 4) : 0);
+        const uint32_t k = k_lo + slot;
 #pragma unroll
         for (int s = 0; s < PA_D / 16; ++s) {
           const uint32_t off = ((s >> 2) * PA_HALF + (s & 3) * 32) >> 4;
@@ -606,9 +610,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     bool ok = true;
     for (; ok && walk.next();) {
       const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
-      rc += 2 * (walk.t1 - walk.t0);
-      if (pa_tail(r, walk.t1)) {
-        const int slot = (rc - 1) % PA_RING;  // a part's last tile in the ring is its last V
+      rc += 2 * (walk.t1 - walk.t0) << r.duo;
+      for (int back = 1 + r.duo; ok && back > 0 && pa_tail(r, walk.t1); --back) {
+        const int slot = (rc - back) % PA_RING;  // a part's last tiles in the ring are its last V
         ok = warp_wait(tail + slot, phases >> slot & 1, err, 8);
         phases ^= 1u << slot;
         uint8_t* v = sKV + slot * PA_TILE_BYTES;
@@ -642,7 +646,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     bool ok = true;
     for (; walk.next(); ++seg) {
       const PaTile& r = walk.rec;
-      const int n = walk.t1 - walk.t0;
+      const int n = (walk.t1 - walk.t0) << r.duo;
+      const bool halves = !r.pair && !r.duo;  // one row tile, its key tiles in two halves
       // this row's token and the keys [lo, hi) it sees
       const int i = (r.pair ? w * tq : 0) + row / G;
       const bool valid = row < tq * G && i < r.nq;
@@ -657,7 +662,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
       const bool active = __any_sync(0xffffffffu, valid);
       const bool whole = walk.t0 == 0 && walk.t1 == r.ntile && (r.kind == PA_PROMPT || prefix == 0);
-      const long long at = (long long)(r.q0 + i) * a.Hq + walk.at.head * G + row % G;
+      const long long at =
+          (long long)(r.q0 + i) * a.Hq + (walk.at.head + (w & r.duo)) * G + row % G;
       // fetched now, looked at at the end
       const __nv_bfloat16 gb = valid && whole && a.gate ? a.gate[at] : __float2bfloat16_rn(1.f);
       float m = -INFINITY, l = 0.f;
@@ -665,8 +671,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const int last = r.pair && w == 0 ? min(n, max(0, r.ntile0 - walk.t0)) : n;
       bool any = false;  // this row tile (or half of the keys) has a key tile
       const int last_t = n - 1 - (n - 1 - w & 1);  // half w's last key tile
-      int kb = r.key0 + (walk.t0 + (r.pair ? 0 : w)) * PA_KEYS;
-      for (int t = r.pair ? 0 : w; t < last; t += stride, kb += stride * PA_KEYS) {
+      int kb = r.key0 + (walk.t0 + (halves ? w : 0)) * PA_KEYS;
+      for (int t = r.pair ? 0 : w; t < last; t += stride, kb += (halves ? 2 : 1) * PA_KEYS) {
         ok = ok && warp_wait(s_full + w, s_phase, err, 6);
         s_phase ^= 1;
         tc_fence_after();
@@ -745,7 +751,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       if (active) {
         if (bad[seg % PA_NBAD] || !ok) l = NAN;
         float f0 = 1.f, f1 = 0.f;
-        if (!r.pair) {
+        if (halves) {
           ml[w * PA_ROWS + row] = make_float2(m, l);
           bar_sync(quad_bar, 64);
           const float2 x0 = ml[row], x1 = ml[PA_ROWS + row];
@@ -755,7 +761,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           l = x0.y * f0 + x1.y * f1;
           if (bad[seg % PA_NBAD] || !ok) l = NAN;
         }
-        const int rr = (r.pair ? w * PA_ROWS : 0) + row;
+        int rr = (halves ? 0 : w * PA_ROWS) + row;
         float* slot = nullptr;
         int rows = PA_WIDE_ROWS;
         if (!whole) {
@@ -766,10 +772,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                    ((size_t)walk.at.tile * a.Hkv + walk.at.head + blockIdx.x) * pa_slot_floats(rows);
           } else {
             rows = pa_own_rows(a.Hq, a.Hkv);
-            slot = a.plan.own + ((size_t)(walk.at.tile - nprefix) * a.Hkv + walk.at.head +
-                                 blockIdx.x) * pa_slot_floats(rows);
+            rr = row;
+            slot = a.plan.own + pa_own_slot(walk.at.tile - nprefix, walk.at.head + (w & r.duo),
+                                            blockIdx.x, a.Hkv) * pa_slot_floats(rows);
           }
-          if (valid && (r.pair || w == 0))
+          if (valid && (!halves || w == 0))
             reinterpret_cast<float2*>(slot)[rr] = make_float2(m, l);
         }
         const float g = bf2f(gb);
@@ -784,13 +791,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         // key tile (a pair's first row tile in a late part) there is no O: m = -inf says so.
         int part = !whole;
 #pragma unroll 1
-        for (int j = r.pair ? 0 : 2 * w; j < (r.pair ? (any ? 4 : 0) : 2 * w + 2); ++j) {
+        for (int j = halves ? 2 * w : 0; j < (halves ? 2 * w + 2 : any ? 4 : 0); ++j) {
           asm volatile("" : "+r"(part));
           float o[32];
-          tmem_ld32_wait(tO + (r.pair ? w * 128 : 0) + 32 * j, o);
+          tmem_ld32_wait(tO + (halves ? 0 : w * 128) + 32 * j, o);
 #pragma unroll
           for (int x = 0; x < 32; ++x) o[x] *= f0;
-          if (!r.pair) {
+          if (halves) {
             float o1[32];
             tmem_ld32_wait(tO + (n > 1 ? 128 : 0) + 32 * j, o1);  // f1 = 0 without a second half
 #pragma unroll
@@ -831,7 +838,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           }
         }
         // neither half's O or ml is overwritten before both have read it
-        if (!r.pair) bar_sync(quad_bar, 64);
+        if (halves) bar_sync(quad_bar, 64);
       }
       walk.step(a.Hkv, then);
     }
@@ -845,7 +852,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 // The CTAs [c0, c1] whose shares hold key tiles of the segment (tile t, head).
 __device__ __forceinline__ void pa_parts(const PaHead& h, const PaTile& t, int head, int* c0,
                                          int* c1) {
-  const long long s = t.before + head * pa_cost(t.ntile, t.w) + PA_SEG;
+  const long long s = t.before + (head >> t.duo) * pa_cost(t.ntile, t.w) + PA_SEG;
   *c0 = (int)(s / h.chunk);
   *c1 = (int)((s + (long long)(t.ntile - 1) * t.w) / h.chunk);
 }
@@ -869,8 +876,9 @@ __global__ void __launch_bounds__(256) pa_join_prompt_kernel(const PaArgs a) {
   const int G = a.Hq / a.Hkv, tq = PA_ROWS / G;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rr = blockIdx.y * JP_ROWS + lane, w = rr / PA_ROWS, row = rr % PA_ROWS;
-  const int i = w * tq + row / G;
-  const bool valid = row < tq * G && i < t.nq && w <= t.pair;
+  const int i = w * t.pair * tq + row / G;
+  const bool valid = row < tq * G && i < t.nq && w <= (t.pair | t.duo);
+  const int head = st.head + (w & t.duo);
   const size_t slot = pa_slot_floats(PA_WIDE_ROWS);
   if (!__syncthreads_or(valid)) return;
   if (valid) {
@@ -901,7 +909,7 @@ __global__ void __launch_bounds__(256) pa_join_prompt_kernel(const PaArgs a) {
       }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const float g = a.gate ? bf2f(a.gate[(long long)(t.q0 + i) * a.Hq + st.head * G + row % G]) : 1.f;
+    const float g = a.gate ? bf2f(a.gate[(long long)(t.q0 + i) * a.Hq + head * G + row % G]) : 1.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float4 v = make_float4(o[j].x * inv, o[j].y * inv, o[j].z * inv, o[j].w * inv);
@@ -914,9 +922,9 @@ __global__ void __launch_bounds__(256) pa_join_prompt_kernel(const PaArgs a) {
   __syncthreads();
   for (int x = warp; x < JP_ROWS; x += 8) {
     const int r2 = blockIdx.y * JP_ROWS + x, w2 = r2 / PA_ROWS, row2 = r2 % PA_ROWS;
-    const int i2 = w2 * tq + row2 / G;
-    if (row2 >= tq * G || i2 >= t.nq || w2 > t.pair) continue;
-    reinterpret_cast<uint2*>(a.out + ((long long)(t.q0 + i2) * a.Hq + st.head * G + row2 % G) *
+    const int i2 = w2 * t.pair * tq + row2 / G, head2 = st.head + (w2 & t.duo);
+    if (row2 >= tq * G || i2 >= t.nq || w2 > (t.pair | t.duo)) continue;
+    reinterpret_cast<uint2*>(a.out + ((long long)(t.q0 + i2) * a.Hq + head2 * G + row2 % G) *
                                          PA_D)[lane] = rows[x][lane];
   }
 }
@@ -926,7 +934,7 @@ __global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
   const PaHead h = *a.plan.head;
   const int b = blockIdx.x, head = blockIdx.y, G = a.Hq / a.Hkv, tq = PA_ROWS / G;
   const PaTile own = a.plan.tiles[h.nprefix + b];
-  int c0, c1, p0 = 0, p1 = -1, rr = 0;
+  int c0, c1, p0 = 0, p1 = -1, rr = 0, first = head;
   pa_parts(h, own, head, &c0, &c1);
   pdl_wait();  // as above
   if (h.nprefix == 0 && c0 == c1) return;  // written by the CTA that had it whole
@@ -935,10 +943,12 @@ __global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
     const PaTile pre = a.plan.tiles[pi];
     pa_parts(h, pre, head, &p0, &p1);
     const int i = b - pre.q0, w = i / tq;
-    rr = w * PA_ROWS + (i - w * tq) * G;
+    rr = pre.duo ? (head & 1) * PA_ROWS + i * G : w * PA_ROWS + (i - w * tq) * G;
+    first = head & ~pre.duo;
   }
-  const float* wide = a.plan.wide + ((size_t)pi * a.Hkv + head) * pa_slot_floats(PA_WIDE_ROWS);
-  const float* ow = a.plan.own + ((size_t)b * a.Hkv + head) * pa_slot_floats(rows);
+  const float* wide = a.plan.wide + ((size_t)pi * a.Hkv + first) * pa_slot_floats(PA_WIDE_ROWS);
+  const float* ow = a.plan.own + pa_own_slot(b, head, 0, a.Hkv) * pa_slot_floats(rows);
+  const size_t step = pa_slot_floats(rows) << own.duo;  // from one CTA's part to the next
   for (int e = threadIdx.x; e < G * 32; e += 128) {
     const int g = e % G, q = e / G;  // neighbours take neighbouring rows of one column quad
     float m = -INFINITY;
@@ -947,7 +957,7 @@ __global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
       m = fmaxf(m, reinterpret_cast<const float2*>(wide + x * pa_slot_floats(PA_WIDE_ROWS))[rr + g].x);
 #pragma unroll 2
     for (int x = c0; x <= c1; ++x)
-      m = fmaxf(m, reinterpret_cast<const float2*>(ow + x * pa_slot_floats(rows))[g].x);
+      m = fmaxf(m, reinterpret_cast<const float2*>(ow + x * step)[g].x);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](const float* p, int n, int r) {
@@ -963,7 +973,7 @@ __global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
 #pragma unroll 2
     for (int x = p0; x <= p1; ++x) add(wide + x * pa_slot_floats(PA_WIDE_ROWS), PA_WIDE_ROWS, rr + g);
 #pragma unroll 2
-    for (int x = c0; x <= c1; ++x) add(ow + x * pa_slot_floats(rows), rows, g);
+    for (int x = c0; x <= c1; ++x) add(ow + x * step, rows, g);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     float4 v = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     const long long at = (long long)b * a.Hq + head * G + g;
