@@ -37,8 +37,8 @@ struct PaTile {
 // Costs: half a row tile's worth of tensor-core time on one key tile is 1, so a key tile of two row
 // tiles is 4 and of one 2; a stream's own key tile waits for HBM rather than the tensor cores.
 // Every segment costs PA_SEG more (Q load, first score, output).
-constexpr int PA_W_TWO = 4, PA_W_ONE = 2, PA_W_OWN = 3, PA_SEG = 8;
-constexpr int PA_MIN_CHUNK = 14;  // at least the largest PA_SEG + w: no CTA below the last is idle
+constexpr int PA_W_TWO = 4, PA_W_ONE = 2, PA_W_OWN = 2, PA_SEG = 8;
+constexpr int PA_MIN_CHUNK = 12;  // at least the largest PA_SEG + w: no CTA below the last is idle
 
 __host__ __device__ inline long long pa_cost(int ntile, int w) {
   return PA_SEG + (long long)ntile * w;
@@ -55,7 +55,7 @@ struct PaStart {
 
 struct PaHead {
   long long total, chunk;
-  int ntiles, nprefix;  // row tiles, and how many of them (the first ones) are PA_PREFIX
+  int ntiles;  // row tiles
   int kind, B, T, Hq, Hkv, R, prefix, window;
   int err;  // a wait that ran out (its code), else 0
 };
@@ -71,6 +71,7 @@ struct PaPlan {
   float* wide;  // slots of 2 * PA_ROWS rows (prompts, prefixes)
   float* own;   // slots of G rows (streams' own keys)
   int ncta, max_tiles;
+  int nprefix;  // streams: row tiles kept for the prefix, before the streams' own
   size_t bytes;
 };
 

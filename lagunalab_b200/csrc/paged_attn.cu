@@ -44,11 +44,14 @@ static int pa_max_tiles(int kind, int T, int B, int Hq, int Hkv) {
   return kind == PA_PROMPT ? T / tq2 + B : B + (B + tq2 - 1) / tq2;
 }
 
+constexpr int JS_PARTS = 192;  // parts that a stream's rows may have: CTAs, and 2
+
 static PaPlan pa_layout(void* buf, int kind, int T, int B, int Hq, int Hkv) {
   PaPlan p;
   Carver c(buf);
-  p.ncta = device_sm_count();
+  p.ncta = min(device_sm_count(), JS_PARTS - 2);
   p.max_tiles = pa_max_tiles(kind, T, B, Hq, Hkv);
+  p.nprefix = kind == PA_PROMPT ? 0 : p.max_tiles - B;
   p.head = c.take<PaHead>(1);
   p.start = c.take<PaStart>(p.ncta + 1);
   p.kv = c.take<int>(B);
@@ -58,7 +61,7 @@ static PaPlan pa_layout(void* buf, int kind, int T, int B, int Hq, int Hkv) {
   // parts in order, segment + CTA
   const size_t wide = kind == PA_PROMPT
                           ? 2 * (size_t)p.ncta
-                          : (size_t)(p.max_tiles - B) * Hkv + p.ncta;
+                          : (size_t)p.nprefix * Hkv + p.ncta;
   const size_t own = kind == PA_PROMPT ? 0 : (size_t)B * Hkv + 2 * (size_t)p.ncta;
   p.wide = c.take<float>(wide * pa_slot_floats(PA_WIDE_ROWS));
   p.own = c.take<float>(own * pa_slot_floats(pa_own_rows(Hq, Hkv)));
@@ -68,11 +71,10 @@ static PaPlan pa_layout(void* buf, int kind, int T, int B, int Hq, int Hkv) {
 
 constexpr int PLAN_THREADS = 1024;
 
-__device__ __forceinline__ PaTile pa_stream_tile(const PaHead& h, const PaPlan& p, int i, int np,
-                                                 int tq) {
+__device__ __forceinline__ PaTile pa_stream_tile(const PaHead& h, const PaPlan& p, int i, int tq) {
   PaTile t = {};
-  if (i >= np) {  // stream i - np: its own keys
-    const int b = i - np, kv = p.kv[b];
+  if (i >= p.nprefix) {  // a stream's own keys
+    const int b = i - p.nprefix, kv = p.kv[b];
     t.row = t.q0 = b;
     t.nq = 1;
     t.kind = PA_OWN;
@@ -108,7 +110,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
   __shared__ long long wsum[32], carry;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tq = pa_tq(h.Hq, h.Hkv), tq2 = 2 * tq;
-  int n = 0, np = 0;
+  int n = 0;
   for (int b0 = 0; b0 < h.B; b0 += PLAN_THREADS) {
     const int b = b0 + tid;
     int v = 0;
@@ -126,10 +128,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     }
     __syncthreads();
   }
-  if (h.kind != PA_PROMPT) {
-    np = h.prefix > 0 ? (h.B + tq2 - 1) / tq2 : 0;
-    n = np + h.B;
-  }
+  if (h.kind != PA_PROMPT) n = p.nprefix + h.B;
   n = min(n, p.max_tiles);  // offsets that do not ascend could ask for more
   if (tid == 0) carry = 0;
   __syncthreads();
@@ -158,13 +157,14 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         t.key0 = min(h.window ? max(0, t.pos0 - h.window + 1) : 0, t.key_end);
         t.w = t.pair || t.duo ? PA_W_TWO : PA_W_ONE;
       } else {
-        t = pa_stream_tile(h, p, i, np, tq);
+        t = pa_stream_tile(h, p, i, tq);
       }
       t.key0 = t.key0 / h.R * h.R;
       t.ntile = t.ntile0 = max(1, (t.key_end - t.key0 + PA_KEYS - 1) / PA_KEYS);
       if (t.kind == PA_PROMPT && t.pair)  // the first row tile's tokens see fewer keys
         t.ntile0 = max(1, (max(0, t.pos0 + tq) - t.key0 + PA_KEYS - 1) / PA_KEYS);
       cost = pa_cost(t.ntile, t.w) * pa_segments(t, h.Hkv);
+      if (t.kind == PA_PREFIX && h.prefix == 0) cost = 0;  // the tiles are there, no CTA gets one
     }
     long long inc = cost;  // sum of the costs up to this tile's
 #pragma unroll
@@ -214,7 +214,6 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     h.total = total;
     h.chunk = chunk;
     h.ntiles = n;
-    h.nprefix = np;
     h.err = 0;
     *p.head = h;
   }
@@ -637,7 +636,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;  // lane field: 32 (warp & 3) << 16
     const uint32_t tS = tmem + w * 128 + quarter, tO = tmem + 256 + quarter;
     const float c = a.scale_log2;
-    const int prefix = head->prefix, window = head->window, nprefix = head->nprefix;
+    const int prefix = head->prefix, window = head->window;
     uint32_t s_phase = 0, o_phase = 0;
     int seg = 0, rc = 0;
     // After a failed wait a warp arrives at no mbarrier any more (each role has then done a prefix
@@ -773,7 +772,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           } else {
             rows = pa_own_rows(a.Hq, a.Hkv);
             rr = row;
-            slot = a.plan.own + pa_own_slot(walk.at.tile - nprefix, walk.at.head + (w & r.duo),
+            slot = a.plan.own + pa_own_slot(walk.at.tile - a.plan.nprefix, walk.at.head + (w & r.duo),
                                             blockIdx.x, a.Hkv) * pa_slot_floats(rows);
           }
           if (valid && (!halves || w == 0))
@@ -858,131 +857,124 @@ __device__ __forceinline__ void pa_parts(const PaHead& h, const PaTile& t, int h
 }
 
 // Joins the parts of prompts' split segments: block x looks at the segment that CTA x + 1 begins
-// inside of, if CTA x began it; block y takes 32 of its rows (lane = row, so a slot's column quads
-// are read 512 bytes at a time), and the rows leave through shared memory, 256 bytes each.
+// inside of, if CTA x began it; block y takes 32 of its rows, eight lanes a row, so that a row
+// leaves as 256 bytes and a slot's column quads are read 64 bytes at a time.
 constexpr int JP_ROWS = 32;
 __global__ void __launch_bounds__(256) pa_join_prompt_kernel(const PaArgs a) {
-  __shared__ uint2 rows[JP_ROWS][33];
   const PaHead h = *a.plan.head;
   const int c = blockIdx.x;
   const PaStart st = a.plan.start[c + 1];
-  pdl_wait();  // so far the plan was read, now the parts; a CTA without work waits too, or this
-               // kernel, and with it what follows, could come before the attention's end
-  if (st.tile >= h.ntiles || st.t == 0) return;
-  const PaTile t = a.plan.tiles[st.tile];
+  const PaTile& t = st.rec;
+  const int G = a.Hq / a.Hkv, tq = PA_ROWS / G;
+  const int rr = blockIdx.y * JP_ROWS + (threadIdx.x >> 3), w = rr / PA_ROWS, row = rr % PA_ROWS;
+  const int q = (threadIdx.x & 7) * 4;  // the lane's column quads [q, q + 4)
+  const int i = w * t.pair * tq + row / G, head = st.head + (w & t.duo);
   int c0, c1;
   pa_parts(h, t, st.head, &c0, &c1);
-  if (c0 != c) return;
-  const int G = a.Hq / a.Hkv, tq = PA_ROWS / G;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rr = blockIdx.y * JP_ROWS + lane, w = rr / PA_ROWS, row = rr % PA_ROWS;
-  const int i = w * t.pair * tq + row / G;
-  const bool valid = row < tq * G && i < t.nq && w <= (t.pair | t.duo);
-  const int head = st.head + (w & t.duo);
+  // so far the plan was read, now the parts; a CTA without work waits too, or this kernel, and with
+  // it what follows, could come before the attention's end
+  pdl_wait();
+  if (st.tile >= h.ntiles || st.t == 0 || c0 != c) return;
+  if (row >= tq * G || i >= t.nq || w > (t.pair | t.duo)) return;
   const size_t slot = pa_slot_floats(PA_WIDE_ROWS);
-  if (!__syncthreads_or(valid)) return;
-  if (valid) {
-    float m = -INFINITY;
-    for (int x = c0; x <= c1; ++x) {
-      const float* p = a.plan.wide + (2 * x + (x == c0)) * slot;
-      m = fmaxf(m, reinterpret_cast<const float2*>(p)[rr].x);
-    }
-    float l = 0.f;
-    float4 o[4] = {};
-    for (int x = c0; x <= c1; ++x) {
-      const float* p = a.plan.wide + (2 * x + (x == c0)) * slot;
-      const float2 ml = reinterpret_cast<const float2*>(p)[rr];
-      if (ml.x == -INFINITY) {  // no key, and maybe no O; a NaN l stays one
-        l += ml.y;
-        continue;
-      }
-      const float f = ex2((ml.x - m) * a.scale_log2);
-      l += ml.y * f;
-      const float4* po = reinterpret_cast<const float4*>(p + 2 * PA_WIDE_ROWS);
+  const long long at = (long long)(t.q0 + i) * a.Hq + head * G + row % G;
+  const float g = a.gate ? bf2f(a.gate[at]) : 1.f;
+  float m = -INFINITY, l = 0.f;
+  float o[16] = {};
+#pragma unroll 1
+  for (int x = c0; x <= c1; ++x) {  // mostly two parts
+    const float* p = a.plan.wide + (2 * x + (x == c0)) * slot;
+    const float2 ml = reinterpret_cast<const float2*>(p)[rr];
+    float4 v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 v = po[(4 * warp + j) * PA_WIDE_ROWS + rr];
-        o[j].x = fmaf(v.x, f, o[j].x);
-        o[j].y = fmaf(v.y, f, o[j].y);
-        o[j].z = fmaf(v.z, f, o[j].z);
-        o[j].w = fmaf(v.w, f, o[j].w);
-      }
+    for (int j = 0; j < 4; ++j)
+      v[j] = reinterpret_cast<const float4*>(p + 2 * PA_WIDE_ROWS)[(q + j) * PA_WIDE_ROWS + rr];
+    if (ml.x == -INFINITY) {  // no key, and maybe no o; a NaN l stays one
+      l += ml.y;
+      continue;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const float g = a.gate ? bf2f(a.gate[(long long)(t.q0 + i) * a.Hq + head * G + row % G]) : 1.f;
+    const float mn = fmaxf(m, ml.x);
+    const float f = m == -INFINITY ? 0.f : ex2((m - mn) * a.scale_log2);
+    const float e = ex2((ml.x - mn) * a.scale_log2);
+    m = mn;
+    l = l * f + ml.y * e;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float4 v = make_float4(o[j].x * inv, o[j].y * inv, o[j].z * inv, o[j].w * inv);
-      if (a.gate)
-        v = make_float4(round_bf16(v.x) * g, round_bf16(v.y) * g, round_bf16(v.z) * g,
-                        round_bf16(v.w) * g);
-      rows[lane][4 * warp + j] = make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
+      o[4 * j] = o[4 * j] * f + v[j].x * e;
+      o[4 * j + 1] = o[4 * j + 1] * f + v[j].y * e;
+      o[4 * j + 2] = o[4 * j + 2] * f + v[j].z * e;
+      o[4 * j + 3] = o[4 * j + 3] * f + v[j].w * e;
     }
   }
-  __syncthreads();
-  for (int x = warp; x < JP_ROWS; x += 8) {
-    const int r2 = blockIdx.y * JP_ROWS + x, w2 = r2 / PA_ROWS, row2 = r2 % PA_ROWS;
-    const int i2 = w2 * t.pair * tq + row2 / G, head2 = st.head + (w2 & t.duo);
-    if (row2 >= tq * G || i2 >= t.nq || w2 > (t.pair | t.duo)) continue;
-    reinterpret_cast<uint2*>(a.out + ((long long)(t.q0 + i2) * a.Hq + head2 * G + row2 % G) *
-                                         PA_D)[lane] = rows[x][lane];
-  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint32_t y[8];
+#pragma unroll
+  for (int x = 0; x < 8; ++x)
+    y[x] = pack2(round_bf16(o[2 * x] * inv) * g, round_bf16(o[2 * x + 1] * inv) * g);
+  uint4* dst = reinterpret_cast<uint4*>(a.out + at * PA_D + 4 * q);
+  dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
+  dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
 }
 
-// Joins a stream's parts for one kv head: its share of the prefix's and its own keys'.
+// Joins a stream's parts for one kv head: its share of the prefix's and its own keys'. The parts'
+// weights first, all at once, then every element's sum over the parts.
 __global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
+  __shared__ float2 ml[JS_PARTS][16];
+  __shared__ float inv[16];
   const PaHead h = *a.plan.head;
   const int b = blockIdx.x, head = blockIdx.y, G = a.Hq / a.Hkv, tq = PA_ROWS / G;
-  const PaTile own = a.plan.tiles[h.nprefix + b];
+  const int pi = b / (2 * tq);
+  const PaTile own = a.plan.tiles[a.plan.nprefix + b], pre = a.plan.tiles[pi];
   int c0, c1, p0 = 0, p1 = -1, rr = 0, first = head;
   pa_parts(h, own, head, &c0, &c1);
-  pdl_wait();  // as above
-  if (h.nprefix == 0 && c0 == c1) return;  // written by the CTA that had it whole
-  const int rows = pa_own_rows(a.Hq, a.Hkv), pi = b / (2 * tq);
-  if (h.nprefix) {
-    const PaTile pre = a.plan.tiles[pi];
+  if (h.prefix) {
     pa_parts(h, pre, head, &p0, &p1);
     const int i = b - pre.q0, w = i / tq;
     rr = pre.duo ? (head & 1) * PA_ROWS + i * G : w * PA_ROWS + (i - w * tq) * G;
     first = head & ~pre.duo;
   }
-  const float* wide = a.plan.wide + ((size_t)pi * a.Hkv + first) * pa_slot_floats(PA_WIDE_ROWS);
-  const float* ow = a.plan.own + pa_own_slot(b, head, 0, a.Hkv) * pa_slot_floats(rows);
-  const size_t step = pa_slot_floats(rows) << own.duo;  // from one CTA's part to the next
+  pdl_wait();  // as above
+  if (h.prefix == 0 && c0 == c1) return;  // written by the CTA that had it whole
+  const int rows = pa_own_rows(a.Hq, a.Hkv), np = p1 - p0 + 1, n = np + c1 - c0 + 1;
+  auto part = [&](int x) {  // the first p1 - p0 + 1 are the prefix's
+    return x < np ? a.plan.wide + ((size_t)pi * a.Hkv + first + p0 + x) * pa_slot_floats(PA_WIDE_ROWS)
+                  : a.plan.own + pa_own_slot(b, head, c0 + x - np, a.Hkv) * pa_slot_floats(rows);
+  };
+  for (int e = threadIdx.x; e < n * G; e += 128) {
+    const int x = e / G, g = e % G;
+    ml[x][g] = reinterpret_cast<const float2*>(part(x))[x < np ? rr + g : g];
+  }
+  __syncthreads();
+  if (threadIdx.x < G) {
+    const int g = threadIdx.x;
+    float m = -INFINITY, l = 0.f;
+    for (int x = 0; x < n; ++x) m = fmaxf(m, ml[x][g].x);
+    for (int x = 0; x < n; ++x) {  // a part without a key has weight 0; a NaN l stays one
+      const float f = ml[x][g].x == -INFINITY ? 0.f : ex2((ml[x][g].x - m) * a.scale_log2);
+      l += ml[x][g].x == -INFINITY ? ml[x][g].y : ml[x][g].y * f;
+      ml[x][g].x = f;
+    }
+    inv[g] = l == 0.f ? 0.f : 1.f / l;
+  }
+  __syncthreads();
   for (int e = threadIdx.x; e < G * 32; e += 128) {
     const int g = e % G, q = e / G;  // neighbours take neighbouring rows of one column quad
-    float m = -INFINITY;
-#pragma unroll 2
-    for (int x = p0; x <= p1; ++x)
-      m = fmaxf(m, reinterpret_cast<const float2*>(wide + x * pa_slot_floats(PA_WIDE_ROWS))[rr + g].x);
-#pragma unroll 2
-    for (int x = c0; x <= c1; ++x)
-      m = fmaxf(m, reinterpret_cast<const float2*>(ow + x * step)[g].x);
-    float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float* p, int n, int r) {
-      const float2 ml = reinterpret_cast<const float2*>(p)[r];
-      const float f = ml.x == -INFINITY ? 0.f : ex2((ml.x - m) * a.scale_log2);
-      const float4 v = reinterpret_cast<const float4*>(p + 2 * n)[q * n + r];
-      l += ml.x == -INFINITY ? ml.y : ml.y * f;
+#pragma unroll 4
+    for (int x = 0; x < n; ++x) {
+      const int m = x < np ? PA_WIDE_ROWS : rows;
+      const float4 v = reinterpret_cast<const float4*>(part(x) + 2 * m)[q * m + (x < np ? rr + g : g)];
+      const float f = ml[x][g].x;
       o.x = fmaf(v.x, f, o.x);
       o.y = fmaf(v.y, f, o.y);
       o.z = fmaf(v.z, f, o.z);
       o.w = fmaf(v.w, f, o.w);
-    };
-#pragma unroll 2
-    for (int x = p0; x <= p1; ++x) add(wide + x * pa_slot_floats(PA_WIDE_ROWS), PA_WIDE_ROWS, rr + g);
-#pragma unroll 2
-    for (int x = c0; x <= c1; ++x) add(ow + x * step, rows, g);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    float4 v = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    const long long at = (long long)b * a.Hq + head * G + g;
-    if (a.gate) {
-      const float s = bf2f(a.gate[at]);
-      v = make_float4(round_bf16(v.x) * s, round_bf16(v.y) * s, round_bf16(v.z) * s,
-                      round_bf16(v.w) * s);
     }
-    reinterpret_cast<uint2*>(a.out + at * PA_D)[q] = make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
+    const long long at = (long long)b * a.Hq + head * G + g;
+    const float s = a.gate ? bf2f(a.gate[at]) : 1.f, r = inv[g];
+    reinterpret_cast<uint2*>(a.out + at * PA_D)[q] =
+        make_uint2(pack2(round_bf16(o.x * r) * s, round_bf16(o.y * r) * s),
+                   pack2(round_bf16(o.z * r) * s, round_bf16(o.w * r) * s));
   }
 }
 
