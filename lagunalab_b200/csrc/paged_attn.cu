@@ -918,7 +918,7 @@ __global__ void __launch_bounds__(256) pa_join_prompt_kernel(const PaArgs a) {
 
 // Joins a stream's parts for one kv head: its share of the prefix's and its own keys'. The parts'
 // weights first, all at once, then every element's sum over the parts.
-__global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
+__global__ void __launch_bounds__(256) pa_join_stream_kernel(const PaArgs a) {
   __shared__ float2 ml[JS_PARTS][16];
   __shared__ float inv[16];
   const PaHead h = *a.plan.head;
@@ -940,7 +940,7 @@ __global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
     return x < np ? a.plan.wide + ((size_t)pi * a.Hkv + first + p0 + x) * pa_slot_floats(PA_WIDE_ROWS)
                   : a.plan.own + pa_own_slot(b, head, c0 + x - np, a.Hkv) * pa_slot_floats(rows);
   };
-  for (int e = threadIdx.x; e < n * G; e += 128) {
+  for (int e = threadIdx.x; e < n * G; e += 256) {
     const int x = e / G, g = e % G;
     ml[x][g] = reinterpret_cast<const float2*>(part(x))[x < np ? rr + g : g];
   }
@@ -957,10 +957,10 @@ __global__ void __launch_bounds__(128) pa_join_stream_kernel(const PaArgs a) {
     inv[g] = l == 0.f ? 0.f : 1.f / l;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < G * 32; e += 128) {
+  for (int e = threadIdx.x; e < G * 32; e += 256) {
     const int g = e % G, q = e / G;  // neighbours take neighbouring rows of one column quad
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
     for (int x = 0; x < n; ++x) {
       const int m = x < np ? PA_WIDE_ROWS : rows;
       const float4 v = reinterpret_cast<const float4*>(part(x) + 2 * m)[q * m + (x < np ? rr + g : g)];
@@ -1085,7 +1085,7 @@ static int attn_run(const char* who, int kind, const void* q, long long q_tok, l
     LG_CUDA_TRY(cudaLaunchKernelEx(&cfg, pa_join_prompt_kernel, a));
   } else {
     cfg.gridDim = dim3(B, Hkv);
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(256);
     LG_CUDA_TRY(cudaLaunchKernelEx(&cfg, pa_join_stream_kernel, a));
   }
   LG_LAUNCH_CHECK("paged_join");
