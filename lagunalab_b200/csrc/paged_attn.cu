@@ -326,6 +326,13 @@ __device__ __forceinline__ uint32_t key_bits(int lo, int hi) {
   return from & to;
 }
 
+// bf16 products, each rounded once: with pack2 the two roundings of bf16(bf16(o) * gate).
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -778,7 +785,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           if (valid && (!halves || w == 0))
             reinterpret_cast<float2*>(slot)[rr] = make_float2(m, l);
         }
-        const float g = bf2f(gb);
+        const uint32_t g2 = __bfloat16_as_ushort(gb) * 0x10001u;  // the gate, twice
+        const int row_to = valid ? (int)at : -1;  // rows of out: below 2^31 (checked on the host)
         if (whole) {  // the sum's reciprocal; a row without a key is 0
           const float inv = l == 0.f ? 0.f : 1.f / l;
           f0 *= inv;
@@ -818,21 +826,25 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             uint32_t y[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-              y[x] = pack2(round_bf16(o[8 * k + 2 * x]) * g, round_bf16(o[8 * k + 2 * x + 1]) * g);
+              y[x] = mul_bf16x2(pack2(o[8 * k + 2 * x], o[8 * k + 2 * x + 1]), g2);
             *reinterpret_cast<uint4*>(stage + lane * 128 + ((4 * (j & 1) + k) ^ (lane & 7)) * 16) =
                 make_uint4(y[0], y[1], y[2], y[3]);
           }
           __syncwarp();
           if (j & 1) {  // 64 columns are there: whole 128-byte lines, 8 lanes a row
+            uint4 v[8];
+            int to[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const int src = 4 * k + (lane >> 3);
-              const long long to = __shfl_sync(0xffffffffu, valid ? at : -1LL, src);
-              const uint4 v = *reinterpret_cast<const uint4*>(stage + src * 128 +
-                                                              ((lane & 7) ^ (src & 7)) * 16);
-              if (to >= 0)
-                *reinterpret_cast<uint4*>(a.out + to * PA_D + 32 * (j - 1) + (lane & 7) * 8) = v;
+              to[k] = __shfl_sync(0xffffffffu, row_to, src);
+              v[k] = *reinterpret_cast<const uint4*>(stage + src * 128 +
+                                                     ((lane & 7) ^ (src & 7)) * 16);
             }
+            __nv_bfloat16* const dst = a.out + 32 * (j - 1) + (lane & 7) * 8;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (to[k] >= 0) *reinterpret_cast<uint4*>(dst + (long long)to[k] * PA_D) = v[k];
             __syncwarp();
           }
         }
@@ -936,13 +948,14 @@ __global__ void __launch_bounds__(256) pa_join_stream_kernel(const PaArgs a) {
   pdl_wait();  // as above
   if (h.prefix == 0 && c0 == c1) return;  // written by the CTA that had it whole
   const int rows = pa_own_rows(a.Hq, a.Hkv), np = p1 - p0 + 1, n = np + c1 - c0 + 1;
-  auto part = [&](int x) {  // the first p1 - p0 + 1 are the prefix's
-    return x < np ? a.plan.wide + ((size_t)pi * a.Hkv + first + p0 + x) * pa_slot_floats(PA_WIDE_ROWS)
-                  : a.plan.own + pa_own_slot(b, head, c0 + x - np, a.Hkv) * pa_slot_floats(rows);
-  };
+  // the prefix's parts, one slot apart, and the own keys', one or two
+  const size_t wide_step = pa_slot_floats(PA_WIDE_ROWS), own_step = pa_slot_floats(rows) << own.duo;
+  const float* wide = a.plan.wide + ((size_t)pi * a.Hkv + first + p0) * wide_step;
+  const float* ow = a.plan.own + pa_own_slot(b, head, c0, a.Hkv) * pa_slot_floats(rows);
   for (int e = threadIdx.x; e < n * G; e += 256) {
     const int x = e / G, g = e % G;
-    ml[x][g] = reinterpret_cast<const float2*>(part(x))[x < np ? rr + g : g];
+    ml[x][g] = x < np ? reinterpret_cast<const float2*>(wide + x * wide_step)[rr + g]
+                      : reinterpret_cast<const float2*>(ow + (x - np) * own_step)[g];
   }
   __syncthreads();
   if (threadIdx.x < G) {
@@ -960,16 +973,19 @@ __global__ void __launch_bounds__(256) pa_join_stream_kernel(const PaArgs a) {
   for (int e = threadIdx.x; e < G * 32; e += 256) {
     const int g = e % G, q = e / G;  // neighbours take neighbouring rows of one column quad
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int x = 0; x < n; ++x) {
-      const int m = x < np ? PA_WIDE_ROWS : rows;
-      const float4 v = reinterpret_cast<const float4*>(part(x) + 2 * m)[q * m + (x < np ? rr + g : g)];
-      const float f = ml[x][g].x;
-      o.x = fmaf(v.x, f, o.x);
-      o.y = fmaf(v.y, f, o.y);
-      o.z = fmaf(v.z, f, o.z);
-      o.w = fmaf(v.w, f, o.w);
-    }
+    auto sum = [&](const float* p, size_t step, int x0, int x1) {
+#pragma unroll 4
+      for (int x = x0; x < x1; ++x, p += step) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        const float f = ml[x][g].x;
+        o.x = fmaf(v.x, f, o.x);
+        o.y = fmaf(v.y, f, o.y);
+        o.z = fmaf(v.z, f, o.z);
+        o.w = fmaf(v.w, f, o.w);
+      }
+    };
+    sum(wide + 2 * PA_WIDE_ROWS + 4 * (q * PA_WIDE_ROWS + rr + g), wide_step, 0, np);
+    sum(ow + 2 * rows + 4 * (q * rows + g), own_step, np, n);
     const long long at = (long long)b * a.Hq + head * G + g;
     const float s = a.gate ? bf2f(a.gate[at]) : 1.f, r = inv[g];
     reinterpret_cast<uint2*>(a.out + at * PA_D)[q] =
@@ -987,6 +1003,7 @@ static int plan_check(const char* who, int T, int B, int Hq, int Hkv, int R, int
                "%s: %d query heads over %d kv heads (a group of at most 16)", who, Hq, Hkv);
   LG_CHECK_ARG(R == 16 || R == 32 || R == 64 || R == 128, "%s: pages of %d rows (16, 32, 64 or 128)",
                who, R);
+  LG_CHECK_ARG((long long)T * Hq < (1LL << 31), "%s: %d tokens of %d heads", who, T, Hq);
   LG_CHECK_ARG(window >= 0, "%s: window %d", who, window);
   return LG_OK;
 }
