@@ -591,6 +591,19 @@ int lg_pages_compact(void* pool, int planes, int H, int R, int row_bytes, int32_
                      size_t workspace_bytes, void* stream);
 
 /*
+ * lg_attn_prep for T packed tokens of B sequences over a paged bf16 cache: token t is at position
+ * pos[t] of sequence seq[t] (device int32 [T]); its k and v rows go into row pos[t] % R of page
+ * table[seq[t], pos[t] / R] of k_pages, v_pages (pages of [Hkv, R, D], page_stride elements apart).
+ * A token without such a page leaves no row. q_out bf16 [T, Hq, D]. The same bits as lg_attn_prep.
+ */
+int lg_attn_prep_pages(const void* qkvg, int T, int Hq, int Hkv, int D, const void* qn_w,
+                       const void* kn_w, float eps, float rope_theta, const int32_t* seq,
+                       const int32_t* pos, const int32_t* table, int B, int M, int P, int R,
+                       long long page_stride, int gate_per_head, void* q_out, void* k_pages,
+                       void* v_pages, void* gate_out, const float* inv_freq, int rot_dims,
+                       float mscale, void* stream);
+
+/*
  * Plans: how a batch's attention work is divided over the GPU, computed on the device from the
  * lengths. A plan serves every layer with the same heads, page rows and window; it also holds the
  * partial results of a call, so two calls that can overlap on the GPU need a plan each.

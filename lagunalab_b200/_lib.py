@@ -98,6 +98,8 @@ SIGNATURES = {
     "lg_pages_free": (c_int, [P, P, P, I, I, I, P, I, P, P]),
     "lg_pages_fork": (c_int, [P, I, I, I, I, P, P, P, I, I, I, P, P, I, P, P, c_size_t, P]),
     "lg_pages_compact": (c_int, [P, I, I, I, I, P, P, I, I, I, P, P, c_size_t, P]),
+    "lg_attn_prep_pages": (c_int, [P, I, I, I, I, P, P, c_float, c_float, P, P, P, I, I, I, I,
+                                   c_longlong, I, P, P, P, P, P, I, c_float, P]),
     "lg_prompt_plan_bytes": (c_size_t, [I, I, I, I]),
     "lg_stream_plan_bytes": (c_size_t, [I, I, I]),
     "lg_plan_status": (c_int, [P, ctypes.POINTER(c_int)]),

@@ -752,6 +752,37 @@ def pages_compact(pool, table, refs):
     return status
 
 
+def attn_prep_pages(qkvg, Hq, Hkv, D, qn_w, kn_w, eps, theta, seq, pos, table, k_pages, v_pages,
+                    gate_per_head=True, rope=None):
+    """``attn_prep`` of T packed tokens over cache pages: token t is at position pos[t] of the
+    sequence of table row seq[t] (device int32 [T]); its k, v rows go into that sequence's page of
+    k_pages, v_pages [P, Hkv, R, D]. Returns (q [T, Hq, D], gate [T, Hq or Hq*D])."""
+    qkvg = _c(qkvg, torch.bfloat16)
+    index, T = qkvg.get_device(), qkvg.shape[0]
+    P, h, R, d = k_pages.shape
+    width = (Hq + 2 * Hkv) * D + (Hq if gate_per_head else Hq * D)
+    if qkvg.shape != (T, width):
+        raise ValueError(f"the projections must be [{T}, {width}], not {tuple(qkvg.shape)}")
+    if (h, d) != (Hkv, D) or v_pages.shape != k_pages.shape or \
+            k_pages.stride() != v_pages.stride() or k_pages[0].is_contiguous() is False or \
+            k_pages.dtype is not _BF16 or v_pages.dtype is not _BF16:
+        raise ValueError(f"k_pages and v_pages must be bf16 [P, {Hkv}, R, {D}] with whole pages")
+    if k_pages.get_device() != index or v_pages.get_device() != index:
+        raise ValueError(f"the pages are not on {qkvg.device}")
+    B, M = _i32(table, "table", 2, index)
+    if _i32(seq, "seq", 1, index)[0] != T or _i32(pos, "pos", 1, index)[0] != T:
+        raise ValueError(f"seq and pos must hold {T} tokens")
+    q = torch.empty(T, Hq, D, dtype=_BF16, device=qkvg.device)
+    gate = torch.empty(T, Hq if gate_per_head else Hq * D, dtype=_BF16, device=qkvg.device)
+    inv, rot, ms, _, _ = _rope_args(rope, 0, 0)
+    _call_on(index, _lib.lib().lg_attn_prep_pages, qkvg.data_ptr(), T, Hq, Hkv, D, _p(_c(qn_w)),
+             _p(_c(kn_w)), float(eps), float(theta), seq.data_ptr(), pos.data_ptr(),
+             table.data_ptr(), B, M, P, R, k_pages.stride(0) if P > 1 else Hkv * R * D,
+             int(bool(gate_per_head)), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+             gate.data_ptr(), inv, rot, ms)
+    return q, gate
+
+
 class AttentionPlan:
     """The division of a batch's paged attention over the GPU (``prompt_plan``, ``stream_plan``).
     It serves every layer with the same heads, page rows and window, and holds a call's partial
