@@ -1,32 +1,45 @@
 // Attention over a paged bf16 K/V cache: packed prompts (causal, grouped heads, optional sliding
 // window) and one-token streams that share a prefix.
 //
-// For a query q at position p of a sequence (token and head), S = {j : max(0, p - W + 1) <= j <= p}:
+// For a query q at position p of a sequence (token and head) and
+// S = {j : max(0, p - W + 1) <= j <= p}:
 //   out = sum_{j in S} softmax_S(scale q . k_j) v_j      (0 where S is empty)
-// with one pass over the keys: a running reference m, l = sum exp(s_j - m), o = sum exp(s_j - m) v_j,
-// all in fp32; out = bf16(o / l), then bf16(out * gate) with a gate per (token, head).
+// with one pass over the keys: a running reference m, l = sum exp(s_j - m),
+// o = sum exp(s_j - m) v_j, all in fp32; out = bf16(o / l), then bf16(out * gate) with a gate per (token, head).
 //
 // One kernel serves all of it. A row tile is 128 query rows of one kv head: the G query heads of
 // 128 / G tokens (or streams) beside each other, so that grouped heads share every key they read
 // and the causal edge costs at most 128 / G keys a tile. Per 128-key tile two products run on the
 // tensor cores, S = Q K^T (both operands in shared memory) and O += P V (P from TMEM, where the
 // softmax warps put it in bf16 over the scores; V as it lies, keys by head dim).
-//   warps 0-3, 4-7  softmax of row tile 0 / 1, a row a thread: scores from TMEM, mask, exponentials,
-//                   P into TMEM, and the output at the end
+//   warps 0-3, 4-7  softmax of row tile 0 / 1, a row a thread: scores from TMEM, mask,
+//                   exponentials, P into TMEM, and the output at the end
 //   warps 8, 11     issue the products of row tile 0 / 1
-//   warp 10         clears what a last V tile holds past the last key
 //   warp 9          TMA: Q, and the pages' rows into a ring of four 32 KB tiles
-// Two row tiles (a pair) take each key tile in turn, so one's softmax runs under the other's
-// products. A lone row tile (streams, short prompts) takes the key tiles in turn as two halves,
-// even and odd ones, whose results are joined at the end: the same overlap, and 128 KB of loads in
-// flight for a cache that is read once.
+//   warp 10         clears what a last V tile holds past the last key
+// Two row tiles are always at work, so that one's softmax runs under the other's products: two of
+// the same head that share each key tile (a pair: 64 KB of keys and values for 256 rows), or, where
+// there is one only (streams, short prompts), the same tokens' of two neighbouring heads (a duo),
+// or with an odd number of kv heads the one row tile with its even and odd key tiles, joined at
+// the end.
 //
-// The reference m of a row follows the maximum only when that moves by more than 2^8 (the rows'
-// sums and O are then rescaled): exponentials up to 2^8 lose nothing in fp32 or bf16, and the
-// common tile touches O only through the tensor cores.
+// The reference m of a row follows the maximum only when that moves by more than 2^8 (the row's sum
+// and O are then rescaled): weights up to 2^8 lose nothing in fp32 or bf16, and the common tile
+// touches O only through the tensor cores. P is rounded to bf16 (relative 2^-8 a weight at most)
+// because the tensor cores take it so; l sums the unrounded weights; O, m and l stay in fp32
+// through the join.
 //
-// P is rounded to bf16 (relative 2^-8 a weight, averaged over the keys) because the tensor cores
-// take it so; l sums the unrounded weights, and O, m and l stay in fp32 through the join.
+// What bounds it. A key tile of a pair is 2,048 cycles of products, 2,048 of the special function
+// units' exponentials and about 2,300 of the softmax warps' issue; the chain scores -> weights ->
+// products of one row tile is 1,420 cycles of softmax alone, 2,200 beside the other's, and 1,024 of
+// products, and takes 3,700 with its hand-overs. Measured (B200, graph replays): one 8,192-token
+// prompt with 32/4 heads 518 us, 1,060 TFLOP/s of the causal half; 2 x 512 tokens over 33,000 rows
+// 503 us, 1,050 TFLOP/s (0.64 of the measured bf16 GEMM rate); 16 prompts of up to 1,500 tokens
+// 156 us; 64 streams on an 8,192-row prefix 32 us, of which the join is 5.
+// Tried without gain: four softmax warpgroups (two threads a row; 560 us for 500), key tiles of 64
+// with two score places each (541; a 64-wide product takes as long as a 128-wide one), a part of
+// the exponentials as a polynomial on the FMA pipes (1/8: 526, 1/3: 546), the two product warps without
+// turns (556), one arrival for all of a tile's weights (519).
 #include <atomic>
 
 #include "paged.cuh"
@@ -289,7 +302,7 @@ __device__ __forceinline__ int pa_ring(int place, int n, bool pair) {
   if (pair) return place;
   if (place < 2) return place == 0 ? 0 : n > 1 ? 2 : 1;
   if (place >= 2 * n - 2) return 2 * (place - n) + 1;  // the last two V
-  return place & 1 ? place + 1 : place - 1;            // K tile (place + 1) / 2, V tile place / 2 - 1
+  return place & 1 ? place + 1 : place - 1;  // K tile (place + 1) / 2, V tile place / 2 - 1
 }
 
 // Whether the part that ends with key tile t1 has keys past the segment's end in its last tile.
@@ -448,193 +461,196 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 8) {  // one setmaxnreg for the whole warpgroup
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_OTHER));
-  if (warp == 9) {
-    // ---- loads: per segment Q, and K and V tiles in the order of use ----
-    int rc = 0, seg = 0, nq = 0;  // ring tiles, segments and Q tiles so far
-    bool ok = true;
-    const int boxes = PA_KEYS / a.R;  // pages a tile; lanes [0, 2 boxes): (page, half)
-    const bool mine = lane < 2 * boxes;
-    const int half = lane & 1, box = lane >> 1;
-    for (; ok && walk.next(); ++seg) {
-      const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
-      const int n = (walk.t1 - walk.t0) << r.duo;
-      const bool clear = pa_tail(r, walk.t1);
-      if (lane == 0) bad[seg % PA_NBAD] = 0;
-      __syncwarp();
-      const int npage = (r.key_end + a.R - 1) / a.R;  // pages the rows need
-      const int* row = a.table + (long long)r.row * a.M;
-      // The table 32 columns at a time, a column a lane, the next 32 fetched ahead: a key tile's
-      // entries lie within one such group or the next.
-      const int c0 = r.key0 / a.R + walk.t0 * boxes;
-      auto entries = [&](int c) { return c + lane < min(npage, a.M) ? __ldg(row + c + lane) : -1; };
-      int group = 0, cur = entries(c0), nxt = entries(c0 + 32);
-#pragma unroll 1
-      for (int place = 0; place < 2 * n; ++place) {
-        const int slot = rc % PA_RING, x = pa_ring(place, n, r.pair), t = x >> 1 >> r.duo;
-        const int col = t * boxes - group + box;  // V tiles trail K tiles by two at most
-        const int in_cur = __shfl_sync(0xffffffffu, cur, col & 31);
-        const int in_nxt = __shfl_sync(0xffffffffu, nxt, col & 31);
-        int page = col < 32 ? in_cur : in_nxt;
-        if ((x & 1) && t * boxes - group >= 32) {  // the last use of the older group has gone
-          group += 32;
-          cur = nxt;
-          nxt = entries(c0 + group + 32);
-        }
-        if (!(ok = warp_wait(empty + slot, ((rc / PA_RING) & 1) ^ 1, err, 1))) break;
-        uint64_t* const bar = (clear && place + 1 + r.duo >= 2 * n ? tail : full) + slot;
-        if (lane == 0) mbar_arrive_expect_tx(bar, PA_TILE_BYTES);
-        if ((unsigned)page >= (unsigned)a.P) {
-          page = a.P;  // outside the pool: reads as zeros
-          if (mine && c0 + t * boxes + box < npage) bad[seg % PA_NBAD] = 1;
-        }
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_OTHER));
+    if (warp == 9) {
+      // ---- loads: per segment Q, and K and V tiles in the order of use ----
+      int rc = 0, seg = 0, nq = 0;  // ring tiles, segments and Q tiles so far
+      bool ok = true;
+      const int boxes = PA_KEYS / a.R;  // pages a tile; lanes [0, 2 boxes): (page, half)
+      const bool mine = lane < 2 * boxes;
+      const int half = lane & 1, box = lane >> 1;
+      for (; ok && walk.next(); ++seg) {
+        const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
+        const int n = (walk.t1 - walk.t0) << r.duo;
+        const bool clear = pa_tail(r, walk.t1);
+        if (lane == 0) bad[seg % PA_NBAD] = 0;
         __syncwarp();
-        if (mine)
-          tma_load_4d(sKV + slot * PA_TILE_BYTES + half * PA_HALF + box * a.R * 128,
-                      x & 1 ? &tm_v : &tm_k, bar, half * 64, 0, walk.at.head + (x >> 1 & r.duo), page);
-        ++rc;
-        if (place == 0) {
-          if (!(ok = warp_wait(q_empty, (seg & 1) ^ 1, err, 2))) break;
-          ++nq;
-          if (lane == 0) {
-            const int halves = r.pair || r.duo ? 4 : 2;
-            mbar_arrive_expect_tx(q_full, halves * 128 * G * tq);
-            for (int f = 0; f < halves; ++f)
-              tma_load_3d(sQ + f * PA_HALF, &tm_q, q_full, (f & 1) * 64,
-                          (walk.at.head + (f >> 1 & r.duo)) * G, r.q0 + (f >> 1) * r.pair * tq);
+        const int npage = (r.key_end + a.R - 1) / a.R;  // pages the rows need
+        const int* row = a.table + (long long)r.row * a.M;
+        // The table 32 columns at a time, a column a lane, the next 32 fetched ahead: a key tile's
+        // entries lie within one such group or the next.
+        const int c0 = r.key0 / a.R + walk.t0 * boxes;
+        auto entries = [&](int c) {
+          return c + lane < min(npage, a.M) ? __ldg(row + c + lane) : -1;
+        };
+        int group = 0, cur = entries(c0), nxt = entries(c0 + 32);
+#pragma unroll 1
+        for (int place = 0; place < 2 * n; ++place) {
+          const int slot = rc % PA_RING, x = pa_ring(place, n, r.pair), t = x >> 1 >> r.duo;
+          const int col = t * boxes - group + box;  // V tiles trail K tiles by two at most
+          const int in_cur = __shfl_sync(0xffffffffu, cur, col & 31);
+          const int in_nxt = __shfl_sync(0xffffffffu, nxt, col & 31);
+          int page = col < 32 ? in_cur : in_nxt;
+          if ((x & 1) && t * boxes - group >= 32) {  // the last use of the older group has gone
+            group += 32;
+            cur = nxt;
+            nxt = entries(c0 + group + 32);
+          }
+          if (!(ok = warp_wait(empty + slot, ((rc / PA_RING) & 1) ^ 1, err, 1))) break;
+          uint64_t* const bar = (clear && place + 1 + r.duo >= 2 * n ? tail : full) + slot;
+          if (lane == 0) mbar_arrive_expect_tx(bar, PA_TILE_BYTES);
+          if ((unsigned)page >= (unsigned)a.P) {
+            page = a.P;  // outside the pool: reads as zeros
+            if (mine && c0 + t * boxes + box < npage) bad[seg % PA_NBAD] = 1;
           }
           __syncwarp();
+          if (mine)
+            tma_load_4d(sKV + slot * PA_TILE_BYTES + half * PA_HALF + box * a.R * 128,
+                        x & 1 ? &tm_v : &tm_k, bar, half * 64, 0,
+                        walk.at.head + (x >> 1 & r.duo), page);
+          ++rc;
+          if (place == 0) {
+            if (!(ok = warp_wait(q_empty, (seg & 1) ^ 1, err, 2))) break;
+            ++nq;
+            if (lane == 0) {
+              const int halves = r.pair || r.duo ? 4 : 2;
+              mbar_arrive_expect_tx(q_full, halves * 128 * G * tq);
+              for (int f = 0; f < halves; ++f)
+                tma_load_3d(sQ + f * PA_HALF, &tm_q, q_full, (f & 1) * 64,
+                            (walk.at.head + (f >> 1 & r.duo)) * G, r.q0 + (f >> 1) * r.pair * tq);
+            }
+            __syncwarp();
+          }
         }
+        walk.step(a.Hkv, then);
       }
-      walk.step(a.Hkv, then);
-    }
-    // every copy issued has landed before the CTA ends (bounded, also after a failed wait)
-    const long long t0 = clock64();
-    for (int i = max(0, rc - PA_RING); i < rc; ++i)
-      while (!mbar_try_wait(full + i % PA_RING, (i / PA_RING) & 1) &&
-             clock64() - t0 < 4000000000LL) {
+      // every copy issued has landed before the CTA ends (bounded, also after a failed wait)
+      const long long t0 = clock64();
+      for (int i = max(0, rc - PA_RING); i < rc; ++i)
+        while (!mbar_try_wait(full + i % PA_RING, (i / PA_RING) & 1) &&
+               clock64() - t0 < 4000000000LL) {
+        }
+      while (nq > 0 && !mbar_try_wait(q_full, (nq - 1) & 1) && clock64() - t0 < 4000000000LL) {
       }
-    while (nq > 0 && !mbar_try_wait(q_full, (nq - 1) & 1) && clock64() - t0 < 4000000000LL) {
-    }
-  } else if (warp == 8 || warp == 11) {
-    // ---- products of row tile (or half of the keys) w: lane 0 issues, the warp stays together so
-    // that all operands are uniform. The tensor cores hold only two or three products ahead, an
-    // issue waits for room and every wait costs 115 cycles or more, so each w has a warp of its
-    // own: one's waits pass under the other's products. Both see every tile of the ring go by (a
-    // skipped phase of a barrier could not be told from the next); one that w does not use it
-    // gives back at once, the others its softmax warps do. ----
-    const int w = warp == 11;
-    int rc = 0, seg = 0;
-    bool ok = true;
-    uint32_t p_phase = 0, turn_phase = 0;
-    const uint32_t one = lane == 0;
-    const uint32_t id_qk = idesc_bf16(PA_ROWS, PA_KEYS);
-    const uint32_t id_pv = idesc_bf16(PA_ROWS, PA_D) | IDESC_B_MN;
-    const uint32_t q_lo = sw128_lo(smem_u32(sQ)), k_lo = sw128_lo(smem_u32(sKV));
-    const uint32_t v_lo = sw128_lo_mn(smem_u32(sKV), PA_HALF);
-    const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
-    for (; ok && walk.next(); ++seg) {
-      const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
-      const int n = (walk.t1 - walk.t0) << r.duo;
-      const int lim = r.pair && w == 0 ? min(n, max(0, r.ntile0 - walk.t0)) : n;
-      const int step = r.pair ? 1 : 2, first = r.pair ? 0 : w;
-      uint32_t slot = 0;  // the tile at hand, in 16-byte units
-      auto qk = [&](int t) {
-        const uint32_t q = q_lo + (r.pair || r.duo ? w * (PA_TILE_BYTES >> 4) : 0);
-        const uint32_t k = k_lo + slot;
+    } else if (warp == 8 || warp == 11) {
+      // ---- products of row tile (or half of the keys) w: lane 0 issues, the warp stays together
+      // so that all operands are uniform. The tensor cores hold only two or three products ahead, an
+      // issue waits for room and every wait costs 115 cycles or more, so each w has a warp of its
+      // own: one's waits pass under the other's products. Both see every tile of the ring go by (a
+      // skipped phase of a barrier could not be told from the next); one that w does not use it
+      // gives back at once, the others its softmax warps do. ----
+      const int w = warp == 11;
+      int rc = 0, seg = 0;
+      bool ok = true;
+      uint32_t p_phase = 0, turn_phase = 0;
+      const uint32_t one = lane == 0;
+      const uint32_t id_qk = idesc_bf16(PA_ROWS, PA_KEYS);
+      const uint32_t id_pv = idesc_bf16(PA_ROWS, PA_D) | IDESC_B_MN;
+      const uint32_t q_lo = sw128_lo(smem_u32(sQ)), k_lo = sw128_lo(smem_u32(sKV));
+      const uint32_t v_lo = sw128_lo_mn(smem_u32(sKV), PA_HALF);
+      const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
+      for (; ok && walk.next(); ++seg) {
+        const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
+        const int n = (walk.t1 - walk.t0) << r.duo;
+        const int lim = r.pair && w == 0 ? min(n, max(0, r.ntile0 - walk.t0)) : n;
+        const int step = r.pair ? 1 : 2, first = r.pair ? 0 : w;
+        uint32_t slot = 0;  // the tile at hand, in 16-byte units
+        auto qk = [&](int t) {
+          const uint32_t q = q_lo + (r.pair || r.duo ? w * (PA_TILE_BYTES >> 4) : 0);
+          const uint32_t k = k_lo + slot;
 #pragma unroll
-        for (int s = 0; s < PA_D / 16; ++s) {
-          const uint32_t off = ((s >> 2) * PA_HALF + (s & 3) * 32) >> 4;
-          umma_bf16_warp(one, tS, q + off, k + off, SW128_HI, id_qk, s > 0);
-        }
-        umma_commit_warp(one, s_full + w);
-        if (t + step >= lim) umma_commit_warp(one, q_empty);  // the last use of Q
-      };
-      // The two warps take turns, each with a weights' and a score product: left alone they fall
-      // into step, both row tiles' products at once and then both softmaxes.
-      auto turn_wait = [&]() {
-        ok = ok && warp_wait(turn + w, turn_phase, err, 9);
-        turn_phase ^= 1;
-      };
-      auto turn_pass = [&]() {
-        if (ok && lane == 0) mbar_arrive(turn + 1 - w);
-      };
-      // O += P V, as soon as each half of the weights is there
-      auto pv = [&](int t) {
-        const uint32_t v = v_lo + slot;
+          for (int s = 0; s < PA_D / 16; ++s) {
+            const uint32_t off = ((s >> 2) * PA_HALF + (s & 3) * 32) >> 4;
+            umma_bf16_warp(one, tS, q + off, k + off, SW128_HI, id_qk, s > 0);
+          }
+          umma_commit_warp(one, s_full + w);
+          if (t + step >= lim) umma_commit_warp(one, q_empty);  // the last use of Q
+        };
+        // The two warps take turns, each with a weights' and a score product: left alone they fall
+        // into step, both row tiles' products at once and then both softmaxes.
+        auto turn_wait = [&]() {
+          ok = ok && warp_wait(turn + w, turn_phase, err, 9);
+          turn_phase ^= 1;
+        };
+        auto turn_pass = [&]() {
+          if (ok && lane == 0) mbar_arrive(turn + 1 - w);
+        };
+        // O += P V, as soon as each half of the weights is there
+        auto pv = [&](int t) {
+          const uint32_t v = v_lo + slot;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          ok = ok && warp_wait(p_ready + 2 * w + half, p_phase, err, 4);
-          if (half == 0) turn_wait();
-          if (!ok) return;
-          tc_fence_after();
+          for (int half = 0; half < 2; ++half) {
+            ok = ok && warp_wait(p_ready + 2 * w + half, p_phase, err, 4);
+            if (half == 0) turn_wait();
+            if (!ok) return;
+            tc_fence_after();
 #pragma unroll
-          for (int s = 4 * half; s < 4 * half + 4; ++s)
-            umma_bf16_ts_warp(one, tO, tS + s * 8, v + s * (2048 >> 4), SW128_HI, id_pv,
-                              s > 0 || t != first);
-        }
-        p_phase ^= 1;
-        if (t + step >= lim) umma_commit_warp(one, o_full + w);
-      };
-      ok = warp_wait(q_full, seg & 1, err, 5);
-      tc_fence_after();
-      if (ok && first >= lim && lane == 0) mbar_arrive(q_empty);
-      const int lead = r.pair ? 1 : 2;
+            for (int s = 4 * half; s < 4 * half + 4; ++s)
+              umma_bf16_ts_warp(one, tO, tS + s * 8, v + s * (2048 >> 4), SW128_HI, id_pv,
+                                s > 0 || t != first);
+          }
+          p_phase ^= 1;
+          if (t + step >= lim) umma_commit_warp(one, o_full + w);
+        };
+        ok = warp_wait(q_full, seg & 1, err, 5);
+        tc_fence_after();
+        if (ok && first >= lim && lane == 0) mbar_arrive(q_empty);
+        const int lead = r.pair ? 1 : 2;
 #pragma unroll 1
-      for (int place = 0; ok && place < 2 * n; ++place, ++rc) {
-        const int x = pa_ring(place, n, r.pair), t = x >> 1, s = rc % PA_RING;
-        const bool own = r.pair || (t & 1) == w;
-        const bool use = own && t < lim;
-        if (!(ok = warp_wait(full + s, (rc / PA_RING) & 1, err, 3))) break;
-        if (!use && lane == 0) mbar_arrive(empty + s);
-        slot = __shfl_sync(0xffffffffu, (uint32_t)s * (PA_TILE_BYTES >> 4), 0);
-        if (x & 1) {
-          if (use) pv(t);
-          else if (own) turn_wait();
-          if (own && t + lead >= n) turn_pass();
-        } else {
-          if (use) qk(t);
-          if (own && t >= lead) turn_pass();
+        for (int place = 0; ok && place < 2 * n; ++place, ++rc) {
+          const int x = pa_ring(place, n, r.pair), t = x >> 1, s = rc % PA_RING;
+          const bool own = r.pair || (t & 1) == w;
+          const bool use = own && t < lim;
+          if (!(ok = warp_wait(full + s, (rc / PA_RING) & 1, err, 3))) break;
+          if (!use && lane == 0) mbar_arrive(empty + s);
+          slot = __shfl_sync(0xffffffffu, (uint32_t)s * (PA_TILE_BYTES >> 4), 0);
+          if (x & 1) {
+            if (use) pv(t);
+            else if (own) turn_wait();
+            if (own && t + lead >= n) turn_pass();
+          } else {
+            if (use) qk(t);
+            if (own && t >= lead) turn_pass();
+          }
         }
-      }
-      if (!r.pair && (n & 1) && w == 1) {  // as many turns for both
-        turn_wait();
-        turn_pass();
-      }
-      walk.step(a.Hkv, then);
-    }
-    umma_commit_warp(one, done + w);
-    const long long t0 = clock64();
-    while (!mbar_try_wait(done + w, 0) && clock64() - t0 < 4000000000LL) {
-    }
-  } else if (warp == 10) {
-    // ---- rows of V past the last key hold anything (also NaN): their weights are 0, they become
-    // 0 too. The last V tile of such a segment lands here first and is passed on when clear. ----
-    // A barrier a slot: a second such tile may be under way before the first has landed.
-    int rc = 0;
-    uint32_t phases = 0;
-    bool ok = true;
-    for (; ok && walk.next();) {
-      const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
-      rc += 2 * (walk.t1 - walk.t0) << r.duo;
-      for (int back = 1 + r.duo; ok && back > 0 && pa_tail(r, walk.t1); --back) {
-        const int slot = (rc - back) % PA_RING;  // a part's last tiles in the ring are its last V
-        ok = warp_wait(tail + slot, phases >> slot & 1, err, 8);
-        phases ^= 1u << slot;
-        uint8_t* v = sKV + slot * PA_TILE_BYTES;
-        const int keep = max(0, r.key_end - (r.key0 + (walk.t1 - 1) * PA_KEYS));
-        for (int x = keep * 8 + lane; ok && x < PA_KEYS * 8; x += 32) {
-          *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(v + PA_HALF + x * 16) = make_uint4(0, 0, 0, 0);
+        if (!r.pair && (n & 1) && w == 1) {  // as many turns for both
+          turn_wait();
+          turn_pass();
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (ok && lane == 0) mbar_arrive(full + slot);
+        walk.step(a.Hkv, then);
       }
-      walk.step(a.Hkv, then);
+      umma_commit_warp(one, done + w);
+      const long long t0 = clock64();
+      while (!mbar_try_wait(done + w, 0) && clock64() - t0 < 4000000000LL) {
+      }
+    } else if (warp == 10) {
+      // ---- rows of V past the last key hold anything (also NaN): their weights are 0, they become
+      // 0 too. The last V tile of such a segment lands here first and is passed on when clear. ----
+      // A barrier a slot: a second such tile may be under way before the first has landed.
+      int rc = 0;
+      uint32_t phases = 0;
+      bool ok = true;
+      for (; ok && walk.next();) {
+        const PaTile r = walk.rec, then = walk.ahead(a.Hkv);
+        rc += 2 * (walk.t1 - walk.t0) << r.duo;
+        for (int back = 1 + r.duo; ok && back > 0 && pa_tail(r, walk.t1); --back) {
+          const int slot = (rc - back) % PA_RING;  // a part's last tiles in the ring are its last V
+          ok = warp_wait(tail + slot, phases >> slot & 1, err, 8);
+          phases ^= 1u << slot;
+          uint8_t* v = sKV + slot * PA_TILE_BYTES;
+          const int keep = max(0, r.key_end - (r.key0 + (walk.t1 - 1) * PA_KEYS));
+          for (int x = keep * 8 + lane; ok && x < PA_KEYS * 8; x += 32) {
+            *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(v + PA_HALF + x * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (ok && lane == 0) mbar_arrive(full + slot);
+        }
+        walk.step(a.Hkv, then);
+      }
     }
-  }
-  __syncwarp();
+    __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_REGS_SOFTMAX));
     // ---- softmax: warpgroup w, a row a thread ----
@@ -755,7 +771,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
       rc += 2 * n;
       if (active) {
-        if (bad[seg % PA_NBAD] || !ok) l = NAN;
+        // The flag is this segment's once one of its key tiles has been seen; a half without one
+        // is ahead of the loads here and looks after it has met the other half.
+        if ((any && bad[seg % PA_NBAD]) || !ok) l = NAN;
         float f0 = 1.f, f1 = 0.f;
         if (halves) {
           ml[w * PA_ROWS + row] = make_float2(m, l);
