@@ -28,17 +28,18 @@ struct PaTile {
   int ntile0;   // pair: key tiles of the first row tile (at most ntile)
   int kind;
   int pair;  // 1: two row tiles (2 * tq tokens) share each key tile
-  int duo;   // 1: the same tokens' row tiles of two neighbouring kv heads, with their own key tiles;
-             // neither (an odd number of kv heads): one row tile, its key tiles in two halves
+  int duo;   // 1: the same tokens' row tiles of two neighbouring kv heads, each with its own key
+             // tiles; neither (an odd number of kv heads): one row tile, its key tiles in halves
   int w;     // cost of a key tile (of both heads')
   long long before;  // cost of all segments before this tile's first
 };
 
-// Costs: half a row tile's worth of tensor-core time on one key tile is 1, so a key tile of two row
-// tiles is 4 and of one 2; a stream's own key tile waits for HBM rather than the tensor cores.
-// Every segment costs PA_SEG more (Q load, first score, output).
-constexpr int PA_W_TWO = 4, PA_W_ONE = 2, PA_W_OWN = 2, PA_SEG = 8;
-constexpr int PA_MIN_CHUNK = 12;  // at least the largest PA_SEG + w: no CTA below the last is idle
+// Costs: a row tile on one key tile is 2, so a key tile of two row tiles is 4 (2.2 us). A stream's
+// own key tile is 2 as well: its few rows leave most of the softmax out, its loads are HBM's (3: 80
+// against 71 us on 128 streams with a 16,384-row prefix). Every segment costs PA_SEG more (Q load,
+// first score, output; 8: 156 against 153 us on 16 ragged prompts, 2: 205).
+constexpr int PA_W_TWO = 4, PA_W_ONE = 2, PA_W_OWN = 2, PA_SEG = 6;
+constexpr int PA_MIN_CHUNK = 10;  // at least the largest PA_SEG + w: no CTA below the last is idle
 
 __host__ __device__ inline long long pa_cost(int ntile, int w) {
   return PA_SEG + (long long)ntile * w;

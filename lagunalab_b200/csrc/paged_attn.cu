@@ -5,7 +5,8 @@
 // S = {j : max(0, p - W + 1) <= j <= p}:
 //   out = sum_{j in S} softmax_S(scale q . k_j) v_j      (0 where S is empty)
 // with one pass over the keys: a running reference m, l = sum exp(s_j - m),
-// o = sum exp(s_j - m) v_j, all in fp32; out = bf16(o / l), then bf16(out * gate) with a gate per (token, head).
+// o = sum exp(s_j - m) v_j, all in fp32; out = bf16(o / l), then bf16(out * gate) with a gate per
+// (token, head).
 //
 // One kernel serves all of it. A row tile is 128 query rows of one kv head: the G query heads of
 // 128 / G tokens (or streams) beside each other, so that grouped heads share every key they read
@@ -35,11 +36,11 @@
 // products, and takes 3,700 with its hand-overs. Measured (B200, graph replays): one 8,192-token
 // prompt with 32/4 heads 518 us, 1,060 TFLOP/s of the causal half; 2 x 512 tokens over 33,000 rows
 // 503 us, 1,050 TFLOP/s (0.64 of the measured bf16 GEMM rate); 16 prompts of up to 1,500 tokens
-// 156 us; 64 streams on an 8,192-row prefix 32 us, of which the join is 5.
+// 153 us; 64 streams on an 8,192-row prefix 32 us, of which the join is 5.
 // Tried without gain: four softmax warpgroups (two threads a row; 560 us for 500), key tiles of 64
 // with two score places each (541; a 64-wide product takes as long as a 128-wide one), a part of
-// the exponentials as a polynomial on the FMA pipes (1/8: 526, 1/3: 546), the two product warps without
-// turns (556), one arrival for all of a tile's weights (519).
+// the exponentials as a polynomial on the FMA pipes (1/8: 526, 1/3: 546), the two product warps
+// without turns (556), one arrival for all of a tile's weights (519).
 #include <atomic>
 
 #include "paged.cuh"
@@ -534,8 +535,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
     } else if (warp == 8 || warp == 11) {
       // ---- products of row tile (or half of the keys) w: lane 0 issues, the warp stays together
-      // so that all operands are uniform. The tensor cores hold only two or three products ahead, an
-      // issue waits for room and every wait costs 115 cycles or more, so each w has a warp of its
+      // so that all operands are uniform. The tensor cores hold only two or three products ahead,
+      // an issue waits for room and every wait costs 115 cycles or more, so each w has a warp of its
       // own: one's waits pass under the other's products. Both see every tile of the ring go by (a
       // skipped phase of a barrier could not be told from the next); one that w does not use it
       // gives back at once, the others its softmax warps do. ----
@@ -792,13 +793,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           if (r.kind == PA_PROMPT) {
             slot = a.plan.wide + (2 * blockIdx.x + (walk.t0 == 0)) * pa_slot_floats(rows);
           } else if (r.kind == PA_PREFIX) {
-            slot = a.plan.wide +
-                   ((size_t)walk.at.tile * a.Hkv + walk.at.head + blockIdx.x) * pa_slot_floats(rows);
+            slot = a.plan.wide + ((size_t)walk.at.tile * a.Hkv + walk.at.head + blockIdx.x) *
+                                     pa_slot_floats(rows);
           } else {
             rows = pa_own_rows(a.Hq, a.Hkv);
             rr = row;
-            slot = a.plan.own + pa_own_slot(walk.at.tile - a.plan.nprefix, walk.at.head + (w & r.duo),
-                                            blockIdx.x, a.Hkv) * pa_slot_floats(rows);
+            slot = a.plan.own + pa_own_slot(walk.at.tile - a.plan.nprefix,
+                                            walk.at.head + (w & r.duo), blockIdx.x, a.Hkv) *
+                                    pa_slot_floats(rows);
           }
           if (valid && (!halves || w == 0))
             reinterpret_cast<float2*>(slot)[rr] = make_float2(m, l);
@@ -1019,8 +1021,8 @@ static int plan_check(const char* who, int T, int B, int Hq, int Hkv, int R, int
                who, T, B);
   LG_CHECK_ARG(Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16 && Hkv <= 1024,
                "%s: %d query heads over %d kv heads (a group of at most 16)", who, Hq, Hkv);
-  LG_CHECK_ARG(R == 16 || R == 32 || R == 64 || R == 128, "%s: pages of %d rows (16, 32, 64 or 128)",
-               who, R);
+  LG_CHECK_ARG(R == 16 || R == 32 || R == 64 || R == 128,
+               "%s: pages of %d rows (16, 32, 64 or 128)", who, R);
   LG_CHECK_ARG((long long)T * Hq < (1LL << 31), "%s: %d tokens of %d heads", who, T, Hq);
   LG_CHECK_ARG(window >= 0, "%s: window %d", who, window);
   return LG_OK;

@@ -55,7 +55,8 @@ extern "C" int lg_attn_prep_pages(const void* qkvg, int T, int Hq, int Hkv, int 
   LG_CHECK_ARG(B > 0 && M > 0 && P > 0 && R > 0 && page_stride >= (long long)Hkv * R * D,
                "attn_prep_pages: %d sequences of %d pages of %d rows", B, M, R);
   if (T == 0) return LG_OK;
-  LG_CHECK_ARG(qkvg && qn_w && kn_w && seq && pos && table && q_out && k_pages && v_pages && gate_out,
+  LG_CHECK_ARG(qkvg && qn_w && kn_w && seq && pos && table && q_out && k_pages && v_pages &&
+                   gate_out,
                "attn_prep_pages: NULL pointer");
   PagedPrep p = {};
   if (int rc = prep_extend(&p.a, D, inv_freq, rot_dims, mscale, 0, 0, "attn_prep_pages")) return rc;

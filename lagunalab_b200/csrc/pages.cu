@@ -351,8 +351,8 @@ extern "C" int lg_pages_reserve(int32_t* table, int32_t* refs, int S, int M, int
                                 const int32_t* ids, const int32_t* rows, int n, int32_t* status,
                                 void* ws, size_t ws_bytes, void* stream) {
   if (int rc = pages_check("pages_reserve", table, refs, S, M, P)) return rc;
-  LG_CHECK_ARG(((ids && rows) || n == 0) && status && n >= 0 && n <= S && R > 0, "pages_reserve: %d streams of %d",
-               n, S);
+  LG_CHECK_ARG(((ids && rows) || n == 0) && status && n >= 0 && n <= S && R > 0,
+               "pages_reserve: %d streams of %d", n, S);
   if (!ws || ws_bytes < lg_pages_workspace_bytes(P, n))
     return fail(LG_ERR_WORKSPACE, "pages_reserve: workspace too small");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -365,7 +365,8 @@ extern "C" int lg_pages_reserve(int32_t* table, int32_t* refs, int S, int M, int
 extern "C" int lg_pages_free(int32_t* table, int32_t* lens, int32_t* refs, int S, int M, int P,
                              const int32_t* ids, int n, int32_t* status, void* stream) {
   if (int rc = pages_check("pages_free", table, refs, S, M, P)) return rc;
-  LG_CHECK_ARG(lens && (ids || n == 0) && status && n >= 0 && n <= S, "pages_free: %d streams of %d", n, S);
+  LG_CHECK_ARG(lens && (ids || n == 0) && status && n >= 0 && n <= S,
+               "pages_free: %d streams of %d", n, S);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long long all = (long long)n * M;
   const int grid = (int)std::min<long long>(64, all / (4 * PG_THREADS) + 1);
@@ -380,8 +381,8 @@ extern "C" int lg_pages_fork(void* pool, int planes, int H, int R, int row_bytes
                              void* stream) {
   if (int rc = pages_check("pages_fork", table, refs, S, M, P)) return rc;
   if (int rc = pool_check("pages_fork", pool, planes, H, R, row_bytes)) return rc;
-  LG_CHECK_ARG(lens && ((src && dst) || n == 0) && status && n >= 0 && n <= S, "pages_fork: %d children of %d", n,
-               S);
+  LG_CHECK_ARG(lens && ((src && dst) || n == 0) && status && n >= 0 && n <= S,
+               "pages_fork: %d children of %d", n, S);
   if (!ws || ws_bytes < lg_pages_workspace_bytes(P, n))
     return fail(LG_ERR_WORKSPACE, "pages_fork: workspace too small");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -389,8 +390,10 @@ extern "C" int lg_pages_fork(void* pool, int planes, int H, int R, int row_bytes
   pages_fork_plan_kernel<<<1, PG_THREADS, 0, st>>>(table, lens, refs, S, M, P, R, src, dst, n, mv,
                                                    status);
   LG_LAUNCH_CHECK("pages_fork_plan");
-  const long long pieces = (long long)n * planes * H * (((long long)R * row_bytes + MV_PIECE - 1) / MV_PIECE);
-  const int grid = (int)std::min<long long>(8LL * device_sm_count(), pieces / (MV_THREADS / 32) + 1);
+  const long long pieces =
+      (long long)n * planes * H * (((long long)R * row_bytes + MV_PIECE - 1) / MV_PIECE);
+  const int grid =
+      (int)std::min<long long>(8LL * device_sm_count(), pieces / (MV_THREADS / 32) + 1);
   pages_fork_kernel<<<grid, MV_THREADS, 0, st>>>(static_cast<char*>(pool), planes, table, lens,
                                                  refs, M, P, H, R, row_bytes, src, dst, n, mv);
   LG_LAUNCH_CHECK("pages_fork");

@@ -50,8 +50,8 @@ class PagedCache:
 
     def fork(self, src, dst):
         """The empty streams ``dst`` become copies of the streams ``src``, sharing whole pages."""
-        return self._done(ops.pages_fork(self.pool, self.table, self.lens, self.refs, self._ids(src),
-                                         self._ids(dst)), "fork")
+        return self._done(ops.pages_fork(self.pool, self.table, self.lens, self.refs,
+                                         self._ids(src), self._ids(dst)), "fork")
 
     def free(self, ids):
         """The streams ``ids`` give their pages back."""
@@ -166,8 +166,8 @@ class Decoder:
         self.kv = self.pos + 1
         self.batch = _Batch(model, cache, self.table,
                             torch.arange(n, dtype=torch.int32, device=dev), self.pos,
-                            lambda Hq, Hkv, R, W: ops.stream_plan(self.kv, Hq, Hkv, R, prefix=prefix,
-                                                                  window=W))
+                            lambda Hq, Hkv, R, W: ops.stream_plan(self.kv, Hq, Hkv, R,
+                                                                  prefix=prefix, window=W))
 
     def step(self, tokens):
         """Logits [n, V] after one token of each stream (device int32 [n])."""
