@@ -41,6 +41,7 @@
 // with two score places each (541; a 64-wide product takes as long as a 128-wide one), a part of
 // the exponentials as a polynomial on the FMA pipes (1/8: 526, 1/3: 546), the two product warps
 // without turns (556), one arrival for all of a tile's weights (519).
+#include <algorithm>
 #include <atomic>
 
 #include "paged.cuh"
@@ -239,7 +240,7 @@ struct PaArgs {
   const __nv_bfloat16* gate;
   __nv_bfloat16* out;
   const int* table;
-  int P, R, M, Hq, Hkv;
+  int kind, B, T, P, R, M, Hq, Hkv;
   float scale_log2;  // scale * log2(e): exponentials are powers of two
   PaPlan plan;
 };
@@ -253,6 +254,13 @@ constexpr int PA_RING = 4;
 constexpr int PA_STAGE = 4096;  // output staging of a softmax warp: 32 rows of 128 bytes
 constexpr int PA_NBAD = 8;
 constexpr size_t PA_SMEM = (2 + PA_RING) * PA_TILE_BYTES + 8 * PA_STAGE + 512 + 2 * PA_ROWS * 8;
+
+// Whether the plan was made for this call's sizes. One that was not (or never made) would send reads
+// and writes anywhere.
+__device__ __forceinline__ bool pa_fits(const PaArgs& a, const PaHead& h) {
+  return h.kind == a.kind && h.B == a.B && h.T == a.T && h.Hq == a.Hq && h.Hkv == a.Hkv &&
+         h.R == a.R;
+}
 
 // The segments of a CTA's share, in order; every warp walks them by itself.
 struct PaWalk {
@@ -428,8 +436,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   const int G = a.Hq / a.Hkv, tq = PA_ROWS / G;
   pdl_trigger();  // the joining kernel waits for this one itself
   PaWalk walk(a.plan);
-  if (smem_u32(smem) & 1023) {
-    if (threadIdx.x == 0) *err = 9;
+  if (!pa_fits(a, *head) || (smem_u32(smem) & 1023)) {
+    if (threadIdx.x == 0) *err = 10;
     return;
   }
 
@@ -906,7 +914,7 @@ __global__ void __launch_bounds__(256) pa_join_prompt_kernel(const PaArgs a) {
   // so far the plan was read, now the parts; a CTA without work waits too, or this kernel, and with
   // it what follows, could come before the attention's end
   pdl_wait();
-  if (st.tile >= h.ntiles || st.t == 0 || c0 != c) return;
+  if (!pa_fits(a, h) || st.tile >= h.ntiles || st.t == 0 || c0 != c) return;
   if (row >= tq * G || i >= t.nq || w > (t.pair | t.duo)) return;
   const size_t slot = pa_slot_floats(PA_WIDE_ROWS);
   const long long at = (long long)(t.q0 + i) * a.Hq + head * G + row % G;
@@ -966,6 +974,7 @@ __global__ void __launch_bounds__(256) pa_join_stream_kernel(const PaArgs a) {
     first = head & ~pre.duo;
   }
   pdl_wait();  // as above
+  if (!pa_fits(a, h)) return;
   if (h.prefix == 0 && c0 == c1) return;  // written by the CTA that had it whole
   const int rows = pa_own_rows(a.Hq, a.Hkv), np = p1 - p0 + 1, n = np + c1 - c0 + 1;
   // the prefix's parts, one slot apart, and the own keys', one or two
@@ -1077,6 +1086,11 @@ static int attn_run(const char* who, int kind, const void* q, long long q_tok, l
   const PaPlan p = pa_layout(plan, kind, T, B, Hq, Hkv);
   if (!plan || !aligned(plan, 256) || bytes < p.bytes)
     return fail(LG_ERR_WORKSPACE, "%s: the plan buffer needs %zu bytes", who, p.bytes);
+  const char* q0 = static_cast<const char*>(q);
+  const char* q1 = q0 + 2 * ((T - 1) * std::max(q_tok, 0LL) + (Hq - 1) * std::max(q_head, 0LL) + D);
+  const char* o0 = static_cast<const char*>(out);
+  LG_CHECK_ARG(o0 >= q1 || q0 >= o0 + 2LL * T * Hq * D,
+               "%s: out shares memory with q, which is read until the end", who);
   // a dimension of one element has no stride to speak of
   if (T == 1) q_tok = D;
   if (Hq == 1) q_head = D;
@@ -1097,6 +1111,9 @@ static int attn_run(const char* who, int kind, const void* q, long long q_tok, l
   a.gate = static_cast<const __nv_bfloat16*>(gate);
   a.out = static_cast<__nv_bfloat16*>(out);
   a.table = table;
+  a.kind = kind;
+  a.B = B;
+  a.T = T;
   a.P = P;
   a.R = R;
   a.M = M;

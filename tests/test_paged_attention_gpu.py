@@ -331,3 +331,41 @@ def test_one_kv_head_and_one_key_tile(Hq, R):
             out, A = _exact(q, kp, v, table, new, new, 0.1, None, 0)
             _near(got[0], out, A, sum(new))
         assert not torch.isnan(got[0]).any()
+
+
+def test_a_plan_of_other_sizes_is_refused_on_the_device():
+    """Through the C interface, which cannot look into the plan: nothing is written, the plan's status
+    says so. (The Python surface refuses before.)"""
+    from lagunalab_b200 import _lib, ops
+    q, k, v, table, cu, kvt, _ = _case([20, 7], [90, 7], 4, 2, 32, seed=1)
+    out = torch.full_like(q, 7.0)
+    plan = ops.prompt_plan(cu, kvt, 27, 4, 2, 32)
+
+    def call(T, Hq, Hkv, R, B):
+        ks = k.stride()
+        _lib.call("lg_prompt_attention", q.data_ptr(), q.stride(0), q.stride(1), T, Hq, Hkv, D,
+                  k.data_ptr(), v.data_ptr(), k.shape[0], R, ks[0], ks[1], ks[2], table.data_ptr(),
+                  B, table.shape[1], 0.1, None, out.data_ptr(), plan.ptr, 1 << 40,
+                  torch.cuda.current_stream().cuda_stream)
+
+    for bad in ((26, 4, 2, 32, 2), (27, 2, 2, 32, 2), (27, 4, 1, 32, 2), (27, 4, 2, 16, 2),
+                (27, 4, 2, 32, 1)):
+        call(*bad)
+        assert (out == 7).all() and plan.status() == 10
+        plan.update()
+    call(27, 4, 2, 32, 2)
+    assert plan.status() == 0 and not (out == 7).any()
+    with pytest.raises(ValueError, match="plan is for"):
+        ops.stream_attention(q, k, v, table, plan, 0.1)
+    with pytest.raises(ValueError, match="plan is for"):
+        ops.prompt_attention(q[:26], k, v, table, plan, 0.1)
+    with pytest.raises(ValueError, match="rows"):
+        ops.prompt_attention(q, k, v, table[:1], plan, 0.1)
+    with pytest.raises(ValueError, match="shares memory"):
+        ops.prompt_attention(q, k, v, table, plan, 0.1, out=q)
+    with pytest.raises(ValueError, match="gate"):
+        ops.prompt_attention(q, k, v, table, plan, 0.1, gate=torch.ones(27, 4, device="cuda"))
+    with pytest.raises(ValueError, match="bf16"):
+        ops.prompt_attention(q.float(), k, v, table, plan, 0.1)
+    with pytest.raises(ValueError, match="strides"):
+        ops.prompt_attention(q, k, v.transpose(1, 2).contiguous().transpose(1, 2), table, plan, 0.1)

@@ -16,6 +16,7 @@ def _attn(kind="prompt", q=None, q_tok=1024, q_head=128, T=5, Hq=8, Hkv=2, D=128
           pg=2 * 64 * 128, hd=64 * 128, rw=128, table=None, B=2, M=4, scale=0.1, gate=None, out=None,
           plan=None, nb=1 << 40):
     f = lambda x: _fake() if x is None else x
+    out = _fake(1000) if out is None else out
     a = [f(q), q_tok, q_head, T, Hq, Hkv, D, f(k), _fake(), P, R, pg, hd, rw, f(table)]
     b = [M, scale, gate, f(out), f(plan), nb, None]
     if kind == "prompt":
@@ -32,7 +33,8 @@ def _attn(kind="prompt", q=None, q_tok=1024, q_head=128, T=5, Hq=8, Hkv=2, D=128
     (dict(table=ctypes.c_void_p(0)), "NULL"), (dict(out=ctypes.c_void_p(0)), "NULL"),
     (dict(q=ctypes.c_void_p(0x1008)), "multiples of 16"), (dict(q_tok=1025), "multiples of 16"),
     (dict(rw=132), "multiples of 16"), (dict(out=ctypes.c_void_p(0x1008)), "multiples of 16"),
-    (dict(T=-1), "tokens"), (dict(T=1 << 30), "tokens")])
+    (dict(T=-1), "tokens"), (dict(T=1 << 30), "tokens"), (dict(out=_fake()), "shares memory"),
+    (dict(q=_fake(3), out=_fake(2)), "shares memory")])
 def test_attention_refuses(kind, bad, match):
     with pytest.raises(ValueError, match=match):
         _attn(kind, **bad)
