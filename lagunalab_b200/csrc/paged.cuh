@@ -54,11 +54,12 @@ struct PaStart {
   PaTile rec;  // that tile's record, so that a CTA has it with the first load
 };
 
-struct PaHead {
+struct alignas(16) PaHead {
   long long total, chunk;
+  int kind, B, T, Hq;  // two 16-byte loads, see pa_fits
+  int Hkv, R, prefix, window;
   int ntiles;  // row tiles
-  int kind, B, T, Hq, Hkv, R, prefix, window;
-  int err;  // a wait that ran out (its code), else 0
+  int err;     // a wait that ran out (its code), else 0
 };
 
 // The parts of a plan buffer.

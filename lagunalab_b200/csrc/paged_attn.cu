@@ -255,11 +255,12 @@ constexpr int PA_STAGE = 4096;  // output staging of a softmax warp: 32 rows of 
 constexpr int PA_NBAD = 8;
 constexpr size_t PA_SMEM = (2 + PA_RING) * PA_TILE_BYTES + 8 * PA_STAGE + 512 + 2 * PA_ROWS * 8;
 
-// Whether the plan was made for this call's sizes. One that was not (or never made) would send reads
-// and writes anywhere.
-__device__ __forceinline__ bool pa_fits(const PaArgs& a, const PaHead& h) {
-  return h.kind == a.kind && h.B == a.B && h.T == a.T && h.Hq == a.Hq && h.Hkv == a.Hkv &&
-         h.R == a.R;
+// Whether the plan was made for this call's sizes. One that was not (or never made) would send
+// reads and writes anywhere.
+__device__ __forceinline__ bool pa_fits(const PaArgs& a, const PaHead* h) {
+  const int4 x = *reinterpret_cast<const int4*>(&h->kind);
+  const int2 y = *reinterpret_cast<const int2*>(&h->Hkv);
+  return x.x == a.kind && x.y == a.B && x.z == a.T && x.w == a.Hq && y.x == a.Hkv && y.y == a.R;
 }
 
 // The segments of a CTA's share, in order; every warp walks them by itself.
@@ -436,9 +437,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   const int G = a.Hq / a.Hkv, tq = PA_ROWS / G;
   pdl_trigger();  // the joining kernel waits for this one itself
   PaWalk walk(a.plan);
-  if (!pa_fits(a, *head) || (smem_u32(smem) & 1023)) {
+  if (!pa_fits(a, head) || (smem_u32(smem) & 1023)) {  // no work; the loads pass with the walk's
+    walk.end = walk.at;
     if (threadIdx.x == 0) *err = 10;
-    return;
   }
 
   if (threadIdx.x == 0) {
@@ -543,9 +544,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
     } else if (warp == 8 || warp == 11) {
       // ---- products of row tile (or half of the keys) w: lane 0 issues, the warp stays together
-      // so that all operands are uniform. The tensor cores hold only two or three products ahead,
-      // an issue waits for room and every wait costs 115 cycles or more, so each w has a warp of its
-      // own: one's waits pass under the other's products. Both see every tile of the ring go by (a
+      // so that all operands are uniform. The tensor cores hold two or three products ahead, past
+      // that an issue waits for room, and any wait costs 115 cycles or more: so each w has a warp of
+      // its own, one's waits pass under the other's products. Both see every tile of the ring go by (a
       // skipped phase of a barrier could not be told from the next); one that w does not use it
       // gives back at once, the others its softmax warps do. ----
       const int w = warp == 11;
@@ -903,6 +904,7 @@ constexpr int JP_ROWS = 32;
 __global__ void __launch_bounds__(256) pa_join_prompt_kernel(const PaArgs a) {
   const PaHead h = *a.plan.head;
   const int c = blockIdx.x;
+  const bool fits = pa_fits(a, a.plan.head);
   const PaStart st = a.plan.start[c + 1];
   const PaTile& t = st.rec;
   const int G = a.Hq / a.Hkv, tq = PA_ROWS / G;
@@ -914,7 +916,7 @@ __global__ void __launch_bounds__(256) pa_join_prompt_kernel(const PaArgs a) {
   // so far the plan was read, now the parts; a CTA without work waits too, or this kernel, and with
   // it what follows, could come before the attention's end
   pdl_wait();
-  if (!pa_fits(a, h) || st.tile >= h.ntiles || st.t == 0 || c0 != c) return;
+  if (!fits || st.tile >= h.ntiles || st.t == 0 || c0 != c) return;
   if (row >= tq * G || i >= t.nq || w > (t.pair | t.duo)) return;
   const size_t slot = pa_slot_floats(PA_WIDE_ROWS);
   const long long at = (long long)(t.q0 + i) * a.Hq + head * G + row % G;
@@ -962,6 +964,7 @@ __global__ void __launch_bounds__(256) pa_join_stream_kernel(const PaArgs a) {
   __shared__ float2 ml[JS_PARTS][16];
   __shared__ float inv[16];
   const PaHead h = *a.plan.head;
+  const bool fits = pa_fits(a, a.plan.head);
   const int b = blockIdx.x, head = blockIdx.y, G = a.Hq / a.Hkv, tq = PA_ROWS / G;
   const int pi = b / (2 * tq);
   const PaTile own = a.plan.tiles[a.plan.nprefix + b], pre = a.plan.tiles[pi];
@@ -974,7 +977,7 @@ __global__ void __launch_bounds__(256) pa_join_stream_kernel(const PaArgs a) {
     first = head & ~pre.duo;
   }
   pdl_wait();  // as above
-  if (!pa_fits(a, h)) return;
+  if (!fits) return;
   if (h.prefix == 0 && c0 == c1) return;  // written by the CTA that had it whole
   const int rows = pa_own_rows(a.Hq, a.Hkv), np = p1 - p0 + 1, n = np + c1 - c0 + 1;
   // the prefix's parts, one slot apart, and the own keys', one or two

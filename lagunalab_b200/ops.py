@@ -787,7 +787,8 @@ class AttentionPlan:
     """The division of a batch's paged attention over the GPU (``prompt_plan``, ``stream_plan``).
     It serves every layer with the same heads, page rows and window, and holds a call's partial
     results: calls that may overlap on the GPU (another stream, another captured graph) need a
-    plan each. ``update()`` divides anew for the lengths that its tensors hold by then."""
+    plan each. ``update()`` divides anew for the lengths that its tensors hold by then; a plan
+    whose lengths have moved on gives wrong rows. A captured graph's plan must outlive it."""
 
     def __init__(self, kind, cu_q, kv_len, T, Hq, Hkv, page_rows, prefix, window):
         self.device, self.index = _dev(kv_len), kv_len.get_device()
@@ -816,7 +817,8 @@ class AttentionPlan:
         return self
 
     def status(self):
-        """0, or the code of a wait that ran out in a call with this plan. Waits for the device."""
+        """0, or what went wrong in a call with this plan: the code of a wait that ran out, or 10
+        where the plan was made for other sizes. Waits for the device."""
         st = ctypes.c_int(0)
         torch.cuda.synchronize(self.index)
         with torch.cuda.device(self.index):
@@ -835,7 +837,8 @@ def stream_plan(kv_len, Hq, Hkv, page_rows, prefix=0, window=0):
     """A plan for ``stream_attention``: one token of each of B streams, the newest of its
     kv_len[b] rows (device int32 [B]). Rows [0, prefix) are the same for every stream that has
     them and are read once for all."""
-    return AttentionPlan("stream", None, kv_len, kv_len.shape[0], Hq, Hkv, page_rows, prefix, window)
+    return AttentionPlan("stream", None, kv_len, kv_len.shape[0], Hq, Hkv, page_rows, prefix,
+                         window)
 
 
 def _paged_attention(kind, q, k_pages, v_pages, table, plan, scale, gate, out):
