@@ -11,7 +11,12 @@
 // call's list, so the result does not depend on timing.
 //
 // Bounds: the moves read and write each row once, 16 bytes a lane, so they run at the copy rate of
-// HBM; the one-CTA kernels are latency (a scan of refs and of the call's list).
+// HBM (118 pages of 80 planes moved: 192 us, 6.4 TB/s); the one-CTA kernels are latency (a scan of
+// refs and of the call's list), and the moving kernel's launch passes under them.
+//
+// A fork's copies are written plane by plane in the order of their pages. Reading a page once for
+// all its copies instead left the reads 26 MB of 228, but the writes jumped between pages: 62 us
+// against 49 for 64 children of 80 planes (202 MB written, 40 us in the moving kernel).
 #include <algorithm>
 
 #include "common.cuh"
@@ -53,12 +58,13 @@ __device__ bool list_ok(const int* ids, int n, int S, unsigned* bm, int* bad) {
 }
 
 // The first `need` free pages in ascending order into out[]; returns how many there are (at most
-// need, or the free count when less). The whole CTA calls it; need is CTA-uniform.
-__device__ int take_free(const int* refs, int P, int need, int* out, int* wt, int* tot) {
+// need, or the free count when less). The whole CTA calls it; need is CTA-uniform; ref0 is page
+// threadIdx.x's count, which the caller fetched early.
+__device__ int take_free(const int* refs, int P, int need, int ref0, int* out, int* wt, int* tot) {
   int have = 0;
   for (int p0 = 0; p0 < P && have < need; p0 += blockDim.x) {
     const int p = p0 + threadIdx.x;
-    const int v = p < P && refs[p] == 0;
+    const int v = p < P && (p0 == 0 ? ref0 : refs[p]) == 0;
     const int r = have + block_excl_scan(v, wt, tot);
     if (v && r < need) out[r] = p;
     have += *tot;
@@ -75,6 +81,7 @@ __global__ void __launch_bounds__(PG_THREADS)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int* first = list + P;  // [n + 1]: where each stream's new pages start in the list
   int* have = first + n + 1;
+  const int ref0 = threadIdx.x < P ? refs[threadIdx.x] : 1;
   const bool ok = list_ok(ids, n, S, bm, &bad);
   if (threadIdx.x == 0) code = ok ? PG_OK : PG_BAD_STREAM;
   __syncthreads();
@@ -108,7 +115,7 @@ __global__ void __launch_bounds__(PG_THREADS)
   }
   if (threadIdx.x == 0) first[n] = total;
   if (code == PG_OK && total > 0) {  // code is CTA-uniform here: written before a barrier
-    const int got = total <= P ? take_free(refs, P, total, list, wt, &tot) : 0;
+    const int got = total <= P ? take_free(refs, P, total, ref0, list, wt, &tot) : 0;
     if (got < total && threadIdx.x == 0) code = PG_NO_PAGES;
   }
   __syncthreads();
@@ -158,6 +165,23 @@ __global__ void __launch_bounds__(PG_THREADS)
                            const int* src, const int* dst, int n, Moves mv, int* status) {
   __shared__ unsigned bm[PG_MAX_STREAMS / 32];
   __shared__ int bad, wt[32], tot, code;
+  pdl_trigger();  // the moving kernel waits for this one itself
+  // What the first children's checks and the search for free pages read is fetched before the
+  // list's check: this kernel's time is that of its loads one after the other.
+  struct Child {
+    int s, d, len, held, page0;
+  };
+  auto child = [&](int i) {
+    Child c = {-1, -1, -1, -1, -1};
+    if (i < n) {
+      c.s = src[i], c.d = dst[i];
+      if (c.s >= 0 && c.s < S) c.len = lens[c.s];
+      if (c.d >= 0 && c.d < S) c.held = lens[c.d], c.page0 = table[(size_t)c.d * M];
+    }
+    return c;
+  };
+  const Child c0 = child(threadIdx.x);
+  const int ref0 = threadIdx.x < P ? refs[threadIdx.x] : 1;
   const bool ok = list_ok(dst, n, S, bm, &bad);
   if (threadIdx.x == 0) code = ok ? PG_OK : PG_BAD_STREAM;
   __syncthreads();
@@ -165,17 +189,17 @@ __global__ void __launch_bounds__(PG_THREADS)
   if (ok) {
     for (int i0 = 0; i0 < n; i0 += blockDim.x) {
       const int i = i0 + threadIdx.x;
+      const Child c = i0 == 0 ? c0 : child(i);
       int part = 0, page = -1;
       if (i < n) {
-        const int s = src[i], d = dst[i];
         // a source that is also a child, or a child that still holds pages
-        if (s < 0 || s >= S || (bm[s >> 5] >> (s & 31) & 1) || lens[d] != 0 ||
-            table[(size_t)d * M] >= 0) {
+        if (c.s < 0 || c.s >= S || (bm[c.s >> 5] >> (c.s & 31) & 1) || c.held != 0 ||
+            c.page0 >= 0) {
           code = PG_BAD_STREAM;
-        } else if (lens[s] < 0 || lens[s] > (long long)M * R) {
+        } else if (c.len < 0 || c.len > (long long)M * R) {
           code = PG_TABLE_FULL;
-        } else if ((part = lens[s] % R) > 0) {
-          page = table[(size_t)s * M + lens[s] / R];
+        } else if ((part = c.len % R) > 0) {
+          page = table[(size_t)c.s * M + c.len / R];
           if (page < 0 || page >= P) code = PG_BAD_PAGE;
         }
       }
@@ -189,7 +213,7 @@ __global__ void __launch_bounds__(PG_THREADS)
       __syncthreads();
     }
     if (code == PG_OK && total > 0) {
-      const int got = total <= P ? take_free(refs, P, total, mv.to, wt, &tot) : 0;
+      const int got = total <= P ? take_free(refs, P, total, ref0, mv.to, wt, &tot) : 0;
       if (got < total && threadIdx.x == 0) code = PG_NO_PAGES;
     }
     __syncthreads();
@@ -208,6 +232,7 @@ __global__ void __launch_bounds__(PG_THREADS)
 __global__ void __launch_bounds__(PG_THREADS)
     pages_compact_plan_kernel(int* refs, int P, int R, int* name, Moves mv, int* status) {
   __shared__ int wt[32], tot, bad;
+  pdl_trigger();
   int live = 0;
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
@@ -252,7 +277,10 @@ __global__ void __launch_bounds__(PG_THREADS)
 }
 
 // One warp's piece of the moves: up to 4 KiB of one head's rows of one page of one plane.
-constexpr int MV_PIECE = 4096, MV_THREADS = 256;
+// CTAs per SM: a fork's pieces are half empty and go round a small grid (8: 49 us for 64 children of
+// 80 planes; 32: 51, 4: 58). A compaction's are whole, and a larger grid's CTAs follow each other in
+// the order of addresses (8: 199 us for 118 pages, 32: 192; with nothing to move 6 and 8 us).
+constexpr int MV_PIECE = 4096, MV_THREADS = 256, MV_FORK_CTAS = 8, MV_COMPACT_CTAS = 32;
 
 __device__ __forceinline__ void move_rows(char* pool, const Moves& mv, int count, int planes, int P,
                                           int H, int R, int row_bytes) {
@@ -280,7 +308,8 @@ __device__ __forceinline__ void move_rows(char* pool, const Moves& mv, int count
 #pragma unroll
     for (int i = 0; i < MV_PIECE / 512; ++i) {
       const int at = piece * MV_PIECE + i * 512 + lane * 16;
-      if (at < end) *reinterpret_cast<uint4*>(d + at) = v[i];
+      if (at < end)  // a copy is not read soon: 3 us less on a fork of 202 MB than plain stores
+        __stcs(reinterpret_cast<uint4*>(d + at), v[i]);
     }
   }
 }
@@ -290,10 +319,11 @@ __device__ __forceinline__ void move_rows(char* pool, const Moves& mv, int count
 __global__ void __launch_bounds__(MV_THREADS)
     pages_fork_kernel(char* pool, int planes, int* table, int* lens, int* refs, int M, int P, int H,
                       int R, int row_bytes, const int* src, const int* dst, int n, Moves mv) {
+  pdl_wait();
   const int count = *mv.count;
   if (count < 0) return;  // the check failed
   const long long all = (long long)n * M;
-  for (long long e = blockIdx.x * (long long)blockDim.x + threadIdx.x; e < all;
+  for (long long e = (gridDim.x - 1 - blockIdx.x) * (long long)blockDim.x + threadIdx.x; e < all;
        e += (long long)gridDim.x * blockDim.x) {
     const int i = (int)(e / M), m = (int)(e % M), len = lens[src[i]];
     int p = -1;
@@ -312,6 +342,7 @@ __global__ void __launch_bounds__(MV_THREADS)
 __global__ void __launch_bounds__(MV_THREADS)
     pages_compact_kernel(char* pool, int planes, int* table, long long entries, int P, int H, int R,
                          int row_bytes, const int* name, Moves mv) {
+  pdl_wait();
   const int count = *mv.count;
   if (count <= 0) return;
   for (long long e = blockIdx.x * (long long)blockDim.x + threadIdx.x; e < entries;
@@ -320,6 +351,23 @@ __global__ void __launch_bounds__(MV_THREADS)
     if (p >= 0 && p < P && name[p] != p) table[e] = name[p];
   }
   move_rows(pool, mv, count, planes, P, H, R, row_bytes);
+}
+
+// A kernel that starts while the one before it (which triggers it and was itself launched plainly)
+// still runs; it waits for that one's end on the GPU.
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_early(void (*kernel)(KArgs...), int grid, int block, cudaStream_t st,
+                                Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
 static int pages_check(const char* who, const void* table, const void* refs, int S, int M, int P) {
@@ -393,9 +441,10 @@ extern "C" int lg_pages_fork(void* pool, int planes, int H, int R, int row_bytes
   const long long pieces =
       (long long)n * planes * H * (((long long)R * row_bytes + MV_PIECE - 1) / MV_PIECE);
   const int grid =
-      (int)std::min<long long>(8LL * device_sm_count(), pieces / (MV_THREADS / 32) + 1);
-  pages_fork_kernel<<<grid, MV_THREADS, 0, st>>>(static_cast<char*>(pool), planes, table, lens,
-                                                 refs, M, P, H, R, row_bytes, src, dst, n, mv);
+      (int)std::min<long long>((long long)MV_FORK_CTAS * device_sm_count(),
+                               pieces / (MV_THREADS / 32) + 1);
+  LG_CUDA_TRY(launch_early(pages_fork_kernel, grid, MV_THREADS, st, static_cast<char*>(pool),
+                           planes, table, lens, refs, M, P, H, R, row_bytes, src, dst, n, mv));
   LG_LAUNCH_CHECK("pages_fork");
   return LG_OK;
 }
@@ -413,9 +462,13 @@ extern "C" int lg_pages_compact(void* pool, int planes, int H, int R, int row_by
   int* name = mv.of;  // [P]
   pages_compact_plan_kernel<<<1, PG_THREADS, 0, st>>>(refs, P, R, name, mv, status);
   LG_LAUNCH_CHECK("pages_compact_plan");
-  const int grid = 8 * device_sm_count();
-  pages_compact_kernel<<<grid, MV_THREADS, 0, st>>>(static_cast<char*>(pool), planes, table,
-                                                    (long long)S * M, P, H, R, row_bytes, name, mv);
+  // at most half of the pages move
+  const long long pieces =
+      (long long)(P / 2) * planes * H * (((long long)R * row_bytes + MV_PIECE - 1) / MV_PIECE);
+  const int grid = (int)std::min<long long>((long long)MV_COMPACT_CTAS * device_sm_count(),
+                                            pieces / (MV_THREADS / 32) + 1);
+  LG_CUDA_TRY(launch_early(pages_compact_kernel, grid, MV_THREADS, st, static_cast<char*>(pool),
+                           planes, table, (long long)S * M, P, H, R, row_bytes, name, mv));
   LG_LAUNCH_CHECK("pages_compact");
   return LG_OK;
 }
