@@ -369,3 +369,26 @@ def test_a_plan_of_other_sizes_is_refused_on_the_device():
         ops.prompt_attention(q.float(), k, v, table, plan, 0.1)
     with pytest.raises(ValueError, match="strides"):
         ops.prompt_attention(q, k, v.transpose(1, 2).contiguous().transpose(1, 2), table, plan, 0.1)
+
+
+def test_offsets_past_32_bits():
+    """Pages, tokens and output rows whose element offsets pass 2^31."""
+    from lagunalab_b200 import ops
+    P, Hq, Hkv, R, n, B = 17000, 32, 8, 128, 128, 4375
+    kv = torch.full((2, P, Hkv, R, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for p in (0, P - 2, P - 1):
+        kv[:, p] = torch.randn(2, Hkv, R, D, generator=g, device="cuda").to(torch.bfloat16)
+    assert kv[0].numel() > 2 ** 31 and n * B * Hq * D > 2 ** 31
+    q = torch.randn(n * B, Hq, D, generator=g, device="cuda", dtype=torch.bfloat16)
+    rows = torch.tensor([[0, P - 1], [P - 1, P - 2]], dtype=torch.int32, device="cuda")
+    table = rows.repeat(B // 2 + 1, 1)[:B].contiguous()
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda") * n
+    lens = torch.full((B,), 200, dtype=torch.int32, device="cuda")
+    plan = ops.prompt_plan(cu, lens, n * B, Hq, Hkv, R)
+    got = ops.prompt_attention(q, kv[0], kv[1], table, plan, D ** -0.5)
+    assert plan.status() == 0
+    for b in (0, 1, B - 2, B - 1):
+        at = slice(b * n, (b + 1) * n)
+        out, A = _exact(q[at], kv[0], kv[1], table[b:b + 1], [n], [200], D ** -0.5, None, 0)
+        _near(got[at], out, A, n)

@@ -179,3 +179,71 @@ def test_empty_lists_and_empty_streams():
     assert ops.pages_fork(pool, d.table, d.lens, d.refs, _t([0]), _t([1])).tolist() == [0, 0]
     assert ops.pages_free(d.table, d.lens, d.refs, _t([0, 1, 2])).tolist() == [0, 3]
     assert d.table.tolist() == [[-1] * M] * S and d.refs.tolist() == [0] * P
+
+
+def test_lists_longer_than_a_cta():
+    """More streams in one call than a CTA has threads, free pages far into the pool, and the same
+    operations captured into a graph and replayed."""
+    from lagunalab_b200 import ops
+    rng = random.Random(5)
+    S, M, P, R, n = 3600, 2, 9000, 16, 1500
+    pool = torch.randint(0, 1 << 15, (1, P, 1, R, 4), dtype=torch.int32, device="cuda")
+    ref = pool.clone()
+    h, d = Host(S, M, P, R), Device(S, M, P)
+    order = rng.sample(range(S), 2 * n)
+    src, dst = order[:n], order[n:]
+    rows = [rng.randint(0, M * R) for _ in src]
+    need = sum(-(-r // R) for r in rows)
+    assert ops.pages_reserve(d.table, d.refs, _t(src), _t(rows), R).tolist() == [0, need]
+    h.reserve(src, rows)
+    for s, r in zip(src, rows):
+        h.lens[s] = r
+    d.lens[torch.tensor(src, device="cuda")] = _t(rows)
+    _same(h, d)
+    parents = [rng.choice(src) for _ in dst]
+    ids = [_t(parents), _t(dst), _t(src[::2])]
+    kept = [t.clone() for t in (pool, d.table, d.lens, d.refs)]
+
+    def life():
+        return (ops.pages_fork(pool, d.table, d.lens, d.refs, ids[0], ids[1]),
+                ops.pages_free(d.table, d.lens, d.refs, ids[2]),
+                ops.pages_compact(pool, d.table, d.refs))
+
+    first = [st.tolist() for st in life()]
+    h.fork(ref, parents, dst)
+    h.free(src[::2])
+    live = sum(r > 0 for r in h.refs)
+    assert first == [[0, sum(h.lens[s] % R > 0 for s in dst)], [0, len(src[::2])],
+                     [0, sum(r > 0 for r in h.refs[live:])]]
+    h.compact(ref)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = life()
+    for replays in range(3):
+        _same(h, d)
+        assert torch.equal(pool, ref)
+        for t, k in zip((pool, d.table, d.lens, d.refs), kept):
+            t.copy_(k)
+        graph.replay()
+        assert [st.tolist() for st in again] == first
+
+
+def test_a_pool_past_32_bit_offsets():
+    """Planes more than 2^32 bytes apart: a fork and a compaction move the last plane's rows."""
+    from lagunalab_b200 import ops
+    planes, P, R = 3, 9000, 128
+    pool = torch.zeros(planes, P, 1, R, 1024, dtype=torch.bfloat16, device="cuda")
+    d = Device(2, 2, P)
+    d.refs[:] = 1
+    d.refs[7], d.refs[11] = 0, 0
+    d.table[0, 0] = P - 1
+    d.lens[0] = 100
+    pool[:, P - 1, 0] = torch.randn(planes, R, 1024, device="cuda").to(torch.bfloat16)
+    want = pool[:, P - 1, 0].clone()
+    assert ops.pages_fork(pool, d.table, d.lens, d.refs, _t([0]), _t([1])).tolist() == [0, 1]
+    assert d.table[1].tolist() == [7, -1] and d.lens[1].item() == 100
+    assert torch.equal(pool[:, 7, 0, :100], want[:, :100])
+    assert not pool[:, 7, 0, 100:].any()
+    assert ops.pages_compact(pool, d.table, d.refs).tolist() == [0, 1]
+    assert d.table[0].tolist() == [11, -1]
+    assert torch.equal(pool[:, 11, 0], want)
