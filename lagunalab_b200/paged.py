@@ -148,8 +148,11 @@ class Decoder:
     """Decode steps of ``streams`` (distinct rows of the cache), one token of each a step. Rows
     [0, prefix) must be the same for all of them (a fork's, or the same tokens' rows); they are read
     once a step. ``reserve`` the rows to come before: a step writes row ``cache.lens`` of each
-    stream and takes no page. ``step`` changes only device memory that the object and the cache
-    hold, so it can be captured in a CUDA graph after a first call."""
+    stream and takes no page. A stream without a page for that row (freed, or past its reserved
+    rows) sits the step out: its length stays, its logits are NaN, ``wrote`` (device bool [n], of
+    the last step) says so; after a ``reserve`` it goes on where it was. ``step`` changes only device
+    memory that the object and the cache hold, so it can be captured in a CUDA graph after a first
+    call."""
 
     def __init__(self, model, cache, streams, prefix=0):
         if len(set(int(s) for s in streams)) != len(streams):
@@ -164,6 +167,7 @@ class Decoder:
         if prefix and int(self.pos.min()) < prefix:
             raise ValueError(f"a stream holds {int(self.pos.min())} rows of the {prefix} shared")
         self.kv = self.pos + 1
+        self.wrote = torch.zeros(n, dtype=torch.bool, device=dev)
         self.batch = _Batch(model, cache, self.table,
                             torch.arange(n, dtype=torch.int32, device=dev), self.pos,
                             lambda Hq, Hkv, R, W: ops.stream_plan(self.kv, Hq, Hkv, R,
@@ -171,14 +175,20 @@ class Decoder:
 
     def step(self, tokens):
         """Logits [n, V] after one token of each stream (device int32 [n])."""
+        R, M = self.cache.page_rows, self.table.shape[1]
         self.pos.copy_(self.cache.lens[self.ids])
-        torch.add(self.pos, 1, out=self.kv)
         self.table.copy_(self.cache.table[self.ids])
+        # A row that no page takes is not written, so the length must not count it: a later reserve
+        # would put a page there with another stream's rows. Such a stream sees no key (kv 0).
+        col = (self.pos // R).long()
+        page = self.table.gather(1, col.clamp(max=M - 1)[:, None])[:, 0]
+        torch.logical_and(page >= 0, col < M, out=self.wrote)
+        torch.mul(self.pos + 1, self.wrote, out=self.kv)
         for plan in self.batch._plans.values():
             plan.update()
         h = _forward(self.model, tokens, self.batch)
-        self.cache.lens[self.ids] = self.kv
-        return self.model.lm_head(h)
+        self.cache.lens[self.ids] = self.pos + self.wrote
+        return self.model.lm_head(h).masked_fill(~self.wrote[:, None], float("nan"))
 
 
 def generate(model, prompts, max_tokens, page_rows=64):
