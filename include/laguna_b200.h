@@ -560,7 +560,7 @@ enum {
   LG_PAGES_BAD_STREAM = 2, /* a stream outside [0, S), listed twice, or a fork's child that holds
                               pages or is a source too */
   LG_PAGES_TABLE_FULL = 3, /* more rows than a table row's M pages hold */
-  LG_PAGES_BAD_PAGE = 4    /* a page id outside [0, P) or a negative count */
+  LG_PAGES_BAD_PAGE = 4    /* a page id outside [0, P) below a source's length, or a negative count */
 };
 
 size_t lg_pages_workspace_bytes(int P, int n);

@@ -165,16 +165,18 @@ __global__ void __launch_bounds__(PG_THREADS)
                            const int* src, const int* dst, int n, Moves mv, int* status) {
   __shared__ unsigned bm[PG_MAX_STREAMS / 32];
   __shared__ int bad, wt[32], tot, code;
+  // this turn's sources whose pages are looked at, their whole and part-filled pages, and the most
+  __shared__ int look[PG_THREADS], pages[PG_THREADS], nlook, most;
   pdl_trigger();  // the moving kernel waits for this one itself
   // What the first children's checks and the search for free pages read is fetched before the
   // list's check: this kernel's time is that of its loads one after the other.
   struct Child {
-    int s, d, len, held, page0;
+    int s, d, before, len, held, page0;
   };
   auto child = [&](int i) {
-    Child c = {-1, -1, -1, -1, -1};
+    Child c = {-1, -1, -1, -1, -1, -1};
     if (i < n) {
-      c.s = src[i], c.d = dst[i];
+      c.s = src[i], c.d = dst[i], c.before = i ? src[i - 1] : -1;
       if (c.s >= 0 && c.s < S) c.len = lens[c.s];
       if (c.d >= 0 && c.d < S) c.held = lens[c.d], c.page0 = table[(size_t)c.d * M];
     }
@@ -183,7 +185,7 @@ __global__ void __launch_bounds__(PG_THREADS)
   const Child c0 = child(threadIdx.x);
   const int ref0 = threadIdx.x < P ? refs[threadIdx.x] : 1;
   const bool ok = list_ok(dst, n, S, bm, &bad);
-  if (threadIdx.x == 0) code = ok ? PG_OK : PG_BAD_STREAM;
+  if (threadIdx.x == 0) code = ok ? PG_OK : PG_BAD_STREAM, nlook = most = 0;
   __syncthreads();
   int total = 0;
   if (ok) {
@@ -198,9 +200,14 @@ __global__ void __launch_bounds__(PG_THREADS)
           code = PG_BAD_STREAM;
         } else if (c.len < 0 || c.len > (long long)M * R) {
           code = PG_TABLE_FULL;
-        } else if ((part = c.len % R) > 0) {
-          page = table[(size_t)c.s * M + c.len / R];
-          if (page < 0 || page >= P) code = PG_BAD_PAGE;
+        } else {
+          if ((part = c.len % R) > 0) page = table[(size_t)c.s * M + c.len / R];
+          if (c.len > 0 && c.s != c.before) {  // children of one source in a row: once
+            const int k = atomicAdd(&nlook, 1), np = c.len / R + (part > 0);
+            look[k] = c.s;
+            pages[k] = np;
+            atomicMax(&most, np);
+          }
         }
       }
       const int at = total + block_excl_scan(part > 0, wt, &tot);
@@ -210,6 +217,18 @@ __global__ void __launch_bounds__(PG_THREADS)
         mv.rows[at] = part;
       }
       total += tot;
+      // every page below a source's length is there, 2^bits threads a source
+      const int bits = most > 1 ? 32 - __clz(most - 1) : 0;
+      const long long all = (long long)nlook << bits;
+      bool gone = false;
+#pragma unroll 4
+      for (long long t = threadIdx.x; t < all; t += PG_THREADS) {
+        const int k = (int)(t >> bits), m = (int)(t & ((1ll << bits) - 1));
+        if (m < pages[k]) gone |= (unsigned)table[(size_t)look[k] * M + m] >= (unsigned)P;
+      }
+      if (gone) code = PG_BAD_PAGE;
+      __syncthreads();
+      if (threadIdx.x == 0) nlook = most = 0;
       __syncthreads();
     }
     if (code == PG_OK && total > 0) {

@@ -59,3 +59,60 @@ def test_a_stream_without_a_page_sits_the_step_out(prefix):
     for i in range(11, 30):
         dec.step(_step_tokens(3, i))
     assert cache.lens.tolist()[2] == 96 and dec.wrote.tolist()[2] is False
+
+
+class _Pool:
+    """Streams of a small pool, and whether a refused operation left all of it alone."""
+
+    def __init__(self, S, M, P, R, rows):
+        from lagunalab_b200 import ops
+        i = dict(dtype=torch.int32, device="cuda")
+        self.pool = torch.randn(2, P, 1, R, 128, device="cuda").to(torch.bfloat16)
+        self.table = torch.full((S, M), -1, **i)
+        self.lens, self.refs = torch.zeros(S, **i), torch.zeros(P, **i)
+        ids = _t(list(range(len(rows))))
+        assert ops.pages_reserve(self.table, self.refs, ids, _t(rows), R).tolist()[0] == 0
+        self.lens[:len(rows)] = _t(rows)
+
+    def state(self):
+        return [t.clone() for t in (self.pool, self.table, self.lens, self.refs)]
+
+    def fork(self, src, dst):
+        from lagunalab_b200 import ops
+        return ops.pages_fork(self.pool, self.table, self.lens, self.refs, _t(src),
+                              _t(dst)).tolist()
+
+    def refused(self, src, dst, code):
+        before = self.state()
+        assert self.fork(src, dst) == [code, 0]
+        assert all(torch.equal(a, b) for a, b in zip(before, self.state()))
+
+
+@pytest.mark.parametrize("page", [-1, 40, 1 << 30])
+@pytest.mark.parametrize("col", [0, 2, 5, 6])  # whole pages, the last whole one, the part-filled one
+def test_a_fork_of_rows_without_a_page_is_refused(page, col):
+    p = _Pool(8, 9, 40, 16, [33, 6 * 16 + 5, 16])
+    good = p.table[1, col].item()
+    p.table[1, col] = page
+    p.refused([1], [3], 4)
+    p.refused([0, 2, 1, 1, 0], [3, 4, 5, 6, 7], 4)
+    p.table[1, col] = good
+    assert p.fork([0, 2, 1, 1, 0], [3, 4, 5, 6, 7]) == [0, 4]
+    assert p.table[5, :6].tolist() == p.table[1, :6].tolist()
+
+
+def test_a_fork_looks_at_every_source_of_a_long_list():
+    """More children than a CTA has threads and sources of very different lengths; the one whole
+    page that is missing is the last, the longest, an early or a middle source's."""
+    S, M, R, n = 4000, 40, 16, 1500
+    rows = [(7 * i) % 48 + 1 for i in range(n)]
+    rows[700] = 39 * R + 3
+    p = _Pool(S, M, 8000, R, rows)
+    src, dst = list(range(n)), list(range(n, 2 * n))
+    for s in (n - 1, 700, 4, 1100):
+        last = rows[s] // R - 1
+        good = p.table[s, last].item()
+        p.table[s, last] = -1
+        p.refused(src, dst, 4)
+        p.table[s, last] = good
+    assert p.fork(src, dst) == [0, sum(r % R > 0 for r in rows)]
