@@ -551,7 +551,8 @@ int lg_ep_status(const void* arena, int reset, int* status);
  *
  * Each operation checks its lists on the device; one whose check fails changes nothing.
  * status int32 [2]: {LG_PAGES_*, count} with the count of pages taken (reserve, fork), streams
- * freed, or pages moved. Pages are taken lowest id first in the order of the call's list.
+ * freed, or pages moved; of several faults the lowest code, LG_PAGES_NONE_FREE only where there is
+ * no other. Pages are taken lowest id first in the order of the call's list.
  * Workspace: lg_pages_workspace_bytes(P, n) for a list of n (compact: n = 0).
  * ------------------------------------------------------------------------------------- */
 enum {

@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(PG_THREADS)
     pages_fork_plan_kernel(const int* table, const int* lens, int* refs, int S, int M, int P, int R,
                            const int* src, const int* dst, int n, Moves mv, int* status) {
   __shared__ unsigned bm[PG_MAX_STREAMS / 32];
-  __shared__ int bad, wt[32], tot, code;
+  __shared__ int bad, wt[32], tot;
+  __shared__ int faults;  // a bit a code; the lowest is told, whichever thread saw its own first
   // this turn's sources whose pages are looked at, their whole and part-filled pages, and the most
   __shared__ int look[PG_THREADS], pages[PG_THREADS], nlook, most;
   pdl_trigger();  // the moving kernel waits for this one itself
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(PG_THREADS)
   const Child c0 = child(threadIdx.x);
   const int ref0 = threadIdx.x < P ? refs[threadIdx.x] : 1;
   const bool ok = list_ok(dst, n, S, bm, &bad);
-  if (threadIdx.x == 0) code = ok ? PG_OK : PG_BAD_STREAM, nlook = most = 0;
+  if (threadIdx.x == 0) faults = ok ? 0 : 1 << PG_BAD_STREAM, nlook = most = 0;
   __syncthreads();
   int total = 0;
   if (ok) {
@@ -197,9 +198,9 @@ __global__ void __launch_bounds__(PG_THREADS)
         // a source that is also a child, or a child that still holds pages
         if (c.s < 0 || c.s >= S || (bm[c.s >> 5] >> (c.s & 31) & 1) || c.held != 0 ||
             c.page0 >= 0) {
-          code = PG_BAD_STREAM;
+          atomicOr(&faults, 1 << PG_BAD_STREAM);
         } else if (c.len < 0 || c.len > (long long)M * R) {
-          code = PG_TABLE_FULL;
+          atomicOr(&faults, 1 << PG_TABLE_FULL);
         } else {
           if ((part = c.len % R) > 0) page = table[(size_t)c.s * M + c.len / R];
           if (c.len > 0 && c.s != c.before) {  // children of one source in a row: once
@@ -226,23 +227,23 @@ __global__ void __launch_bounds__(PG_THREADS)
         const int k = (int)(t >> bits), m = (int)(t & ((1ll << bits) - 1));
         if (m < pages[k]) gone |= (unsigned)table[(size_t)look[k] * M + m] >= (unsigned)P;
       }
-      if (gone) code = PG_BAD_PAGE;
+      if (gone) atomicOr(&faults, 1 << PG_BAD_PAGE);
       __syncthreads();
       if (threadIdx.x == 0) nlook = most = 0;
       __syncthreads();
     }
-    if (code == PG_OK && total > 0) {
+    if (!faults && total > 0) {
       const int got = total <= P ? take_free(refs, P, total, ref0, mv.to, wt, &tot) : 0;
-      if (got < total && threadIdx.x == 0) code = PG_NO_PAGES;
+      if (got < total && threadIdx.x == 0) faults = 1 << PG_NO_PAGES;
     }
     __syncthreads();
   }
-  if (code == PG_OK)
+  if (!faults)
     for (int k = threadIdx.x; k < total; k += blockDim.x) refs[mv.to[k]] = 1;
   if (threadIdx.x == 0) {
-    *mv.count = code == PG_OK ? total : -1;
-    status[0] = code;
-    status[1] = code == PG_OK ? total : 0;
+    *mv.count = faults ? -1 : total;
+    status[0] = faults ? __ffs(faults) - 1 : PG_OK;
+    status[1] = faults ? 0 : total;
   }
 }
 

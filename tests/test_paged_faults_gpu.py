@@ -116,3 +116,25 @@ def test_a_fork_looks_at_every_source_of_a_long_list():
         p.refused(src, dst, 4)
         p.table[s, last] = good
     assert p.fork(src, dst) == [0, sum(r % R > 0 for r in rows)]
+
+
+def test_of_several_faults_the_lowest_code_is_told():
+    """Whatever their places in the list: a stream out of range (2) or that holds pages (2), a length
+    past the table (3), a page that is missing (4)."""
+    S, M, R, n = 2400, 4, 16, 1200
+    p = _Pool(S, M, 2000, R, [20] * 900)
+    p.lens[5], p.table[7, 0] = M * R + 1, -1
+    for i in (0, 40, 800, 1199):
+        for j in (1, 30, 900, 1198):
+            src, dst = [9] * n, list(range(1000, 1000 + n))
+            src[i], src[j] = 7, 5
+            p.refused(src, dst, 3)
+            src[j] = 9
+            p.refused(src, dst, 4)
+            dst[j] = 8
+            p.refused(src, dst, 2)
+            dst[j], src[j] = 1000 + j, -1
+            p.refused(src, dst, 2)
+    # nothing is free either: 900 streams hold 1,800 pages, 200 are left for 1,200 children
+    p.lens[5], p.table[7, 0] = 20, 1999
+    p.refused([9] * n, list(range(1000, 1000 + n)), 1)
