@@ -78,12 +78,13 @@ __global__ void __launch_bounds__(PG_THREADS)
                          const int* rows, int n, int* list, int* status) {
   __shared__ unsigned bm[PG_MAX_STREAMS / 32];
   __shared__ int bad, wt[32], tot, code;
+  __shared__ unsigned long long asked;  // pages in all: the sums in 32 bits hold only up to P
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int* first = list + P;  // [n + 1]: where each stream's new pages start in the list
   int* have = first + n + 1;
   const int ref0 = threadIdx.x < P ? refs[threadIdx.x] : 1;
   const bool ok = list_ok(ids, n, S, bm, &bad);
-  if (threadIdx.x == 0) code = ok ? PG_OK : PG_BAD_STREAM;
+  if (threadIdx.x == 0) code = ok ? PG_OK : PG_BAD_STREAM, asked = 0;
   __syncthreads();
   if (!ok) {
     if (threadIdx.x == 0) status[0] = PG_BAD_STREAM, status[1] = 0;
@@ -106,17 +107,22 @@ __global__ void __launch_bounds__(PG_THREADS)
     int need = 0;
     if (i < n) {
       if (rows[i] < 0 || rows[i] > (long long)M * R) code = PG_TABLE_FULL;
-      else need = max(0, (rows[i] + R - 1) / R - have[i]);
+      else need = max(0, rows[i] / R + (rows[i] % R > 0) - have[i]);
     }
+    unsigned long long all = need;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0 && all) atomicAdd(&asked, all);
     const int at = total + block_excl_scan(need, wt, &tot);
     if (i < n) first[i] = at;
     total += tot;
     __syncthreads();
   }
   if (threadIdx.x == 0) first[n] = total;
-  if (code == PG_OK && total > 0) {  // code is CTA-uniform here: written before a barrier
-    const int got = total <= P ? take_free(refs, P, total, ref0, list, wt, &tot) : 0;
-    if (got < total && threadIdx.x == 0) code = PG_NO_PAGES;
+  const bool fit = asked <= (unsigned long long)P;  // then total is the sum
+  if (code == PG_OK && (total > 0 || !fit)) {  // code is CTA-uniform here: written before a barrier
+    const int got = fit ? take_free(refs, P, total, ref0, list, wt, &tot) : 0;
+    if ((!fit || got < total) && threadIdx.x == 0) code = PG_NO_PAGES;
   }
   __syncthreads();
   if (code == PG_OK)

@@ -138,3 +138,30 @@ def test_of_several_faults_the_lowest_code_is_told():
     # nothing is free either: 900 streams hold 1,800 pages, 200 are left for 1,200 children
     p.lens[5], p.table[7, 0] = 20, 1999
     p.refused([9] * n, list(range(1000, 1000 + n)), 1)
+
+
+@pytest.mark.parametrize("S,M", [(65536, 32769), (65536, 65537)])
+def test_a_reserve_of_more_pages_than_32_bits_count(S, M):
+    """Sums of 2^31 + 2^16 and of 2^32 + 2^16 pages, which are negative or 2^16 in 32 bits."""
+    from lagunalab_b200 import ops
+    table = torch.full((S, M), -1, dtype=torch.int32, device="cuda")
+    refs = torch.zeros(70000, dtype=torch.int32, device="cuda")
+    ids = torch.arange(S, dtype=torch.int32, device="cuda")
+    rows = torch.full((S,), M * 16, dtype=torch.int32, device="cuda")
+    assert ops.pages_reserve(table, refs, ids, rows, 16).tolist() == [1, 0]
+    assert int(table.max()) == -1 and not refs.any()
+    rows[1:] = 0  # one stream alone
+    rows[0] = 16 * min(M, 60000) - 5
+    assert ops.pages_reserve(table, refs, ids, rows, 16).tolist() == [0, min(M, 60000)]
+    assert int(refs.sum()) == min(M, 60000) and int((table >= 0).sum()) == min(M, 60000)
+
+
+def test_a_reserve_of_as_many_rows_as_32_bits_count():
+    from lagunalab_b200 import ops
+    table = torch.full((2, 2 ** 24 + 1), -1, dtype=torch.int32, device="cuda")
+    refs = torch.zeros(10, dtype=torch.int32, device="cuda")
+    call = lambda r: ops.pages_reserve(table, refs, _t([1]), _t([r]), 128).tolist()
+    for r in (2 ** 31 - 1, 2 ** 31 - 127, 2 ** 31 - 128):
+        assert call(r) == [1, 0]
+        assert int(table.max()) == -1 and not refs.any()
+    assert call(10 * 128) == [0, 10]
