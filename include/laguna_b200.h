@@ -614,9 +614,10 @@ size_t lg_prompt_plan_bytes(int T, int B, int Hq, int Hkv);
 size_t lg_stream_plan_bytes(int B, int Hq, int Hkv);
 
 /* 0, or what went wrong in a call with this plan: the code of a wait that ran out (the call then
- * ended with wrong rows instead of hanging), or 10 where the plan was made for other sizes or never
- * (out is left as it was). The code stays until the plan is made again. Synchronous (copies the
- * plan's head to the host). */
+ * ended with wrong rows instead of hanging, and later calls with the plan may, too), or 10 where
+ * the plan was made for other sizes or never (out is left as it was, and calls of the plan's own
+ * sizes are as before). The code stays until the plan is made again. Synchronous (copies the plan's
+ * head to the host). */
 int lg_plan_status(const void* plan, int* status);
 
 /* B sequences' new tokens, packed: tokens [cu_q[b], cu_q[b + 1]) (device int32 [B + 1], ascending,

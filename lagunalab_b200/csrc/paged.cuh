@@ -17,6 +17,7 @@ constexpr int PA_KEYS = 128;  // keys per tile
 constexpr int PA_ROWS = 128;  // query rows (token, head) per row tile
 
 enum { PA_PROMPT = 0, PA_PREFIX = 1, PA_OWN = 2 };
+constexpr int PA_MISFIT = 10;  // beside the codes of waits, 1 to 9
 
 struct PaTile {
   int row;      // table row
@@ -59,7 +60,8 @@ struct alignas(16) PaHead {
   int kind, B, T, Hq;  // two 16-byte loads, see pa_fits
   int Hkv, R, prefix, window;
   int ntiles;  // row tiles
-  int err;     // a wait that ran out (its code), else 0
+  int err;     // a wait that ran out (its code), else 0: ends the others' waits
+  int misfit;  // PA_MISFIT after a call of other sizes, which did nothing
 };
 
 // The parts of a plan buffer.

@@ -439,7 +439,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   PaWalk walk(a.plan);
   if (!pa_fits(a, head) || (smem_u32(smem) & 1023)) {  // no work; the loads pass with the walk's
     walk.end = walk.at;
-    if (threadIdx.x == 0) *err = 10;
+    // not in err, which the waits of later calls look at
+    if (threadIdx.x == 0) head->misfit = PA_MISFIT;
   }
 
   if (threadIdx.x == 0) {
@@ -1167,7 +1168,7 @@ extern "C" int lg_plan_status(const void* plan, int* status) {
   LG_CHECK_ARG(plan && status, "plan_status: NULL pointer");
   PaHead h;
   LG_CUDA_TRY(cudaMemcpy(&h, plan, sizeof(h), cudaMemcpyDeviceToHost));
-  *status = h.err;
+  *status = h.misfit == PA_MISFIT ? PA_MISFIT : h.err;
   return LG_OK;
 }
 

@@ -165,3 +165,28 @@ def test_a_reserve_of_as_many_rows_as_32_bits_count():
         assert call(r) == [1, 0]
         assert int(table.max()) == -1 and not refs.any()
     assert call(10 * 128) == [0, 10]
+
+
+def test_a_refused_call_leaves_the_plan_good():
+    """A call of other sizes (through the C interface, which cannot look into the plan) writes nothing;
+    the calls of the plan's own sizes that follow give their rows, with waits of every length: short
+    parts, parts of many key tiles, last tiles that end inside a page."""
+    from lagunalab_b200 import _lib, ops
+    from tests.test_paged_attention_gpu import D, _case
+    for new, kv, Hq, Hkv in (([20, 7], [90, 7], 4, 2), ([3000, 1, 700], [8001, 20001, 701], 32, 4),
+                             ([1], [60001], 3, 3)):
+        q, k, v, table, cu, kvt, _ = _case(new, kv, Hq, Hkv, 32, seed=1)
+        T, ks = q.shape[0], k.stride()
+        plan = ops.prompt_plan(cu, kvt, T, Hq, Hkv, 32)
+        want = ops.prompt_attention(q, k, v, table, plan, 0.1)
+        out = torch.full_like(q, 7.0)
+        for _ in range(3):
+            _lib.call("lg_prompt_attention", q.data_ptr(), q.stride(0), q.stride(1), T, Hq, Hkv, D,
+                      k.data_ptr(), v.data_ptr(), k.shape[0], 32, ks[0], ks[1], ks[2],
+                      table.data_ptr(), len(new) - 1 or 2, table.shape[1], 0.1, None,
+                      out.data_ptr(), plan.ptr, 1 << 40, torch.cuda.current_stream().cuda_stream)
+            assert (out == 7).all() and plan.status() == 10
+            for _ in range(5):
+                assert torch.equal(ops.prompt_attention(q, k, v, table, plan, 0.1), want)
+        assert plan.status() == 10
+        assert plan.update().status() == 0
