@@ -640,7 +640,7 @@ int lg_stream_plan(const int32_t* kv_len, int B, int Hq, int Hkv, int page_rows,
  * v_pages bf16 [P, Hkv, R, 128] with one set of element strides; table int32 [B, M]; gate bf16
  * [T, Hq] or NULL; out bf16 [T, Hq, 128], whose rows outside [cu_q[0], cu_q[B]) stay as they were.
  * R in {16, 32, 64, 128}; Hq % Hkv == 0, Hq / Hkv <= 16; scale > 0; pointers 16-byte aligned,
- * strides multiples of 8 elements. Rows of a sequence below its length are finite; what lies in
+ * strides positive multiples of 8 elements. Rows of a sequence below its length are finite; what lies in
  * its pages past the length does not matter. A sequence whose table names no page of the pool
  * for a row it needs gives NaN.
  */

@@ -1100,6 +1100,9 @@ static int attn_run(const char* who, int kind, const void* q, long long q_tok, l
   if (Hq == 1) q_head = D;
   if (P == 1) pg = D;
   if (Hkv == 1) hd = D;
+  // a tensor map's strides: steps of 0 bytes (a broadcast dimension) or back are not among them
+  LG_CHECK_ARG(q_tok > 0 && q_head > 0 && pg > 0 && hd > 0 && rw > 0,
+               "%s: strides of dimensions of more than one element must be positive", who);
   const int G = Hq / Hkv;
   CUtensorMap tm_q, tm_k, tm_v;
   const uint64_t qd[3] = {(uint64_t)D, (uint64_t)Hq, (uint64_t)T};

@@ -12,7 +12,9 @@
 //
 // Bounds: the moves read and write each row once, 16 bytes a lane, so they run at the copy rate of
 // HBM (118 pages of 80 planes moved: 192 us, 6.4 TB/s); the one-CTA kernels are latency (a scan of
-// refs and of the call's list), and the moving kernel's launch passes under them.
+// refs, of the call's list and of the sources' table rows: a fork of 3 streams 8.5 us with the free
+// before it, 8.1 without a look at the sources' whole pages), and the moving kernel's launch passes
+// under them. Times here are graph replays; calls in a row of 64 children take 57 us for 49.
 //
 // A fork's copies are written plane by plane in the order of their pages. Reading a page once for
 // all its copies instead left the reads 26 MB of 228, but the writes jumped between pages: 62 us

@@ -859,7 +859,7 @@ def _paged_attention(kind, q, k_pages, v_pages, table, plan, scale, gate, out):
     if B != plan.B:
         raise ValueError(f"the table has {B} rows, the plan {plan.B} sequences")
     qs = q.stride()
-    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or q.data_ptr() % 16:
+    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or q.data_ptr() % 16 or 0 in qs:
         q = q.clone(memory_format=torch.contiguous_format)
         qs = q.stride()
     if gate is None:

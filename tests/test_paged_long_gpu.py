@@ -106,3 +106,12 @@ def test_long_parts_of_streams(B, prefix, own, Hq, Hkv, R):
     out, A = _exact(q, k, v, table, [1] * B, kv, D ** -0.5, None, 0)
     _near(got, out, A, B)
     assert plan.status() == 0
+
+
+def test_a_query_broadcast_over_heads_or_tokens():
+    from lagunalab_b200 import ops
+    q, k, v, table, cu, kvt = _inputs([7, 40], [300, 90], 8, 2, 32, 0, seed=3)
+    plan = ops.prompt_plan(cu, kvt, 47, 8, 2, 32)
+    for x in (q[:, :1].expand(47, 8, D), q[:1].expand(47, 8, D)):
+        want = ops.prompt_attention(x.contiguous(), k, v, table, plan, D ** -0.5)
+        assert torch.equal(ops.prompt_attention(x, k, v, table, plan, D ** -0.5), want)
