@@ -786,7 +786,8 @@ def attn_prep_pages(qkvg, Hq, Hkv, D, qn_w, kn_w, eps, theta, seq, pos, table, k
 class AttentionPlan:
     """The division of a batch's paged attention over the GPU (``prompt_plan``, ``stream_plan``).
     It serves every layer with the same heads, page rows and window, and holds a call's partial
-    results: calls that may overlap on the GPU (another stream, another captured graph) need a
+    results (``nbytes``: 39 MB for prompts on 148 SMs however short they are, 21 MB and more for
+    streams): calls that may overlap on the GPU (another stream, another captured graph) need a
     plan each. ``update()`` divides anew for the lengths that its tensors hold by then; a plan
     whose lengths have moved on gives wrong rows. A captured graph's plan must outlive it."""
 
@@ -817,8 +818,9 @@ class AttentionPlan:
         return self
 
     def status(self):
-        """0, or what went wrong in a call with this plan: the code of a wait that ran out, or 10
-        where the plan was made for other sizes. Waits for the device."""
+        """0, or what went wrong in a call with this plan since its last ``update()``: the code of a
+        wait that ran out, or 10 where the plan was made for other sizes (calls of its own sizes
+        are as before). Waits for the device."""
         st = ctypes.c_int(0)
         torch.cuda.synchronize(self.index)
         with torch.cuda.device(self.index):
@@ -890,8 +892,10 @@ def prompt_attention(q, k_pages, v_pages, table, plan, scale, gate=None, out=Non
     """Causal attention of packed prompts over cache pages. q bf16 [T, Hq, 128]; k_pages, v_pages
     bf16 [P, Hkv, R, 128] (one layer of a pool) that hold the new tokens' rows already; table int32
     [B, M]; ``plan`` from ``prompt_plan``; gate bf16 [T, Hq] or None. Returns bf16 [T, Hq, 128]:
-    bf16(attention) * gate per token and head, 0 for a token without keys; with ``out`` given, rows
-    of no sequence stay as they were."""
+    bf16(attention) * gate per token and head, 0 for a token without keys. Rows of no sequence are
+    not written: they stay as they were in an ``out`` that is given, and are uninitialised in one
+    that is not. The softmax's weights are rounded to bf16 for the tensor cores (2^-8 relative a
+    weight at most), all sums are fp32."""
     return _paged_attention("prompt", q, k_pages, v_pages, table, plan, scale, gate, out)
 
 
