@@ -61,6 +61,41 @@ def test_a_stream_without_a_page_sits_the_step_out(prefix):
     assert cache.lens.tolist()[2] == 96 and dec.wrote.tolist()[2] is False
 
 
+def test_a_replayed_step_leaves_a_freed_stream_out():
+    """A step captured while all streams had pages gives the bits of eager steps after one is freed, and
+    after pages that were missing have come."""
+    from lagunalab_b200 import paged
+    _, model, _, _ = _model("sliding")
+    prompts = [p.tolist() for p in _prompts([37, 30, 20], 9)]
+    runs = []
+    for _ in range(2):
+        cache = paged.PagedCache(model, 3, 12, 32)
+        paged.prefill(model, cache, [0, 1, 2], prompts)  # two, one and one page
+        runs.append((cache, paged.Decoder(model, cache, [0, 1, 2])))
+    (cache, dec), (cache_e, eager) = runs
+    tok = _step_tokens(3, 0)
+    assert torch.equal(dec.step(tok), eager.step(tok))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        logits = dec.step(tok)
+    for i in range(1, 12):
+        for c in (cache, cache_e):
+            if i == 6:
+                c.free([2])
+            if i == 9:
+                c.reserve([1], [64])
+        tok.copy_(_step_tokens(3, i))
+        graph.replay()
+        want = eager.step(tok)
+        assert torch.equal(torch.nan_to_num(logits), torch.nan_to_num(want))
+        assert torch.equal(dec.wrote, eager.wrote)
+        assert torch.isnan(logits).all(1).tolist() == (~dec.wrote).tolist()
+        assert dec.wrote.tolist() == [True, i < 2 or i >= 9, i < 6]
+        assert cache.lens.tolist() == cache_e.lens.tolist()
+    assert cache.lens.tolist() == [49, 35, 0] and torch.equal(cache.pool, cache_e.pool)
+
+
 class _Pool:
     """Streams of a small pool, and whether a refused operation left all of it alone."""
 
