@@ -35,9 +35,9 @@
 // products of one row tile is 1,420 cycles of softmax alone, 2,200 beside the other's, and 1,024 of
 // products, and takes 3,700 with its hand-overs. Measured (B200; calls in a row, in brackets graph
 // replays of 10 ms, which end before the power limit acts): one 8,192-token prompt with 32/4 heads
-// 585 us (518), 940 TFLOP/s of the causal half; 2 x 512 tokens over 33,000 rows 590 us (503-568),
+// 585 us (515-547), 940 TFLOP/s of the causal half; 2 x 512 tokens over 33,000 rows 590 us (503-568),
 // 900 TFLOP/s, 0.54 of the measured bf16 GEMM rate and 0.65 of the one measured over seconds; 16
-// prompts of up to 1,500 tokens 171 us (158); 64 streams on an 8,192-row prefix 36 us (33), of which
+// prompts of up to 1,500 tokens 171 us (153-158); 64 streams on an 8,192-row prefix 36 us (32-39), of which
 // the join is 5; 64 streams of 8,192 rows each 176 us (6.1 TB/s; pages of 16 rows 203). The plan is
 // not in these times. The variants below were compared by graph replays.
 // The compiler spills 188 bytes a thread of the softmax warps' 216 registers (-Xptxas -v).
@@ -121,7 +121,7 @@ __device__ __forceinline__ PaTile pa_stream_tile(const PaHead& h, const PaPlan& 
   return t;
 }
 
-// Row tiles, their costs summed, and each CTA's start: one CTA; 4.5 to 7.2 us (one stream; 16 ragged
+// Row tiles, their costs summed, and each CTA's start: one CTA; 4.5 to 7.4 us (one stream; 16 ragged
 // prompts), once for all layers of a step with the same heads and window.
 __global__ void __launch_bounds__(PLAN_THREADS)
     pa_plan_kernel(const int* cu, const int* kv_len, PaHead h, PaPlan p) {
