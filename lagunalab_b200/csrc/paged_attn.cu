@@ -37,10 +37,10 @@
 // replays of 10 ms, which end before the power limit acts): one 8,192-token prompt with 32/4 heads
 // 585 us (515-547), 940 TFLOP/s of the causal half; 2 x 512 tokens over 33,000 rows 590 us (503-568),
 // 900 TFLOP/s, 0.54 of the measured bf16 GEMM rate and 0.65 of the one measured over seconds; 16
-// prompts of up to 1,500 tokens 171 us (153-158); 64 streams on an 8,192-row prefix 36 us (32-39), of which
-// the join is 5; 64 streams of 8,192 rows each 176 us (6.1 TB/s; pages of 16 rows 203). The plan is
-// not in these times. The variants below were compared by graph replays.
-// The compiler spills 188 bytes a thread of the softmax warps' 216 registers (-Xptxas -v).
+// prompts of up to 1,500 tokens 171 us (153-158); 64 streams on an 8,192-row prefix 36 us (32-39), of
+// which the join is 5; 64 streams of 8,192 rows each 176 us (6.1 TB/s; pages of 16 rows 203). The plan
+// is not in these times. The compiler reports 168 registers and 188 bytes of spill stores a thread.
+// The variants below were compared by graph replays.
 // Tried without gain: four softmax warpgroups (two threads a row; 560 us for 500), key tiles of 64
 // with two score places each (541; a 64-wide product takes as long as a 128-wide one), a part of
 // the exponentials as a polynomial on the FMA pipes (1/8: 526, 1/3: 546), the two product warps
