@@ -657,6 +657,41 @@ int lg_stream_attention(const void* q, long long q_tok, long long q_head, int B,
                         const int32_t* table, int M, float scale, const void* gate, void* out,
                         void* plan, size_t plan_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Fitting a model again: the head's cross entropy without its logits, and its gradient; the
+ * router's balance loss and gradient (no counterpart in the reference, whose replay harness
+ * scores log-softmax rows of materialised logits, replay/replay.py:93-114).
+ *
+ * Head: x bf16 [T, H] with rows ldx elements apart; w bf16 [V, H] with rows ldw elements apart
+ * (w_scales and w_biases NULL, H % 8 == 0), or the words of a 4-bit group-64 matrix with its
+ * scales and biases (ldw == H, H % 64 == 0), read as the bf16 weights bf16(scale * code + bias).
+ * ids int32 [T, K], 1 <= K <= 64, each with a weight (fp32 [T, K], or NULL: 1). A negative id is
+ * left out; a token whose ids are all left out has no target. An id may be listed twice.
+ *   z = x w^T,  lse[t] = log sum_v exp(z[t, v]),  loss[t] = sum_j weights[t, j] (lse[t] - z[t, ids[t, j]])
+ * fp32 [T] each; 0 for a token without a target, NaN for one with an id >= V. top (int32 [T] or
+ * NULL): the id of the largest logit, the lowest of equal ones. lse and top are of every token.
+ * x and w 16-byte aligned, strides multiples of 8 elements; the workspace 256-byte aligned.
+ */
+size_t lg_head_loss_workspace_bytes(int T, int H, int V, int K, int bits, int top);
+int lg_head_loss(const void* x, long long ldx, int T, int H, const void* w, long long ldw,
+                 const void* w_scales, const void* w_biases, int V, const int32_t* ids,
+                 const float* weights, int K, float* loss, float* lse, int32_t* top,
+                 void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The gradient of sum_t g[t] loss[t] (g, lse fp32 [T]; lse as lg_head_loss gives it):
+ *   dz[t, v] = g[t] (S[t] exp(z[t, v] - lse[t]) - sum_{j: ids[t, j] = v} weights[t, j]), S[t] the counted
+ *   weights' sum,  dx = dz w (bf16 [T, H]),  dw = dz^T x (bf16 [V, H]).
+ * dx or dw may be NULL (not both); a 4-bit head has no dw. A token without a target adds nothing to dw
+ * and gives a row of zeros in dx, whatever its row of x holds; an id >= V counts as left out. dz is
+ * rounded to bf16 for the tensor cores (2^-8 relative at most), sums are fp32.
+ */
+size_t lg_head_loss_grad_workspace_bytes(int T, int H, int V, int K, int bits, int dx, int dw);
+int lg_head_loss_grad(const void* x, long long ldx, int T, int H, const void* w, long long ldw,
+                      const void* w_scales, const void* w_biases, int V, const int32_t* ids,
+                      const float* weights, int K, const float* lse, const float* g, void* dx,
+                      void* dw, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -110,6 +110,12 @@ SIGNATURES = {
                                     P]),
     "lg_stream_attention": (c_int, [P, c_longlong, c_longlong, I, I, I, I, P, P, I, I, c_longlong,
                                     c_longlong, c_longlong, P, I, c_float, P, P, P, c_size_t, P]),
+    "lg_head_loss_workspace_bytes": (c_size_t, [I, I, I, I, I, I]),
+    "lg_head_loss": (c_int, [P, c_longlong, I, I, P, c_longlong, P, P, I, P, P, I, P, P, P, P,
+                             c_size_t, P]),
+    "lg_head_loss_grad_workspace_bytes": (c_size_t, [I, I, I, I, I, I, I]),
+    "lg_head_loss_grad": (c_int, [P, c_longlong, I, I, P, c_longlong, P, P, I, P, P, I, P, P, P, P,
+                                  P, c_size_t, P]),
 }
 
 _lib = None

@@ -1,0 +1,848 @@
+// The head's cross entropy without its logits, and its gradient.
+//
+//   z = x W^T (x bf16 [T, H], W bf16 [V, H], or a 4-bit head read as its bf16 weights),
+//   lse_t = log sum_v exp z_tv,   loss_t = sum_j w_tj (lse_t - z_t,id_tj)  over the ids in [0, V),
+//   dz_tv = g_t (S_t exp(z_tv - lse_t) - sum_{j: id_tj = v} w_tj),   S_t = sum_j w_tj,
+//   dx = dz W,   dW = dz^T x.
+//
+// Four tiled products in one kernel template (hd_kernel): HD_LOSS leaves each 256-column tile's
+// maximum and sum of exponentials per token (a second kernel joins them), HD_PROB computes z again
+// and leaves dz as bf16 for a piece of the vocabulary, HD_XGRAD and HD_WGRAD take the piece's dz to
+// dx (fp32, added over the pieces) and to its rows of dW. Nothing of size [T, V] is kept.
+//
+// Roundings: z, the softmax statistics and every sum are fp32. dz is rounded to bf16 (2^-8 relative
+// at most) because the tensor cores take bf16 operands; its errors are independent, so that sums over
+// the vocabulary or the tokens average them. dx and dW are rounded once, at the end.
+//
+// Every mbarrier wait is bounded (tc::mbar_wait). A CTA whose wait ran out writes NaN for what is
+// left of its tiles, waits (bounded) for its copies and products in flight, frees its TMEM and ends.
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "common.cuh"
+#include "tc_ptx.cuh"
+#include "tmap.cuh"
+
+namespace lg {
+
+using namespace tc;
+
+enum { HD_LOSS = 0, HD_PROB = 1, HD_XGRAD = 2, HD_WGRAD = 3 };
+
+constexpr int HD_BM = 128, HD_BN = 256, HD_BK = 64;
+constexpr int HD_STAGES = 4;
+constexpr int HD_THREADS = 256;
+constexpr int HD_A_BYTES = HD_BM * HD_BK * 2;  // 16 KB
+constexpr int HD_B_BYTES = HD_BN * HD_BK * 2;  // 32 KB
+constexpr int HD_STAGE_BYTES = HD_A_BYTES + HD_B_BYTES;
+constexpr int HD_BOX = 64 * HD_BK * 2;  // an MN-major box: 64 K rows of 64 elements
+constexpr size_t HD_SMEM = 1024 + (size_t)HD_STAGES * HD_STAGE_BYTES + 256;
+constexpr int HD_MAXK = 64;
+constexpr float HD_LOG2E = 1.4426950408889634f;
+
+struct HdArgs {
+  int M, N;          // rows of the output tile grid, and its columns
+  int mt, nt;        // tiles of 128 x 256
+  int kblocks;       // 64-wide blocks of the contraction
+  int splits;        // HD_XGRAD: parts of the contraction, each with a sum of its own
+  int b_row0;        // HD_LOSS, HD_PROB: B's first row; HD_XGRAD: B's first row along the contraction
+  int v0;            // the piece's first vocabulary id
+  int V;
+  int K;             // targets a token
+  const int* ids;    // [T, K]; K > 1: sorted (with `order`, `start`)
+  const float* weights;       // [T, K] or NULL, in the caller's order
+  const unsigned char* order;  // K > 1: [T, K] the caller's index of a sorted id
+  const unsigned char* start;  // K > 1: [T, nt_all + 1] first sorted id of each vocabulary tile
+  int nt_all;
+  // HD_LOSS
+  float2* part;  // [T, nt_all] (maximum, sum)
+  int* top;      // [T, nt_all] the maximum's id, or NULL
+  float* ztgt;   // [T, K]
+  // HD_PROB
+  const float* lse;
+  const float* g;
+  const float* wsum;  // K > 1: [T]
+  __nv_bfloat16* dz;  // [T, ldz]
+  int ldz;
+  // HD_XGRAD
+  float* dx;  // [splits, T, H]
+  int add;    // 0: the first piece
+  // HD_WGRAD
+  __nv_bfloat16* dw;  // [V, H]
+};
+
+__device__ __forceinline__ float hd_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// v[c] with a runtime c, by selects (registers have no index).
+__device__ __forceinline__ float hd_pick(const float (&v)[32], int c) {
+  float r = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r = i == c ? v[i] : r;
+  return r;
+}
+__device__ __forceinline__ void hd_sub(float (&v)[32], int c, float w) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = i == c ? v[i] - w : v[i];
+}
+
+__device__ __forceinline__ uint32_t hd_pack(float a, float b) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// A unit of work: tile (m, n) of the output, and the part [k0, k1) of the contraction's blocks.
+struct HdUnit {
+  int m, n, split, k0, k1;
+};
+template <int KIND>
+__device__ __forceinline__ HdUnit hd_unit(const HdArgs& a, int i) {
+  HdUnit u;
+  if (KIND == HD_LOSS || KIND == HD_PROB) {  // tokens inner: a tile of W serves all of them from L2
+    u.m = i % a.mt;
+    u.n = i / a.mt;
+    u.split = 0;
+  } else {
+    u.n = i % a.nt;
+    const int r = i / a.nt;
+    u.m = r % a.mt;
+    u.split = r / a.mt;
+  }
+  u.k0 = (int)((long long)a.kblocks * u.split / a.splits);
+  u.k1 = (int)((long long)a.kblocks * (u.split + 1) / a.splits);
+  return u;
+}
+
+// One output tile's row of this thread. `ok` is false after a wait that ran out: NaN is written.
+template <int KIND>
+__device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, int row, uint32_t taddr,
+                                            bool ok) {
+  const int t = u.m * HD_BM + row;
+  const int n0 = u.n * HD_BN;  // in the piece (or in H)
+  const bool live = t < a.M;
+  const float nan = __int_as_float(0x7fffffff);
+  float v[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = nan;
+  if (KIND == HD_LOSS || KIND == HD_PROB) {
+    const int ntile = a.v0 / HD_BN + u.n;
+    const int c0 = a.v0 + n0;  // the tile's first vocabulary id
+    const size_t row_k = (size_t)t * a.K;
+    int p = 0, p1 = 0, next = -1;  // K > 1: sorted ids [p, p1) of this tile; `next`: the next id
+    if (live) {
+      if (a.K == 1) {
+        next = a.ids[t];
+      } else {
+        const unsigned char* st = a.start + (size_t)t * (a.nt_all + 1) + ntile;
+        p = st[0];
+        p1 = st[1];
+        next = p < p1 ? a.ids[row_k + p] : -1;
+      }
+    }
+    if (KIND == HD_LOSS) {
+      float mx = -INFINITY, sum = 0.f;
+      int arg = 0;
+#pragma unroll 1
+      for (int c = 0; c < HD_BN; c += 32) {
+        const int id0 = c0 + c;
+        if (id0 >= a.V) break;
+        __syncwarp();
+        if (ok) tmem_ld32_wait(taddr + c, v);
+        if (id0 + 32 > a.V) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = id0 + i < a.V ? v[i] : -INFINITY;
+        }
+        while ((unsigned)next - (unsigned)id0 < 32u) {
+          const float z = hd_pick(v, next - id0);
+          if (a.K == 1) {
+            a.ztgt[t] = z;
+            break;
+          }
+          a.ztgt[row_k + a.order[row_k + p]] = z;
+          next = ++p < p1 ? a.ids[row_k + p] : -1;
+        }
+        float cm = v[0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) cm = fmaxf(cm, v[i]);
+        if (cm > mx) {
+          if (a.top) {
+            int at = 0;
+#pragma unroll
+            for (int i = 31; i >= 0; --i) at = v[i] == cm ? i : at;
+            arg = id0 + at;
+          }
+          sum *= hd_ex2((mx - cm) * HD_LOG2E);  // mx = -inf: sum is 0
+          mx = cm;
+        }
+        const float off = mx == -INFINITY ? 0.f : -mx * HD_LOG2E;
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          s0 += hd_ex2(fmaf(v[i], HD_LOG2E, off));
+          s1 += hd_ex2(fmaf(v[i + 1], HD_LOG2E, off));
+        }
+        sum += s0 + s1;
+      }
+      if (live) {
+        a.part[(size_t)t * a.nt_all + ntile] = make_float2(mx, ok ? sum : nan);
+        if (a.top) a.top[(size_t)t * a.nt_all + ntile] = arg;
+      }
+    } else {
+      float gs = 0.f, gg = 0.f, off = 0.f;
+      bool counts = false;
+      if (live) {
+        gg = a.g[t];
+        off = -a.lse[t] * HD_LOG2E;
+        if (a.K == 1) {
+          counts = next >= 0 && next < a.V;
+          gs = gg * (a.weights ? a.weights[t] : 1.f);
+        } else {
+          counts = a.start[(size_t)t * (a.nt_all + 1) + a.nt_all] > 0;
+          gs = gg * a.wsum[t];
+        }
+      }
+      __nv_bfloat16* out = a.dz + (size_t)t * a.ldz + n0;
+#pragma unroll 1
+      for (int c = 0; c < HD_BN && n0 + c < a.ldz; c += 32) {
+        const int id0 = c0 + c;
+        __syncwarp();
+        if (ok) tmem_ld32_wait(taddr + c, v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = ok ? gs * hd_ex2(fmaf(v[i], HD_LOG2E, off)) : nan;
+        while ((unsigned)next - (unsigned)id0 < 32u) {
+          if (a.K == 1) {
+            hd_sub(v, next - id0, gs);
+            break;
+          }
+          const float w = a.weights ? a.weights[row_k + a.order[row_k + p]] : 1.f;
+          hd_sub(v, next - id0, gg * w);
+          next = ++p < p1 ? a.ids[row_k + p] : -1;
+        }
+        if (!counts) {  // a token without a target: nothing of it, whatever its row holds
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        }
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            *reinterpret_cast<uint4*>(out + c + i) =
+                make_uint4(hd_pack(v[i], v[i + 1]), hd_pack(v[i + 2], v[i + 3]),
+                           hd_pack(v[i + 4], v[i + 5]), hd_pack(v[i + 6], v[i + 7]));
+        }
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (int c = 0; c < HD_BN && n0 + c < a.N; c += 32) {
+      __syncwarp();
+      if (ok) tmem_ld32_wait(taddr + c, v);
+      if (!live) continue;
+      if (KIND == HD_XGRAD) {
+        float* out = a.dx + ((size_t)u.split * a.M + t) * a.N + n0 + c;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          if (n0 + c + i >= a.N) break;
+          float4 w = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          if (a.add) {
+            const float4 o = *reinterpret_cast<const float4*>(out + i);
+            w = make_float4(w.x + o.x, w.y + o.y, w.z + o.z, w.w + o.w);
+          }
+          *reinterpret_cast<float4*>(out + i) = w;
+        }
+      } else {
+        __nv_bfloat16* out = a.dw + ((size_t)a.v0 + t) * a.N + n0 + c;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          if (n0 + c + i >= a.N) break;
+          *reinterpret_cast<uint4*>(out + i) =
+              make_uint4(hd_pack(v[i], v[i + 1]), hd_pack(v[i + 2], v[i + 3]),
+                         hd_pack(v[i + 4], v[i + 5]), hd_pack(v[i + 6], v[i + 7]));
+        }
+      }
+    }
+  }
+}
+
+// D[M, N] = A B^T over tiles of 128 x 256. A and B are K-major ([rows, contraction]) or MN-major
+// ([contraction, rows]): HD_LOSS, HD_PROB: x and W, both K-major; HD_XGRAD: dz K-major, W MN-major;
+// HD_WGRAD: dz and x, both MN-major. Warp 0: TMA; warp 1: products into one of two TMEM tiles;
+// warps 4 to 7: the finished tile's rows, one a thread, while the next one's products run.
+template <int KIND>
+__global__ void __launch_bounds__(HD_THREADS, 1)
+    hd_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
+              const HdArgs a) {
+  constexpr bool A_MN = KIND == HD_WGRAD, B_MN = KIND == HD_XGRAD || KIND == HD_WGRAD;
+  extern __shared__ uint8_t hd_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)hd_smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + HD_STAGES * HD_STAGE_BYTES);
+  uint64_t* empty = full + HD_STAGES;
+  uint64_t* acc_full = empty + HD_STAGES;  // [2]
+  uint64_t* acc_empty = acc_full + 2;      // [2]
+  uint64_t* done = acc_empty + 2;
+  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(done + 1);
+  int* err = reinterpret_cast<int*>(tmem_base + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < HD_STAGES; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + i, 1);
+      mbar_init(acc_empty + i, 4);
+    }
+    mbar_init(done, 1);
+    err[0] = err[1] = err[2] = 0;  // of all roles; of the copies' end; of the products' end
+    fence_mbar_init();
+    prefetch_tmap(&ma);
+    prefetch_tmap(&mb);
+  }
+  if (warp == 2) {
+    tmem_alloc(tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_base;
+  const int units = a.mt * a.nt * a.splits;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int st = 0, used = 0;  // used: stages that hold a copy in this or an earlier turn
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
+        const HdUnit u = hd_unit<KIND>(a, i);
+        const int ar = u.m * HD_BM, br = u.n * HD_BN;
+        for (int kb = u.k0; kb < u.k1; ++kb) {
+          if (!mbar_wait(empty + st, ph ^ 1, err, 1)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sa = smem + st * HD_STAGE_BYTES;
+          uint8_t* sb = sa + HD_A_BYTES;
+          mbar_arrive_expect_tx(full + st, HD_STAGE_BYTES);
+          const int k = kb * HD_BK;
+          if (A_MN) {
+#pragma unroll
+            for (int j = 0; j < HD_BM / 64; ++j)
+              tma_load_2d(sa + j * HD_BOX, &ma, full + st, ar + j * 64, k);
+          } else {
+            tma_load_2d(sa, &ma, full + st, k, ar);
+          }
+          if (B_MN) {
+#pragma unroll
+            for (int j = 0; j < HD_BN / 64; ++j)
+              tma_load_2d(sb + j * HD_BOX, &mb, full + st, br + j * 64,
+                          (KIND == HD_XGRAD ? a.b_row0 : 0) + k);
+          } else {
+            tma_load_2d(sb, &mb, full + st, k, a.b_row0 + br);
+          }
+          if (used < HD_STAGES) ++used;
+          if (++st == HD_STAGES) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      // Every copy has landed before the CTA ends: the last `used` ones, oldest first.
+      for (int j = used; j > 0; --j) {
+        const int s = (st - j + HD_STAGES) % HD_STAGES;
+        const uint32_t p = s < st ? ph : ph ^ 1;
+        mbar_wait(full + s, p, err + 1, 2, 400000000LL);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_bf16(HD_BM, HD_BN) | (A_MN ? 1u << 15 : 0u) |
+                                 (B_MN ? IDESC_B_MN : 0u);
+      const uint64_t hi = (uint64_t)SW128_HI << 32;
+      int st = 0, n = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; i < units && ok; i += gridDim.x, ++n) {
+        const HdUnit u = hd_unit<KIND>(a, i);
+        const int acc = n & 1;
+        if (!mbar_wait(acc_empty + acc, ((n >> 1) & 1) ^ 1, err, 3)) break;
+        tc_fence_after();
+        for (int kb = u.k0; kb < u.k1; ++kb) {
+          if (!mbar_wait(full + st, ph, err, 4)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + st * HD_STAGE_BYTES), sb = sa + HD_A_BYTES;
+          const uint32_t da = A_MN ? sw128_lo_mn(sa, HD_BOX) : sw128_lo(sa);
+          const uint32_t db = B_MN ? sw128_lo_mn(sb, HD_BOX) : sw128_lo(sb);
+#pragma unroll
+          for (int k = 0; k < HD_BK / 16; ++k)  // 16 along K: 32 bytes, or two groups of 8 rows
+            umma_bf16(tmem + acc * HD_BN, hi | (da + k * (A_MN ? 128 : 2)),
+                      hi | (db + k * (B_MN ? 128 : 2)), idesc, kb > u.k0 || k > 0);
+          umma_commit(empty + st);
+          if (++st == HD_STAGES) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+        if (ok) umma_commit(acc_full + acc);
+      }
+      umma_commit(done);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int q = warp & 3;
+    bool ok = true;
+    int n = 0;
+    for (int i = blockIdx.x; i < units; i += gridDim.x, ++n) {
+      const HdUnit u = hd_unit<KIND>(a, i);
+      const int acc = n & 1;
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + acc, (n >> 1) & 1, err, 5));
+      tc_fence_after();
+      hd_epilogue<KIND>(a, u, q * 32 + lane, tmem + acc * HD_BN + ((uint32_t)(q * 32) << 16), ok);
+      tc_fence_before();
+      __syncwarp();
+      if (ok && lane == 0) mbar_arrive(acc_empty + acc);
+    }
+  }
+  // The products have ended before their TMEM goes.
+  if (warp == 2) {
+    mbar_wait(done, 0, err + 2, 6, 8000000000LL);
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+// ---- small kernels ------------------------------------------------------------------------------
+
+// K > 1: a warp sorts a token's ids (those in [0, V), ascending, equal ones in their order), with each
+// one's place in the caller's list, the first of each vocabulary tile, and the weights' sum.
+__global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ ids,
+                                                      const float* __restrict__ weights, int T, int K,
+                                                      int V, int nt, int* __restrict__ sorted,
+                                                      unsigned char* __restrict__ order,
+                                                      unsigned char* __restrict__ start,
+                                                      float* __restrict__ wsum) {
+  __shared__ int sh[8][HD_MAXK];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x * 8 + warp;
+  if (t >= T) return;
+  int* row = sh[warp];
+  float sum = 0.f;
+  for (int j = lane; j < HD_MAXK; j += 32) {
+    const int id = j < K ? ids[(size_t)t * K + j] : -1;
+    const bool in = id >= 0 && id < V;
+    row[j] = in ? id : 0x7fffffff;
+    if (in) sum += weights ? weights[(size_t)t * K + j] : 1.f;
+  }
+  sum = warp_sum(sum);
+  __syncwarp();
+  for (int j = lane; j < K; j += 32) {
+    const int id = row[j];
+    int rank = 0;
+    for (int i = 0; i < K; ++i) rank += row[i] < id || (row[i] == id && i < j);
+    sorted[(size_t)t * K + rank] = id;
+    order[(size_t)t * K + rank] = (unsigned char)j;
+  }
+  for (int n = lane; n <= nt; n += 32) {  // n = nt: all that count
+    const int lim = n == nt ? V : n * HD_BN;
+    int c = 0;
+    for (int i = 0; i < K; ++i) c += row[i] < lim;
+    start[(size_t)t * (nt + 1) + n] = (unsigned char)c;
+  }
+  if (lane == 0) wsum[t] = sum;
+}
+
+// A warp joins a token's tiles: lse, the loss, and the id of the largest logit.
+__global__ void __launch_bounds__(256) hd_join_kernel(const float2* __restrict__ part,
+                                                      const int* __restrict__ tops, int T, int nt,
+                                                      const int* __restrict__ ids,
+                                                      const float* __restrict__ weights, int K, int V,
+                                                      const float* __restrict__ ztgt,
+                                                      float* __restrict__ loss,
+                                                      float* __restrict__ lse_out,
+                                                      int* __restrict__ top) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x * 8 + warp;
+  if (t >= T) return;
+  const float2* row = part + (size_t)t * nt;
+  float mx = -INFINITY, sum = 0.f;
+  int at = -1;
+#pragma unroll 4
+  for (int n = lane; n < nt; n += 32) {
+    const float2 v = row[n];
+    if (v.x > mx) {
+      sum = sum * hd_ex2((mx - v.x) * HD_LOG2E) + v.y;
+      mx = v.x;
+      at = n;
+    } else {
+      sum += v.x == -INFINITY ? v.y : v.y * hd_ex2((v.x - mx) * HD_LOG2E);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, mx, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
+    const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
+    const float m = fmaxf(mx, m2);
+    const float ea = mx == m ? 1.f : hd_ex2((mx - m) * HD_LOG2E);
+    const float eb = m2 == m ? 1.f : hd_ex2((m2 - m) * HD_LOG2E);
+    // Both lanes of a pair add in the same order, the lower lane's part first.
+    sum = (lane & o) ? s2 * eb + sum * ea : sum * ea + s2 * eb;
+    at = m2 > mx || (m2 == mx && (unsigned)a2 < (unsigned)at) ? a2 : at;
+    mx = m;
+  }
+  const float lse = __shfl_sync(0xffffffffu, mx + logf(sum), 0);
+  float l = 0.f;
+  bool bad = false;
+  for (int j = lane; j < K; j += 32) {
+    const int id = ids[(size_t)t * K + j];
+    if (id >= V) bad = true;
+    if (id < 0 || id >= V) continue;
+    l += (weights ? weights[(size_t)t * K + j] : 1.f) * (lse - ztgt[(size_t)t * K + j]);
+  }
+  l = warp_sum(l);
+  bad = __any_sync(0xffffffffu, bad);
+  if (lane == 0) {
+    loss[t] = bad ? __int_as_float(0x7fffffff) : l;
+    lse_out[t] = lse;
+    if (top) top[t] = at >= 0 ? tops[(size_t)t * nt + at] : 0;
+  }
+}
+
+// x with the rows of tokens without a target at 0, so that dW has nothing of them (0 * NaN is NaN).
+__global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx,
+                                                      int T, int H, const int* __restrict__ ids, int K,
+                                                      int V, __nv_bfloat16* __restrict__ out) {
+  const int per = H / 8;
+  const long long n = (long long)T * per;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
+    const int t = (int)(i / per), c = (int)(i % per) * 8;
+    bool in = false;
+    for (int j = 0; j < K && !in; ++j) {
+      const int id = ids[(size_t)t * K + j];
+      in = id >= 0 && id < V;
+    }
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (in) v = *reinterpret_cast<const uint4*>(x + (size_t)t * ldx + c);
+    *reinterpret_cast<uint4*>(out + (size_t)t * H + c) = v;
+  }
+}
+
+// Rows of a 4-bit group-64 head as bf16: bf16(scale * code + bias), eight of a word a thread.
+__global__ void __launch_bounds__(256) hd_dequant_kernel(const uint32_t* __restrict__ q,
+                                                         const __nv_bfloat16* __restrict__ s,
+                                                         const __nv_bfloat16* __restrict__ b,
+                                                         long long words, __nv_bfloat16* __restrict__ out) {
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < words; i += gridDim.x * 256LL) {
+    const uint32_t w = q[i];
+    const float sc = bf2f(s[i >> 3]), bi = bf2f(b[i >> 3]);
+    uint32_t r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      r[j] = hd_pack(fmaf(sc, (float)((w >> (8 * j)) & 15u), bi),
+                     fmaf(sc, (float)((w >> (8 * j + 4)) & 15u), bi));
+    *reinterpret_cast<uint4*>(out + 8 * i) = make_uint4(r[0], r[1], r[2], r[3]);
+  }
+}
+
+// dx = the sum of its parts, in their order, rounded once.
+__global__ void __launch_bounds__(256) hd_sum_kernel(const float* __restrict__ parts, int n,
+                                                     long long size, __nv_bfloat16* __restrict__ out) {
+  const long long q = size / 4;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < q; i += gridDim.x * 256LL) {
+    float4 s = reinterpret_cast<const float4*>(parts)[i];
+    for (int j = 1; j < n; ++j) {
+      const float4 v = reinterpret_cast<const float4*>(parts + j * size)[i];
+      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+    }
+    *reinterpret_cast<uint2*>(out + 4 * i) = make_uint2(hd_pack(s.x, s.y), hd_pack(s.z, s.w));
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+
+constexpr long long HD_DZ_BYTES = 256LL << 20;  // dz of a piece
+constexpr long long HD_WQ_BYTES = 64LL << 20;   // bf16 rows of a piece of a 4-bit head: they stay in L2
+
+// Vocabulary ids a piece: a multiple of 256.
+static int hd_piece(int T, int H, int V, bool quant, bool grad) {
+  long long n = ((long long)V + HD_BN - 1) / HD_BN;
+  if (grad) n = std::min(n, HD_DZ_BYTES / (2LL * T * HD_BN));
+  if (quant) n = std::min(n, HD_WQ_BYTES / (2LL * H * HD_BN));
+  return (int)(std::max(n, 1LL) * HD_BN);
+}
+
+static int hd_splits(int T, int H, int piece) {
+  const int tiles = ((T + HD_BM - 1) / HD_BM) * ((H + HD_BN - 1) / HD_BN);
+  const int sms = device_sm_count();
+  if (tiles >= sms) return 1;
+  return std::max(1, std::min(sms / tiles, piece / (4 * HD_BK)));
+}
+
+struct HdWork {
+  float2* part;
+  int* tops;
+  float* ztgt;
+  int* sorted;
+  unsigned char *order, *start;
+  float* wsum;
+  __nv_bfloat16 *wq, *dz, *xz;
+  float* dx;
+  size_t bytes;
+  int piece, nt, splits;
+};
+
+static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool grad, bool dx, bool dw,
+                       bool top) {
+  HdWork w = {};
+  Carver c(base);
+  w.nt = (V + HD_BN - 1) / HD_BN;
+  w.piece = hd_piece(T, H, V, quant, grad);
+  if (!grad) {
+    w.part = c.take<float2>((size_t)T * w.nt);
+    if (top) w.tops = c.take<int>((size_t)T * w.nt);
+    w.ztgt = c.take<float>((size_t)T * K);
+  }
+  if (K > 1) {
+    w.sorted = c.take<int>((size_t)T * K);
+    w.order = c.take<unsigned char>((size_t)T * K);
+    w.start = c.take<unsigned char>((size_t)T * (w.nt + 1));
+    w.wsum = c.take<float>(T);
+  }
+  if (quant) w.wq = c.take<__nv_bfloat16>((size_t)std::min(w.piece, V) * H);
+  if (grad) {
+    w.dz = c.take<__nv_bfloat16>((size_t)T * w.piece);
+    if (dw) w.xz = c.take<__nv_bfloat16>((size_t)T * H);
+    if (dx) {
+      w.splits = hd_splits(T, H, w.piece);
+      w.dx = c.take<float>((size_t)w.splits * T * H);
+    }
+  }
+  w.bytes = align_up(c.used, 256);
+  return w;
+}
+
+template <int KIND>
+static int hd_launch(const CUtensorMap& ma, const CUtensorMap& mb, const HdArgs& a, cudaStream_t st) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  LG_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !done[dev].load(std::memory_order_relaxed)) {
+    LG_CUDA_TRY(cudaFuncSetAttribute(hd_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)HD_SMEM));
+    if (dev < 64) done[dev].store(true, std::memory_order_relaxed);
+  }
+  const long long units = (long long)a.mt * a.nt * a.splits;
+  const int grid = (int)std::min<long long>(units, device_sm_count());
+  hd_kernel<KIND><<<grid, HD_THREADS, HD_SMEM, st>>>(ma, mb, a);
+  LG_LAUNCH_CHECK("head");
+  return LG_OK;
+}
+
+static int hd_map(CUtensorMap* m, const void* p, long long inner, long long rows, long long ld,
+                  int box_rows) {
+  return make_map_2d(m, p, true, inner, rows, (uint64_t)ld * 2, 64, box_rows, 128);
+}
+
+static int hd_check(const char* who, const void* x, long long ldx, int T, int H, const void* w,
+                    long long ldw, const void* ws, const void* wb, int V, const int* ids, int K) {
+  LG_CHECK_ARG(T >= 0 && V >= 1 && V <= (1 << 30), "%s: T=%d V=%d", who, T, V);
+  LG_CHECK_ARG(K >= 1 && K <= HD_MAXK, "%s: K=%d targets not in [1, %d]", who, K, HD_MAXK);
+  LG_CHECK_ARG((ws == nullptr) == (wb == nullptr), "%s: scales and biases go together", who);
+  const int unit = ws ? 64 : 8;
+  LG_CHECK_ARG(H >= unit && H <= (1 << 20) && H % unit == 0, "%s: H=%d is not a multiple of %d", who, H, unit);
+  LG_CHECK_ARG(w && (T == 0 || (x && ids)), "%s: NULL pointer", who);
+  LG_CHECK_ARG(aligned(x, 16) && aligned(w, 16) && aligned(ws, 2) && aligned(wb, 2),
+               "%s: x and the weights must be 16-byte aligned", who);
+  LG_CHECK_ARG(ldx >= H && ldx % 8 == 0 && ldx < (1LL << 38), "%s: x's row stride %lld", who, ldx);
+  LG_CHECK_ARG(ws ? ldw == H : ldw >= H && ldw % 8 == 0 && ldw < (1LL << 38),
+               "%s: the weights' row stride %lld", who, ldw);
+  LG_CHECK_ARG((long long)((T + HD_BM - 1) / HD_BM) * ((V + HD_BN - 1) / HD_BN) < (1LL << 30),
+               "%s: T=%d times V=%d is too large", who, T, V);
+  return LG_OK;
+}
+
+static int hd_blocks(long long n) { return (int)std::min<long long>((n + 255) / 256, 148 * 16); }
+
+// The piece's bf16 weights and B's first row in them.
+static int hd_weights(const void* w, const void* ws, const void* wb, int H, int v0, int rows,
+                      const HdWork& k, cudaStream_t st) {
+  if (!ws) return LG_OK;
+  const long long words = (long long)rows * (H / 8);
+  const size_t at = (size_t)v0 * (H / 8);
+  hd_dequant_kernel<<<hd_blocks(words), 256, 0, st>>>(
+      static_cast<const uint32_t*>(w) + at, static_cast<const __nv_bfloat16*>(ws) + at / 8,
+      static_cast<const __nv_bfloat16*>(wb) + at / 8, words, k.wq);
+  LG_LAUNCH_CHECK("head_dequant");
+  return LG_OK;
+}
+
+static int hd_sort(const int* ids, const float* weights, int T, int K, int V, const HdWork& k,
+                   cudaStream_t st) {
+  if (K == 1) return LG_OK;
+  hd_sort_kernel<<<(T + 7) / 8, 256, 0, st>>>(ids, weights, T, K, V, k.nt, k.sorted, k.order, k.start,
+                                              k.wsum);
+  LG_LAUNCH_CHECK("head_sort");
+  return LG_OK;
+}
+
+#define HD_TRY(expr)           \
+  do {                         \
+    const int rc_ = (expr);    \
+    if (rc_ != LG_OK) return rc_; \
+  } while (0)
+
+static HdArgs hd_args(int T, int V, int K, const int* ids, const float* weights, const HdWork& k) {
+  HdArgs a = {};
+  a.V = V;
+  a.K = K;
+  a.ids = K > 1 ? k.sorted : ids;
+  a.weights = weights;
+  a.order = k.order;
+  a.start = k.start;
+  a.nt_all = k.nt;
+  a.splits = 1;
+  a.M = T;
+  a.mt = (T + HD_BM - 1) / HD_BM;
+  return a;
+}
+
+}  // namespace lg
+
+using namespace lg;
+
+extern "C" size_t lg_head_loss_workspace_bytes(int T, int H, int V, int K, int bits, int top) {
+  if (T < 1 || H < 8 || V < 1 || K < 1) return 256;
+  return hd_carve(nullptr, T, H, V, K, bits == 4, false, false, false, top != 0).bytes;
+}
+
+extern "C" size_t lg_head_loss_grad_workspace_bytes(int T, int H, int V, int K, int bits, int dx, int dw) {
+  if (T < 1 || H < 8 || V < 1 || K < 1) return 256;
+  return hd_carve(nullptr, T, H, V, K, bits == 4, true, dx != 0, dw != 0, false).bytes;
+}
+
+extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const void* w, long long ldw,
+                            const void* w_scales, const void* w_biases, int V, const int32_t* ids,
+                            const float* weights, int K, float* loss, float* lse, int32_t* top,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  HD_TRY(hd_check("head_loss", x, ldx, T, H, w, ldw, w_scales, w_biases, V, ids, K));
+  if (T == 0) return LG_OK;
+  LG_CHECK_ARG(loss && lse, "head_loss: NULL output");
+  const bool quant = w_scales != nullptr;
+  const HdWork k = hd_carve(workspace, T, H, V, K, quant, false, false, false, top != nullptr);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < k.bytes)
+    return fail(LG_ERR_WORKSPACE, "head_loss: workspace of %zu bytes, need %zu", workspace_bytes, k.bytes);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
+  CUtensorMap mx, mw;
+  HD_TRY(hd_map(&mx, x, H, T, ldx, HD_BM));
+  HdArgs a = hd_args(T, V, K, ids, weights, k);
+  a.kblocks = (H + HD_BK - 1) / HD_BK;
+  a.part = k.part;
+  a.top = k.tops;
+  a.ztgt = k.ztgt;
+  for (int v0 = 0; v0 < V; v0 += k.piece) {
+    const int n = std::min(k.piece, V - v0);
+    HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, st));
+    HD_TRY(quant ? hd_map(&mw, k.wq, H, n, H, HD_BN) : hd_map(&mw, w, H, V, ldw, HD_BN));
+    a.N = n;
+    a.nt = (n + HD_BN - 1) / HD_BN;
+    a.v0 = v0;
+    a.b_row0 = quant ? 0 : v0;
+    HD_TRY(hd_launch<HD_LOSS>(mx, mw, a, st));
+  }
+  hd_join_kernel<<<(T + 7) / 8, 256, 0, st>>>(k.part, k.tops, T, k.nt, ids, weights, K, V, k.ztgt, loss, lse,
+                                              top);
+  LG_LAUNCH_CHECK("head_join");
+  return LG_OK;
+}
+
+extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, const void* w, long long ldw,
+                                 const void* w_scales, const void* w_biases, int V, const int32_t* ids,
+                                 const float* weights, int K, const float* lse, const float* g, void* dx,
+                                 void* dw, void* workspace, size_t workspace_bytes, void* stream) {
+  HD_TRY(hd_check("head_loss_grad", x, ldx, T, H, w, ldw, w_scales, w_biases, V, ids, K));
+  const bool quant = w_scales != nullptr;
+  LG_CHECK_ARG(dx || dw, "head_loss_grad: neither dx nor dw is asked for");
+  LG_CHECK_ARG(!(dw && quant), "head_loss_grad: a 4-bit head has no gradient");
+  LG_CHECK_ARG(aligned(dx, 16) && aligned(dw, 16), "head_loss_grad: outputs must be 16-byte aligned");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (T == 0) {
+    if (dw) LG_CUDA_TRY(cudaMemsetAsync(dw, 0, (size_t)V * H * 2, st));
+    return LG_OK;
+  }
+  LG_CHECK_ARG(lse && g, "head_loss_grad: NULL pointer");
+  const HdWork k = hd_carve(workspace, T, H, V, K, quant, true, dx != nullptr, dw != nullptr, false);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < k.bytes)
+    return fail(LG_ERR_WORKSPACE, "head_loss_grad: workspace of %zu bytes, need %zu", workspace_bytes,
+                k.bytes);
+  HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
+  CUtensorMap mx, mxt, mw, mwt, mz, mzt;
+  HD_TRY(hd_map(&mx, x, H, T, ldx, HD_BM));
+  if (dw) {
+    hd_rows_kernel<<<hd_blocks((long long)T * (H / 8)), 256, 0, st>>>(
+        static_cast<const __nv_bfloat16*>(x), ldx, T, H, ids, K, V, k.xz);
+    LG_LAUNCH_CHECK("head_rows");
+    HD_TRY(hd_map(&mxt, k.xz, H, T, H, HD_BK));
+  }
+  for (int v0 = 0; v0 < V; v0 += k.piece) {
+    const int n = std::min(k.piece, V - v0);
+    HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, st));
+    const void* wp = quant ? k.wq : w;
+    const long long rows = quant ? n : V, ld = quant ? H : ldw;
+    HdArgs a = hd_args(T, V, K, ids, weights, k);
+    a.v0 = v0;
+    a.b_row0 = quant ? 0 : v0;
+    a.N = n;
+    a.nt = (n + HD_BN - 1) / HD_BN;
+    a.kblocks = (H + HD_BK - 1) / HD_BK;
+    a.lse = lse;
+    a.g = g;
+    a.wsum = k.wsum;
+    a.dz = k.dz;
+    a.ldz = (n + 63) / 64 * 64;
+    HD_TRY(hd_map(&mw, wp, H, rows, ld, HD_BN));
+    HD_TRY(hd_launch<HD_PROB>(mx, mw, a, st));
+    if (dx) {
+      HdArgs b = a;
+      b.N = H;
+      b.nt = (H + HD_BN - 1) / HD_BN;
+      b.kblocks = (n + HD_BK - 1) / HD_BK;
+      b.splits = std::min(k.splits, b.kblocks);
+      b.dx = k.dx;
+      b.add = v0 > 0;
+      HD_TRY(hd_map(&mz, k.dz, n, T, a.ldz, HD_BM));
+      HD_TRY(hd_map(&mwt, wp, H, rows, ld, HD_BK));
+      HD_TRY(hd_launch<HD_XGRAD>(mz, mwt, b, st));
+    }
+    if (dw) {
+      HdArgs b = a;
+      b.M = n;
+      b.mt = (n + HD_BM - 1) / HD_BM;
+      b.N = H;
+      b.nt = (H + HD_BN - 1) / HD_BN;
+      b.kblocks = (T + HD_BK - 1) / HD_BK;
+      b.dw = static_cast<__nv_bfloat16*>(dw);
+      HD_TRY(hd_map(&mzt, k.dz, n, T, a.ldz, HD_BK));
+      HD_TRY(hd_launch<HD_WGRAD>(mzt, mxt, b, st));
+    }
+  }
+  if (dx) {
+    // The last piece may have fewer parts than the first; later parts then kept the earlier sums.
+    const int parts = std::min(k.splits, (std::min(k.piece, V) + HD_BK - 1) / HD_BK);
+    hd_sum_kernel<<<hd_blocks((long long)T * H / 4), 256, 0, st>>>(k.dx, parts, (long long)T * H,
+                                                                  static_cast<__nv_bfloat16*>(dx));
+    LG_LAUNCH_CHECK("head_sum");
+  }
+  return LG_OK;
+}

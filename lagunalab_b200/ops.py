@@ -903,3 +903,125 @@ def stream_attention(q, k_pages, v_pages, table, plan, scale, gate=None, out=Non
     """``prompt_attention`` for one token of each of B streams (q bf16 [B, Hq, 128], ``plan`` from
     ``stream_plan``); the plan's shared prefix is read once for all streams."""
     return _paged_attention("stream", q, k_pages, v_pages, table, plan, scale, gate, out)
+
+
+# ---------------------------------------------------------------------------------------
+# Fitting a model again: the head's loss without its logits (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------
+
+HEAD_TARGETS = 64  # ids a token of head_loss, at most
+
+
+def _rows16(t):
+    """``t`` [n, H] bf16 with rows that TMA reads in place (unit columns, 16-byte steps), or a copy."""
+    n, H = t.shape
+    ld = t.stride(0) if n > 1 else max(t.stride(0), H)
+    if t.stride(1) != 1 or ld % 8 or ld < H or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        ld = H
+    return t, ld
+
+
+def _head_args(who, x, head, ids, weights):
+    """(device index, T, H, V, K, the leading arguments of lg_head_loss and lg_head_loss_grad, what
+    they point to)."""
+    _dev(x)
+    index = x.get_device()
+    if x.dim() != 2 or x.dtype is not _BF16:
+        raise ValueError(f"{who}: x must be bf16 [T, H]")
+    T, H = x.shape
+    if isinstance(head, tuple):
+        q, s, b = (_dev(m) and (m if m.is_contiguous() else m.contiguous()) for m in head)
+        if q.dtype is torch.uint32:
+            q = q.view(_I32)
+        V = q.shape[0]
+        if q.dtype is not _I32 or q.shape != (V, H // 8) or H % 64 or \
+                s.shape != (V, H // 64) or b.shape != s.shape or \
+                s.dtype is not _BF16 or b.dtype is not _BF16:
+            raise ValueError(f"{who}: a 4-bit group-64 head of {H} columns is int32 words [V, {H // 8}], "
+                             f"bf16 scales and biases [V, {H // 64}]")
+        if q.data_ptr() % 16:
+            q = q.clone()
+        keep = (q, s, b)
+        w, ldw, sp, bp = q.data_ptr(), H, s.data_ptr(), b.data_ptr()
+    else:
+        _dev(head)
+        if head.dim() != 2 or head.dtype is not _BF16 or head.shape[1] != H or H % 8:
+            raise ValueError(f"{who}: a head is bf16 [V, {H}] (a multiple of 8) or a 4-bit "
+                             "(words, scales, biases)")
+        V = head.shape[0]
+        head, ldw = _rows16(head)
+        keep = (head,)
+        w, sp, bp = head.data_ptr(), None, None
+    if V < 1:
+        raise ValueError(f"{who}: the head has no rows")
+    if any(m.get_device() != index for m in keep):
+        raise ValueError(f"{who}: the head is not on {x.device}")
+    _dev(ids)
+    if ids.dtype is not _I32 or ids.dim() not in (1, 2) or ids.shape[0] != T or \
+            ids.get_device() != index:
+        raise ValueError(f"{who}: ids must be int32 [{T}] or [{T}, K] on {x.device}")
+    K = 1 if ids.dim() == 1 else ids.shape[1]
+    if not 1 <= K <= HEAD_TARGETS:
+        raise ValueError(f"{who}: {K} targets a token, not 1 to {HEAD_TARGETS}")
+    ids = ids.contiguous()
+    if weights is not None:
+        _dev(weights)
+        if weights.dtype is not torch.float32 or weights.numel() != T * K or \
+                weights.shape[:1] != (T,) or weights.get_device() != index:
+            raise ValueError(f"{who}: weights must be fp32 like ids, {tuple(ids.shape)}, on {x.device}")
+        weights = weights.contiguous()
+    x, ldx = _rows16(x)
+    args = (x.data_ptr(), ldx, T, H, w, ldw, sp, bp, V, ids.data_ptr(), _p(weights), K)
+    return index, T, H, V, K, args, (x, keep, ids, weights)
+
+
+def head_loss(x, head, ids, weights=None, top=False):
+    """Cross entropy of the head's softmax, without its logits: for each row of x bf16 [T, H],
+
+        loss[t] = sum_j weights[t, j] * (lse[t] - z[t, ids[t, j]]),   z = x @ head^T,
+
+    with lse[t] the logarithm of sum_v exp(z[t, v]). ``head``: bf16 [V, H], or a 4-bit group-64 tuple
+    (``QuantizedLinear.mat``), read as the bf16 weights that ``dequantize`` gives. ``ids`` int32 [T], or
+    [T, K] with up to ``HEAD_TARGETS`` a token (a reference's largest probabilities as ``weights``:
+    with sum(p * log p) added, the KL divergence over them); ``weights`` fp32 of the same shape,
+    or None for 1. Negative ids are left out; a token without any other has loss 0, one with an id
+    >= V has loss NaN. Returns (loss, lse) fp32 [T], with ``top`` also the id of each token's
+    largest logit, int32 [T]. Logits and sums are fp32."""
+    index, T, H, V, K, args, keep = _head_args("head_loss", x, head, ids, weights)
+    dev = x.device
+    loss, lse = torch.empty(2, T, dtype=torch.float32, device=dev)
+    ti = torch.empty(T, dtype=_I32, device=dev) if top else None
+    if T:
+        nb = _lib.lib().lg_head_loss_workspace_bytes(T, H, V, K, 4 if args[6] else 16, int(bool(top)))
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)  # of this call alone
+        _call_on(index, _lib.lib().lg_head_loss, *args, loss.data_ptr(), lse.data_ptr(), _p(ti),
+                 ws.data_ptr(), nb)
+    return (loss, lse, ti) if top else (loss, lse)
+
+
+def head_loss_grad(x, head, ids, lse, g, weights=None, dx=True, dw=True):
+    """The gradient of sum(g * loss) for ``head_loss``'s loss, from the same x, head, ids and weights, its
+    ``lse`` and g fp32 [T]: (dx bf16 [T, H] or None, dw bf16 [V, H] or None). A 4-bit head has no
+    gradient (``dw=False``). The vocabulary is taken in pieces: the workspace holds at most 256 MB of
+    the logits' gradient. Tokens without a target give a row of zeros in dx and nothing to dw,
+    whatever their rows of x hold. The logits' gradient is rounded to bf16 for the tensor cores,
+    sums are fp32, results rounded once."""
+    index, T, H, V, K, args, keep = _head_args("head_loss_grad", x, head, ids, weights)
+    if not (dx or dw):
+        raise ValueError("head_loss_grad: neither dx nor dw is asked for")
+    if dw and args[6]:
+        raise ValueError("head_loss_grad: a 4-bit head has no gradient (dw=False)")
+    for t, name in ((lse, "lse"), (g, "g")):
+        _dev(t)
+        if t.dtype is not torch.float32 or t.shape != (T,) or t.get_device() != index:
+            raise ValueError(f"head_loss_grad: {name} must be fp32 [{T}] on {x.device}")
+    lse, g = lse.contiguous(), g.contiguous()
+    gx = torch.empty(T, H, dtype=_BF16, device=x.device) if dx else None
+    gw = torch.empty(V, H, dtype=_BF16, device=x.device) if dw else None
+    nb = _lib.lib().lg_head_loss_grad_workspace_bytes(T, H, V, K, 4 if args[6] else 16, int(bool(dx)),
+                                                      int(bool(dw)))
+    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    _call_on(index, _lib.lib().lg_head_loss_grad, *args, lse.data_ptr(), g.data_ptr(), _p(gx), _p(gw),
+             ws.data_ptr(), nb)
+    return gx, gw

@@ -1,0 +1,317 @@
+"""The head's cross entropy without logits and its gradient against 64 bits, over sizes that end inside
+tiles, both kinds of head, several targets a token, left-out tokens, strides, streams and graphs."""
+import pytest
+import torch
+
+from lagunalab_b200 import ops
+from tests._head_util import dequant64, reference, within
+
+pytestmark = pytest.mark.gpu
+
+
+def make(T, V, H, bits=16, K=1, skip=0.0, seed=0, std=0.05):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    W = torch.randn(V, H, generator=g, device="cuda") * std
+    if bits == 4:
+        head = ops.quantize(W, 64, 4)
+        W = dequant64(head)
+    else:
+        head = W = W.bfloat16()
+    x = torch.randn(T, H, generator=g, device="cuda").bfloat16()
+    ids = torch.randint(0, V, (T, K), generator=g, device="cuda", dtype=torch.int32)
+    ids[torch.rand(T, K, generator=g, device="cuda") < skip] = -1
+    weights = torch.rand(T, K, generator=g, device="cuda") if K > 1 else None
+    gr = torch.randn(T, generator=g, device="cuda")
+    return x, head, W, ids[:, 0].contiguous() if K == 1 else ids, weights, gr
+
+
+def check(x, head, W, ids, weights, g, dw=True):
+    r = reference(x, W, ids, weights, g)
+    loss, lse = ops.head_loss(x, head, ids, weights)
+    within(loss, r["loss"], r["bloss"])
+    within(lse, r["lse"], r["blse"])
+    gx, gw = ops.head_loss_grad(x, head, ids, lse, g, weights, dw=dw)
+    within(gx, r["dx"], r["bdx"])
+    if dw:
+        within(gw, r["dw"], r["bdw"])
+    return r, loss, lse, gx, gw
+
+
+@pytest.mark.parametrize("T,V,H", [(1, 1, 8), (1, 257, 64), (2, 5, 72), (64, 512, 256), (127, 255, 136),
+                                   (128, 256, 64), (129, 1000, 200), (300, 5003, 128), (257, 513, 264),
+                                   (5, 40000, 64), (700, 300, 520)])
+def test_bf16_head(T, V, H):
+    check(*make(T, V, H, seed=T + V))
+
+
+@pytest.mark.parametrize("T,V,H", [(1, 300, 64), (37, 1003, 128), (200, 257, 320), (520, 700, 192)])
+@pytest.mark.parametrize("K", [1, 64])
+def test_4bit_head(T, V, H, K):
+    x, head, W, ids, weights, g = make(T, V, H, bits=4, K=K, skip=0.2, seed=K + T)
+    check(x, head, W, ids, weights, g, dw=False)
+
+
+@pytest.mark.parametrize("T,V,K", [(1, 64, 64), (33, 100, 2), (130, 900, 5), (260, 3, 17), (64, 2000, 63)])
+def test_several_targets(T, V, K):
+    """Few ids, so that the same one is listed twice or more."""
+    check(*make(T, V, 64, K=K, skip=0.3, seed=K))
+
+
+def test_targets_with_unit_weights_are_a_sum_of_losses():
+    x, head, W, ids, _, g = make(50, 200, 64, K=3)
+    check(x, head, W, ids, None, g)
+    loss, lse = ops.head_loss(x, head, ids)
+    one = sum(ops.head_loss(x, head, ids[:, j].contiguous())[0].double() for j in range(3))
+    assert (loss.double() - one).abs().max() < 8 * 2 ** -24 * one.max()
+
+
+def test_one_target_with_a_weight():
+    x, head, W, ids, _, g = make(70, 300, 64, skip=0.2)
+    weights = torch.rand(70, device="cuda")
+    check(x, head, W, ids, weights, g)
+    a, b = ops.head_loss(x, head, ids.view(70, 1), weights.view(70, 1)), ops.head_loss(x, head, ids, weights)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@pytest.mark.parametrize("K", [1, 7])
+def test_tokens_without_a_target_may_hold_anything(K):
+    x, head, W, ids, weights, g = make(200, 700, 128, K=K)
+    clean = x.clone()
+    out = torch.arange(0, 200, 3, device="cuda")
+    ids[out] = -1
+    clean[out] = 0
+    x[out[::2]] = float("nan")
+    x[out[1::2]] = float("inf")
+    r, loss, lse, gx, gw = check(clean, head, W, ids, weights, g)
+    loss2, lse2 = ops.head_loss(x, head, ids, weights)
+    assert torch.equal(loss, loss2) and (loss[out] == 0).all() and lse2[out].isnan().all()
+    gx2, gw2 = ops.head_loss_grad(x, head, ids, lse2, g, weights)
+    assert torch.equal(gx, gx2) and torch.equal(gw, gw2) and (gx2[out] == 0).all()
+
+
+def test_every_token_left_out():
+    x, head, W, ids, _, g = make(130, 300, 64)
+    ids.fill_(-1)
+    loss, lse = ops.head_loss(x, head, ids)
+    gx, gw = ops.head_loss_grad(x, head, ids, lse, g)
+    assert (loss == 0).all() and (gx == 0).all() and (gw == 0).all()
+
+
+@pytest.mark.parametrize("K", [1, 4])
+def test_an_id_past_the_vocabulary(K):
+    """Its token's loss is NaN; in the gradient it counts as left out."""
+    x, head, W, ids, weights, g = make(140, 300, 64, K=K)
+    ids.view(140, K)[17, 0] = 300
+    ids.view(140, K)[18, 0] = 2 ** 31 - 1
+    check(x, head, W, ids, weights, g)
+
+
+def test_a_nan_row_stays_its_own():
+    x, head, W, ids, _, g = make(140, 600, 64)
+    r, loss, lse, gx, _ = check(x, head, W, ids, None, g)
+    x[9] = float("nan")
+    loss2, lse2 = ops.head_loss(x, head, ids)
+    gx2, _ = ops.head_loss_grad(x, head, ids, lse2, g, dw=False)
+    keep = torch.arange(140, device="cuda") != 9
+    assert loss2[9].isnan() and gx2[9].isnan().all()
+    assert torch.equal(loss[keep], loss2[keep]) and torch.equal(gx[keep], gx2[keep])
+
+
+def test_large_logits():
+    """Logits of several hundred: the maximum is taken out before the exponentials."""
+    x, head, W, ids, _, g = make(130, 700, 256, std=4.0)
+    loss, lse = ops.head_loss(x, head, ids)
+    r = reference(x, W, ids, None)
+    # the exponential's argument is up to |z| log2(e), rounded to 2^-24 of itself
+    far = r["lse"].abs().max() * 2 ** -21
+    within(loss, r["loss"], r["bloss"] + far)
+    within(lse, r["lse"], r["blse"] + far)
+
+
+@pytest.mark.parametrize("T,V", [(1, 300), (200, 1000), (3, 1)])
+def test_top(T, V):
+    x, head, W, ids, _, _ = make(T, V, 64)
+    r = reference(x, W, ids, None)
+    loss, lse, top = ops.head_loss(x, head, ids, top=True)
+    z = x.double().cpu() @ W.double().cpu().T
+    got = z.gather(1, top.long().cpu()[:, None])[:, 0]
+    assert (z.amax(1) - got <= 2 * r["blse"]).all()  # the largest, or one as large within fp32
+    a, b = ops.head_loss(x, head, ids)
+    assert torch.equal(a, loss) and torch.equal(b, lse)
+
+
+def test_top_of_equal_logits_is_the_lowest_id():
+    head = torch.zeros(900, 64, dtype=torch.bfloat16, device="cuda")
+    head[[37, 300, 301, 899]] = 1
+    x = torch.ones(150, 64, dtype=torch.bfloat16, device="cuda")
+    x[1] = -1
+    top = ops.head_loss(x, head, torch.zeros(150, dtype=torch.int32, device="cuda"), top=True)[2]
+    assert top[1] == 0 and (top[[0, 2, 149]] == 37).all()
+
+
+def test_strides_and_alignment():
+    x, head, W, ids, _, g = make(140, 500, 64)
+    want = ops.head_loss(x, head, ids)
+    gw = ops.head_loss_grad(x, head, ids, want[1], g)
+    wide = torch.full((140, 80), float("nan"), dtype=torch.bfloat16, device="cuda")
+    wide[:, 8:72] = x
+    odd = torch.full((140 * 65 + 1,), float("nan"), dtype=torch.bfloat16, device="cuda")[1:].view(140, 65)
+    odd[:, :64] = x
+    tall = torch.full((500, 96), float("nan"), dtype=torch.bfloat16, device="cuda")
+    tall[:, :64] = head
+    cases = [(wide[:, 8:72], head), (odd[:, :64], head), (x.t().contiguous().t(), head),
+             (x, tall[:, :64]), (x, head.t().contiguous().t())]
+    for a, b in cases:
+        got = ops.head_loss(a, b, ids)
+        gg = ops.head_loss_grad(a, b, ids, got[1], g)
+        assert all(torch.equal(u, v) for u, v in zip(want + gw, got + gg))
+    every = torch.stack([ids, ids], 1)[:, 0]  # a column
+    assert torch.equal(ops.head_loss(x, head, every)[0], want[0])
+    same = x[:1].expand(140, 64)  # a broadcast row
+    got = ops.head_loss(same, head, ids)[1]
+    assert (got == got[0]).all()
+
+
+def test_no_tokens():
+    x, head, W, ids, _, g = make(4, 300, 64)
+    loss, lse, top = ops.head_loss(x[:0], head, ids[:0], top=True)
+    gx, gw = ops.head_loss_grad(x[:0], head, ids[:0], lse, g[:0])
+    assert loss.shape == lse.shape == top.shape == (0,) and gx.shape == (0, 64) and (gw == 0).all()
+
+
+def test_one_gradient_alone():
+    x, head, W, ids, _, g = make(150, 400, 128)
+    lse = ops.head_loss(x, head, ids)[1]
+    gx, gw = ops.head_loss_grad(x, head, ids, lse, g)
+    assert torch.equal(ops.head_loss_grad(x, head, ids, lse, g, dw=False)[0], gx)
+    assert torch.equal(ops.head_loss_grad(x, head, ids, lse, g, dx=False)[1], gw)
+
+
+def _many(T, V, H, K, dw, bits=16):
+    """Sizes at which the vocabulary is taken in several pieces; the check runs on some rows."""
+    x, head, W, ids, weights, g = make(T, V, H, bits=bits, K=K, skip=0.1, seed=V)
+    loss, lse = ops.head_loss(x, head, ids, weights)
+    gx, gw = ops.head_loss_grad(x, head, ids, lse, g, weights, dw=dw)
+    some = torch.tensor([0, 1, 127, 128, T // 2, T - 1], device="cuda")
+    r = reference(x[some], W, ids[some], None if weights is None else weights[some], g[some])
+    within(loss[some], r["loss"], r["bloss"])
+    within(lse[some], r["lse"], r["blse"])
+    within(gx[some], r["dx"], r["bdx"])
+    if dw:  # columns of the vocabulary on either side of the pieces' ends
+        z = x.double() @ W.double().cuda().T
+        p = torch.exp(z - torch.logsumexp(z, 1, keepdim=True))
+        id2 = ids.view(T, -1).long()
+        w = (torch.ones_like(id2, dtype=torch.float64) if weights is None else weights.double()) * (id2 >= 0)
+        dz = p * w.sum(1, keepdim=True)
+        dz.scatter_add_(1, id2.clamp(min=0), -w)
+        dz *= g.double()[:, None]
+        want = dz.T @ x.double()
+        bound = (2 ** -8 + 2 ** -10) * (dz.abs().T @ x.double().abs()) + 2 ** -8 * want.abs()
+        within(gw, want.cpu(), bound.cpu())
+
+
+@pytest.mark.parametrize("T,V,K", [(4099, 40007, 1), (4099, 33000, 3)])
+def test_vocabulary_in_pieces(T, V, K):
+    _many(T, V, 64, K, True)
+
+
+def test_4bit_vocabulary_in_pieces():
+    _many(257, 40001, 2048, 2, False, bits=4)
+
+
+def test_repeatable():
+    x, head, W, ids, weights, g = make(300, 5000, 256, K=8)
+    first = None
+    for _ in range(4):
+        loss, lse = ops.head_loss(x, head, ids, weights)
+        out = (loss, lse) + ops.head_loss_grad(x, head, ids, lse, g, weights)
+        if first is not None:
+            assert all(torch.equal(a, b) for a, b in zip(first, out))
+        first = out
+
+
+def test_two_streams_at_once():
+    sets = [make(200 + 57 * i, 3000, 128, K=1 + 3 * i, seed=i) for i in range(2)]
+    want = []
+    for x, head, W, ids, weights, g in sets:
+        loss, lse = ops.head_loss(x, head, ids, weights)
+        want.append((loss, lse) + ops.head_loss_grad(x, head, ids, lse, g, weights))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        got = []
+        for st, (x, head, W, ids, weights, g) in zip(streams, sets):
+            with torch.cuda.stream(st):
+                loss, lse = ops.head_loss(x, head, ids, weights)
+                got.append((loss, lse) + ops.head_loss_grad(x, head, ids, lse, g, weights))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_captured_graphs_replayed_with_new_inputs():
+    x, head, W, ids, weights, g = make(150, 2000, 128, K=4)
+    graphs = []
+    ops.head_loss(x, head, ids, weights)
+    for _ in range(2):  # two graphs: neither has the other's workspace
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            loss, lse = ops.head_loss(x, head, ids, weights)
+            out = (loss, lse) + ops.head_loss_grad(x, head, ids, lse, g, weights)
+        graphs.append((gr, out))
+    y = make(150, 2000, 128, K=4, skip=0.5, seed=9)
+    x.copy_(y[0]), ids.copy_(y[3]), weights.copy_(y[4]), g.copy_(y[5])
+    for gr, _ in graphs:
+        gr.replay()
+    loss, lse = ops.head_loss(x, head, ids, weights)
+    want = (loss, lse) + ops.head_loss_grad(x, head, ids, lse, g, weights)
+    for _, out in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+def test_gradient_against_differences():
+    """d loss / d x along a direction, from fp32-accurate losses at two points on either side."""
+    x, head, W, ids, weights, g = make(40, 300, 64, K=3)
+    loss, lse = ops.head_loss(x, head, ids, weights)
+    gx, gw = ops.head_loss_grad(x, head, ids, lse, g, weights)
+    d = torch.randn(40, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * 0.25
+    a, b = (x + d).bfloat16(), (x - d).bfloat16()
+    step = (a.double() - b.double())
+    la, lb = (ops.head_loss(p, head, ids, weights)[0].double() for p in (a, b))
+    want = g.double() * (la - lb)
+    got = (gx.double() * step).sum(1)
+    # third-order term: at most |g| S max|step . (W_v - W_u)|^3 / 24 (the softmax's third cumulant is
+    # below a sixth of the spread cubed); rounding: 2^-8 of the gradient's terms and fp32 of the losses
+    spread = (step @ W.double().cuda().T)
+    spread = spread.amax(1) - spread.amin(1)
+    r = reference(x, W, ids, weights, g)
+    middle = ((a.double() + b.double()) / 2 - x.double()).abs() @ W.double().cuda().abs().amax(0)
+    bound = g.abs().double() * weights.sum(1).double() * (spread ** 3 / 24 + 2 * middle * spread) \
+        + (r["bdx"].cuda() * step.abs()).sum(1) + 2 * g.abs().double() * r["bloss"].cuda() * 2
+    assert ((got - want).abs() <= bound).all()
+
+
+def test_refusals():
+    x, head, W, ids, _, g = make(4, 300, 64)
+    lse = torch.zeros(4, device="cuda")
+    q = ops.quantize(head.float(), 64, 4)
+    bad = [(x.float(), head, ids), (x[0], head, ids), (x, head.float(), ids), (x, head[:, :32], ids),
+           (x, head, ids.long()), (x, head, ids[:3]), (x, head[:0], ids), (x, q[:2] + (q[2][:3],), ids),
+           (x, head, ids.view(4, 1).expand(4, 65)), (x, head, ids.view(4, 1)[:, :0]),
+           (x[:, :12].contiguous(), head[:, :12].contiguous(), ids), (x.cpu(), head, ids),
+           (x, head.cpu(), ids), (x, head, ids.cpu())]
+    for a in bad:
+        with pytest.raises(ValueError):
+            ops.head_loss(*a)
+        with pytest.raises(ValueError):
+            ops.head_loss_grad(*a, lse, g)
+    with pytest.raises(ValueError):
+        ops.head_loss(x, head, ids, torch.ones(4, 2, device="cuda"))
+    with pytest.raises(ValueError, match="4-bit"):
+        ops.head_loss_grad(x, q, ids, lse, g)
+    with pytest.raises(ValueError, match="neither"):
+        ops.head_loss_grad(x, head, ids, lse, g, dx=False, dw=False)
+    with pytest.raises(ValueError, match="lse"):
+        ops.head_loss_grad(x, head, ids, lse[:3], g)
+    with pytest.raises(ValueError, match="g must"):
+        ops.head_loss_grad(x, head, ids, lse, g.double())
