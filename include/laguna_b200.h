@@ -692,6 +692,30 @@ int lg_head_loss_grad(const void* x, long long ldx, int T, int H, const void* w,
                       const float* weights, int K, const float* lse, const float* g, void* dx,
                       void* dw, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * The router's balance loss with its counts. logits fp32 [T, E] and inds int32 [T, k] as lg_router_topk
+ * gives them (a pick outside [0, E) does not count); mask (bytes [T] or NULL: all) keeps a token where it
+ * is not 0, whatever the others' logits hold. With scores s = sigmoid or softmax of the logits and the
+ * N tokens kept:
+ *   counts[e] = picks of e,  probs[e] = mean over tokens of s[t, e] / sum_e s[t, e],
+ *   loss[0] = E sum_e counts[e] / (sum counts) probs[e],  tokens[0] = N;
+ * all 0 where no token is kept. E <= 256, k <= 32. Sums are fp32, in an order that depends on T alone.
+ */
+size_t lg_router_balance_workspace_bytes(int T, int E);
+int lg_router_balance(const float* logits, const int32_t* inds, const uint8_t* mask, int T, int E,
+                      int k, int score_fn, float* loss, int32_t* counts, float* probs, int32_t* tokens,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The gradient of sum_tj dw[t, j] w[t, j] + weight * balance loss with respect to the logits, fp32
+ * [T, E]: w are the routing weights of lg_router_topk before their rounding to bf16 (dw fp32 [T, k], or
+ * NULL: none), counts and tokens are lg_router_balance's (both NULL: no balance loss). Rows of tokens that
+ * the mask leaves out are 0. An expert listed twice among a token's picks gets both gradients.
+ */
+int lg_router_grad(const float* logits, const int32_t* inds, const float* dw, const uint8_t* mask, int T,
+                   int E, int k, int norm_topk_prob, int score_fn, const int32_t* counts,
+                   const int32_t* tokens, float weight, float* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

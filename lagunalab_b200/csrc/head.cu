@@ -773,7 +773,7 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
                                  void* dw, void* workspace, size_t workspace_bytes, void* stream) {
   HD_TRY(hd_check("head_loss_grad", x, ldx, T, H, w, ldw, w_scales, w_biases, V, ids, K));
   const bool quant = w_scales != nullptr;
-  LG_CHECK_ARG(dx || dw, "head_loss_grad: neither dx nor dw is asked for");
+  LG_CHECK_ARG(T == 0 || dx || dw, "head_loss_grad: neither dx nor dw is asked for");
   LG_CHECK_ARG(!(dw && quant), "head_loss_grad: a 4-bit head has no gradient");
   LG_CHECK_ARG(aligned(dx, 16) && aligned(dw, 16), "head_loss_grad: outputs must be 16-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);

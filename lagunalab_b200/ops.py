@@ -8,6 +8,7 @@ as int32.
 """
 import ctypes
 import functools
+from typing import NamedTuple
 
 import torch
 
@@ -906,7 +907,8 @@ def stream_attention(q, k_pages, v_pages, table, plan, scale, gate=None, out=Non
 
 
 # ---------------------------------------------------------------------------------------
-# Fitting a model again: the head's loss without its logits (no counterpart in the reference)
+# Fitting a model again: the head's loss without its logits, the router's balance loss, their
+# gradients (no counterpart in the reference)
 # ---------------------------------------------------------------------------------------
 
 HEAD_TARGETS = 64  # ids a token of head_loss, at most
@@ -1025,3 +1027,77 @@ def head_loss_grad(x, head, ids, lse, g, weights=None, dx=True, dw=True):
     _call_on(index, _lib.lib().lg_head_loss_grad, *args, lse.data_ptr(), g.data_ptr(), _p(gx), _p(gw),
              ws.data_ptr(), nb)
     return gx, gw
+
+
+class RouterBalance(NamedTuple):
+    """``router_balance``'s results, on the device."""
+    loss: torch.Tensor    # fp32 [1]
+    counts: torch.Tensor  # int32 [E], picks of each expert
+    probs: torch.Tensor   # fp32 [E], mean share of the scores
+    tokens: torch.Tensor  # int32 [1], tokens that the mask keeps
+
+
+_SCORES = {"sigmoid": _lib.LG_SCORE_SIGMOID, "softmax": _lib.LG_SCORE_SOFTMAX}
+
+
+def _router_args(who, logits, inds, score_fn, mask):
+    """(device index, T, E, k, logits, inds, mask), checked and contiguous."""
+    _dev(logits)
+    index = logits.get_device()
+    if logits.dim() != 2 or logits.dtype is not torch.float32:
+        raise ValueError(f"{who}: logits must be fp32 [T, E]")
+    T, E = logits.shape
+    _dev(inds)
+    if inds.dim() != 2 or inds.dtype is not _I32 or inds.shape[0] != T or inds.get_device() != index:
+        raise ValueError(f"{who}: inds must be int32 [{T}, k] on {logits.device}")
+    if score_fn not in _SCORES:
+        raise ValueError(f"{who}: score_fn {score_fn!r} is neither 'sigmoid' nor 'softmax'")
+    if mask is not None:
+        _dev(mask)
+        if mask.dtype is not torch.bool or mask.shape != (T,) or mask.get_device() != index:
+            raise ValueError(f"{who}: mask must be bool [{T}] on {logits.device}")
+        mask = mask.contiguous()
+    return index, T, E, inds.shape[1], logits.contiguous(), inds.contiguous(), mask
+
+
+def router_balance(logits, inds, score_fn="sigmoid", mask=None):
+    """The balance loss of a batch's routing and its per-expert counts, from ``router_topk``'s logits fp32
+    [T, E] and picks int32 [T, k]: ``E * sum(share of picks * mean share of scores)``, 1 where
+    both are even, over the tokens that ``mask`` (bool [T]) keeps; what masked rows hold does not matter. Returns a
+    ``RouterBalance``; its gradient is ``router_grad``'s, through the scores (counts have none)."""
+    index, T, E, k, logits, inds, mask = _router_args("router_balance", logits, inds, score_fn, mask)
+    dev = logits.device
+    real = torch.empty(1 + E, dtype=torch.float32, device=dev)
+    whole = torch.empty(1 + E, dtype=_I32, device=dev)
+    nb = _lib.lib().lg_router_balance_workspace_bytes(T, E)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    fp, wp = real.data_ptr(), whole.data_ptr()
+    _call_on(index, _lib.lib().lg_router_balance, logits.data_ptr(), inds.data_ptr(), _p(mask), T, E, k,
+             _SCORES[score_fn], fp, wp + 4, fp + 4, wp, ws.data_ptr(), nb)
+    return RouterBalance(real[:1], whole[1:], real[1:], whole[:1])
+
+
+def router_grad(logits, inds, dw=None, norm_topk_prob=True, score_fn="sigmoid", balance=None,
+                balance_weight=0.0, mask=None):
+    """The gradient with respect to the router's logits, fp32 [T, E]: of ``sum(dw * w)`` for the routing
+    weights w that ``router_topk`` gives (dw fp32 [T, k], straight through their rounding to bf16), plus
+    ``balance_weight`` times the balance loss whose ``RouterBalance`` is given. Rows that ``mask`` leaves
+    out are 0. The router's weight then has ``dlogits.t() @ x``."""
+    index, T, E, k, logits, inds, mask = _router_args("router_grad", logits, inds, score_fn, mask)
+    if dw is None and balance is None:
+        raise ValueError("router_grad: neither dw nor a balance loss")
+    if dw is not None:
+        _dev(dw)
+        if dw.dtype is not torch.float32 or dw.shape != inds.shape or dw.get_device() != index:
+            raise ValueError(f"router_grad: dw must be fp32 {tuple(inds.shape)} on {logits.device}")
+        dw = dw.contiguous()
+    counts = tokens = None
+    if balance is not None:
+        _, counts, _, tokens = balance
+        if _i32(counts, "counts", 1, index) != (E,) or _i32(tokens, "tokens", 1, index) != (1,):
+            raise ValueError(f"router_grad: the balance is not of {E} experts")
+    out = torch.empty(T, E, dtype=torch.float32, device=logits.device)
+    _call_on(index, _lib.lib().lg_router_grad, logits.data_ptr(), inds.data_ptr(), _p(dw), _p(mask), T, E, k,
+             int(bool(norm_topk_prob)), _SCORES[score_fn], _p(counts), _p(tokens), float(balance_weight),
+             out.data_ptr())
+    return out

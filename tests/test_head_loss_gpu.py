@@ -177,6 +177,8 @@ def test_no_tokens():
     loss, lse, top = ops.head_loss(x[:0], head, ids[:0], top=True)
     gx, gw = ops.head_loss_grad(x[:0], head, ids[:0], lse, g[:0])
     assert loss.shape == lse.shape == top.shape == (0,) and gx.shape == (0, 64) and (gw == 0).all()
+    gx, gw = ops.head_loss_grad(x[:0], head, ids[:0], lse, g[:0], dw=False)
+    assert gx.shape == (0, 64) and gw is None
 
 
 def test_one_gradient_alone():
