@@ -21,8 +21,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "common.cuh"
-#include "tc_ptx.cuh"
+#include "head.cuh"
 #include "tmap.cuh"
 
 namespace lg {
@@ -39,8 +38,6 @@ constexpr int HD_B_BYTES = HD_BN * HD_BK * 2;  // 32 KB
 constexpr int HD_STAGE_BYTES = HD_A_BYTES + HD_B_BYTES;
 constexpr int HD_BOX = 64 * HD_BK * 2;  // an MN-major box: 64 K rows of 64 elements
 constexpr size_t HD_SMEM = 1024 + (size_t)HD_STAGES * HD_STAGE_BYTES + 256;
-constexpr int HD_MAXK = 64;
-constexpr float HD_LOG2E = 1.4426950408889634f;
 
 struct HdArgs {
   int M, N;          // rows of the output tile grid, and its columns
@@ -57,9 +54,7 @@ struct HdArgs {
   const unsigned char* start;  // K > 1: [T, nt_all + 1] first sorted id of each vocabulary tile
   int nt_all;
   // HD_LOSS
-  float2* part;  // [T, nt_all] (maximum, sum)
-  int* top;      // [T, nt_all] the maximum's id, or NULL
-  float* ztgt;   // [T, K]
+  HdParts out;  // a part a tile of 256 ids
   // HD_PROB
   const float* lse;
   const float* g;
@@ -73,27 +68,9 @@ struct HdArgs {
   __nv_bfloat16* dw;  // [V, H]
 };
 
-__device__ __forceinline__ float hd_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// v[c] with a runtime c, by selects (registers have no index).
-__device__ __forceinline__ float hd_pick(const float (&v)[32], int c) {
-  float r = 0.f;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) r = i == c ? v[i] : r;
-  return r;
-}
 __device__ __forceinline__ void hd_sub(float (&v)[32], int c, float w) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = i == c ? v[i] - w : v[i];
-}
-
-__device__ __forceinline__ uint32_t hd_pack(float a, float b) {
-  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
 }
 
 // A unit of work: tile (m, n) of the output, and the part [k0, k1) of the contraction's blocks.
@@ -160,17 +137,17 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
         while ((unsigned)next - (unsigned)id0 < 32u) {
           const float z = hd_pick(v, next - id0);
           if (a.K == 1) {
-            a.ztgt[t] = z;
+            a.out.ztgt[t] = z;
             break;
           }
-          a.ztgt[row_k + a.order[row_k + p]] = z;
+          a.out.ztgt[row_k + a.order[row_k + p]] = z;
           next = ++p < p1 ? a.ids[row_k + p] : -1;
         }
         float cm = v[0];
 #pragma unroll
         for (int i = 1; i < 32; ++i) cm = fmaxf(cm, v[i]);
         if (cm > mx) {
-          if (a.top) {
+          if (a.out.top) {
             int at = 0;
 #pragma unroll
             for (int i = 31; i >= 0; --i) at = v[i] == cm ? i : at;
@@ -189,8 +166,8 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
         sum += s0 + s1;
       }
       if (live) {
-        a.part[(size_t)t * a.nt_all + ntile] = make_float2(mx, ok ? sum : nan);
-        if (a.top) a.top[(size_t)t * a.nt_all + ntile] = arg;
+        a.out.part[(size_t)t * a.nt_all + ntile] = make_float2(mx, ok ? sum : nan);
+        if (a.out.top) a.out.top[(size_t)t * a.nt_all + ntile] = arg;
       }
     } else {
       float gs = 0.f, gg = 0.f, off = 0.f;
@@ -423,6 +400,14 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
   if (warp == 2) tmem_dealloc(tmem, 512);
 }
 
+// The eight weights of a word: bf16(scale * code + bias).
+__device__ __forceinline__ void hd_unpack(uint32_t q, float scale, float bias, uint32_t (&r)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    r[j] = hd_pack(fmaf(scale, (float)((q >> (8 * j)) & 15u), bias),
+                   fmaf(scale, (float)((q >> (8 * j + 4)) & 15u), bias));
+}
+
 // ---- small kernels ------------------------------------------------------------------------------
 
 // K > 1: a warp sorts a token's ids (those in [0, V), ascending, equal ones in their order), with each
@@ -463,23 +448,58 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
   if (lane == 0) wsum[t] = sum;
 }
 
-// A warp joins a token's tiles: lse, the loss, and the id of the largest logit.
-__global__ void __launch_bounds__(256) hd_join_kernel(const float2* __restrict__ part,
-                                                      const int* __restrict__ tops, int T, int nt,
+// sum_h x_h W_vh of one row each by a warp, in fp32 with each sum rounded to nearest.
+__device__ __forceinline__ float hd_dot(const HdHead& w, const __nv_bfloat16* x, int H, int v) {
+  const int lane = threadIdx.x & 31;
+  float s = 0.f;
+  for (int c = lane * 8; c < H; c += 256) {
+    const uint4 xv = *reinterpret_cast<const uint4*>(x + c);
+    const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
+    uint32_t ws[4];
+    if (w.scales) {
+      const uint32_t q = static_cast<const uint32_t*>(w.w)[(size_t)v * (H / 8) + c / 8];
+      const size_t g = (size_t)v * (H / 64) + c / 64;
+      hd_unpack(q, bf2f(w.scales[g]), bf2f(w.biases[g]), ws);
+    } else {
+      const uint4 wv = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w.w) + (size_t)v * w.ld + c);
+      ws[0] = wv.x;
+      ws[1] = wv.y;
+      ws[2] = wv.z;
+      ws[3] = wv.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ws[i] << 16), s);
+      s = fmaf(__uint_as_float(xs[i] & 0xffff0000u), __uint_as_float(ws[i] & 0xffff0000u), s);
+    }
+  }
+  return warp_sum(s);
+}
+
+// A warp joins a token's parts (maximum, sum of exponentials, the maximum's id): lse, the loss, the id of the
+// largest logit.
+//
+// The tensor cores' accumulators are cut, not rounded, after each step: a logit of 11 that H = 2048 like-signed
+// products make is 1e-5 too small, more than all other errors together (loss off by 1.5e-6 in the 2-norm
+// against 64 bits, 3e-7 with an fp32 product). The logits of targets with an eighth or more of the token's
+// weight are therefore summed again here, in fp32 rounded to nearest, and take their first value's
+// place in lse too.
+__global__ void __launch_bounds__(256) hd_join_kernel(HdParts in, int T, const __nv_bfloat16* __restrict__ x,
+                                                      long long ldx, int H, HdHead w,
                                                       const int* __restrict__ ids,
                                                       const float* __restrict__ weights, int K, int V,
-                                                      const float* __restrict__ ztgt,
                                                       float* __restrict__ loss,
                                                       float* __restrict__ lse_out,
                                                       int* __restrict__ top) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x * 8 + warp;
   if (t >= T) return;
-  const float2* row = part + (size_t)t * nt;
+  const int parts = in.parts;
+  const float2* row = in.part + (size_t)t * parts;
   float mx = -INFINITY, sum = 0.f;
   int at = -1;
 #pragma unroll 4
-  for (int n = lane; n < nt; n += 32) {
+  for (int n = lane; n < parts; n += 32) {
     const float2 v = row[n];
     if (v.x > mx) {
       sum = sum * hd_ex2((mx - v.x) * HD_LOG2E) + v.y;
@@ -489,33 +509,67 @@ __global__ void __launch_bounds__(256) hd_join_kernel(const float2* __restrict__
       sum += v.x == -INFINITY ? v.y : v.y * hd_ex2((v.x - mx) * HD_LOG2E);
     }
   }
+  int arg = top && at >= 0 ? in.top[(size_t)t * parts + at] : 0x7fffffff;
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, mx, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
-    const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
+    const int a2 = __shfl_xor_sync(0xffffffffu, arg, o);
     const float m = fmaxf(mx, m2);
     const float ea = mx == m ? 1.f : hd_ex2((mx - m) * HD_LOG2E);
     const float eb = m2 == m ? 1.f : hd_ex2((m2 - m) * HD_LOG2E);
     // Both lanes of a pair add in the same order, the lower lane's part first.
     sum = (lane & o) ? s2 * eb + sum * ea : sum * ea + s2 * eb;
-    at = m2 > mx || (m2 == mx && (unsigned)a2 < (unsigned)at) ? a2 : at;
+    arg = m2 > mx || (m2 == mx && a2 < arg) ? a2 : arg;
     mx = m;
   }
-  const float lse = __shfl_sync(0xffffffffu, mx + logf(sum), 0);
-  float l = 0.f;
+  sum = __shfl_sync(0xffffffffu, sum, 0);
+  // the targets: two a lane
+  int id[2];
+  float wt[2], z[2];
+  float all = 0.f;
   bool bad = false;
-  for (int j = lane; j < K; j += 32) {
-    const int id = ids[(size_t)t * K + j];
-    if (id >= V) bad = true;
-    if (id < 0 || id >= V) continue;
-    l += (weights ? weights[(size_t)t * K + j] : 1.f) * (lse - ztgt[(size_t)t * K + j]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int j = lane + 32 * i;
+    id[i] = j < K ? ids[(size_t)t * K + j] : -1;
+    if (id[i] >= V) {
+      bad = true;
+      id[i] = -1;
+    }
+    wt[i] = id[i] < 0 ? 0.f : weights ? weights[(size_t)t * K + j] : 1.f;
+    z[i] = id[i] < 0 ? 0.f : in.ztgt[(size_t)t * K + j];
+    all += fabsf(wt[i]);
   }
+  all = warp_sum(all);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    unsigned todo = __ballot_sync(0xffffffffu, id[i] >= 0 && 8.f * fabsf(wt[i]) >= all);
+    while (todo) {
+      const int src = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const int v = __shfl_sync(0xffffffffu, id[i], src);
+      const float was = __shfl_sync(0xffffffffu, z[i], src);
+      const float now = hd_dot(w, x + (size_t)t * ldx, H, v);
+      sum += hd_ex2((now - mx) * HD_LOG2E) - hd_ex2((was - mx) * HD_LOG2E);
+      // every place of the list that names it: once in the sum
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (id[u] == v) z[u] = now;
+      todo &= ~__ballot_sync(0xffffffffu, id[i] == v);
+      if (i == 0 && id[1] == v) id[1] = -2;  // summed already
+    }
+  }
+  const float lse = mx + logf(sum);
+  float l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (id[i] != -1) l += wt[i] * (lse - z[i]);
   l = warp_sum(l);
   bad = __any_sync(0xffffffffu, bad);
   if (lane == 0) {
     loss[t] = bad ? __int_as_float(0x7fffffff) : l;
     lse_out[t] = lse;
-    if (top) top[t] = at >= 0 ? tops[(size_t)t * nt + at] : 0;
+    if (top) top[t] = arg == 0x7fffffff ? 0 : arg;
   }
 }
 
@@ -544,13 +598,8 @@ __global__ void __launch_bounds__(256) hd_dequant_kernel(const uint32_t* __restr
                                                          const __nv_bfloat16* __restrict__ b,
                                                          long long words, __nv_bfloat16* __restrict__ out) {
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < words; i += gridDim.x * 256LL) {
-    const uint32_t w = q[i];
-    const float sc = bf2f(s[i >> 3]), bi = bf2f(b[i >> 3]);
     uint32_t r[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      r[j] = hd_pack(fmaf(sc, (float)((w >> (8 * j)) & 15u), bi),
-                     fmaf(sc, (float)((w >> (8 * j + 4)) & 15u), bi));
+    hd_unpack(q[i], bf2f(s[i >> 3]), bf2f(b[i >> 3]), r);
     *reinterpret_cast<uint4*>(out + 8 * i) = make_uint4(r[0], r[1], r[2], r[3]);
   }
 }
@@ -590,9 +639,8 @@ static int hd_splits(int T, int H, int piece) {
 }
 
 struct HdWork {
-  float2* part;
-  int* tops;
-  float* ztgt;
+  HdParts out;
+  __nv_bfloat16* xp;  // few tokens and 4 bits: x in the order of a word's codes
   int* sorted;
   unsigned char *order, *start;
   float* wsum;
@@ -602,16 +650,22 @@ struct HdWork {
   int piece, nt, splits;
 };
 
-static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool grad, bool dx, bool dw,
-                       bool top) {
+static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool few, bool grad, bool dx,
+                       bool dw, bool top) {
   HdWork w = {};
   Carver c(base);
   w.nt = (V + HD_BN - 1) / HD_BN;
   w.piece = hd_piece(T, H, V, quant, grad);
   if (!grad) {
-    w.part = c.take<float2>((size_t)T * w.nt);
-    if (top) w.tops = c.take<int>((size_t)T * w.nt);
-    w.ztgt = c.take<float>((size_t)T * K);
+    w.out.parts = few ? hq_parts(V) : w.nt;
+    w.out.part = c.take<float2>((size_t)T * w.out.parts);
+    if (top) w.out.top = c.take<int>((size_t)T * w.out.parts);
+    w.out.ztgt = c.take<float>((size_t)T * K);
+    if (few) {
+      w.xp = c.take<__nv_bfloat16>((size_t)T * H);
+      w.bytes = align_up(c.used, 256);
+      return w;
+    }
   }
   if (K > 1) {
     w.sorted = c.take<int>((size_t)T * K);
@@ -723,12 +777,18 @@ using namespace lg;
 
 extern "C" size_t lg_head_loss_workspace_bytes(int T, int H, int V, int K, int bits, int top) {
   if (T < 1 || H < 8 || V < 1 || K < 1) return 256;
-  return hd_carve(nullptr, T, H, V, K, bits == 4, false, false, false, top != 0).bytes;
+  // The larger of the two ways: which one a 4-bit head takes also depends on its pointers.
+  const bool quant = bits == 4;
+  const size_t n = hd_carve(nullptr, T, H, V, K, quant, false, false, false, false, top != 0).bytes;
+  if (!quant) return n;
+  const HdHead head = {nullptr, nullptr, nullptr, H};
+  if (!hq_takes(T, H, V, K, head)) return n;
+  return std::max(n, hd_carve(nullptr, T, H, V, K, true, true, false, false, false, top != 0).bytes);
 }
 
 extern "C" size_t lg_head_loss_grad_workspace_bytes(int T, int H, int V, int K, int bits, int dx, int dw) {
   if (T < 1 || H < 8 || V < 1 || K < 1) return 256;
-  return hd_carve(nullptr, T, H, V, K, bits == 4, true, dx != 0, dw != 0, false).bytes;
+  return hd_carve(nullptr, T, H, V, K, bits == 4, false, true, dx != 0, dw != 0, false).bytes;
 }
 
 extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const void* w, long long ldw,
@@ -739,30 +799,35 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
   if (T == 0) return LG_OK;
   LG_CHECK_ARG(loss && lse, "head_loss: NULL output");
   const bool quant = w_scales != nullptr;
-  const HdWork k = hd_carve(workspace, T, H, V, K, quant, false, false, false, top != nullptr);
+  const HdHead head = {w, static_cast<const __nv_bfloat16*>(w_scales),
+                       static_cast<const __nv_bfloat16*>(w_biases), ldw};
+  const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);
+  const bool few = quant && hq_takes(T, H, V, K, head);
+  const HdWork k = hd_carve(workspace, T, H, V, K, quant, few, false, false, false, top != nullptr);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < k.bytes)
     return fail(LG_ERR_WORKSPACE, "head_loss: workspace of %zu bytes, need %zu", workspace_bytes, k.bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
-  CUtensorMap mx, mw;
-  HD_TRY(hd_map(&mx, x, H, T, ldx, HD_BM));
-  HdArgs a = hd_args(T, V, K, ids, weights, k);
-  a.kblocks = (H + HD_BK - 1) / HD_BK;
-  a.part = k.part;
-  a.top = k.tops;
-  a.ztgt = k.ztgt;
-  for (int v0 = 0; v0 < V; v0 += k.piece) {
-    const int n = std::min(k.piece, V - v0);
-    HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, st));
-    HD_TRY(quant ? hd_map(&mw, k.wq, H, n, H, HD_BN) : hd_map(&mw, w, H, V, ldw, HD_BN));
-    a.N = n;
-    a.nt = (n + HD_BN - 1) / HD_BN;
-    a.v0 = v0;
-    a.b_row0 = quant ? 0 : v0;
-    HD_TRY(hd_launch<HD_LOSS>(mx, mw, a, st));
+  if (few) {
+    HD_TRY(hq_loss_parts(xb, ldx, T, H, head, V, ids, K, k.xp, k.out, st));
+  } else {
+    HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
+    CUtensorMap mx, mw;
+    HD_TRY(hd_map(&mx, x, H, T, ldx, HD_BM));
+    HdArgs a = hd_args(T, V, K, ids, weights, k);
+    a.kblocks = (H + HD_BK - 1) / HD_BK;
+    a.out = k.out;
+    for (int v0 = 0; v0 < V; v0 += k.piece) {
+      const int n = std::min(k.piece, V - v0);
+      HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, st));
+      HD_TRY(quant ? hd_map(&mw, k.wq, H, n, H, HD_BN) : hd_map(&mw, w, H, V, ldw, HD_BN));
+      a.N = n;
+      a.nt = (n + HD_BN - 1) / HD_BN;
+      a.v0 = v0;
+      a.b_row0 = quant ? 0 : v0;
+      HD_TRY(hd_launch<HD_LOSS>(mx, mw, a, st));
+    }
   }
-  hd_join_kernel<<<(T + 7) / 8, 256, 0, st>>>(k.part, k.tops, T, k.nt, ids, weights, K, V, k.ztgt, loss, lse,
-                                              top);
+  hd_join_kernel<<<(T + 7) / 8, 256, 0, st>>>(k.out, T, xb, ldx, H, head, ids, weights, K, V, loss, lse, top);
   LG_LAUNCH_CHECK("head_join");
   return LG_OK;
 }
@@ -782,7 +847,7 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     return LG_OK;
   }
   LG_CHECK_ARG(lse && g, "head_loss_grad: NULL pointer");
-  const HdWork k = hd_carve(workspace, T, H, V, K, quant, true, dx != nullptr, dw != nullptr, false);
+  const HdWork k = hd_carve(workspace, T, H, V, K, quant, false, true, dx != nullptr, dw != nullptr, false);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < k.bytes)
     return fail(LG_ERR_WORKSPACE, "head_loss_grad: workspace of %zu bytes, need %zu", workspace_bytes,
                 k.bytes);

@@ -1,0 +1,527 @@
+// The head's loss for few tokens (up to 128) from 4-bit weights that never become bf16 in memory.
+//
+// z^T = W x^T in tiles of 128 vocabulary ids (the rows, M) by the tokens (the columns, N = T rounded up to 16):
+// the weights are the product's A operand, taken from TMEM, where the warps that unpack them write them; x is B.
+// So few tokens cost few columns, and an unpacked weight crosses neither memory nor shared memory.
+//
+//   warp 0       TMA: packed words (32 rows x 256 codes a box, 128-byte swizzle), scales and biases
+//   warp 2       TMA: x, 64 columns a slot
+//   warps 4-11   unpack: a row a thread, 64 codes at a time (a quantization group), two groups of four warps
+//                in turns: code + 128 as bf16 by one LOP3 a pair, - 128, * scale + bias in packed bf16 with one
+//                rounding; tcgen05.st of 32 columns
+//   warp 1       four products (M 128, N, K 16) a slot into one of two accumulators
+//   warps 12-15  per tile and token the maximum and the sum of exponentials over the warp's 32 rows, which lie
+//                across its lanes: a transposing reduction (31 shuffles for 32 columns) leaves token i with lane i
+//
+// K order: one LOP3 splits a word into the pairs (0,4), (1,5), (2,6), (3,7); x is copied in that order first
+// (hq_order_kernel), so that no code is moved.
+//
+// Each CTA has 1/148 of the blocks of 32 ids. What is bound: HBM (0.56 bytes a weight); the unpacking's
+// instructions take about as long (2 a weight).
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "head.cuh"
+#include "tmap.cuh"
+
+namespace lg {
+
+using namespace tc;
+
+constexpr int HQ_MAXT = 128;
+constexpr int HQ_THREADS = 512;
+constexpr int HQ_BLOCK = 32;               // ids a block: a warp's TMEM lanes
+constexpr int HQ_W_BYTES = 4 * 32 * 128;   // a stage of packed words: 128 rows x 256 codes
+constexpr int HQ_SMEM_MAX = 232448;
+
+struct HqArgs {
+  int T, N, H, V, K;
+  int kb;       // 64-wide blocks of H
+  int blocks;   // blocks of 32 ids
+  int xs, ws;   // slots of x (and of unpacked weights), stages of packed words
+  int sc_bytes;  // scales of a tile, a multiple of 512
+  const int* ids;
+  HdParts out;
+};
+
+__host__ __device__ __forceinline__ int hq_x_bytes(int N) { return (N * 128 + 1023) / 1024 * 1024; }
+
+// A[tmem] B[smem]: M 128 x N x 16.
+__device__ __forceinline__ void hq_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void hq_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+      "%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// Codes 4 i and 4 i + 16 of v (already shifted) -> bf16 pair scale * code + bias.
+__device__ __forceinline__ uint32_t hq_pair(uint32_t v, uint32_t s2, uint32_t b2) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 c;\n\t"
+      "lop3.b32 c, %1, 0x000F000F, 0x43004300, 0xEA;\n\t"
+      "sub.rn.bf16x2 c, c, %4;\n\t"
+      "fma.rn.bf16x2 %0, c, %2, %3;\n\t}"
+      : "=r"(r)
+      : "r"(v), "r"(s2), "r"(b2), "r"(0x43004300u));
+  return r;
+}
+
+// Over the warp's lanes: lane i ends with op over all lanes of v[i].
+template <typename Op>
+__device__ __forceinline__ float hq_across(float (&v)[32], Op op) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+      v[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, o));
+    }
+  }
+  return v[0];
+}
+
+template <int NT>  // blocks of 32 tokens
+__global__ void __launch_bounds__(HQ_THREADS, 1)
+    hq_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap ms,
+              const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mx, const HqArgs a) {
+  extern __shared__ uint8_t hq_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)hq_raw + 1023) & ~(uintptr_t)1023);
+  const int x_bytes = hq_x_bytes(a.N);
+  uint8_t* sm_w = smem;
+  uint8_t* sm_x = sm_w + a.ws * HQ_W_BYTES;
+  uint8_t* sm_s = sm_x + a.xs * x_bytes;        // [2][scales, biases]
+  int* sm_id = reinterpret_cast<int*>(sm_s + 4 * a.sc_bytes);  // [K][32 NT]
+  float* sm_m = reinterpret_cast<float*>(sm_id + a.K * 32 * NT);
+  float* sm_sum = sm_m + 4 * 32 * NT;
+  int* sm_top = reinterpret_cast<int*>(sm_sum + 4 * 32 * NT);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm_top + 4 * 32 * NT);
+  uint64_t *w_full = bars, *w_empty = bars + 8, *full = bars + 16, *empty = bars + 24;
+  uint64_t *s_full = bars + 32, *s_empty = bars + 34, *acc_full = bars + 36, *acc_empty = bars + 38;
+  uint64_t* done = bars + 40;
+  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(bars + 41);
+  int* err = reinterpret_cast<int*>(tmem_base + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b0 = (int)((long long)a.blocks * blockIdx.x / gridDim.x);
+  const int b1 = (int)((long long)a.blocks * (blockIdx.x + 1) / gridDim.x);
+  const int tiles = (b1 - b0 + 3) / 4;
+  const int stages = (a.kb + 3) / 4;  // of packed words, a tile
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.ws; ++i) {
+      mbar_init(w_full + i, 1);
+      mbar_init(w_empty + i, 8);
+    }
+    for (int i = 0; i < a.xs; ++i) {
+      mbar_init(full + i, 5);  // x's copy and four warps
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(s_empty + i, 8);
+      mbar_init(acc_full + i, 1);
+      mbar_init(acc_empty + i, 4);
+    }
+    mbar_init(done, 1);
+    for (int i = 0; i < 4; ++i) err[i] = 0;  // of all roles; of the two copies' ends; of the products' end
+    fence_mbar_init();
+    prefetch_tmap(&mw);
+    prefetch_tmap(&ms);
+    prefetch_tmap(&mb);
+    prefetch_tmap(&mx);
+  }
+  if (warp == 3) {
+    tmem_alloc(tmem_base, 512);
+    tmem_relinquish();
+  }
+  for (int i = threadIdx.x; i < a.K * 32 * NT; i += HQ_THREADS) {
+    const int t = i % (32 * NT), j = i / (32 * NT);
+    sm_id[i] = t < a.T ? a.ids[(size_t)t * a.K + j] : -1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_base;        // accumulators: columns [0, 64 NT)
+  const uint32_t tmem_a = tmem + 256;      // weights: 32 columns a slot
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int st = 0, used = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      int i = 0;
+      for (; i < tiles && ok; ++i) {
+        const int row = (b0 + 4 * i) * HQ_BLOCK, nb = min(4, b1 - b0 - 4 * i);
+        const int sb = i & 1;
+        if (!mbar_wait(s_empty + sb, ((i >> 1) & 1) ^ 1, err, 1)) break;
+        const int groups = nb * HQ_BLOCK * a.kb, boxes = (groups + 255) / 256;
+        mbar_arrive_expect_tx(s_full + sb, 2 * boxes * 512);
+        uint8_t* s = sm_s + sb * 2 * a.sc_bytes;
+        for (int j = 0; j < boxes; ++j) {
+          tma_load_2d(s + j * 512, &ms, s_full + sb, row * a.kb + j * 256, 0);
+          tma_load_2d(s + a.sc_bytes + j * 512, &mb, s_full + sb, row * a.kb + j * 256, 0);
+        }
+        for (int k = 0; k < stages; ++k) {
+          if (!mbar_wait(w_empty + st, ph ^ 1, err, 2)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(w_full + st, nb * 4096);
+          for (int j = 0; j < nb; ++j)
+            tma_load_2d(sm_w + st * HQ_W_BYTES + j * 4096, &mw, w_full + st, k * 32, row + j * HQ_BLOCK);
+          if (used < a.ws) ++used;
+          if (++st == a.ws) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      // Every copy has landed before the CTA ends.
+      for (int j = used; j > 0; --j) {
+        const int s = (st - j + a.ws) % a.ws;
+        mbar_wait(w_full + s, s < st ? ph : ph ^ 1, err + 1, 2, 400000000LL);
+      }
+      for (int j = max(0, i - 2); j < i; ++j)
+        mbar_wait(s_full + (j & 1), (j >> 1) & 1, err + 1, 1, 400000000LL);
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    if (lane == 0) {
+      int st = 0, used = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int i = 0; i < tiles && ok; ++i) {
+        for (int k = 0; k < a.kb; ++k) {
+          if (!mbar_wait(empty + st, ph ^ 1, err, 3)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(full + st, a.N * 128);
+          tma_load_2d(sm_x + st * x_bytes, &mx, full + st, k * 64, 0);
+          if (used < a.xs) ++used;
+          if (++st == a.xs) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      for (int j = used; j > 0; --j) {
+        const int s = (st - j + a.xs) % a.xs;
+        mbar_wait(full + s, s < st ? ph : ph ^ 1, err + 2, 3, 400000000LL);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_bf16(128, a.N);
+      const uint64_t hi = (uint64_t)SW128_HI << 32;
+      int st = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int acc = i & 1;
+        if (!mbar_wait(acc_empty + acc, ((i >> 1) & 1) ^ 1, err, 4)) break;
+        tc_fence_after();
+        for (int k = 0; k < a.kb; ++k) {
+          if (!mbar_wait(full + st, ph, err, 5)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t db = sw128_lo(smem_u32(sm_x + st * x_bytes));
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            hq_mma(tmem + acc * 32 * NT, tmem_a + st * 32 + j * 8, hi | (db + j * 2), idesc, k > 0 || j > 0);
+          umma_commit(empty + st);
+          if (++st == a.xs) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+        if (ok) umma_commit(acc_full + acc);
+      }
+      umma_commit(done);
+    }
+    __syncwarp();
+  } else if (warp >= 4 && warp < 12) {
+    // Block n of all tiles' blocks is unpacked by the four warps of parity n.
+    const int q = warp & 3, turn = (warp >> 2) & 1;  // warps 4 to 7: 1, 8 to 11: 0
+    const int r = q * 32 + lane;
+    const uint32_t lanes = (uint32_t)(q * 32) << 16;
+    int n = 0, slot = 0, ws = 0;
+    uint32_t ph = 0, wph = 0;
+    bool ok = true;
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int nb = min(4, b1 - b0 - 4 * i), sb = i & 1;
+      const bool mine = q < nb;
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full + sb, (i >> 1) & 1, err, 6));
+      const uint8_t* sc = sm_s + sb * 2 * a.sc_bytes;
+      const bool wide = (a.kb & 7) == 0;
+      uint4 s8 = make_uint4(0, 0, 0, 0), o8 = s8;  // eight groups' scales and biases
+      for (int k = 0; k < a.kb && ok; ++k, ++n) {
+        if ((k & 3) == 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(w_full + ws, wph, err, 7));
+          if (!ok) break;
+        }
+        if (wide && (k & 7) == 0) {
+          s8 = *reinterpret_cast<const uint4*>(sc + ((size_t)r * a.kb + k) * 2);
+          o8 = *reinterpret_cast<const uint4*>(sc + a.sc_bytes + ((size_t)r * a.kb + k) * 2);
+        }
+        if ((n & 1) == turn) {
+          uint32_t s2, b2;
+          if (wide) {
+            const int e = k & 7;
+            const uint32_t sw = e < 4 ? (e < 2 ? s8.x : s8.y) : (e < 6 ? s8.z : s8.w);
+            const uint32_t bw = e < 4 ? (e < 2 ? o8.x : o8.y) : (e < 6 ? o8.z : o8.w);
+            s2 = __byte_perm(sw, 0, (e & 1) ? 0x3232 : 0x1010);
+            b2 = __byte_perm(bw, 0, (e & 1) ? 0x3232 : 0x1010);
+          } else {
+            const uint16_t s = reinterpret_cast<const uint16_t*>(sc)[r * a.kb + k];
+            const uint16_t b = reinterpret_cast<const uint16_t*>(sc + a.sc_bytes)[r * a.kb + k];
+            s2 = s | (uint32_t)s << 16;
+            b2 = b | (uint32_t)b << 16;
+          }
+          const uint8_t* row = sm_w + ws * HQ_W_BYTES + r * 128;
+          const uint4 w0 = *reinterpret_cast<const uint4*>(row + ((((k & 3) * 2) ^ (lane & 7)) << 4));
+          const uint4 w1 = *reinterpret_cast<const uint4*>(row + ((((k & 3) * 2 + 1) ^ (lane & 7)) << 4));
+          const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+          uint32_t v[32];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int p = 0; p < 4; ++p) v[4 * j + p] = hq_pair(w[j] >> (4 * p), s2, b2);
+          }
+          ok = __all_sync(0xffffffffu, mbar_wait(empty + slot, ph ^ 1, err, 8));
+          if (!ok) break;
+          tc_fence_after();
+          if (mine) {
+            hq_st32(tmem_a + slot * 32 + lanes, v);
+            tmem_st_wait();
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full + slot);
+        }
+        if (++slot == a.xs) {
+          slot = 0;
+          ph ^= 1;
+        }
+        if ((k & 3) == 3 || k == a.kb - 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(w_empty + ws);
+          if (++ws == a.ws) {
+            ws = 0;
+            wph ^= 1;
+          }
+        }
+      }
+      __syncwarp();
+      if (ok && lane == 0) mbar_arrive(s_empty + sb);
+    }
+  } else if (warp >= 12) {
+    const int q = warp & 3;
+    const float nan = __int_as_float(0x7fffffff);
+    float mx[NT], sum[NT];
+    int top[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+      mx[c] = -INFINITY;
+      sum[c] = 0.f;
+      top[c] = 0x7fffffff;
+    }
+    bool ok = true;
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int acc = i & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(acc_full + acc, (i >> 1) & 1, err, 9));
+      if (!ok) break;
+      tc_fence_after();
+      const int blk = b0 + 4 * i + q;
+      if (blk < b1) {
+        const int id0 = blk * HQ_BLOCK;  // this warp's ids: id0 + lane
+        const bool in = id0 + lane < a.V;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          float v[32];
+          tmem_ld32_wait(tmem + acc * 32 * NT + c * 32 + ((uint32_t)(q * 32) << 16), v);
+          for (int j = 0; j < a.K; ++j) {
+            const int id = sm_id[j * 32 * NT + c * 32 + lane];
+            unsigned hit = __ballot_sync(0xffffffffu, (unsigned)id - (unsigned)id0 < 32u);
+            while (hit) {  // token c * 32 + b has its target in lane id - id0
+              const int b = __ffs(hit) - 1;
+              hit &= hit - 1;
+              const int at = __shfl_sync(0xffffffffu, id, b) - id0;
+              if (lane == at) a.out.ztgt[(size_t)(c * 32 + b) * a.K + j] = hd_pick(v, b);
+            }
+          }
+          __syncwarp();
+          if (!in) {
+#pragma unroll
+            for (int b = 0; b < 32; ++b) v[b] = -INFINITY;
+          }
+          float w[32];
+#pragma unroll
+          for (int b = 0; b < 32; ++b) w[b] = v[b];
+          const float cm = hq_across(w, [](float x, float y) { return fmaxf(x, y); });
+          int arg = 0;
+          if (a.out.top) {
+#pragma unroll
+            for (int b = 0; b < 32; ++b) {
+              const unsigned hit = __ballot_sync(0xffffffffu, v[b] == __shfl_sync(0xffffffffu, cm, b));
+              if (lane == b && hit) arg = __ffs(hit) - 1;
+            }
+          }
+          const float off = cm == -INFINITY ? 0.f : -cm * HD_LOG2E;
+#pragma unroll
+          for (int b = 0; b < 32; ++b) w[b] = hd_ex2(fmaf(v[b], HD_LOG2E, __shfl_sync(0xffffffffu, off, b)));
+          const float cs = hq_across(w, [](float x, float y) { return x + y; });
+          if (cm > mx[c]) {
+            sum[c] = sum[c] * hd_ex2((mx[c] - cm) * HD_LOG2E) + cs;
+            mx[c] = cm;
+            top[c] = id0 + arg;
+          } else {
+            sum[c] += cm == -INFINITY ? cs : cs * hd_ex2((cm - mx[c]) * HD_LOG2E);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty + acc);
+    }
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+      sm_m[q * 32 * NT + c * 32 + lane] = mx[c];
+      sm_sum[q * 32 * NT + c * 32 + lane] = ok ? sum[c] : nan;
+      sm_top[q * 32 * NT + c * 32 + lane] = top[c];
+    }
+  }
+  if (warp == 3) {
+    mbar_wait(done, 0, err + 3, 10, 8000000000LL);
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 3) tmem_dealloc(tmem, 512);
+  // The four warps' parts, in their order.
+  if (threadIdx.x < a.T) {
+    const int t = threadIdx.x;
+    float mx = -INFINITY, sum = 0.f;
+    int top = 0x7fffffff;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float m = sm_m[q * 32 * NT + t], s = sm_sum[q * 32 * NT + t];
+      const int p = sm_top[q * 32 * NT + t];
+      if (m > mx) {
+        sum = sum * hd_ex2((mx - m) * HD_LOG2E) + s;
+        mx = m;
+        top = p;
+      } else {
+        sum += m == -INFINITY ? s : s * hd_ex2((m - mx) * HD_LOG2E);
+        if (m == mx && p < top) top = p;
+      }
+    }
+    a.out.part[(size_t)t * a.out.parts + blockIdx.x] = make_float2(mx, sum);
+    if (a.out.top) a.out.top[(size_t)t * a.out.parts + blockIdx.x] = top;
+  }
+}
+
+// x with every eight columns in the order 0, 4, 1, 5, 2, 6, 3, 7.
+__global__ void __launch_bounds__(256) hq_order_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int n,
+                                                       int per, __nv_bfloat16* __restrict__ out) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int t = i / per, c = i % per;
+  const uint4 v = *reinterpret_cast<const uint4*>(x + (size_t)t * ldx + 8 * c);
+  reinterpret_cast<uint4*>(out)[i] =
+      make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                 __byte_perm(v.y, v.w, 0x7632));
+}
+
+// Slots and stages that fit, or false.
+static bool hq_layout(int T, int H, int K, HqArgs* a, size_t* smem) {
+  const int NT = T <= 32 ? 1 : T <= 64 ? 2 : 4;
+  a->N = (T + 15) / 16 * 16;
+  a->kb = H / 64;
+  a->sc_bytes = (128 * a->kb * 2 + 511) / 512 * 512;
+  const size_t fixed = 1024 + 4 * (size_t)a->sc_bytes + (size_t)(K + 12) * 32 * NT * 4 + 42 * 8 + 32;
+  for (int xs = 6; xs >= 4; xs -= 2) {
+    a->xs = xs;
+    a->ws = 5;
+    for (; a->ws >= 3; --a->ws) {
+      *smem = fixed + (size_t)xs * hq_x_bytes(a->N) + (size_t)a->ws * HQ_W_BYTES;
+      if (*smem <= HQ_SMEM_MAX) return true;
+    }
+  }
+  return false;
+}
+
+bool hq_takes(int T, int H, int V, int K, const HdHead& w) {
+  HqArgs a;
+  size_t smem;
+  return T <= HQ_MAXT && (long long)V * (H / 64) < (1LL << 31) && aligned(w.scales, 16) &&
+         aligned(w.biases, 16) && hq_layout(T, H, K, &a, &smem);
+}
+
+int hq_parts(int V) { return std::min(device_sm_count(), (V + HQ_BLOCK - 1) / HQ_BLOCK); }
+
+template <int NT>
+static int hq_launch(const CUtensorMap (&m)[4], const HqArgs& a, int grid, size_t smem, cudaStream_t st) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  LG_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !done[dev].load(std::memory_order_relaxed)) {
+    LG_CUDA_TRY(cudaFuncSetAttribute(hq_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, HQ_SMEM_MAX));
+    if (dev < 64) done[dev].store(true, std::memory_order_relaxed);
+  }
+  hq_kernel<NT><<<grid, HQ_THREADS, smem, st>>>(m[0], m[1], m[2], m[3], a);
+  LG_LAUNCH_CHECK("head_q4");
+  return LG_OK;
+}
+
+int hq_loss_parts(const __nv_bfloat16* x, long long ldx, int T, int H, const HdHead& w, int V, const int* ids,
+                  int K, __nv_bfloat16* xp, const HdParts& out, cudaStream_t st) {
+  HqArgs a = {};
+  size_t smem = 0;
+  if (!hq_layout(T, H, K, &a, &smem)) return fail(LG_ERR_UNSUPPORTED, "head_loss: H=%d K=%d", H, K);
+  a.T = T;
+  a.H = H;
+  a.V = V;
+  a.K = K;
+  a.blocks = (V + HQ_BLOCK - 1) / HQ_BLOCK;
+  a.ids = ids;
+  a.out = out;
+  const int n = T * (H / 8);
+  hq_order_kernel<<<(n + 255) / 256, 256, 0, st>>>(x, ldx, n, H / 8, xp);
+  LG_LAUNCH_CHECK("head_order");
+  const uint64_t groups = (uint64_t)V * (H / 64), gbytes = align_up(groups * 2, 16);
+  CUtensorMap m[4];
+  int rc = make_map_2d(&m[0], w.w, false, H / 8, V, (uint64_t)H / 2, 32, 32, 128);
+  if (rc == LG_OK) rc = make_map_2d(&m[1], w.scales, true, groups, 1, gbytes, 256, 1, 0);
+  if (rc == LG_OK) rc = make_map_2d(&m[2], w.biases, true, groups, 1, gbytes, 256, 1, 0);
+  if (rc == LG_OK) rc = make_map_2d(&m[3], xp, true, H, T, (uint64_t)H * 2, 64, a.N, 128);
+  if (rc != LG_OK) return rc;
+  const int grid = out.parts;
+  return T <= 32 ? hq_launch<1>(m, a, grid, smem, st)
+         : T <= 64 ? hq_launch<2>(m, a, grid, smem, st)
+                   : hq_launch<4>(m, a, grid, smem, st);
+}
+
+}  // namespace lg

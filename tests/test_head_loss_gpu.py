@@ -51,6 +51,46 @@ def test_4bit_head(T, V, H, K):
     check(x, head, W, ids, weights, g, dw=False)
 
 
+@pytest.mark.parametrize("T,V,H,K", [(1, 1, 64, 1), (1, 33, 512, 1), (16, 31, 128, 2), (17, 129, 448, 1),
+                                     (31, 4740, 64, 1), (32, 700, 1024, 64), (33, 40000, 576, 3),
+                                     (64, 5003, 512, 1), (65, 20000, 192, 1), (100, 9001, 2048, 64),
+                                     (128, 40001, 1536, 1), (128, 300, 4096, 64), (129, 40001, 512, 1)])
+def test_4bit_head_of_few_tokens(T, V, H, K):
+    """The 4-bit form for up to 128 tokens, one of 129 beside it: a CTA's ids in up to three tiles, its last of
+    one to four blocks, groups of scales that come eight at a time (H % 512 == 0) or one by one."""
+    x, head, W, ids, weights, _ = make(T, V, H, bits=4, K=K, skip=0.2, seed=V, std=0.02)
+    ids.view(T, K)[T // 2] = V - 1
+    r = reference(x, W, ids, weights)
+    loss, lse, top = ops.head_loss(x, head, ids, weights, top=True)
+    within(loss, r["loss"], r["bloss"])
+    within(lse, r["lse"], r["blse"])
+    z = x.double().cpu() @ W.double().cpu().T
+    assert (z.amax(1) - z.gather(1, top.long().cpu()[:, None])[:, 0] <= 2 * r["blse"]).all()
+    again = ops.head_loss(x, head, ids, weights)
+    assert torch.equal(again[0], loss) and torch.equal(again[1], lse)
+
+
+@pytest.mark.parametrize("T", [7, 40, 90])
+def test_4bit_top_of_equal_logits_is_the_lowest_id(T):
+    rows = torch.zeros(6000, 64, device="cuda")
+    rows[[37, 300, 301, 5990]] = 1
+    x = torch.ones(T, 64, dtype=torch.bfloat16, device="cuda")
+    x[1] = -1
+    top = ops.head_loss(x, ops.quantize(rows, 64, 4), torch.zeros(T, dtype=torch.int32, device="cuda"),
+                        top=True)[2]
+    assert top[1] == 0 and (top[[0, 2, T - 1]] == 37).all()
+
+
+@pytest.mark.parametrize("T", [5, 60, 128])
+def test_4bit_head_with_tokens_that_hold_nan(T):
+    x, head, W, ids, _, _ = make(T, 3000, 128, bits=4)
+    want = ops.head_loss(x, head, ids)
+    x[3] = float("nan")
+    got = ops.head_loss(x, head, ids)
+    keep = torch.arange(T, device="cuda") != 3
+    assert got[0][3].isnan() and all(torch.equal(a[keep], b[keep]) for a, b in zip(want, got))
+
+
 @pytest.mark.parametrize("T,V,K", [(1, 64, 64), (33, 100, 2), (130, 900, 5), (260, 3, 17), (64, 2000, 63)])
 def test_several_targets(T, V, K):
     """Few ids, so that the same one is listed twice or more."""
