@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
   const int units = a.mt * a.nt * a.splits;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int st = 0, used = 0;  // used: stages that hold a copy in this or an earlier turn
       uint32_t ph = 0;
       bool ok = true;
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc = idesc_bf16(HD_BM, HD_BN) | (A_MN ? 1u << 15 : 0u) |
                                  (B_MN ? IDESC_B_MN : 0u);
       const uint64_t hi = (uint64_t)SW128_HI << 32;
@@ -452,6 +452,7 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
 __device__ __forceinline__ float hd_dot(const HdHead& w, const __nv_bfloat16* x, int H, int v) {
   const int lane = threadIdx.x & 31;
   float s = 0.f;
+#pragma unroll 8
   for (int c = lane * 8; c < H; c += 256) {
     const uint4 xv = *reinterpret_cast<const uint4*>(x + c);
     const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
@@ -498,7 +499,7 @@ __global__ void __launch_bounds__(256) hd_join_kernel(HdParts in, int T, const _
   const float2* row = in.part + (size_t)t * parts;
   float mx = -INFINITY, sum = 0.f;
   int at = -1;
-#pragma unroll 4
+#pragma unroll 8
   for (int n = lane; n < parts; n += 32) {
     const float2 v = row[n];
     if (v.x > mx) {
@@ -640,7 +641,8 @@ static int hd_splits(int T, int H, int piece) {
 
 struct HdWork {
   HdParts out;
-  __nv_bfloat16* xp;  // few tokens and 4 bits: x in the order of a word's codes
+  __nv_bfloat16* xp;  // few tokens and 4 bits: x in the order of a word's codes, ids by target
+  int* idt;
   int* sorted;
   unsigned char *order, *start;
   float* wsum;
@@ -663,6 +665,7 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
     w.out.ztgt = c.take<float>((size_t)T * K);
     if (few) {
       w.xp = c.take<__nv_bfloat16>((size_t)T * H);
+      w.idt = c.take<int>((size_t)HQ_MAXT * K);
       w.bytes = align_up(c.used, 256);
       return w;
     }
@@ -808,7 +811,7 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
     return fail(LG_ERR_WORKSPACE, "head_loss: workspace of %zu bytes, need %zu", workspace_bytes, k.bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (few) {
-    HD_TRY(hq_loss_parts(xb, ldx, T, H, head, V, ids, K, k.xp, k.out, st));
+    HD_TRY(hq_loss_parts(xb, ldx, T, H, head, V, ids, K, k.xp, k.idt, k.out, st));
   } else {
     HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
     CUtensorMap mx, mw;

@@ -6,18 +6,23 @@
 //
 //   warp 0       TMA: packed words (32 rows x 256 codes a box, 128-byte swizzle), scales and biases
 //   warp 2       TMA: x, 64 columns a slot
-//   warps 4-11   unpack: a row a thread, 64 codes at a time (a quantization group), two groups of four warps
-//                in turns: code + 128 as bf16 by one LOP3 a pair, - 128, * scale + bias in packed bf16 with one
-//                rounding; tcgen05.st of 32 columns
-//   warp 1       four products (M 128, N, K 16) a slot into one of two accumulators
-//   warps 12-15  per tile and token the maximum and the sum of exponentials over the warp's 32 rows, which lie
+//   warps 4-19   unpack: a row a thread, 128 codes a turn (two quantization groups), four groups of four warps in
+//                turns; tcgen05.st of 32 columns a group
+//   warp 1       four products (M 128, N, K 16) a 64-wide block into one of two accumulators
+//   warps 20-23  per tile and token the maximum and the sum of exponentials over the warp's 32 rows, which lie
 //                across its lanes: a transposing reduction (31 shuffles for 32 columns) leaves token i with lane i
+//
+// Unpacking: the 16 bits of a pair's half that hold a code c, all else masked away, are the bf16 number c 2^-133
+// (codes in bits 0-3) or c 2^-129 (bits 4-7): a subnormal's bits count units of 2^-133. A packed bf16 fma with
+// scale 2^133 or scale 2^129 and the bias therefore gives bf16(scale c + bias) in one rounding: a shift, four LOP3 and
+// four fma for a word's eight codes. It takes scales in [2^-126, 2^-5); a warp with another one
+// puts 128 + c together, takes 128 off and has 15 instructions a word.
 //
 // K order: one LOP3 splits a word into the pairs (0,4), (1,5), (2,6), (3,7); x is copied in that order first
 // (hq_order_kernel), so that no code is moved.
 //
-// Each CTA has 1/148 of the blocks of 32 ids. What is bound: HBM (0.56 bytes a weight); the unpacking's
-// instructions take about as long (2 a weight).
+// Each CTA has 1/148 of the blocks of 32 ids. HBM needs 0.56 bytes a weight; what bounds it are the unpacking
+// warps' instructions.
 #include <math.h>
 
 #include <algorithm>
@@ -30,8 +35,8 @@ namespace lg {
 
 using namespace tc;
 
-constexpr int HQ_MAXT = 128;
-constexpr int HQ_THREADS = 512;
+constexpr int HQ_UNPACK = 16;  // warps
+constexpr int HQ_THREADS = (8 + HQ_UNPACK) * 32;
 constexpr int HQ_BLOCK = 32;               // ids a block: a warp's TMEM lanes
 constexpr int HQ_W_BYTES = 4 * 32 * 128;   // a stage of packed words: 128 rows x 256 codes
 constexpr int HQ_SMEM_MAX = 232448;
@@ -40,9 +45,10 @@ struct HqArgs {
   int T, N, H, V, K;
   int kb;       // 64-wide blocks of H
   int blocks;   // blocks of 32 ids
-  int xs, ws;   // slots of x (and of unpacked weights), stages of packed words
-  int sc_bytes;  // scales of a tile, a multiple of 512
-  const int* ids;
+  int as, ws;   // slots of unpacked weights and x (128 columns), stages of packed words (256 codes)
+  int sc_bytes;  // scales of a tile, a multiple of 2,048
+  int wide;      // scales by eight groups: [H / 512][128 rows][8]; else [128 rows][H / 64]
+  const int* ids;  // [K][32 NT], -1 past T
   HdParts out;
 };
 
@@ -68,6 +74,12 @@ __device__ __forceinline__ void hq_st32(uint32_t taddr, const uint32_t (&r)[32])
       "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+
+__device__ __forceinline__ uint32_t hq_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
 }
 
 // Codes 4 i and 4 i + 16 of v (already shifted) -> bf16 pair scale * code + bias.
@@ -107,9 +119,8 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   const int x_bytes = hq_x_bytes(a.N);
   uint8_t* sm_w = smem;
   uint8_t* sm_x = sm_w + a.ws * HQ_W_BYTES;
-  uint8_t* sm_s = sm_x + a.xs * x_bytes;        // [2][scales, biases]
-  int* sm_id = reinterpret_cast<int*>(sm_s + 4 * a.sc_bytes);  // [K][32 NT]
-  float* sm_m = reinterpret_cast<float*>(sm_id + a.K * 32 * NT);
+  uint8_t* sm_s = sm_x + 2 * a.as * x_bytes;  // [2][scales, biases]
+  float* sm_m = reinterpret_cast<float*>(sm_s + 4 * a.sc_bytes);
   float* sm_sum = sm_m + 4 * 32 * NT;
   int* sm_top = reinterpret_cast<int*>(sm_sum + 4 * 32 * NT);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm_top + 4 * 32 * NT);
@@ -128,15 +139,15 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.ws; ++i) {
       mbar_init(w_full + i, 1);
-      mbar_init(w_empty + i, 8);
+      mbar_init(w_empty + i, HQ_UNPACK);
     }
-    for (int i = 0; i < a.xs; ++i) {
+    for (int i = 0; i < a.as; ++i) {
       mbar_init(full + i, 5);  // x's copy and four warps
       mbar_init(empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(s_empty + i, 8);
+      mbar_init(s_empty + i, HQ_UNPACK);
       mbar_init(acc_full + i, 1);
       mbar_init(acc_empty + i, 4);
     }
@@ -152,18 +163,14 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
     tmem_alloc(tmem_base, 512);
     tmem_relinquish();
   }
-  for (int i = threadIdx.x; i < a.K * 32 * NT; i += HQ_THREADS) {
-    const int t = i % (32 * NT), j = i / (32 * NT);
-    sm_id[i] = t < a.T ? a.ids[(size_t)t * a.K + j] : -1;
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_base;        // accumulators: columns [0, 64 NT)
-  const uint32_t tmem_a = tmem + 256;      // weights: 32 columns a slot
+  const uint32_t tmem_a = tmem + 64 * NT;  // weights: 64 columns a slot
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int st = 0, used = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -172,12 +179,14 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
         const int row = (b0 + 4 * i) * HQ_BLOCK, nb = min(4, b1 - b0 - 4 * i);
         const int sb = i & 1;
         if (!mbar_wait(s_empty + sb, ((i >> 1) & 1) ^ 1, err, 1)) break;
-        const int groups = nb * HQ_BLOCK * a.kb, boxes = (groups + 255) / 256;
-        mbar_arrive_expect_tx(s_full + sb, 2 * boxes * 512);
+        const int boxes = a.wide ? a.kb / 8 : (nb * HQ_BLOCK * a.kb + 255) / 256;
+        const int box = a.wide ? 2048 : 512;
+        mbar_arrive_expect_tx(s_full + sb, 2 * boxes * box);
         uint8_t* s = sm_s + sb * 2 * a.sc_bytes;
         for (int j = 0; j < boxes; ++j) {
-          tma_load_2d(s + j * 512, &ms, s_full + sb, row * a.kb + j * 256, 0);
-          tma_load_2d(s + a.sc_bytes + j * 512, &mb, s_full + sb, row * a.kb + j * 256, 0);
+          const int x = a.wide ? j * 8 : row * a.kb + j * 256, y = a.wide ? row : 0;
+          tma_load_2d(s + j * box, &ms, s_full + sb, x, y);
+          tma_load_2d(s + a.sc_bytes + j * box, &mb, s_full + sb, x, y);
         }
         for (int k = 0; k < stages; ++k) {
           if (!mbar_wait(w_empty + st, ph ^ 1, err, 2)) {
@@ -204,55 +213,63 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
     }
     __syncwarp();
   } else if (warp == 2) {
-    if (lane == 0) {
+    if (elect_one()) {
       int st = 0, used = 0;
       uint32_t ph = 0;
       bool ok = true;
       for (int i = 0; i < tiles && ok; ++i) {
-        for (int k = 0; k < a.kb; ++k) {
+        for (int k = 0; k < a.kb; k += 2) {
           if (!mbar_wait(empty + st, ph ^ 1, err, 3)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(full + st, a.N * 128);
-          tma_load_2d(sm_x + st * x_bytes, &mx, full + st, k * 64, 0);
-          if (used < a.xs) ++used;
-          if (++st == a.xs) {
+          const int n = min(2, a.kb - k);
+          mbar_arrive_expect_tx(full + st, n * a.N * 128);
+          for (int j = 0; j < n; ++j)
+            tma_load_2d(sm_x + (2 * st + j) * x_bytes, &mx, full + st, (k + j) * 64, 0);
+          if (used < a.as) ++used;
+          if (++st == a.as) {
             st = 0;
             ph ^= 1;
           }
         }
       }
       for (int j = used; j > 0; --j) {
-        const int s = (st - j + a.xs) % a.xs;
+        const int s = (st - j + a.as) % a.as;
         mbar_wait(full + s, s < st ? ph : ph ^ 1, err + 2, 3, 400000000LL);
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc = idesc_bf16(128, a.N);
       const uint64_t hi = (uint64_t)SW128_HI << 32;
-      int st = 0;
+      // One wait and one commit for 128 columns: with one each for 64 columns of x beside them this thread took 630
+      // cycles a turn, three times what the products take.
+      int slot = 0;
       uint32_t ph = 0;
       bool ok = true;
       for (int i = 0; i < tiles && ok; ++i) {
         const int acc = i & 1;
         if (!mbar_wait(acc_empty + acc, ((i >> 1) & 1) ^ 1, err, 4)) break;
-        tc_fence_after();
-        for (int k = 0; k < a.kb; ++k) {
-          if (!mbar_wait(full + st, ph, err, 5)) {
+        for (int k = 0; k < a.kb; k += 2) {
+          if (!mbar_wait(full + slot, ph, err, 5)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t db = sw128_lo(smem_u32(sm_x + st * x_bytes));
+          const uint32_t d = tmem + acc * 32 * NT, da = tmem_a + slot * 64;
+          const uint32_t db = sw128_lo(smem_u32(sm_x + 2 * slot * x_bytes));
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            hq_mma(tmem + acc * 32 * NT, tmem_a + st * 32 + j * 8, hi | (db + j * 2), idesc, k > 0 || j > 0);
-          umma_commit(empty + st);
-          if (++st == a.xs) {
-            st = 0;
+          for (int j = 0; j < 4; ++j) hq_mma(d, da + j * 8, hi | (db + j * 2), idesc, k > 0 || j > 0);
+          if (k + 1 < a.kb) {
+            const uint32_t d2 = db + (x_bytes >> 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) hq_mma(d, da + 32 + j * 8, hi | (d2 + j * 2), idesc, 1);
+          }
+          umma_commit(empty + slot);
+          if (++slot == a.as) {
+            slot = 0;
             ph ^= 1;
           }
         }
@@ -261,70 +278,91 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
       umma_commit(done);
     }
     __syncwarp();
-  } else if (warp >= 4 && warp < 12) {
-    // Block n of all tiles' blocks is unpacked by the four warps of parity n.
-    const int q = warp & 3, turn = (warp >> 2) & 1;  // warps 4 to 7: 1, 8 to 11: 0
+  } else if (warp >= 4 && warp < 4 + HQ_UNPACK) {
+    // Turn n of all tiles' turns (128 codes, at a tile's end 64 or 128) is unpacked by the warps of group n % 4.
+    const int q = warp & 3, group = (warp >> 2) & 3;
     const int r = q * 32 + lane;
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
+    const int turns = (a.kb + 1) / 2;
+    // Every warp waits for every stage and gives it back, used or not: a warp that left some out could look at a
+    // barrier two phases early or late, whose parity is the same. (The slots' barriers have no such case: the
+    // products end in order, and the turn before this group's last one in a slot is at least as old.)
     int n = 0, slot = 0, ws = 0;
     uint32_t ph = 0, wph = 0;
     bool ok = true;
     for (int i = 0; i < tiles && ok; ++i) {
-      const int nb = min(4, b1 - b0 - 4 * i), sb = i & 1;
-      const bool mine = q < nb;
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full + sb, (i >> 1) & 1, err, 6));
+      const int sb = i & 1;
+      const bool mine = q < b1 - b0 - 4 * i;
       const uint8_t* sc = sm_s + sb * 2 * a.sc_bytes;
-      const bool wide = (a.kb & 7) == 0;
-      uint4 s8 = make_uint4(0, 0, 0, 0), o8 = s8;  // eight groups' scales and biases
-      for (int k = 0; k < a.kb && ok; ++k, ++n) {
-        if ((k & 3) == 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full + sb, (i >> 1) & 1, err, 6));
+      for (int k2 = 0; k2 < turns && ok; ++k2) {
+        if (!(k2 & 1)) {
           ok = __all_sync(0xffffffffu, mbar_wait(w_full + ws, wph, err, 7));
           if (!ok) break;
         }
-        if (wide && (k & 7) == 0) {
-          s8 = *reinterpret_cast<const uint4*>(sc + ((size_t)r * a.kb + k) * 2);
-          o8 = *reinterpret_cast<const uint4*>(sc + a.sc_bytes + ((size_t)r * a.kb + k) * 2);
-        }
-        if ((n & 1) == turn) {
-          uint32_t s2, b2;
-          if (wide) {
-            const int e = k & 7;
-            const uint32_t sw = e < 4 ? (e < 2 ? s8.x : s8.y) : (e < 6 ? s8.z : s8.w);
-            const uint32_t bw = e < 4 ? (e < 2 ? o8.x : o8.y) : (e < 6 ? o8.z : o8.w);
-            s2 = __byte_perm(sw, 0, (e & 1) ? 0x3232 : 0x1010);
-            b2 = __byte_perm(bw, 0, (e & 1) ? 0x3232 : 0x1010);
+        if ((n & 3) == group) {
+          const int k = 2 * k2;
+          const bool two = k + 1 < a.kb;
+          uint32_t sw, bw;  // two groups' scales and biases
+          if (a.wide) {
+            const uint8_t* at = sc + (k >> 3) * 2048 + r * 16 + (k & 7) * 2;
+            sw = *reinterpret_cast<const uint32_t*>(at);
+            bw = *reinterpret_cast<const uint32_t*>(at + a.sc_bytes);
           } else {
-            const uint16_t s = reinterpret_cast<const uint16_t*>(sc)[r * a.kb + k];
-            const uint16_t b = reinterpret_cast<const uint16_t*>(sc + a.sc_bytes)[r * a.kb + k];
-            s2 = s | (uint32_t)s << 16;
-            b2 = b | (uint32_t)b << 16;
+            const uint16_t* at = reinterpret_cast<const uint16_t*>(sc) + r * a.kb + k;
+            const uint16_t* bt = reinterpret_cast<const uint16_t*>(sc + a.sc_bytes) + r * a.kb + k;
+            sw = at[0] | (uint32_t)at[two] << 16;
+            bw = bt[0] | (uint32_t)bt[two] << 16;
           }
+          // exponents in [1, 121] (bit 15 of a half says not)
+          const uint32_t e = sw & 0x7F807F80u;
+          const bool fast = __all_sync(0xffffffffu, (((e + 0x43004300u) | (e - 0x00800080u)) & 0x80008000u) == 0);
           const uint8_t* row = sm_w + ws * HQ_W_BYTES + r * 128;
-          const uint4 w0 = *reinterpret_cast<const uint4*>(row + ((((k & 3) * 2) ^ (lane & 7)) << 4));
-          const uint4 w1 = *reinterpret_cast<const uint4*>(row + ((((k & 3) * 2 + 1) ^ (lane & 7)) << 4));
-          const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-          uint32_t v[32];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int h = 0; h < 2; ++h) {
+            if (h == 1 && !two) break;
+            const int c = (k2 & 1) * 4 + h * 2;  // 16-byte chunks of the row's 128
+            const uint4 w0 = *reinterpret_cast<const uint4*>(row + ((c ^ (lane & 7)) << 4));
+            const uint4 w1 = *reinterpret_cast<const uint4*>(row + (((c + 1) ^ (lane & 7)) << 4));
+            const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+            const uint32_t s2 = __byte_perm(sw, 0, h ? 0x3232 : 0x1010), b2 = __byte_perm(bw, 0, h ? 0x3232 : 0x1010);
+            uint32_t v[32];
+            if (fast) {
+              const uint32_t lo = s2 + 0x42804280u, hi = s2 + 0x40804080u;  // * 2^133, * 2^129
 #pragma unroll
-            for (int p = 0; p < 4; ++p) v[4 * j + p] = hq_pair(w[j] >> (4 * p), s2, b2);
+              for (int j = 0; j < 8; ++j) {
+                const uint32_t u = w[j] >> 8;
+                v[4 * j] = hq_fma(w[j] & 0x000F000Fu, lo, b2);
+                v[4 * j + 1] = hq_fma(w[j] & 0x00F000F0u, hi, b2);
+                v[4 * j + 2] = hq_fma(u & 0x000F000Fu, lo, b2);
+                v[4 * j + 3] = hq_fma(u & 0x00F000F0u, hi, b2);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+#pragma unroll
+                for (int p = 0; p < 4; ++p) v[4 * j + p] = hq_pair(w[j] >> (4 * p), s2, b2);
+              }
+            }
+            if (h == 0) {
+              ok = __all_sync(0xffffffffu, mbar_wait(empty + slot, ph ^ 1, err, 8));
+              if (!ok) break;
+              tc_fence_after();
+            }
+            if (mine) hq_st32(tmem_a + slot * 64 + h * 32 + lanes, v);
           }
-          ok = __all_sync(0xffffffffu, mbar_wait(empty + slot, ph ^ 1, err, 8));
           if (!ok) break;
-          tc_fence_after();
-          if (mine) {
-            hq_st32(tmem_a + slot * 32 + lanes, v);
-            tmem_st_wait();
-          }
+          tmem_st_wait();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(full + slot);
         }
-        if (++slot == a.xs) {
+        ++n;
+        if (++slot == a.as) {
           slot = 0;
           ph ^= 1;
         }
-        if ((k & 3) == 3 || k == a.kb - 1) {
+        if ((k2 & 1) || k2 == turns - 1) {
           __syncwarp();
           if (lane == 0) mbar_arrive(w_empty + ws);
           if (++ws == a.ws) {
@@ -336,7 +374,7 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
       __syncwarp();
       if (ok && lane == 0) mbar_arrive(s_empty + sb);
     }
-  } else if (warp >= 12) {
+  } else if (warp >= 4 + HQ_UNPACK) {
     const int q = warp & 3;
     const float nan = __int_as_float(0x7fffffff);
     float mx[NT], sum[NT];
@@ -361,8 +399,9 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
         for (int c = 0; c < NT; ++c) {
           float v[32];
           tmem_ld32_wait(tmem + acc * 32 * NT + c * 32 + ((uint32_t)(q * 32) << 16), v);
+#pragma unroll 4
           for (int j = 0; j < a.K; ++j) {
-            const int id = sm_id[j * 32 * NT + c * 32 + lane];
+            const int id = a.ids[j * 32 * NT + c * 32 + lane];
             unsigned hit = __ballot_sync(0xffffffffu, (unsigned)id - (unsigned)id0 < 32u);
             while (hit) {  // token c * 32 + b has its target in lane id - id0
               const int b = __ffs(hit) - 1;
@@ -376,10 +415,13 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
 #pragma unroll
             for (int b = 0; b < 32; ++b) v[b] = -INFINITY;
           }
-          float w[32];
+          const float cm = hq_across(v, [](float x, float y) { return fmaxf(x, y); });
+          // the logits again, in the reduction's registers
+          tmem_ld32_wait(tmem + acc * 32 * NT + c * 32 + ((uint32_t)(q * 32) << 16), v);
+          if (!in) {
 #pragma unroll
-          for (int b = 0; b < 32; ++b) w[b] = v[b];
-          const float cm = hq_across(w, [](float x, float y) { return fmaxf(x, y); });
+            for (int b = 0; b < 32; ++b) v[b] = -INFINITY;
+          }
           int arg = 0;
           if (a.out.top) {
 #pragma unroll
@@ -390,8 +432,8 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
           }
           const float off = cm == -INFINITY ? 0.f : -cm * HD_LOG2E;
 #pragma unroll
-          for (int b = 0; b < 32; ++b) w[b] = hd_ex2(fmaf(v[b], HD_LOG2E, __shfl_sync(0xffffffffu, off, b)));
-          const float cs = hq_across(w, [](float x, float y) { return x + y; });
+          for (int b = 0; b < 32; ++b) v[b] = hd_ex2(fmaf(v[b], HD_LOG2E, __shfl_sync(0xffffffffu, off, b)));
+          const float cs = hq_across(v, [](float x, float y) { return x + y; });
           if (cm > mx[c]) {
             sum[c] = sum[c] * hd_ex2((mx[c] - cm) * HD_LOG2E) + cs;
             mx[c] = cm;
@@ -443,10 +485,16 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   }
 }
 
-// x with every eight columns in the order 0, 4, 1, 5, 2, 6, 3, 7.
+// x with every eight columns in the order 0, 4, 1, 5, 2, 6, 3, 7, and the ids by target [K][nt] (-1 past T).
 __global__ void __launch_bounds__(256) hq_order_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int n,
-                                                       int per, __nv_bfloat16* __restrict__ out) {
+                                                       int per, __nv_bfloat16* __restrict__ out,
+                                                       const int* __restrict__ ids, int T, int K, int nt,
+                                                       int* __restrict__ idt) {
   const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < K * nt) {
+    const int t = i % nt, j = i / nt;
+    idt[i] = t < T ? ids[(size_t)t * K + j] : -1;
+  }
   if (i >= n) return;
   const int t = i / per, c = i % per;
   const uint4 v = *reinterpret_cast<const uint4*>(x + (size_t)t * ldx + 8 * c);
@@ -456,17 +504,18 @@ __global__ void __launch_bounds__(256) hq_order_kernel(const __nv_bfloat16* __re
 }
 
 // Slots and stages that fit, or false.
-static bool hq_layout(int T, int H, int K, HqArgs* a, size_t* smem) {
-  const int NT = T <= 32 ? 1 : T <= 64 ? 2 : 4;
+static int hq_nt(int T) { return T <= 32 ? 1 : T <= 64 ? 2 : 4; }
+
+static bool hq_layout(int T, int H, HqArgs* a, size_t* smem) {
+  const int NT = hq_nt(T);
   a->N = (T + 15) / 16 * 16;
   a->kb = H / 64;
-  a->sc_bytes = (128 * a->kb * 2 + 511) / 512 * 512;
-  const size_t fixed = 1024 + 4 * (size_t)a->sc_bytes + (size_t)(K + 12) * 32 * NT * 4 + 42 * 8 + 32;
-  for (int xs = 6; xs >= 4; xs -= 2) {
-    a->xs = xs;
-    a->ws = 5;
-    for (; a->ws >= 3; --a->ws) {
-      *smem = fixed + (size_t)xs * hq_x_bytes(a->N) + (size_t)a->ws * HQ_W_BYTES;
+  a->wide = H % 512 == 0;
+  a->sc_bytes = (128 * a->kb * 2 + 2047) / 2048 * 2048;
+  const size_t fixed = 1024 + 4 * (size_t)a->sc_bytes + (size_t)12 * 32 * NT * 4 + 42 * 8 + 32;
+  for (a->as = std::min(6, (512 - 64 * NT) / 64); a->as >= 4; --a->as) {  // below 4 a group could pass its own slot
+    for (a->ws = 6; a->ws >= 3; --a->ws) {
+      *smem = fixed + 2 * (size_t)a->as * hq_x_bytes(a->N) + (size_t)a->ws * HQ_W_BYTES;
       if (*smem <= HQ_SMEM_MAX) return true;
     }
   }
@@ -477,7 +526,7 @@ bool hq_takes(int T, int H, int V, int K, const HdHead& w) {
   HqArgs a;
   size_t smem;
   return T <= HQ_MAXT && (long long)V * (H / 64) < (1LL << 31) && aligned(w.scales, 16) &&
-         aligned(w.biases, 16) && hq_layout(T, H, K, &a, &smem);
+         aligned(w.biases, 16) && hq_layout(T, H, &a, &smem);
 }
 
 int hq_parts(int V) { return std::min(device_sm_count(), (V + HQ_BLOCK - 1) / HQ_BLOCK); }
@@ -497,25 +546,29 @@ static int hq_launch(const CUtensorMap (&m)[4], const HqArgs& a, int grid, size_
 }
 
 int hq_loss_parts(const __nv_bfloat16* x, long long ldx, int T, int H, const HdHead& w, int V, const int* ids,
-                  int K, __nv_bfloat16* xp, const HdParts& out, cudaStream_t st) {
+                  int K, __nv_bfloat16* xp, int* idt, const HdParts& out, cudaStream_t st) {
   HqArgs a = {};
   size_t smem = 0;
-  if (!hq_layout(T, H, K, &a, &smem)) return fail(LG_ERR_UNSUPPORTED, "head_loss: H=%d K=%d", H, K);
+  if (!hq_layout(T, H, &a, &smem)) return fail(LG_ERR_UNSUPPORTED, "head_loss: H=%d", H);
   a.T = T;
   a.H = H;
   a.V = V;
   a.K = K;
   a.blocks = (V + HQ_BLOCK - 1) / HQ_BLOCK;
-  a.ids = ids;
+  a.ids = idt;
   a.out = out;
   const int n = T * (H / 8);
-  hq_order_kernel<<<(n + 255) / 256, 256, 0, st>>>(x, ldx, n, H / 8, xp);
+  const int nt = 32 * hq_nt(T);
+  hq_order_kernel<<<(std::max(n, K * nt) + 255) / 256, 256, 0, st>>>(x, ldx, n, H / 8, xp, ids, T, K, nt, idt);
   LG_LAUNCH_CHECK("head_order");
   const uint64_t groups = (uint64_t)V * (H / 64), gbytes = align_up(groups * 2, 16);
   CUtensorMap m[4];
   int rc = make_map_2d(&m[0], w.w, false, H / 8, V, (uint64_t)H / 2, 32, 32, 128);
-  if (rc == LG_OK) rc = make_map_2d(&m[1], w.scales, true, groups, 1, gbytes, 256, 1, 0);
-  if (rc == LG_OK) rc = make_map_2d(&m[2], w.biases, true, groups, 1, gbytes, 256, 1, 0);
+  for (int i = 1; i < 3 && rc == LG_OK; ++i) {
+    const void* p = i == 1 ? w.scales : w.biases;
+    rc = a.wide ? make_map_2d(&m[i], p, true, H / 64, V, (uint64_t)H / 32, 8, 128, 0)
+                : make_map_2d(&m[i], p, true, groups, 1, gbytes, 256, 1, 0);
+  }
   if (rc == LG_OK) rc = make_map_2d(&m[3], xp, true, H, T, (uint64_t)H * 2, 64, a.N, 128);
   if (rc != LG_OK) return rc;
   const int grid = out.parts;
