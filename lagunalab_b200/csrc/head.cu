@@ -31,17 +31,15 @@ using namespace tc;
 enum { HD_LOSS = 0, HD_PROB = 1, HD_XGRAD = 2, HD_WGRAD = 3 };
 
 constexpr int HD_BM = 128, HD_BN = 256, HD_BK = 64;
-constexpr int HD_STAGES = 4;
 constexpr int HD_THREADS = 256;
 constexpr int HD_A_BYTES = HD_BM * HD_BK * 2;  // 16 KB
-constexpr int HD_B_BYTES = HD_BN * HD_BK * 2;  // 32 KB
-constexpr int HD_STAGE_BYTES = HD_A_BYTES + HD_B_BYTES;
 constexpr int HD_BOX = 64 * HD_BK * 2;  // an MN-major box: 64 K rows of 64 elements
-constexpr size_t HD_SMEM = 1024 + (size_t)HD_STAGES * HD_STAGE_BYTES + 256;
+constexpr int HD_RING = 192 << 10;      // stages of A and B
+constexpr size_t HD_SMEM = 1024 + HD_RING + 256;
 
 struct HdArgs {
   int M, N;          // rows of the output tile grid, and its columns
-  int mt, nt;        // tiles of 128 x 256
+  int mt, nt;        // tiles of 128 CG x 256
   int kblocks;       // 64-wide blocks of the contraction
   int splits;        // HD_XGRAD: parts of the contraction, each with a sum of its own
   int b_row0;        // HD_LOSS, HD_PROB: B's first row; HD_XGRAD: B's first row along the contraction
@@ -97,9 +95,7 @@ __device__ __forceinline__ HdUnit hd_unit(const HdArgs& a, int i) {
 
 // One output tile's row of this thread. `ok` is false after a wait that ran out: NaN is written.
 template <int KIND>
-__device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, int row, uint32_t taddr,
-                                            bool ok) {
-  const int t = u.m * HD_BM + row;
+__device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, int t, uint32_t taddr, bool ok) {
   const int n0 = u.n * HD_BN;  // in the piece (or in H)
   const bool live = t < a.M;
   const float nan = __int_as_float(0x7fffffff);
@@ -245,34 +241,43 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
   }
 }
 
-// D[M, N] = A B^T over tiles of 128 x 256. A and B are K-major ([rows, contraction]) or MN-major
+// D[M, N] = A B^T over tiles of 128 CG x 256. A and B are K-major ([rows, contraction]) or MN-major
 // ([contraction, rows]): HD_LOSS, HD_PROB: x and W, both K-major; HD_XGRAD: dz K-major, W MN-major;
 // HD_WGRAD: dz and x, both MN-major. Warp 0: TMA; warp 1: products into one of two TMEM tiles;
 // warps 4 to 7: the finished tile's rows, one a thread, while the next one's products run.
-template <int KIND>
+//
+// CG = 2: a pair of CTAs shares a tile, each loads its 128 rows of A and half of B, and the leader issues for
+// both. Per 64 of the contraction an SM then loads 32 KB instead of 48 in 512 cycles of products: one CTA alone
+// waits for L2 (60 bytes a cycle; 204 cycles a product instead of 128).
+template <int KIND, int CG>
 __global__ void __launch_bounds__(HD_THREADS, 1)
     hd_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
               const HdArgs a) {
   constexpr bool A_MN = KIND == HD_WGRAD, B_MN = KIND == HD_XGRAD || KIND == HD_WGRAD;
+  constexpr int B_ROWS = HD_BN / CG;  // of B in this CTA
+  constexpr int STAGE = HD_A_BYTES + B_ROWS * HD_BK * 2;
+  constexpr int STAGES = HD_RING / STAGE;
   extern __shared__ uint8_t hd_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)hd_smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + HD_STAGES * HD_STAGE_BYTES);
-  uint64_t* empty = full + HD_STAGES;
-  uint64_t* acc_full = empty + HD_STAGES;  // [2]
-  uint64_t* acc_empty = acc_full + 2;      // [2]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + HD_RING);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;  // [2]
+  uint64_t* acc_empty = acc_full + 2;   // [2]
   uint64_t* done = acc_empty + 2;
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(done + 1);
   int* err = reinterpret_cast<int*>(tmem_base + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? (int)cluster_rank() : 0;
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < HD_STAGES; ++i) {
+    for (int i = 0; i < STAGES; ++i) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + i, 1);
-      mbar_init(acc_empty + i, 4);
+      mbar_init(acc_empty + i, 4 * CG);
     }
     mbar_init(done, 1);
     err[0] = err[1] = err[2] = 0;  // of all roles; of the copies' end; of the products' end
@@ -281,11 +286,16 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
     prefetch_tmap(&mb);
   }
   if (warp == 2) {
-    tmem_alloc(tmem_base, 512);
-    tmem_relinquish();
+    if (CG == 2) {
+      tmem_alloc_pair(tmem_base, 512);
+    } else {
+      tmem_alloc(tmem_base, 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (CG == 2) cluster_sync();  // the other CTA's barriers are ready
   tc_fence_after();
   const uint32_t tmem = *tmem_base;
   const int units = a.mt * a.nt * a.splits;
@@ -295,57 +305,70 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
       int st = 0, used = 0;  // used: stages that hold a copy in this or an earlier turn
       uint32_t ph = 0;
       bool ok = true;
-      for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
+      for (int i = first; i < units && ok; i += step) {
         const HdUnit u = hd_unit<KIND>(a, i);
-        const int ar = u.m * HD_BM, br = u.n * HD_BN;
+        const int ar = (u.m * CG + rank) * HD_BM, br = u.n * HD_BN + rank * B_ROWS;
         for (int kb = u.k0; kb < u.k1; ++kb) {
           if (!mbar_wait(empty + st, ph ^ 1, err, 1)) {
             ok = false;
             break;
           }
-          uint8_t* sa = smem + st * HD_STAGE_BYTES;
+          uint8_t* sa = smem + st * STAGE;
           uint8_t* sb = sa + HD_A_BYTES;
-          mbar_arrive_expect_tx(full + st, HD_STAGE_BYTES);
           const int k = kb * HD_BK;
+          // Both CTAs' copies complete on the leader's barrier, which expects the bytes of both.
+          if (rank == 0) mbar_arrive_expect_tx(full + st, CG * STAGE);
+          const uint32_t bar = CG == 2 ? mapa(full + st, 0) : smem_u32(full + st);
+          const auto load = [&](void* dst, const CUtensorMap* m, int x, int y) {
+            if (CG == 2)
+              tma_load_2d_pair(dst, m, bar, x, y);
+            else
+              tma_load_2d(dst, m, full + st, x, y);
+          };
           if (A_MN) {
 #pragma unroll
-            for (int j = 0; j < HD_BM / 64; ++j)
-              tma_load_2d(sa + j * HD_BOX, &ma, full + st, ar + j * 64, k);
+            for (int j = 0; j < HD_BM / 64; ++j) load(sa + j * HD_BOX, &ma, ar + j * 64, k);
           } else {
-            tma_load_2d(sa, &ma, full + st, k, ar);
+            load(sa, &ma, k, ar);
           }
           if (B_MN) {
 #pragma unroll
-            for (int j = 0; j < HD_BN / 64; ++j)
-              tma_load_2d(sb + j * HD_BOX, &mb, full + st, br + j * 64,
-                          (KIND == HD_XGRAD ? a.b_row0 : 0) + k);
+            for (int j = 0; j < B_ROWS / 64; ++j)
+              load(sb + j * HD_BOX, &mb, br + j * 64, (KIND == HD_XGRAD ? a.b_row0 : 0) + k);
           } else {
-            tma_load_2d(sb, &mb, full + st, k, a.b_row0 + br);
+            load(sb, &mb, k, a.b_row0 + br);
           }
-          if (used < HD_STAGES) ++used;
-          if (++st == HD_STAGES) {
+          if (used < STAGES) ++used;
+          if (++st == STAGES) {
             st = 0;
             ph ^= 1;
           }
         }
       }
-      // Every copy has landed before the CTA ends: the last `used` ones, oldest first.
-      for (int j = used; j > 0; --j) {
-        const int s = (st - j + HD_STAGES) % HD_STAGES;
+      // Every copy has landed before the CTA (or the pair, at its last barrier) ends: the last `used` ones, oldest
+      // first.
+      for (int j = used; rank == 0 && j > 0; --j) {
+        const int s = (st - j + STAGES) % STAGES;
         const uint32_t p = s < st ? ph : ph ^ 1;
         mbar_wait(full + s, p, err + 1, 2, 400000000LL);
       }
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else if (warp == 1 && rank == 0) {
     if (elect_one()) {
-      constexpr uint32_t idesc = idesc_bf16(HD_BM, HD_BN) | (A_MN ? 1u << 15 : 0u) |
+      constexpr uint32_t idesc = idesc_bf16(HD_BM * CG, HD_BN) | (A_MN ? 1u << 15 : 0u) |
                                  (B_MN ? IDESC_B_MN : 0u);
       const uint64_t hi = (uint64_t)SW128_HI << 32;
+      const auto commit = [](uint64_t* bar) {
+        if (CG == 2)
+          umma_commit_pair(bar);
+        else
+          umma_commit(bar);
+      };
       int st = 0, n = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int i = blockIdx.x; i < units && ok; i += gridDim.x, ++n) {
+      for (int i = first; i < units && ok; i += step, ++n) {
         const HdUnit u = hd_unit<KIND>(a, i);
         const int acc = n & 1;
         if (!mbar_wait(acc_empty + acc, ((n >> 1) & 1) ^ 1, err, 3)) break;
@@ -356,37 +379,47 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + st * HD_STAGE_BYTES), sb = sa + HD_A_BYTES;
+          const uint32_t sa = smem_u32(smem + st * STAGE), sb = sa + HD_A_BYTES;
           const uint32_t da = A_MN ? sw128_lo_mn(sa, HD_BOX) : sw128_lo(sa);
           const uint32_t db = B_MN ? sw128_lo_mn(sb, HD_BOX) : sw128_lo(sb);
 #pragma unroll
-          for (int k = 0; k < HD_BK / 16; ++k)  // 16 along K: 32 bytes, or two groups of 8 rows
-            umma_bf16(tmem + acc * HD_BN, hi | (da + k * (A_MN ? 128 : 2)),
-                      hi | (db + k * (B_MN ? 128 : 2)), idesc, kb > u.k0 || k > 0);
-          umma_commit(empty + st);
-          if (++st == HD_STAGES) {
+          for (int k = 0; k < HD_BK / 16; ++k) {  // 16 along K: 32 bytes, or two groups of 8 rows
+            const uint64_t ad = hi | (da + k * (A_MN ? 128 : 2)), bd = hi | (db + k * (B_MN ? 128 : 2));
+            if (CG == 2)
+              umma_bf16_pair(tmem + acc * HD_BN, ad, bd, idesc, kb > u.k0 || k > 0);
+            else
+              umma_bf16(tmem + acc * HD_BN, ad, bd, idesc, kb > u.k0 || k > 0);
+          }
+          commit(empty + st);
+          if (++st == STAGES) {
             st = 0;
             ph ^= 1;
           }
         }
-        if (ok) umma_commit(acc_full + acc);
+        if (ok) commit(acc_full + acc);
       }
-      umma_commit(done);
+      commit(done);
     }
     __syncwarp();
   } else if (warp >= 4) {
     const int q = warp & 3;
     bool ok = true;
     int n = 0;
-    for (int i = blockIdx.x; i < units; i += gridDim.x, ++n) {
+    for (int i = first; i < units; i += step, ++n) {
       const HdUnit u = hd_unit<KIND>(a, i);
       const int acc = n & 1;
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + acc, (n >> 1) & 1, err, 5));
       tc_fence_after();
-      hd_epilogue<KIND>(a, u, q * 32 + lane, tmem + acc * HD_BN + ((uint32_t)(q * 32) << 16), ok);
+      hd_epilogue<KIND>(a, u, (u.m * CG + rank) * HD_BM + q * 32 + lane,
+                        tmem + acc * HD_BN + ((uint32_t)(q * 32) << 16), ok);
       tc_fence_before();
       __syncwarp();
-      if (ok && lane == 0) mbar_arrive(acc_empty + acc);
+      if (ok && lane == 0) {
+        if (CG == 2)
+          mbar_arrive_cluster(mapa(acc_empty + acc, 0));
+        else
+          mbar_arrive(acc_empty + acc);
+      }
     }
   }
   // The products have ended before their TMEM goes.
@@ -396,8 +429,14 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (CG == 2) cluster_sync();  // nothing of the pair's reaches a CTA that has ended
   tc_fence_after();
-  if (warp == 2) tmem_dealloc(tmem, 512);
+  if (warp == 2) {
+    if (CG == 2)
+      tmem_dealloc_pair(tmem, 512);
+    else
+      tmem_dealloc(tmem, 512);
+  }
 }
 
 // The eight weights of a word: bf16(scale * code + bias).
@@ -632,11 +671,24 @@ static int hd_piece(int T, int H, int V, bool quant, bool grad) {
   return (int)(std::max(n, 1LL) * HD_BN);
 }
 
+// Parts of dx's contraction, so that the tiles fill the SMs in whole rounds: the fewest whose last round is within
+// 6 % of full, or the best of up to 8 rounds' worth; each part keeps at least 8 blocks of 64.
 static int hd_splits(int T, int H, int piece) {
-  const int tiles = ((T + HD_BM - 1) / HD_BM) * ((H + HD_BN - 1) / HD_BN);
-  const int sms = device_sm_count();
-  if (tiles >= sms) return 1;
-  return std::max(1, std::min(sms / tiles, piece / (4 * HD_BK)));
+  const int cg = T > HD_BM ? 2 : 1, slots = device_sm_count() / cg;
+  const int tiles = ((T + HD_BM * cg - 1) / (HD_BM * cg)) * ((H + HD_BN - 1) / HD_BN);
+  const int most = std::max(1, std::min(piece / (8 * HD_BK), std::max(8, slots / tiles)));
+  int best = 1;
+  double best_fill = 0;
+  for (int s = 1; s <= most; ++s) {
+    const long long units = (long long)tiles * s, rounds = (units + slots - 1) / slots;
+    const double fill = (double)units / (double)(rounds * slots);
+    if (fill > best_fill + 0.02) {
+      best_fill = fill;
+      best = s;
+    }
+    if (best_fill > 0.94) break;
+  }
+  return best;
 }
 
 struct HdWork {
@@ -689,26 +741,56 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
   return w;
 }
 
-template <int KIND>
-static int hd_launch(const CUtensorMap& ma, const CUtensorMap& mb, const HdArgs& a, cudaStream_t st) {
+#define HD_TRY(expr)           \
+  do {                         \
+    const int rc_ = (expr);    \
+    if (rc_ != LG_OK) return rc_; \
+  } while (0)
+
+template <int KIND, int CG>
+static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const HdArgs& a, cudaStream_t st) {
   static std::atomic<bool> done[64];
   int dev = 0;
   LG_CUDA_TRY(cudaGetDevice(&dev));
   if (dev >= 64 || !done[dev].load(std::memory_order_relaxed)) {
-    LG_CUDA_TRY(cudaFuncSetAttribute(hd_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    LG_CUDA_TRY(cudaFuncSetAttribute(hd_kernel<KIND, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)HD_SMEM));
     if (dev < 64) done[dev].store(true, std::memory_order_relaxed);
   }
   const long long units = (long long)a.mt * a.nt * a.splits;
-  const int grid = (int)std::min<long long>(units, device_sm_count());
-  hd_kernel<KIND><<<grid, HD_THREADS, HD_SMEM, st>>>(ma, mb, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = CG * (int)std::max(1LL, std::min<long long>(units, device_sm_count() / CG));
+  cfg.blockDim = HD_THREADS;
+  cfg.dynamicSmemBytes = HD_SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CG > 1;
+  LG_CUDA_TRY(cudaLaunchKernelEx(&cfg, hd_kernel<KIND, CG>, ma, mb, a));
   LG_LAUNCH_CHECK("head");
   return LG_OK;
 }
 
-static int hd_map(CUtensorMap* m, const void* p, long long inner, long long rows, long long ld,
-                  int box_rows) {
-  return make_map_2d(m, p, true, inner, rows, (uint64_t)ld * 2, 64, box_rows, 128);
+// Operands of a product: [contraction, rows] (mn) or [rows, contraction] matrices of bf16.
+struct HdOperand {
+  const void* p;
+  long long inner, rows, ld;
+};
+
+// One CTA a tile where the output has no more than 128 rows, else a pair.
+template <int KIND>
+static int hd_launch(const HdOperand& a, const HdOperand& b, HdArgs g, cudaStream_t st) {
+  constexpr bool A_MN = KIND == HD_WGRAD, B_MN = KIND == HD_XGRAD || KIND == HD_WGRAD;
+  const int cg = g.M > HD_BM ? 2 : 1;
+  g.mt = (g.M + HD_BM * cg - 1) / (HD_BM * cg);
+  g.nt = (g.N + HD_BN - 1) / HD_BN;
+  CUtensorMap ma, mb;
+  HD_TRY(make_map_2d(&ma, a.p, true, a.inner, a.rows, (uint64_t)a.ld * 2, 64, A_MN ? HD_BK : HD_BM, 128));
+  HD_TRY(make_map_2d(&mb, b.p, true, b.inner, b.rows, (uint64_t)b.ld * 2, 64, B_MN ? HD_BK : HD_BN / cg, 128));
+  return cg == 2 ? hd_launch_as<KIND, 2>(ma, mb, g, st) : hd_launch_as<KIND, 1>(ma, mb, g, st);
 }
 
 static int hd_check(const char* who, const void* x, long long ldx, int T, int H, const void* w,
@@ -753,12 +835,6 @@ static int hd_sort(const int* ids, const float* weights, int T, int K, int V, co
   return LG_OK;
 }
 
-#define HD_TRY(expr)           \
-  do {                         \
-    const int rc_ = (expr);    \
-    if (rc_ != LG_OK) return rc_; \
-  } while (0)
-
 static HdArgs hd_args(int T, int V, int K, const int* ids, const float* weights, const HdWork& k) {
   HdArgs a = {};
   a.V = V;
@@ -770,7 +846,6 @@ static HdArgs hd_args(int T, int V, int K, const int* ids, const float* weights,
   a.nt_all = k.nt;
   a.splits = 1;
   a.M = T;
-  a.mt = (T + HD_BM - 1) / HD_BM;
   return a;
 }
 
@@ -814,20 +889,17 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
     HD_TRY(hq_loss_parts(xb, ldx, T, H, head, V, ids, K, k.xp, k.idt, k.out, st));
   } else {
     HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
-    CUtensorMap mx, mw;
-    HD_TRY(hd_map(&mx, x, H, T, ldx, HD_BM));
     HdArgs a = hd_args(T, V, K, ids, weights, k);
     a.kblocks = (H + HD_BK - 1) / HD_BK;
     a.out = k.out;
     for (int v0 = 0; v0 < V; v0 += k.piece) {
       const int n = std::min(k.piece, V - v0);
       HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, st));
-      HD_TRY(quant ? hd_map(&mw, k.wq, H, n, H, HD_BN) : hd_map(&mw, w, H, V, ldw, HD_BN));
       a.N = n;
-      a.nt = (n + HD_BN - 1) / HD_BN;
       a.v0 = v0;
       a.b_row0 = quant ? 0 : v0;
-      HD_TRY(hd_launch<HD_LOSS>(mx, mw, a, st));
+      const HdOperand mw = quant ? HdOperand{k.wq, H, n, H} : HdOperand{w, H, V, ldw};
+      HD_TRY(hd_launch<HD_LOSS>({x, H, T, ldx}, mw, a, st));
     }
   }
   hd_join_kernel<<<(T + 7) / 8, 256, 0, st>>>(k.out, T, xb, ldx, H, head, ids, weights, K, V, loss, lse, top);
@@ -855,54 +927,43 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     return fail(LG_ERR_WORKSPACE, "head_loss_grad: workspace of %zu bytes, need %zu", workspace_bytes,
                 k.bytes);
   HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
-  CUtensorMap mx, mxt, mw, mwt, mz, mzt;
-  HD_TRY(hd_map(&mx, x, H, T, ldx, HD_BM));
   if (dw) {
     hd_rows_kernel<<<hd_blocks((long long)T * (H / 8)), 256, 0, st>>>(
         static_cast<const __nv_bfloat16*>(x), ldx, T, H, ids, K, V, k.xz);
     LG_LAUNCH_CHECK("head_rows");
-    HD_TRY(hd_map(&mxt, k.xz, H, T, H, HD_BK));
   }
   for (int v0 = 0; v0 < V; v0 += k.piece) {
     const int n = std::min(k.piece, V - v0);
     HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, st));
-    const void* wp = quant ? k.wq : w;
-    const long long rows = quant ? n : V, ld = quant ? H : ldw;
+    const HdOperand mw = quant ? HdOperand{k.wq, H, n, H} : HdOperand{w, H, V, ldw};
     HdArgs a = hd_args(T, V, K, ids, weights, k);
     a.v0 = v0;
     a.b_row0 = quant ? 0 : v0;
     a.N = n;
-    a.nt = (n + HD_BN - 1) / HD_BN;
     a.kblocks = (H + HD_BK - 1) / HD_BK;
     a.lse = lse;
     a.g = g;
     a.wsum = k.wsum;
     a.dz = k.dz;
     a.ldz = (n + 63) / 64 * 64;
-    HD_TRY(hd_map(&mw, wp, H, rows, ld, HD_BN));
-    HD_TRY(hd_launch<HD_PROB>(mx, mw, a, st));
+    HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, a, st));
+    const HdOperand mz = {k.dz, n, T, a.ldz};
     if (dx) {
       HdArgs b = a;
       b.N = H;
-      b.nt = (H + HD_BN - 1) / HD_BN;
       b.kblocks = (n + HD_BK - 1) / HD_BK;
       b.splits = std::min(k.splits, b.kblocks);
       b.dx = k.dx;
       b.add = v0 > 0;
-      HD_TRY(hd_map(&mz, k.dz, n, T, a.ldz, HD_BM));
-      HD_TRY(hd_map(&mwt, wp, H, rows, ld, HD_BK));
-      HD_TRY(hd_launch<HD_XGRAD>(mz, mwt, b, st));
+      HD_TRY(hd_launch<HD_XGRAD>(mz, mw, b, st));
     }
     if (dw) {
       HdArgs b = a;
       b.M = n;
-      b.mt = (n + HD_BM - 1) / HD_BM;
       b.N = H;
-      b.nt = (H + HD_BN - 1) / HD_BN;
       b.kblocks = (T + HD_BK - 1) / HD_BK;
       b.dw = static_cast<__nv_bfloat16*>(dw);
-      HD_TRY(hd_map(&mzt, k.dz, n, T, a.ldz, HD_BK));
-      HD_TRY(hd_launch<HD_WGRAD>(mzt, mxt, b, st));
+      HD_TRY(hd_launch<HD_WGRAD>(mz, {k.xz, H, T, H}, b, st));
     }
   }
   if (dx) {
