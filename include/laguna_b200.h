@@ -699,7 +699,8 @@ int lg_head_loss_grad(const void* x, long long ldx, int T, int H, const void* w,
  * N tokens kept:
  *   counts[e] = picks of e,  probs[e] = mean over tokens of s[t, e] / sum_e s[t, e],
  *   loss[0] = E sum_e counts[e] / (sum counts) probs[e],  tokens[0] = N;
- * all 0 where no token is kept. E <= 256, k <= 32. Sums are fp32, in an order that depends on T alone.
+ * all 0 where no token is kept. E <= 256, k <= 32. Sums are fp32, in an order that depends on T alone. A short
+ * batch needs no workspace (0 bytes: NULL is taken).
  */
 size_t lg_router_balance_workspace_bytes(int T, int E);
 int lg_router_balance(const float* logits, const int32_t* inds, const uint8_t* mask, int T, int E,

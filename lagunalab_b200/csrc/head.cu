@@ -64,11 +64,23 @@ struct HdArgs {
   int add;    // 0: the first piece
   // HD_WGRAD
   __nv_bfloat16* dw;  // [V, H]
+  bool wide;          // its rows are 32-byte aligned
 };
 
 __device__ __forceinline__ void hd_sub(float (&v)[32], int c, float w) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = i == c ? v[i] - w : v[i];
+}
+
+// Sixteen bf16 of a row as one 32-byte store: a thread has a row of its own, so that a narrower store would leave
+// its sector of L2 half written.
+__device__ __forceinline__ void hd_store16(__nv_bfloat16* p, const float* v) {
+  uint32_t r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = hd_pack(v[2 * i], v[2 * i + 1]);
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 // A unit of work: tile (m, n) of the output, and the part [k0, k1) of the contraction's blocks.
@@ -201,11 +213,8 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
           for (int i = 0; i < 32; ++i) v[i] = 0.f;
         }
         if (live) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            *reinterpret_cast<uint4*>(out + c + i) =
-                make_uint4(hd_pack(v[i], v[i + 1]), hd_pack(v[i + 2], v[i + 3]),
-                           hd_pack(v[i + 4], v[i + 5]), hd_pack(v[i + 6], v[i + 7]));
+          hd_store16(out + c, v);  // rows of dz are 128-byte aligned
+          hd_store16(out + c + 16, v + 16);
         }
       }
     }
@@ -229,6 +238,11 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
         }
       } else {
         __nv_bfloat16* out = a.dw + ((size_t)a.v0 + t) * a.N + n0 + c;
+        if (a.wide && n0 + c + 32 <= a.N) {
+          hd_store16(out, v);
+          hd_store16(out + 16, v + 16);
+          continue;
+        }
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {
           if (n0 + c + i >= a.N) break;
@@ -297,6 +311,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
   __syncthreads();
   if (CG == 2) cluster_sync();  // the other CTA's barriers are ready
   tc_fence_after();
+  pdl_wait();  // nothing of an earlier kernel's is touched before
+  pdl_trigger();
   const uint32_t tmem = *tmem_base;
   const int units = a.mt * a.nt * a.splits;
 
@@ -457,7 +473,9 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
                                                       unsigned char* __restrict__ order,
                                                       unsigned char* __restrict__ start,
                                                       float* __restrict__ wsum) {
-  __shared__ int sh[8][HD_MAXK];
+  pdl_wait();
+  pdl_trigger();
+  __shared__ int sh[8][2 * HD_MAXK];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x * 8 + warp;
   if (t >= T) return;
@@ -471,17 +489,27 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
   }
   sum = warp_sum(sum);
   __syncwarp();
+  int* up = sh[warp] + HD_MAXK;  // ascending
+  up[lane] = up[lane + 32] = 0x7fffffff;
+  __syncwarp();
+#pragma unroll 1
   for (int j = lane; j < K; j += 32) {
     const int id = row[j];
     int rank = 0;
+#pragma unroll 8
     for (int i = 0; i < K; ++i) rank += row[i] < id || (row[i] == id && i < j);
+    up[rank] = id;
     sorted[(size_t)t * K + rank] = id;
     order[(size_t)t * K + rank] = (unsigned char)j;
   }
-  for (int n = lane; n <= nt; n += 32) {  // n = nt: all that count
+  __syncwarp();
+  for (int n = lane; n <= nt; n += 32) {  // ids below the tile's first; n = nt: all that count
     const int lim = n == nt ? V : n * HD_BN;
     int c = 0;
-    for (int i = 0; i < K; ++i) c += row[i] < lim;
+#pragma unroll
+    for (int b = HD_MAXK / 2; b; b >>= 1)
+      if (up[c + b - 1] < lim) c += b;
+    if (up[c] < lim) ++c;
     start[(size_t)t * (nt + 1) + n] = (unsigned char)c;
   }
   if (lane == 0) wsum[t] = sum;
@@ -531,6 +559,8 @@ __global__ void __launch_bounds__(256) hd_join_kernel(HdParts in, int T, const _
                                                       float* __restrict__ loss,
                                                       float* __restrict__ lse_out,
                                                       int* __restrict__ top) {
+  pdl_wait();
+  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x * 8 + warp;
   if (t >= T) return;
@@ -615,38 +645,63 @@ __global__ void __launch_bounds__(256) hd_join_kernel(HdParts in, int T, const _
 
 // x with the rows of tokens without a target at 0, so that dW has nothing of them (0 * NaN is NaN).
 __global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx,
-                                                      int T, int H, const int* __restrict__ ids, int K,
-                                                      int V, __nv_bfloat16* __restrict__ out) {
+                                                      int T, int H, const int* __restrict__ ids, int V,
+                                                      const unsigned char* __restrict__ start, int nt,
+                                                      __nv_bfloat16* __restrict__ out) {
+  pdl_wait();
+  pdl_trigger();
   const int per = H / 8;
   const long long n = (long long)T * per;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
     const int t = (int)(i / per), c = (int)(i % per) * 8;
-    bool in = false;
-    for (int j = 0; j < K && !in; ++j) {
-      const int id = ids[(size_t)t * K + j];
-      in = id >= 0 && id < V;
-    }
+    const bool in = start ? start[(size_t)t * (nt + 1) + nt] > 0 : ids[t] >= 0 && ids[t] < V;
     uint4 v = make_uint4(0, 0, 0, 0);
     if (in) v = *reinterpret_cast<const uint4*>(x + (size_t)t * ldx + c);
     *reinterpret_cast<uint4*>(out + (size_t)t * H + c) = v;
   }
 }
 
-// Rows of a 4-bit group-64 head as bf16: bf16(scale * code + bias), eight of a word a thread.
-__global__ void __launch_bounds__(256) hd_dequant_kernel(const uint32_t* __restrict__ q,
+// Rows of a 4-bit group-64 head as bf16: bf16(scale * code + bias), half a group (four words) a thread.
+__global__ void __launch_bounds__(256) hd_dequant_kernel(const uint4* __restrict__ q,
                                                          const __nv_bfloat16* __restrict__ s,
-                                                         const __nv_bfloat16* __restrict__ b,
-                                                         long long words, __nv_bfloat16* __restrict__ out) {
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < words; i += gridDim.x * 256LL) {
-    uint32_t r[4];
-    hd_unpack(q[i], bf2f(s[i >> 3]), bf2f(b[i >> 3]), r);
-    *reinterpret_cast<uint4*>(out + 8 * i) = make_uint4(r[0], r[1], r[2], r[3]);
+                                                         const __nv_bfloat16* __restrict__ b, long long n,
+                                                         uint4* __restrict__ out) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int U = 4;
+  const long long step = gridDim.x * 256LL;
+  for (long long i0 = blockIdx.x * 256LL + threadIdx.x; i0 < n; i0 += U * step) {
+    uint4 w[U];
+    float sc[U], bi[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long i = i0 + u * step;
+      if (i < n) {
+        w[u] = q[i];
+        sc[u] = bf2f(s[i >> 1]);
+        bi[u] = bf2f(b[i >> 1]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long i = i0 + u * step;
+      if (i >= n) break;
+      const uint32_t v[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t r[4];
+        hd_unpack(v[j], sc[u], bi[u], r);
+        out[4 * i + j] = make_uint4(r[0], r[1], r[2], r[3]);
+      }
+    }
   }
 }
 
 // dx = the sum of its parts, in their order, rounded once.
 __global__ void __launch_bounds__(256) hd_sum_kernel(const float* __restrict__ parts, int n,
                                                      long long size, __nv_bfloat16* __restrict__ out) {
+  pdl_wait();
+  pdl_trigger();
   const long long q = size / 4;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < q; i += gridDim.x * 256LL) {
     float4 s = reinterpret_cast<const float4*>(parts)[i];
@@ -661,20 +716,49 @@ __global__ void __launch_bounds__(256) hd_sum_kernel(const float* __restrict__ p
 // ---- host ---------------------------------------------------------------------------------------
 
 constexpr long long HD_DZ_BYTES = 256LL << 20;  // dz of a piece
-constexpr long long HD_WQ_BYTES = 64LL << 20;   // bf16 rows of a piece of a 4-bit head: they stay in L2
+// bf16 rows of a piece of a 4-bit head: few tokens leave the products bound by memory, and a piece that stays in
+// L2 is not read from there.
+static long long hd_wq_bytes(int T) { return (T <= 256 ? 64LL : 256LL) << 20; }
 
-// Vocabulary ids a piece: a multiple of 256.
-static int hd_piece(int T, int H, int V, bool quant, bool grad) {
-  long long n = ((long long)V + HD_BN - 1) / HD_BN;
-  if (grad) n = std::min(n, HD_DZ_BYTES / (2LL * T * HD_BN));
-  if (quant) n = std::min(n, HD_WQ_BYTES / (2LL * H * HD_BN));
-  return (int)(std::max(n, 1LL) * HD_BN);
+static int hd_cg(int rows) { return rows > HD_BM ? 2 : 1; }
+static long long hd_rounds(long long units, int cg) {
+  const int slots = device_sm_count() / cg;
+  return (units + slots - 1) / slots;
+}
+
+// Vocabulary ids a piece: a multiple of 256, within the bytes above, such that the tiles of its products fill the
+// SMs in few whole rounds (8,192 tokens: pieces of 14,080 instead of 16,384 ids, grad_8k 6 % faster). Costs in
+// blocks of 64 of a contraction; a launch costs about 15.
+static int hd_piece(int T, int H, int V, bool quant, bool grad, bool dw) {
+  const long long all = ((long long)V + HD_BN - 1) / HD_BN;
+  long long most = all;
+  if (grad) most = std::min(most, HD_DZ_BYTES / (2LL * T * HD_BN));
+  if (quant) most = std::min(most, hd_wq_bytes(T) / (2LL * H * HD_BN));
+  most = std::max(most, 1LL);
+  if (most == all) return (int)(all * HD_BN);
+  const int cg = hd_cg(T);
+  const long long mt = (T + HD_BM * cg - 1) / (HD_BM * cg), nt = (H + HD_BN - 1) / HD_BN;
+  const long long kh = (H + HD_BK - 1) / HD_BK, kt = (T + HD_BK - 1) / HD_BK;
+  const auto cost = [&](long long n) {
+    long long c = 15 * (1 + (quant ? 1 : 0) + (grad ? 1 : 0) + (dw ? 1 : 0)) + kh * hd_rounds(mt * n, cg);
+    if (dw) c += kt * hd_rounds(nt * n, 2);
+    return c;
+  };
+  long long best = most, best_cost = -1;
+  for (long long n = most; n >= 1 && 2 * n >= most; --n) {
+    const long long last = all % n, c = all / n * cost(n) + (last ? cost(last) : 0);
+    if (best_cost < 0 || c < best_cost) {
+      best = n;
+      best_cost = c;
+    }
+  }
+  return (int)(best * HD_BN);
 }
 
 // Parts of dx's contraction, so that the tiles fill the SMs in whole rounds: the fewest whose last round is within
 // 6 % of full, or the best of up to 8 rounds' worth; each part keeps at least 8 blocks of 64.
 static int hd_splits(int T, int H, int piece) {
-  const int cg = T > HD_BM ? 2 : 1, slots = device_sm_count() / cg;
+  const int cg = hd_cg(T), slots = device_sm_count() / cg;
   const int tiles = ((T + HD_BM * cg - 1) / (HD_BM * cg)) * ((H + HD_BN - 1) / HD_BN);
   const int most = std::max(1, std::min(piece / (8 * HD_BK), std::max(8, slots / tiles)));
   int best = 1;
@@ -709,7 +793,7 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
   HdWork w = {};
   Carver c(base);
   w.nt = (V + HD_BN - 1) / HD_BN;
-  w.piece = hd_piece(T, H, V, quant, grad);
+  w.piece = hd_piece(T, H, V, quant, grad, dw);
   if (!grad) {
     w.out.parts = few ? hq_parts(V) : w.nt;
     w.out.part = c.take<float2>((size_t)T * w.out.parts);
@@ -733,7 +817,7 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
     w.dz = c.take<__nv_bfloat16>((size_t)T * w.piece);
     if (dw) w.xz = c.take<__nv_bfloat16>((size_t)T * H);
     if (dx) {
-      w.splits = hd_splits(T, H, w.piece);
+      w.splits = hd_splits(T, H, std::min(w.piece, V));
       w.dx = c.take<float>((size_t)w.splits * T * H);
     }
   }
@@ -763,12 +847,14 @@ static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const HdAr
   cfg.blockDim = HD_THREADS;
   cfg.dynamicSmemBytes = HD_SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CG;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = CG;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = CG > 1;
+  cfg.numAttrs = CG;
   LG_CUDA_TRY(cudaLaunchKernelEx(&cfg, hd_kernel<KIND, CG>, ma, mb, a));
   LG_LAUNCH_CHECK("head");
   return LG_OK;
@@ -784,7 +870,7 @@ struct HdOperand {
 template <int KIND>
 static int hd_launch(const HdOperand& a, const HdOperand& b, HdArgs g, cudaStream_t st) {
   constexpr bool A_MN = KIND == HD_WGRAD, B_MN = KIND == HD_XGRAD || KIND == HD_WGRAD;
-  const int cg = g.M > HD_BM ? 2 : 1;
+  const int cg = hd_cg(g.M);
   g.mt = (g.M + HD_BM * cg - 1) / (HD_BM * cg);
   g.nt = (g.N + HD_BN - 1) / HD_BN;
   CUtensorMap ma, mb;
@@ -817,11 +903,11 @@ static int hd_blocks(long long n) { return (int)std::min<long long>((n + 255) / 
 static int hd_weights(const void* w, const void* ws, const void* wb, int H, int v0, int rows,
                       const HdWork& k, cudaStream_t st) {
   if (!ws) return LG_OK;
-  const long long words = (long long)rows * (H / 8);
-  const size_t at = (size_t)v0 * (H / 8);
-  hd_dequant_kernel<<<hd_blocks(words), 256, 0, st>>>(
-      static_cast<const uint32_t*>(w) + at, static_cast<const __nv_bfloat16*>(ws) + at / 8,
-      static_cast<const __nv_bfloat16*>(wb) + at / 8, words, k.wq);
+  const long long n = (long long)rows * (H / 32);
+  const size_t at = (size_t)v0 * (H / 32);
+  LG_CUDA_TRY(launch_early(hd_dequant_kernel, hd_blocks(n), 256, 0, st, static_cast<const uint4*>(w) + at,
+                           static_cast<const __nv_bfloat16*>(ws) + at / 2,
+                           static_cast<const __nv_bfloat16*>(wb) + at / 2, n, reinterpret_cast<uint4*>(k.wq)));
   LG_LAUNCH_CHECK("head_dequant");
   return LG_OK;
 }
@@ -829,8 +915,8 @@ static int hd_weights(const void* w, const void* ws, const void* wb, int H, int 
 static int hd_sort(const int* ids, const float* weights, int T, int K, int V, const HdWork& k,
                    cudaStream_t st) {
   if (K == 1) return LG_OK;
-  hd_sort_kernel<<<(T + 7) / 8, 256, 0, st>>>(ids, weights, T, K, V, k.nt, k.sorted, k.order, k.start,
-                                              k.wsum);
+  LG_CUDA_TRY(launch_early(hd_sort_kernel, (T + 7) / 8, 256, 0, st, ids, weights, T, K, V, k.nt, k.sorted, k.order,
+                           k.start, k.wsum));
   LG_LAUNCH_CHECK("head_sort");
   return LG_OK;
 }
@@ -902,7 +988,8 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
       HD_TRY(hd_launch<HD_LOSS>({x, H, T, ldx}, mw, a, st));
     }
   }
-  hd_join_kernel<<<(T + 7) / 8, 256, 0, st>>>(k.out, T, xb, ldx, H, head, ids, weights, K, V, loss, lse, top);
+  LG_CUDA_TRY(launch_early(hd_join_kernel, (T + 7) / 8, 256, 0, st, k.out, T, xb, ldx, H, head, ids, weights, K, V,
+                           loss, lse, (int*)top));
   LG_LAUNCH_CHECK("head_join");
   return LG_OK;
 }
@@ -928,8 +1015,9 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
                 k.bytes);
   HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
   if (dw) {
-    hd_rows_kernel<<<hd_blocks((long long)T * (H / 8)), 256, 0, st>>>(
-        static_cast<const __nv_bfloat16*>(x), ldx, T, H, ids, K, V, k.xz);
+    LG_CUDA_TRY(launch_early(hd_rows_kernel, hd_blocks((long long)T * (H / 8)), 256, 0, st,
+                             static_cast<const __nv_bfloat16*>(x), ldx, T, H, ids, V,
+                             (const unsigned char*)k.start, k.nt, k.xz));
     LG_LAUNCH_CHECK("head_rows");
   }
   for (int v0 = 0; v0 < V; v0 += k.piece) {
@@ -963,14 +1051,15 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
       b.N = H;
       b.kblocks = (T + HD_BK - 1) / HD_BK;
       b.dw = static_cast<__nv_bfloat16*>(dw);
+      b.wide = aligned(dw, 32) && H % 16 == 0;
       HD_TRY(hd_launch<HD_WGRAD>(mz, {k.xz, H, T, H}, b, st));
     }
   }
   if (dx) {
     // The last piece may have fewer parts than the first; later parts then kept the earlier sums.
     const int parts = std::min(k.splits, (std::min(k.piece, V) + HD_BK - 1) / HD_BK);
-    hd_sum_kernel<<<hd_blocks((long long)T * H / 4), 256, 0, st>>>(k.dx, parts, (long long)T * H,
-                                                                  static_cast<__nv_bfloat16*>(dx));
+    LG_CUDA_TRY(launch_early(hd_sum_kernel, hd_blocks((long long)T * H / 4), 256, 0, st, (const float*)k.dx, parts,
+                             (long long)T * H, static_cast<__nv_bfloat16*>(dx)));
     LG_LAUNCH_CHECK("head_sum");
   }
   return LG_OK;

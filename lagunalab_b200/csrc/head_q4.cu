@@ -169,6 +169,9 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   const uint32_t tmem = *tmem_base;        // accumulators: columns [0, 64 NT)
   const uint32_t tmem_a = tmem + 64 * NT;  // weights: 64 columns a slot
 
+  // Every kernel of the call's stream before hq_order_kernel has ended; that one's x and ids are waited for by those
+  // who read them, while the words already come.
+  if (warp == 2 || warp >= 4 + HQ_UNPACK) pdl_wait();
   if (warp == 0) {
     if (elect_one()) {
       int st = 0, used = 0;
@@ -463,6 +466,7 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   tc_fence_after();
   if (warp == 3) tmem_dealloc(tmem, 512);
   // The four warps' parts, in their order.
+  pdl_trigger();
   if (threadIdx.x < a.T) {
     const int t = threadIdx.x;
     float mx = -INFINITY, sum = 0.f;
@@ -490,6 +494,8 @@ __global__ void __launch_bounds__(256) hq_order_kernel(const __nv_bfloat16* __re
                                                        int per, __nv_bfloat16* __restrict__ out,
                                                        const int* __restrict__ ids, int T, int K, int nt,
                                                        int* __restrict__ idt) {
+  pdl_wait();
+  pdl_trigger();
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i < K * nt) {
     const int t = i % nt, j = i / nt;
@@ -540,7 +546,7 @@ static int hq_launch(const CUtensorMap (&m)[4], const HqArgs& a, int grid, size_
     LG_CUDA_TRY(cudaFuncSetAttribute(hq_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, HQ_SMEM_MAX));
     if (dev < 64) done[dev].store(true, std::memory_order_relaxed);
   }
-  hq_kernel<NT><<<grid, HQ_THREADS, smem, st>>>(m[0], m[1], m[2], m[3], a);
+  LG_CUDA_TRY(launch_early(hq_kernel<NT>, grid, HQ_THREADS, smem, st, m[0], m[1], m[2], m[3], a));
   LG_LAUNCH_CHECK("head_q4");
   return LG_OK;
 }
@@ -559,7 +565,8 @@ int hq_loss_parts(const __nv_bfloat16* x, long long ldx, int T, int H, const HdH
   a.out = out;
   const int n = T * (H / 8);
   const int nt = 32 * hq_nt(T);
-  hq_order_kernel<<<(std::max(n, K * nt) + 255) / 256, 256, 0, st>>>(x, ldx, n, H / 8, xp, ids, T, K, nt, idt);
+  LG_CUDA_TRY(launch_early(hq_order_kernel, (std::max(n, K * nt) + 255) / 256, 256, 0, st, x, ldx, n, H / 8, xp, ids, T,
+                           K, nt, idt));
   LG_LAUNCH_CHECK("head_order");
   const uint64_t groups = (uint64_t)V * (H / 64), gbytes = align_up(groups * 2, 16);
   CUtensorMap m[4];

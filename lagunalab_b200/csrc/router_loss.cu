@@ -18,9 +18,11 @@
 
 namespace lg {
 
-constexpr int RB_WARPS = 16;      // warps a CTA
+constexpr int RB_WARPS = 32;       // warps a CTA of the balance
+constexpr int RG_WARPS = 16;       // and of the gradient
 constexpr int RB_MAXE = 256;
-constexpr int RB_CTA_TOKENS = 64;  // a CTA for so many tokens, up to one CTA an SM
+constexpr int RB_CTA_TOKENS = 64;  // a CTA for so many tokens, up to RB_CTAS: the join reads all of them at once
+constexpr int RB_CTAS = 144;
 constexpr float RB_LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float rb_exp(float x) {  // within 2^-22 + |x| 2^-23
@@ -108,11 +110,13 @@ __device__ __forceinline__ void rb_finish(float prob, int count, int n, int E, c
   }
 }
 
-// Each CTA's sums over its tokens; a grid of one CTA writes the outputs itself.
+// Each CTA's sums over its tokens; a grid of one CTA writes the outputs itself. A warp has four tokens' logits in
+// flight, whatever the mask says of them (a load that waits for the mask costs a second trip to memory).
 template <int N>
 __global__ void __launch_bounds__(RB_WARPS * 32) router_balance_kernel(
     const float* __restrict__ logits, const int* __restrict__ inds, const uint8_t* __restrict__ mask, int T,
     int E, int k, int score_fn, float* __restrict__ part_p, int* __restrict__ part_c, RbOut o) {
+  constexpr int U = N > 4 ? 2 : 4;
   __shared__ float sum_p[RB_WARPS][32 * N];
   __shared__ int hist[RB_MAXE + 1];  // the last: tokens kept
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -121,30 +125,32 @@ __global__ void __launch_bounds__(RB_WARPS * 32) router_balance_kernel(
   float acc[N] = {};
   int kept = 0;
   const int step = gridDim.x * RB_WARPS;
-  for (int t0 = blockIdx.x * RB_WARPS + warp; t0 < T; t0 += 2 * step) {
-    float v[2][N], unused[N];
-    bool keep[2];
+  for (int t0 = blockIdx.x * RB_WARPS + warp; t0 < T; t0 += U * step) {
+    float v[U][N], unused[N];
+    int pick[U];
+    bool keep[U];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {  // two tokens' loads in flight
+    for (int u = 0; u < U; ++u) {
       const int t = t0 + u * step;
-      keep[u] = t < T && (!mask || mask[t]);
+      keep[u] = t < T;
+      pick[u] = -1;
       if (keep[u]) {
         rb_load<N>(v[u], logits + (size_t)t * E, E);
-        for (int j = lane; j < k; j += 32) {
-          const int e = inds[(size_t)t * k + j];
-          if (e >= 0 && e < E) atomicAdd(&hist[e], 1);
-        }
+        if (lane < k) pick[u] = inds[(size_t)t * k + lane];
+        if (mask) keep[u] = mask[t];
       }
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (!keep[u]) continue;
+      if (pick[u] >= 0 && pick[u] < E) atomicAdd(&hist[pick[u]], 1);
       ++kept;
       const float r = 1.f / rb_scores<N, false>(v[u], unused, E, score_fn);
 #pragma unroll
       for (int j = 0; j < N; ++j) acc[j] = fmaf(v[u][j], r, acc[j]);
     }
   }
+  pdl_trigger();
 #pragma unroll
   for (int j = 0; j < N; ++j) sum_p[warp][lane + 32 * j] = acc[j];
   if (lane == 0) atomicAdd(&hist[RB_MAXE], kept);
@@ -160,40 +166,55 @@ __global__ void __launch_bounds__(RB_WARPS * 32) router_balance_kernel(
   } else {
     if (e < E) {
       part_p[(size_t)blockIdx.x * E + e] = p;
-      part_c[(size_t)blockIdx.x * (E + 1) + e] = hist[e];
+      part_c[(size_t)blockIdx.x * E + e] = hist[e];
     }
-    if (e == 0) part_c[(size_t)blockIdx.x * (E + 1) + E] = hist[RB_MAXE];
+    if (e == E) part_c[(size_t)RB_CTAS * E + blockIdx.x] = hist[RB_MAXE];
   }
 }
 
-// Joins the CTAs' sums, in their order: 1,024 threads, 256 a slice of the CTAs.
+// Joins the CTAs' sums, in their order: 1,024 threads, 256 a quarter of the CTAs, each with all of its loads in
+// flight.
 __global__ void __launch_bounds__(1024) router_balance_join_kernel(const float* __restrict__ part_p,
                                                                    const int* __restrict__ part_c, int C,
                                                                    int E, RbOut o) {
+  constexpr int PER = RB_CTAS / 4, HALF = PER / 2;
   __shared__ float sp[4][RB_MAXE];
-  __shared__ int sc[4][RB_MAXE + 1];
+  __shared__ int sc[4][RB_MAXE];
+  __shared__ int sn[32];
+  pdl_wait();
   const int e = threadIdx.x & 255, s = threadIdx.x >> 8;
-  const int a = C * s / 4, b = C * (s + 1) / 4;
   float p = 0.f;
-  int c = 0, n = 0;
-  if (e < E) {
-#pragma unroll 8
-    for (int i = a; i < b; ++i) {
-      p += part_p[(size_t)i * E + e];
-      c += part_c[(size_t)i * (E + 1) + e];
+  int c = 0;
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    const int a = s * PER + h * HALF;
+    float pv[HALF];
+    int cv[HALF];
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) {
+      const bool in = e < E && a + i < C;
+      pv[i] = in ? part_p[(size_t)(a + i) * E + e] : 0.f;
+      cv[i] = in ? part_c[(size_t)(a + i) * E + e] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) {
+      p += pv[i];
+      c += cv[i];
     }
   }
   sp[s][e] = p;
   sc[s][e] = c;
-  if (e == 0) {
-    for (int i = a; i < b; ++i) n += part_c[(size_t)i * (E + 1) + E];
-    sc[s][RB_MAXE] = n;
-  }
+  int n = threadIdx.x < C ? part_c[(size_t)RB_CTAS * E + threadIdx.x] : 0;
+#pragma unroll
+  for (int i = 16; i; i >>= 1) n += __shfl_xor_sync(0xffffffffu, n, i);
+  if ((threadIdx.x & 31) == 0) sn[threadIdx.x >> 5] = n;
   __syncthreads();
   const bool first = s == 0;
   p = first ? sp[0][e] + sp[1][e] + sp[2][e] + sp[3][e] : 0.f;
   c = first ? sc[0][e] + sc[1][e] + sc[2][e] + sc[3][e] : 0;
-  n = sc[0][RB_MAXE] + sc[1][RB_MAXE] + sc[2][RB_MAXE] + sc[3][RB_MAXE];
+  n = 0;
+#pragma unroll
+  for (int i = 0; i < (RB_CTAS + 31) / 32; ++i) n += sn[i];
   rb_finish(p, c, n, E, o);
 }
 
@@ -210,10 +231,10 @@ struct RgArgs {
 };
 
 template <int N>
-__global__ void __launch_bounds__(RB_WARPS * 32) router_grad_kernel(const RgArgs a) {
-  __shared__ float sh_s[RB_WARPS][32 * N];  // a token's scores, for its picks
-  __shared__ float sh_d[RB_WARPS][32 * N];  // its picks' gradients; zeros between tokens
-  __shared__ int sh_t[RB_WARPS][32 * N];    // which pick has an expert
+__global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs a) {
+  __shared__ float sh_s[RG_WARPS][32 * N];  // a token's scores, for its picks
+  __shared__ float sh_d[RG_WARPS][32 * N];  // its picks' gradients; zeros between tokens
+  __shared__ int sh_t[RG_WARPS][32 * N];    // which pick has an expert
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float *ss = sh_s[warp], *sd = sh_d[warp];
   int* st = sh_t[warp];
@@ -239,7 +260,7 @@ __global__ void __launch_bounds__(RB_WARPS * 32) router_grad_kernel(const RgArgs
     for (int j = 0; j < N; ++j) dq[j] = f * (float)c[j];
   }
   __syncwarp();
-  for (int t = blockIdx.x * RB_WARPS + warp; t < a.T; t += gridDim.x * RB_WARPS) {
+  for (int t = blockIdx.x * RG_WARPS + warp; t < a.T; t += gridDim.x * RG_WARPS) {
     float* out = a.dl + (size_t)t * a.E;
     if (a.mask && !a.mask[t]) {
 #pragma unroll
@@ -311,7 +332,7 @@ __global__ void __launch_bounds__(RB_WARPS * 32) router_grad_kernel(const RgArgs
 }
 
 static int rb_ctas(int T) {
-  return std::max(1, std::min(device_sm_count(), (T + RB_CTA_TOKENS - 1) / RB_CTA_TOKENS));
+  return std::max(1, std::min(RB_CTAS, (T + RB_CTA_TOKENS - 1) / RB_CTA_TOKENS));
 }
 
 static int rb_check(const char* who, const void* logits, const void* inds, int T, int E, int k, int score_fn) {
@@ -337,8 +358,8 @@ static int rb_check(const char* who, const void* logits, const void* inds, int T
 using namespace lg;
 
 extern "C" size_t lg_router_balance_workspace_bytes(int T, int E) {
-  const size_t C = rb_ctas(T), e = E > 0 ? E : 1;
-  return align_up(C * e * 4, 256) + align_up(C * (e + 1) * 4, 256);
+  const size_t C = rb_ctas(T) > 1 ? RB_CTAS : 0, e = E > 0 ? E : 1;
+  return align_up(C * e * 4, 256) + align_up(C * (e + 1) * 4, 256);  // 0: one CTA needs none
 }
 
 extern "C" int lg_router_balance(const float* logits, const int32_t* inds, const uint8_t* mask, int T, int E,
@@ -348,12 +369,12 @@ extern "C" int lg_router_balance(const float* logits, const int32_t* inds, const
   if (rc != LG_OK) return rc;
   LG_CHECK_ARG(loss && counts && probs && tokens, "router_balance: NULL output");
   const size_t need = lg_router_balance_workspace_bytes(T, E);
-  if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
+  if (need && (!workspace || !aligned(workspace, 256) || workspace_bytes < need))
     return fail(LG_ERR_WORKSPACE, "router_balance: workspace of %zu bytes, need %zu", workspace_bytes, need);
   const int C = rb_ctas(T);
   Carver w(workspace);
-  float* pp = w.take<float>((size_t)C * E);
-  int* pc = w.take<int>((size_t)C * (E + 1));
+  float* pp = w.take<float>((size_t)RB_CTAS * E);
+  int* pc = w.take<int>((size_t)RB_CTAS * (E + 1));
   const RbOut o = {loss, counts, probs, tokens};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define RB_CALL(N)                                                                               \
@@ -362,7 +383,7 @@ extern "C" int lg_router_balance(const float* logits, const int32_t* inds, const
 #undef RB_CALL
   LG_LAUNCH_CHECK("router_balance");
   if (C > 1) {
-    router_balance_join_kernel<<<1, 1024, 0, st>>>(pp, pc, C, E, o);
+    LG_CUDA_TRY(launch_early(router_balance_join_kernel, 1, 1024, 0, st, (const float*)pp, (const int*)pc, C, E, o));
     LG_LAUNCH_CHECK("router_balance_join");
   }
   return LG_OK;
@@ -378,9 +399,9 @@ extern "C" int lg_router_grad(const float* logits, const int32_t* inds, const fl
   LG_CHECK_ARG(dw || counts, "router_grad: neither dw nor a balance loss");
   LG_CHECK_ARG(dlogits, "router_grad: NULL output");
   const RgArgs a = {logits, inds, dw, mask, counts, tokens, weight, T, E, k, norm_topk_prob, score_fn, dlogits};
-  const int grid = std::max(1, std::min(2 * device_sm_count(), (T + RB_WARPS - 1) / RB_WARPS));
+  const int grid = std::max(1, std::min(2 * device_sm_count(), (T + RG_WARPS - 1) / RG_WARPS));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define RB_CALL(N) router_grad_kernel<N><<<grid, RB_WARPS * 32, 0, st>>>(a)
+#define RB_CALL(N) router_grad_kernel<N><<<grid, RG_WARPS * 32, 0, st>>>(a)
   RB_BY_E(E, RB_CALL);
 #undef RB_CALL
   LG_LAUNCH_CHECK("router_grad");

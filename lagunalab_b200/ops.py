@@ -915,25 +915,31 @@ HEAD_TARGETS = 64  # ids a token of head_loss, at most
 
 
 def _rows16(t):
-    """``t`` [n, H] bf16 with rows that TMA reads in place (unit columns, 16-byte steps), or a copy."""
+    """``t`` [n, H] bf16 with rows that TMA reads in place (unit columns, 16-byte steps), and their
+    distance; or a copy."""
+    ld, one = t.stride()
     n, H = t.shape
-    ld = t.stride(0) if n > 1 else max(t.stride(0), H)
-    if t.stride(1) != 1 or ld % 8 or ld < H or t.data_ptr() % 16:
+    if n == 1 and ld < H:
+        ld = H
+    if one != 1 or ld % 8 or ld < H or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
         ld = H
     return t, ld
 
 
 def _head_args(who, x, head, ids, weights):
-    """(device index, T, H, V, K, the leading arguments of lg_head_loss and lg_head_loss_grad, what
-    they point to)."""
+    """(device index, sizes and bits as the workspace functions take them, the leading arguments of
+    lg_head_loss and lg_head_loss_grad, what they point to)."""
     _dev(x)
     index = x.get_device()
     if x.dim() != 2 or x.dtype is not _BF16:
         raise ValueError(f"{who}: x must be bf16 [T, H]")
     T, H = x.shape
+    x, ldx = _rows16(x)
     if isinstance(head, tuple):
-        q, s, b = (_dev(m) and (m if m.is_contiguous() else m.contiguous()) for m in head)
+        q, s, b = head
+        for m in head:
+            _dev(m)
         if q.dtype is torch.uint32:
             q = q.view(_I32)
         V = q.shape[0]
@@ -942,9 +948,10 @@ def _head_args(who, x, head, ids, weights):
                 s.dtype is not _BF16 or b.dtype is not _BF16:
             raise ValueError(f"{who}: a 4-bit group-64 head of {H} columns is int32 words [V, {H // 8}], "
                              f"bf16 scales and biases [V, {H // 64}]")
+        q, s, b = q.contiguous(), s.contiguous(), b.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-        keep = (q, s, b)
+        keep, bits = (q, s, b), 4
         w, ldw, sp, bp = q.data_ptr(), H, s.data_ptr(), b.data_ptr()
     else:
         _dev(head)
@@ -953,29 +960,39 @@ def _head_args(who, x, head, ids, weights):
                              "(words, scales, biases)")
         V = head.shape[0]
         head, ldw = _rows16(head)
-        keep = (head,)
+        keep, bits = (head,), 16
         w, sp, bp = head.data_ptr(), None, None
     if V < 1:
         raise ValueError(f"{who}: the head has no rows")
-    if any(m.get_device() != index for m in keep):
-        raise ValueError(f"{who}: the head is not on {x.device}")
+    for m in keep:
+        if m.get_device() != index:
+            raise ValueError(f"{who}: the head is not on {x.device}")
     _dev(ids)
-    if ids.dtype is not _I32 or ids.dim() not in (1, 2) or ids.shape[0] != T or \
-            ids.get_device() != index:
+    shape = ids.shape
+    if ids.dtype is not _I32 or len(shape) not in (1, 2) or shape[0] != T or ids.get_device() != index:
         raise ValueError(f"{who}: ids must be int32 [{T}] or [{T}, K] on {x.device}")
-    K = 1 if ids.dim() == 1 else ids.shape[1]
+    K = 1 if len(shape) == 1 else shape[1]
     if not 1 <= K <= HEAD_TARGETS:
         raise ValueError(f"{who}: {K} targets a token, not 1 to {HEAD_TARGETS}")
-    ids = ids.contiguous()
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    wp = None
     if weights is not None:
         _dev(weights)
-        if weights.dtype is not torch.float32 or weights.numel() != T * K or \
-                weights.shape[:1] != (T,) or weights.get_device() != index:
-            raise ValueError(f"{who}: weights must be fp32 like ids, {tuple(ids.shape)}, on {x.device}")
-        weights = weights.contiguous()
-    x, ldx = _rows16(x)
-    args = (x.data_ptr(), ldx, T, H, w, ldw, sp, bp, V, ids.data_ptr(), _p(weights), K)
-    return index, T, H, V, K, args, (x, keep, ids, weights)
+        if weights.dtype is not torch.float32 or weights.shape != shape or weights.get_device() != index:
+            raise ValueError(f"{who}: weights must be fp32 like ids, {tuple(shape)}, on {x.device}")
+        if not weights.is_contiguous():
+            weights = weights.contiguous()
+        wp = weights.data_ptr()
+    args = (x.data_ptr(), ldx, T, H, w, ldw, sp, bp, V, ids.data_ptr(), wp, K)
+    return index, (T, H, V, K, bits), args, (x, keep, ids, weights)
+
+
+@functools.lru_cache(maxsize=256)
+def _on_index(index, name, *sizes):
+    """A size function of the library with device ``index`` current (sizes go by its multiprocessors)."""
+    with torch.cuda.device(index):
+        return getattr(_lib.lib(), name)(*sizes)
 
 
 def head_loss(x, head, ids, weights=None, top=False):
@@ -990,12 +1007,13 @@ def head_loss(x, head, ids, weights=None, top=False):
     or None for 1. Negative ids are left out; a token without any other has loss 0, one with an id
     >= V has loss NaN. Returns (loss, lse) fp32 [T], with ``top`` also the id of each token's
     largest logit, int32 [T]. Logits and sums are fp32."""
-    index, T, H, V, K, args, keep = _head_args("head_loss", x, head, ids, weights)
-    dev = x.device
-    loss, lse = torch.empty(2, T, dtype=torch.float32, device=dev)
+    index, sizes, args, keep = _head_args("head_loss", x, head, ids, weights)
+    dev, T = x.device, sizes[0]
+    loss = torch.empty(T, dtype=torch.float32, device=dev)
+    lse = torch.empty_like(loss)
     ti = torch.empty(T, dtype=_I32, device=dev) if top else None
     if T:
-        nb = _lib.lib().lg_head_loss_workspace_bytes(T, H, V, K, 4 if args[6] else 16, int(bool(top)))
+        nb = _on_index(index, "lg_head_loss_workspace_bytes", *sizes, int(bool(top)))
         ws = torch.empty(nb, dtype=torch.uint8, device=dev)  # of this call alone
         _call_on(index, _lib.lib().lg_head_loss, *args, loss.data_ptr(), lse.data_ptr(), _p(ti),
                  ws.data_ptr(), nb)
@@ -1006,13 +1024,14 @@ def head_loss_grad(x, head, ids, lse, g, weights=None, dx=True, dw=True):
     """The gradient of sum(g * loss) for ``head_loss``'s loss, from the same x, head, ids and weights, its
     ``lse`` and g fp32 [T]: (dx bf16 [T, H] or None, dw bf16 [V, H] or None). A 4-bit head has no
     gradient (``dw=False``). The vocabulary is taken in pieces: the workspace holds at most 256 MB of
-    the logits' gradient. Tokens without a target give a row of zeros in dx and nothing to dw,
-    whatever their rows of x hold. The logits' gradient is rounded to bf16 for the tensor cores,
-    sums are fp32, results rounded once."""
-    index, T, H, V, K, args, keep = _head_args("head_loss_grad", x, head, ids, weights)
+    the logits' gradient, and of a 4-bit head's weights. Tokens without a target give a row of zeros in dx
+    and nothing to dw, whatever their rows of x hold. The logits' gradient is rounded to bf16 for the
+    tensor cores, sums are fp32, results rounded once."""
+    index, sizes, args, keep = _head_args("head_loss_grad", x, head, ids, weights)
+    T, H, V, _, bits = sizes
     if not (dx or dw):
         raise ValueError("head_loss_grad: neither dx nor dw is asked for")
-    if dw and args[6]:
+    if dw and bits == 4:
         raise ValueError("head_loss_grad: a 4-bit head has no gradient (dw=False)")
     for t, name in ((lse, "lse"), (g, "g")):
         _dev(t)
@@ -1021,8 +1040,7 @@ def head_loss_grad(x, head, ids, lse, g, weights=None, dx=True, dw=True):
     lse, g = lse.contiguous(), g.contiguous()
     gx = torch.empty(T, H, dtype=_BF16, device=x.device) if dx else None
     gw = torch.empty(V, H, dtype=_BF16, device=x.device) if dw else None
-    nb = _lib.lib().lg_head_loss_grad_workspace_bytes(T, H, V, K, 4 if args[6] else 16, int(bool(dx)),
-                                                      int(bool(dw)))
+    nb = _on_index(index, "lg_head_loss_grad_workspace_bytes", *sizes, int(bool(dx)), int(bool(dw)))
     ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
     _call_on(index, _lib.lib().lg_head_loss_grad, *args, lse.data_ptr(), g.data_ptr(), _p(gx), _p(gw),
              ws.data_ptr(), nb)
@@ -1069,12 +1087,13 @@ def router_balance(logits, inds, score_fn="sigmoid", mask=None):
     dev = logits.device
     real = torch.empty(1 + E, dtype=torch.float32, device=dev)
     whole = torch.empty(1 + E, dtype=_I32, device=dev)
-    nb = _lib.lib().lg_router_balance_workspace_bytes(T, E)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    nb = _on_index(index, "lg_router_balance_workspace_bytes", T, E)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
     fp, wp = real.data_ptr(), whole.data_ptr()
     _call_on(index, _lib.lib().lg_router_balance, logits.data_ptr(), inds.data_ptr(), _p(mask), T, E, k,
-             _SCORES[score_fn], fp, wp + 4, fp + 4, wp, ws.data_ptr(), nb)
-    return RouterBalance(real[:1], whole[1:], real[1:], whole[:1])
+             _SCORES[score_fn], fp, wp + 4, fp + 4, wp, _p(ws), nb)
+    (loss, probs), (tokens, counts) = real.split_with_sizes((1, E)), whole.split_with_sizes((1, E))
+    return RouterBalance(loss, counts, probs, tokens)
 
 
 def router_grad(logits, inds, dw=None, norm_topk_prob=True, score_fn="sigmoid", balance=None,

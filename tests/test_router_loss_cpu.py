@@ -38,8 +38,8 @@ def test_gradient_refuses(bad):
 
 
 def test_workspace():
-    need = _lib.lib().lg_router_balance_workspace_bytes(4, 16)
+    need = _lib.lib().lg_router_balance_workspace_bytes(4000, 16)
     for bad in (dict(ws=None), dict(nb=need - 1), dict(ws=ctypes.c_void_p(0x1010))):
         with pytest.raises(_lib.LagunaError) as e:
-            _balance(**bad)
+            _balance(T=4000, **bad)
         assert e.value.code == _lib.LG_ERR_WORKSPACE
