@@ -74,13 +74,16 @@ __device__ __forceinline__ void hd_sub(float (&v)[32], int c, float w) {
 
 // Sixteen bf16 of a row as one 32-byte store: a thread has a row of its own, so that a narrower store would leave
 // its sector of L2 half written.
+__device__ __forceinline__ void hd_store32(__nv_bfloat16* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void hd_store16(__nv_bfloat16* p, const float* v) {
   uint32_t r[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) r[i] = hd_pack(v[2 * i], v[2 * i + 1]);
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
+  hd_store32(p, r);
 }
 
 // A unit of work: tile (m, n) of the output, and the part [k0, k1) of the contraction's blocks.
@@ -455,12 +458,18 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
   }
 }
 
-// The eight weights of a word: bf16(scale * code + bias).
-__device__ __forceinline__ void hd_unpack(uint32_t q, float scale, float bias, uint32_t (&r)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    r[j] = hd_pack(fmaf(scale, (float)((q >> (8 * j)) & 15u), bias),
-                   fmaf(scale, (float)((q >> (8 * j + 4)) & 15u), bias));
+// The eight weights of a word, in their order, from the bf16 bits of scale and bias.
+__device__ __forceinline__ void hd_unpack(uint32_t q, uint16_t scale, uint16_t bias, uint32_t* r) {
+  const uint32_t s2 = scale | (uint32_t)scale << 16, b2 = bias | (uint32_t)bias << 16;
+  uint32_t v[4];
+  if (q4_fast(s2))
+    q4_word(q, s2, b2, v);
+  else
+    q4_word_any(q, s2, b2, v);
+  r[0] = __byte_perm(v[0], v[1], 0x5410);
+  r[1] = __byte_perm(v[2], v[3], 0x5410);
+  r[2] = __byte_perm(v[0], v[1], 0x7632);
+  r[3] = __byte_perm(v[2], v[3], 0x7632);
 }
 
 // ---- small kernels ------------------------------------------------------------------------------
@@ -515,131 +524,164 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
   if (lane == 0) wsum[t] = sum;
 }
 
-// sum_h x_h W_vh of one row each by a warp, in fp32 with each sum rounded to nearest.
+constexpr int HJ_THREADS = 128;
+
+// sum_h x_h W_vh by a warp, in fp32 with each sum rounded to nearest.
+template <bool QUANT>
 __device__ __forceinline__ float hd_dot(const HdHead& w, const __nv_bfloat16* x, int H, int v) {
+  constexpr int U = 4;
   const int lane = threadIdx.x & 31;
   float s = 0.f;
-#pragma unroll 8
-  for (int c = lane * 8; c < H; c += 256) {
-    const uint4 xv = *reinterpret_cast<const uint4*>(x + c);
-    const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
-    uint32_t ws[4];
-    if (w.scales) {
-      const uint32_t q = static_cast<const uint32_t*>(w.w)[(size_t)v * (H / 8) + c / 8];
-      const size_t g = (size_t)v * (H / 64) + c / 64;
-      hd_unpack(q, bf2f(w.scales[g]), bf2f(w.biases[g]), ws);
-    } else {
-      const uint4 wv = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w.w) + (size_t)v * w.ld + c);
-      ws[0] = wv.x;
-      ws[1] = wv.y;
-      ws[2] = wv.z;
-      ws[3] = wv.w;
+  for (int c0 = lane * 8; c0 < H; c0 += U * 256) {  // four chunks' loads before their sums
+    uint4 xv[U], wv[U];
+    uint32_t q[U];
+    uint16_t sc[U], bi[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * 256;
+      xv[u] = wv[u] = make_uint4(0, 0, 0, 0);
+      q[u] = 0;
+      sc[u] = bi[u] = 0;
+      if (c < H) {
+        xv[u] = *reinterpret_cast<const uint4*>(x + c);
+        if (QUANT) {
+          q[u] = static_cast<const uint32_t*>(w.w)[(size_t)v * (H / 8) + c / 8];
+          sc[u] = reinterpret_cast<const uint16_t*>(w.scales)[(size_t)v * (H / 64) + c / 64];
+          bi[u] = reinterpret_cast<const uint16_t*>(w.biases)[(size_t)v * (H / 64) + c / 64];
+        } else {
+          wv[u] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w.w) + (size_t)v * w.ld + c);
+        }
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ws[i] << 16), s);
-      s = fmaf(__uint_as_float(xs[i] & 0xffff0000u), __uint_as_float(ws[i] & 0xffff0000u), s);
+    for (int u = 0; u < U; ++u) {
+      const uint32_t xs[4] = {xv[u].x, xv[u].y, xv[u].z, xv[u].w};
+      uint32_t ws[4] = {wv[u].x, wv[u].y, wv[u].z, wv[u].w};
+      if (QUANT) hd_unpack(q[u], sc[u], bi[u], ws);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ws[i] << 16), s);
+        s = fmaf(__uint_as_float(xs[i] & 0xffff0000u), __uint_as_float(ws[i] & 0xffff0000u), s);
+      }
     }
   }
   return warp_sum(s);
 }
 
-// A warp joins a token's parts (maximum, sum of exponentials, the maximum's id): lse, the loss, the id of the
+// (maximum, sum of exponentials from it, the maximum's lowest id) of two parts, the first before the second.
+struct HdStat {
+  float mx, sum;
+  int arg;
+};
+__device__ __forceinline__ HdStat hd_merge(const HdStat& a, const HdStat& b) {
+  HdStat r;
+  r.mx = fmaxf(a.mx, b.mx);
+  const float ea = a.mx == r.mx ? 1.f : hd_ex2((a.mx - r.mx) * HD_LOG2E);
+  const float eb = b.mx == r.mx ? 1.f : hd_ex2((b.mx - r.mx) * HD_LOG2E);
+  r.sum = a.sum * ea + b.sum * eb;
+  r.arg = b.mx > a.mx || (b.mx == a.mx && b.arg < a.arg) ? b.arg : a.arg;
+  return r;
+}
+
+// A CTA joins a token's parts (maximum, sum of exponentials, the maximum's id): lse, the loss, the id of the
 // largest logit.
 //
 // The tensor cores' accumulators are cut, not rounded, after each step: a logit of 11 that H = 2048 like-signed
 // products make is 1e-5 too small, more than all other errors together (loss off by 1.5e-6 in the 2-norm
 // against 64 bits, 3e-7 with an fp32 product). The logits of targets with an eighth or more of the token's
-// weight are therefore summed again here, in fp32 rounded to nearest, and take their first value's
-// place in lse too.
-__global__ void __launch_bounds__(256) hd_join_kernel(HdParts in, int T, const __nv_bfloat16* __restrict__ x,
-                                                      long long ldx, int H, HdHead w,
-                                                      const int* __restrict__ ids,
-                                                      const float* __restrict__ weights, int K, int V,
-                                                      float* __restrict__ loss,
-                                                      float* __restrict__ lse_out,
-                                                      int* __restrict__ top) {
+// weight, eight at most, are therefore summed again here, in fp32 rounded to nearest, and take their first
+// value's place in lse too. A warp sums one target's; the four work side by side.
+template <bool QUANT>
+__global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const __nv_bfloat16* __restrict__ x,
+                                                             long long ldx, int H, HdHead w,
+                                                             const int* __restrict__ ids,
+                                                             const float* __restrict__ weights, int K, int V,
+                                                             float* __restrict__ loss,
+                                                             float* __restrict__ lse_out,
+                                                             int* __restrict__ top) {
+  constexpr int WARPS = HJ_THREADS / 32;
+  __shared__ HdStat sh[WARPS];
+  __shared__ float sh_dot[HD_MAXK];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = blockIdx.x * 8 + warp;
-  if (t >= T) return;
+  const int t = blockIdx.x;
   const int parts = in.parts;
-  const float2* row = in.part + (size_t)t * parts;
-  float mx = -INFINITY, sum = 0.f;
-  int at = -1;
-#pragma unroll 8
-  for (int n = lane; n < parts; n += 32) {
-    const float2 v = row[n];
-    if (v.x > mx) {
-      sum = sum * hd_ex2((mx - v.x) * HD_LOG2E) + v.y;
-      mx = v.x;
-      at = n;
-    } else {
-      sum += v.x == -INFINITY ? v.y : v.y * hd_ex2((v.x - mx) * HD_LOG2E);
-    }
-  }
-  int arg = top && at >= 0 ? in.top[(size_t)t * parts + at] : 0x7fffffff;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, mx, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
-    const int a2 = __shfl_xor_sync(0xffffffffu, arg, o);
-    const float m = fmaxf(mx, m2);
-    const float ea = mx == m ? 1.f : hd_ex2((mx - m) * HD_LOG2E);
-    const float eb = m2 == m ? 1.f : hd_ex2((m2 - m) * HD_LOG2E);
-    // Both lanes of a pair add in the same order, the lower lane's part first.
-    sum = (lane & o) ? s2 * eb + sum * ea : sum * ea + s2 * eb;
-    arg = m2 > mx || (m2 == mx && a2 < arg) ? a2 : arg;
-    mx = m;
-  }
-  sum = __shfl_sync(0xffffffffu, sum, 0);
-  // the targets: two a lane
+  // the targets: two a lane, the same in every warp
   int id[2];
   float wt[2], z[2];
-  float all = 0.f;
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int j = lane + 32 * i;
     id[i] = j < K ? ids[(size_t)t * K + j] : -1;
-    if (id[i] >= V) {
-      bad = true;
-      id[i] = -1;
-    }
+    bad = bad || id[i] >= V;
+    if (id[i] >= V) id[i] = -1;
     wt[i] = id[i] < 0 ? 0.f : weights ? weights[(size_t)t * K + j] : 1.f;
     z[i] = id[i] < 0 ? 0.f : in.ztgt[(size_t)t * K + j];
-    all += fabsf(wt[i]);
   }
-  all = warp_sum(all);
+  const float2* row = in.part + (size_t)t * parts;
+  HdStat st = {-INFINITY, 0.f, 0x7fffffff};
+#pragma unroll 4
+  for (int n = threadIdx.x; n < parts; n += HJ_THREADS) {
+    const float2 v = row[n];
+    st = hd_merge(st, {v.x, v.y, top ? in.top[(size_t)t * parts + n] : 0});
+  }
+  const float all = warp_sum(fabsf(wt[0]) + fabsf(wt[1]));
+  // The list of heavy targets, an id once: every warp has it, and sums its share.
+  unsigned long long todo = 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    unsigned todo = __ballot_sync(0xffffffffu, id[i] >= 0 && 8.f * fabsf(wt[i]) >= all);
-    while (todo) {
-      const int src = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const int v = __shfl_sync(0xffffffffu, id[i], src);
-      const float was = __shfl_sync(0xffffffffu, z[i], src);
-      const float now = hd_dot(w, x + (size_t)t * ldx, H, v);
-      sum += hd_ex2((now - mx) * HD_LOG2E) - hd_ex2((was - mx) * HD_LOG2E);
-      // every place of the list that names it: once in the sum
+  for (int i = 0; i < 2; ++i)
+    todo |= (unsigned long long)__ballot_sync(0xffffffffu, id[i] >= 0 && 8.f * fabsf(wt[i]) >= all) << (32 * i);
+  const unsigned long long heavy = todo;
+  int n = 0;
+  while (todo) {
+    const int j = __ffsll(todo) - 1;
+    const int v = __shfl_sync(0xffffffffu, j < 32 ? id[0] : id[1], j & 31);
+    if (n % WARPS == warp) {
+      const float d = hd_dot<QUANT>(w, x + (size_t)t * ldx, H, v);
+      if (lane == 0) sh_dot[n] = d;
+    }
+    ++n;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (id[u] == v) z[u] = now;
-      todo &= ~__ballot_sync(0xffffffffu, id[i] == v);
-      if (i == 0 && id[1] == v) id[1] = -2;  // summed already
+    for (int i = 0; i < 2; ++i)
+      todo &= ~((unsigned long long)__ballot_sync(0xffffffffu, id[i] == v) << (32 * i));
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const HdStat p = {__shfl_xor_sync(0xffffffffu, st.mx, o), __shfl_xor_sync(0xffffffffu, st.sum, o),
+                      __shfl_xor_sync(0xffffffffu, st.arg, o)};
+    st = (lane & o) ? hd_merge(p, st) : hd_merge(st, p);
+  }
+  if (lane == 0) sh[warp] = st;
+  __syncthreads();
+  if (warp) return;
+  st = sh[0];
+#pragma unroll
+  for (int i = 1; i < WARPS; ++i) st = hd_merge(st, sh[i]);
+  todo = heavy;
+  for (n = 0; todo; ++n) {
+    const int j = __ffsll(todo) - 1;
+    const int v = __shfl_sync(0xffffffffu, j < 32 ? id[0] : id[1], j & 31);
+    const float was = __shfl_sync(0xffffffffu, j < 32 ? z[0] : z[1], j & 31), now = sh_dot[n];
+    st.sum += hd_ex2((now - st.mx) * HD_LOG2E) - hd_ex2((was - st.mx) * HD_LOG2E);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (id[i] == v) z[i] = now;  // every place of the list that names it
+      todo &= ~((unsigned long long)__ballot_sync(0xffffffffu, id[i] == v) << (32 * i));
     }
   }
-  const float lse = mx + logf(sum);
+  const float lse = st.mx + logf(st.sum);
   float l = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    if (id[i] != -1) l += wt[i] * (lse - z[i]);
+    if (id[i] >= 0) l += wt[i] * (lse - z[i]);
   l = warp_sum(l);
   bad = __any_sync(0xffffffffu, bad);
   if (lane == 0) {
     loss[t] = bad ? __int_as_float(0x7fffffff) : l;
     lse_out[t] = lse;
-    if (top) top[t] = arg == 0x7fffffff ? 0 : arg;
+    if (top) top[t] = st.arg == 0x7fffffff ? 0 : st.arg;
   }
 }
 
@@ -661,38 +703,36 @@ __global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __res
   }
 }
 
-// Rows of a 4-bit group-64 head as bf16: bf16(scale * code + bias), half a group (four words) a thread.
-__global__ void __launch_bounds__(256) hd_dequant_kernel(const uint4* __restrict__ q,
-                                                         const __nv_bfloat16* __restrict__ s,
-                                                         const __nv_bfloat16* __restrict__ b, long long n,
-                                                         uint4* __restrict__ out) {
+// Rows of a 4-bit group-64 head as bf16: bf16(scale * code + bias), two words a thread: a warp writes 1 KB in one
+// store (four words a thread with 16-byte stores: 3 TB/s written instead of 4.3).
+__global__ void __launch_bounds__(256) hd_dequant_kernel(const uint2* __restrict__ q,
+                                                         const uint16_t* __restrict__ s,
+                                                         const uint16_t* __restrict__ b, long long n,
+                                                         __nv_bfloat16* __restrict__ out) {
   pdl_wait();
   pdl_trigger();
   constexpr int U = 4;
   const long long step = gridDim.x * 256LL;
   for (long long i0 = blockIdx.x * 256LL + threadIdx.x; i0 < n; i0 += U * step) {
-    uint4 w[U];
-    float sc[U], bi[U];
+    uint2 w[U];
+    uint16_t sc[U], bi[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long long i = i0 + u * step;
       if (i < n) {
         w[u] = q[i];
-        sc[u] = bf2f(s[i >> 1]);
-        bi[u] = bf2f(b[i >> 1]);
+        sc[u] = s[i >> 2];
+        bi[u] = b[i >> 2];
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long long i = i0 + u * step;
       if (i >= n) break;
-      const uint32_t v[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t r[4];
-        hd_unpack(v[j], sc[u], bi[u], r);
-        out[4 * i + j] = make_uint4(r[0], r[1], r[2], r[3]);
-      }
+      uint32_t r[8];
+      hd_unpack(w[u].x, sc[u], bi[u], r);
+      hd_unpack(w[u].y, sc[u], bi[u], r + 4);
+      hd_store32(out + 16 * i, r);
     }
   }
 }
@@ -903,11 +943,10 @@ static int hd_blocks(long long n) { return (int)std::min<long long>((n + 255) / 
 static int hd_weights(const void* w, const void* ws, const void* wb, int H, int v0, int rows,
                       const HdWork& k, cudaStream_t st) {
   if (!ws) return LG_OK;
-  const long long n = (long long)rows * (H / 32);
-  const size_t at = (size_t)v0 * (H / 32);
-  LG_CUDA_TRY(launch_early(hd_dequant_kernel, hd_blocks(n), 256, 0, st, static_cast<const uint4*>(w) + at,
-                           static_cast<const __nv_bfloat16*>(ws) + at / 2,
-                           static_cast<const __nv_bfloat16*>(wb) + at / 2, n, reinterpret_cast<uint4*>(k.wq)));
+  const long long n = (long long)rows * (H / 16);
+  const size_t at = (size_t)v0 * (H / 16);
+  LG_CUDA_TRY(launch_early(hd_dequant_kernel, hd_blocks(n), 256, 0, st, static_cast<const uint2*>(w) + at,
+                           static_cast<const uint16_t*>(ws) + at / 4, static_cast<const uint16_t*>(wb) + at / 4, n, k.wq));
   LG_LAUNCH_CHECK("head_dequant");
   return LG_OK;
 }
@@ -988,8 +1027,8 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
       HD_TRY(hd_launch<HD_LOSS>({x, H, T, ldx}, mw, a, st));
     }
   }
-  LG_CUDA_TRY(launch_early(hd_join_kernel, (T + 7) / 8, 256, 0, st, k.out, T, xb, ldx, H, head, ids, weights, K, V,
-                           loss, lse, (int*)top));
+  LG_CUDA_TRY(launch_early(quant ? hd_join_kernel<true> : hd_join_kernel<false>, T, HJ_THREADS, 0, st, k.out, xb, ldx, H,
+                           head, ids, weights, K, V, loss, lse, (int*)top));
   LG_LAUNCH_CHECK("head_join");
   return LG_OK;
 }

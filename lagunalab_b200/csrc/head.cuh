@@ -27,6 +27,43 @@ __device__ __forceinline__ uint32_t hd_pack(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// Unpacking a word of eight 4-bit codes to bf16(scale * code + bias) in one rounding, as the pairs (0,4), (1,5),
+// (2,6), (3,7); s2, b2: scale and bias twice.
+//
+// The 16 bits of a pair's half that hold a code c, all else masked away, are the bf16 number c 2^-133 (codes in bits
+// 0-3) or c 2^-129 (bits 4-7): below the exponent 2 a bf16's bits count units of 2^-133. A packed fma with
+// scale 2^133 or scale 2^129 and the bias is the result: a shift, four LOP3 and four fma a word. That takes scales
+// in [2^-126, 2^-5) (q4_fast); any other: 128 + c put together, 128 taken off, 15 instructions a word.
+__device__ __forceinline__ uint32_t q4_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ bool q4_fast(uint32_t s2) {  // both halves' exponents in [1, 121]
+  const uint32_t e = s2 & 0x7F807F80u;
+  return (((e + 0x43004300u) | (e - 0x00800080u)) & 0x80008000u) == 0;
+}
+__device__ __forceinline__ void q4_word(uint32_t w, uint32_t s2, uint32_t b2, uint32_t* v) {
+  const uint32_t lo = s2 + 0x42804280u, hi = s2 + 0x40804080u;  // * 2^133, * 2^129
+  const uint32_t u = w >> 8;
+  v[0] = q4_fma(w & 0x000F000Fu, lo, b2);
+  v[1] = q4_fma(w & 0x00F000F0u, hi, b2);
+  v[2] = q4_fma(u & 0x000F000Fu, lo, b2);
+  v[3] = q4_fma(u & 0x00F000F0u, hi, b2);
+}
+__device__ __forceinline__ void q4_word_any(uint32_t w, uint32_t s2, uint32_t b2, uint32_t* v) {
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    uint32_t c;
+    asm("{\n\t"
+        "lop3.b32 %0, %1, 0x000F000F, 0x43004300, 0xEA;\n\t"
+        "sub.rn.bf16x2 %0, %0, %2;\n\t}"
+        : "=r"(c)
+        : "r"(w >> (4 * p)), "r"(0x43004300u));
+    v[p] = q4_fma(c, s2, b2);
+  }
+}
+
 // The head as the caller has it: bf16 rows `ld` apart, or (scales not NULL) 4-bit words.
 struct HdHead {
   const void* w;

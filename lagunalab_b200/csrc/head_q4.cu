@@ -12,11 +12,7 @@
 //   warps 20-23  per tile and token the maximum and the sum of exponentials over the warp's 32 rows, which lie
 //                across its lanes: a transposing reduction (31 shuffles for 32 columns) leaves token i with lane i
 //
-// Unpacking: the 16 bits of a pair's half that hold a code c, all else masked away, are the bf16 number c 2^-133
-// (codes in bits 0-3) or c 2^-129 (bits 4-7): a subnormal's bits count units of 2^-133. A packed bf16 fma with
-// scale 2^133 or scale 2^129 and the bias therefore gives bf16(scale c + bias) in one rounding: a shift, four LOP3 and
-// four fma for a word's eight codes. It takes scales in [2^-126, 2^-5); a warp with another one
-// puts 128 + c together, takes 128 off and has 15 instructions a word.
+// Unpacking: q4_word (head.cuh); a warp that holds a scale it does not take unpacks by q4_word_any.
 //
 // K order: one LOP3 splits a word into the pairs (0,4), (1,5), (2,6), (3,7); x is copied in that order first
 // (hq_order_kernel), so that no code is moved.
@@ -74,24 +70,6 @@ __device__ __forceinline__ void hq_st32(uint32_t taddr, const uint32_t (&r)[32])
       "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
-}
-
-__device__ __forceinline__ uint32_t hq_fma(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-
-// Codes 4 i and 4 i + 16 of v (already shifted) -> bf16 pair scale * code + bias.
-__device__ __forceinline__ uint32_t hq_pair(uint32_t v, uint32_t s2, uint32_t b2) {
-  uint32_t r;
-  asm("{\n\t.reg .b32 c;\n\t"
-      "lop3.b32 c, %1, 0x000F000F, 0x43004300, 0xEA;\n\t"
-      "sub.rn.bf16x2 c, c, %4;\n\t"
-      "fma.rn.bf16x2 %0, c, %2, %3;\n\t}"
-      : "=r"(r)
-      : "r"(v), "r"(s2), "r"(b2), "r"(0x43004300u));
-  return r;
 }
 
 // Over the warp's lanes: lane i ends with op over all lanes of v[i].
@@ -317,9 +295,7 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
             sw = at[0] | (uint32_t)at[two] << 16;
             bw = bt[0] | (uint32_t)bt[two] << 16;
           }
-          // exponents in [1, 121] (bit 15 of a half says not)
-          const uint32_t e = sw & 0x7F807F80u;
-          const bool fast = __all_sync(0xffffffffu, (((e + 0x43004300u) | (e - 0x00800080u)) & 0x80008000u) == 0);
+          const bool fast = __all_sync(0xffffffffu, q4_fast(sw));
           const uint8_t* row = sm_w + ws * HQ_W_BYTES + r * 128;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -331,21 +307,11 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
             const uint32_t s2 = __byte_perm(sw, 0, h ? 0x3232 : 0x1010), b2 = __byte_perm(bw, 0, h ? 0x3232 : 0x1010);
             uint32_t v[32];
             if (fast) {
-              const uint32_t lo = s2 + 0x42804280u, hi = s2 + 0x40804080u;  // * 2^133, * 2^129
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const uint32_t u = w[j] >> 8;
-                v[4 * j] = hq_fma(w[j] & 0x000F000Fu, lo, b2);
-                v[4 * j + 1] = hq_fma(w[j] & 0x00F000F0u, hi, b2);
-                v[4 * j + 2] = hq_fma(u & 0x000F000Fu, lo, b2);
-                v[4 * j + 3] = hq_fma(u & 0x00F000F0u, hi, b2);
-              }
+              for (int j = 0; j < 8; ++j) q4_word(w[j], s2, b2, v + 4 * j);
             } else {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-#pragma unroll
-                for (int p = 0; p < 4; ++p) v[4 * j + p] = hq_pair(w[j] >> (4 * p), s2, b2);
-              }
+              for (int j = 0; j < 8; ++j) q4_word_any(w[j], s2, b2, v + 4 * j);
             }
             if (h == 0) {
               ok = __all_sync(0xffffffffu, mbar_wait(empty + slot, ph ^ 1, err, 8));

@@ -8,8 +8,10 @@
 // Routing weights w_j = s_j / sum over the token's picks of s (norm) or s_j, for dw given:
 //   ds_j = (dw_j - sum_i dw_i w_i) / sum s (norm) or dw_j;  a sigmoid's or softmax's backward from there.
 //
-// A warp a token, E / 32 scores a lane in registers. Both kernels read the logits once and are bound by
-// HBM on long batches, by launch latency on short ones.
+// A token is worked on by G = 8, 16 or 32 lanes (E up to 64, 128, 256), eight scores a lane, so that a reduction's
+// shuffles serve 32 / G tokens at once: with a warp a token the gradient of 32,768 tokens of 64 experts took 254
+// instructions a token and 14 us. Both kernels read the logits once; the bound is HBM on long batches, launch
+// latency on short ones.
 #include <math.h>
 
 #include <algorithm>
@@ -18,11 +20,11 @@
 
 namespace lg {
 
-constexpr int RB_WARPS = 32;       // warps a CTA of the balance
-constexpr int RG_WARPS = 16;       // and of the gradient
+constexpr int RB_WARPS = 32;  // warps a CTA of the balance
+constexpr int RG_WARPS = 8;   // and of the gradient
+constexpr int RB_N = 8;       // scores a lane
 constexpr int RB_MAXE = 256;
-constexpr int RB_CTA_TOKENS = 64;  // a CTA for so many tokens, up to RB_CTAS: the join reads all of them at once
-constexpr int RB_CTAS = 144;
+constexpr int RB_CTAS = 144;  // of the balance, at most
 constexpr float RB_LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float rb_exp(float x) {  // within 2^-22 + |x| 2^-23
@@ -30,44 +32,83 @@ __device__ __forceinline__ float rb_exp(float x) {  // within 2^-22 + |x| 2^-23
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * RB_LOG2E));
   return y;
 }
+__device__ __forceinline__ float rb_rcp(float x) { return __fdividef(1.f, x); }  // within 2^-22
 
-// The token's scores in place of its logits (0 past E), and their sum over the experts. For a sigmoid `tail` is
-// s (1 - s), without the difference that cancels.
-template <int N, bool TAIL>
-__device__ __forceinline__ float rb_scores(float (&v)[N], float (&tail)[N], int E, int score_fn) {
-  const int lane = threadIdx.x & 31;
+template <int G>
+__device__ __forceinline__ float rb_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int G>
+__device__ __forceinline__ float rb_max(float v) {
+#pragma unroll
+  for (int o = G / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// The expert of a lane's score j: fours of neighbours (VEC: E % 4 == 0, 16-byte rows), or every G-th.
+template <int G, bool VEC>
+__device__ __forceinline__ int rb_expert(int j) {
+  const int l = threadIdx.x % G;
+  return VEC ? 4 * (l + G * (j / 4)) + j % 4 : l + G * j;
+}
+
+template <int G, bool VEC>
+__device__ __forceinline__ void rb_load(float (&v)[RB_N], const float* row, int E, bool in) {
+  const float none = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < RB_N; j += VEC ? 4 : 1) {
+    const int e = rb_expert<G, VEC>(j);
+    if (VEC) {
+      float4 q = make_float4(none, none, none, none);
+      if (in && e < E) q = __ldg(reinterpret_cast<const float4*>(row + e));
+      v[j] = q.x;
+      v[j + 1] = q.y;
+      v[j + 2] = q.z;
+      v[j + 3] = q.w;
+    } else {
+      v[j] = in && e < E ? __ldg(row + e) : none;
+    }
+  }
+}
+
+__device__ __forceinline__ float rb_sigmoid(float x, float* tail) {  // tail: s (1 - s), without the difference
+  const float t = rb_exp(-fabsf(x));                                 // NaN stays
+  const float r = rb_rcp(1.f + t);
+  *tail = t * r * r;
+  return x >= 0.f ? r : t * r;
+}
+
+// The token's scores in place of its logits (-inf past E gives 0). A sigmoid: their sum; softmax: 1, with what one
+// more logit's score takes (the maximum, and the reciprocal of the sum).
+template <int G>
+__device__ __forceinline__ float rb_scores(float (&v)[RB_N], float (&tail)[RB_N], int score_fn, float* mx,
+                                           float* rs) {
   float sum = 0.f;
   if (score_fn == LG_SCORE_SOFTMAX) {
-    float mx = -INFINITY;
+    float m = v[0];
 #pragma unroll
-    for (int j = 0; j < N; ++j) mx = fmaxf(mx, v[j]);
-    mx = warp_max(mx);
+    for (int j = 1; j < RB_N; ++j) m = fmaxf(m, v[j]);
+    m = rb_max<G>(m);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      v[j] = lane + 32 * j < E ? rb_exp(v[j] - mx) : 0.f;
+    for (int j = 0; j < RB_N; ++j) {
+      v[j] = rb_exp(v[j] - m);
       sum += v[j];
     }
-    const float r = 1.f / warp_sum(sum);
+    const float r = rb_rcp(rb_sum<G>(sum));
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] *= r;
+    for (int j = 0; j < RB_N; ++j) v[j] *= r;
+    *mx = m;
+    *rs = r;
     return 1.f;
   }
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const float t = rb_exp(-fabsf(v[j]));  // NaN stays
-    const float r = __fdividef(1.f, 1.f + t);
-    if (TAIL) tail[j] = t * r * r;
-    v[j] = lane + 32 * j < E ? (v[j] >= 0.f ? r : t * r) : 0.f;
+  for (int j = 0; j < RB_N; ++j) {
+    v[j] = rb_sigmoid(v[j], &tail[j]);
     sum += v[j];
   }
-  return warp_sum(sum);
-}
-
-template <int N>
-__device__ __forceinline__ void rb_load(float (&v)[N], const float* row, int E) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int j = 0; j < N; ++j) v[j] = lane + 32 * j < E ? __ldg(row + lane + 32 * j) : -INFINITY;
+  return rb_sum<G>(sum);
 }
 
 struct RbOut {
@@ -77,7 +118,7 @@ struct RbOut {
   int* tokens;
 };
 
-// The sums of one expert over all tokens -> outputs; called by whole CTAs of at least E threads.
+// The sums of expert threadIdx.x over all tokens -> outputs; called by whole CTAs of at least E threads.
 __device__ __forceinline__ void rb_finish(float prob, int count, int n, int E, const RbOut& o) {
   __shared__ float sh_f[32];
   __shared__ long long sh_c[32];
@@ -87,9 +128,8 @@ __device__ __forceinline__ void rb_finish(float prob, int count, int n, int E, c
     o.counts[e] = count;
     o.probs[e] = p;
   }
-  if (e >= E) count = 0;
   float fp = e < E ? (float)count * p : 0.f;
-  long long c = count;
+  long long c = e < E ? count : 0;
   fp = warp_sum(fp);
 #pragma unroll
   for (int s = 16; s; s >>= 1) c += __shfl_xor_sync(0xffffffffu, c, s);
@@ -101,7 +141,7 @@ __device__ __forceinline__ void rb_finish(float prob, int count, int n, int E, c
   if (e == 0) {
     float f = 0.f;
     long long all = 0;
-    for (int i = 0; i < (int)(blockDim.x + 31) / 32; ++i) {
+    for (int i = 0; i < (E + 31) / 32; ++i) {
       f += sh_f[i];
       all += sh_c[i];
     }
@@ -110,108 +150,117 @@ __device__ __forceinline__ void rb_finish(float prob, int count, int n, int E, c
   }
 }
 
-// Each CTA's sums over its tokens; a grid of one CTA writes the outputs itself. A warp has four tokens' logits in
-// flight, whatever the mask says of them (a load that waits for the mask costs a second trip to memory).
-template <int N>
+// A CTA's sums over its tokens; a grid of one CTA writes the outputs itself. Each lane has the logits of two tokens
+// in flight, whatever the mask says of them (a load that waits for the mask costs a second trip to memory).
+template <int G, bool VEC>
 __global__ void __launch_bounds__(RB_WARPS * 32) router_balance_kernel(
     const float* __restrict__ logits, const int* __restrict__ inds, const uint8_t* __restrict__ mask, int T,
     int E, int k, int score_fn, float* __restrict__ part_p, int* __restrict__ part_c, RbOut o) {
-  constexpr int U = N > 4 ? 2 : 4;
-  __shared__ float sum_p[RB_WARPS][32 * N];
+  constexpr int U = 2, PER = 32 / G;  // tokens a warp works on at a time
+  __shared__ float sum_p[RB_WARPS][G * RB_N];
   __shared__ int hist[RB_MAXE + 1];  // the last: tokens kept
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % G;
   for (int i = threadIdx.x; i <= RB_MAXE; i += blockDim.x) hist[i] = 0;
   __syncthreads();
-  float acc[N] = {};
+  float acc[RB_N] = {};
   int kept = 0;
-  const int step = gridDim.x * RB_WARPS;
-  for (int t0 = blockIdx.x * RB_WARPS + warp; t0 < T; t0 += U * step) {
-    float v[U][N], unused[N];
+  const int step = gridDim.x * RB_WARPS * PER;
+  for (int t0 = (blockIdx.x * RB_WARPS + warp) * PER; t0 < T; t0 += U * step) {
+    float v[U][RB_N], unused[RB_N], mx, rs;
     int pick[U];
     bool keep[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int t = t0 + u * step;
+      const int t = t0 + u * step + lane / G;
       keep[u] = t < T;
-      pick[u] = -1;
-      if (keep[u]) {
-        rb_load<N>(v[u], logits + (size_t)t * E, E);
-        if (lane < k) pick[u] = inds[(size_t)t * k + lane];
-        if (mask) keep[u] = mask[t];
-      }
+      rb_load<G, VEC>(v[u], logits + (size_t)t * E, E, keep[u]);
+      pick[u] = keep[u] && l < k ? inds[(size_t)t * k + l] : -1;
+      if (keep[u] && mask) keep[u] = mask[t];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!keep[u]) continue;
-      if (pick[u] >= 0 && pick[u] < E) atomicAdd(&hist[pick[u]], 1);
-      ++kept;
-      const float r = 1.f / rb_scores<N, false>(v[u], unused, E, score_fn);
+      if (keep[u] && pick[u] >= 0 && pick[u] < E) atomicAdd(&hist[pick[u]], 1);
+      const float r = rb_rcp(rb_scores<G>(v[u], unused, score_fn, &mx, &rs));
+      if (keep[u]) {
+        ++kept;
 #pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] = fmaf(v[u][j], r, acc[j]);
+        for (int j = 0; j < RB_N; ++j) acc[j] = fmaf(v[u][j], r, acc[j]);
+      }
     }
   }
   pdl_trigger();
+  if (l == 0 && kept) atomicAdd(&hist[RB_MAXE], kept);
 #pragma unroll
-  for (int j = 0; j < N; ++j) sum_p[warp][lane + 32 * j] = acc[j];
-  if (lane == 0) atomicAdd(&hist[RB_MAXE], kept);
+  for (int s = 16; s >= G; s >>= 1) {
+#pragma unroll
+    for (int j = 0; j < RB_N; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], s);
+  }
+  if (lane < G) {
+#pragma unroll
+    for (int j = 0; j < RB_N; ++j) sum_p[warp][rb_expert<G, VEC>(j)] = acc[j];
+  }
   __syncthreads();
   const int e = threadIdx.x;
   float p = 0.f;
-  if (e < 32 * N) {
+  if (e < E) {
 #pragma unroll
     for (int w = 0; w < RB_WARPS; ++w) p += sum_p[w][e];
   }
   if (gridDim.x == 1) {
     rb_finish(p, e < E ? hist[e] : 0, hist[RB_MAXE], E, o);
-  } else {
-    if (e < E) {
-      part_p[(size_t)blockIdx.x * E + e] = p;
-      part_c[(size_t)blockIdx.x * E + e] = hist[e];
-    }
-    if (e == E) part_c[(size_t)RB_CTAS * E + blockIdx.x] = hist[RB_MAXE];
+    return;
   }
+  if (e < E) {
+    part_p[(size_t)blockIdx.x * E + e] = p;
+    part_c[(size_t)blockIdx.x * E + e] = hist[e];
+  }
+  if (e == E) part_c[(size_t)RB_CTAS * E + blockIdx.x] = hist[RB_MAXE];
 }
 
-// Joins the CTAs' sums, in their order: 1,024 threads, 256 a quarter of the CTAs, each with all of its loads in
-// flight.
+// Joins the CTAs' sums in their order: W threads a slice of the CTAs (W: E rounded up to 32), 18 rows in flight
+// each. (Joining eight CTAs over the shared memory of a cluster before takes longer, 17 us with 4 here against 8 with
+// 5: no more than 14 to 16 clusters of eight CTAs of 1,024 threads are on the GPU at once.)
 __global__ void __launch_bounds__(1024) router_balance_join_kernel(const float* __restrict__ part_p,
                                                                    const int* __restrict__ part_c, int C,
                                                                    int E, RbOut o) {
-  constexpr int PER = RB_CTAS / 4, HALF = PER / 2;
-  __shared__ float sp[4][RB_MAXE];
-  __shared__ int sc[4][RB_MAXE];
+  constexpr int ROWS = 18;
+  __shared__ float sp[1024];
+  __shared__ int sc[1024];
   __shared__ int sn[32];
   pdl_wait();
-  const int e = threadIdx.x & 255, s = threadIdx.x >> 8;
+  const int W = (E + 31) / 32 * 32, S = 1024 / W;
+  const int e = threadIdx.x % W, s = threadIdx.x / W;
+  const int a = C * s / S, b = s < S ? C * (s + 1) / S : 0;
   float p = 0.f;
   int c = 0;
-#pragma unroll 1
-  for (int h = 0; h < 2; ++h) {
-    const int a = s * PER + h * HALF;
-    float pv[HALF];
-    int cv[HALF];
+  int n = threadIdx.x < C ? part_c[(size_t)RB_CTAS * E + threadIdx.x] : 0;
+  for (int i = a; i < b; i += ROWS) {
+    float pv[ROWS];
+    int cv[ROWS];
 #pragma unroll
-    for (int i = 0; i < HALF; ++i) {
-      const bool in = e < E && a + i < C;
-      pv[i] = in ? part_p[(size_t)(a + i) * E + e] : 0.f;
-      cv[i] = in ? part_c[(size_t)(a + i) * E + e] : 0;
+    for (int r = 0; r < ROWS; ++r) {
+      const bool in = e < E && i + r < b;
+      pv[r] = in ? part_p[(size_t)(i + r) * E + e] : 0.f;
+      cv[r] = in ? part_c[(size_t)(i + r) * E + e] : 0;
     }
 #pragma unroll
-    for (int i = 0; i < HALF; ++i) {
-      p += pv[i];
-      c += cv[i];
+    for (int r = 0; r < ROWS; ++r) {
+      p += pv[r];
+      c += cv[r];
     }
   }
-  sp[s][e] = p;
-  sc[s][e] = c;
-  int n = threadIdx.x < C ? part_c[(size_t)RB_CTAS * E + threadIdx.x] : 0;
+  sp[threadIdx.x] = p;
+  sc[threadIdx.x] = c;
 #pragma unroll
   for (int i = 16; i; i >>= 1) n += __shfl_xor_sync(0xffffffffu, n, i);
   if ((threadIdx.x & 31) == 0) sn[threadIdx.x >> 5] = n;
   __syncthreads();
-  const bool first = s == 0;
-  p = first ? sp[0][e] + sp[1][e] + sp[2][e] + sp[3][e] : 0.f;
-  c = first ? sc[0][e] + sc[1][e] + sc[2][e] + sc[3][e] : 0;
+  if (s == 0) {
+    for (int i = 1; i < S; ++i) {
+      p += sp[i * W + e];
+      c += sc[i * W + e];
+    }
+  }
   n = 0;
 #pragma unroll
   for (int i = 0; i < (RB_CTAS + 31) / 32; ++i) n += sn[i];
@@ -230,73 +279,71 @@ struct RgArgs {
   float* dl;
 };
 
-template <int N>
+template <int G, bool VEC>
 __global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs a) {
-  __shared__ float sh_s[RG_WARPS][32 * N];  // a token's scores, for its picks
-  __shared__ float sh_d[RG_WARPS][32 * N];  // its picks' gradients; zeros between tokens
-  __shared__ int sh_t[RG_WARPS][32 * N];    // which pick has an expert
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float *ss = sh_s[warp], *sd = sh_d[warp];
-  int* st = sh_t[warp];
-  float dq[N];
+  constexpr int PER = 32 / G;
+  __shared__ float sh_d[RG_WARPS * PER][G * RB_N];          // a token's picks' gradients; zeros between tokens
+  __shared__ unsigned char sh_t[RG_WARPS * PER][G * RB_N];  // which pick has an expert
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % G;
+  float* sd = sh_d[warp * PER + lane / G];
+  unsigned char* st = sh_t[warp * PER + lane / G];
+  float dq[RB_N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    sd[lane + 32 * j] = 0.f;
+  for (int j = 0; j < RB_N; ++j) {
+    sd[l + G * j] = 0.f;
     dq[j] = 0.f;
   }
   if (a.counts) {
-    int c[N];
+    int c[RB_N];
     long long all = 0;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      c[j] = lane + 32 * j < a.E ? a.counts[lane + 32 * j] : 0;
+    for (int j = 0; j < RB_N; ++j) {
+      const int e = rb_expert<G, VEC>(j);
+      c[j] = e < a.E ? a.counts[e] : 0;
       all += c[j];
     }
 #pragma unroll
-    for (int s = 16; s; s >>= 1) all += __shfl_xor_sync(0xffffffffu, all, s);
+    for (int s = G / 2; s; s >>= 1) all += __shfl_xor_sync(0xffffffffu, all, s);
     const int n = *a.tokens;
     const float f = all > 0 && n > 0 ? a.weight * (float)a.E / ((float)all * (float)n) : 0.f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) dq[j] = f * (float)c[j];
+    for (int j = 0; j < RB_N; ++j) dq[j] = f * (float)c[j];
   }
   __syncwarp();
-  for (int t = blockIdx.x * RG_WARPS + warp; t < a.T; t += gridDim.x * RG_WARPS) {
-    float* out = a.dl + (size_t)t * a.E;
-    if (a.mask && !a.mask[t]) {
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (lane + 32 * j < a.E) out[lane + 32 * j] = 0.f;
-      continue;
-    }
-    float s[N], tail[N];
-    rb_load<N>(s, a.logits + (size_t)t * a.E, a.E);
+  const int step = gridDim.x * RG_WARPS * PER;
+  for (int t0 = (blockIdx.x * RG_WARPS + warp) * PER; t0 < a.T; t0 += step) {
+    const int t = t0 + lane / G;
+    const bool in = t < a.T;
+    const float* row = a.logits + (size_t)t * a.E;
+    float s[RB_N], tail[RB_N], mx = 0.f, rs = 0.f;
+    rb_load<G, VEC>(s, row, a.E, in);
     int id = -1;
     float d = 0.f;
-    if (a.dw && lane < a.k) {
-      id = a.inds[(size_t)t * a.k + lane];
-      if (id >= a.E) id = -1;
-      d = a.dw[(size_t)t * a.k + lane];
+    if (a.dw && in && l < a.k) {
+      id = a.inds[(size_t)t * a.k + l];
+      d = a.dw[(size_t)t * a.k + l];
     }
-    const float total = rb_scores<N, true>(s, tail, a.E, a.score_fn);
+    const bool keep = in && (!a.mask || a.mask[t]);
+    if (!keep || id >= a.E) id = -1;
+    const float x = id >= 0 ? __ldg(row + id) : 0.f;
+    const float total = rb_scores<G>(s, tail, a.score_fn, &mx, &rs);
     float pick = 0.f;  // softmax: sum_e s_e ds_e
     if (a.dw) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) ss[lane + 32 * j] = s[j];
-      __syncwarp();
-      if (id >= 0) st[id] = lane;
-      const float p = id >= 0 ? ss[id] : 0.f;
-      const float dot = warp_sum(id >= 0 ? d * p : 0.f);
+      float unused;
+      const float p = id < 0 ? 0.f : a.score_fn == LG_SCORE_SOFTMAX ? rb_exp(x - mx) * rs : rb_sigmoid(x, &unused);
+      if (id >= 0) st[id] = (unsigned char)l;
+      const float dot = rb_sum<G>(id >= 0 ? d * p : 0.f);
       if (a.norm) {
-        const float r = 1.f / warp_sum(p);
+        const float r = rb_rcp(rb_sum<G>(p));
         d = (d - dot * r) * r;
       } else {
         pick = dot;
       }
       __syncwarp();
-      const bool twice = id >= 0 && st[id] != lane;
+      const bool twice = id >= 0 && st[id] != l;
       if (__any_sync(0xffffffffu, twice)) {  // an expert picked twice: its gradients in their order
         for (int j = 0; j < a.k; ++j) {
-          if (lane == j && id >= 0) sd[id] += d;
+          if (l == j && id >= 0) sd[id] += d;
           __syncwarp();
         }
       } else if (id >= 0) {
@@ -304,17 +351,17 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs
       }
       __syncwarp();
     }
+    const float r = rb_rcp(total);
     float mean = 0.f;
     if (a.counts) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) mean = fmaf(s[j], dq[j], mean);
-      mean = warp_sum(mean) / total;
+      for (int j = 0; j < RB_N; ++j) mean = fmaf(s[j], dq[j], mean);
+      mean = rb_sum<G>(mean) * r;
     }
-    const float r = 1.f / total;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int e = lane + 32 * j;
-      float ds = a.dw ? sd[e] : 0.f;
+    for (int j = 0; j < RB_N; ++j) {
+      const int e = rb_expert<G, VEC>(j);
+      float ds = a.dw && e < a.E ? sd[e] : 0.f;
       float g;
       if (a.score_fn == LG_SCORE_SOFTMAX) {
         if (a.counts) ds += dq[j] - mean;
@@ -323,7 +370,19 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs
         if (a.counts) ds += (dq[j] - mean) * r;
         g = ds * tail[j];
       }
-      if (e < a.E) out[e] = g;
+      s[j] = keep ? g : 0.f;
+    }
+    if (in) {
+      float* out = a.dl + (size_t)t * a.E;
+#pragma unroll
+      for (int j = 0; j < RB_N; j += VEC ? 4 : 1) {
+        const int e = rb_expert<G, VEC>(j);
+        if (e >= a.E) continue;
+        if (VEC)
+          *reinterpret_cast<float4*>(out + e) = make_float4(s[j], s[j + 1], s[j + 2], s[j + 3]);
+        else
+          out[e] = s[j];
+      }
     }
     __syncwarp();
     if (id >= 0) sd[id] = 0.f;
@@ -331,26 +390,29 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs
   }
 }
 
-static int rb_ctas(int T) {
-  return std::max(1, std::min(RB_CTAS, (T + RB_CTA_TOKENS - 1) / RB_CTA_TOKENS));
-}
+// One CTA up to 256 tokens (its 32 warps have two times 32 / G in flight), above that one for every 64.
+static int rb_ctas(int T) { return T <= 256 ? 1 : std::min(RB_CTAS, (T + 63) / 64); }
 
 static int rb_check(const char* who, const void* logits, const void* inds, int T, int E, int k, int score_fn) {
   LG_CHECK_ARG(E >= 1 && E <= RB_MAXE, "%s: E=%d not in [1, %d]", who, E, RB_MAXE);
   LG_CHECK_ARG(k >= 1 && k <= 32, "%s: k=%d not in [1, 32]", who, k);
-  LG_CHECK_ARG(T >= 0, "%s: T=%d", who, T);
+  LG_CHECK_ARG(T >= 0 && T <= (1 << 30), "%s: T=%d", who, T);
   LG_CHECK_ARG(score_fn == LG_SCORE_SIGMOID || score_fn == LG_SCORE_SOFTMAX, "%s: score_fn %d", who, score_fn);
   LG_CHECK_ARG(T == 0 || (logits && inds), "%s: NULL pointer", who);
+  LG_CHECK_ARG(aligned(logits, 4), "%s: logits must be 4-byte aligned", who);
   return LG_OK;
 }
 
-// N: 32 * N experts a warp's registers hold
-#define RB_BY_E(E, CALL)             \
-  do {                               \
-    if ((E) <= 32) { CALL(1); }      \
-    else if ((E) <= 64) { CALL(2); } \
-    else if ((E) <= 128) { CALL(4); } \
-    else { CALL(8); }                \
+// Lanes a token: eight scores each, and one pick each.
+#define RB_BY_SIZE(E, k, vec, CALL)                      \
+  do {                                                   \
+    if ((E) <= 64 && (k) <= 8) {                         \
+      if (vec) CALL(8, true); else CALL(8, false);       \
+    } else if ((E) <= 128 && (k) <= 16) {                \
+      if (vec) CALL(16, true); else CALL(16, false);     \
+    } else {                                             \
+      if (vec) CALL(32, true); else CALL(32, false);     \
+    }                                                    \
   } while (0)
 
 }  // namespace lg
@@ -358,8 +420,8 @@ static int rb_check(const char* who, const void* logits, const void* inds, int T
 using namespace lg;
 
 extern "C" size_t lg_router_balance_workspace_bytes(int T, int E) {
-  const size_t C = rb_ctas(T) > 1 ? RB_CTAS : 0, e = E > 0 ? E : 1;
-  return align_up(C * e * 4, 256) + align_up(C * (e + 1) * 4, 256);  // 0: one CTA needs none
+  if (rb_ctas(T) == 1 || E < 1) return 0;
+  return align_up((size_t)RB_CTAS * E * 4, 256) + align_up((size_t)RB_CTAS * (E + 1) * 4, 256);
 }
 
 extern "C" int lg_router_balance(const float* logits, const int32_t* inds, const uint8_t* mask, int T, int E,
@@ -376,10 +438,11 @@ extern "C" int lg_router_balance(const float* logits, const int32_t* inds, const
   float* pp = w.take<float>((size_t)RB_CTAS * E);
   int* pc = w.take<int>((size_t)RB_CTAS * (E + 1));
   const RbOut o = {loss, counts, probs, tokens};
+  const bool vec = E % 4 == 0 && aligned(logits, 16);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define RB_CALL(N)                                                                               \
-  router_balance_kernel<N><<<C, RB_WARPS * 32, 0, st>>>(logits, inds, mask, T, E, k, score_fn, pp, pc, o)
-  RB_BY_E(E, RB_CALL);
+#define RB_CALL(G, VEC)                                                                                     \
+  router_balance_kernel<G, VEC><<<C, RB_WARPS * 32, 0, st>>>(logits, inds, mask, T, E, k, score_fn, pp, pc, o)
+  RB_BY_SIZE(E, k, vec, RB_CALL);
 #undef RB_CALL
   LG_LAUNCH_CHECK("router_balance");
   if (C > 1) {
@@ -399,10 +462,13 @@ extern "C" int lg_router_grad(const float* logits, const int32_t* inds, const fl
   LG_CHECK_ARG(dw || counts, "router_grad: neither dw nor a balance loss");
   LG_CHECK_ARG(dlogits, "router_grad: NULL output");
   const RgArgs a = {logits, inds, dw, mask, counts, tokens, weight, T, E, k, norm_topk_prob, score_fn, dlogits};
-  const int grid = std::max(1, std::min(2 * device_sm_count(), (T + RG_WARPS - 1) / RG_WARPS));
+  const bool vec = E % 4 == 0 && aligned(logits, 16) && aligned(dlogits, 16);
+  const int sms = device_sm_count();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define RB_CALL(N) router_grad_kernel<N><<<grid, RG_WARPS * 32, 0, st>>>(a)
-  RB_BY_E(E, RB_CALL);
+#define RB_CALL(G, VEC)                                                                                     \
+  router_grad_kernel<G, VEC><<<std::max(1, std::min(8 * sms, (T + RG_WARPS * 32 / G - 1) / (RG_WARPS * 32 / G))), \
+                               RG_WARPS * 32, 0, st>>>(a)
+  RB_BY_SIZE(E, k, vec, RB_CALL);
 #undef RB_CALL
   LG_LAUNCH_CHECK("router_grad");
   return LG_OK;

@@ -1085,14 +1085,13 @@ def router_balance(logits, inds, score_fn="sigmoid", mask=None):
     ``RouterBalance``; its gradient is ``router_grad``'s, through the scores (counts have none)."""
     index, T, E, k, logits, inds, mask = _router_args("router_balance", logits, inds, score_fn, mask)
     dev = logits.device
-    real = torch.empty(1 + E, dtype=torch.float32, device=dev)
-    whole = torch.empty(1 + E, dtype=_I32, device=dev)
+    loss, probs = torch.empty(1, dtype=torch.float32, device=dev), torch.empty(E, dtype=torch.float32, device=dev)
+    counts, tokens = torch.empty(E, dtype=_I32, device=dev), torch.empty(1, dtype=_I32, device=dev)
     nb = _on_index(index, "lg_router_balance_workspace_bytes", T, E)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-    fp, wp = real.data_ptr(), whole.data_ptr()
     _call_on(index, _lib.lib().lg_router_balance, logits.data_ptr(), inds.data_ptr(), _p(mask), T, E, k,
-             _SCORES[score_fn], fp, wp + 4, fp + 4, wp, _p(ws), nb)
-    (loss, probs), (tokens, counts) = real.split_with_sizes((1, E)), whole.split_with_sizes((1, E))
+             _SCORES[score_fn], loss.data_ptr(), counts.data_ptr(), probs.data_ptr(), tokens.data_ptr(), _p(ws),
+             nb)
     return RouterBalance(loss, counts, probs, tokens)
 
 

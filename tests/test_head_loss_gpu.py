@@ -357,3 +357,28 @@ def test_refusals():
         ops.head_loss_grad(x, head, ids, lse[:3], g)
     with pytest.raises(ValueError, match="g must"):
         ops.head_loss_grad(x, head, ids, lse, g.double())
+
+
+@pytest.mark.parametrize("T", [20, 200])
+def test_4bit_scales_of_every_size(T):
+    """Scales that the packed fma takes and others (0, 2^-133, 2^-5 and more, negative) in one head, some groups
+    beside one another: the weights are bf16(scale * code + bias) all the same."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    V, H = 700, 512
+    q = torch.randint(-2 ** 31, 2 ** 31, (V, H // 8), generator=g, device="cuda", dtype=torch.int32)
+    s = torch.rand(V, H // 64, generator=g, device="cuda") * 0.01
+    for at, v in enumerate([0.0, 2.0 ** -133, 2.0 ** -126, 0.0312, 2.0 ** -5, 0.11, -0.004, -0.2]):
+        s[at * 64:at * 64 + 40, at] = v
+    s = s.bfloat16()
+    b = (torch.randn(V, H // 64, generator=g, device="cuda") * 0.03).bfloat16()
+    x = torch.randn(T, H, generator=g, device="cuda").bfloat16()
+    ids = torch.randint(0, V, (T,), generator=g, device="cuda", dtype=torch.int32)
+    W = dequant64((q, s, b))
+    assert torch.equal(ops.dequantize(q, s, b).cpu().double(), W)
+    gr = torch.randn(T, generator=g, device="cuda")
+    r = reference(x, W, ids, None, gr)
+    loss, lse = ops.head_loss(x, (q, s, b), ids)
+    far = r["lse"].abs().max() * 2 ** -21
+    within(loss, r["loss"], r["bloss"] + far)
+    within(lse, r["lse"], r["blse"] + far)
+    within(ops.head_loss_grad(x, (q, s, b), ids, lse, gr, dw=False)[0], r["dx"], r["bdx"])
