@@ -35,7 +35,8 @@ constexpr int HD_THREADS = 256;
 constexpr int HD_A_BYTES = HD_BM * HD_BK * 2;  // 16 KB
 constexpr int HD_BOX = 64 * HD_BK * 2;  // an MN-major box: 64 K rows of 64 elements
 constexpr int HD_RING = 192 << 10;      // stages of A and B
-constexpr size_t HD_SMEM = 1024 + HD_RING + 256;
+constexpr int HD_OUT = 4096;            // an output box: 32 rows of 128 bytes, swizzled
+constexpr size_t HD_SMEM = 1024 + HD_RING + 4 * 2 * HD_OUT + 256;
 
 struct HdArgs {
   int M, N;          // rows of the output tile grid, and its columns
@@ -57,14 +58,9 @@ struct HdArgs {
   const float* lse;
   const float* g;
   const float* wsum;  // K > 1: [T]
-  __nv_bfloat16* dz;  // [T, ldz]
-  int ldz;
+  int ldz;            // columns of dz [T, ldz]
   // HD_XGRAD
-  float* dx;  // [splits, T, H]
-  int add;    // 0: the first piece
-  // HD_WGRAD
-  __nv_bfloat16* dw;  // [V, H]
-  bool wide;          // its rows are 32-byte aligned
+  int add;  // 0: the first piece
 };
 
 __device__ __forceinline__ void hd_sub(float (&v)[32], int c, float w) {
@@ -72,20 +68,12 @@ __device__ __forceinline__ void hd_sub(float (&v)[32], int c, float w) {
   for (int i = 0; i < 32; ++i) v[i] = i == c ? v[i] - w : v[i];
 }
 
-// Sixteen bf16 of a row as one 32-byte store: a thread has a row of its own, so that a narrower store would leave
-// its sector of L2 half written.
+// Sixteen bf16 as one 32-byte store.
 __device__ __forceinline__ void hd_store32(__nv_bfloat16* p, const uint32_t* r) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-__device__ __forceinline__ void hd_store16(__nv_bfloat16* p, const float* v) {
-  uint32_t r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = hd_pack(v[2 * i], v[2 * i + 1]);
-  hd_store32(p, r);
-}
-
 // A unit of work: tile (m, n) of the output, and the part [k0, k1) of the contraction's blocks.
 struct HdUnit {
   int m, n, split, k0, k1;
@@ -109,10 +97,48 @@ __device__ __forceinline__ HdUnit hd_unit(const HdArgs& a, int i) {
 }
 
 // One output tile's row of this thread. `ok` is false after a wait that ran out: NaN is written.
+//
+// Outputs leave as boxes of 32 rows x 128 bytes: a thread puts its row into shared memory, a lane stores the box by
+// TMA (HD_XGRAD: adds it to what earlier pieces left). Stored by the threads themselves, a row each, a tile of
+// dW took 8,500 cycles and dx's addition 16 us of 66.
+struct HdBox {
+  const CUtensorMap* map;
+  uint8_t* smem;  // two boxes, in turn
+  int turn;
+};
+
+// This thread's 128 bytes of a box at (x, y) (and plane z), y the warp's first row; `in`: it is one of the output's.
 template <int KIND>
-__device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, int t, uint32_t taddr, bool ok) {
+__device__ __forceinline__ void hd_box(HdBox& b, const uint32_t (&r)[32], int x, int y, int z, bool add, bool in) {
+  const int lane = threadIdx.x & 31;
+  uint8_t* box = b.smem + b.turn * HD_OUT;
+  b.turn ^= 1;
+  if (lane == 0) tma_store_wait_read<1>();  // the box's last store has read it
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+        make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0 && in) {
+    if (KIND != HD_XGRAD)
+      tma_store_2d(b.map, box, x, y);
+    else if (add)
+      tma_add_3d(b.map, box, x, y, z);
+    else
+      tma_store_3d(b.map, box, x, y, z);
+    tma_store_commit();
+  }
+  __syncwarp();  // a tcgen05.ld may follow: of the whole warp
+}
+
+template <int KIND>
+__device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, int t, uint32_t taddr, bool ok,
+                                            HdBox& box) {
   const int n0 = u.n * HD_BN;  // in the piece (or in H)
   const bool live = t < a.M;
+  const int y = t & ~31;
   const float nan = __int_as_float(0x7fffffff);
   float v[32];
 #pragma unroll
@@ -194,66 +220,58 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
           gs = gg * a.wsum[t];
         }
       }
-      __nv_bfloat16* out = a.dz + (size_t)t * a.ldz + n0;
 #pragma unroll 1
-      for (int c = 0; c < HD_BN && n0 + c < a.ldz; c += 32) {
-        const int id0 = c0 + c;
-        __syncwarp();
-        if (ok) tmem_ld32_wait(taddr + c, v);
+      for (int c = 0; c < HD_BN && n0 + c < a.ldz; c += 64) {
+        uint32_t r[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = ok ? gs * hd_ex2(fmaf(v[i], HD_LOG2E, off)) : nan;
-        while ((unsigned)next - (unsigned)id0 < 32u) {
-          if (a.K == 1) {
-            hd_sub(v, next - id0, gs);
-            break;
+        for (int h = 0; h < 2; ++h) {
+          const int id0 = c0 + c + 32 * h;
+          __syncwarp();
+          if (ok) tmem_ld32_wait(taddr + c + 32 * h, v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = ok ? gs * hd_ex2(fmaf(v[i], HD_LOG2E, off)) : nan;
+          while ((unsigned)next - (unsigned)id0 < 32u) {
+            if (a.K == 1) {
+              hd_sub(v, next - id0, gs);
+              break;
+            }
+            const float w = a.weights ? a.weights[row_k + a.order[row_k + p]] : 1.f;
+            hd_sub(v, next - id0, gg * w);
+            next = ++p < p1 ? a.ids[row_k + p] : -1;
           }
-          const float w = a.weights ? a.weights[row_k + a.order[row_k + p]] : 1.f;
-          hd_sub(v, next - id0, gg * w);
-          next = ++p < p1 ? a.ids[row_k + p] : -1;
-        }
-        if (!counts) {  // a token without a target: nothing of it, whatever its row holds
+          if (!counts) {  // a token without a target: nothing of it, whatever its row holds
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) r[16 * h + i] = hd_pack(v[2 * i], v[2 * i + 1]);
         }
-        if (live) {
-          hd_store16(out + c, v);  // rows of dz are 128-byte aligned
-          hd_store16(out + c + 16, v + 16);
-        }
+        __syncwarp();
+        hd_box<KIND>(box, r, n0 + c, y, 0, false, y < a.M);
       }
     }
-  } else {
+  } else if (KIND == HD_XGRAD) {
 #pragma unroll 1
     for (int c = 0; c < HD_BN && n0 + c < a.N; c += 32) {
       __syncwarp();
       if (ok) tmem_ld32_wait(taddr + c, v);
-      if (!live) continue;
-      if (KIND == HD_XGRAD) {
-        float* out = a.dx + ((size_t)u.split * a.M + t) * a.N + n0 + c;
+      uint32_t r[32];
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          if (n0 + c + i >= a.N) break;
-          float4 w = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-          if (a.add) {
-            const float4 o = *reinterpret_cast<const float4*>(out + i);
-            w = make_float4(w.x + o.x, w.y + o.y, w.z + o.z, w.w + o.w);
-          }
-          *reinterpret_cast<float4*>(out + i) = w;
-        }
-      } else {
-        __nv_bfloat16* out = a.dw + ((size_t)a.v0 + t) * a.N + n0 + c;
-        if (a.wide && n0 + c + 32 <= a.N) {
-          hd_store16(out, v);
-          hd_store16(out + 16, v + 16);
-          continue;
-        }
+      for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
+      hd_box<KIND>(box, r, n0 + c, y, u.split, a.add, y < a.M);
+    }
+  } else {
+#pragma unroll 1
+    for (int c = 0; c < HD_BN && n0 + c < a.N; c += 64) {
+      uint32_t r[32];
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          if (n0 + c + i >= a.N) break;
-          *reinterpret_cast<uint4*>(out + i) =
-              make_uint4(hd_pack(v[i], v[i + 1]), hd_pack(v[i + 2], v[i + 3]),
-                         hd_pack(v[i + 4], v[i + 5]), hd_pack(v[i + 6], v[i + 7]));
-        }
+      for (int h = 0; h < 2; ++h) {
+        __syncwarp();
+        if (ok) tmem_ld32_wait(taddr + c + 32 * h, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r[16 * h + i] = hd_pack(v[2 * i], v[2 * i + 1]);
       }
+      hd_box<KIND>(box, r, n0 + c, a.v0 + y, 0, false, y < a.M);
     }
   }
 }
@@ -269,14 +287,14 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
 template <int KIND, int CG>
 __global__ void __launch_bounds__(HD_THREADS, 1)
     hd_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
-              const HdArgs a) {
+              const __grid_constant__ CUtensorMap mo, const HdArgs a) {
   constexpr bool A_MN = KIND == HD_WGRAD, B_MN = KIND == HD_XGRAD || KIND == HD_WGRAD;
   constexpr int B_ROWS = HD_BN / CG;  // of B in this CTA
   constexpr int STAGE = HD_A_BYTES + B_ROWS * HD_BK * 2;
   constexpr int STAGES = HD_RING / STAGE;
   extern __shared__ uint8_t hd_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)hd_smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + HD_RING);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + HD_RING + 4 * 2 * HD_OUT);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;  // [2]
   uint64_t* acc_empty = acc_full + 2;   // [2]
@@ -315,7 +333,6 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
   if (CG == 2) cluster_sync();  // the other CTA's barriers are ready
   tc_fence_after();
   pdl_wait();  // nothing of an earlier kernel's is touched before
-  pdl_trigger();
   const uint32_t tmem = *tmem_base;
   const int units = a.mt * a.nt * a.splits;
 
@@ -422,6 +439,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
     __syncwarp();
   } else if (warp >= 4) {
     const int q = warp & 3;
+    HdBox box = {&mo, smem + HD_RING + q * 2 * HD_OUT, 0};
     bool ok = true;
     int n = 0;
     for (int i = first; i < units; i += step, ++n) {
@@ -430,7 +448,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + acc, (n >> 1) & 1, err, 5));
       tc_fence_after();
       hd_epilogue<KIND>(a, u, (u.m * CG + rank) * HD_BM + q * 32 + lane,
-                        tmem + acc * HD_BN + ((uint32_t)(q * 32) << 16), ok);
+                        tmem + acc * HD_BN + ((uint32_t)(q * 32) << 16), ok, box);
       tc_fence_before();
       __syncwarp();
       if (ok && lane == 0) {
@@ -440,6 +458,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
           mbar_arrive(acc_empty + acc);
       }
     }
+    if (KIND != HD_LOSS && lane == 0) tma_store_wait();
+    __syncwarp();
   }
   // The products have ended before their TMEM goes.
   if (warp == 2) {
@@ -482,7 +502,6 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
                                                       unsigned char* __restrict__ order,
                                                       unsigned char* __restrict__ start,
                                                       float* __restrict__ wsum) {
-  pdl_wait();
   pdl_trigger();
   __shared__ int sh[8][2 * HD_MAXK];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -602,8 +621,6 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
   constexpr int WARPS = HJ_THREADS / 32;
   __shared__ HdStat sh[WARPS];
   __shared__ float sh_dot[HD_MAXK];
-  pdl_wait();
-  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x;
   const int parts = in.parts;
@@ -690,7 +707,6 @@ __global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __res
                                                       int T, int H, const int* __restrict__ ids, int V,
                                                       const unsigned char* __restrict__ start, int nt,
                                                       __nv_bfloat16* __restrict__ out) {
-  pdl_wait();
   pdl_trigger();
   const int per = H / 8;
   const long long n = (long long)T * per;
@@ -709,7 +725,6 @@ __global__ void __launch_bounds__(256) hd_dequant_kernel(const uint2* __restrict
                                                          const uint16_t* __restrict__ s,
                                                          const uint16_t* __restrict__ b, long long n,
                                                          __nv_bfloat16* __restrict__ out) {
-  pdl_wait();
   pdl_trigger();
   constexpr int U = 4;
   const long long step = gridDim.x * 256LL;
@@ -740,8 +755,6 @@ __global__ void __launch_bounds__(256) hd_dequant_kernel(const uint2* __restrict
 // dx = the sum of its parts, in their order, rounded once.
 __global__ void __launch_bounds__(256) hd_sum_kernel(const float* __restrict__ parts, int n,
                                                      long long size, __nv_bfloat16* __restrict__ out) {
-  pdl_wait();
-  pdl_trigger();
   const long long q = size / 4;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < q; i += gridDim.x * 256LL) {
     float4 s = reinterpret_cast<const float4*>(parts)[i];
@@ -872,7 +885,8 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
   } while (0)
 
 template <int KIND, int CG>
-static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const HdArgs& a, cudaStream_t st) {
+static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const HdArgs& a,
+                        bool early, cudaStream_t st) {
   static std::atomic<bool> done[64];
   int dev = 0;
   LG_CUDA_TRY(cudaGetDevice(&dev));
@@ -888,35 +902,55 @@ static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const HdAr
   cfg.dynamicSmemBytes = HD_SMEM;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = CG;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  int n = 0;
+  if (CG > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = CG;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (early) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = CG;
-  LG_CUDA_TRY(cudaLaunchKernelEx(&cfg, hd_kernel<KIND, CG>, ma, mb, a));
+  cfg.numAttrs = n;
+  LG_CUDA_TRY(cudaLaunchKernelEx(&cfg, hd_kernel<KIND, CG>, ma, mb, mo, a));
   LG_LAUNCH_CHECK("head");
   return LG_OK;
 }
 
-// Operands of a product: [contraction, rows] (mn) or [rows, contraction] matrices of bf16.
+// Operands of a product: [contraction, rows] (mn) or [rows, contraction] matrices of bf16; its output alike (dx:
+// fp32, `ld` matrices of it).
 struct HdOperand {
   const void* p;
   long long inner, rows, ld;
 };
 
 // One CTA a tile where the output has no more than 128 rows, else a pair.
+//
+// `early`: it may start under the kernel before it, one of this call's small ones that says so (pdl_trigger). Nothing
+// is launched early behind an hd_kernel: its CTAs take nearly all of an SM, and where some of its pairs are not on the
+// GPU yet (the SMs were busy with the kernel before), waiting CTAs of a later kernel can take their SMs and
+// wait for them for ever.
 template <int KIND>
-static int hd_launch(const HdOperand& a, const HdOperand& b, HdArgs g, cudaStream_t st) {
+static int hd_launch(const HdOperand& a, const HdOperand& b, const HdOperand& out, HdArgs g, bool early,
+                     cudaStream_t st) {
   constexpr bool A_MN = KIND == HD_WGRAD, B_MN = KIND == HD_XGRAD || KIND == HD_WGRAD;
   const int cg = hd_cg(g.M);
   g.mt = (g.M + HD_BM * cg - 1) / (HD_BM * cg);
   g.nt = (g.N + HD_BN - 1) / HD_BN;
-  CUtensorMap ma, mb;
+  CUtensorMap ma, mb, mo;
   HD_TRY(make_map_2d(&ma, a.p, true, a.inner, a.rows, (uint64_t)a.ld * 2, 64, A_MN ? HD_BK : HD_BM, 128));
   HD_TRY(make_map_2d(&mb, b.p, true, b.inner, b.rows, (uint64_t)b.ld * 2, 64, B_MN ? HD_BK : HD_BN / cg, 128));
-  return cg == 2 ? hd_launch_as<KIND, 2>(ma, mb, g, st) : hd_launch_as<KIND, 1>(ma, mb, g, st);
+  if (KIND == HD_LOSS)
+    mo = ma;  // none
+  else if (KIND == HD_XGRAD)
+    HD_TRY(make_map_f32_planes(&mo, out.p, out.inner, out.rows, out.ld, 32));
+  else
+    HD_TRY(make_map_2d(&mo, out.p, true, out.inner, out.rows, (uint64_t)out.ld * 2, 64, 32, 128));
+  return cg == 2 ? hd_launch_as<KIND, 2>(ma, mb, mo, g, early, st) : hd_launch_as<KIND, 1>(ma, mb, mo, g, early, st);
 }
 
 static int hd_check(const char* who, const void* x, long long ldx, int T, int H, const void* w,
@@ -945,8 +979,9 @@ static int hd_weights(const void* w, const void* ws, const void* wb, int H, int 
   if (!ws) return LG_OK;
   const long long n = (long long)rows * (H / 16);
   const size_t at = (size_t)v0 * (H / 16);
-  LG_CUDA_TRY(launch_early(hd_dequant_kernel, hd_blocks(n), 256, 0, st, static_cast<const uint2*>(w) + at,
-                           static_cast<const uint16_t*>(ws) + at / 4, static_cast<const uint16_t*>(wb) + at / 4, n, k.wq));
+  hd_dequant_kernel<<<hd_blocks(n), 256, 0, st>>>(static_cast<const uint2*>(w) + at,
+                                                  static_cast<const uint16_t*>(ws) + at / 4,
+                                                  static_cast<const uint16_t*>(wb) + at / 4, n, k.wq);
   LG_LAUNCH_CHECK("head_dequant");
   return LG_OK;
 }
@@ -954,8 +989,7 @@ static int hd_weights(const void* w, const void* ws, const void* wb, int H, int 
 static int hd_sort(const int* ids, const float* weights, int T, int K, int V, const HdWork& k,
                    cudaStream_t st) {
   if (K == 1) return LG_OK;
-  LG_CUDA_TRY(launch_early(hd_sort_kernel, (T + 7) / 8, 256, 0, st, ids, weights, T, K, V, k.nt, k.sorted, k.order,
-                           k.start, k.wsum));
+  hd_sort_kernel<<<(T + 7) / 8, 256, 0, st>>>(ids, weights, T, K, V, k.nt, k.sorted, k.order, k.start, k.wsum);
   LG_LAUNCH_CHECK("head_sort");
   return LG_OK;
 }
@@ -1024,11 +1058,11 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
       a.v0 = v0;
       a.b_row0 = quant ? 0 : v0;
       const HdOperand mw = quant ? HdOperand{k.wq, H, n, H} : HdOperand{w, H, V, ldw};
-      HD_TRY(hd_launch<HD_LOSS>({x, H, T, ldx}, mw, a, st));
+      HD_TRY(hd_launch<HD_LOSS>({x, H, T, ldx}, mw, {}, a, quant || (K > 1 && v0 == 0), st));
     }
   }
-  LG_CUDA_TRY(launch_early(quant ? hd_join_kernel<true> : hd_join_kernel<false>, T, HJ_THREADS, 0, st, k.out, xb, ldx, H,
-                           head, ids, weights, K, V, loss, lse, (int*)top));
+  const auto join = quant ? hd_join_kernel<true> : hd_join_kernel<false>;
+  join<<<T, HJ_THREADS, 0, st>>>(k.out, xb, ldx, H, head, ids, weights, K, V, loss, lse, top);
   LG_LAUNCH_CHECK("head_join");
   return LG_OK;
 }
@@ -1054,9 +1088,8 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
                 k.bytes);
   HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
   if (dw) {
-    LG_CUDA_TRY(launch_early(hd_rows_kernel, hd_blocks((long long)T * (H / 8)), 256, 0, st,
-                             static_cast<const __nv_bfloat16*>(x), ldx, T, H, ids, V,
-                             (const unsigned char*)k.start, k.nt, k.xz));
+    hd_rows_kernel<<<hd_blocks((long long)T * (H / 8)), 256, 0, st>>>(static_cast<const __nv_bfloat16*>(x), ldx, T, H,
+                                                                       ids, V, k.start, k.nt, k.xz);
     LG_LAUNCH_CHECK("head_rows");
   }
   for (int v0 = 0; v0 < V; v0 += k.piece) {
@@ -1071,34 +1104,30 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     a.lse = lse;
     a.g = g;
     a.wsum = k.wsum;
-    a.dz = k.dz;
     a.ldz = (n + 63) / 64 * 64;
-    HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, a, st));
+    HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, {k.dz, a.ldz, T, a.ldz}, a, quant || (v0 == 0 && (dw || K > 1)), st));
     const HdOperand mz = {k.dz, n, T, a.ldz};
     if (dx) {
       HdArgs b = a;
       b.N = H;
       b.kblocks = (n + HD_BK - 1) / HD_BK;
       b.splits = std::min(k.splits, b.kblocks);
-      b.dx = k.dx;
       b.add = v0 > 0;
-      HD_TRY(hd_launch<HD_XGRAD>(mz, mw, b, st));
+      HD_TRY(hd_launch<HD_XGRAD>(mz, mw, {k.dx, H, T, k.splits}, b, false, st));
     }
     if (dw) {
       HdArgs b = a;
       b.M = n;
       b.N = H;
       b.kblocks = (T + HD_BK - 1) / HD_BK;
-      b.dw = static_cast<__nv_bfloat16*>(dw);
-      b.wide = aligned(dw, 32) && H % 16 == 0;
-      HD_TRY(hd_launch<HD_WGRAD>(mz, {k.xz, H, T, H}, b, st));
+      HD_TRY(hd_launch<HD_WGRAD>(mz, {k.xz, H, T, H}, {dw, H, V, H}, b, false, st));
     }
   }
   if (dx) {
     // The last piece may have fewer parts than the first; later parts then kept the earlier sums.
     const int parts = std::min(k.splits, (std::min(k.piece, V) + HD_BK - 1) / HD_BK);
-    LG_CUDA_TRY(launch_early(hd_sum_kernel, hd_blocks((long long)T * H / 4), 256, 0, st, (const float*)k.dx, parts,
-                             (long long)T * H, static_cast<__nv_bfloat16*>(dx)));
+    hd_sum_kernel<<<hd_blocks((long long)T * H / 4), 256, 0, st>>>(k.dx, parts, (long long)T * H,
+                                                                   static_cast<__nv_bfloat16*>(dx));
     LG_LAUNCH_CHECK("head_sum");
   }
   return LG_OK;

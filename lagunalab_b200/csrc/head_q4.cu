@@ -35,7 +35,7 @@ constexpr int HQ_UNPACK = 16;  // warps
 constexpr int HQ_THREADS = (8 + HQ_UNPACK) * 32;
 constexpr int HQ_BLOCK = 32;               // ids a block: a warp's TMEM lanes
 constexpr int HQ_W_BYTES = 4 * 32 * 128;   // a stage of packed words: 128 rows x 256 codes
-constexpr int HQ_SMEM_MAX = 232448;
+constexpr int HQ_SMEM_MAX = 224 << 10;     // a CTA of hq_order_kernel has room beside it
 
 struct HqArgs {
   int T, N, H, V, K;
@@ -432,7 +432,6 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   tc_fence_after();
   if (warp == 3) tmem_dealloc(tmem, 512);
   // The four warps' parts, in their order.
-  pdl_trigger();
   if (threadIdx.x < a.T) {
     const int t = threadIdx.x;
     float mx = -INFINITY, sum = 0.f;
@@ -460,7 +459,6 @@ __global__ void __launch_bounds__(256) hq_order_kernel(const __nv_bfloat16* __re
                                                        int per, __nv_bfloat16* __restrict__ out,
                                                        const int* __restrict__ ids, int T, int K, int nt,
                                                        int* __restrict__ idt) {
-  pdl_wait();
   pdl_trigger();
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i < K * nt) {
@@ -531,8 +529,7 @@ int hq_loss_parts(const __nv_bfloat16* x, long long ldx, int T, int H, const HdH
   a.out = out;
   const int n = T * (H / 8);
   const int nt = 32 * hq_nt(T);
-  LG_CUDA_TRY(launch_early(hq_order_kernel, (std::max(n, K * nt) + 255) / 256, 256, 0, st, x, ldx, n, H / 8, xp, ids, T,
-                           K, nt, idt));
+  hq_order_kernel<<<(std::max(n, K * nt) + 255) / 256, 256, 0, st>>>(x, ldx, n, H / 8, xp, ids, T, K, nt, idt);
   LG_LAUNCH_CHECK("head_order");
   const uint64_t groups = (uint64_t)V * (H / 64), gbytes = align_up(groups * 2, 16);
   CUtensorMap m[4];
