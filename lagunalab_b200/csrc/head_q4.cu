@@ -4,13 +4,15 @@
 // the weights are the product's A operand, taken from TMEM, where the warps that unpack them write them; x is B.
 // So few tokens cost few columns, and an unpacked weight crosses neither memory nor shared memory.
 //
-//   warp 0       TMA: packed words (32 rows x 256 codes a box, 128-byte swizzle), scales and biases
-//   warp 2       TMA: x, 64 columns a slot
+//   warp 0       TMA: packed words (32 rows x 128 codes a box, 64-byte swizzle), scales and biases
+//   warp 2       TMA: x, 128 columns a slot
 //   warps 4-19   unpack: a row a thread, 128 codes a turn (two quantization groups), four groups of four warps in
 //                turns; tcgen05.st of 32 columns a group
 //   warp 1       four products (M 128, N, K 16) a 64-wide block into one of two accumulators
-//   warps 20-23  per tile and token the maximum and the sum of exponentials over the warp's 32 rows, which lie
-//                across its lanes: a transposing reduction (31 shuffles for 32 columns) leaves token i with lane i
+//   warps 20-23  per tile and token the sum of exponentials over the warp's 32 rows, which lie across its lanes: a
+//                transposing reduction (31 shuffles for 32 columns) leaves token i with lane i. The exponentials are
+//                taken from a reference per token, the maximum of the warp's first tile, until one lies 2^90 above
+//                it; then (and always where the maximum's id is asked for) the maximum is reduced like the sum
 //
 // Unpacking: q4_word (head.cuh); a warp that holds a scale it does not take unpacks by q4_word_any.
 //
@@ -34,14 +36,15 @@ using namespace tc;
 constexpr int HQ_UNPACK = 16;  // warps
 constexpr int HQ_THREADS = (8 + HQ_UNPACK) * 32;
 constexpr int HQ_BLOCK = 32;               // ids a block: a warp's TMEM lanes
-constexpr int HQ_W_BYTES = 4 * 32 * 128;   // a stage of packed words: 128 rows x 256 codes
+constexpr int HQ_W_BYTES = 4 * 32 * 64;    // a stage of packed words, one turn's: 128 rows x 128 codes
+constexpr float HQ_FAR = 90.f;             // of exponents of 2: 100,000 terms of 2^90 are below 2^127
 constexpr int HQ_SMEM_MAX = 224 << 10;     // a CTA of hq_order_kernel has room beside it
 
 struct HqArgs {
   int T, N, H, V, K;
   int kb;       // 64-wide blocks of H
   int blocks;   // blocks of 32 ids
-  int as, ws;   // slots of unpacked weights and x (128 columns), stages of packed words (256 codes)
+  int as, ws;   // slots of unpacked weights and x (128 columns), stages of packed words: a multiple of 4
   int sc_bytes;  // scales of a tile, a multiple of 2,048
   int wide;      // scales by eight groups: [H / 512][128 rows][8]; else [128 rows][H / 64]
   const int* ids;  // [K][32 NT], -1 past T
@@ -101,23 +104,24 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   float* sm_m = reinterpret_cast<float*>(sm_s + 4 * a.sc_bytes);
   float* sm_sum = sm_m + 4 * 32 * NT;
   int* sm_top = reinterpret_cast<int*>(sm_sum + 4 * 32 * NT);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm_top + 4 * 32 * NT);
-  uint64_t *w_full = bars, *w_empty = bars + 8, *full = bars + 16, *empty = bars + 24;
-  uint64_t *s_full = bars + 32, *s_empty = bars + 34, *acc_full = bars + 36, *acc_empty = bars + 38;
-  uint64_t* done = bars + 40;
-  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(bars + 41);
+  float* sm_ref = reinterpret_cast<float*>(sm_top + 4 * 32 * NT);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm_ref + 4 * 32 * NT);
+  uint64_t *w_full = bars, *w_empty = bars + 12, *full = bars + 24, *empty = bars + 32;
+  uint64_t *s_full = bars + 40, *s_empty = bars + 42, *acc_full = bars + 44, *acc_empty = bars + 46;
+  uint64_t* done = bars + 48;
+  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(bars + 49);
   int* err = reinterpret_cast<int*>(tmem_base + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b0 = (int)((long long)a.blocks * blockIdx.x / gridDim.x);
   const int b1 = (int)((long long)a.blocks * (blockIdx.x + 1) / gridDim.x);
   const int tiles = (b1 - b0 + 3) / 4;
-  const int stages = (a.kb + 3) / 4;  // of packed words, a tile
+  const int turns = (a.kb + 1) / 2;  // of 128 codes (the last perhaps 64), a tile
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.ws; ++i) {
       mbar_init(w_full + i, 1);
-      mbar_init(w_empty + i, HQ_UNPACK);
+      mbar_init(w_empty + i, 4);
     }
     for (int i = 0; i < a.as; ++i) {
       mbar_init(full + i, 5);  // x's copy and four warps
@@ -169,14 +173,14 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
           tma_load_2d(s + j * box, &ms, s_full + sb, x, y);
           tma_load_2d(s + a.sc_bytes + j * box, &mb, s_full + sb, x, y);
         }
-        for (int k = 0; k < stages; ++k) {
+        for (int k = 0; k < turns; ++k) {
           if (!mbar_wait(w_empty + st, ph ^ 1, err, 2)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(w_full + st, nb * 4096);
+          mbar_arrive_expect_tx(w_full + st, nb * 2048);
           for (int j = 0; j < nb; ++j)
-            tma_load_2d(sm_w + st * HQ_W_BYTES + j * 4096, &mw, w_full + st, k * 32, row + j * HQ_BLOCK);
+            tma_load_2d(sm_w + st * HQ_W_BYTES + j * 2048, &mw, w_full + st, k * 16, row + j * HQ_BLOCK);
           if (used < a.ws) ++used;
           if (++st == a.ws) {
             st = 0;
@@ -260,28 +264,26 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
     }
     __syncwarp();
   } else if (warp >= 4 && warp < 4 + HQ_UNPACK) {
-    // Turn n of all tiles' turns (128 codes, at a tile's end 64 or 128) is unpacked by the warps of group n % 4.
+    // Turn n of all tiles' turns is unpacked by the warps of group n % 4. A stage of packed words holds one turn, and
+    // their number is a multiple of 4, so that a stage is always the same group's: nobody looks at the barrier of
+    // another's, two phases early or late, where the parity is the same. (The slots' barriers have no such case: the
+    // products end in order, and the turn before this group's last one in a slot is at least as old.)
     const int q = warp & 3, group = (warp >> 2) & 3;
     const int r = q * 32 + lane;
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
-    const int turns = (a.kb + 1) / 2;
-    // Every warp waits for every stage and gives it back, used or not: a warp that left some out could look at a
-    // barrier two phases early or late, whose parity is the same. (The slots' barriers have no such case: the
-    // products end in order, and the turn before this group's last one in a slot is at least as old.)
-    int n = 0, slot = 0, ws = 0;
+    int k2 = group;               // this group's next turn, counted from the tile's first
+    int ws = group, slot = group;  // its stage and slot (there are at least 4 of each)
     uint32_t ph = 0, wph = 0;
     bool ok = true;
-    for (int i = 0; i < tiles && ok; ++i) {
+    for (int i = 0; i < tiles && ok; ++i, k2 -= turns) {
       const int sb = i & 1;
       const bool mine = q < b1 - b0 - 4 * i;
       const uint8_t* sc = sm_s + sb * 2 * a.sc_bytes;
       ok = __all_sync(0xffffffffu, mbar_wait(s_full + sb, (i >> 1) & 1, err, 6));
-      for (int k2 = 0; k2 < turns && ok; ++k2) {
-        if (!(k2 & 1)) {
-          ok = __all_sync(0xffffffffu, mbar_wait(w_full + ws, wph, err, 7));
-          if (!ok) break;
-        }
-        if ((n & 3) == group) {
+      for (; k2 < turns && ok; k2 += 4) {
+        ok = __all_sync(0xffffffffu, mbar_wait(w_full + ws, wph, err, 7));
+        if (!ok) break;
+        {
           const int k = 2 * k2;
           const bool two = k + 1 < a.kb;
           uint32_t sw, bw;  // two groups' scales and biases
@@ -296,13 +298,13 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
             bw = bt[0] | (uint32_t)bt[two] << 16;
           }
           const bool fast = __all_sync(0xffffffffu, q4_fast(sw));
-          const uint8_t* row = sm_w + ws * HQ_W_BYTES + r * 128;
+          const uint8_t* row = sm_w + ws * HQ_W_BYTES + r * 64;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (h == 1 && !two) break;
-            const int c = (k2 & 1) * 4 + h * 2;  // 16-byte chunks of the row's 128
-            const uint4 w0 = *reinterpret_cast<const uint4*>(row + ((c ^ (lane & 7)) << 4));
-            const uint4 w1 = *reinterpret_cast<const uint4*>(row + (((c + 1) ^ (lane & 7)) << 4));
+            const int c = h * 2, swz = (lane >> 1) & 3;  // 16-byte chunks of the row's 64
+            const uint4 w0 = *reinterpret_cast<const uint4*>(row + ((c ^ swz) << 4));
+            const uint4 w1 = *reinterpret_cast<const uint4*>(row + (((c + 1) ^ swz) << 4));
             const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
             const uint32_t s2 = __byte_perm(sw, 0, h ? 0x3232 : 0x1010), b2 = __byte_perm(bw, 0, h ? 0x3232 : 0x1010);
             uint32_t v[32];
@@ -326,18 +328,14 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(full + slot);
         }
-        ++n;
-        if (++slot == a.as) {
-          slot = 0;
-          ph ^= 1;
+        if (lane == 0) mbar_arrive(w_empty + ws);
+        if ((ws += 4) >= a.ws) {
+          ws -= a.ws;
+          wph ^= 1;
         }
-        if ((k2 & 1) || k2 == turns - 1) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(w_empty + ws);
-          if (++ws == a.ws) {
-            ws = 0;
-            wph ^= 1;
-          }
+        if ((slot += 4) >= a.as) {
+          slot -= a.as;
+          ph ^= 1;
         }
       }
       __syncwarp();
@@ -346,13 +344,15 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   } else if (warp >= 4 + HQ_UNPACK) {
     const int q = warp & 3;
     const float nan = __int_as_float(0x7fffffff);
-    float mx[NT], sum[NT];
+    float mx[NT], sum[NT];  // of token c * 32 + lane: the reference (its maximum so far, or that of some tile), the sum
     int top[NT];
+    float* ref = sm_ref + q * 32 * NT;  // -reference * log2(e) of each token; -inf past T: their columns hold anything
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
       mx[c] = -INFINITY;
       sum[c] = 0.f;
       top[c] = 0x7fffffff;
+      ref[c * 32 + lane] = -INFINITY;
     }
     bool ok = true;
     for (int i = 0; i < tiles && ok; ++i) {
@@ -367,7 +367,15 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
           float v[32];
-          tmem_ld32_wait(tmem + acc * 32 * NT + c * 32 + ((uint32_t)(q * 32) << 16), v);
+          const auto load = [&](float (&v)[32]) {
+            __syncwarp();
+            tmem_ld32_wait(tmem + acc * 32 * NT + c * 32 + ((uint32_t)(q * 32) << 16), v);
+            if (!in) {
+#pragma unroll
+              for (int b = 0; b < 32; ++b) v[b] = -INFINITY;
+            }
+          };
+          load(v);
 #pragma unroll 4
           for (int j = 0; j < a.K; ++j) {
             const int id = a.ids[j * 32 * NT + c * 32 + lane];
@@ -379,37 +387,49 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
               if (lane == at) a.out.ztgt[(size_t)(c * 32 + b) * a.K + j] = hd_pick(v, b);
             }
           }
-          __syncwarp();
-          if (!in) {
+          const bool live = c * 32 + lane < a.T;
+          float far = 0.f;
+          const auto exponents = [&]() {
+            far = -INFINITY;
 #pragma unroll
-            for (int b = 0; b < 32; ++b) v[b] = -INFINITY;
-          }
-          const float cm = hq_across(v, [](float x, float y) { return fmaxf(x, y); });
-          // the logits again, in the reduction's registers
-          tmem_ld32_wait(tmem + acc * 32 * NT + c * 32 + ((uint32_t)(q * 32) << 16), v);
-          if (!in) {
-#pragma unroll
-            for (int b = 0; b < 32; ++b) v[b] = -INFINITY;
-          }
-          int arg = 0;
-          if (a.out.top) {
-#pragma unroll
-            for (int b = 0; b < 32; ++b) {
-              const unsigned hit = __ballot_sync(0xffffffffu, v[b] == __shfl_sync(0xffffffffu, cm, b));
-              if (lane == b && hit) arg = __ffs(hit) - 1;
+            for (int b = 0; b < 32; b += 4) {
+              const float4 o = *reinterpret_cast<const float4*>(ref + c * 32 + b);
+              v[b] = fmaf(v[b], HD_LOG2E, o.x);
+              v[b + 1] = fmaf(v[b + 1], HD_LOG2E, o.y);
+              v[b + 2] = fmaf(v[b + 2], HD_LOG2E, o.z);
+              v[b + 3] = fmaf(v[b + 3], HD_LOG2E, o.w);
+              far = fmaxf(far, fmaxf(fmaxf(v[b], v[b + 1]), fmaxf(v[b + 2], v[b + 3])));
             }
+          };
+          bool anew = a.out.top || __any_sync(0xffffffffu, live && mx[c] == -INFINITY);
+          if (!anew) {
+            exponents();
+            anew = __any_sync(0xffffffffu, far > HQ_FAR);
+            if (anew) load(v);
           }
-          const float off = cm == -INFINITY ? 0.f : -cm * HD_LOG2E;
+          if (anew) {
+            const float cm = hq_across(v, [](float x, float y) { return fmaxf(x, y); });
+            load(v);  // the logits again, in the reduction's registers
+            if (a.out.top) {
+              int arg = 0;
 #pragma unroll
-          for (int b = 0; b < 32; ++b) v[b] = hd_ex2(fmaf(v[b], HD_LOG2E, __shfl_sync(0xffffffffu, off, b)));
-          const float cs = hq_across(v, [](float x, float y) { return x + y; });
-          if (cm > mx[c]) {
-            sum[c] = sum[c] * hd_ex2((mx[c] - cm) * HD_LOG2E) + cs;
-            mx[c] = cm;
-            top[c] = id0 + arg;
-          } else {
-            sum[c] += cm == -INFINITY ? cs : cs * hd_ex2((cm - mx[c]) * HD_LOG2E);
+              for (int b = 0; b < 32; ++b) {
+                const unsigned hit = __ballot_sync(0xffffffffu, v[b] == __shfl_sync(0xffffffffu, cm, b));
+                if (lane == b && hit) arg = __ffs(hit) - 1;
+              }
+              if (cm > mx[c]) top[c] = id0 + arg;
+            }
+            if (cm > mx[c]) {
+              sum[c] *= hd_ex2((mx[c] - cm) * HD_LOG2E);  // mx = -inf: sum is 0 (or NaN)
+              mx[c] = cm;
+            }
+            if (live) ref[c * 32 + lane] = mx[c] == -INFINITY ? 0.f : -mx[c] * HD_LOG2E;
+            __syncwarp();
+            exponents();
           }
+#pragma unroll
+          for (int b = 0; b < 32; ++b) v[b] = hd_ex2(v[b]);
+          sum[c] += hq_across(v, [](float x, float y) { return x + y; });
         }
       }
       tc_fence_before();
@@ -482,9 +502,9 @@ static bool hq_layout(int T, int H, HqArgs* a, size_t* smem) {
   a->kb = H / 64;
   a->wide = H % 512 == 0;
   a->sc_bytes = (128 * a->kb * 2 + 2047) / 2048 * 2048;
-  const size_t fixed = 1024 + 4 * (size_t)a->sc_bytes + (size_t)12 * 32 * NT * 4 + 42 * 8 + 32;
+  const size_t fixed = 1024 + 4 * (size_t)a->sc_bytes + (size_t)16 * 32 * NT * 4 + 50 * 8 + 32;
   for (a->as = std::min(6, (512 - 64 * NT) / 64); a->as >= 4; --a->as) {  // below 4 a group could pass its own slot
-    for (a->ws = 6; a->ws >= 3; --a->ws) {
+    for (a->ws = 12; a->ws >= 4; a->ws -= 4) {
       *smem = fixed + 2 * (size_t)a->as * hq_x_bytes(a->N) + (size_t)a->ws * HQ_W_BYTES;
       if (*smem <= HQ_SMEM_MAX) return true;
     }
@@ -533,7 +553,7 @@ int hq_loss_parts(const __nv_bfloat16* x, long long ldx, int T, int H, const HdH
   LG_LAUNCH_CHECK("head_order");
   const uint64_t groups = (uint64_t)V * (H / 64), gbytes = align_up(groups * 2, 16);
   CUtensorMap m[4];
-  int rc = make_map_2d(&m[0], w.w, false, H / 8, V, (uint64_t)H / 2, 32, 32, 128);
+  int rc = make_map_2d(&m[0], w.w, false, H / 8, V, (uint64_t)H / 2, 16, 32, 64);
   for (int i = 1; i < 3 && rc == LG_OK; ++i) {
     const void* p = i == 1 ? w.scales : w.biases;
     rc = a.wide ? make_map_2d(&m[i], p, true, H / 64, V, (uint64_t)H / 32, 8, 128, 0)

@@ -66,6 +66,9 @@ def test_4bit_head_of_few_tokens(T, V, H, K):
     within(lse, r["lse"], r["blse"])
     z = x.double().cpu() @ W.double().cpu().T
     assert (z.amax(1) - z.gather(1, top.long().cpu()[:, None])[:, 0] <= 2 * r["blse"]).all()
+    loss, lse = ops.head_loss(x, head, ids, weights)  # without ids of maxima the sums have other references
+    within(loss, r["loss"], r["bloss"])
+    within(lse, r["lse"], r["blse"])
     again = ops.head_loss(x, head, ids, weights)
     assert torch.equal(again[0], loss) and torch.equal(again[1], lse)
 
@@ -382,3 +385,26 @@ def test_4bit_scales_of_every_size(T):
     within(loss, r["loss"], r["bloss"] + far)
     within(lse, r["lse"], r["blse"] + far)
     within(ops.head_loss_grad(x, (q, s, b), ids, lse, gr, dw=False)[0], r["dx"], r["bdx"])
+
+
+@pytest.mark.parametrize("T", [9, 50, 128])
+@pytest.mark.parametrize("order", [1, -1])
+def test_4bit_logits_far_above_those_before(T, order):
+    """Logits that rise (or fall) by hundreds along the vocabulary: the reference of the exponentials has to follow,
+    within a CTA's tiles and between CTAs."""
+    V, H = 40000, 64
+    g = torch.Generator(device="cuda").manual_seed(T)
+    steps = order * torch.linspace(-900, 900, V // 32, device="cuda").repeat_interleave(32)
+    rows = (torch.randn(V, H, generator=g, device="cuda") * 0.1 + (steps / H)[:, None])
+    head = ops.quantize(rows, 64, 4)
+    W = dequant64(head)
+    x = (1 + 0.1 * torch.randn(T, H, generator=g, device="cuda")).bfloat16()
+    x[1] *= -1  # this token's logits go the other way
+    ids = torch.randint(0, V, (T,), generator=g, device="cuda", dtype=torch.int32)
+    ids[:2] = torch.tensor([0, V - 1])
+    r = reference(x, W, ids, None)
+    far = 1000 * 2 ** -21  # the exponentials' arguments: up to 1,500, rounded to 2^-24 of that
+    for top in (False, True):
+        loss, lse = ops.head_loss(x, head, ids, top=top)[:2]
+        within(loss, r["loss"], r["bloss"] + far)
+        within(lse, r["lse"], r["blse"] + far)
