@@ -1014,13 +1014,8 @@ using namespace lg;
 
 extern "C" size_t lg_head_loss_workspace_bytes(int T, int H, int V, int K, int bits, int top) {
   if (T < 1 || H < 8 || V < 1 || K < 1) return 256;
-  // The larger of the two ways: which one a 4-bit head takes also depends on its pointers.
   const bool quant = bits == 4;
-  const size_t n = hd_carve(nullptr, T, H, V, K, quant, false, false, false, false, top != 0).bytes;
-  if (!quant) return n;
-  const HdHead head = {nullptr, nullptr, nullptr, H};
-  if (!hq_takes(T, H, V, K, head)) return n;
-  return std::max(n, hd_carve(nullptr, T, H, V, K, true, true, false, false, false, top != 0).bytes);
+  return hd_carve(nullptr, T, H, V, K, quant, quant && hq_takes(T, H), false, false, false, top != 0).bytes;
 }
 
 extern "C" size_t lg_head_loss_grad_workspace_bytes(int T, int H, int V, int K, int bits, int dx, int dw) {
@@ -1039,7 +1034,7 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
   const HdHead head = {w, static_cast<const __nv_bfloat16*>(w_scales),
                        static_cast<const __nv_bfloat16*>(w_biases), ldw};
   const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);
-  const bool few = quant && hq_takes(T, H, V, K, head);
+  const bool few = quant && hq_takes(T, H);
   const HdWork k = hd_carve(workspace, T, H, V, K, quant, few, false, false, false, top != nullptr);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < k.bytes)
     return fail(LG_ERR_WORKSPACE, "head_loss: workspace of %zu bytes, need %zu", workspace_bytes, k.bytes);

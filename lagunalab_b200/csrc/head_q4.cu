@@ -4,10 +4,11 @@
 // the weights are the product's A operand, taken from TMEM, where the warps that unpack them write them; x is B.
 // So few tokens cost few columns, and an unpacked weight crosses neither memory nor shared memory.
 //
-//   warp 0       TMA: packed words (32 rows x 128 codes a box, 64-byte swizzle), scales and biases
+//   warp 0       TMA: packed words (32 rows x 256 codes a box, 128-byte swizzle)
 //   warp 2       TMA: x, 128 columns a slot
 //   warps 4-19   unpack: a row a thread, 128 codes a turn (two quantization groups), four groups of four warps in
-//                turns; tcgen05.st of 32 columns a group
+//                turns; tcgen05.st of 32 columns a group. Scales and biases come by plain loads a turn ahead: as
+//                TMA boxes (16 bytes of a row) they were a quarter of all rows that TMA moved, and waited for
 //   warp 1       four products (M 128, N, K 16) a 64-wide block into one of two accumulators
 //   warps 20-23  per tile and token the sum of exponentials over the warp's 32 rows, which lie across its lanes: a
 //                transposing reduction (31 shuffles for 32 columns) leaves token i with lane i. The exponentials are
@@ -36,7 +37,7 @@ using namespace tc;
 constexpr int HQ_UNPACK = 16;  // warps
 constexpr int HQ_THREADS = (8 + HQ_UNPACK) * 32;
 constexpr int HQ_BLOCK = 32;               // ids a block: a warp's TMEM lanes
-constexpr int HQ_W_BYTES = 4 * 32 * 64;    // a stage of packed words, one turn's: 128 rows x 128 codes
+constexpr int HQ_W_BYTES = 4 * 32 * 128;   // a stage of packed words, two turns': 128 rows x 256 codes
 constexpr float HQ_FAR = 90.f;             // of exponents of 2: 100,000 terms of 2^90 are below 2^127
 constexpr int HQ_SMEM_MAX = 224 << 10;     // a CTA of hq_order_kernel has room beside it
 
@@ -44,9 +45,10 @@ struct HqArgs {
   int T, N, H, V, K;
   int kb;       // 64-wide blocks of H
   int blocks;   // blocks of 32 ids
-  int as, ws;   // slots of unpacked weights and x (128 columns), stages of packed words: a multiple of 4
-  int sc_bytes;  // scales of a tile, a multiple of 2,048
-  int wide;      // scales by eight groups: [H / 512][128 rows][8]; else [128 rows][H / 64]
+  int as, ws;   // slots of unpacked weights and x (128 columns), stages of packed words: even
+  unsigned inv;  // 2^32 / as, up
+  bool pairs;    // two groups' scales are one aligned load
+  const uint16_t *scales, *biases;
   const int* ids;  // [K][32 NT], -1 past T
   HdParts out;
 };
@@ -93,23 +95,21 @@ __device__ __forceinline__ float hq_across(float (&v)[32], Op op) {
 
 template <int NT>  // blocks of 32 tokens
 __global__ void __launch_bounds__(HQ_THREADS, 1)
-    hq_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap ms,
-              const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mx, const HqArgs a) {
+    hq_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx, const HqArgs a) {
   extern __shared__ uint8_t hq_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)hq_raw + 1023) & ~(uintptr_t)1023);
   const int x_bytes = hq_x_bytes(a.N);
   uint8_t* sm_w = smem;
   uint8_t* sm_x = sm_w + a.ws * HQ_W_BYTES;
-  uint8_t* sm_s = sm_x + 2 * a.as * x_bytes;  // [2][scales, biases]
-  float* sm_m = reinterpret_cast<float*>(sm_s + 4 * a.sc_bytes);
+  float* sm_m = reinterpret_cast<float*>(sm_x + 2 * a.as * x_bytes);
   float* sm_sum = sm_m + 4 * 32 * NT;
   int* sm_top = reinterpret_cast<int*>(sm_sum + 4 * 32 * NT);
   float* sm_ref = reinterpret_cast<float*>(sm_top + 4 * 32 * NT);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm_ref + 4 * 32 * NT);
-  uint64_t *w_full = bars, *w_empty = bars + 12, *full = bars + 24, *empty = bars + 32;
-  uint64_t *s_full = bars + 40, *s_empty = bars + 42, *acc_full = bars + 44, *acc_empty = bars + 46;
-  uint64_t* done = bars + 48;
-  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(bars + 49);
+  uint64_t *w_full = bars, *w_empty = bars + 8, *full = bars + 16, *empty = bars + 24;
+  uint64_t *acc_full = bars + 32, *acc_empty = bars + 34;
+  uint64_t* done = bars + 36;
+  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(bars + 37);
   int* err = reinterpret_cast<int*>(tmem_base + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -117,19 +117,18 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   const int b1 = (int)((long long)a.blocks * (blockIdx.x + 1) / gridDim.x);
   const int tiles = (b1 - b0 + 3) / 4;
   const int turns = (a.kb + 1) / 2;  // of 128 codes (the last perhaps 64), a tile
+  const int stages = (turns + 1) / 2;  // of packed words, a tile
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.ws; ++i) {
       mbar_init(w_full + i, 1);
-      mbar_init(w_empty + i, 4);
+      mbar_init(w_empty + i, 8);  // the two groups of its turns
     }
     for (int i = 0; i < a.as; ++i) {
       mbar_init(full + i, 5);  // x's copy and four warps
       mbar_init(empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + i, 1);
-      mbar_init(s_empty + i, HQ_UNPACK);
       mbar_init(acc_full + i, 1);
       mbar_init(acc_empty + i, 4);
     }
@@ -137,8 +136,6 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
     for (int i = 0; i < 4; ++i) err[i] = 0;  // of all roles; of the two copies' ends; of the products' end
     fence_mbar_init();
     prefetch_tmap(&mw);
-    prefetch_tmap(&ms);
-    prefetch_tmap(&mb);
     prefetch_tmap(&mx);
   }
   if (warp == 3) {
@@ -159,28 +156,16 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
       int st = 0, used = 0;
       uint32_t ph = 0;
       bool ok = true;
-      int i = 0;
-      for (; i < tiles && ok; ++i) {
+      for (int i = 0; i < tiles && ok; ++i) {
         const int row = (b0 + 4 * i) * HQ_BLOCK, nb = min(4, b1 - b0 - 4 * i);
-        const int sb = i & 1;
-        if (!mbar_wait(s_empty + sb, ((i >> 1) & 1) ^ 1, err, 1)) break;
-        const int boxes = a.wide ? a.kb / 8 : (nb * HQ_BLOCK * a.kb + 255) / 256;
-        const int box = a.wide ? 2048 : 512;
-        mbar_arrive_expect_tx(s_full + sb, 2 * boxes * box);
-        uint8_t* s = sm_s + sb * 2 * a.sc_bytes;
-        for (int j = 0; j < boxes; ++j) {
-          const int x = a.wide ? j * 8 : row * a.kb + j * 256, y = a.wide ? row : 0;
-          tma_load_2d(s + j * box, &ms, s_full + sb, x, y);
-          tma_load_2d(s + a.sc_bytes + j * box, &mb, s_full + sb, x, y);
-        }
-        for (int k = 0; k < turns; ++k) {
+        for (int k = 0; k < stages; ++k) {
           if (!mbar_wait(w_empty + st, ph ^ 1, err, 2)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(w_full + st, nb * 2048);
+          mbar_arrive_expect_tx(w_full + st, nb * 4096);
           for (int j = 0; j < nb; ++j)
-            tma_load_2d(sm_w + st * HQ_W_BYTES + j * 2048, &mw, w_full + st, k * 16, row + j * HQ_BLOCK);
+            tma_load_2d(sm_w + st * HQ_W_BYTES + j * 4096, &mw, w_full + st, k * 32, row + j * HQ_BLOCK);
           if (used < a.ws) ++used;
           if (++st == a.ws) {
             st = 0;
@@ -193,8 +178,6 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
         const int s = (st - j + a.ws) % a.ws;
         mbar_wait(w_full + s, s < st ? ph : ph ^ 1, err + 1, 2, 400000000LL);
       }
-      for (int j = max(0, i - 2); j < i; ++j)
-        mbar_wait(s_full + (j & 1), (j >> 1) & 1, err + 1, 1, 400000000LL);
     }
     __syncwarp();
   } else if (warp == 2) {
@@ -264,47 +247,63 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
     }
     __syncwarp();
   } else if (warp >= 4 && warp < 4 + HQ_UNPACK) {
-    // Turn n of all tiles' turns is unpacked by the warps of group n % 4. A stage of packed words holds one turn, and
-    // their number is a multiple of 4, so that a stage is always the same group's: nobody looks at the barrier of
-    // another's, two phases early or late, where the parity is the same. (The slots' barriers have no such case: the
-    // products end in order, and the turn before this group's last one in a slot is at least as old.)
-    const int q = warp & 3, group = (warp >> 2) & 3;
+    // Stage s holds two turns, of groups 2 s % 4 and the next one (a tile's last stage may have one turn: its second
+    // group unpacks nothing). The number of stages is even, so that a stage is always the same groups': nobody looks at
+    // the barrier of another's, two phases early or late, where the parity is the same. The slots' barriers have no
+    // such case as long as a group waits for one of every four turns, or of as many as there are slots: the products
+    // end in order, so that the turn two rounds before the one waited for has then ended. A group without a turn
+    // therefore waits as the next turn's group does.
+    const int q = warp & 3, group = (warp >> 2) & 3, half = group & 1;
     const int r = q * 32 + lane;
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
-    int k2 = group;               // this group's next turn, counted from the tile's first
-    int ws = group, slot = group;  // its stage and slot (there are at least 4 of each)
-    uint32_t ph = 0, wph = 0;
+    int i = 0, st = group >> 1;  // tile, stage in it
+    while (st >= stages) st -= stages, ++i;
+    int ws = group >> 1;
+    uint32_t wph = 0;
     bool ok = true;
-    for (int i = 0; i < tiles && ok; ++i, k2 -= turns) {
-      const int sb = i & 1;
+    // Scales and biases of this row's two groups in turn 2 st + half of tile i.
+    const auto scales = [&](int i, int st, uint32_t& sw, uint32_t& bw) {
+      const int blk = b0 + 4 * i + q, row = blk * HQ_BLOCK + lane, k = 2 * (2 * st + half);
+      sw = bw = 0;
+      if (blk < b1 && row < a.V && k < a.kb) {
+        const size_t at = (size_t)row * a.kb + k;
+        if (a.pairs) {
+          sw = __ldg(reinterpret_cast<const uint32_t*>(a.scales + at));
+          bw = __ldg(reinterpret_cast<const uint32_t*>(a.biases + at));
+        } else {
+          const int two = k + 1 < a.kb;
+          sw = __ldg(a.scales + at) | (uint32_t)__ldg(a.scales + at + two) << 16;
+          bw = __ldg(a.biases + at) | (uint32_t)__ldg(a.biases + at + two) << 16;
+        }
+      }
+    };
+    uint32_t next_s = 0, next_b = 0;
+    if (i < tiles) scales(i, st, next_s, next_b);
+    while (i < tiles) {
       const bool mine = q < b1 - b0 - 4 * i;
-      const uint8_t* sc = sm_s + sb * 2 * a.sc_bytes;
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full + sb, (i >> 1) & 1, err, 6));
-      for (; k2 < turns && ok; k2 += 4) {
-        ok = __all_sync(0xffffffffu, mbar_wait(w_full + ws, wph, err, 7));
+      const int k2 = 2 * st + half;
+      const uint32_t sw = next_s, bw = next_b;
+      int ni = i, ns = st + 2;
+      while (ns >= stages) ns -= stages, ++ni;
+      if (ni < tiles) scales(ni, ns, next_s, next_b);
+      ok = __all_sync(0xffffffffu, mbar_wait(w_full + ws, wph, err, 7));
+      if (!ok) break;
+      const unsigned n = i * turns + min(k2, turns), turn = __umulhi(n, a.inv);
+      const int slot = n - turn * a.as;
+      if (k2 == turns) {
+        ok = __all_sync(0xffffffffu, mbar_wait(empty + slot, (turn & 1) ^ 1, err, 8));
         if (!ok) break;
+      } else {
         {
-          const int k = 2 * k2;
-          const bool two = k + 1 < a.kb;
-          uint32_t sw, bw;  // two groups' scales and biases
-          if (a.wide) {
-            const uint8_t* at = sc + (k >> 3) * 2048 + r * 16 + (k & 7) * 2;
-            sw = *reinterpret_cast<const uint32_t*>(at);
-            bw = *reinterpret_cast<const uint32_t*>(at + a.sc_bytes);
-          } else {
-            const uint16_t* at = reinterpret_cast<const uint16_t*>(sc) + r * a.kb + k;
-            const uint16_t* bt = reinterpret_cast<const uint16_t*>(sc + a.sc_bytes) + r * a.kb + k;
-            sw = at[0] | (uint32_t)at[two] << 16;
-            bw = bt[0] | (uint32_t)bt[two] << 16;
-          }
-          const bool fast = __all_sync(0xffffffffu, q4_fast(sw));
-          const uint8_t* row = sm_w + ws * HQ_W_BYTES + r * 64;
+          const bool two = 2 * k2 + 1 < a.kb;
+          const bool fast = __all_sync(0xffffffffu, !mine || q4_fast(sw));
+          const uint8_t* row = sm_w + ws * HQ_W_BYTES + r * 128;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (h == 1 && !two) break;
-            const int c = h * 2, swz = (lane >> 1) & 3;  // 16-byte chunks of the row's 64
-            const uint4 w0 = *reinterpret_cast<const uint4*>(row + ((c ^ swz) << 4));
-            const uint4 w1 = *reinterpret_cast<const uint4*>(row + (((c + 1) ^ swz) << 4));
+            const int c = half * 4 + h * 2;  // 16-byte chunks of the row's 128
+            const uint4 w0 = *reinterpret_cast<const uint4*>(row + ((c ^ (lane & 7)) << 4));
+            const uint4 w1 = *reinterpret_cast<const uint4*>(row + (((c + 1) ^ (lane & 7)) << 4));
             const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
             const uint32_t s2 = __byte_perm(sw, 0, h ? 0x3232 : 0x1010), b2 = __byte_perm(bw, 0, h ? 0x3232 : 0x1010);
             uint32_t v[32];
@@ -316,7 +315,7 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
               for (int j = 0; j < 8; ++j) q4_word_any(w[j], s2, b2, v + 4 * j);
             }
             if (h == 0) {
-              ok = __all_sync(0xffffffffu, mbar_wait(empty + slot, ph ^ 1, err, 8));
+              ok = __all_sync(0xffffffffu, mbar_wait(empty + slot, (turn & 1) ^ 1, err, 8));
               if (!ok) break;
               tc_fence_after();
             }
@@ -328,18 +327,15 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(full + slot);
         }
-        if (lane == 0) mbar_arrive(w_empty + ws);
-        if ((ws += 4) >= a.ws) {
-          ws -= a.ws;
-          wph ^= 1;
-        }
-        if ((slot += 4) >= a.as) {
-          slot -= a.as;
-          ph ^= 1;
-        }
       }
       __syncwarp();
-      if (ok && lane == 0) mbar_arrive(s_empty + sb);
+      if (lane == 0) mbar_arrive(w_empty + ws);
+      if ((ws += 2) >= a.ws) {
+        ws -= a.ws;
+        wph ^= 1;
+      }
+      i = ni;
+      st = ns;
     }
   } else if (warp >= 4 + HQ_UNPACK) {
     const int q = warp & 3;
@@ -500,29 +496,29 @@ static bool hq_layout(int T, int H, HqArgs* a, size_t* smem) {
   const int NT = hq_nt(T);
   a->N = (T + 15) / 16 * 16;
   a->kb = H / 64;
-  a->wide = H % 512 == 0;
-  a->sc_bytes = (128 * a->kb * 2 + 2047) / 2048 * 2048;
-  const size_t fixed = 1024 + 4 * (size_t)a->sc_bytes + (size_t)16 * 32 * NT * 4 + 50 * 8 + 32;
-  for (a->as = std::min(6, (512 - 64 * NT) / 64); a->as >= 4; --a->as) {  // below 4 a group could pass its own slot
-    for (a->ws = 12; a->ws >= 4; a->ws -= 4) {
+  const size_t fixed = 1024 + (size_t)16 * 32 * NT * 4 + 38 * 8 + 32;
+  for (a->as = std::min(6, (512 - 64 * NT) / 64); a->as >= 4; --a->as) {
+    for (a->ws = 8; a->ws >= 4; a->ws -= 2) {
       *smem = fixed + 2 * (size_t)a->as * hq_x_bytes(a->N) + (size_t)a->ws * HQ_W_BYTES;
-      if (*smem <= HQ_SMEM_MAX) return true;
+      if (*smem <= HQ_SMEM_MAX) {
+        a->inv = (unsigned)(((1ULL << 32) + a->as - 1) / a->as);
+        return true;
+      }
     }
   }
   return false;
 }
 
-bool hq_takes(int T, int H, int V, int K, const HdHead& w) {
+bool hq_takes(int T, int H) {
   HqArgs a;
   size_t smem;
-  return T <= HQ_MAXT && (long long)V * (H / 64) < (1LL << 31) && aligned(w.scales, 16) &&
-         aligned(w.biases, 16) && hq_layout(T, H, &a, &smem);
+  return T <= HQ_MAXT && hq_layout(T, H, &a, &smem);
 }
 
 int hq_parts(int V) { return std::min(device_sm_count(), (V + HQ_BLOCK - 1) / HQ_BLOCK); }
 
 template <int NT>
-static int hq_launch(const CUtensorMap (&m)[4], const HqArgs& a, int grid, size_t smem, cudaStream_t st) {
+static int hq_launch(const CUtensorMap (&m)[2], const HqArgs& a, int grid, size_t smem, cudaStream_t st) {
   static std::atomic<bool> done[64];
   int dev = 0;
   LG_CUDA_TRY(cudaGetDevice(&dev));
@@ -530,7 +526,7 @@ static int hq_launch(const CUtensorMap (&m)[4], const HqArgs& a, int grid, size_
     LG_CUDA_TRY(cudaFuncSetAttribute(hq_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, HQ_SMEM_MAX));
     if (dev < 64) done[dev].store(true, std::memory_order_relaxed);
   }
-  LG_CUDA_TRY(launch_early(hq_kernel<NT>, grid, HQ_THREADS, smem, st, m[0], m[1], m[2], m[3], a));
+  LG_CUDA_TRY(launch_early(hq_kernel<NT>, grid, HQ_THREADS, smem, st, m[0], m[1], a));
   LG_LAUNCH_CHECK("head_q4");
   return LG_OK;
 }
@@ -546,20 +542,17 @@ int hq_loss_parts(const __nv_bfloat16* x, long long ldx, int T, int H, const HdH
   a.K = K;
   a.blocks = (V + HQ_BLOCK - 1) / HQ_BLOCK;
   a.ids = idt;
+  a.scales = reinterpret_cast<const uint16_t*>(w.scales);
+  a.biases = reinterpret_cast<const uint16_t*>(w.biases);
+  a.pairs = a.kb % 2 == 0 && aligned(w.scales, 4) && aligned(w.biases, 4);
   a.out = out;
   const int n = T * (H / 8);
   const int nt = 32 * hq_nt(T);
   hq_order_kernel<<<(std::max(n, K * nt) + 255) / 256, 256, 0, st>>>(x, ldx, n, H / 8, xp, ids, T, K, nt, idt);
   LG_LAUNCH_CHECK("head_order");
-  const uint64_t groups = (uint64_t)V * (H / 64), gbytes = align_up(groups * 2, 16);
-  CUtensorMap m[4];
-  int rc = make_map_2d(&m[0], w.w, false, H / 8, V, (uint64_t)H / 2, 16, 32, 64);
-  for (int i = 1; i < 3 && rc == LG_OK; ++i) {
-    const void* p = i == 1 ? w.scales : w.biases;
-    rc = a.wide ? make_map_2d(&m[i], p, true, H / 64, V, (uint64_t)H / 32, 8, 128, 0)
-                : make_map_2d(&m[i], p, true, groups, 1, gbytes, 256, 1, 0);
-  }
-  if (rc == LG_OK) rc = make_map_2d(&m[3], xp, true, H, T, (uint64_t)H * 2, 64, a.N, 128);
+  CUtensorMap m[2];
+  int rc = make_map_2d(&m[0], w.w, false, H / 8, V, (uint64_t)H / 2, 32, 32, 128);
+  if (rc == LG_OK) rc = make_map_2d(&m[1], xp, true, H, T, (uint64_t)H * 2, 64, a.N, 128);
   if (rc != LG_OK) return rc;
   const int grid = out.parts;
   return T <= 32 ? hq_launch<1>(m, a, grid, smem, st)

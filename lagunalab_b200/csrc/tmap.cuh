@@ -23,7 +23,7 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tmap_encode_fn() {
 }
 
 // 2D row-major map: `rows` rows of `inner` elements (bf16 or uint32), `row_bytes` apart; a
-// box of box_inner x box_rows; swz = 128 / 64 / 32 / 0 for the 128-, 64-, 32-byte or no swizzle.
+// box of box_inner x box_rows; swz = 128 / 32 / 0 for the 128-byte, 32-byte or no swizzle.
 // Rows past `rows` read as zeros.
 inline int make_map_2d(CUtensorMap* m, const void* base, bool bf16, uint64_t inner,
                        uint64_t rows, uint64_t row_bytes, uint32_t box_inner, uint32_t box_rows,
@@ -36,10 +36,8 @@ inline int make_map_2d(CUtensorMap* m, const void* base, bool bf16, uint64_t inn
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, 2,
                   const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swz == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                  : swz == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                  : swz == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
-                              : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  swz == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                             : (swz == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_NONE),
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(LG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return LG_OK;
