@@ -1015,7 +1015,7 @@ using namespace lg;
 extern "C" size_t lg_head_loss_workspace_bytes(int T, int H, int V, int K, int bits, int top) {
   if (T < 1 || H < 8 || V < 1 || K < 1) return 256;
   const bool quant = bits == 4;
-  return hd_carve(nullptr, T, H, V, K, quant, quant && hq_takes(T, H), false, false, false, top != 0).bytes;
+  return hd_carve(nullptr, T, H, V, K, quant, quant && T <= HQ_MAXT, false, false, false, top != 0).bytes;
 }
 
 extern "C" size_t lg_head_loss_grad_workspace_bytes(int T, int H, int V, int K, int bits, int dx, int dw) {
@@ -1034,7 +1034,7 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
   const HdHead head = {w, static_cast<const __nv_bfloat16*>(w_scales),
                        static_cast<const __nv_bfloat16*>(w_biases), ldw};
   const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);
-  const bool few = quant && hq_takes(T, H);
+  const bool few = quant && T <= HQ_MAXT;
   const HdWork k = hd_carve(workspace, T, H, V, K, quant, few, false, false, false, top != nullptr);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < k.bytes)
     return fail(LG_ERR_WORKSPACE, "head_loss: workspace of %zu bytes, need %zu", workspace_bytes, k.bytes);

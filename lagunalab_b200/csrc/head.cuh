@@ -83,7 +83,6 @@ struct HdParts {
 // head_q4.cu: the loss's parts from a 4-bit head for few tokens, without the bf16 weights in memory. xp: T H
 // bf16, idt: HQ_MAXT K ints of workspace.
 constexpr int HQ_MAXT = 128;
-bool hq_takes(int T, int H);
 int hq_parts(int V);
 int hq_loss_parts(const __nv_bfloat16* x, long long ldx, int T, int H, const HdHead& w, int V, const int* ids,
                   int K, __nv_bfloat16* xp, int* idt, const HdParts& out, cudaStream_t st);

@@ -45,15 +45,17 @@ struct HqArgs {
   int T, N, H, V, K;
   int kb;       // 64-wide blocks of H
   int blocks;   // blocks of 32 ids
-  int as, ws;   // slots of unpacked weights and x (128 columns), stages of packed words: even
-  unsigned inv;  // 2^32 / as, up
+  int ws;        // stages of packed words: even
   bool pairs;    // two groups' scales are one aligned load
   const uint16_t *scales, *biases;
   const int* ids;  // [K][32 NT], -1 past T
   HdParts out;
 };
 
-__host__ __device__ __forceinline__ int hq_x_bytes(int N) { return (N * 128 + 1023) / 1024 * 1024; }
+// Slots of unpacked weights and x, 128 columns each: 64 columns of TMEM beside two accumulators of 32 NT. At least 4
+// (four groups of warps write side by side).
+template <int NT>
+constexpr int HQ_SLOTS = NT == 4 ? 4 : 6;
 
 // A[tmem] B[smem]: M 128 x N x 16.
 __device__ __forceinline__ void hq_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -95,13 +97,15 @@ __device__ __forceinline__ float hq_across(float (&v)[32], Op op) {
 
 template <int NT>  // blocks of 32 tokens
 __global__ void __launch_bounds__(HQ_THREADS, 1)
-    hq_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx, const HqArgs a) {
+    hq_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mw4,
+              const __grid_constant__ CUtensorMap mx, const HqArgs a) {
+  constexpr int AS = HQ_SLOTS<NT>;
   extern __shared__ uint8_t hq_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)hq_raw + 1023) & ~(uintptr_t)1023);
-  const int x_bytes = hq_x_bytes(a.N);
+  const int x_bytes = a.N * 128;  // 64 columns of x
   uint8_t* sm_w = smem;
   uint8_t* sm_x = sm_w + a.ws * HQ_W_BYTES;
-  float* sm_m = reinterpret_cast<float*>(sm_x + 2 * a.as * x_bytes);
+  float* sm_m = reinterpret_cast<float*>(sm_x + 2 * AS * x_bytes);
   float* sm_sum = sm_m + 4 * 32 * NT;
   int* sm_top = reinterpret_cast<int*>(sm_sum + 4 * 32 * NT);
   float* sm_ref = reinterpret_cast<float*>(sm_top + 4 * 32 * NT);
@@ -112,7 +116,7 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(bars + 37);
   int* err = reinterpret_cast<int*>(tmem_base + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // uniform, and known to be
   const int b0 = (int)((long long)a.blocks * blockIdx.x / gridDim.x);
   const int b1 = (int)((long long)a.blocks * (blockIdx.x + 1) / gridDim.x);
   const int tiles = (b1 - b0 + 3) / 4;
@@ -124,7 +128,7 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
       mbar_init(w_full + i, 1);
       mbar_init(w_empty + i, 8);  // the two groups of its turns
     }
-    for (int i = 0; i < a.as; ++i) {
+    for (int i = 0; i < AS; ++i) {
       mbar_init(full + i, 5);  // x's copy and four warps
       mbar_init(empty + i, 1);
     }
@@ -136,6 +140,7 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
     for (int i = 0; i < 4; ++i) err[i] = 0;  // of all roles; of the two copies' ends; of the products' end
     fence_mbar_init();
     prefetch_tmap(&mw);
+    prefetch_tmap(&mw4);
     prefetch_tmap(&mx);
   }
   if (warp == 3) {
@@ -164,8 +169,12 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
             break;
           }
           mbar_arrive_expect_tx(w_full + st, nb * 4096);
-          for (int j = 0; j < nb; ++j)
-            tma_load_2d(sm_w + st * HQ_W_BYTES + j * 4096, &mw, w_full + st, k * 32, row + j * HQ_BLOCK);
+          if (nb == 4) {
+            tma_load_2d(sm_w + st * HQ_W_BYTES, &mw4, w_full + st, k * 32, row);
+          } else {
+            for (int j = 0; j < nb; ++j)
+              tma_load_2d(sm_w + st * HQ_W_BYTES + j * 4096, &mw, w_full + st, k * 32, row + j * HQ_BLOCK);
+          }
           if (used < a.ws) ++used;
           if (++st == a.ws) {
             st = 0;
@@ -185,66 +194,71 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
       int st = 0, used = 0;
       uint32_t ph = 0;
       bool ok = true;
+#pragma unroll 1
       for (int i = 0; i < tiles && ok; ++i) {
+#pragma unroll 1
         for (int k = 0; k < a.kb; k += 2) {
           if (!mbar_wait(empty + st, ph ^ 1, err, 3)) {
             ok = false;
             break;
           }
-          const int n = min(2, a.kb - k);
-          mbar_arrive_expect_tx(full + st, n * a.N * 128);
-          for (int j = 0; j < n; ++j)
-            tma_load_2d(sm_x + (2 * st + j) * x_bytes, &mx, full + st, (k + j) * 64, 0);
-          if (used < a.as) ++used;
-          if (++st == a.as) {
+          // both 64s of the turn: [2][N][64] (the second of an odd H / 64 lies past H: zeros)
+          mbar_arrive_expect_tx(full + st, 2 * x_bytes);
+          tma_load_3d(sm_x + 2 * st * x_bytes, &mx, full + st, 0, 0, k);
+          if (used < AS) ++used;
+          if (++st == AS) {
             st = 0;
             ph ^= 1;
           }
         }
       }
       for (int j = used; j > 0; --j) {
-        const int s = (st - j + a.as) % a.as;
+        const int s = (st - j + AS) % AS;
         mbar_wait(full + s, s < st ? ph : ph ^ 1, err + 2, 3, 400000000LL);
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (elect_one()) {
-      const uint32_t idesc = idesc_bf16(128, a.N);
-      const uint64_t hi = (uint64_t)SW128_HI << 32;
-      // One wait and one commit for 128 columns: with one each for 64 columns of x beside them this thread took 630
-      // cycles a turn, three times what the products take.
-      int slot = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int i = 0; i < tiles && ok; ++i) {
-        const int acc = i & 1;
-        if (!mbar_wait(acc_empty + acc, ((i >> 1) & 1) ^ 1, err, 4)) break;
-        for (int k = 0; k < a.kb; k += 2) {
-          if (!mbar_wait(full + slot, ph, err, 5)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t d = tmem + acc * 32 * NT, da = tmem_a + slot * 64;
-          const uint32_t db = sw128_lo(smem_u32(sm_x + 2 * slot * x_bytes));
+    // The whole warp goes through the loop and one lane issues: counters and descriptors then stay in uniform
+    // registers. With a lane's own loop each product's operands were moved there first, and this warp, which has
+    // a sixth of its scheduler's issue slots beside the unpacking ones, was what all others waited for.
+    const uint32_t idesc = idesc_bf16(128, a.N);
+    const uint64_t hi = (uint64_t)SW128_HI << 32;
+    const uint32_t xd = sw128_lo(smem_u32(sm_x)), step = x_bytes >> 4;
+    int slot = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int acc = i & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + acc, ((i >> 1) & 1) ^ 1, err, 4));
+      if (!ok) break;
+      const uint32_t d = tmem + acc * 32 * NT;
+#pragma unroll 1
+      for (int k = 0; k < a.kb; k += 2) {
+        ok = __all_sync(0xffffffffu, mbar_wait(full + slot, ph, err, 5));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t da = tmem_a + slot * 64, db = xd + 2 * slot * step;
+        if (elect_one()) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) hq_mma(d, da + j * 8, hi | (db + j * 2), idesc, k > 0 || j > 0);
           if (k + 1 < a.kb) {
-            const uint32_t d2 = db + (x_bytes >> 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) hq_mma(d, da + 32 + j * 8, hi | (d2 + j * 2), idesc, 1);
+            for (int j = 0; j < 4; ++j) hq_mma(d, da + 32 + j * 8, hi | (db + step + j * 2), idesc, 1);
           }
           umma_commit(empty + slot);
-          if (++slot == a.as) {
-            slot = 0;
-            ph ^= 1;
-          }
         }
-        if (ok) umma_commit(acc_full + acc);
+        __syncwarp();
+        if (++slot == AS) {
+          slot = 0;
+          ph ^= 1;
+        }
       }
-      umma_commit(done);
+      if (ok && elect_one()) umma_commit(acc_full + acc);
+      __syncwarp();
     }
+    if (elect_one()) umma_commit(done);
     __syncwarp();
   } else if (warp >= 4 && warp < 4 + HQ_UNPACK) {
     // Stage s holds two turns, of groups 2 s % 4 and the next one (a tile's last stage may have one turn: its second
@@ -288,8 +302,8 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
       if (ni < tiles) scales(ni, ns, next_s, next_b);
       ok = __all_sync(0xffffffffu, mbar_wait(w_full + ws, wph, err, 7));
       if (!ok) break;
-      const unsigned n = i * turns + min(k2, turns), turn = __umulhi(n, a.inv);
-      const int slot = n - turn * a.as;
+      const unsigned n = i * turns + min(k2, turns), turn = n / AS;
+      const int slot = n - turn * AS;
       if (k2 == turns) {
         ok = __all_sync(0xffffffffu, mbar_wait(empty + slot, (turn & 1) ^ 1, err, 8));
         if (!ok) break;
@@ -489,36 +503,25 @@ __global__ void __launch_bounds__(256) hq_order_kernel(const __nv_bfloat16* __re
                  __byte_perm(v.y, v.w, 0x7632));
 }
 
-// Slots and stages that fit, or false.
 static int hq_nt(int T) { return T <= 32 ? 1 : T <= 64 ? 2 : 4; }
 
-static bool hq_layout(int T, int H, HqArgs* a, size_t* smem) {
+// Sizes and the stages that fit; returns the bytes of shared memory (at most 128 tokens: 64 KB of stages and 128 of x
+// always do).
+static size_t hq_layout(int T, int H, HqArgs* a) {
   const int NT = hq_nt(T);
   a->N = (T + 15) / 16 * 16;
   a->kb = H / 64;
-  const size_t fixed = 1024 + (size_t)16 * 32 * NT * 4 + 38 * 8 + 32;
-  for (a->as = std::min(6, (512 - 64 * NT) / 64); a->as >= 4; --a->as) {
-    for (a->ws = 8; a->ws >= 4; a->ws -= 2) {
-      *smem = fixed + 2 * (size_t)a->as * hq_x_bytes(a->N) + (size_t)a->ws * HQ_W_BYTES;
-      if (*smem <= HQ_SMEM_MAX) {
-        a->inv = (unsigned)(((1ULL << 32) + a->as - 1) / a->as);
-        return true;
-      }
-    }
+  const int slots = NT == 4 ? HQ_SLOTS<4> : HQ_SLOTS<1>;
+  const size_t fixed = 1024 + (size_t)16 * 32 * NT * 4 + 38 * 8 + 32 + (size_t)2 * slots * a->N * 128;
+  for (a->ws = 8; a->ws > 4 && fixed + (size_t)a->ws * HQ_W_BYTES > HQ_SMEM_MAX; a->ws -= 2) {
   }
-  return false;
-}
-
-bool hq_takes(int T, int H) {
-  HqArgs a;
-  size_t smem;
-  return T <= HQ_MAXT && hq_layout(T, H, &a, &smem);
+  return fixed + (size_t)a->ws * HQ_W_BYTES;
 }
 
 int hq_parts(int V) { return std::min(device_sm_count(), (V + HQ_BLOCK - 1) / HQ_BLOCK); }
 
 template <int NT>
-static int hq_launch(const CUtensorMap (&m)[2], const HqArgs& a, int grid, size_t smem, cudaStream_t st) {
+static int hq_launch(const CUtensorMap (&m)[3], const HqArgs& a, int grid, size_t smem, cudaStream_t st) {
   static std::atomic<bool> done[64];
   int dev = 0;
   LG_CUDA_TRY(cudaGetDevice(&dev));
@@ -526,7 +529,7 @@ static int hq_launch(const CUtensorMap (&m)[2], const HqArgs& a, int grid, size_
     LG_CUDA_TRY(cudaFuncSetAttribute(hq_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, HQ_SMEM_MAX));
     if (dev < 64) done[dev].store(true, std::memory_order_relaxed);
   }
-  LG_CUDA_TRY(launch_early(hq_kernel<NT>, grid, HQ_THREADS, smem, st, m[0], m[1], a));
+  LG_CUDA_TRY(launch_early(hq_kernel<NT>, grid, HQ_THREADS, smem, st, m[0], m[1], m[2], a));
   LG_LAUNCH_CHECK("head_q4");
   return LG_OK;
 }
@@ -534,8 +537,7 @@ static int hq_launch(const CUtensorMap (&m)[2], const HqArgs& a, int grid, size_
 int hq_loss_parts(const __nv_bfloat16* x, long long ldx, int T, int H, const HdHead& w, int V, const int* ids,
                   int K, __nv_bfloat16* xp, int* idt, const HdParts& out, cudaStream_t st) {
   HqArgs a = {};
-  size_t smem = 0;
-  if (!hq_layout(T, H, &a, &smem)) return fail(LG_ERR_UNSUPPORTED, "head_loss: H=%d", H);
+  const size_t smem = hq_layout(T, H, &a);
   a.T = T;
   a.H = H;
   a.V = V;
@@ -550,9 +552,12 @@ int hq_loss_parts(const __nv_bfloat16* x, long long ldx, int T, int H, const HdH
   const int nt = 32 * hq_nt(T);
   hq_order_kernel<<<(std::max(n, K * nt) + 255) / 256, 256, 0, st>>>(x, ldx, n, H / 8, xp, ids, T, K, nt, idt);
   LG_LAUNCH_CHECK("head_order");
-  CUtensorMap m[2];
+  CUtensorMap m[3];
   int rc = make_map_2d(&m[0], w.w, false, H / 8, V, (uint64_t)H / 2, 32, 32, 128);
-  if (rc == LG_OK) rc = make_map_2d(&m[1], xp, true, H, T, (uint64_t)H * 2, 64, a.N, 128);
+  if (rc == LG_OK) rc = make_map_2d(&m[1], w.w, false, H / 8, V, (uint64_t)H / 2, 32, 128, 128);
+  const uint64_t dims[3] = {64, (uint64_t)T, (uint64_t)H / 64}, strides[2] = {(uint64_t)H * 2, 128};
+  const uint32_t box[3] = {64, (uint32_t)a.N, 2};
+  if (rc == LG_OK) rc = make_map_nd(&m[2], xp, 3, dims, strides, box);
   if (rc != LG_OK) return rc;
   const int grid = out.parts;
   return T <= 32 ? hq_launch<1>(m, a, grid, smem, st)
