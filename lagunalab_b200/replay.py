@@ -10,13 +10,15 @@ a reference; an engine outside this package plugs in through ``forward(ids [1, L
 logits [1, L, V]`` with ``make_cache``.
 
     python -m lagunalab_b200.replay build-ref --model PACK --traces traces --refs refs
-    python -m lagunalab_b200.replay score --model PACK --refs refs --out results/x.json
+    python -m lagunalab_b200.replay score --model PACK --refs refs --out results/x.json [--fused]
 
 Everything per position stays on the device: the session's assistant positions are one index
 tensor, each prefill chunk's hidden rows at those positions go through the head in
 sub-batches, and the log-softmax, the top-64 (``build_ref``) or the gathered KL and the
 argmax agreement (``score``) are batched reductions written into preallocated per-session
-tensors. The host sees one copy per session, not one per sub-batch.
+tensors. The host sees one copy per session, not one per sub-batch. ``score(fused=True)`` and
+``assistant_nll`` take the loss from the hidden rows without logits (``ops.head_loss``): fp32 logits
+where the head's output is rounded to bf16 otherwise, and a chunk's positions in one call.
 """
 import argparse
 import json
@@ -74,6 +76,40 @@ def assistant_logprobs(model, ids, mask, chunk=2048, make_cache=None, forward=No
     tgt = _targets(mask)
     for i, lp in _chunks(model, ids, mask, chunk, make_cache, forward):
         yield tgt[i:i + lp.shape[0]], lp
+
+
+def _hidden(model, ids, mask, chunk, make_cache):
+    """Per prefill chunk: (index of its first target in the session's list, hidden rows [n, H])."""
+    ids = np.asarray(ids)
+    tgt = _targets(mask)
+    cache = (make_cache or model.make_cache)()
+    dev = _device(model, None)
+    for a in range(0, len(ids), chunk):
+        b = min(a + chunk, len(ids))
+        lo, hi = np.searchsorted(tgt, [a, b])
+        x = torch.from_numpy(np.ascontiguousarray(ids[None, a:b], dtype=np.int32)).to(dev)
+        out = model.model(x, cache=cache)[0]
+        if hi > lo:
+            yield int(lo), out[torch.from_numpy(tgt[lo:hi] - a).to(dev)]
+
+
+def _head(model):
+    """The head as ``ops.head_loss`` takes it."""
+    h = model.lm_head
+    return h.mat if (h.bits, h.group_size) == (4, 64) else h.dequantize()
+
+
+def assistant_nll(model, ids, mask, chunk=2048, make_cache=None):
+    """(positions int64 [n] whose next token is the assistant's, -log p of that token fp32 [n] on the
+    model's device), prefilling like ``assistant_logprobs``."""
+    from . import ops
+    tgt = _targets(mask)
+    nxt = torch.from_numpy(np.asarray(ids)[tgt + 1].astype(np.int32)).to(_device(model, None))
+    nll = torch.empty(len(tgt), dtype=torch.float32, device=nxt.device)
+    head = _head(model)
+    for i, h in _hidden(model, ids, mask, chunk, make_cache):
+        nll[i:i + len(h)] = ops.head_loss(h, head, nxt[i:i + len(h)])[0]
+    return tgt, nll
 
 
 def _action(reply):
@@ -172,10 +208,13 @@ def build_ref(model, tokenizer, session_path, out_path, max_tokens=65536, n_acti
                         model=model_id or "")
 
 
-def score(model, ref_path, chunk=2048, make_cache=None, forward=None):
+def score(model, ref_path, chunk=2048, make_cache=None, forward=None, fused=False):
     """Truncated KL (over the reference's top-64) and top-1 agreement of ``model`` (or
     ``forward``) against a reference ``.npz`` (replay.py:93-114); ``peak_mem_gb`` is torch's
-    peak allocation on the current CUDA device (0 without one)."""
+    peak allocation on the current CUDA device (0 without one). ``fused`` (a model of this package on
+    the GPU): from the hidden rows, without logits."""
+    if fused and forward is not None:
+        raise ValueError("fused scoring goes by a model's head, not by forward=")
     ref = np.load(ref_path)
     ids, mask = ref["ids"], ref["mask"]
     tgt = _targets(mask)
@@ -190,7 +229,17 @@ def score(model, ref_path, chunk=2048, make_cache=None, forward=None):
     if cuda:
         torch.cuda.reset_peak_memory_stats()
     t0 = time.perf_counter()
-    for i, lp in _chunks(model, ids, mask, chunk, make_cache, forward):
+    if fused:
+        from . import ops
+        head, r_p = _head(model), r_lp.exp()
+        own = (r_p * r_lp).sum(-1)
+        r_ids = r_ids.to(torch.int32)
+        for i, h in _hidden(model, ids, mask, chunk, make_cache):
+            at = slice(i, i + len(h))
+            loss, _, top = ops.head_loss(h, head, r_ids[at], r_p[at], top=True)
+            kl[at] = loss + own[at]
+            agree[at] = top == r_ids[at, 0]
+    for i, lp in () if fused else _chunks(model, ids, mask, chunk, make_cache, forward):
         n = lp.shape[0]
         rid, rlp = r_ids[i:i + n].to(lp.device), r_lp[i:i + n].to(lp.device)
         kl[i:i + n] = (rlp.exp() * (rlp - lp.gather(-1, rid))).sum(-1).to(dev)
@@ -233,6 +282,7 @@ def main(argv=None):
     ap.add_argument("--out")
     ap.add_argument("--max-tokens", type=int, default=65536)
     ap.add_argument("--actions", action="store_true")
+    ap.add_argument("--fused", action="store_true", help="score without logits")
     a = ap.parse_args(argv)
     pack = (Path(a.model) / "layout.json").exists()
     model, tok = load_streaming(a.model, slots=0) if pack else load(a.model)
@@ -247,7 +297,7 @@ def main(argv=None):
         return
     rows = []
     for r in sorted(refs.glob("*.npz")):
-        row = {"session": r.stem, **score(model, r)}
+        row = {"session": r.stem, **score(model, r, fused=a.fused)}
         if a.actions:
             row["action_match"] = score_actions(model, tok, r)
         rows.append(row)
