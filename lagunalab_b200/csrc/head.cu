@@ -502,7 +502,6 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
                                                       unsigned char* __restrict__ order,
                                                       unsigned char* __restrict__ start,
                                                       float* __restrict__ wsum) {
-  pdl_trigger();
   __shared__ int sh[8][2 * HD_MAXK];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x * 8 + warp;
@@ -930,10 +929,10 @@ struct HdOperand {
 
 // One CTA a tile where the output has no more than 128 rows, else a pair.
 //
-// `early`: it may start under the kernel before it, one of this call's small ones that says so (pdl_trigger). Nothing
-// is launched early behind an hd_kernel: its CTAs take nearly all of an SM, and where some of its pairs are not on the
-// GPU yet (the SMs were busy with the kernel before), waiting CTAs of a later kernel can take their SMs and
-// wait for them for ever.
+// `early`: it may start under the kernel before it, one of this call's that says so (pdl_trigger) and whose CTAs have
+// room beside an hd_kernel's on an SM (no shared memory of their own). Nothing else is launched early: where a
+// kernel's CTAs are not all on the GPU yet, waiting CTAs of a later one can take their SMs and wait for them
+// for ever. (It happened behind hd_kernel, some of whose pairs had to wait for the dequantization's CTAs.)
 template <int KIND>
 static int hd_launch(const HdOperand& a, const HdOperand& b, const HdOperand& out, HdArgs g, bool early,
                      cudaStream_t st) {
@@ -1053,7 +1052,7 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
       a.v0 = v0;
       a.b_row0 = quant ? 0 : v0;
       const HdOperand mw = quant ? HdOperand{k.wq, H, n, H} : HdOperand{w, H, V, ldw};
-      HD_TRY(hd_launch<HD_LOSS>({x, H, T, ldx}, mw, {}, a, quant || (K > 1 && v0 == 0), st));
+      HD_TRY(hd_launch<HD_LOSS>({x, H, T, ldx}, mw, {}, a, quant, st));
     }
   }
   const auto join = quant ? hd_join_kernel<true> : hd_join_kernel<false>;
@@ -1100,7 +1099,7 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     a.g = g;
     a.wsum = k.wsum;
     a.ldz = (n + 63) / 64 * 64;
-    HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, {k.dz, a.ldz, T, a.ldz}, a, quant || (v0 == 0 && (dw || K > 1)), st));
+    HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, {k.dz, a.ldz, T, a.ldz}, a, quant || (v0 == 0 && dw), st));
     const HdOperand mz = {k.dz, n, T, a.ldz};
     if (dx) {
       HdArgs b = a;
