@@ -31,12 +31,16 @@ using namespace tc;
 enum { HD_LOSS = 0, HD_PROB = 1, HD_XGRAD = 2, HD_WGRAD = 3 };
 
 constexpr int HD_BM = 128, HD_BN = 256, HD_BK = 64;
-constexpr int HD_THREADS = 256;
+// Warps of the epilogue, from warp 4 on: a thread a row, and two for the halves of its 256 columns where the tile
+// leaves as boxes (one: 10,700 cycles a tile of HD_PROB, 5,400 of HD_WGRAD, when 1,024 of a contraction take
+// 8,200). HD_LOSS keeps one: each part would double what the join reads.
+constexpr int hd_epi(int kind) { return kind == 0 ? 4 : 8; }
+constexpr int hd_threads(int kind) { return 128 + 32 * hd_epi(kind); }
 constexpr int HD_A_BYTES = HD_BM * HD_BK * 2;  // 16 KB
 constexpr int HD_BOX = 64 * HD_BK * 2;  // an MN-major box: 64 K rows of 64 elements
 constexpr int HD_RING = 192 << 10;      // stages of A and B
 constexpr int HD_OUT = 4096;            // an output box: 32 rows of 128 bytes, swizzled
-constexpr size_t HD_SMEM = 1024 + HD_RING + 4 * 2 * HD_OUT + 256;
+constexpr size_t HD_SMEM = 1024 + HD_RING + 8 * HD_OUT + 256;
 
 struct HdArgs {
   int M, N;          // rows of the output tile grid, and its columns
@@ -48,7 +52,7 @@ struct HdArgs {
   int V;
   int K;             // targets a token
   const int* ids;    // [T, K]; K > 1: sorted (with `order`, `start`)
-  const float* weights;       // [T, K] or NULL, in the caller's order
+  const float* weights;        // [T, K] or NULL; K > 1: by sorted id
   const unsigned char* order;  // K > 1: [T, K] the caller's index of a sorted id
   const unsigned char* start;  // K > 1: [T, nt_all + 1] first sorted id of each vocabulary tile
   int nt_all;
@@ -96,24 +100,54 @@ __device__ __forceinline__ HdUnit hd_unit(const HdArgs& a, int i) {
   return u;
 }
 
-// One output tile's row of this thread. `ok` is false after a wait that ran out: NaN is written.
-//
+// What an epilogue thread needs of its row, loaded while the tile before is worked on.
+struct HdRow {
+  int p, p1, next;       // K > 1: sorted ids [p, p1) of the tile; the next id (K == 1: the id, of any tile)
+  float w, gs, gg, off;  // its weight; HD_PROB: g S, g, -lse log2(e)
+  bool counts;           // the token has a target
+};
+template <int KIND>
+__device__ __forceinline__ HdRow hd_row(const HdArgs& a, const HdUnit& u, int t) {
+  HdRow r = {0, 0, -1, 1.f, 0.f, 0.f, 0.f, false};
+  if (KIND > HD_PROB || t >= a.M) return r;
+  const size_t row_k = (size_t)t * a.K;
+  if (KIND == HD_PROB) {
+    r.gg = a.g[t];
+    r.off = -a.lse[t] * HD_LOG2E;
+  }
+  if (a.K == 1) {
+    r.next = a.ids[t];
+    if (KIND == HD_PROB) {
+      r.counts = r.next >= 0 && r.next < a.V;
+      r.gs = r.gg * (a.weights ? a.weights[t] : 1.f);
+    }
+  } else {
+    const unsigned char* st = a.start + (size_t)t * (a.nt_all + 1);
+    const int tile = a.v0 / HD_BN + u.n;
+    r.p = st[tile];
+    r.p1 = st[tile + 1];
+    if (KIND == HD_PROB) {
+      r.counts = st[a.nt_all] > 0;
+      r.gs = r.gg * a.wsum[t];
+    }
+    if (r.p < r.p1) {
+      r.next = a.ids[row_k + r.p];
+      if (KIND == HD_PROB) r.w = a.weights[row_k + r.p];
+    }
+  }
+  return r;
+}
+
 // Outputs leave as boxes of 32 rows x 128 bytes: a thread puts its row into shared memory, a lane stores the box by
 // TMA (HD_XGRAD: adds it to what earlier pieces left). Stored by the threads themselves, a row each, a tile of
 // dW took 8,500 cycles and dx's addition 16 us of 66.
-struct HdBox {
-  const CUtensorMap* map;
-  uint8_t* smem;  // two boxes, in turn
-  int turn;
-};
-
+//
 // This thread's 128 bytes of a box at (x, y) (and plane z), y the warp's first row; `in`: it is one of the output's.
 template <int KIND>
-__device__ __forceinline__ void hd_box(HdBox& b, const uint32_t (&r)[32], int x, int y, int z, bool add, bool in) {
+__device__ __forceinline__ void hd_box(const CUtensorMap* map, uint8_t* box, const uint32_t (&r)[32], int x, int y,
+                                       int z, bool add, bool in) {
   const int lane = threadIdx.x & 31;
-  uint8_t* box = b.smem + b.turn * HD_OUT;
-  b.turn ^= 1;
-  if (lane == 0) tma_store_wait_read<1>();  // the box's last store has read it
+  if (lane == 0) tma_store_wait_read<0>();  // the warp's last store has read the box
   __syncwarp();
 #pragma unroll
   for (int c = 0; c < 8; ++c)
@@ -123,155 +157,125 @@ __device__ __forceinline__ void hd_box(HdBox& b, const uint32_t (&r)[32], int x,
   __syncwarp();
   if (lane == 0 && in) {
     if (KIND != HD_XGRAD)
-      tma_store_2d(b.map, box, x, y);
+      tma_store_2d(map, box, x, y);
     else if (add)
-      tma_add_3d(b.map, box, x, y, z);
+      tma_add_3d(map, box, x, y, z);
     else
-      tma_store_3d(b.map, box, x, y, z);
+      tma_store_3d(map, box, x, y, z);
     tma_store_commit();
   }
   __syncwarp();  // a tcgen05.ld may follow: of the whole warp
 }
 
+// Columns [c0, c1) of one output tile's row t of this thread. `ok` is false after a wait that ran out: NaN is written.
 template <int KIND>
-__device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, int t, uint32_t taddr, bool ok,
-                                            HdBox& box) {
+__device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, int t, HdRow row, uint32_t taddr, bool ok,
+                                            const CUtensorMap* map, uint8_t* box, int begin) {
   const int n0 = u.n * HD_BN;  // in the piece (or in H)
   const bool live = t < a.M;
   const int y = t & ~31;
   const float nan = __int_as_float(0x7fffffff);
+  constexpr int COLS = HD_BN / (hd_epi(KIND) / 4);
   float v[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = nan;
-  if (KIND == HD_LOSS || KIND == HD_PROB) {
+  if (KIND == HD_LOSS) {
     const int ntile = a.v0 / HD_BN + u.n;
-    const int c0 = a.v0 + n0;  // the tile's first vocabulary id
     const size_t row_k = (size_t)t * a.K;
-    int p = 0, p1 = 0, next = -1;  // K > 1: sorted ids [p, p1) of this tile; `next`: the next id
-    if (live) {
-      if (a.K == 1) {
-        next = a.ids[t];
-      } else {
-        const unsigned char* st = a.start + (size_t)t * (a.nt_all + 1) + ntile;
-        p = st[0];
-        p1 = st[1];
-        next = p < p1 ? a.ids[row_k + p] : -1;
-      }
-    }
-    if (KIND == HD_LOSS) {
-      float mx = -INFINITY, sum = 0.f;
-      int arg = 0;
+    float mx = -INFINITY, sum = 0.f;
+    int arg = 0;
 #pragma unroll 1
-      for (int c = 0; c < HD_BN; c += 32) {
-        const int id0 = c0 + c;
-        if (id0 >= a.V) break;
-        __syncwarp();
-        if (ok) tmem_ld32_wait(taddr + c, v);
-        if (id0 + 32 > a.V) {
+    for (int c = 0; c < COLS; c += 32) {
+      const int id0 = a.v0 + n0 + c;  // vocabulary ids
+      if (id0 >= a.V) break;
+      __syncwarp();
+      if (ok) tmem_ld32_wait(taddr + c, v);
+      if (id0 + 32 > a.V) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = id0 + i < a.V ? v[i] : -INFINITY;
-        }
-        while ((unsigned)next - (unsigned)id0 < 32u) {
-          const float z = hd_pick(v, next - id0);
-          if (a.K == 1) {
-            a.out.ztgt[t] = z;
-            break;
-          }
-          a.out.ztgt[row_k + a.order[row_k + p]] = z;
-          next = ++p < p1 ? a.ids[row_k + p] : -1;
-        }
-        float cm = v[0];
-#pragma unroll
-        for (int i = 1; i < 32; ++i) cm = fmaxf(cm, v[i]);
-        if (cm > mx) {
-          if (a.out.top) {
-            int at = 0;
-#pragma unroll
-            for (int i = 31; i >= 0; --i) at = v[i] == cm ? i : at;
-            arg = id0 + at;
-          }
-          sum *= hd_ex2((mx - cm) * HD_LOG2E);  // mx = -inf: sum is 0
-          mx = cm;
-        }
-        const float off = mx == -INFINITY ? 0.f : -mx * HD_LOG2E;
-        float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          s0 += hd_ex2(fmaf(v[i], HD_LOG2E, off));
-          s1 += hd_ex2(fmaf(v[i + 1], HD_LOG2E, off));
-        }
-        sum += s0 + s1;
+        for (int i = 0; i < 32; ++i) v[i] = id0 + i < a.V ? v[i] : -INFINITY;
       }
-      if (live) {
-        a.out.part[(size_t)t * a.nt_all + ntile] = make_float2(mx, ok ? sum : nan);
-        if (a.out.top) a.out.top[(size_t)t * a.nt_all + ntile] = arg;
-      }
-    } else {
-      float gs = 0.f, gg = 0.f, off = 0.f;
-      bool counts = false;
-      if (live) {
-        gg = a.g[t];
-        off = -a.lse[t] * HD_LOG2E;
+      while ((unsigned)row.next - (unsigned)id0 < 32u) {
+        const float z = hd_pick(v, row.next - id0);
         if (a.K == 1) {
-          counts = next >= 0 && next < a.V;
-          gs = gg * (a.weights ? a.weights[t] : 1.f);
-        } else {
-          counts = a.start[(size_t)t * (a.nt_all + 1) + a.nt_all] > 0;
-          gs = gg * a.wsum[t];
+          a.out.ztgt[t] = z;
+          break;
         }
+        a.out.ztgt[row_k + a.order[row_k + row.p]] = z;
+        row.next = ++row.p < row.p1 ? a.ids[row_k + row.p] : -1;
       }
-#pragma unroll 1
-      for (int c = 0; c < HD_BN && n0 + c < a.ldz; c += 64) {
-        uint32_t r[32];
+      float cm = v[0];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int id0 = c0 + c + 32 * h;
-          __syncwarp();
-          if (ok) tmem_ld32_wait(taddr + c + 32 * h, v);
+      for (int i = 1; i < 32; ++i) cm = fmaxf(cm, v[i]);
+      if (cm > mx) {
+        if (a.out.top) {
+          int at = 0;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = ok ? gs * hd_ex2(fmaf(v[i], HD_LOG2E, off)) : nan;
-          while ((unsigned)next - (unsigned)id0 < 32u) {
-            if (a.K == 1) {
-              hd_sub(v, next - id0, gs);
-              break;
-            }
-            const float w = a.weights ? a.weights[row_k + a.order[row_k + p]] : 1.f;
-            hd_sub(v, next - id0, gg * w);
-            next = ++p < p1 ? a.ids[row_k + p] : -1;
-          }
-          if (!counts) {  // a token without a target: nothing of it, whatever its row holds
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.f;
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) r[16 * h + i] = hd_pack(v[2 * i], v[2 * i + 1]);
+          for (int i = 31; i >= 0; --i) at = v[i] == cm ? i : at;
+          arg = id0 + at;
         }
-        __syncwarp();
-        hd_box<KIND>(box, r, n0 + c, y, 0, false, y < a.M);
+        sum *= hd_ex2((mx - cm) * HD_LOG2E);  // mx = -inf: sum is 0
+        mx = cm;
       }
+      const float off = mx == -INFINITY ? 0.f : -mx * HD_LOG2E;
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        s0 += hd_ex2(fmaf(v[i], HD_LOG2E, off));
+        s1 += hd_ex2(fmaf(v[i + 1], HD_LOG2E, off));
+      }
+      sum += s0 + s1;
+    }
+    if (live) {
+      a.out.part[(size_t)t * a.nt_all + ntile] = make_float2(mx, ok ? sum : nan);
+      if (a.out.top) a.out.top[(size_t)t * a.nt_all + ntile] = arg;
     }
   } else if (KIND == HD_XGRAD) {
 #pragma unroll 1
-    for (int c = 0; c < HD_BN && n0 + c < a.N; c += 32) {
+    for (int c = begin; c < begin + COLS && n0 + c < a.N; c += 32) {
       __syncwarp();
       if (ok) tmem_ld32_wait(taddr + c, v);
       uint32_t r[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
-      hd_box<KIND>(box, r, n0 + c, y, u.split, a.add, y < a.M);
+      hd_box<KIND>(map, box, r, n0 + c, y, u.split, a.add, y < a.M);
     }
   } else {
+    const int width = KIND == HD_PROB ? a.ldz : a.N;
 #pragma unroll 1
-    for (int c = 0; c < HD_BN && n0 + c < a.N; c += 64) {
+    for (int c = begin; c < begin + COLS && n0 + c < width; c += 64) {
       uint32_t r[32];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         __syncwarp();
         if (ok) tmem_ld32_wait(taddr + c + 32 * h, v);
+        if (KIND == HD_PROB) {
+          const int id0 = a.v0 + n0 + c + 32 * h;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = ok ? row.gs * hd_ex2(fmaf(v[i], HD_LOG2E, row.off)) : nan;
+          // K > 1: of the tile's ids in order, those of the other half of the columns only pass by
+          while (a.K > 1 ? row.next >= 0 && row.next < id0 + 32 : (unsigned)row.next - (unsigned)id0 < 32u) {
+            if (a.K == 1) {
+              hd_sub(v, row.next - id0, row.gs);
+              break;
+            }
+            if (row.next >= id0) hd_sub(v, row.next - id0, row.gg * row.w);
+            const size_t at = (size_t)t * a.K + ++row.p;
+            row.next = -1;
+            if (row.p < row.p1) {
+              row.next = a.ids[at];
+              row.w = a.weights[at];
+            }
+          }
+          if (!row.counts) {  // a token without a target: nothing of it, whatever its row holds
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) r[16 * h + i] = hd_pack(v[2 * i], v[2 * i + 1]);
       }
-      hd_box<KIND>(box, r, n0 + c, a.v0 + y, 0, false, y < a.M);
+      __syncwarp();
+      hd_box<KIND>(map, box, r, n0 + c, KIND == HD_PROB ? y : a.v0 + y, 0, false, y < a.M);
     }
   }
 }
@@ -279,13 +283,13 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
 // D[M, N] = A B^T over tiles of 128 CG x 256. A and B are K-major ([rows, contraction]) or MN-major
 // ([contraction, rows]): HD_LOSS, HD_PROB: x and W, both K-major; HD_XGRAD: dz K-major, W MN-major;
 // HD_WGRAD: dz and x, both MN-major. Warp 0: TMA; warp 1: products into one of two TMEM tiles;
-// warps 4 to 7: the finished tile's rows, one a thread, while the next one's products run.
+// warps 4 to 7 (11): the finished tile's rows, one a thread, while the next one's products run.
 //
 // CG = 2: a pair of CTAs shares a tile, each loads its 128 rows of A and half of B, and the leader issues for
 // both. Per 64 of the contraction an SM then loads 32 KB instead of 48 in 512 cycles of products: one CTA alone
 // waits for L2 (60 bytes a cycle; 204 cycles a product instead of 128).
 template <int KIND, int CG>
-__global__ void __launch_bounds__(HD_THREADS, 1)
+__global__ void __launch_bounds__(hd_threads(KIND), 1)
     hd_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
               const __grid_constant__ CUtensorMap mo, const HdArgs a) {
   constexpr bool A_MN = KIND == HD_WGRAD, B_MN = KIND == HD_XGRAD || KIND == HD_WGRAD;
@@ -294,7 +298,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
   constexpr int STAGES = HD_RING / STAGE;
   extern __shared__ uint8_t hd_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)hd_smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + HD_RING + 4 * 2 * HD_OUT);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + HD_RING + 8 * HD_OUT);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;  // [2]
   uint64_t* acc_empty = acc_full + 2;   // [2]
@@ -312,7 +316,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + i, 1);
-      mbar_init(acc_empty + i, 4 * CG);
+      mbar_init(acc_empty + i, hd_epi(KIND) * CG);
     }
     mbar_init(done, 1);
     err[0] = err[1] = err[2] = 0;  // of all roles; of the copies' end; of the products' end
@@ -438,17 +442,23 @@ __global__ void __launch_bounds__(HD_THREADS, 1)
     }
     __syncwarp();
   } else if (warp >= 4) {
-    const int q = warp & 3;
-    HdBox box = {&mo, smem + HD_RING + q * 2 * HD_OUT, 0};
+    const int q = warp & 3, begin = warp < 8 ? 0 : HD_BN / 2;
+    uint8_t* box = smem + HD_RING + (warp - 4) * HD_OUT;
     bool ok = true;
     int n = 0;
+    const auto row_of = [&](const HdUnit& u) { return (u.m * CG + rank) * HD_BM + q * 32 + lane; };
+    HdUnit u = hd_unit<KIND>(a, first);
+    HdRow row = first < units ? hd_row<KIND>(a, u, row_of(u)) : HdRow{};
     for (int i = first; i < units; i += step, ++n) {
-      const HdUnit u = hd_unit<KIND>(a, i);
+      const HdUnit un = hd_unit<KIND>(a, i + step);
+      HdRow next = {};
+      if (i + step < units) next = hd_row<KIND>(a, un, row_of(un));
       const int acc = n & 1;
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + acc, (n >> 1) & 1, err, 5));
       tc_fence_after();
-      hd_epilogue<KIND>(a, u, (u.m * CG + rank) * HD_BM + q * 32 + lane,
-                        tmem + acc * HD_BN + ((uint32_t)(q * 32) << 16), ok, box);
+      hd_epilogue<KIND>(a, u, row_of(u), row, tmem + acc * HD_BN + ((uint32_t)(q * 32) << 16), ok, &mo, box, begin);
+      u = un;
+      row = next;
       tc_fence_before();
       __syncwarp();
       if (ok && lane == 0) {
@@ -494,12 +504,13 @@ __device__ __forceinline__ void hd_unpack(uint32_t q, uint16_t scale, uint16_t b
 
 // ---- small kernels ------------------------------------------------------------------------------
 
-// K > 1: a warp sorts a token's ids (those in [0, V), ascending, equal ones in their order), with each
-// one's place in the caller's list, the first of each vocabulary tile, and the weights' sum.
+// K > 1: a warp sorts a token's ids (those in [0, V), ascending, equal ones in their order) with each one's
+// weight and place in the caller's list, the first of each vocabulary tile, and the weights' sum.
 __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ ids,
                                                       const float* __restrict__ weights, int T, int K,
                                                       int V, int nt, int* __restrict__ sorted,
                                                       unsigned char* __restrict__ order,
+                                                      float* __restrict__ sorted_w,
                                                       unsigned char* __restrict__ start,
                                                       float* __restrict__ wsum) {
   __shared__ int sh[8][2 * HD_MAXK];
@@ -528,6 +539,7 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
     up[rank] = id;
     sorted[(size_t)t * K + rank] = id;
     order[(size_t)t * K + rank] = (unsigned char)j;
+    sorted_w[(size_t)t * K + rank] = weights ? weights[(size_t)t * K + j] : 1.f;
   }
   __syncwarp();
   for (int n = lane; n <= nt; n += 32) {  // ids below the tile's first; n = nt: all that count
@@ -833,7 +845,7 @@ struct HdWork {
   int* idt;
   int* sorted;
   unsigned char *order, *start;
-  float* wsum;
+  float *sorted_w, *wsum;
   __nv_bfloat16 *wq, *dz, *xz;
   float* dx;
   size_t bytes;
@@ -861,6 +873,7 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
   if (K > 1) {
     w.sorted = c.take<int>((size_t)T * K);
     w.order = c.take<unsigned char>((size_t)T * K);
+    w.sorted_w = c.take<float>((size_t)T * K);
     w.start = c.take<unsigned char>((size_t)T * (w.nt + 1));
     w.wsum = c.take<float>(T);
   }
@@ -897,7 +910,7 @@ static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const CUte
   const long long units = (long long)a.mt * a.nt * a.splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = CG * (int)std::max(1LL, std::min<long long>(units, device_sm_count() / CG));
-  cfg.blockDim = HD_THREADS;
+  cfg.blockDim = hd_threads(KIND);
   cfg.dynamicSmemBytes = HD_SMEM;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
@@ -988,7 +1001,7 @@ static int hd_weights(const void* w, const void* ws, const void* wb, int H, int 
 static int hd_sort(const int* ids, const float* weights, int T, int K, int V, const HdWork& k,
                    cudaStream_t st) {
   if (K == 1) return LG_OK;
-  hd_sort_kernel<<<(T + 7) / 8, 256, 0, st>>>(ids, weights, T, K, V, k.nt, k.sorted, k.order, k.start, k.wsum);
+  hd_sort_kernel<<<(T + 7) / 8, 256, 0, st>>>(ids, weights, T, K, V, k.nt, k.sorted, k.order, k.sorted_w, k.start, k.wsum);
   LG_LAUNCH_CHECK("head_sort");
   return LG_OK;
 }
@@ -998,7 +1011,7 @@ static HdArgs hd_args(int T, int V, int K, const int* ids, const float* weights,
   a.V = V;
   a.K = K;
   a.ids = K > 1 ? k.sorted : ids;
-  a.weights = weights;
+  a.weights = K > 1 ? k.sorted_w : weights;
   a.order = k.order;
   a.start = k.start;
   a.nt_all = k.nt;
