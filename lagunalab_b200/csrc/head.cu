@@ -62,9 +62,10 @@ struct HdArgs {
   const float* lse;
   const float* g;
   const float* wsum;  // K > 1: [T]
-  int ldz;            // columns of dz [T, ldz]
-  // HD_XGRAD
-  int add;  // 0: the first piece
+  // not HD_LOSS: bf16 [M, width], HD_XGRAD: fp32 [splits, M, width]
+  void* tile_out;
+  int width;
+  int add;  // HD_XGRAD: 0 for the first piece
 };
 
 __device__ __forceinline__ void hd_sub(float (&v)[32], int c, float w) {
@@ -86,17 +87,21 @@ template <int KIND>
 __device__ __forceinline__ HdUnit hd_unit(const HdArgs& a, int i) {
   HdUnit u;
   if (KIND == HD_LOSS || KIND == HD_PROB) {  // tokens inner: a tile of W serves all of them from L2
-    u.m = i % a.mt;
-    u.n = i / a.mt;
+    u.n = (unsigned)i / (unsigned)a.mt;
+    u.m = i - u.n * a.mt;
     u.split = 0;
   } else {
-    u.n = i % a.nt;
-    const int r = i / a.nt;
-    u.m = r % a.mt;
-    u.split = r / a.mt;
+    const unsigned r = (unsigned)i / (unsigned)a.nt;
+    u.n = i - r * a.nt;
+    u.split = KIND == HD_XGRAD ? r / (unsigned)a.mt : 0;
+    u.m = r - u.split * a.mt;
   }
-  u.k0 = (int)((long long)a.kblocks * u.split / a.splits);
-  u.k1 = (int)((long long)a.kblocks * (u.split + 1) / a.splits);
+  u.k0 = 0;
+  u.k1 = a.kblocks;
+  if (KIND == HD_XGRAD && a.splits > 1) {  // at most 2^24 blocks of a piece's ids times 148 parts
+    u.k0 = (unsigned)a.kblocks * u.split / (unsigned)a.splits;
+    u.k1 = (unsigned)a.kblocks * (u.split + 1) / (unsigned)a.splits;
+  }
   return u;
 }
 
@@ -138,39 +143,45 @@ __device__ __forceinline__ HdRow hd_row(const HdArgs& a, const HdUnit& u, int t)
   return r;
 }
 
-// Outputs leave as boxes of 32 rows x 128 bytes: a thread puts its row into shared memory, a lane stores the box by
-// TMA (HD_XGRAD: adds it to what earlier pieces left). Stored by the threads themselves, a row each, a tile of
-// dW took 8,500 cycles and dx's addition 16 us of 66.
+// Outputs leave as boxes of 32 rows x 128 bytes: a thread puts its row into shared memory, and the warp stores four
+// whole rows of the box at a time (HD_XGRAD: adds them to what earlier pieces left). Stored by the threads themselves,
+// a row each, a tile of dW took 8,500 cycles and dx's addition 16 us of 66; stored by TMA, a box waits for
+// 2,000 to 5,000 cycles behind the loads that are queued there.
 //
-// This thread's 128 bytes of a box at (x, y) (and plane z), y the warp's first row; `in`: it is one of the output's.
+// This thread's 128 bytes of a box: rows y ... of the output's `rows`, from its column x (of a.width) on.
 template <int KIND>
-__device__ __forceinline__ void hd_box(const CUtensorMap* map, uint8_t* box, const uint32_t (&r)[32], int x, int y,
-                                       int z, bool add, bool in) {
+__device__ __forceinline__ void hd_box(const HdArgs& a, uint8_t* box, const uint32_t (&r)[32], int x, int y, int split) {
+  constexpr int PER = KIND == HD_XGRAD ? 4 : 8;  // elements in 16 bytes
   const int lane = threadIdx.x & 31;
-  if (lane == 0) tma_store_wait_read<0>();  // the warp's last store has read the box
-  __syncwarp();
 #pragma unroll
   for (int c = 0; c < 8; ++c)
     *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) =
         make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
-  fence_proxy_async_smem();
   __syncwarp();
-  if (lane == 0 && in) {
-    if (KIND != HD_XGRAD)
-      tma_store_2d(map, box, x, y);
-    else if (add)
-      tma_add_3d(map, box, x, y, z);
-    else
-      tma_store_3d(map, box, x, y, z);
-    tma_store_commit();
+  const int chunk = lane & 7, col = x + chunk * PER;
+  const bool in = col < a.width;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = 4 * i + (lane >> 3);
+    const uint4 v = *reinterpret_cast<const uint4*>(box + row * 128 + ((chunk ^ (row & 7)) << 4));
+    if (!in || y + row >= a.M) continue;
+    if (KIND == HD_XGRAD) {
+      float* out = static_cast<float*>(a.tile_out) + ((size_t)split * a.M + y + row) * a.width + col;
+      if (a.add)
+        red_add_v4_f32(out, __uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+      else
+        *reinterpret_cast<uint4*>(out) = v;
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.tile_out) + (size_t)(y + row) * a.width + col) = v;
+    }
   }
-  __syncwarp();  // a tcgen05.ld may follow: of the whole warp
+  __syncwarp();  // the box is free, and a tcgen05.ld of the whole warp may follow
 }
 
 // Columns [c0, c1) of one output tile's row t of this thread. `ok` is false after a wait that ran out: NaN is written.
 template <int KIND>
 __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, int t, HdRow row, uint32_t taddr, bool ok,
-                                            const CUtensorMap* map, uint8_t* box, int begin) {
+                                            uint8_t* box, int begin) {
   const int n0 = u.n * HD_BN;  // in the piece (or in H)
   const bool live = t < a.M;
   const int y = t & ~31;
@@ -231,18 +242,17 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
     }
   } else if (KIND == HD_XGRAD) {
 #pragma unroll 1
-    for (int c = begin; c < begin + COLS && n0 + c < a.N; c += 32) {
+    for (int c = begin; c < begin + COLS && n0 + c < a.width; c += 32) {
       __syncwarp();
       if (ok) tmem_ld32_wait(taddr + c, v);
       uint32_t r[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
-      hd_box<KIND>(map, box, r, n0 + c, y, u.split, a.add, y < a.M);
+      hd_box<KIND>(a, box, r, n0 + c, y, u.split);
     }
   } else {
-    const int width = KIND == HD_PROB ? a.ldz : a.N;
 #pragma unroll 1
-    for (int c = begin; c < begin + COLS && n0 + c < width; c += 64) {
+    for (int c = begin; c < begin + COLS && n0 + c < a.width; c += 64) {
       uint32_t r[32];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -275,7 +285,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
         for (int i = 0; i < 16; ++i) r[16 * h + i] = hd_pack(v[2 * i], v[2 * i + 1]);
       }
       __syncwarp();
-      hd_box<KIND>(map, box, r, n0 + c, KIND == HD_PROB ? y : a.v0 + y, 0, false, y < a.M);
+      hd_box<KIND>(a, box, r, n0 + c, y, 0);
     }
   }
 }
@@ -291,7 +301,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
 template <int KIND, int CG>
 __global__ void __launch_bounds__(hd_threads(KIND), 1)
     hd_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb,
-              const __grid_constant__ CUtensorMap mo, const HdArgs a) {
+              const HdArgs a) {
   constexpr bool A_MN = KIND == HD_WGRAD, B_MN = KIND == HD_XGRAD || KIND == HD_WGRAD;
   constexpr int B_ROWS = HD_BN / CG;  // of B in this CTA
   constexpr int STAGE = HD_A_BYTES + B_ROWS * HD_BK * 2;
@@ -456,7 +466,7 @@ __global__ void __launch_bounds__(hd_threads(KIND), 1)
       const int acc = n & 1;
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + acc, (n >> 1) & 1, err, 5));
       tc_fence_after();
-      hd_epilogue<KIND>(a, u, row_of(u), row, tmem + acc * HD_BN + ((uint32_t)(q * 32) << 16), ok, &mo, box, begin);
+      hd_epilogue<KIND>(a, u, row_of(u), row, tmem + acc * HD_BN + ((uint32_t)(q * 32) << 16), ok, box, begin);
       u = un;
       row = next;
       tc_fence_before();
@@ -468,8 +478,6 @@ __global__ void __launch_bounds__(hd_threads(KIND), 1)
           mbar_arrive(acc_empty + acc);
       }
     }
-    if (KIND != HD_LOSS && lane == 0) tma_store_wait();
-    __syncwarp();
   }
   // The products have ended before their TMEM goes.
   if (warp == 2) {
@@ -897,8 +905,8 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
   } while (0)
 
 template <int KIND, int CG>
-static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const HdArgs& a,
-                        bool early, cudaStream_t st) {
+static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const HdArgs& a, bool early,
+                        cudaStream_t st) {
   static std::atomic<bool> done[64];
   int dev = 0;
   LG_CUDA_TRY(cudaGetDevice(&dev));
@@ -928,13 +936,12 @@ static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const CUte
   }
   cfg.attrs = at;
   cfg.numAttrs = n;
-  LG_CUDA_TRY(cudaLaunchKernelEx(&cfg, hd_kernel<KIND, CG>, ma, mb, mo, a));
+  LG_CUDA_TRY(cudaLaunchKernelEx(&cfg, hd_kernel<KIND, CG>, ma, mb, a));
   LG_LAUNCH_CHECK("head");
   return LG_OK;
 }
 
-// Operands of a product: [contraction, rows] (mn) or [rows, contraction] matrices of bf16; its output alike (dx:
-// fp32, `ld` matrices of it).
+// Operands of a product: [contraction, rows] (mn) or [rows, contraction] matrices of bf16.
 struct HdOperand {
   const void* p;
   long long inner, rows, ld;
@@ -947,22 +954,15 @@ struct HdOperand {
 // kernel's CTAs are not all on the GPU yet, waiting CTAs of a later one can take their SMs and wait for them
 // for ever. (It happened behind hd_kernel, some of whose pairs had to wait for the dequantization's CTAs.)
 template <int KIND>
-static int hd_launch(const HdOperand& a, const HdOperand& b, const HdOperand& out, HdArgs g, bool early,
-                     cudaStream_t st) {
+static int hd_launch(const HdOperand& a, const HdOperand& b, HdArgs g, bool early, cudaStream_t st) {
   constexpr bool A_MN = KIND == HD_WGRAD, B_MN = KIND == HD_XGRAD || KIND == HD_WGRAD;
   const int cg = hd_cg(g.M);
   g.mt = (g.M + HD_BM * cg - 1) / (HD_BM * cg);
   g.nt = (g.N + HD_BN - 1) / HD_BN;
-  CUtensorMap ma, mb, mo;
+  CUtensorMap ma, mb;
   HD_TRY(make_map_2d(&ma, a.p, true, a.inner, a.rows, (uint64_t)a.ld * 2, 64, A_MN ? HD_BK : HD_BM, 128));
   HD_TRY(make_map_2d(&mb, b.p, true, b.inner, b.rows, (uint64_t)b.ld * 2, 64, B_MN ? HD_BK : HD_BN / cg, 128));
-  if (KIND == HD_LOSS)
-    mo = ma;  // none
-  else if (KIND == HD_XGRAD)
-    HD_TRY(make_map_f32_planes(&mo, out.p, out.inner, out.rows, out.ld, 32));
-  else
-    HD_TRY(make_map_2d(&mo, out.p, true, out.inner, out.rows, (uint64_t)out.ld * 2, 64, 32, 128));
-  return cg == 2 ? hd_launch_as<KIND, 2>(ma, mb, mo, g, early, st) : hd_launch_as<KIND, 1>(ma, mb, mo, g, early, st);
+  return cg == 2 ? hd_launch_as<KIND, 2>(ma, mb, g, early, st) : hd_launch_as<KIND, 1>(ma, mb, g, early, st);
 }
 
 static int hd_check(const char* who, const void* x, long long ldx, int T, int H, const void* w,
@@ -1065,7 +1065,7 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
       a.v0 = v0;
       a.b_row0 = quant ? 0 : v0;
       const HdOperand mw = quant ? HdOperand{k.wq, H, n, H} : HdOperand{w, H, V, ldw};
-      HD_TRY(hd_launch<HD_LOSS>({x, H, T, ldx}, mw, {}, a, quant, st));
+      HD_TRY(hd_launch<HD_LOSS>({x, H, T, ldx}, mw, a, quant, st));
     }
   }
   const auto join = quant ? hd_join_kernel<true> : hd_join_kernel<false>;
@@ -1111,23 +1111,29 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     a.lse = lse;
     a.g = g;
     a.wsum = k.wsum;
-    a.ldz = (n + 63) / 64 * 64;
-    HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, {k.dz, a.ldz, T, a.ldz}, a, quant || (v0 == 0 && dw), st));
-    const HdOperand mz = {k.dz, n, T, a.ldz};
+    const int ldz = (n + 63) / 64 * 64;
+    a.tile_out = k.dz;
+    a.width = ldz;
+    HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, a, quant || (v0 == 0 && dw), st));
+    const HdOperand mz = {k.dz, n, T, ldz};
     if (dx) {
       HdArgs b = a;
       b.N = H;
       b.kblocks = (n + HD_BK - 1) / HD_BK;
       b.splits = std::min(k.splits, b.kblocks);
       b.add = v0 > 0;
-      HD_TRY(hd_launch<HD_XGRAD>(mz, mw, {k.dx, H, T, k.splits}, b, false, st));
+      b.tile_out = k.dx;
+      b.width = H;
+      HD_TRY(hd_launch<HD_XGRAD>(mz, mw, b, false, st));
     }
     if (dw) {
       HdArgs b = a;
       b.M = n;
       b.N = H;
       b.kblocks = (T + HD_BK - 1) / HD_BK;
-      HD_TRY(hd_launch<HD_WGRAD>(mz, {k.xz, H, T, H}, {dw, H, V, H}, b, false, st));
+      b.tile_out = static_cast<__nv_bfloat16*>(dw) + (size_t)v0 * H;
+      b.width = H;
+      HD_TRY(hd_launch<HD_WGRAD>(mz, {k.xz, H, T, H}, b, false, st));
     }
   }
   if (dx) {

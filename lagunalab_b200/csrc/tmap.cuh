@@ -65,19 +65,4 @@ inline int make_map_nd(CUtensorMap* m, const void* base, int n, const uint64_t* 
   return LG_OK;
 }
 
-// fp32 map of `planes` row-major matrices [rows, inner], one behind the other; box of 32 x box_rows, 128-byte swizzle.
-inline int make_map_f32_planes(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t planes,
-                               uint32_t box_rows) {
-  auto fn = tmap_encode_fn();
-  if (!fn) return fail(LG_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-  cuuint64_t dims[3] = {inner, rows, planes};
-  cuuint64_t strides[2] = {inner * 4, inner * rows * 4};
-  cuuint32_t box[3] = {32, box_rows, 1}, estr[3] = {1, 1, 1};
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(LG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return LG_OK;
-}
-
 }  // namespace lg
