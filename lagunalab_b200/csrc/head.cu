@@ -472,10 +472,9 @@ __global__ void __launch_bounds__(hd_threads(KIND), 1)
       tc_fence_before();
       __syncwarp();
       if (ok && lane == 0) {
-        if (CG == 2)
-          mbar_arrive_cluster(mapa(acc_empty + acc, 0));
-        else
-          mbar_arrive(acc_empty + acc);
+        // The tile has been read (each tcgen05.ld waited for); what was stored meanwhile is nobody's here. (Arriving
+        // before the last box is stored gains nothing.)
+        mbar_arrive_cluster_relaxed(mapa(acc_empty + acc, 0));
       }
     }
   }
