@@ -932,10 +932,12 @@ def _head_args(who, x, head, ids, weights):
     lg_head_loss and lg_head_loss_grad, what they point to)."""
     _dev(x)
     index = x.get_device()
-    if x.dim() != 2 or x.dtype is not _BF16:
+    if x.dtype is not _BF16 or x.dim() != 2:
         raise ValueError(f"{who}: x must be bf16 [T, H]")
     T, H = x.shape
     x, ldx = _rows16(x)
+    sp = bp = wp = None
+    bits = 16
     if isinstance(head, tuple):
         q, s, b = head
         for m in head:
@@ -948,25 +950,21 @@ def _head_args(who, x, head, ids, weights):
                 s.dtype is not _BF16 or b.dtype is not _BF16:
             raise ValueError(f"{who}: a 4-bit group-64 head of {H} columns is int32 words [V, {H // 8}], "
                              f"bf16 scales and biases [V, {H // 64}]")
-        q, s, b = q.contiguous(), s.contiguous(), b.contiguous()
-        if q.data_ptr() % 16:
-            q = q.clone()
-        keep, bits = (q, s, b), 4
-        w, ldw, sp, bp = q.data_ptr(), H, s.data_ptr(), b.data_ptr()
+        if s.get_device() != index or b.get_device() != index:
+            raise ValueError(f"{who}: the head is not on {x.device}")
+        w, s, b, ldw, bits = q.contiguous(), s.contiguous(), b.contiguous(), H, 4
+        if w.data_ptr() % 16:
+            w = w.clone()
+        sp, bp, keep = s.data_ptr(), b.data_ptr(), (s, b)
     else:
         _dev(head)
         if head.dim() != 2 or head.dtype is not _BF16 or head.shape[1] != H or H % 8:
             raise ValueError(f"{who}: a head is bf16 [V, {H}] (a multiple of 8) or a 4-bit "
                              "(words, scales, biases)")
-        V = head.shape[0]
-        head, ldw = _rows16(head)
-        keep, bits = (head,), 16
-        w, sp, bp = head.data_ptr(), None, None
-    if V < 1:
-        raise ValueError(f"{who}: the head has no rows")
-    for m in keep:
-        if m.get_device() != index:
-            raise ValueError(f"{who}: the head is not on {x.device}")
+        V, keep = head.shape[0], None
+        w, ldw = _rows16(head)
+    if V < 1 or w.get_device() != index:
+        raise ValueError(f"{who}: the head has no rows, or is not on {x.device}")
     _dev(ids)
     shape = ids.shape
     if ids.dtype is not _I32 or len(shape) not in (1, 2) or shape[0] != T or ids.get_device() != index:
@@ -976,7 +974,6 @@ def _head_args(who, x, head, ids, weights):
         raise ValueError(f"{who}: {K} targets a token, not 1 to {HEAD_TARGETS}")
     if not ids.is_contiguous():
         ids = ids.contiguous()
-    wp = None
     if weights is not None:
         _dev(weights)
         if weights.dtype is not torch.float32 or weights.shape != shape or weights.get_device() != index:
@@ -984,8 +981,8 @@ def _head_args(who, x, head, ids, weights):
         if not weights.is_contiguous():
             weights = weights.contiguous()
         wp = weights.data_ptr()
-    args = (x.data_ptr(), ldx, T, H, w, ldw, sp, bp, V, ids.data_ptr(), wp, K)
-    return index, (T, H, V, K, bits), args, (x, keep, ids, weights)
+    return index, (T, H, V, K, bits), (x.data_ptr(), ldx, T, H, w.data_ptr(), ldw, sp, bp, V, ids.data_ptr(),
+                                       wp, K), (x, w, keep, ids, weights)
 
 
 @functools.lru_cache(maxsize=256)
@@ -1008,13 +1005,13 @@ def head_loss(x, head, ids, weights=None, top=False):
     >= V has loss NaN. Returns (loss, lse) fp32 [T], with ``top`` also the id of each token's
     largest logit, int32 [T]. Logits and sums are fp32."""
     index, sizes, args, keep = _head_args("head_loss", x, head, ids, weights)
-    dev, T = x.device, sizes[0]
-    loss = torch.empty(T, dtype=torch.float32, device=dev)
+    T = sizes[0]
+    loss = torch.empty(T, dtype=torch.float32, device=x.device)
     lse = torch.empty_like(loss)
-    ti = torch.empty(T, dtype=_I32, device=dev) if top else None
+    ti = torch.empty(T, dtype=_I32, device=x.device) if top else None
     if T:
         nb = _on_index(index, "lg_head_loss_workspace_bytes", *sizes, int(bool(top)))
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev)  # of this call alone
+        ws = loss.new_empty(nb // 4)  # of this call alone
         _call_on(index, _lib.lib().lg_head_loss, *args, loss.data_ptr(), lse.data_ptr(), _p(ti),
                  ws.data_ptr(), nb)
     return (loss, lse, ti) if top else (loss, lse)
@@ -1038,10 +1035,10 @@ def head_loss_grad(x, head, ids, lse, g, weights=None, dx=True, dw=True):
         if t.dtype is not torch.float32 or t.shape != (T,) or t.get_device() != index:
             raise ValueError(f"head_loss_grad: {name} must be fp32 [{T}] on {x.device}")
     lse, g = lse.contiguous(), g.contiguous()
-    gx = torch.empty(T, H, dtype=_BF16, device=x.device) if dx else None
-    gw = torch.empty(V, H, dtype=_BF16, device=x.device) if dw else None
+    gx = x.new_empty(T, H) if dx else None
+    gw = x.new_empty(V, H) if dw else None
     nb = _on_index(index, "lg_head_loss_grad_workspace_bytes", *sizes, int(bool(dx)), int(bool(dw)))
-    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    ws = lse.new_empty(nb // 4)  # of this call alone
     _call_on(index, _lib.lib().lg_head_loss_grad, *args, lse.data_ptr(), g.data_ptr(), _p(gx), _p(gw),
              ws.data_ptr(), nb)
     return gx, gw
@@ -1084,11 +1081,9 @@ def router_balance(logits, inds, score_fn="sigmoid", mask=None):
     both are even, over the tokens that ``mask`` (bool [T]) keeps; what masked rows hold does not matter. Returns a
     ``RouterBalance``; its gradient is ``router_grad``'s, through the scores (counts have none)."""
     index, T, E, k, logits, inds, mask = _router_args("router_balance", logits, inds, score_fn, mask)
-    dev = logits.device
-    loss, probs = torch.empty(1, dtype=torch.float32, device=dev), torch.empty(E, dtype=torch.float32, device=dev)
-    counts, tokens = torch.empty(E, dtype=_I32, device=dev), torch.empty(1, dtype=_I32, device=dev)
+    loss, probs, counts, tokens = logits.new_empty(1), logits.new_empty(E), inds.new_empty(E), inds.new_empty(1)
     nb = _on_index(index, "lg_router_balance_workspace_bytes", T, E)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    ws = logits.new_empty(nb // 4) if nb else None
     _call_on(index, _lib.lib().lg_router_balance, logits.data_ptr(), inds.data_ptr(), _p(mask), T, E, k,
              _SCORES[score_fn], loss.data_ptr(), counts.data_ptr(), probs.data_ptr(), tokens.data_ptr(), _p(ws),
              nb)
@@ -1114,7 +1109,7 @@ def router_grad(logits, inds, dw=None, norm_topk_prob=True, score_fn="sigmoid", 
         _, counts, _, tokens = balance
         if _i32(counts, "counts", 1, index) != (E,) or _i32(tokens, "tokens", 1, index) != (1,):
             raise ValueError(f"router_grad: the balance is not of {E} experts")
-    out = torch.empty(T, E, dtype=torch.float32, device=logits.device)
+    out = logits.new_empty(T, E)
     _call_on(index, _lib.lib().lg_router_grad, logits.data_ptr(), inds.data_ptr(), _p(dw), _p(mask), T, E, k,
              int(bool(norm_topk_prob)), _SCORES[score_fn], _p(counts), _p(tokens), float(balance_weight),
              out.data_ptr())
