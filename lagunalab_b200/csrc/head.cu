@@ -872,7 +872,7 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
     w.out.ztgt = c.take<float>((size_t)T * K);
     if (few) {
       w.xp = c.take<__nv_bfloat16>((size_t)T * H);
-      w.idt = c.take<int>((size_t)HQ_MAXT * K);
+      w.idt = c.take<int>((size_t)HQ_PASSES * HQ_MAXT * K);
       w.bytes = align_up(c.used, 256);
       return w;
     }
@@ -1026,7 +1026,7 @@ using namespace lg;
 extern "C" size_t lg_head_loss_workspace_bytes(int T, int H, int V, int K, int bits, int top) {
   if (T < 1 || H < 8 || V < 1 || K < 1) return 256;
   const bool quant = bits == 4;
-  return hd_carve(nullptr, T, H, V, K, quant, quant && T <= HQ_MAXT, false, false, false, top != 0).bytes;
+  return hd_carve(nullptr, T, H, V, K, quant, quant && T <= HQ_PASSES * HQ_MAXT, false, false, false, top != 0).bytes;
 }
 
 extern "C" size_t lg_head_loss_grad_workspace_bytes(int T, int H, int V, int K, int bits, int dx, int dw) {
@@ -1045,13 +1045,22 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
   const HdHead head = {w, static_cast<const __nv_bfloat16*>(w_scales),
                        static_cast<const __nv_bfloat16*>(w_biases), ldw};
   const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);
-  const bool few = quant && T <= HQ_MAXT;
+  const bool few = quant && T <= HQ_PASSES * HQ_MAXT;
   const HdWork k = hd_carve(workspace, T, H, V, K, quant, few, false, false, false, top != nullptr);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < k.bytes)
     return fail(LG_ERR_WORKSPACE, "head_loss: workspace of %zu bytes, need %zu", workspace_bytes, k.bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (few) {
-    HD_TRY(hq_loss_parts(xb, ldx, T, H, head, V, ids, K, k.xp, k.idt, k.out, st));
+    const int passes = (T + HQ_MAXT - 1) / HQ_MAXT;
+    for (int i = 0; i < passes; ++i) {  // even shares: a pass's time goes by its blocks of 32 tokens
+      const int t0 = (int)((long long)T * i / passes), n = (int)((long long)T * (i + 1) / passes) - t0;
+      HdParts out = k.out;
+      out.part += (size_t)t0 * out.parts;
+      if (out.top) out.top += (size_t)t0 * out.parts;
+      out.ztgt += (size_t)t0 * K;
+      HD_TRY(hq_loss_parts(xb + (size_t)t0 * ldx, ldx, n, H, head, V, ids + (size_t)t0 * K, K, k.xp + (size_t)t0 * H,
+                           k.idt + (size_t)i * HQ_MAXT * K, out, st));
+    }
   } else {
     HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
     HdArgs a = hd_args(T, V, K, ids, weights, k);

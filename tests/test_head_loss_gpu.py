@@ -54,9 +54,11 @@ def test_4bit_head(T, V, H, K):
 @pytest.mark.parametrize("T,V,H,K", [(1, 1, 64, 1), (1, 33, 512, 1), (16, 31, 128, 2), (17, 129, 448, 1),
                                      (31, 4740, 64, 1), (32, 700, 1024, 64), (33, 40000, 576, 3),
                                      (64, 5003, 512, 1), (65, 20000, 192, 1), (100, 9001, 2048, 64),
-                                     (128, 40001, 1536, 1), (128, 300, 4096, 64), (129, 40001, 512, 1)])
+                                     (128, 40001, 1536, 1), (128, 300, 4096, 64), (129, 40001, 512, 1),
+                                     (255, 3001, 192, 5), (256, 700, 512, 1), (384, 5000, 320, 2),
+                                     (385, 5000, 320, 2)])
 def test_4bit_head_of_few_tokens(T, V, H, K):
-    """The 4-bit form for up to 128 tokens, one of 129 beside it: a CTA's ids in up to three tiles, its last of
+    """The 4-bit form for up to 384 tokens in passes of up to 128, one of 385 beside it: a CTA's ids in up to three tiles, its last of
     one to four blocks, groups of scales that come eight at a time (H % 512 == 0) or one by one."""
     x, head, W, ids, weights, _ = make(T, V, H, bits=4, K=K, skip=0.2, seed=V, std=0.02)
     ids.view(T, K)[T // 2] = V - 1
