@@ -57,4 +57,4 @@ def test_workspace_sizes():
     # a head of the benchmark's size: no [T, V] array in either
     assert L.lg_head_loss_workspace_bytes(8192, 2048, 100352, 1, 16, 0) < 64 << 20
     assert L.lg_head_loss_grad_workspace_bytes(8192, 2048, 100352, 1, 16, 1, 1) < 512 << 20
-    assert L.lg_head_loss_grad_workspace_bytes(1, 2048, 100352, 64, 4, 1, 0) < 128 << 20
+    assert L.lg_head_loss_grad_workspace_bytes(1, 2048, 100352, 64, 4, 1, 0) < 260 << 20  # a piece's weights

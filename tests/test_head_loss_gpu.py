@@ -262,8 +262,9 @@ def test_vocabulary_in_pieces(T, V, K):
     _many(T, V, 64, K, True)
 
 
-def test_4bit_vocabulary_in_pieces():
-    _many(257, 40001, 2048, 2, False, bits=4)
+@pytest.mark.parametrize("T,V", [(257, 40001), (390, 70001)])
+def test_4bit_vocabulary_in_pieces(T, V):
+    _many(T, V, 2048, 2, False, bits=4)
 
 
 def test_repeatable():
