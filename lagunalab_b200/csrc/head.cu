@@ -11,8 +11,10 @@
 // dx (fp32, added over the pieces) and to its rows of dW. Nothing of size [T, V] is kept.
 //
 // Roundings: z, the softmax statistics and every sum are fp32. dz is rounded to bf16 (2^-8 relative
-// at most) because the tensor cores take bf16 operands; its errors are independent, so that sums over
-// the vocabulary or the tokens average them. dx and dW are rounded once, at the end.
+// at most) because the tensor cores take bf16 operands. It is kept as dz / c, with c = max |g_t w_tj|, and
+// dx and dW are multiplied by c before they are rounded, once, at the end. So the usual g (1/n for every token)
+// and weight leave S exp(z - lse) - 1, whose -1 is exact; as -g it was off by up to 2^-8, in all tokens by the
+// same, and dx and dW with it. The other errors are independent: sums over the vocabulary or the tokens average them.
 //
 // Every mbarrier wait is bounded (tc::mbar_wait). A CTA whose wait ran out writes NaN for what is
 // left of its tiles, waits (bounded) for its copies and products in flight, frees its TMEM and ends.
@@ -61,7 +63,8 @@ struct HdArgs {
   // HD_PROB
   const float* lse;
   const float* g;
-  const float* wsum;  // K > 1: [T]
+  const float2* wsum;  // K > 1: [T] sum and largest size of the weights that count
+  float* scale;        // HD_PROB, HD_WGRAD: c
   // not HD_LOSS: bf16 [M, width], HD_XGRAD: fp32 [splits, M, width]
   void* tile_out;
   int width;
@@ -117,14 +120,14 @@ __device__ __forceinline__ HdRow hd_row(const HdArgs& a, const HdUnit& u, int t)
   if (KIND > HD_PROB || t >= a.M) return r;
   const size_t row_k = (size_t)t * a.K;
   if (KIND == HD_PROB) {
-    r.gg = a.g[t];
+    r.gg = a.g[t] / *a.scale;
     r.off = -a.lse[t] * HD_LOG2E;
   }
   if (a.K == 1) {
     r.next = a.ids[t];
     if (KIND == HD_PROB) {
       r.counts = r.next >= 0 && r.next < a.V;
-      r.gs = r.gg * (a.weights ? a.weights[t] : 1.f);
+      r.gs = a.weights ? a.g[t] * a.weights[t] / *a.scale : r.gg;
     }
   } else {
     const unsigned char* st = a.start + (size_t)t * (a.nt_all + 1);
@@ -133,7 +136,7 @@ __device__ __forceinline__ HdRow hd_row(const HdArgs& a, const HdUnit& u, int t)
     r.p1 = st[tile + 1];
     if (KIND == HD_PROB) {
       r.counts = st[a.nt_all] > 0;
-      r.gs = r.gg * a.wsum[t];
+      r.gs = r.gg * a.wsum[t].x;
     }
     if (r.p < r.p1) {
       r.next = a.ids[row_k + r.p];
@@ -251,6 +254,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
       hd_box<KIND>(a, box, r, n0 + c, y, u.split);
     }
   } else {
+    const float scale = KIND == HD_WGRAD ? *a.scale : 1.f;
 #pragma unroll 1
     for (int c = begin; c < begin + COLS && n0 + c < a.width; c += 64) {
       uint32_t r[32];
@@ -280,6 +284,10 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.f;
           }
+        }
+        if (KIND == HD_WGRAD) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] *= scale;
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) r[16 * h + i] = hd_pack(v[2 * i], v[2 * i + 1]);
@@ -519,20 +527,25 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
                                                       unsigned char* __restrict__ order,
                                                       float* __restrict__ sorted_w,
                                                       unsigned char* __restrict__ start,
-                                                      float* __restrict__ wsum) {
+                                                      float2* __restrict__ wsum) {
   __shared__ int sh[8][2 * HD_MAXK];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x * 8 + warp;
   if (t >= T) return;
   int* row = sh[warp];
-  float sum = 0.f;
+  float sum = 0.f, big = 0.f;
   for (int j = lane; j < HD_MAXK; j += 32) {
     const int id = j < K ? ids[(size_t)t * K + j] : -1;
     const bool in = id >= 0 && id < V;
     row[j] = in ? id : 0x7fffffff;
-    if (in) sum += weights ? weights[(size_t)t * K + j] : 1.f;
+    if (in) {
+      const float w = weights ? weights[(size_t)t * K + j] : 1.f;
+      sum += w;
+      big = fmaxf(big, fabsf(w));
+    }
   }
   sum = warp_sum(sum);
+  big = warp_max(big);
   __syncwarp();
   int* up = sh[warp] + HD_MAXK;  // ascending
   up[lane] = up[lane + 32] = 0x7fffffff;
@@ -558,7 +571,7 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
     if (up[c] < lim) ++c;
     start[(size_t)t * (nt + 1) + n] = (unsigned char)c;
   }
-  if (lane == 0) wsum[t] = sum;
+  if (lane == 0) wsum[t] = make_float2(sum, big);
 }
 
 constexpr int HJ_THREADS = 128;
@@ -720,15 +733,37 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
   }
 }
 
-// x with the rows of tokens without a target at 0, so that dW has nothing of them (0 * NaN is NaN).
+// Block 0: c, the largest |g_t w_tj| that counts (1 if there is none above 0, or an infinite one). The others, for dW:
+// x with the rows of tokens without a target at 0, so that dW has nothing of them (0 * NaN is NaN). One launch, because
+// c takes a block 3 us of its own.
 __global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx,
                                                       int T, int H, const int* __restrict__ ids, int V,
+                                                      const float* __restrict__ g, const float* __restrict__ weights,
                                                       const unsigned char* __restrict__ start, int nt,
+                                                      const float2* __restrict__ wsum, float* __restrict__ scale,
                                                       __nv_bfloat16* __restrict__ out) {
   pdl_trigger();
+  if (blockIdx.x == 0) {
+    __shared__ float sh[8];
+    float big = 0.f;
+#pragma unroll 4
+    for (int t = threadIdx.x; t < T; t += 256) {
+      const bool in = start ? start[(size_t)t * (nt + 1) + nt] > 0 : ids[t] >= 0 && ids[t] < V;
+      const float w = start ? wsum[t].y : weights ? weights[t] : 1.f;
+      if (in) big = fmaxf(big, fabsf(g[t] * w));
+    }
+    big = warp_max(big);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = big;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 8; ++i) big = fmaxf(big, sh[i]);
+      *scale = big > 0.f && big < INFINITY ? big : 1.f;
+    }
+    return;
+  }
   const int per = H / 8;
   const long long n = (long long)T * per;
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
+  for (long long i = (blockIdx.x - 1) * 256LL + threadIdx.x; i < n; i += (gridDim.x - 1) * 256LL) {
     const int t = (int)(i / per), c = (int)(i % per) * 8;
     const bool in = start ? start[(size_t)t * (nt + 1) + nt] > 0 : ids[t] >= 0 && ids[t] < V;
     uint4 v = make_uint4(0, 0, 0, 0);
@@ -770,9 +805,11 @@ __global__ void __launch_bounds__(256) hd_dequant_kernel(const uint2* __restrict
   }
 }
 
-// dx = the sum of its parts, in their order, rounded once.
+// dx = c times the sum of its parts, in their order, rounded once.
 __global__ void __launch_bounds__(256) hd_sum_kernel(const float* __restrict__ parts, int n,
-                                                     long long size, __nv_bfloat16* __restrict__ out) {
+                                                     long long size, const float* __restrict__ scale,
+                                                     __nv_bfloat16* __restrict__ out) {
+  const float c = *scale;
   const long long q = size / 4;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < q; i += gridDim.x * 256LL) {
     float4 s = reinterpret_cast<const float4*>(parts)[i];
@@ -780,7 +817,7 @@ __global__ void __launch_bounds__(256) hd_sum_kernel(const float* __restrict__ p
       const float4 v = reinterpret_cast<const float4*>(parts + j * size)[i];
       s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
     }
-    *reinterpret_cast<uint2*>(out + 4 * i) = make_uint2(hd_pack(s.x, s.y), hd_pack(s.z, s.w));
+    *reinterpret_cast<uint2*>(out + 4 * i) = make_uint2(hd_pack(c * s.x, c * s.y), hd_pack(c * s.z, c * s.w));
   }
 }
 
@@ -852,7 +889,9 @@ struct HdWork {
   int* idt;
   int* sorted;
   unsigned char *order, *start;
-  float *sorted_w, *wsum;
+  float* sorted_w;
+  float2* wsum;
+  float* scale;
   __nv_bfloat16 *wq, *dz, *xz;
   float* dx;
   size_t bytes;
@@ -882,10 +921,11 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
     w.order = c.take<unsigned char>((size_t)T * K);
     w.sorted_w = c.take<float>((size_t)T * K);
     w.start = c.take<unsigned char>((size_t)T * (w.nt + 1));
-    w.wsum = c.take<float>(T);
+    w.wsum = c.take<float2>(T);
   }
   if (quant) w.wq = c.take<__nv_bfloat16>((size_t)std::min(w.piece, V) * H);
   if (grad) {
+    w.scale = c.take<float>(1);
     w.dz = c.take<__nv_bfloat16>((size_t)T * w.piece);
     if (dw) w.xz = c.take<__nv_bfloat16>((size_t)T * H);
     if (dx) {
@@ -1102,11 +1142,9 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     return fail(LG_ERR_WORKSPACE, "head_loss_grad: workspace of %zu bytes, need %zu", workspace_bytes,
                 k.bytes);
   HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
-  if (dw) {
-    hd_rows_kernel<<<hd_blocks((long long)T * (H / 8)), 256, 0, st>>>(static_cast<const __nv_bfloat16*>(x), ldx, T, H,
-                                                                       ids, V, k.start, k.nt, k.xz);
-    LG_LAUNCH_CHECK("head_rows");
-  }
+  hd_rows_kernel<<<1 + (dw ? hd_blocks((long long)T * (H / 8)) : 0), 256, 0, st>>>(
+      static_cast<const __nv_bfloat16*>(x), ldx, T, H, ids, V, g, weights, k.start, k.nt, k.wsum, k.scale, k.xz);
+  LG_LAUNCH_CHECK("head_rows");
   for (int v0 = 0; v0 < V; v0 += k.piece) {
     const int n = std::min(k.piece, V - v0);
     HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, st));
@@ -1119,10 +1157,11 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     a.lse = lse;
     a.g = g;
     a.wsum = k.wsum;
+    a.scale = k.scale;
     const int ldz = (n + 63) / 64 * 64;
     a.tile_out = k.dz;
     a.width = ldz;
-    HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, a, quant || (v0 == 0 && dw), st));
+    HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, a, quant || v0 == 0, st));
     const HdOperand mz = {k.dz, n, T, ldz};
     if (dx) {
       HdArgs b = a;
@@ -1147,7 +1186,7 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
   if (dx) {
     // The last piece may have fewer parts than the first; later parts then kept the earlier sums.
     const int parts = std::min(k.splits, (std::min(k.piece, V) + HD_BK - 1) / HD_BK);
-    hd_sum_kernel<<<hd_blocks((long long)T * H / 4), 256, 0, st>>>(k.dx, parts, (long long)T * H,
+    hd_sum_kernel<<<hd_blocks((long long)T * H / 4), 256, 0, st>>>(k.dx, parts, (long long)T * H, k.scale,
                                                                    static_cast<__nv_bfloat16*>(dx));
     LG_LAUNCH_CHECK("head_sum");
   }

@@ -118,6 +118,48 @@ def test_one_target_with_a_weight():
     assert all(torch.equal(u, v) for u, v in zip(a, b))
 
 
+@pytest.mark.parametrize("K", [1, 3])
+@pytest.mark.parametrize("in_weights", [False, True])
+def test_a_common_factor_is_not_rounded(K, in_weights):
+    """g (or the weights) a constant just below the middle between two bf16 numbers. dz / g is K p - 1 at a target, which
+    rounds to -1 (K p < 2^-9, half a step below 1), an error of K p; elsewhere an error of 2^-8 K p.
+    -g itself would be off by 2^-8 g: as much again as the result's rounding allows."""
+    c, V, T = 1 + 2 ** -8 * 0.99, 3001, 150
+    x, head, W, _, _, _ = make(T, V, 128, std=0.02, seed=3)
+    x = x * 0.5
+    ids = torch.randperm(V, device="cuda")[:T * K].view(T, K).int()
+    ones, cs = torch.ones(T, K, device="cuda"), torch.full((T, K), c, device="cuda")
+    weights, g = (cs, ones[:, 0].contiguous()) if in_weights else (ones, cs[:, 0].contiguous())
+    _, lse = ops.head_loss(x, head, ids, weights)
+    gx, gw = ops.head_loss_grad(x, head, ids, lse, g, weights)
+    X, W64 = x.double().cpu(), W.double().cpu()
+    at = ids.long().cpu()
+    c = float(torch.tensor(c, dtype=torch.float32))
+    p = torch.softmax(X @ W64.T, 1)
+    assert K * p.max() < 2 ** -9
+    hot = torch.zeros_like(p).scatter_(1, at, 1.0)
+    dz, off = c * (K * p - hot), c * K * p * (hot + 2 ** -8 + 2 ** -12) + c * hot * 2 ** -18
+    for got, l, b, m in ((gx, dz, off, W64), (gw, dz.T, off.T, X)):
+        want = l @ m
+        within(got, want, b @ m.abs() + 2 ** -8 * want.abs() * (1 + 2 ** -8) + 2 ** -18 * (l.abs() @ m.abs()))
+
+
+def test_gradients_of_every_scale():
+    """g of any size: tiny, huge, zeros, one infinite (its own row and dW are not finite)."""
+    x, head, W, ids, _, g = make(70, 300, 64)
+    _, lse = ops.head_loss(x, head, ids)
+    one = ops.head_loss_grad(x, head, ids, lse, g)
+    for e in (-60, 60):
+        for a, b in zip(ops.head_loss_grad(x, head, ids, lse, g * 2.0 ** e), one):
+            assert torch.equal(a.float(), b.float() * 2.0 ** e)
+    for a in ops.head_loss_grad(x, head, ids, lse, torch.zeros_like(g)):
+        assert not a.any()
+    far = torch.zeros_like(g)
+    far[3] = float("inf")
+    gx, gw = ops.head_loss_grad(x, head, ids, lse, far)
+    assert not gx[3].isfinite().any() and not gx[:3].any() and not gx[4:].any()
+
+
 @pytest.mark.parametrize("K", [1, 7])
 def test_tokens_without_a_target_may_hold_anything(K):
     x, head, W, ids, weights, g = make(200, 700, 128, K=K)
