@@ -823,10 +823,11 @@ __global__ void __launch_bounds__(256) hd_sum_kernel(const float* __restrict__ p
 
 // ---- host ---------------------------------------------------------------------------------------
 
-constexpr long long HD_DZ_BYTES = 256LL << 20;  // dz of a piece
-// bf16 rows of a piece of a 4-bit head. Pieces that stay in L2 are no faster, even for few tokens: the launches cost
-// more (37 tokens, dx of 100,352 ids: 388 us with 32 MB, 276 with 64, 234 with 256, 229 with 512).
-constexpr long long HD_WQ_BYTES = 256LL << 20;
+// dz of a piece (8,192 tokens, dx and dW of 100,352 ids: 7.25 ms with 256 MB, 7.10 with 512, 7.53 with 128).
+constexpr long long HD_DZ_BYTES = 512LL << 20;
+// bf16 rows of a piece of a 4-bit head: 100,352 ids of 2,048 are one. Pieces that stay in L2 are no faster, even for few
+// tokens: the launches cost more (37 tokens, dx of 100,352 ids: 388 us with 32 MB, 276 with 64, 234 with 256, 229 with 512).
+constexpr long long HD_WQ_BYTES = 512LL << 20;
 
 static int hd_cg(int rows) { return rows > HD_BM ? 2 : 1; }
 static long long hd_rounds(long long units, int cg) {
@@ -835,8 +836,8 @@ static long long hd_rounds(long long units, int cg) {
 }
 
 // Vocabulary ids a piece: a multiple of 256, within the bytes above, such that the tiles of its products fill the
-// SMs in few whole rounds (8,192 tokens: pieces of 14,080 instead of 16,384 ids, grad_8k 6 % faster). Costs in
-// blocks of 64 of a contraction; a launch costs about 15.
+// SMs in few whole rounds (8,192 tokens, dx and dW of 100,352 ids: 6.26 to 6.62 ms; as many ids as fit 6.63 to 6.84,
+// even pieces 6.52 to 6.67). Costs in blocks of 64 of a contraction; a launch costs about 15.
 static int hd_piece(int T, int H, int V, bool quant, bool grad, bool dw) {
   const long long all = ((long long)V + HD_BN - 1) / HD_BN;
   long long most = all;

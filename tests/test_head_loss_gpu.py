@@ -299,12 +299,12 @@ def _many(T, V, H, K, dw, bits=16):
         within(gw, want.cpu(), bound.cpu())
 
 
-@pytest.mark.parametrize("T,V,K", [(4099, 40007, 1), (4099, 33000, 3)])
+@pytest.mark.parametrize("T,V,K", [(8195, 40007, 1), (8195, 36000, 3)])
 def test_vocabulary_in_pieces(T, V, K):
     _many(T, V, 64, K, True)
 
 
-@pytest.mark.parametrize("T,V", [(257, 40001), (390, 70001)])
+@pytest.mark.parametrize("T,V", [(257, 140001), (390, 140001)])
 def test_4bit_vocabulary_in_pieces(T, V):
     _many(T, V, 2048, 2, False, bits=4)
 
