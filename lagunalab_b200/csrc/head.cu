@@ -884,6 +884,25 @@ static int hd_splits(int T, int H, int piece) {
   return best;
 }
 
+// The 4-bit loss of few tokens: straight from the codes (head_q4.cu), or by the products over unpacked weights. The
+// first takes time by the passes (of up to 128 tokens) and their blocks of 32 tokens, the second by the bytes to unpack.
+// Both, us, as measured over V = 6,264 and 77,689, H = 64 to 2,048; of 77,689 ids (codes against products):
+//   tokens   H = 64     512        1,024       2,048
+//   32       15 : 20    18 : 41    25 : 74     41 : 141
+//   128      33 : 20    35 : 38    39 : 72     55 : 142
+//   256      58 : 27    64 : 46    71 : 75     100 : 144
+//   384      84 : 41    92 : 59    104 : 91    143 : 177
+// and of 6,264 ids 24 : 25 for 128 tokens of 2,048, 59 : 26 for 384.
+static bool hd_few(int T, int H, int V) {
+  if (T > HQ_PASSES * HQ_MAXT) return false;
+  if (T <= 32) return true;
+  const int passes = (T + HQ_MAXT - 1) / HQ_MAXT, n = (T + passes - 1) / passes, blocks = (n + 31) / 32;
+  const double ids = V * 1e-3;
+  const double codes = 3 + passes * (7 + 0.04 * n + 0.0026 * H + ids * (0.052 * blocks + 0.00011 * H));
+  const double products = 11 + 0.0017 * H + ids * (0.11 * ((T + HD_BM - 1) / HD_BM) + 0.00076 * H);
+  return codes < products;
+}
+
 struct HdWork {
   HdParts out;
   __nv_bfloat16* xp;  // few tokens and 4 bits: x in the order of a word's codes, ids by target
@@ -1067,7 +1086,7 @@ using namespace lg;
 extern "C" size_t lg_head_loss_workspace_bytes(int T, int H, int V, int K, int bits, int top) {
   if (T < 1 || H < 8 || V < 1 || K < 1) return 256;
   const bool quant = bits == 4;
-  return hd_carve(nullptr, T, H, V, K, quant, quant && T <= HQ_PASSES * HQ_MAXT, false, false, false, top != 0).bytes;
+  return hd_carve(nullptr, T, H, V, K, quant, quant && hd_few(T, H, V), false, false, false, top != 0).bytes;
 }
 
 extern "C" size_t lg_head_loss_grad_workspace_bytes(int T, int H, int V, int K, int bits, int dx, int dw) {
@@ -1086,7 +1105,7 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
   const HdHead head = {w, static_cast<const __nv_bfloat16*>(w_scales),
                        static_cast<const __nv_bfloat16*>(w_biases), ldw};
   const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);
-  const bool few = quant && T <= HQ_PASSES * HQ_MAXT;
+  const bool few = quant && hd_few(T, H, V);
   const HdWork k = hd_carve(workspace, T, H, V, K, quant, few, false, false, false, top != nullptr);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < k.bytes)
     return fail(LG_ERR_WORKSPACE, "head_loss: workspace of %zu bytes, need %zu", workspace_bytes, k.bytes);

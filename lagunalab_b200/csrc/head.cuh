@@ -81,8 +81,8 @@ struct HdParts {
 };
 
 // head_q4.cu: the loss's parts from a 4-bit head for few tokens, without the bf16 weights in memory: up to HQ_MAXT
-// tokens a pass over the weights. xp: T H bf16, idt: HQ_MAXT K ints of workspace. Three passes take less time than
-// unpacking the weights for the products of head.cu (129 tokens: 202 us there, 108 here; 384: 215 and 174).
+// tokens a pass over the weights. xp: T H bf16, idt: HQ_MAXT K ints of workspace. Taken for up to
+// HQ_PASSES passes, where that is faster than the products of head.cu over unpacked weights.
 constexpr int HQ_MAXT = 128, HQ_PASSES = 3;
 int hq_parts(int V);
 int hq_loss_parts(const __nv_bfloat16* x, long long ldx, int T, int H, const HdHead& w, int V, const int* ids,

@@ -58,3 +58,13 @@ def test_workspace_sizes():
     assert L.lg_head_loss_workspace_bytes(8192, 2048, 100352, 1, 16, 0) < 64 << 20
     assert L.lg_head_loss_grad_workspace_bytes(8192, 2048, 100352, 1, 16, 1, 1) < 768 << 20
     assert L.lg_head_loss_grad_workspace_bytes(1, 2048, 100352, 64, 4, 1, 0) < 520 << 20  # a piece's weights
+
+
+def test_which_form_a_4bit_loss_takes():
+    """From the codes (a small workspace) for up to 32 tokens, and further where unpacking the weights costs more."""
+    def codes(T, H, V):
+        return _lib.lib().lg_head_loss_workspace_bytes(T, H, V, 1, 4, 0) < V * H
+    assert all(codes(T, H, V) for T in (1, 32) for H in (64, 2048) for V in (6264, 100352))
+    assert all(codes(T, 2048, 100352) for T in (33, 128, 129, 256, 384))
+    assert not any(codes(T, 64, V) for T in (128, 384) for V in (6264, 77689))
+    assert not any(codes(T, H, V) for T in (385, 8192) for H in (64, 2048) for V in (6264, 100352))

@@ -3,7 +3,7 @@ tiles, both kinds of head, several targets a token, left-out tokens, strides, st
 import pytest
 import torch
 
-from lagunalab_b200 import ops
+from lagunalab_b200 import _lib, ops
 from tests._head_util import dequant64, reference, within
 
 pytestmark = pytest.mark.gpu
@@ -23,6 +23,11 @@ def make(T, V, H, bits=16, K=1, skip=0.0, seed=0, std=0.05):
     weights = torch.rand(T, K, generator=g, device="cuda") if K > 1 else None
     gr = torch.randn(T, generator=g, device="cuda")
     return x, head, W, ids[:, 0].contiguous() if K == 1 else ids, weights, gr
+
+
+def from_codes(T, H, V):
+    """Whether the 4-bit loss of these sizes reads the codes themselves: no workspace of V H bf16 then."""
+    return _lib.lib().lg_head_loss_workspace_bytes(T, H, V, 1, 4, 0) < V * H
 
 
 def check(x, head, W, ids, weights, g, dw=True):
@@ -56,10 +61,13 @@ def test_4bit_head(T, V, H, K):
                                      (64, 5003, 512, 1), (65, 20000, 192, 1), (100, 9001, 2048, 64),
                                      (128, 40001, 1536, 1), (128, 300, 4096, 64), (129, 40001, 512, 1),
                                      (255, 3001, 192, 5), (256, 700, 512, 1), (384, 5000, 320, 2),
-                                     (385, 5000, 320, 2)])
+                                     (385, 5000, 320, 2), (64, 30001, 1024, 2), (129, 50001, 1024, 1),
+                                     (255, 60001, 1088, 5), (384, 90001, 2048, 1)])
 def test_4bit_head_of_few_tokens(T, V, H, K):
-    """The 4-bit form for up to 384 tokens in passes of up to 128, one of 385 beside it: a CTA's ids in up to three tiles, its last of
-    one to four blocks, groups of scales that come eight at a time (H % 512 == 0) or one by one."""
+    """Both forms of the 4-bit loss. From the codes, in passes of up to 128 tokens: a CTA's ids in up to three tiles, its
+    last of one to four blocks, groups of scales that come eight at a time (H % 512 == 0) or one by one."""
+    if V * H > 1e6:
+        assert from_codes(T, H, V) == (T <= 32 or T <= 384 and V * H > 15e6 and H >= 576)
     x, head, W, ids, weights, _ = make(T, V, H, bits=4, K=K, skip=0.2, seed=V, std=0.02)
     ids.view(T, K)[T // 2] = V - 1
     r = reference(x, W, ids, weights)
@@ -75,20 +83,24 @@ def test_4bit_head_of_few_tokens(T, V, H, K):
     assert torch.equal(again[0], loss) and torch.equal(again[1], lse)
 
 
-@pytest.mark.parametrize("T", [7, 40, 90])
-def test_4bit_top_of_equal_logits_is_the_lowest_id(T):
-    rows = torch.zeros(6000, 64, device="cuda")
+@pytest.mark.parametrize("T,H,codes", [(7, 64, True), (40, 64, False), (40, 2048, True), (90, 64, False),
+                                       (90, 2048, True)])
+def test_4bit_top_of_equal_logits_is_the_lowest_id(T, H, codes):
+    assert from_codes(T, H, 6000) == codes
+    rows = torch.zeros(6000, H, device="cuda")
     rows[[37, 300, 301, 5990]] = 1
-    x = torch.ones(T, 64, dtype=torch.bfloat16, device="cuda")
+    x = torch.ones(T, H, dtype=torch.bfloat16, device="cuda")
     x[1] = -1
     top = ops.head_loss(x, ops.quantize(rows, 64, 4), torch.zeros(T, dtype=torch.int32, device="cuda"),
                         top=True)[2]
     assert top[1] == 0 and (top[[0, 2, T - 1]] == 37).all()
 
 
-@pytest.mark.parametrize("T", [5, 60, 128])
-def test_4bit_head_with_tokens_that_hold_nan(T):
-    x, head, W, ids, _, _ = make(T, 3000, 128, bits=4)
+@pytest.mark.parametrize("T,V,H,codes", [(5, 3000, 128, True), (60, 3000, 128, False), (128, 3000, 128, False),
+                                         (60, 9001, 2048, True), (128, 9001, 2048, True)])
+def test_4bit_head_with_tokens_that_hold_nan(T, V, H, codes):
+    assert from_codes(T, H, V) == codes
+    x, head, W, ids, _, _ = make(T, V, H, bits=4)
     want = ops.head_loss(x, head, ids)
     x[3] = float("nan")
     got = ops.head_loss(x, head, ids)
@@ -432,12 +444,14 @@ def test_4bit_scales_of_every_size(T):
     within(ops.head_loss_grad(x, (q, s, b), ids, lse, gr, dw=False)[0], r["dx"], r["bdx"])
 
 
-@pytest.mark.parametrize("T", [9, 50, 128])
+@pytest.mark.parametrize("T,H,codes", [(9, 64, True), (50, 64, True), (128, 64, False), (50, 1024, True),
+                                       (128, 1024, True)])
 @pytest.mark.parametrize("order", [1, -1])
-def test_4bit_logits_far_above_those_before(T, order):
+def test_4bit_logits_far_above_those_before(T, H, codes, order):
     """Logits that rise (or fall) by hundreds along the vocabulary: the reference of the exponentials has to follow,
     within a CTA's tiles and between CTAs."""
-    V, H = 40000, 64
+    V = 40000
+    assert from_codes(T, H, V) == codes
     g = torch.Generator(device="cuda").manual_seed(T)
     steps = order * torch.linspace(-900, 900, V // 32, device="cuda").repeat_interleave(32)
     rows = (torch.randn(V, H, generator=g, device="cuda") * 0.1 + (steps / H)[:, None])
