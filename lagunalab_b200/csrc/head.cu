@@ -10,6 +10,10 @@
 // and leaves dz as bf16 for a piece of the vocabulary, HD_XGRAD and HD_WGRAD take the piece's dz to
 // dx (fp32, added over the pieces) and to its rows of dW. Nothing of size [T, V] is kept.
 //
+// Bound: the tensor cores, and for more than some hundred us the power limit. 8,192 tokens and 100,352 ids of 2,048:
+// loss 2.2 ms (1.5 PFLOP/s; tensor pipe 98 % busy), both gradients 7.1 ms (1.4). With few rows the tiles' ends and the
+// chain of launches: 301 tokens and 32,003 ids of 1,024, 87 us (31 for dz, 27 dx, 25 dW, the rest sorting and joining).
+//
 // Roundings: z, the softmax statistics and every sum are fp32. dz is rounded to bf16 (2^-8 relative
 // at most) because the tensor cores take bf16 operands. It is kept as dz / c, with c = max |g_t w_tj|, and
 // dx and dW are multiplied by c before they are rounded, once, at the end. So the usual g (1/n for every token)

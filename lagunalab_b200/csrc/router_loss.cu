@@ -11,7 +11,8 @@
 // A token is worked on by G = 8, 16 or 32 lanes (E up to 64, 128, 256), eight scores a lane, so that a reduction's
 // shuffles serve 32 / G tokens at once: with a warp a token the gradient of 32,768 tokens of 64 experts took 254
 // instructions a token and 14 us. Both kernels read the logits once; the bound is HBM on long batches, launch
-// latency on short ones.
+// latency on short ones. 32,768 tokens: balance of 128 experts 15 to 17 us (17 MB: 8 for the sums, 5 for their join,
+// the rest between them), gradient of 64 experts 8 to 10 us (19 MB); 64 tokens 6 us, 4,096 tokens' gradient 4 us.
 #include <math.h>
 
 #include <algorithm>
