@@ -1021,9 +1021,10 @@ def head_loss_grad(x, head, ids, lse, g, weights=None, dx=True, dw=True):
     """The gradient of sum(g * loss) for ``head_loss``'s loss, from the same x, head, ids and weights, its
     ``lse`` and g fp32 [T]: (dx bf16 [T, H] or None, dw bf16 [V, H] or None). A 4-bit head has no
     gradient (``dw=False``). The vocabulary is taken in pieces: the workspace holds at most 512 MB of
-    the logits' gradient, and of a 4-bit head's weights. Tokens without a target give a row of zeros in dx
-    and nothing to dw, whatever their rows of x hold. The logits' gradient is rounded to bf16 for the
-    tensor cores, sums are fp32, results rounded once."""
+    the logits' gradient, and of a 4-bit head's weights. Ids that are negative or >= V are left out; tokens
+    without any other give a row of zeros in dx and nothing to dw, whatever their rows of x hold. The
+    logits' gradient, without the factor that all tokens share, is rounded to bf16 for the tensor cores;
+    sums are fp32, results rounded once."""
     index, sizes, args, keep = _head_args("head_loss_grad", x, head, ids, weights)
     T, H, V, _, bits = sizes
     if not (dx or dw):
