@@ -684,7 +684,7 @@ int lg_head_loss(const void* x, long long ldx, int T, int H, const void* w, long
  *   weights' sum,  dx = dz w (bf16 [T, H]),  dw = dz^T x (bf16 [V, H]).
  * dx or dw may be NULL (not both); a 4-bit head has no dw. A token without a target adds nothing to dw
  * and gives a row of zeros in dx, whatever its row of x holds; an id >= V counts as left out. dz is
- * rounded to bf16 for the tensor cores (2^-8 relative at most), sums are fp32.
+ * rounded to bf16 for the tensor cores (2^-8 relative at most) without the factor max |g weights|, sums are fp32.
  */
 size_t lg_head_loss_grad_workspace_bytes(int T, int H, int V, int K, int bits, int dx, int dw);
 int lg_head_loss_grad(const void* x, long long ldx, int T, int H, const void* w, long long ldw,
