@@ -7,6 +7,8 @@
 //   softmax: dl = s (dq - sum q dq),   sigmoid: dl = s (1 - s) (dq - sum q dq) / sum_e s.
 // Routing weights w_j = s_j / sum over the token's picks of s (norm) or s_j, for dw given:
 //   ds_j = (dw_j - sum_i dw_i w_i) / sum s (norm) or dw_j;  a sigmoid's or softmax's backward from there.
+// Such differences from a mean are taken of values less that of the largest share: where one share is nearly 1 (or the
+// only one: k = 1 with norm), its value and the mean are nearly the same number, and their roundings would be the result.
 //
 // A token is worked on by G = 8, 16 or 32 lanes (E up to 64, 128, 256), eight scores a lane, so that a reduction's
 // shuffles serve 32 / G tokens at once: with a warp a token the gradient of 32,768 tokens of 64 experts took 254
@@ -110,6 +112,14 @@ __device__ __forceinline__ float rb_scores(float (&v)[RB_N], float (&tail)[RB_N]
     sum += v[j];
   }
   return rb_sum<G>(sum);
+}
+
+// `v` of the first lane of this token's G that holds `mine` (of its lane 0 if none does).
+template <int G>
+__device__ __forceinline__ float rb_first(bool mine, float v) {
+  const unsigned lanes = __ballot_sync(0xffffffffu, mine) >> (threadIdx.x % 32 / G * G);
+  const int at = G == 32 ? __ffs(lanes) : __ffs(lanes & ((1u << G % 32) - 1));
+  return __shfl_sync(0xffffffffu, v, max(at - 1, 0), G);
 }
 
 struct RbOut {
@@ -328,17 +338,16 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs
     if (!keep || id >= a.E) id = -1;
     const float x = id >= 0 ? __ldg(row + id) : 0.f;
     const float total = rb_scores<G>(s, tail, a.score_fn, &mx, &rs);
-    float pick = 0.f;  // softmax: sum_e s_e ds_e
+    const bool softmax = a.score_fn == LG_SCORE_SOFTMAX;
     if (a.dw) {
       float unused;
-      const float p = id < 0 ? 0.f : a.score_fn == LG_SCORE_SOFTMAX ? rb_exp(x - mx) * rs : rb_sigmoid(x, &unused);
+      const float p = id < 0 ? 0.f : softmax ? rb_exp(x - mx) * rs : rb_sigmoid(x, &unused);
       if (id >= 0) st[id] = (unsigned char)l;
-      const float dot = rb_sum<G>(id >= 0 ? d * p : 0.f);
       if (a.norm) {
-        const float r = rb_rcp(rb_sum<G>(p));
+        const float top = rb_max<G>(p);
+        d -= rb_first<G>(id >= 0 && p == top, d);
+        const float dot = rb_sum<G>(id >= 0 ? d * p : 0.f), r = rb_rcp(rb_sum<G>(p));
         d = (d - dot * r) * r;
-      } else {
-        pick = dot;
       }
       __syncwarp();
       const bool twice = id >= 0 && st[id] != l;
@@ -352,26 +361,38 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs
       }
       __syncwarp();
     }
+    // What goes through the shares: h - sum q h. (A softmax's gradient of weights with norm sums to 0 by itself.)
+    const bool through = softmax && a.dw && !a.norm;
     const float r = rb_rcp(total);
-    float mean = 0.f;
-    if (a.counts) {
+    float h[RB_N];
 #pragma unroll
-      for (int j = 0; j < RB_N; ++j) mean = fmaf(s[j], dq[j], mean);
+    for (int j = 0; j < RB_N; ++j) {
+      const int e = rb_expert<G, VEC>(j);
+      h[j] = dq[j] + (through && e < a.E ? sd[e] : 0.f);
+    }
+    if (a.counts || through) {
+      float best = s[0], at = h[0], mean = 0.f;
+#pragma unroll
+      for (int j = 1; j < RB_N; ++j) {
+        at = s[j] > best ? h[j] : at;
+        best = fmaxf(best, s[j]);
+      }
+      const float top = rb_max<G>(best);
+      const float ref = rb_first<G>(best == top, at);
+#pragma unroll
+      for (int j = 0; j < RB_N; ++j) {
+        h[j] -= ref;
+        mean = fmaf(s[j], h[j], mean);
+      }
       mean = rb_sum<G>(mean) * r;
+#pragma unroll
+      for (int j = 0; j < RB_N; ++j) h[j] -= mean;
     }
 #pragma unroll
     for (int j = 0; j < RB_N; ++j) {
       const int e = rb_expert<G, VEC>(j);
-      float ds = a.dw && e < a.E ? sd[e] : 0.f;
-      float g;
-      if (a.score_fn == LG_SCORE_SOFTMAX) {
-        if (a.counts) ds += dq[j] - mean;
-        g = s[j] * (ds - pick);
-      } else {
-        if (a.counts) ds += (dq[j] - mean) * r;
-        g = ds * tail[j];
-      }
-      s[j] = keep ? g : 0.f;
+      const float ds = a.dw && !through && e < a.E ? sd[e] : 0.f;
+      s[j] = keep ? softmax ? s[j] * (ds + h[j]) : tail[j] * fmaf(h[j], r, ds) : 0.f;
     }
     if (in) {
       float* out = a.dl + (size_t)t * a.E;

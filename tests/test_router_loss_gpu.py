@@ -176,6 +176,56 @@ def test_far_logits(fn):
     assert g.isfinite().all() and (g[:, 7] == 0).all()
 
 
+@pytest.mark.parametrize("fn", ["sigmoid", "softmax"])
+def test_weights_of_one_pick_have_no_gradient(fn):
+    logits, inds, dw, _ = make(300, 20, 1)
+    assert (ops.router_grad(logits, inds, dw, True, fn) == 0).all()
+    logits, inds, dw, _ = make(300, 1, 1)  # one expert: its share is 1 whatever its logit
+    bal = ops.router_balance(logits, inds, "softmax")
+    assert (ops.router_grad(logits, inds, dw, False, "softmax", bal, 0.3) == 0).all()
+
+
+@pytest.mark.parametrize("E,k", [(7, 6), (60, 4), (128, 8), (250, 20)])
+@pytest.mark.parametrize("weight", [None, 0.5])
+@pytest.mark.parametrize("norm,fn", [(True, "sigmoid"), (True, "softmax"), (False, "softmax")])
+def test_one_share_near_one(E, k, weight, norm, fn):
+    """A pick whose share is nearly all of it. Each gradient is a score times a sum of differences from the largest
+    share's value; a score is off by 2^-17 relative (arguments up to 40), the sums' other roundings by less: 2^-15 of
+    the differences' absolute sum. Differences from the mean itself would be off by 2^-24 of the values."""
+    logits, inds, dw, _ = make(200, E, k)
+    if fn == "sigmoid":
+        logits = logits - 12
+    logits[torch.arange(200, device="cuda"), inds[:, 0].long()] += 12
+    bal = None if weight is None else ops.router_balance(logits, inds, fn)
+    got = ops.router_grad(logits, inds, dw, norm, fn, bal, weight or 0.0).cpu().double()
+    want = grad64(logits, inds, dw, norm, fn, None, weight)
+    s, i, d = scores(logits.cpu().double(), fn), inds.cpu().long(), dw.cpu().double()
+    tail = s if fn == "softmax" else torch.sigmoid(-logits.cpu().double()) * s
+    total = s.sum(1, keepdim=True)
+    if norm:
+        p = s.gather(1, i)
+        w, d = p / p.sum(1, keepdim=True), (d - d[:, :1]).abs()
+        part = torch.zeros_like(s).scatter_(1, i, (d + (w * d).sum(1, keepdim=True)) / p.sum(1, keepdim=True))
+        h = torch.zeros_like(s)
+    else:
+        part, h = torch.zeros_like(s), torch.zeros_like(s).scatter_(1, i, d)
+    dq = torch.zeros(E, dtype=torch.float64)
+    if weight is not None:
+        dq = weight * E * bal.counts.cpu().double() / int(bal.counts.sum()) / 200
+    top = s.argmax(1, keepdim=True)
+    own = 2.0 ** -22 * dq + 2.0 ** -23 * h.abs()  # of dq and of its sum with dw; none for the largest share
+    own = (own + own.gather(1, top)).scatter(1, top, 0.0)
+    h = h + dq
+    h = (h - h.gather(1, top)).abs()
+    both = [a + (s * a).sum(1, keepdim=True) / total for a in (h, own)]
+    if fn == "sigmoid":
+        both = [a / total for a in both]
+    # the formula's own roundings: an expert that is not picked has exactly 0 where 64 bits leave a sum that cancels, off
+    # by 2^-53 of each of up to 2 k terms of up to 2 |dw| / sum s (sum s > 0.5 here) and their own few roundings
+    exact = 2.0 ** -47 * dw.cpu().double().abs().sum(1, keepdim=True)
+    assert ((got - want).abs() <= tail * (2.0 ** -15 * (part + both[0]) + 2 * both[1] + exact) + 1e-37).all()
+
+
 def test_strides_streams_and_graphs():
     logits, inds, dw, mask = make(500, 40, 4)
     bal = ops.router_balance(logits, inds, mask=mask)
