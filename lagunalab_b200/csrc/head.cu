@@ -737,55 +737,70 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
   }
 }
 
-// Block 0: c, the largest |g_t w_tj| that counts (1 if there is none above 0, or an infinite one). The others, for dW:
-// x with the rows of tokens without a target at 0, so that dW has nothing of them (0 * NaN is NaN). One launch, because
-// c takes a block 3 us of its own.
-__global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx,
-                                                      int T, int H, const int* __restrict__ ids, int V,
-                                                      const float* __restrict__ g, const float* __restrict__ weights,
-                                                      const unsigned char* __restrict__ start, int nt,
-                                                      const float2* __restrict__ wsum, float* __restrict__ scale,
-                                                      __nv_bfloat16* __restrict__ out) {
+// c, the largest |g_t w_tj| that counts (1 if there is none above 0, or an infinite one), by a block of 256 threads of a
+// kernel that runs before the products anyway: it takes 3 us.
+struct HdScale {
+  const int* ids;
+  const float *g, *weights;
+  const unsigned char* start;  // K > 1: as in HdArgs
+  const float2* wsum;
+  float* scale;  // NULL: not asked for
+  int T, V, nt;
+};
+__device__ __forceinline__ bool hd_counts(const HdScale& a, int t) {
+  return a.start ? a.start[(size_t)t * (a.nt + 1) + a.nt] > 0 : a.ids[t] >= 0 && a.ids[t] < a.V;
+}
+__device__ __forceinline__ void hd_scale(const HdScale& a) {
+  __shared__ float sh[8];
+  float big = 0.f;
+#pragma unroll 4
+  for (int t = threadIdx.x; t < a.T; t += 256) {
+    const float w = a.start ? a.wsum[t].y : a.weights ? a.weights[t] : 1.f;
+    if (hd_counts(a, t)) big = fmaxf(big, fabsf(a.g[t] * w));
+  }
+  big = warp_max(big);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = big;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) big = fmaxf(big, sh[i]);
+    *a.scale = big > 0.f && big < INFINITY ? big : 1.f;
+  }
+}
+
+// Block 0: c. The others, for dW: x with the rows of tokens without a target at 0, so that dW has nothing of them
+// (0 * NaN is NaN).
+__global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int H,
+                                                      const HdScale a, __nv_bfloat16* __restrict__ out) {
   pdl_trigger();
   if (blockIdx.x == 0) {
-    __shared__ float sh[8];
-    float big = 0.f;
-#pragma unroll 4
-    for (int t = threadIdx.x; t < T; t += 256) {
-      const bool in = start ? start[(size_t)t * (nt + 1) + nt] > 0 : ids[t] >= 0 && ids[t] < V;
-      const float w = start ? wsum[t].y : weights ? weights[t] : 1.f;
-      if (in) big = fmaxf(big, fabsf(g[t] * w));
-    }
-    big = warp_max(big);
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = big;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int i = 1; i < 8; ++i) big = fmaxf(big, sh[i]);
-      *scale = big > 0.f && big < INFINITY ? big : 1.f;
-    }
+    hd_scale(a);
     return;
   }
   const int per = H / 8;
-  const long long n = (long long)T * per;
+  const long long n = (long long)a.T * per;
   for (long long i = (blockIdx.x - 1) * 256LL + threadIdx.x; i < n; i += (gridDim.x - 1) * 256LL) {
     const int t = (int)(i / per), c = (int)(i % per) * 8;
-    const bool in = start ? start[(size_t)t * (nt + 1) + nt] > 0 : ids[t] >= 0 && ids[t] < V;
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (in) v = *reinterpret_cast<const uint4*>(x + (size_t)t * ldx + c);
+    if (hd_counts(a, t)) v = *reinterpret_cast<const uint4*>(x + (size_t)t * ldx + c);
     *reinterpret_cast<uint4*>(out + (size_t)t * H + c) = v;
   }
 }
 
 // Rows of a 4-bit group-64 head as bf16: bf16(scale * code + bias), two words a thread: a warp writes 1 KB in one
-// store (four words a thread with 16-byte stores: 3 TB/s written instead of 4.3).
+// store (four words a thread with 16-byte stores: 3 TB/s written instead of 4.3). Block 0 may have c to find instead.
 __global__ void __launch_bounds__(256) hd_dequant_kernel(const uint2* __restrict__ q,
                                                          const uint16_t* __restrict__ s,
                                                          const uint16_t* __restrict__ b, long long n,
-                                                         __nv_bfloat16* __restrict__ out) {
+                                                         const HdScale a, __nv_bfloat16* __restrict__ out) {
   pdl_trigger();
+  const int first = a.scale != nullptr;  // of the blocks that unpack
+  if (first && blockIdx.x == 0) {
+    hd_scale(a);
+    return;
+  }
   constexpr int U = 4;
-  const long long step = gridDim.x * 256LL;
-  for (long long i0 = blockIdx.x * 256LL + threadIdx.x; i0 < n; i0 += U * step) {
+  const long long step = (gridDim.x - first) * 256LL;
+  for (long long i0 = (blockIdx.x - first) * 256LL + threadIdx.x; i0 < n; i0 += U * step) {
     uint2 w[U];
     uint16_t sc[U], bi[U];
 #pragma unroll
@@ -1013,7 +1028,7 @@ struct HdOperand {
 // One CTA a tile where the output has no more than 128 rows, else a pair.
 //
 // `early`: it may start under the kernel before it, one of this call's that says so (pdl_trigger) and whose CTAs have
-// room beside an hd_kernel's on an SM (no shared memory of their own). Nothing else is launched early: where a
+// room beside an hd_kernel's on an SM (next to no shared memory of their own). Nothing else is launched early: where a
 // kernel's CTAs are not all on the GPU yet, waiting CTAs of a later one can take their SMs and wait for them
 // for ever. (It happened behind hd_kernel, some of whose pairs had to wait for the dequantization's CTAs.)
 template <int KIND>
@@ -1048,15 +1063,15 @@ static int hd_check(const char* who, const void* x, long long ldx, int T, int H,
 
 static int hd_blocks(long long n) { return (int)std::min<long long>((n + 255) / 256, 148 * 16); }
 
-// The piece's bf16 weights and B's first row in them.
+// The piece's bf16 weights, and c if it is asked for.
 static int hd_weights(const void* w, const void* ws, const void* wb, int H, int v0, int rows,
-                      const HdWork& k, cudaStream_t st) {
+                      const HdWork& k, const HdScale& scale, cudaStream_t st) {
   if (!ws) return LG_OK;
   const long long n = (long long)rows * (H / 16);
   const size_t at = (size_t)v0 * (H / 16);
-  hd_dequant_kernel<<<hd_blocks(n), 256, 0, st>>>(static_cast<const uint2*>(w) + at,
-                                                  static_cast<const uint16_t*>(ws) + at / 4,
-                                                  static_cast<const uint16_t*>(wb) + at / 4, n, k.wq);
+  hd_dequant_kernel<<<hd_blocks(n) + (scale.scale != nullptr), 256, 0, st>>>(
+      static_cast<const uint2*>(w) + at, static_cast<const uint16_t*>(ws) + at / 4,
+      static_cast<const uint16_t*>(wb) + at / 4, n, scale, k.wq);
   LG_LAUNCH_CHECK("head_dequant");
   return LG_OK;
 }
@@ -1132,7 +1147,7 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
     a.out = k.out;
     for (int v0 = 0; v0 < V; v0 += k.piece) {
       const int n = std::min(k.piece, V - v0);
-      HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, st));
+      HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, {}, st));
       a.N = n;
       a.v0 = v0;
       a.b_row0 = quant ? 0 : v0;
@@ -1166,12 +1181,15 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     return fail(LG_ERR_WORKSPACE, "head_loss_grad: workspace of %zu bytes, need %zu", workspace_bytes,
                 k.bytes);
   HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
-  hd_rows_kernel<<<1 + (dw ? hd_blocks((long long)T * (H / 8)) : 0), 256, 0, st>>>(
-      static_cast<const __nv_bfloat16*>(x), ldx, T, H, ids, V, g, weights, k.start, k.nt, k.wsum, k.scale, k.xz);
-  LG_LAUNCH_CHECK("head_rows");
+  const HdScale scale = {ids, g, weights, k.start, k.wsum, k.scale, T, V, k.nt};
+  if (!quant) {
+    hd_rows_kernel<<<1 + (dw ? hd_blocks((long long)T * (H / 8)) : 0), 256, 0, st>>>(
+        static_cast<const __nv_bfloat16*>(x), ldx, H, scale, k.xz);
+    LG_LAUNCH_CHECK("head_rows");
+  }
   for (int v0 = 0; v0 < V; v0 += k.piece) {
     const int n = std::min(k.piece, V - v0);
-    HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, st));
+    HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, v0 == 0 ? scale : HdScale{}, st));
     const HdOperand mw = quant ? HdOperand{k.wq, H, n, H} : HdOperand{w, H, V, ldw};
     HdArgs a = hd_args(T, V, K, ids, weights, k);
     a.v0 = v0;
