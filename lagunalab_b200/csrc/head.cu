@@ -52,7 +52,7 @@ struct HdArgs {
   int M, N;          // rows of the output tile grid, and its columns
   int mt, nt;        // tiles of 128 CG x 256
   int kblocks;       // 64-wide blocks of the contraction
-  int splits;        // HD_XGRAD: parts of the contraction, each with a sum of its own
+  int splits;        // HD_XGRAD, HD_WGRAD: parts of the contraction, each with a sum of its own
   int b_row0;        // HD_LOSS, HD_PROB: B's first row; HD_XGRAD: B's first row along the contraction
   int v0;            // the piece's first vocabulary id
   int V;
@@ -69,7 +69,7 @@ struct HdArgs {
   const float* g;
   const float2* wsum;  // K > 1: [T] sum and largest size of the weights that count
   float* scale;        // HD_PROB, HD_WGRAD: c
-  // not HD_LOSS: bf16 [M, width], HD_XGRAD: fp32 [splits, M, width]
+  // not HD_LOSS: bf16 [M, width], HD_XGRAD and parts of HD_WGRAD: fp32 [splits, M, width]
   void* tile_out;
   int width;
   int add;  // HD_XGRAD: 0 for the first piece
@@ -100,12 +100,12 @@ __device__ __forceinline__ HdUnit hd_unit(const HdArgs& a, int i) {
   } else {
     const unsigned r = (unsigned)i / (unsigned)a.nt;
     u.n = i - r * a.nt;
-    u.split = KIND == HD_XGRAD ? r / (unsigned)a.mt : 0;
+    u.split = r / (unsigned)a.mt;
     u.m = r - u.split * a.mt;
   }
   u.k0 = 0;
   u.k1 = a.kblocks;
-  if (KIND == HD_XGRAD && a.splits > 1) {  // at most 2^24 blocks of a piece's ids times 148 parts
+  if (KIND >= HD_XGRAD && a.splits > 1) {  // at most 2^24 blocks of a contraction times 148 parts
     u.k0 = (unsigned)a.kblocks * u.split / (unsigned)a.splits;
     u.k1 = (unsigned)a.kblocks * (u.split + 1) / (unsigned)a.splits;
   }
@@ -247,7 +247,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
       a.out.part[(size_t)t * a.nt_all + ntile] = make_float2(mx, ok ? sum : nan);
       if (a.out.top) a.out.top[(size_t)t * a.nt_all + ntile] = arg;
     }
-  } else if (KIND == HD_XGRAD) {
+  } else if (KIND == HD_XGRAD || (KIND == HD_WGRAD && a.splits > 1)) {
 #pragma unroll 1
     for (int c = begin; c < begin + COLS && n0 + c < a.width; c += 32) {
       __syncwarp();
@@ -255,7 +255,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
       uint32_t r[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
-      hd_box<KIND>(a, box, r, n0 + c, y, u.split);
+      hd_box<HD_XGRAD>(a, box, r, n0 + c, y, u.split);
     }
   } else {
     const float scale = KIND == HD_WGRAD ? *a.scale : 1.f;
@@ -824,7 +824,7 @@ __global__ void __launch_bounds__(256) hd_dequant_kernel(const uint2* __restrict
   }
 }
 
-// dx = c times the sum of its parts, in their order, rounded once.
+// dx (dW) = c times the sum of its parts, in their order, rounded once.
 __global__ void __launch_bounds__(256) hd_sum_kernel(const float* __restrict__ parts, int n,
                                                      long long size, const float* __restrict__ scale,
                                                      __nv_bfloat16* __restrict__ out) {
@@ -903,6 +903,17 @@ static int hd_splits(int T, int H, int piece) {
   return best;
 }
 
+// Parts of dW's contraction, the tokens: where its tiles fill less than half the SMs, as many as fit, of at least 8
+// blocks of 64 each (8,192 tokens, 512 ids of 256: 65 us with one part, 36 with 16; 4,757 tokens, 380 ids of 136: 52 and
+// 36). Not below 40 blocks: the join costs as much (2,048 tokens, 4,000 ids of 256: 39 and 38 us, with a launch more).
+static int hd_wsplits(int T, int H, int rows) {
+  const int cg = hd_cg(rows);
+  const long long tiles = (((long long)rows + HD_BM * cg - 1) / (HD_BM * cg)) * ((H + HD_BN - 1) / HD_BN);
+  if (T < 40 * HD_BK) return 1;
+  const long long fit = device_sm_count() / cg / tiles;
+  return (int)std::max(1LL, std::min<long long>(fit, T / (8 * HD_BK)));
+}
+
 // The 4-bit loss of few tokens: straight from the codes (head_q4.cu), or by the products over unpacked weights. The
 // first takes time by the passes (of up to 128 tokens) and their blocks of 32 tokens, the second by the bytes to unpack.
 // Both, us, as measured over V = 6,264 and 77,689, H = 64 to 2,048; of 77,689 ids (codes against products):
@@ -932,9 +943,9 @@ struct HdWork {
   float2* wsum;
   float* scale;
   __nv_bfloat16 *wq, *dz, *xz;
-  float* dx;
+  float *dx, *dw;  // fp32 parts (dw: NULL where it has one)
   size_t bytes;
-  int piece, nt, splits;
+  int piece, nt, splits, wsplits;
 };
 
 static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool few, bool grad, bool dx,
@@ -966,7 +977,11 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
   if (grad) {
     w.scale = c.take<float>(1);
     w.dz = c.take<__nv_bfloat16>((size_t)T * w.piece);
-    if (dw) w.xz = c.take<__nv_bfloat16>((size_t)T * H);
+    if (dw) {
+      w.xz = c.take<__nv_bfloat16>((size_t)T * H);
+      w.wsplits = hd_wsplits(T, H, std::min(w.piece, V));
+      if (w.wsplits > 1) w.dw = c.take<float>((size_t)w.wsplits * std::min(w.piece, V) * H);
+    }
     if (dx) {
       w.splits = hd_splits(T, H, std::min(w.piece, V));
       w.dx = c.take<float>((size_t)w.splits * T * H);
@@ -1073,6 +1088,12 @@ static int hd_weights(const void* w, const void* ws, const void* wb, int H, int 
       static_cast<const uint2*>(w) + at, static_cast<const uint16_t*>(ws) + at / 4,
       static_cast<const uint16_t*>(wb) + at / 4, n, scale, k.wq);
   LG_LAUNCH_CHECK("head_dequant");
+  return LG_OK;
+}
+
+static int hd_join_parts(const float* parts, int n, long long size, const float* scale, void* out, cudaStream_t st) {
+  hd_sum_kernel<<<hd_blocks(size / 4), 256, 0, st>>>(parts, n, size, scale, static_cast<__nv_bfloat16*>(out));
+  LG_LAUNCH_CHECK("head_sum");
   return LG_OK;
 }
 
@@ -1220,17 +1241,18 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
       b.M = n;
       b.N = H;
       b.kblocks = (T + HD_BK - 1) / HD_BK;
-      b.tile_out = static_cast<__nv_bfloat16*>(dw) + (size_t)v0 * H;
+      b.splits = k.wsplits;
+      __nv_bfloat16* rows = static_cast<__nv_bfloat16*>(dw) + (size_t)v0 * H;
+      b.tile_out = k.wsplits > 1 ? static_cast<void*>(k.dw) : rows;
       b.width = H;
       HD_TRY(hd_launch<HD_WGRAD>(mz, {k.xz, H, T, H}, b, false, st));
+      if (k.wsplits > 1) HD_TRY(hd_join_parts(k.dw, k.wsplits, (long long)n * H, k.scale, rows, st));
     }
   }
   if (dx) {
     // The last piece may have fewer parts than the first; later parts then kept the earlier sums.
     const int parts = std::min(k.splits, (std::min(k.piece, V) + HD_BK - 1) / HD_BK);
-    hd_sum_kernel<<<hd_blocks((long long)T * H / 4), 256, 0, st>>>(k.dx, parts, (long long)T * H, k.scale,
-                                                                   static_cast<__nv_bfloat16*>(dx));
-    LG_LAUNCH_CHECK("head_sum");
+    HD_TRY(hd_join_parts(k.dx, parts, (long long)T * H, k.scale, dx, st));
   }
   return LG_OK;
 }

@@ -316,6 +316,16 @@ def test_vocabulary_in_pieces(T, V, K):
     _many(T, V, 64, K, True)
 
 
+@pytest.mark.parametrize("T,V,H", [(1024, 1, 8), (1100, 130, 264), (2050, 300, 72), (4757, 380, 136), (3000, 5000, 64)])
+def test_many_tokens_over_few_ids(T, V, H):
+    """dW's contraction in parts, as its tiles alone would leave most SMs idle."""
+    check(*make(T, V, H, K=2, skip=0.3, seed=V))
+
+
+def test_many_tokens_over_few_ids_in_pieces():
+    _many(600000, 500, 64, 1, True)
+
+
 @pytest.mark.parametrize("T,V", [(257, 140001), (390, 140001)])
 def test_4bit_vocabulary_in_pieces(T, V):
     _many(T, V, 2048, 2, False, bits=4)
