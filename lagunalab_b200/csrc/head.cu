@@ -157,7 +157,8 @@ __device__ __forceinline__ HdRow hd_row(const HdArgs& a, const HdUnit& u, int t)
 //
 // This thread's 128 bytes of a box: rows y ... of the output's `rows`, from its column x (of a.width) on.
 template <int KIND>
-__device__ __forceinline__ void hd_box(const HdArgs& a, uint8_t* box, const uint32_t (&r)[32], int x, int y, int split) {
+__device__ __forceinline__ void hd_box(const HdArgs& a, uint8_t* box, const uint32_t (&r)[32], int x, int y,
+                                       int split) {
   constexpr int PER = KIND == HD_XGRAD ? 4 : 8;  // elements in 16 bytes
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -737,8 +738,8 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
   }
 }
 
-// c, the largest |g_t w_tj| that counts (1 if there is none above 0, or an infinite one), by a block of 256 threads of a
-// kernel that runs before the products anyway: it takes 3 us.
+// c, the largest |g_t w_tj| that counts (1 if there is none above 0, or an infinite one), by a block of 256 threads
+// of a kernel that runs before the products anyway: it takes 3 us.
 struct HdScale {
   const int* ids;
   const float *g, *weights;
@@ -844,8 +845,9 @@ __global__ void __launch_bounds__(256) hd_sum_kernel(const float* __restrict__ p
 
 // dz of a piece (8,192 tokens, dx and dW of 100,352 ids: 7.25 ms with 256 MB, 7.10 with 512, 7.53 with 128).
 constexpr long long HD_DZ_BYTES = 512LL << 20;
-// bf16 rows of a piece of a 4-bit head: 100,352 ids of 2,048 are one. Pieces that stay in L2 are no faster, even for few
-// tokens: the launches cost more (37 tokens, dx of 100,352 ids: 388 us with 32 MB, 276 with 64, 234 with 256, 229 with 512).
+// bf16 rows of a piece of a 4-bit head: 100,352 ids of 2,048 are one. Pieces that stay in L2 are no faster, even for
+// few tokens: the launches cost more (37 tokens, dx of 100,352 ids: 388 us with 32 MB, 276 with 64, 234 with 256, 229
+// with 512).
 constexpr long long HD_WQ_BYTES = 512LL << 20;
 
 static int hd_cg(int rows) { return rows > HD_BM ? 2 : 1; }
@@ -904,8 +906,9 @@ static int hd_splits(int T, int H, int piece) {
 }
 
 // Parts of dW's contraction, the tokens: where its tiles fill less than half the SMs, as many as fit, of at least 8
-// blocks of 64 each (8,192 tokens, 512 ids of 256: 65 us with one part, 36 with 16; 4,757 tokens, 380 ids of 136: 52 and
-// 36). Not below 40 blocks: the join costs as much (2,048 tokens, 4,000 ids of 256: 39 and 38 us, with a launch more).
+// blocks of 64 each (8,192 tokens, 512 ids of 256: 65 us with one part, 36 with 16; 4,757 tokens, 380 ids of 136: 52
+// and 36). Not below 40 blocks: the join costs as much (2,048 tokens, 4,000 ids of 256: 39 and 38 us, with a launch
+// more).
 static int hd_wsplits(int T, int H, int rows) {
   const int cg = hd_cg(rows);
   const long long tiles = (((long long)rows + HD_BM * cg - 1) / (HD_BM * cg)) * ((H + HD_BN - 1) / HD_BN);
@@ -915,8 +918,8 @@ static int hd_wsplits(int T, int H, int rows) {
 }
 
 // The 4-bit loss of few tokens: straight from the codes (head_q4.cu), or by the products over unpacked weights. The
-// first takes time by the passes (of up to 128 tokens) and their blocks of 32 tokens, the second by the bytes to unpack.
-// Both, us, as measured over V = 6,264 and 77,689, H = 64 to 2,048; of 77,689 ids (codes against products):
+// first takes time by the passes (of up to 128 tokens) and their blocks of 32 tokens, the second by the bytes to
+// unpack. Both, us, as measured over V = 6,264 and 77,689, H = 64 to 2,048; of 77,689 ids (codes against products):
 //   tokens   H = 64     512        1,024       2,048
 //   32       15 : 20    18 : 41    25 : 74     41 : 141
 //   128      33 : 20    35 : 38    39 : 72     55 : 142
@@ -1100,7 +1103,8 @@ static int hd_join_parts(const float* parts, int n, long long size, const float*
 static int hd_sort(const int* ids, const float* weights, int T, int K, int V, const HdWork& k,
                    cudaStream_t st) {
   if (K == 1) return LG_OK;
-  hd_sort_kernel<<<(T + 7) / 8, 256, 0, st>>>(ids, weights, T, K, V, k.nt, k.sorted, k.order, k.sorted_w, k.start, k.wsum);
+  hd_sort_kernel<<<(T + 7) / 8, 256, 0, st>>>(ids, weights, T, K, V, k.nt, k.sorted, k.order, k.sorted_w, k.start,
+                                              k.wsum);
   LG_LAUNCH_CHECK("head_sort");
   return LG_OK;
 }
