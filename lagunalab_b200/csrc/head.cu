@@ -22,6 +22,8 @@
 //
 // Every mbarrier wait is bounded (tc::mbar_wait). A CTA whose wait ran out writes NaN for what is
 // left of its tiles, waits (bounded) for its copies and products in flight, frees its TMEM and ends.
+// Nothing asynchronous outlives the CTA that it writes to: copies, the commits that free a stage, and the epilogue's
+// arrivals (remote ones, even where the barrier is the CTA's own) are all waited for at the end of their roles.
 #include <math.h>
 
 #include <algorithm>
@@ -408,12 +410,13 @@ __global__ void __launch_bounds__(hd_threads(KIND), 1)
           }
         }
       }
-      // Every copy has landed before the CTA (or the pair, at its last barrier) ends: the last `used` ones, oldest
-      // first.
-      for (int j = used; rank == 0 && j > 0; --j) {
+      // Before the CTA ends, the products have freed the last `used` stages, oldest first: both CTAs' copies into them
+      // have then landed, and the commits' arrivals are here. Where products are missing after a wait that ran out,
+      // 0.2 s pass instead, for the copies in flight to land (those of rank 1 arrive at the leader's barrier).
+      for (int j = used; j > 0; --j) {
         const int s = (st - j + STAGES) % STAGES;
         const uint32_t p = s < st ? ph : ph ^ 1;
-        mbar_wait(full + s, p, err + 1, 2, 400000000LL);
+        mbar_wait(empty + s, p, err + 1, 2, 400000000LL);
       }
     }
     __syncwarp();
@@ -462,6 +465,9 @@ __global__ void __launch_bounds__(hd_threads(KIND), 1)
         if (ok) commit(acc_full + acc);
       }
       commit(done);
+      // The epilogue's arrivals for the last two tiles, which nothing else waits for.
+      for (int j = min(n, 2); j > 0; --j)
+        mbar_wait(acc_empty + ((n - j) & 1), ((n - j) >> 1) & 1, err, 7, 400000000LL);
     }
     __syncwarp();
   } else if (warp >= 4) {

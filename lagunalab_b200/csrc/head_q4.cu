@@ -213,9 +213,11 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
           }
         }
       }
+      // The products have freed the last slots before the CTA ends: their copies have landed, the commits have
+      // arrived. (After a wait that ran out, 0.2 s pass for the copies.)
       for (int j = used; j > 0; --j) {
         const int s = (st - j + AS) % AS;
-        mbar_wait(full + s, s < st ? ph : ph ^ 1, err + 2, 3, 400000000LL);
+        mbar_wait(empty + s, s < st ? ph : ph ^ 1, err + 2, 3, 400000000LL);
       }
     }
     __syncwarp();
