@@ -685,6 +685,8 @@ int lg_head_loss(const void* x, long long ldx, int T, int H, const void* w, long
  * dx or dw may be NULL (not both); a 4-bit head has no dw. A token without a target adds nothing to dw
  * and gives a row of zeros in dx, whatever its row of x holds; an id >= V counts as left out. dz is
  * rounded to bf16 for the tensor cores (2^-8 relative at most) without the factor max |g weights|, sums are fp32.
+ * A target that carries an eighth or more of its token's weight has its logit from the same fp32 sum as in lse:
+ * its S p - w is then off by lse's own rounding at most, also where it is nearly 0.
  */
 size_t lg_head_loss_grad_workspace_bytes(int T, int H, int V, int K, int bits, int dx, int dw);
 int lg_head_loss_grad(const void* x, long long ldx, int T, int H, const void* w, long long ldw,

@@ -19,6 +19,9 @@
 // dx and dW are multiplied by c before they are rounded, once, at the end. So the usual g (1/n for every token)
 // and weight leave S exp(z - lse) - 1, whose -1 is exact; as -g it was off by up to 2^-8, in all tokens by the
 // same, and dx and dW with it. The other errors are independent: sums over the vocabulary or the tokens average them.
+// z is the tensor cores' sum, which is cut after each step, but for targets that carry an eighth or more of their
+// token's weight: loss and gradient take both their logits from one fp32 sum (hd_dot), since a target's S p - w of
+// nearly 0 has all of z's error, and lse's with the other sign: what is left of it is lse's own rounding.
 //
 // Every mbarrier wait is bounded (tc::mbar_wait). A CTA whose wait ran out writes NaN for what is
 // left of its tiles, waits (bounded) for its copies and products in flight, frees its TMEM and ends.
@@ -71,15 +74,21 @@ struct HdArgs {
   const float* g;
   const float2* wsum;  // K > 1: [T] sum and largest size of the weights that count
   float* scale;        // HD_PROB, HD_WGRAD: c
+  const float* again;  // HD_PROB: [T, K] exp(z - lse) - 1 of targets summed again, HD_LIGHT elsewhere
   // not HD_LOSS: bf16 [M, width], HD_XGRAD and parts of HD_WGRAD: fp32 [splits, M, width]
   void* tile_out;
   int width;
   int add;  // HD_XGRAD: 0 for the first piece
 };
 
-__device__ __forceinline__ void hd_sub(float (&v)[32], int c, float w) {
+constexpr float HD_LIGHT = -2.f;  // exp(d) - 1 is never below -1
+
+// v[c], which is gs p, becomes gs p - w; p - 1 = `again` where that is given.
+__device__ __forceinline__ void hd_target(float (&v)[32], int c, float w, float gs, float again) {
+  const bool light = again == HD_LIGHT;
+  const float heavy = fmaf(gs, again, gs - w);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = i == c ? v[i] - w : v[i];
+  for (int i = 0; i < 32; ++i) v[i] = i == c ? (light ? v[i] - w : heavy) : v[i];
 }
 
 // Sixteen bf16 as one 32-byte store.
@@ -118,11 +127,12 @@ __device__ __forceinline__ HdUnit hd_unit(const HdArgs& a, int i) {
 struct HdRow {
   int p, p1, next;       // K > 1: sorted ids [p, p1) of the tile; the next id (K == 1: the id, of any tile)
   float w, gs, gg, off;  // its weight; HD_PROB: g S, g, -lse log2(e)
+  float again;           // HD_PROB: as in HdArgs
   bool counts;           // the token has a target
 };
 template <int KIND>
 __device__ __forceinline__ HdRow hd_row(const HdArgs& a, const HdUnit& u, int t) {
-  HdRow r = {0, 0, -1, 1.f, 0.f, 0.f, 0.f, false};
+  HdRow r = {0, 0, -1, 1.f, 0.f, 0.f, 0.f, HD_LIGHT, false};
   if (KIND > HD_PROB || t >= a.M) return r;
   const size_t row_k = (size_t)t * a.K;
   if (KIND == HD_PROB) {
@@ -134,6 +144,7 @@ __device__ __forceinline__ HdRow hd_row(const HdArgs& a, const HdUnit& u, int t)
     if (KIND == HD_PROB) {
       r.counts = r.next >= 0 && r.next < a.V;
       r.gs = a.weights ? a.g[t] * a.weights[t] / *a.scale : r.gg;
+      r.again = a.again[t];
     }
   } else {
     const unsigned char* st = a.start + (size_t)t * (a.nt_all + 1);
@@ -146,7 +157,10 @@ __device__ __forceinline__ HdRow hd_row(const HdArgs& a, const HdUnit& u, int t)
     }
     if (r.p < r.p1) {
       r.next = a.ids[row_k + r.p];
-      if (KIND == HD_PROB) r.w = a.weights[row_k + r.p];
+      if (KIND == HD_PROB) {
+        r.w = a.weights[row_k + r.p];
+        r.again = a.again[row_k + r.p];
+      }
     }
   }
   return r;
@@ -276,15 +290,16 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
           // K > 1: of the tile's ids in order, those of the other half of the columns only pass by
           while (a.K > 1 ? row.next >= 0 && row.next < id0 + 32 : (unsigned)row.next - (unsigned)id0 < 32u) {
             if (a.K == 1) {
-              hd_sub(v, row.next - id0, row.gs);
+              hd_target(v, row.next - id0, row.gs, row.gs, row.again);
               break;
             }
-            if (row.next >= id0) hd_sub(v, row.next - id0, row.gg * row.w);
+            if (row.next >= id0) hd_target(v, row.next - id0, row.gg * row.w, row.gs, row.again);
             const size_t at = (size_t)t * a.K + ++row.p;
             row.next = -1;
             if (row.p < row.p1) {
               row.next = a.ids[at];
               row.w = a.weights[at];
+              row.again = a.again[at];
             }
           }
           if (!row.counts) {  // a token without a target: nothing of it, whatever its row holds
@@ -587,13 +602,12 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
 
 constexpr int HJ_THREADS = 128;
 
-// sum_h x_h W_vh by a warp, in fp32 with each sum rounded to nearest.
-template <bool QUANT>
+// sum_h x_h W_vh by a warp, in fp32 with each sum rounded to nearest; the same bits for every U.
+template <bool QUANT, int U>
 __device__ __forceinline__ float hd_dot(const HdHead& w, const __nv_bfloat16* x, int H, int v) {
-  constexpr int U = 4;
   const int lane = threadIdx.x & 31;
   float s = 0.f;
-  for (int c0 = lane * 8; c0 < H; c0 += U * 256) {  // four chunks' loads before their sums
+  for (int c0 = lane * 8; c0 < H; c0 += U * 256) {  // U chunks' loads before their sums
     uint4 xv[U], wv[U];
     uint32_t q[U];
     uint16_t sc[U], bi[U];
@@ -627,6 +641,22 @@ __device__ __forceinline__ float hd_dot(const HdHead& w, const __nv_bfloat16* x,
     }
   }
   return warp_sum(s);
+}
+
+// Of a warp's targets, two a lane (id -1: none): those with an eighth or more of all weights, eight ids at most unless
+// all weights are 0.
+__device__ __forceinline__ unsigned long long hd_heavy(const int (&id)[2], const float (&wt)[2]) {
+  const float all = warp_sum(fabsf(wt[0]) + fabsf(wt[1]));
+  unsigned long long heavy = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    heavy |= (unsigned long long)__ballot_sync(0xffffffffu, id[i] >= 0 && 8.f * fabsf(wt[i]) >= all) << (32 * i);
+  return heavy;
+}
+// The targets that hold id v.
+__device__ __forceinline__ unsigned long long hd_same(const int (&id)[2], int v) {
+  return __ballot_sync(0xffffffffu, id[0] == v) |
+         (unsigned long long)__ballot_sync(0xffffffffu, id[1] == v) << 32;
 }
 
 // (maximum, sum of exponentials from it, the maximum's lowest id) of two parts, the first before the second.
@@ -686,25 +716,19 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
     const float2 v = row[n];
     st = hd_merge(st, {v.x, v.y, top ? in.top[(size_t)t * parts + n] : 0});
   }
-  const float all = warp_sum(fabsf(wt[0]) + fabsf(wt[1]));
   // The list of heavy targets, an id once: every warp has it, and sums its share.
-  unsigned long long todo = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    todo |= (unsigned long long)__ballot_sync(0xffffffffu, id[i] >= 0 && 8.f * fabsf(wt[i]) >= all) << (32 * i);
+  unsigned long long todo = hd_heavy(id, wt);
   const unsigned long long heavy = todo;
   int n = 0;
   while (todo) {
     const int j = __ffsll(todo) - 1;
     const int v = __shfl_sync(0xffffffffu, j < 32 ? id[0] : id[1], j & 31);
     if (n % WARPS == warp) {
-      const float d = hd_dot<QUANT>(w, x + (size_t)t * ldx, H, v);
+      const float d = hd_dot<QUANT, 4>(w, x + (size_t)t * ldx, H, v);
       if (lane == 0) sh_dot[n] = d;
     }
     ++n;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      todo &= ~((unsigned long long)__ballot_sync(0xffffffffu, id[i] == v) << (32 * i));
+    todo &= ~hd_same(id, v);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -725,10 +749,9 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
     const float was = __shfl_sync(0xffffffffu, j < 32 ? z[0] : z[1], j & 31), now = sh_dot[n];
     st.sum += hd_ex2((now - st.mx) * HD_LOG2E) - hd_ex2((was - st.mx) * HD_LOG2E);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2; ++i)
       if (id[i] == v) z[i] = now;  // every place of the list that names it
-      todo &= ~((unsigned long long)__ballot_sync(0xffffffffu, id[i] == v) << (32 * i));
-    }
+    todo &= ~hd_same(id, v);
   }
   const float lse = st.mx + logf(st.sum);
   float l = 0.f;
@@ -744,8 +767,9 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
   }
 }
 
-// c, the largest |g_t w_tj| that counts (1 if there is none above 0, or an infinite one), by a block of 256 threads
-// of a kernel that runs before the products anyway: it takes 3 us.
+// What HD_PROB needs besides z, by blocks of 256 threads of a kernel that runs before the products anyway: block 0
+// finds c, the largest |g_t w_tj| that counts (1 if there is none above 0, or an infinite one), in 3 us; the others
+// (hd_again) sum heavy targets' logits again.
 struct HdScale {
   const int* ids;
   const float *g, *weights;
@@ -753,6 +777,18 @@ struct HdScale {
   const float2* wsum;
   float* scale;  // NULL: not asked for
   int T, V, nt;
+  // hd_again
+  const __nv_bfloat16* x;
+  long long ldx;
+  int H, K;
+  HdHead w;
+  const int* sorted;  // K > 1: as in HdArgs
+  const float* sorted_w;
+  const float* lse;
+  float* again;
+
+  __host__ __device__ int warps() const { return K > 1 ? 4 : 1; }  // a token
+  __host__ __device__ int blocks() const { return scale ? 1 + (T + 8 / warps() - 1) / (8 / warps()) : 0; }
 };
 __device__ __forceinline__ bool hd_counts(const HdScale& a, int t) {
   return a.start ? a.start[(size_t)t * (a.nt + 1) + a.nt] > 0 : a.ids[t] >= 0 && a.ids[t] < a.V;
@@ -774,18 +810,64 @@ __device__ __forceinline__ void hd_scale(const HdScale& a) {
   }
 }
 
-// Block 0: c. The others, for dW: x with the rows of tokens without a target at 0, so that dW has nothing of them
-// (0 * NaN is NaN).
+// exp(z - lse) - 1 of a token's heavy targets, at the first of the places that name an id. Its warps take the targets in
+// turn (301 tokens of 5 targets, both gradients: 92.5 us with one warp a token, 90 with four).
+template <bool QUANT>
+__device__ __forceinline__ void hd_again(const HdScale& a, int block) {
+  const int lane = threadIdx.x & 31, warps = a.warps(), part = (threadIdx.x >> 5) % warps;
+  const int t = block * (8 / warps) + (threadIdx.x >> 5) / warps;
+  if (t >= a.T) return;
+  const bool many = a.start != nullptr;
+  const int n = many ? a.start[(size_t)t * (a.nt + 1) + a.nt] : 1;
+  int id[2];
+  float wt[2], again[2] = {HD_LIGHT, HD_LIGHT};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int j = lane + 32 * i;
+    const size_t at = (size_t)t * a.K + j;
+    id[i] = j < n ? (many ? a.sorted : a.ids)[at] : -1;
+    if (id[i] >= a.V) id[i] = -1;
+    wt[i] = id[i] < 0 ? 0.f : many ? a.sorted_w[at] : a.weights ? a.weights[at] : 1.f;
+  }
+  const float lse = a.lse[t];
+  bool mine[2] = {part == 0, part == 0};  // the places that this warp writes
+  int turn = 0;
+  for (unsigned long long todo = hd_heavy(id, wt); todo; ++turn) {
+    const int j = __ffsll(todo) - 1;
+    const int v = __shfl_sync(0xffffffffu, j < 32 ? id[0] : id[1], j & 31);
+    const unsigned long long same = hd_same(id, v);
+    const int first = __ffsll(same) - 1;
+    const bool own = turn % warps == part;
+    const float d = own ? expm1f(hd_dot<QUANT, QUANT ? 2 : 4>(a.w, a.x + (size_t)t * a.ldx, a.H, v) - lse) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (lane + 32 * i == first) {
+        again[i] = d;
+        mine[i] = own;
+      }
+    todo &= ~same;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (mine[i] && lane + 32 * i < a.K) a.again[(size_t)t * a.K + lane + 32 * i] = again[i];
+}
+
+// Blocks [0, a.blocks()): as HdScale says. The others, for dW: x with the rows of tokens without a target at 0, so
+// that dW has nothing of them (0 * NaN is NaN).
 __global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int H,
                                                       const HdScale a, __nv_bfloat16* __restrict__ out) {
   pdl_trigger();
-  if (blockIdx.x == 0) {
-    hd_scale(a);
+  const int first = a.blocks();
+  if ((int)blockIdx.x < first) {
+    if (blockIdx.x == 0)
+      hd_scale(a);
+    else
+      hd_again<false>(a, blockIdx.x - 1);
     return;
   }
   const int per = H / 8;
   const long long n = (long long)a.T * per;
-  for (long long i = (blockIdx.x - 1) * 256LL + threadIdx.x; i < n; i += (gridDim.x - 1) * 256LL) {
+  for (long long i = (blockIdx.x - first) * 256LL + threadIdx.x; i < n; i += (gridDim.x - first) * 256LL) {
     const int t = (int)(i / per), c = (int)(i % per) * 8;
     uint4 v = make_uint4(0, 0, 0, 0);
     if (hd_counts(a, t)) v = *reinterpret_cast<const uint4*>(x + (size_t)t * ldx + c);
@@ -794,15 +876,19 @@ __global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __res
 }
 
 // Rows of a 4-bit group-64 head as bf16: bf16(scale * code + bias), two words a thread: a warp writes 1 KB in one
-// store (four words a thread with 16-byte stores: 3 TB/s written instead of 4.3). Block 0 may have c to find instead.
-__global__ void __launch_bounds__(256) hd_dequant_kernel(const uint2* __restrict__ q,
-                                                         const uint16_t* __restrict__ s,
-                                                         const uint16_t* __restrict__ b, long long n,
-                                                         const HdScale a, __nv_bfloat16* __restrict__ out) {
+// store (four words a thread with 16-byte stores: 3 TB/s written instead of 4.3). Blocks [0, a.blocks()): as HdScale
+// says; they take two chunks of hd_dot at a time, which leaves 48 registers.
+__global__ void __launch_bounds__(256, 5) hd_dequant_kernel(const uint2* __restrict__ q,
+                                                            const uint16_t* __restrict__ s,
+                                                            const uint16_t* __restrict__ b, long long n,
+                                                            const HdScale a, __nv_bfloat16* __restrict__ out) {
   pdl_trigger();
-  const int first = a.scale != nullptr;  // of the blocks that unpack
-  if (first && blockIdx.x == 0) {
-    hd_scale(a);
+  const int first = a.blocks();  // of the blocks that unpack
+  if ((int)blockIdx.x < first) {
+    if (blockIdx.x == 0)
+      hd_scale(a);
+    else
+      hd_again<true>(a, blockIdx.x - 1);
     return;
   }
   constexpr int U = 4;
@@ -950,7 +1036,7 @@ struct HdWork {
   unsigned char *order, *start;
   float* sorted_w;
   float2* wsum;
-  float* scale;
+  float *scale, *again;
   __nv_bfloat16 *wq, *dz, *xz;
   float *dx, *dw;  // fp32 parts (dw: NULL where it has one)
   size_t bytes;
@@ -985,6 +1071,7 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
   if (quant) w.wq = c.take<__nv_bfloat16>((size_t)std::min(w.piece, V) * H);
   if (grad) {
     w.scale = c.take<float>(1);
+    w.again = c.take<float>((size_t)T * K);
     w.dz = c.take<__nv_bfloat16>((size_t)T * w.piece);
     if (dw) {
       w.xz = c.take<__nv_bfloat16>((size_t)T * H);
@@ -1093,7 +1180,7 @@ static int hd_weights(const void* w, const void* ws, const void* wb, int H, int 
   if (!ws) return LG_OK;
   const long long n = (long long)rows * (H / 16);
   const size_t at = (size_t)v0 * (H / 16);
-  hd_dequant_kernel<<<hd_blocks(n) + (scale.scale != nullptr), 256, 0, st>>>(
+  hd_dequant_kernel<<<hd_blocks(n) + scale.blocks(), 256, 0, st>>>(
       static_cast<const uint2*>(w) + at, static_cast<const uint16_t*>(ws) + at / 4,
       static_cast<const uint16_t*>(wb) + at / 4, n, scale, k.wq);
   LG_LAUNCH_CHECK("head_dequant");
@@ -1212,9 +1299,12 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     return fail(LG_ERR_WORKSPACE, "head_loss_grad: workspace of %zu bytes, need %zu", workspace_bytes,
                 k.bytes);
   HD_TRY(hd_sort(ids, weights, T, K, V, k, st));
-  const HdScale scale = {ids, g, weights, k.start, k.wsum, k.scale, T, V, k.nt};
+  const HdHead head = {w, static_cast<const __nv_bfloat16*>(w_scales),
+                       static_cast<const __nv_bfloat16*>(w_biases), ldw};
+  const HdScale scale = {ids, g, weights, k.start, k.wsum, k.scale, T, V, k.nt,
+                         static_cast<const __nv_bfloat16*>(x), ldx, H, K, head, k.sorted, k.sorted_w, lse, k.again};
   if (!quant) {
-    hd_rows_kernel<<<1 + (dw ? hd_blocks((long long)T * (H / 8)) : 0), 256, 0, st>>>(
+    hd_rows_kernel<<<scale.blocks() + (dw ? hd_blocks((long long)T * (H / 8)) : 0), 256, 0, st>>>(
         static_cast<const __nv_bfloat16*>(x), ldx, H, scale, k.xz);
     LG_LAUNCH_CHECK("head_rows");
   }
@@ -1231,6 +1321,7 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     a.g = g;
     a.wsum = k.wsum;
     a.scale = k.scale;
+    a.again = k.again;
     const int ldz = (n + 63) / 64 * 64;
     a.tile_out = k.dz;
     a.width = ldz;
