@@ -63,7 +63,7 @@ struct HdArgs {
   int V;
   int K;             // targets a token
   const int* ids;    // [T, K]; K > 1: sorted (with `order`, `start`)
-  const float* weights;        // [T, K] or NULL; K > 1: by sorted id
+  const float* weights;        // [T, K] or NULL; K > 1: by sorted id, times hd_up
   const unsigned char* order;  // K > 1: [T, K] the caller's index of a sorted id
   const unsigned char* start;  // K > 1: [T, nt_all + 1] first sorted id of each vocabulary tile
   int nt_all;
@@ -72,7 +72,7 @@ struct HdArgs {
   // HD_PROB
   const float* lse;
   const float* g;
-  const float2* wsum;  // K > 1: [T] sum and largest size of the weights that count
+  const float2* wsum;  // K > 1: [T] sum (times hd_up) and largest size of the weights that count
   float* scale;        // HD_PROB, HD_WGRAD: c
   const float* again;  // HD_PROB: [T, K] exp(z - lse) - 1 of targets summed again, HD_LIGHT elsewhere
   // not HD_LOSS: bf16 [M, width], HD_XGRAD and parts of HD_WGRAD: fp32 [splits, M, width]
@@ -80,6 +80,10 @@ struct HdArgs {
   int width;
   int add;  // HD_XGRAD: 0 for the first piece
 };
+
+// K > 1: what a token's weights are multiplied with, and its g divided by, by its largest weight. g / c is at most
+// 1 / largest, which overflows below 2^-128.
+__device__ __forceinline__ float hd_up(float largest) { return largest < 0x1p-100f ? 0x1p60f : 1.f; }
 
 constexpr float HD_LIGHT = -2.f;  // exp(d) - 1 is never below -1
 
@@ -136,7 +140,12 @@ __device__ __forceinline__ HdRow hd_row(const HdArgs& a, const HdUnit& u, int t)
   if (KIND > HD_PROB || t >= a.M) return r;
   const size_t row_k = (size_t)t * a.K;
   if (KIND == HD_PROB) {
-    r.gg = a.g[t] / *a.scale;
+    r.gg = a.g[t];
+    if (a.K > 1) {
+      const float big = a.wsum[t].y;  // 0: all weights are, and g may be any size above c
+      r.gg = big > 0.f ? r.gg / hd_up(big) : r.gg * 0.f;
+    }
+    r.gg /= *a.scale;
     r.off = -a.lse[t] * HD_LOG2E;
   }
   if (a.K == 1) {
@@ -572,6 +581,7 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
   }
   sum = warp_sum(sum);
   big = warp_max(big);
+  const float times = hd_up(big);
   __syncwarp();
   int* up = sh[warp] + HD_MAXK;  // ascending
   up[lane] = up[lane + 32] = 0x7fffffff;
@@ -585,7 +595,7 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
     up[rank] = id;
     sorted[(size_t)t * K + rank] = id;
     order[(size_t)t * K + rank] = (unsigned char)j;
-    sorted_w[(size_t)t * K + rank] = weights ? weights[(size_t)t * K + j] : 1.f;
+    sorted_w[(size_t)t * K + rank] = (weights ? weights[(size_t)t * K + j] : 1.f) * times;
   }
   __syncwarp();
   for (int n = lane; n <= nt; n += 32) {  // ids below the tile's first; n = nt: all that count
@@ -597,7 +607,7 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
     if (up[c] < lim) ++c;
     start[(size_t)t * (nt + 1) + n] = (unsigned char)c;
   }
-  if (lane == 0) wsum[t] = make_float2(sum, big);
+  if (lane == 0) wsum[t] = make_float2(sum * times, big);
 }
 
 constexpr int HJ_THREADS = 128;
