@@ -653,14 +653,15 @@ __device__ __forceinline__ float hd_dot(const HdHead& w, const __nv_bfloat16* x,
   return warp_sum(s);
 }
 
-// Of a warp's targets, two a lane (id -1: none): those with an eighth or more of all weights, eight ids at most unless
-// all weights are 0.
+// Of a warp's targets, two a lane (id -1: none): those with an eighth or more of all weights, eight ids at most. None
+// where all weights are 0.
 __device__ __forceinline__ unsigned long long hd_heavy(const int (&id)[2], const float (&wt)[2]) {
   const float all = warp_sum(fabsf(wt[0]) + fabsf(wt[1]));
   unsigned long long heavy = 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    heavy |= (unsigned long long)__ballot_sync(0xffffffffu, id[i] >= 0 && 8.f * fabsf(wt[i]) >= all) << (32 * i);
+    heavy |= (unsigned long long)__ballot_sync(0xffffffffu, id[i] >= 0 && all > 0.f && 8.f * fabsf(wt[i]) >= all)
+             << (32 * i);
   return heavy;
 }
 // The targets that hold id v.
