@@ -1167,7 +1167,8 @@ static int hd_launch(const HdOperand& a, const HdOperand& b, HdArgs g, bool earl
 
 static int hd_check(const char* who, const void* x, long long ldx, int T, int H, const void* w,
                     long long ldw, const void* ws, const void* wb, int V, const int* ids, int K) {
-  LG_CHECK_ARG(T >= 0 && V >= 1 && V <= (1 << 30), "%s: T=%d V=%d", who, T, V);
+  // tokens rounded up to whole tiles stay below 2^31
+  LG_CHECK_ARG(T >= 0 && T < 0x7fffffff - 1024 && V >= 1 && V <= (1 << 30), "%s: T=%d V=%d", who, T, V);
   LG_CHECK_ARG(K >= 1 && K <= HD_MAXK, "%s: K=%d targets not in [1, %d]", who, K, HD_MAXK);
   LG_CHECK_ARG((ws == nullptr) == (wb == nullptr), "%s: scales and biases go together", who);
   const int unit = ws ? 64 : 8;
