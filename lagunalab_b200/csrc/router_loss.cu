@@ -9,6 +9,9 @@
 //   ds_j = (dw_j - sum_i dw_i w_i) / sum s (norm) or dw_j;  a sigmoid's or softmax's backward from there.
 // Such differences from a mean are taken of values less that of the largest share: where one share is nearly 1 (or the
 // only one: k = 1 with norm), its value and the mean are nearly the same number, and their roundings would be the result.
+// Shares are quotients: where a token's scores (or its picks') are all below 2^-80, down to 0 in fp32, they are taken
+// again relative to exp of the largest logit (rb_faint). Gradients are sums of shares times differences, so that
+// no score is divided by alone.
 //
 // A token is worked on by G = 8, 16 or 32 lanes (E up to 64, 128, 256), eight scores a lane, so that a reduction's
 // shuffles serve 32 / G tokens at once: with a warp a token the gradient of 32,768 tokens of 64 experts took 254
@@ -76,17 +79,35 @@ __device__ __forceinline__ void rb_load(float (&v)[RB_N], const float* row, int 
   }
 }
 
-__device__ __forceinline__ float rb_sigmoid(float x, float* tail) {  // tail: s (1 - s), without the difference
+__device__ __forceinline__ float rb_sigmoid(float x, float* rest) {  // rest: 1 - s, without the difference
   const float t = rb_exp(-fabsf(x));                                 // NaN stays
   const float r = rb_rcp(1.f + t);
-  *tail = t * r * r;
+  *rest = x >= 0.f ? t * r : r;
   return x >= 0.f ? r : t * r;
 }
 
-// The token's scores in place of its logits (-inf past E gives 0). A sigmoid: their sum; softmax: 1, with what one
-// more logit's score takes (the maximum, and the reciprocal of the sum).
+// Sums of scores below this are taken again. Above it, what fp32 leaves out of a sum (scores below 2^-126) is nothing.
+constexpr float RB_FAINT = 0x1p-80f;
+
+// exp(v - the largest v) in place of logits far below 0, where a sigmoid is exp(v); their sum.
 template <int G>
-__device__ __forceinline__ float rb_scores(float (&v)[RB_N], float (&tail)[RB_N], int score_fn, float* mx,
+__device__ __forceinline__ float rb_faint(float (&v)[RB_N]) {
+  float m = v[0], sum = 0.f;
+#pragma unroll
+  for (int j = 1; j < RB_N; ++j) m = fmaxf(m, v[j]);
+  m = rb_max<G>(m);
+#pragma unroll
+  for (int j = 0; j < RB_N; ++j) {
+    v[j] = rb_exp(v[j] - m);
+    sum += v[j];
+  }
+  return rb_sum<G>(sum);
+}
+
+// The token's scores in place of its logits (-inf past E gives 0). A sigmoid: their sum, and 1 - s of each; softmax: 1,
+// with what one more logit's score takes (the maximum, and the reciprocal of the sum).
+template <int G>
+__device__ __forceinline__ float rb_scores(float (&v)[RB_N], float (&rest)[RB_N], int score_fn, float* mx,
                                            float* rs) {
   float sum = 0.f;
   if (score_fn == LG_SCORE_SOFTMAX) {
@@ -108,10 +129,24 @@ __device__ __forceinline__ float rb_scores(float (&v)[RB_N], float (&tail)[RB_N]
   }
 #pragma unroll
   for (int j = 0; j < RB_N; ++j) {
-    v[j] = rb_sigmoid(v[j], &tail[j]);
+    v[j] = rb_sigmoid(v[j], &rest[j]);
     sum += v[j];
   }
   return rb_sum<G>(sum);
+}
+
+// rb_scores' sigmoids and their sum once more for a token whose sum is faint. Called by whole warps.
+template <int G, bool VEC>
+__device__ __forceinline__ void rb_again(float (&v)[RB_N], float& total, const float* row, int E, bool keep) {
+  const bool faint = keep && total < RB_FAINT;
+  if (!__any_sync(0xffffffffu, faint)) return;
+  float z[RB_N];
+  rb_load<G, VEC>(z, row, E, faint);
+  const float sum = rb_faint<G>(z);
+  if (!faint) return;
+  total = sum;
+#pragma unroll
+  for (int j = 0; j < RB_N; ++j) v[j] = z[j];
 }
 
 // `v` of the first lane of this token's G that holds `mine` (of its lane 0 if none does).
@@ -191,7 +226,9 @@ __global__ void __launch_bounds__(RB_WARPS * 32) router_balance_kernel(
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (keep[u] && pick[u] >= 0 && pick[u] < E) atomicAdd(&hist[pick[u]], 1);
-      const float r = rb_rcp(rb_scores<G>(v[u], unused, score_fn, &mx, &rs));
+      float total = rb_scores<G>(v[u], unused, score_fn, &mx, &rs);
+      rb_again<G, VEC>(v[u], total, logits + (size_t)(t0 + u * step + lane / G) * E, E, keep[u]);
+      const float r = rb_rcp(total);
       if (keep[u]) {
         ++kept;
 #pragma unroll
@@ -293,7 +330,7 @@ struct RgArgs {
 template <int G, bool VEC>
 __global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs a) {
   constexpr int PER = 32 / G;
-  __shared__ float sh_d[RG_WARPS * PER][G * RB_N];          // a token's picks' gradients; zeros between tokens
+  __shared__ float sh_d[RG_WARPS * PER][G * RB_N];          // a token's picks' parts; zeros between tokens
   __shared__ unsigned char sh_t[RG_WARPS * PER][G * RB_N];  // which pick has an expert
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % G;
   float* sd = sh_d[warp * PER + lane / G];
@@ -326,7 +363,7 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs
     const int t = t0 + lane / G;
     const bool in = t < a.T;
     const float* row = a.logits + (size_t)t * a.E;
-    float s[RB_N], tail[RB_N], mx = 0.f, rs = 0.f;
+    float s[RB_N], rest[RB_N], mx = 0.f, rs = 0.f;
     rb_load<G, VEC>(s, row, a.E, in);
     int id = -1;
     float d = 0.f;
@@ -336,22 +373,37 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs
     }
     const bool keep = in && (!a.mask || a.mask[t]);
     if (!keep || id >= a.E) id = -1;
-    const float x = id >= 0 ? __ldg(row + id) : 0.f;
-    const float total = rb_scores<G>(s, tail, a.score_fn, &mx, &rs);
+    const float x = id >= 0 ? __ldg(row + id) : -INFINITY;
+    float total = rb_scores<G>(s, rest, a.score_fn, &mx, &rs);
+    rb_again<G, VEC>(s, total, row, a.E, keep && a.counts);
     const bool softmax = a.score_fn == LG_SCORE_SOFTMAX;
+    // What goes through the shares: h - sum q h. (A softmax's gradient of weights with norm sums to 0 by itself.)
+    const bool through = softmax && a.dw && !a.norm;
     if (a.dw) {
       float unused;
-      const float p = id < 0 ? 0.f : softmax ? rb_exp(x - mx) * rs : rb_sigmoid(x, &unused);
+      float p = id < 0 ? 0.f : softmax ? rb_exp(x - mx) * rs : rb_sigmoid(x, &unused);
       if (id >= 0) st[id] = (unsigned char)l;
       if (a.norm) {
+        float sum = rb_sum<G>(p);
+        const bool faint = id >= 0 && sum < RB_FAINT;
+        if (__any_sync(0xffffffffu, faint)) {
+          const float m = rb_max<G>(x);
+          const float e = id < 0 ? 0.f : rb_exp(x - m), all = rb_sum<G>(e);
+          if (faint) {
+            p = e;
+            sum = all;
+          }
+        }
         const float top = rb_max<G>(p);
         d -= rb_first<G>(id >= 0 && p == top, d);
-        const float dot = rb_sum<G>(id >= 0 ? d * p : 0.f), r = rb_rcp(rb_sum<G>(p));
-        d = (d - dot * r) * r;
+        const float dot = rb_sum<G>(id >= 0 ? d * p : 0.f), r = rb_rcp(sum);
+        d = (d - dot * r) * (p * r);
+      } else if (!softmax) {
+        d *= p;
       }
       __syncwarp();
       const bool twice = id >= 0 && st[id] != l;
-      if (__any_sync(0xffffffffu, twice)) {  // an expert picked twice: its gradients in their order
+      if (__any_sync(0xffffffffu, twice)) {  // an expert picked twice: its parts in their order
         for (int j = 0; j < a.k; ++j) {
           if (l == j && id >= 0) sd[id] += d;
           __syncwarp();
@@ -361,9 +413,7 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs
       }
       __syncwarp();
     }
-    // What goes through the shares: h - sum q h. (A softmax's gradient of weights with norm sums to 0 by itself.)
-    const bool through = softmax && a.dw && !a.norm;
-    const float r = rb_rcp(total);
+    const float r = a.counts ? rb_rcp(total) : 1.f;  // softmax: 1
     float h[RB_N];
 #pragma unroll
     for (int j = 0; j < RB_N; ++j) {
@@ -391,8 +441,9 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_grad_kernel(const RgArgs
 #pragma unroll
     for (int j = 0; j < RB_N; ++j) {
       const int e = rb_expert<G, VEC>(j);
-      const float ds = a.dw && !through && e < a.E ? sd[e] : 0.f;
-      s[j] = keep ? softmax ? s[j] * (ds + h[j]) : tail[j] * fmaf(h[j], r, ds) : 0.f;
+      const float part = a.dw && !through && e < a.E ? sd[e] : 0.f;
+      const float g = a.counts || through ? fmaf(s[j] * r, h[j], part) : part;
+      s[j] = keep ? softmax ? g : rest[j] * g : 0.f;
     }
     if (in) {
       float* out = a.dl + (size_t)t * a.E;
