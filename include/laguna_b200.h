@@ -695,6 +695,14 @@ int lg_head_loss_grad(const void* x, long long ldx, int T, int H, const void* w,
                       void* dw, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * The first wait of the head's product kernels on the current device that ran out (each ends after some seconds, and
+ * its call's results hold NaN where they are not right): 0, or kernel << 8 | wait, with kernel 1 for the loss,
+ * 2 dz, 3 dx, 4 dw, 5 the loss from 4-bit codes. Synchronous with the default stream; the caller has waited for others.
+ * reset != 0 clears it.
+ */
+int lg_head_status(int* status, int reset);
+
+/*
  * The router's balance loss with its counts. logits fp32 [T, E] and inds int32 [T, k] as lg_router_topk
  * gives them (a pick outside [0, E) does not count); mask (bytes [T] or NULL: all) keeps a token where it
  * is not 0, whatever the others' logits hold. With scores s = sigmoid or softmax of the logits and the

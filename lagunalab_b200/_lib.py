@@ -116,6 +116,7 @@ SIGNATURES = {
     "lg_head_loss_grad_workspace_bytes": (c_size_t, [I, I, I, I, I, I, I]),
     "lg_head_loss_grad": (c_int, [P, c_longlong, I, I, P, c_longlong, P, P, I, P, P, I, P, P, P, P,
                                   P, c_size_t, P]),
+    "lg_head_status": (c_int, [ctypes.POINTER(c_int), c_int]),
     "lg_router_balance_workspace_bytes": (c_size_t, [I, I]),
     "lg_router_balance": (c_int, [P, P, P, I, I, I, I, P, P, P, P, P, c_size_t, P]),
     "lg_router_grad": (c_int, [P, P, P, P, I, I, I, I, I, P, P, c_float, P, P]),

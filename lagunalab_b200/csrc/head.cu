@@ -24,7 +24,8 @@
 // nearly 0 has all of z's error, and lse's with the other sign: what is left of it is lse's own rounding.
 //
 // Every mbarrier wait is bounded (tc::mbar_wait). A CTA whose wait ran out writes NaN for what is
-// left of its tiles, waits (bounded) for its copies and products in flight, frees its TMEM and ends.
+// left of its tiles (zeros stay in dz for tokens without a target, and the ids of largest logits have no mark), waits
+// (bounded) for its copies and products in flight, frees its TMEM, records its code for lg_head_status and ends.
 // Nothing asynchronous outlives the CTA that it writes to: copies, the commits that free a stage, and the epilogue's
 // arrivals (remote ones, even where the barrier is the CTA's own) are all waited for at the end of their roles.
 #include <math.h>
@@ -536,6 +537,7 @@ __global__ void __launch_bounds__(hd_threads(KIND), 1)
     else
       tmem_dealloc(tmem, 512);
   }
+  if (threadIdx.x == 0 && (err[0] || err[1] || err[2])) hd_record(1 + KIND, err[0] ? err[0] : err[1] ? err[1] : err[2]);
 }
 
 // The eight weights of a word, in their order, from the bf16 bits of scale and bias.
@@ -1241,6 +1243,19 @@ extern "C" size_t lg_head_loss_workspace_bytes(int T, int H, int V, int K, int b
 extern "C" size_t lg_head_loss_grad_workspace_bytes(int T, int H, int V, int K, int bits, int dx, int dw) {
   if (T < 1 || H < 8 || V < 1 || K < 1) return 256;
   return hd_carve(nullptr, T, H, V, K, bits == 4, false, true, dx != 0, dw != 0, false).bytes;
+}
+
+extern "C" int lg_head_status(int* status, int reset) {
+  LG_CHECK_ARG(status, "head_status: NULL pointer");
+  int here = 0, q4 = 0;
+  LG_CUDA_TRY(cudaMemcpyFromSymbol(&here, hd_status_word, sizeof(int)));
+  HD_TRY(hq_status(&q4, reset));
+  if (reset) {
+    const int zero = 0;
+    LG_CUDA_TRY(cudaMemcpyToSymbol(hd_status_word, &zero, sizeof(int)));
+  }
+  *status = here ? here : q4;
+  return LG_OK;
 }
 
 extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const void* w, long long ldw,

@@ -80,11 +80,16 @@ struct HdParts {
   int parts;
 };
 
+// The first wait of a source file's kernels that ran out: kernel << 8 | code of the wait (lg_head_status).
+static __device__ int hd_status_word;
+__device__ __forceinline__ void hd_record(int kernel, int code) { atomicCAS(&hd_status_word, 0, kernel << 8 | code); }
+
 // head_q4.cu: the loss's parts from a 4-bit head for few tokens, without the bf16 weights in memory: up to HQ_MAXT
 // tokens a pass over the weights. xp: T H bf16, idt: HQ_MAXT K ints of workspace. Taken for up to
 // HQ_PASSES passes, where that is faster than the products of head.cu over unpacked weights.
 constexpr int HQ_MAXT = 128, HQ_PASSES = 3;
 int hq_parts(int V);
+int hq_status(int* status, int reset);
 int hq_loss_parts(const __nv_bfloat16* x, long long ldx, int T, int H, const HdHead& w, int V, const int* ids,
                   int K, __nv_bfloat16* xp, int* idt, const HdParts& out, cudaStream_t st);
 

@@ -464,6 +464,8 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   if (warp == 3) tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0 && (err[0] || err[1] || err[2] || err[3]))
+    hd_record(5, err[0] ? err[0] : err[1] ? err[1] : err[2] ? err[2] : err[3]);
   // The four warps' parts, in their order.
   if (threadIdx.x < a.T) {
     const int t = threadIdx.x;
@@ -519,6 +521,13 @@ static size_t hq_layout(int T, int H, HqArgs* a) {
   for (a->ws = 8; a->ws > 4 && fixed + (size_t)a->ws * HQ_W_BYTES > HQ_SMEM_MAX; a->ws -= 2) {
   }
   return fixed + (size_t)a->ws * HQ_W_BYTES;
+}
+
+int hq_status(int* status, int reset) {
+  LG_CUDA_TRY(cudaMemcpyFromSymbol(status, hd_status_word, sizeof(int)));
+  const int zero = 0;
+  if (reset) LG_CUDA_TRY(cudaMemcpyToSymbol(hd_status_word, &zero, sizeof(int)));
+  return LG_OK;
 }
 
 int hq_parts(int V) { return std::min(device_sm_count(), (V + HQ_BLOCK - 1) / HQ_BLOCK); }

@@ -1045,6 +1045,16 @@ def head_loss_grad(x, head, ids, lse, g, weights=None, dx=True, dw=True):
     return gx, gw
 
 
+def head_status(device=None, reset=True):
+    """0, or which wait of ``head_loss``'s and ``head_loss_grad``'s product kernels on ``device`` (default: the current
+    one) was the first to run out (``lg_head_status``); the results of its call hold NaN. Waits for the device."""
+    with torch.cuda.device(device):
+        torch.cuda.synchronize()
+        st = ctypes.c_int(0)
+        _lib.call("lg_head_status", ctypes.byref(st), int(bool(reset)))
+    return st.value
+
+
 class RouterBalance(NamedTuple):
     """``router_balance``'s results, on the device."""
     loss: torch.Tensor    # fp32 [1]
