@@ -687,6 +687,8 @@ int lg_head_loss(const void* x, long long ldx, int T, int H, const void* w, long
  * rounded to bf16 for the tensor cores (2^-8 relative at most) without the factor max |g weights|, sums are fp32.
  * A target that carries an eighth or more of its token's weight has its logit from the same fp32 sum as in lse:
  * its S p - w is then off by lse's own rounding at most, also where it is nearly 0.
+ * The workspace holds up to 512 MB of dz (256 ids a token at least: more from 2^20 tokens on), up to 512 MB of a 4-bit
+ * head's rows in bf16, fp32 parts of dx (up to 8, or 20 MB) and of dw (20 MB), and for dw a copy of x.
  */
 size_t lg_head_loss_grad_workspace_bytes(int T, int H, int V, int K, int bits, int dx, int dw);
 int lg_head_loss_grad(const void* x, long long ldx, int T, int H, const void* w, long long ldw,
@@ -709,8 +711,10 @@ int lg_head_status(int* status, int reset);
  * N tokens kept:
  *   counts[e] = picks of e,  probs[e] = mean over tokens of s[t, e] / sum_e s[t, e],
  *   loss[0] = E sum_e counts[e] / (sum counts) probs[e],  tokens[0] = N;
- * all 0 where no token is kept. E <= 256, k <= 32. Sums are fp32, in an order that depends on T alone. A short
- * batch needs no workspace (0 bytes: NULL is taken).
+ * all 0 where no token is kept. E <= 256, k <= 32. E is the number of columns: an expert that cannot be picked
+ * still has its share, unless its logits are -inf; even routing over n experts then gives E / n. Sums are fp32, in an
+ * order that depends on T, E, k and the logits' address (16-byte aligned or not) alone. A short batch needs no
+ * workspace (0 bytes: NULL is taken).
  */
 size_t lg_router_balance_workspace_bytes(int T, int E);
 int lg_router_balance(const float* logits, const int32_t* inds, const uint8_t* mask, int T, int E,

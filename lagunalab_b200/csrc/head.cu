@@ -1151,10 +1151,12 @@ struct HdOperand {
 
 // One CTA a tile where the output has no more than 128 rows, else a pair.
 //
-// `early`: it may start under the kernel before it, one of this call's that says so (pdl_trigger) and whose CTAs have
-// room beside an hd_kernel's on an SM (next to no shared memory of their own). Nothing else is launched early: where a
-// kernel's CTAs are not all on the GPU yet, waiting CTAs of a later one can take their SMs and wait for them
-// for ever. (It happened behind hd_kernel, some of whose pairs had to wait for the dequantization's CTAs.)
+// `early`: it may start under the kernel before it, one of this call's small ones, which call pdl_trigger in their first
+// instruction: the early kernel starts when every CTA before has called it, so that all of them are on the GPU by then
+// and end without an SM that the early one's waiting CTAs have taken. (Those leave no room on an SM: 384 threads of
+// 168 registers, 225 KB.) A trigger stays a kernel's first instruction, and nothing starts early behind an hd_kernel,
+// whose CTAs wait in pdl_wait first: some of its pairs may still wait for SMs, which CTAs of a later kernel that wait
+// for them could take for ever. (It happened.)
 template <int KIND>
 static int hd_launch(const HdOperand& a, const HdOperand& b, HdArgs g, bool early, cudaStream_t st) {
   constexpr bool A_MN = KIND == HD_WGRAD, B_MN = KIND == HD_XGRAD || KIND == HD_WGRAD;

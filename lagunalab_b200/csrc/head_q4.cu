@@ -20,9 +20,10 @@
 // K order: one LOP3 splits a word into the pairs (0,4), (1,5), (2,6), (3,7); x is copied in that order first
 // (hq_order_kernel), so that no code is moved.
 //
-// Each CTA has 1/148 of the blocks of 32 ids. HBM needs 0.56 bytes a weight; what bounds it are the unpacking
-// warps' instructions. 37 tokens, 100,352 ids of 2,048: 48 us a call with the order and the join (40 this kernel: 116 MB,
-// 2.9 TB/s; an instruction issued in 54 % of the cycles, the tensor pipe busy in 24 %).
+// Each CTA has 1/148 of the blocks of 32 ids. HBM needs 0.56 bytes a weight. 37 tokens, 100,352 ids of 2,048: 48 us a
+// call with the order and the join (40 this kernel: 116 MB, 2.9 TB/s). No pipe is near its limit then (HBM 31 %, an
+// instruction issued in 54 % of the cycles, a third of those unpacking at nine a word, the tensor pipe busy in 24 %):
+// the roles wait for one another. A part of it: 21 or 22 blocks a CTA are six tiles of four, 5.3 of them full.
 #include <math.h>
 
 #include <algorithm>

@@ -8,7 +8,8 @@
 // Routing weights w_j = s_j / sum over the token's picks of s (norm) or s_j, for dw given:
 //   ds_j = (dw_j - sum_i dw_i w_i) / sum s (norm) or dw_j;  a sigmoid's or softmax's backward from there.
 // Such differences from a mean are taken of values less that of the largest share: where one share is nearly 1 (or the
-// only one: k = 1 with norm), its value and the mean are nearly the same number, and their roundings would be the result.
+// only one: k = 1 with norm), its value and the mean are nearly the same number, and their roundings would be the
+// result.
 // Shares are quotients: where a token's scores (or its picks') are all below 2^-80, down to 0 in fp32, they are taken
 // again relative to exp of the largest logit (rb_faint). Gradients are sums of shares times differences, so that
 // no score is divided by alone.
@@ -16,8 +17,8 @@
 // A token is worked on by G = 8, 16 or 32 lanes (E up to 64, 128, 256), eight scores a lane, so that a reduction's
 // shuffles serve 32 / G tokens at once: with a warp a token the gradient of 32,768 tokens of 64 experts took 254
 // instructions a token and 14 us. Both kernels read the logits once; the bound is HBM on long batches, launch
-// latency on short ones. 32,768 tokens: balance of 128 experts 15 to 17 us (17 MB: 8 for the sums, 5 for their join,
-// the rest between them), gradient of 64 experts 8 to 10 us (19 MB); 64 tokens 6 us, 4,096 tokens' gradient 4 us.
+// latency on short ones. 32,768 tokens: balance of 128 experts 11 to 17 us (17 MB: 8 for the sums, 5 for their join,
+// the rest between them), gradient of 64 experts 7 to 11 us (19 MB); 64 tokens 5 to 7 us, 4,096 tokens' gradient 4 us.
 #include <math.h>
 
 #include <algorithm>

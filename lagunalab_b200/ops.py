@@ -1020,8 +1020,9 @@ def head_loss(x, head, ids, weights=None, top=False):
 def head_loss_grad(x, head, ids, lse, g, weights=None, dx=True, dw=True):
     """The gradient of sum(g * loss) for ``head_loss``'s loss, from the same x, head, ids and weights, its
     ``lse`` and g fp32 [T]: (dx bf16 [T, H] or None, dw bf16 [V, H] or None). A 4-bit head has no
-    gradient (``dw=False``). The vocabulary is taken in pieces: the workspace holds at most 512 MB of
-    the logits' gradient, and of a 4-bit head's weights. Ids that are negative or >= V are left out; tokens
+    gradient (``dw=False``). The vocabulary is taken in pieces: the workspace holds up to 512 MB of
+    the logits' gradient (256 ids a token at least: more from 2^20 tokens on) and of a 4-bit head's weights, and
+    fp32 parts of dx (up to eight, or 20 MB). Ids that are negative or >= V are left out; tokens
     without any other give a row of zeros in dx and nothing to dw, whatever their rows of x hold. The
     logits' gradient, without the factor that all tokens share, is rounded to bf16 for the tensor cores;
     sums are fp32, results rounded once."""
@@ -1089,8 +1090,10 @@ def _router_args(who, logits, inds, score_fn, mask):
 def router_balance(logits, inds, score_fn="sigmoid", mask=None):
     """The balance loss of a batch's routing and its per-expert counts, from ``router_topk``'s logits fp32
     [T, E] and picks int32 [T, k]: ``E * sum(share of picks * mean share of scores)``, 1 where
-    both are even, over the tokens that ``mask`` (bool [T]) keeps; what masked rows hold does not matter. Returns a
-    ``RouterBalance``; its gradient is ``router_grad``'s, through the scores (counts have none)."""
+    both are even, over the tokens that ``mask`` (bool [T]) keeps; what masked rows hold does not matter. Experts that a
+    bias of -inf rules out still have their shares: set their logits to -inf as well; E stays, so that even routing over
+    n of them gives E / n. Returns a ``RouterBalance``; its gradient is ``router_grad``'s, through the scores (counts
+    have none)."""
     index, T, E, k, logits, inds, mask = _router_args("router_balance", logits, inds, score_fn, mask)
     loss, probs, counts, tokens = logits.new_empty(1), logits.new_empty(E), inds.new_empty(E), inds.new_empty(1)
     nb = _on_index(index, "lg_router_balance_workspace_bytes", T, E)
