@@ -795,8 +795,6 @@ struct HdScale {
   long long ldx;
   int H, K;
   HdHead w;
-  const int* sorted;  // K > 1: as in HdArgs
-  const float* sorted_w;
   const float* lse;
   float* again;
 
@@ -823,46 +821,44 @@ __device__ __forceinline__ void hd_scale(const HdScale& a) {
   }
 }
 
-// exp(z - lse) - 1 of a token's heavy targets, at the first of the places that name an id. Its warps take the targets in
+// exp(z - lse) - 1 of a token's heavy targets, at the first of an id's places in order. The targets are those of
+// hd_join_kernel to the bit: the sum of weights is taken in the caller's order in both. Its warps take the targets in
 // turn (301 tokens of 5 targets, both gradients: 92.5 us with one warp a token, 90 with four).
 template <bool QUANT>
 __device__ __forceinline__ void hd_again(const HdScale& a, int block) {
   const int lane = threadIdx.x & 31, warps = a.warps(), part = (threadIdx.x >> 5) % warps;
   const int t = block * (8 / warps) + (threadIdx.x >> 5) / warps;
   if (t >= a.T) return;
-  const bool many = a.start != nullptr;
-  const int n = many ? a.start[(size_t)t * (a.nt + 1) + a.nt] : 1;
+  const size_t row = (size_t)t * a.K;
   int id[2];
-  float wt[2], again[2] = {HD_LIGHT, HD_LIGHT};
+  float wt[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int j = lane + 32 * i;
-    const size_t at = (size_t)t * a.K + j;
-    id[i] = j < n ? (many ? a.sorted : a.ids)[at] : -1;
+    id[i] = j < a.K ? a.ids[row + j] : -1;
     if (id[i] >= a.V) id[i] = -1;
-    wt[i] = id[i] < 0 ? 0.f : many ? a.sorted_w[at] : a.weights ? a.weights[at] : 1.f;
+    wt[i] = id[i] < 0 ? 0.f : a.weights ? a.weights[row + j] : 1.f;
   }
   const float lse = a.lse[t];
-  bool mine[2] = {part == 0, part == 0};  // the places that this warp writes
+  unsigned long long heavy = 0;  // places in order
   int turn = 0;
   for (unsigned long long todo = hd_heavy(id, wt); todo; ++turn) {
     const int j = __ffsll(todo) - 1;
     const int v = __shfl_sync(0xffffffffu, j < 32 ? id[0] : id[1], j & 31);
-    const unsigned long long same = hd_same(id, v);
-    const int first = __ffsll(same) - 1;
-    const bool own = turn % warps == part;
-    const float d = own ? expm1f(hd_dot<QUANT, QUANT ? 2 : 4>(a.w, a.x + (size_t)t * a.ldx, a.H, v) - lse) : 0.f;
+    int place = 0;  // ids that come before
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (lane + 32 * i == first) {
-        again[i] = d;
-        mine[i] = own;
-      }
-    todo &= ~same;
+    for (int i = 0; i < 2; ++i) place += __popc(__ballot_sync(0xffffffffu, id[i] >= 0 && id[i] < v));
+    heavy |= 1ull << place;
+    if (turn % warps == part) {
+      const float d = expm1f(hd_dot<QUANT, QUANT ? 2 : 4>(a.w, a.x + (size_t)t * a.ldx, a.H, v) - lse);
+      if (lane == 0) a.again[row + place] = d;
+    }
+    todo &= ~hd_same(id, v);
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (mine[i] && lane + 32 * i < a.K) a.again[(size_t)t * a.K + lane + 32 * i] = again[i];
+  if (part == 0) {
+    for (int j = lane; j < a.K; j += 32)
+      if (!(heavy >> j & 1)) a.again[row + j] = HD_LIGHT;
+  }
 }
 
 // Blocks [0, a.blocks()): as HdScale says. The others, for dW: x with the rows of tokens without a target at 0, so
@@ -1151,8 +1147,8 @@ struct HdOperand {
 
 // One CTA a tile where the output has no more than 128 rows, else a pair.
 //
-// `early`: it may start under the kernel before it, one of this call's small ones, which call pdl_trigger in their first
-// instruction: the early kernel starts when every CTA before has called it, so that all of them are on the GPU by then
+// `early`: it may start under the kernel before it, one of this call's small ones, which call pdl_trigger in their
+// first instruction: the early kernel starts when every CTA before has called it, so that all of them are on the GPU by then
 // and end without an SM that the early one's waiting CTAs have taken. (Those leave no room on an SM: 384 threads of
 // 168 registers, 225 KB.) A trigger stays a kernel's first instruction, and nothing starts early behind an hd_kernel,
 // whose CTAs wait in pdl_wait first: some of its pairs may still wait for SMs, which CTAs of a later kernel that wait
@@ -1331,7 +1327,7 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
   const HdHead head = {w, static_cast<const __nv_bfloat16*>(w_scales),
                        static_cast<const __nv_bfloat16*>(w_biases), ldw};
   const HdScale scale = {ids, g, weights, k.start, k.wsum, k.scale, T, V, k.nt,
-                         static_cast<const __nv_bfloat16*>(x), ldx, H, K, head, k.sorted, k.sorted_w, lse, k.again};
+                         static_cast<const __nv_bfloat16*>(x), ldx, H, K, head, lse, k.again};
   if (!quant) {
     hd_rows_kernel<<<scale.blocks() + (dw ? hd_blocks((long long)T * (H / 8)) : 0), 256, 0, st>>>(
         static_cast<const __nv_bfloat16*>(x), ldx, H, scale, k.xz);
