@@ -699,8 +699,8 @@ int lg_head_loss_grad(const void* x, long long ldx, int T, int H, const void* w,
 /*
  * The first wait of the head's product kernels on the current device that ran out (each ends after some seconds, and
  * its call's results hold NaN where they are not right): 0, or kernel << 8 | wait, with kernel 1 for the loss,
- * 2 dz, 3 dx, 4 dw, 5 the loss from 4-bit codes. Synchronous with the default stream; the caller has waited for others.
- * reset != 0 clears it.
+ * 2 dz, 3 dx, 4 dw, 5 the loss from 4-bit codes; or 6 << 8 | site for an index out of its bounds, whose access was left
+ * out. Synchronous with the default stream; the caller has waited for others. reset != 0 clears it.
  */
 int lg_head_status(int* status, int reset);
 

@@ -159,8 +159,13 @@ __device__ __forceinline__ HdRow hd_row(const HdArgs& a, const HdUnit& u, int t)
   } else {
     const unsigned char* st = a.start + (size_t)t * (a.nt_all + 1);
     const int tile = a.v0 / HD_BN + u.n;
+    if (!hd_ok(tile >= 0 && tile < a.nt_all, 1)) return r;
     r.p = st[tile];
     r.p1 = st[tile + 1];
+    if (!hd_ok(r.p <= r.p1 && r.p1 <= a.K, 2)) {
+      r.p = r.p1 = 0;
+      return r;
+    }
     if (KIND == HD_PROB) {
       r.counts = st[a.nt_all] > 0;
       r.gs = r.gg * a.wsum[t].x;
@@ -199,6 +204,7 @@ __device__ __forceinline__ void hd_box(const HdArgs& a, uint8_t* box, const uint
     const int row = 4 * i + (lane >> 3);
     const uint4 v = *reinterpret_cast<const uint4*>(box + row * 128 + ((chunk ^ (row & 7)) << 4));
     if (!in || y + row >= a.M) continue;
+    if (!hd_ok(y >= 0 && x >= 0 && split >= 0 && split < a.splits && col + PER <= a.width, 6)) continue;
     if (KIND == HD_XGRAD) {
       float* out = static_cast<float*>(a.tile_out) + ((size_t)split * a.M + y + row) * a.width + col;
       if (a.add)
@@ -242,9 +248,10 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
       while ((unsigned)row.next - (unsigned)id0 < 32u) {
         const float z = hd_pick(v, row.next - id0);
         if (a.K == 1) {
-          a.out.ztgt[t] = z;
+          if (hd_ok(t < a.M, 4)) a.out.ztgt[t] = z;
           break;
         }
+        if (!hd_ok(row.p < a.K && t < a.M && a.order[row_k + row.p] < a.K, 3)) break;
         a.out.ztgt[row_k + a.order[row_k + row.p]] = z;
         row.next = ++row.p < row.p1 ? a.ids[row_k + row.p] : -1;
       }
@@ -271,7 +278,8 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
       sum += s0 + s1;
     }
     if (live) {
-      a.out.part[(size_t)t * a.nt_all + ntile] = make_float2(mx, ok ? sum : nan);
+      if (hd_ok(ntile < a.nt_all && ntile >= 0, 5))
+        a.out.part[(size_t)t * a.nt_all + ntile] = make_float2(mx, ok ? sum : nan);
       if (a.out.top) a.out.top[(size_t)t * a.nt_all + ntile] = arg;
     }
   } else if (KIND == HD_XGRAD || (KIND == HD_WGRAD && a.splits > 1)) {
@@ -403,6 +411,12 @@ __global__ void __launch_bounds__(hd_threads(KIND), 1)
             ok = false;
             break;
           }
+          if (!hd_ok(st >= 0 && st < STAGES && kb >= 0 && kb < a.kblocks && ar >= 0 && br >= 0 && u.m < a.mt &&
+                         u.n < a.nt && u.split < a.splits,
+                     7)) {
+            ok = false;
+            break;
+          }
           uint8_t* sa = smem + st * STAGE;
           uint8_t* sb = sa + HD_A_BYTES;
           const int k = kb * HD_BK;
@@ -470,6 +484,10 @@ __global__ void __launch_bounds__(hd_threads(KIND), 1)
             break;
           }
           tc_fence_after();
+          if (!hd_ok((tmem & 0x1ff) == 0 && st < STAGES, 8)) {
+            ok = false;
+            break;
+          }
           const uint32_t sa = smem_u32(smem + st * STAGE), sb = sa + HD_A_BYTES;
           const uint32_t da = A_MN ? sw128_lo_mn(sa, HD_BOX) : sw128_lo(sa);
           const uint32_t db = B_MN ? sw128_lo_mn(sb, HD_BOX) : sw128_lo(sb);
@@ -594,6 +612,7 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
     int rank = 0;
 #pragma unroll 8
     for (int i = 0; i < K; ++i) rank += row[i] < id || (row[i] == id && i < j);
+    if (!hd_ok(rank >= 0 && rank < K, 9)) continue;
     up[rank] = id;
     sorted[(size_t)t * K + rank] = id;
     order[(size_t)t * K + rank] = (unsigned char)j;
@@ -736,6 +755,7 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
   while (todo) {
     const int j = __ffsll(todo) - 1;
     const int v = __shfl_sync(0xffffffffu, j < 32 ? id[0] : id[1], j & 31);
+    if (!hd_ok(v >= 0 && v < V && n < HD_MAXK, 10)) break;
     if (n % WARPS == warp) {
       const float d = hd_dot<QUANT, 4>(w, x + (size_t)t * ldx, H, v);
       if (lane == 0) sh_dot[n] = d;
@@ -848,6 +868,7 @@ __device__ __forceinline__ void hd_again(const HdScale& a, int block) {
     int place = 0;  // ids that come before
 #pragma unroll
     for (int i = 0; i < 2; ++i) place += __popc(__ballot_sync(0xffffffffu, id[i] >= 0 && id[i] < v));
+    if (!hd_ok(v >= 0 && v < a.V && place >= 0 && place < a.K, 11)) break;
     heavy |= 1ull << place;
     if (turn % warps == part) {
       const float d = expm1f(hd_dot<QUANT, QUANT ? 2 : 4>(a.w, a.x + (size_t)t * a.ldx, a.H, v) - lse);
@@ -879,6 +900,7 @@ __global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __res
   for (long long i = (blockIdx.x - first) * 256LL + threadIdx.x; i < n; i += (gridDim.x - first) * 256LL) {
     const int t = (int)(i / per), c = (int)(i % per) * 8;
     uint4 v = make_uint4(0, 0, 0, 0);
+    if (!hd_ok(t >= 0 && t < a.T && c + 8 <= H, 12)) continue;
     if (hd_counts(a, t)) v = *reinterpret_cast<const uint4*>(x + (size_t)t * ldx + c);
     *reinterpret_cast<uint4*>(out + (size_t)t * H + c) = v;
   }

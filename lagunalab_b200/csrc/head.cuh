@@ -84,6 +84,13 @@ struct HdParts {
 static __device__ int hd_status_word;
 __device__ __forceinline__ void hd_record(int kernel, int code) { atomicCAS(&hd_status_word, 0, kernel << 8 | code); }
 
+// An index that the kernels' own arithmetic keeps in bounds: where it is not, the access is left out and its site
+// recorded as kernel 6. The kernels stay in this form: it is the one that long runs were made with.
+__device__ __forceinline__ bool hd_ok(bool in, int site) {
+  if (!in) hd_record(6, site);
+  return in;
+}
+
 // head_q4.cu: the loss's parts from a 4-bit head for few tokens, without the bf16 weights in memory: up to HQ_MAXT
 // tokens a pass over the weights. xp: T H bf16, idt: HQ_MAXT K ints of workspace. Taken for up to
 // HQ_PASSES passes, where that is faster than the products of head.cu over unpacked weights.

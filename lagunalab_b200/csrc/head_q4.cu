@@ -285,6 +285,7 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
       sw = bw = 0;
       if (blk < b1 && row < a.V && k < a.kb) {
         const size_t at = (size_t)row * a.kb + k;
+        if (!hd_ok(row >= 0 && k >= 0 && k < a.kb, 21)) return;
         if (a.pairs) {
           sw = __ldg(reinterpret_cast<const uint32_t*>(a.scales + at));
           bw = __ldg(reinterpret_cast<const uint32_t*>(a.biases + at));
@@ -315,6 +316,10 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
         {
           const bool two = 2 * k2 + 1 < a.kb;
           const bool fast = __all_sync(0xffffffffu, !mine || q4_fast(sw));
+          if (!hd_ok(ws >= 0 && ws < a.ws && slot >= 0 && slot < AS && (tmem & 0x1ff) == 0, 22)) {
+            ok = false;
+            break;
+          }
           const uint8_t* row = sm_w + ws * HQ_W_BYTES + r * 128;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -398,7 +403,8 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
               const int b = __ffs(hit) - 1;
               hit &= hit - 1;
               const int at = __shfl_sync(0xffffffffu, id, b) - id0;
-              if (lane == at) a.out.ztgt[(size_t)(c * 32 + b) * a.K + j] = hd_pick(v, b);
+              if (lane == at && hd_ok(c * 32 + b < a.T, 20))
+                a.out.ztgt[(size_t)(c * 32 + b) * a.K + j] = hd_pick(v, b);
             }
           }
           const bool live = c * 32 + lane < a.T;
@@ -485,7 +491,7 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
         if (m == mx && p < top) top = p;
       }
     }
-    a.out.part[(size_t)t * a.out.parts + blockIdx.x] = make_float2(mx, sum);
+    if (hd_ok(blockIdx.x < a.out.parts, 23)) a.out.part[(size_t)t * a.out.parts + blockIdx.x] = make_float2(mx, sum);
     if (a.out.top) a.out.top[(size_t)t * a.out.parts + blockIdx.x] = top;
   }
 }
