@@ -394,7 +394,6 @@ __global__ void __launch_bounds__(hd_threads(KIND), 1)
   __syncthreads();
   if (CG == 2) cluster_sync();  // the other CTA's barriers are ready
   tc_fence_after();
-  pdl_wait();  // nothing of an earlier kernel's is touched before
   const uint32_t tmem = *tmem_base;
   const int units = a.mt * a.nt * a.splits;
 
@@ -886,7 +885,6 @@ __device__ __forceinline__ void hd_again(const HdScale& a, int block) {
 // that dW has nothing of them (0 * NaN is NaN).
 __global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int H,
                                                       const HdScale a, __nv_bfloat16* __restrict__ out) {
-  pdl_trigger();
   const int first = a.blocks();
   if ((int)blockIdx.x < first) {
     if (blockIdx.x == 0)
@@ -913,7 +911,6 @@ __global__ void __launch_bounds__(256, 5) hd_dequant_kernel(const uint2* __restr
                                                             const uint16_t* __restrict__ s,
                                                             const uint16_t* __restrict__ b, long long n,
                                                             const HdScale a, __nv_bfloat16* __restrict__ out) {
-  pdl_trigger();
   const int first = a.blocks();  // of the blocks that unpack
   if ((int)blockIdx.x < first) {
     if (blockIdx.x == 0)
@@ -1125,8 +1122,7 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
   } while (0)
 
 template <int KIND, int CG>
-static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const HdArgs& a, bool early,
-                        cudaStream_t st) {
+static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const HdArgs& a, cudaStream_t st) {
   static std::atomic<bool> done[64];
   int dev = 0;
   LG_CUDA_TRY(cudaGetDevice(&dev));
@@ -1141,21 +1137,12 @@ static int hd_launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const HdAr
   cfg.blockDim = hd_threads(KIND);
   cfg.dynamicSmemBytes = HD_SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  int n = 0;
-  if (CG > 1) {
-    at[n].id = cudaLaunchAttributeClusterDimension;
-    at[n].val.clusterDim.x = CG;
-    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (early) {
-    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = n;
+  cfg.numAttrs = 1;
   LG_CUDA_TRY(cudaLaunchKernelEx(&cfg, hd_kernel<KIND, CG>, ma, mb, a));
   LG_LAUNCH_CHECK("head");
   return LG_OK;
@@ -1169,14 +1156,11 @@ struct HdOperand {
 
 // One CTA a tile where the output has no more than 128 rows, else a pair.
 //
-// `early`: it may start under the kernel before it, one of this call's small ones, which call pdl_trigger in their
-// first instruction: the early kernel starts when every CTA before has called it, so that all of them are on the GPU by then
-// and end without an SM that the early one's waiting CTAs have taken. (Those leave no room on an SM: 384 threads of
-// 168 registers, 225 KB.) A trigger stays a kernel's first instruction, and nothing starts early behind an hd_kernel,
-// whose CTAs wait in pdl_wait first: some of its pairs may still wait for SMs, which CTAs of a later kernel that wait
-// for them could take for ever. (It happened.)
+// Every kernel of a call starts when the one before has ended. (Starting the products under the small kernels before
+// them, by programmatic serialization, took 1 to 2.5 us less a call: 301 tokens of 5 targets 95.5 against 98 us. It is
+// not worth the reasoning that it needs: CTAs of 225 KB that wait on an SM for a kernel whose CTAs need SMs.)
 template <int KIND>
-static int hd_launch(const HdOperand& a, const HdOperand& b, HdArgs g, bool early, cudaStream_t st) {
+static int hd_launch(const HdOperand& a, const HdOperand& b, HdArgs g, cudaStream_t st) {
   constexpr bool A_MN = KIND == HD_WGRAD, B_MN = KIND == HD_XGRAD || KIND == HD_WGRAD;
   const int cg = hd_cg(g.M);
   g.mt = (g.M + HD_BM * cg - 1) / (HD_BM * cg);
@@ -1184,7 +1168,7 @@ static int hd_launch(const HdOperand& a, const HdOperand& b, HdArgs g, bool earl
   CUtensorMap ma, mb;
   HD_TRY(make_map_2d(&ma, a.p, true, a.inner, a.rows, (uint64_t)a.ld * 2, 64, A_MN ? HD_BK : HD_BM, 128));
   HD_TRY(make_map_2d(&mb, b.p, true, b.inner, b.rows, (uint64_t)b.ld * 2, 64, B_MN ? HD_BK : HD_BN / cg, 128));
-  return cg == 2 ? hd_launch_as<KIND, 2>(ma, mb, g, early, st) : hd_launch_as<KIND, 1>(ma, mb, g, early, st);
+  return cg == 2 ? hd_launch_as<KIND, 2>(ma, mb, g, st) : hd_launch_as<KIND, 1>(ma, mb, g, st);
 }
 
 static int hd_check(const char* who, const void* x, long long ldx, int T, int H, const void* w,
@@ -1317,7 +1301,7 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
       a.v0 = v0;
       a.b_row0 = quant ? 0 : v0;
       const HdOperand mw = quant ? HdOperand{k.wq, H, n, H} : HdOperand{w, H, V, ldw};
-      HD_TRY(hd_launch<HD_LOSS>({x, H, T, ldx}, mw, a, quant, st));
+      HD_TRY(hd_launch<HD_LOSS>({x, H, T, ldx}, mw, a, st));
     }
   }
   const auto join = quant ? hd_join_kernel<true> : hd_join_kernel<false>;
@@ -1372,7 +1356,7 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     const int ldz = (n + 63) / 64 * 64;
     a.tile_out = k.dz;
     a.width = ldz;
-    HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, a, quant || v0 == 0, st));
+    HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, a, st));
     const HdOperand mz = {k.dz, n, T, ldz};
     if (dx) {
       HdArgs b = a;
@@ -1382,7 +1366,7 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
       b.add = v0 > 0;
       b.tile_out = k.dx;
       b.width = H;
-      HD_TRY(hd_launch<HD_XGRAD>(mz, mw, b, false, st));
+      HD_TRY(hd_launch<HD_XGRAD>(mz, mw, b, st));
     }
     if (dw) {
       HdArgs b = a;
@@ -1393,7 +1377,7 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
       __nv_bfloat16* rows = static_cast<__nv_bfloat16*>(dw) + (size_t)v0 * H;
       b.tile_out = k.wsplits > 1 ? static_cast<void*>(k.dw) : rows;
       b.width = H;
-      HD_TRY(hd_launch<HD_WGRAD>(mz, {k.xz, H, T, H}, b, false, st));
+      HD_TRY(hd_launch<HD_WGRAD>(mz, {k.xz, H, T, H}, b, st));
       if (k.wsplits > 1) HD_TRY(hd_join_parts(k.dw, k.wsplits, (long long)n * H, k.scale, rows, st));
     }
   }

@@ -41,7 +41,7 @@ constexpr int HQ_THREADS = (8 + HQ_UNPACK) * 32;
 constexpr int HQ_BLOCK = 32;               // ids a block: a warp's TMEM lanes
 constexpr int HQ_W_BYTES = 4 * 32 * 128;   // a stage of packed words, two turns': 128 rows x 256 codes
 constexpr float HQ_FAR = 90.f;             // of exponents of 2: 100,000 terms of 2^90 are below 2^127
-constexpr int HQ_SMEM_MAX = 224 << 10;     // a CTA of hq_order_kernel has room beside it
+constexpr int HQ_SMEM_MAX = 224 << 10;
 
 struct HqArgs {
   int T, N, V, K;
@@ -155,9 +155,6 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   const uint32_t tmem = *tmem_base;        // accumulators: columns [0, 64 NT)
   const uint32_t tmem_a = tmem + 64 * NT;  // weights: 64 columns a slot
 
-  // Every kernel of the call's stream before hq_order_kernel has ended; that one's x and ids are waited for by those
-  // who read them, while the words already come.
-  if (warp == 2 || warp >= 4 + HQ_UNPACK) pdl_wait();
   if (warp == 0) {
     if (elect_one()) {
       int st = 0, used = 0;
@@ -501,7 +498,6 @@ __global__ void __launch_bounds__(256) hq_order_kernel(const __nv_bfloat16* __re
                                                        int per, __nv_bfloat16* __restrict__ out,
                                                        const int* __restrict__ ids, int T, int K, int nt,
                                                        int* __restrict__ idt) {
-  pdl_trigger();
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i < K * nt) {
     const int t = i % nt, j = i / nt;
@@ -548,7 +544,7 @@ static int hq_launch(const CUtensorMap (&m)[3], const HqArgs& a, int grid, size_
     LG_CUDA_TRY(cudaFuncSetAttribute(hq_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, HQ_SMEM_MAX));
     if (dev < 64) done[dev].store(true, std::memory_order_relaxed);
   }
-  LG_CUDA_TRY(launch_early(hq_kernel<NT>, grid, HQ_THREADS, smem, st, m[0], m[1], m[2], a));
+  hq_kernel<NT><<<grid, HQ_THREADS, smem, st>>>(m[0], m[1], m[2], a);
   LG_LAUNCH_CHECK("head_q4");
   return LG_OK;
 }

@@ -237,7 +237,6 @@ __global__ void __launch_bounds__(RB_WARPS * 32) router_balance_kernel(
       }
     }
   }
-  pdl_trigger();
   if (l == 0 && kept) atomicAdd(&hist[RB_MAXE], kept);
 #pragma unroll
   for (int s = 16; s >= G; s >>= 1) {
@@ -276,7 +275,6 @@ __global__ void __launch_bounds__(1024) router_balance_join_kernel(const float* 
   __shared__ float sp[1024];
   __shared__ int sc[1024];
   __shared__ int sn[32];
-  pdl_wait();
   const int W = (E + 31) / 32 * 32, S = 1024 / W;
   const int e = threadIdx.x % W, s = threadIdx.x / W;
   const int a = C * s / S, b = s < S ? C * (s + 1) / S : 0;
@@ -520,7 +518,7 @@ extern "C" int lg_router_balance(const float* logits, const int32_t* inds, const
 #undef RB_CALL
   LG_LAUNCH_CHECK("router_balance");
   if (C > 1) {
-    LG_CUDA_TRY(launch_early(router_balance_join_kernel, 1, 1024, 0, st, (const float*)pp, (const int*)pc, C, E, o));
+    router_balance_join_kernel<<<1, 1024, 0, st>>>(pp, pc, C, E, o);
     LG_LAUNCH_CHECK("router_balance_join");
   }
   return LG_OK;
