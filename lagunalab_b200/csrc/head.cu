@@ -12,7 +12,7 @@
 //
 // Bound: the tensor cores, and for more than some hundred us the power limit. 8,192 tokens and 100,352 ids of 2,048:
 // loss 2.2 ms (1.5 PFLOP/s; tensor pipe 98 % busy), both gradients 7.1 ms (1.4). With few rows the tiles' ends and the
-// chain of launches: 301 tokens and 32,003 ids of 1,024, 87 us (31 for dz, 27 dx, 25 dW, the rest sorting and joining).
+// chain of launches: 301 tokens and 32,003 ids of 1,024, 94 us (31 for dz, 27 dx, 25 dW, the rest sorting and joining).
 //
 // Roundings: z, the softmax statistics and every sum are fp32. dz is rounded to bf16 (2^-8 relative
 // at most) because the tensor cores take bf16 operands. It is kept as dz / c, with c = max |g_t w_tj|, and
@@ -198,13 +198,13 @@ __device__ __forceinline__ void hd_box(const HdArgs& a, uint8_t* box, const uint
         make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
   __syncwarp();
   const int chunk = lane & 7, col = x + chunk * PER;
-  const bool in = col < a.width;
+  const bool in = col < a.width &&
+                  hd_ok(y >= 0 && x >= 0 && split >= 0 && split < a.splits && col + PER <= a.width, 6);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int row = 4 * i + (lane >> 3);
     const uint4 v = *reinterpret_cast<const uint4*>(box + row * 128 + ((chunk ^ (row & 7)) << 4));
     if (!in || y + row >= a.M) continue;
-    if (!hd_ok(y >= 0 && x >= 0 && split >= 0 && split < a.splits && col + PER <= a.width, 6)) continue;
     if (KIND == HD_XGRAD) {
       float* out = static_cast<float*>(a.tile_out) + ((size_t)split * a.M + y + row) * a.width + col;
       if (a.add)
