@@ -21,7 +21,8 @@
 // same, and dx and dW with it. The other errors are independent: sums over the vocabulary or the tokens average them.
 // z is the tensor cores' sum, which is cut after each step, but for targets that carry an eighth or more of their
 // token's weight: loss and gradient take both their logits from one fp32 sum (hd_dot), since a target's S p - w of
-// nearly 0 has all of z's error, and lse's with the other sign: what is left of it is lse's own rounding.
+// nearly 0 has all of z's error, and lse's with the other sign: what is left of it is lse's own rounding. For lse
+// the logits around one that is a fourth of the softmax are summed again too (hd_join_kernel).
 //
 // Every mbarrier wait is bounded (tc::mbar_wait). A CTA whose wait ran out writes NaN for what is
 // left of its tiles (zeros stay in dz for tokens without a target, and the ids of largest logits have no mark), waits
@@ -233,8 +234,8 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
   if (KIND == HD_LOSS) {
     const int ntile = a.v0 / HD_BN + u.n;
     const size_t row_k = (size_t)t * a.K;
-    float mx = -INFINITY, sum = 0.f;
-    int arg = 0;
+    float mx = -INFINITY, sum = 0.f, best = 0.f;  // best: of the 32 ids that hold the maximum
+    int arg = 0, at = 0;
 #pragma unroll 1
     for (int c = 0; c < COLS; c += 32) {
       const int id0 = a.v0 + n0 + c;  // vocabulary ids
@@ -258,12 +259,13 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
       float cm = v[0];
 #pragma unroll
       for (int i = 1; i < 32; ++i) cm = fmaxf(cm, v[i]);
-      if (cm > mx) {
+      const bool higher = cm > mx;
+      if (higher) {
         if (a.out.top) {
-          int at = 0;
+          int first = 0;
 #pragma unroll
-          for (int i = 31; i >= 0; --i) at = v[i] == cm ? i : at;
-          arg = id0 + at;
+          for (int i = 31; i >= 0; --i) first = v[i] == cm ? i : first;
+          arg = id0 + first;
         }
         sum *= hd_ex2((mx - cm) * HD_LOG2E);  // mx = -inf: sum is 0
         mx = cm;
@@ -276,10 +278,13 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
         s1 += hd_ex2(fmaf(v[i + 1], HD_LOG2E, off));
       }
       sum += s0 + s1;
+      best = higher ? s0 + s1 : best;
+      at = higher ? c : at;
     }
     if (live) {
       if (hd_ok(ntile < a.nt_all && ntile >= 0, 5))
-        a.out.part[(size_t)t * a.nt_all + ntile] = make_float2(mx, ok ? sum : nan);
+        a.out.part[(size_t)t * a.nt_all + ntile] =
+            make_float4(mx, ok ? sum : nan, best, __int_as_float(a.v0 + n0 + at));
       if (a.out.top) a.out.top[(size_t)t * a.nt_all + ntile] = arg;
     }
   } else if (KIND == HD_XGRAD || (KIND == HD_WGRAD && a.splits > 1)) {
@@ -630,7 +635,10 @@ __global__ void __launch_bounds__(256) hd_sort_kernel(const int* __restrict__ id
   if (lane == 0) wsum[t] = make_float2(sum * times, big);
 }
 
-constexpr int HJ_THREADS = 128;
+// Of hd_join_kernel. Few tokens: twice as many, for the 32 ids around a large logit (37 tokens, 4-bit: 16.4 us against
+// 11.2 where a token has one, 7 where none has); many: 2,048 tokens' loss takes 632 us with 256, 625 with 128.
+constexpr int HJ_THREADS = 256;
+static int hj_threads(bool few) { return few ? HJ_THREADS : HJ_THREADS / 2; }
 
 // sum_h x_h W_vh by a warp, in fp32 with each sum rounded to nearest; the same bits for every U.
 template <bool QUANT, int U>
@@ -673,6 +681,66 @@ __device__ __forceinline__ float hd_dot(const HdHead& w, const __nv_bfloat16* x,
   return warp_sum(s);
 }
 
+// hd_dot of N rows from v on (below V; the others give -inf), two chunks of each in flight: each row's sum goes in
+// hd_dot's order, to the same bits.
+template <bool QUANT, int N>
+__device__ __forceinline__ void hd_dots(const HdHead& w, const __nv_bfloat16* x, int H, int v, int V, float (&out)[N]) {
+  constexpr int U = 2;
+  const int lane = threadIdx.x & 31;
+  float s[N] = {};
+  for (int c0 = lane * 8; c0 < H; c0 += U * 256) {
+    uint4 xv[U], wv[U][QUANT ? 1 : N];
+    uint32_t q[U][QUANT ? N : 1];
+    uint16_t sc[U][QUANT ? N : 1], bi[U][QUANT ? N : 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * 256;
+      xv[u] = make_uint4(0, 0, 0, 0);
+      if (c < H) xv[u] = *reinterpret_cast<const uint4*>(x + c);
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        const bool in = c < H && v + r < V;
+        const size_t row = v + r;
+        if (QUANT) {
+          q[u][r] = 0;
+          sc[u][r] = bi[u][r] = 0;
+          if (in) {
+            q[u][r] = static_cast<const uint32_t*>(w.w)[row * (H / 8) + c / 8];
+            sc[u][r] = reinterpret_cast<const uint16_t*>(w.scales)[row * (H / 64) + c / 64];
+            bi[u][r] = reinterpret_cast<const uint16_t*>(w.biases)[row * (H / 64) + c / 64];
+          }
+        } else {
+          wv[u][r] = make_uint4(0, 0, 0, 0);
+          if (in) wv[u][r] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w.w) + row * w.ld + c);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t xs[4] = {xv[u].x, xv[u].y, xv[u].z, xv[u].w};
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        uint32_t ws[4];
+        if (QUANT) {
+          hd_unpack(q[u][r], sc[u][r], bi[u][r], ws);
+        } else {
+          ws[0] = wv[u][r].x;
+          ws[1] = wv[u][r].y;
+          ws[2] = wv[u][r].z;
+          ws[3] = wv[u][r].w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[r] = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ws[i] << 16), s[r]);
+          s[r] = fmaf(__uint_as_float(xs[i] & 0xffff0000u), __uint_as_float(ws[i] & 0xffff0000u), s[r]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < N; ++r) out[r] = v + r < V ? warp_sum(s[r]) : -INFINITY;
+}
+
 // Of a warp's targets, two a lane (id -1: none): those with an eighth or more of all weights, eight ids at most. None
 // where all weights are 0.
 __device__ __forceinline__ unsigned long long hd_heavy(const int (&id)[2], const float (&wt)[2]) {
@@ -690,10 +758,12 @@ __device__ __forceinline__ unsigned long long hd_same(const int (&id)[2], int v)
          (unsigned long long)__ballot_sync(0xffffffffu, id[1] == v) << 32;
 }
 
-// (maximum, sum of exponentials from it, the maximum's lowest id) of two parts, the first before the second.
+// HdParts of two parts, the first before the second; arg: the maximum's lowest id.
 struct HdStat {
   float mx, sum;
   int arg;
+  float best;
+  int at;
 };
 __device__ __forceinline__ HdStat hd_merge(const HdStat& a, const HdStat& b) {
   HdStat r;
@@ -702,6 +772,8 @@ __device__ __forceinline__ HdStat hd_merge(const HdStat& a, const HdStat& b) {
   const float eb = b.mx == r.mx ? 1.f : hd_ex2((b.mx - r.mx) * HD_LOG2E);
   r.sum = a.sum * ea + b.sum * eb;
   r.arg = b.mx > a.mx || (b.mx == a.mx && b.arg < a.arg) ? b.arg : a.arg;
+  r.best = fmaxf(a.best * ea, b.best * eb);
+  r.at = b.best * eb > a.best * ea ? b.at : a.at;
   return r;
 }
 
@@ -712,7 +784,9 @@ __device__ __forceinline__ HdStat hd_merge(const HdStat& a, const HdStat& b) {
 // products make is 1e-5 too small, more than all other errors together (loss off by 1.5e-6 in the 2-norm
 // against 64 bits, 3e-7 with an fp32 product). The logits of targets with an eighth or more of the token's
 // weight, eight at most, are therefore summed again here, in fp32 rounded to nearest, and take their first
-// value's place in lse too. A warp sums one target's; the four work side by side.
+// value's place in lse too. A warp sums one target's; all work side by side. So are, for lse's sake, the
+// 32 ids around a logit that has a fourth of the softmax or more, unless a target among them is nearly all of it: lse of
+// a token without a target was off by up to 2.3e-6 of itself.
 template <bool QUANT>
 __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const __nv_bfloat16* __restrict__ x,
                                                              long long ldx, int H, HdHead w,
@@ -721,9 +795,9 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
                                                              float* __restrict__ loss,
                                                              float* __restrict__ lse_out,
                                                              int* __restrict__ top) {
-  constexpr int WARPS = HJ_THREADS / 32;
-  __shared__ HdStat sh[WARPS];
-  __shared__ float sh_dot[HD_MAXK];
+  const int warps = blockDim.x >> 5;
+  __shared__ HdStat sh[HJ_THREADS / 32];
+  __shared__ float sh_dot[HD_MAXK], sh_near[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x;
   const int parts = in.parts;
@@ -740,12 +814,12 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
     wt[i] = id[i] < 0 ? 0.f : weights ? weights[(size_t)t * K + j] : 1.f;
     z[i] = id[i] < 0 ? 0.f : in.ztgt[(size_t)t * K + j];
   }
-  const float2* row = in.part + (size_t)t * parts;
-  HdStat st = {-INFINITY, 0.f, 0x7fffffff};
+  const float4* row = in.part + (size_t)t * parts;
+  HdStat st = {-INFINITY, 0.f, 0x7fffffff, 0.f, 0};
 #pragma unroll 4
-  for (int n = threadIdx.x; n < parts; n += HJ_THREADS) {
-    const float2 v = row[n];
-    st = hd_merge(st, {v.x, v.y, top ? in.top[(size_t)t * parts + n] : 0});
+  for (int n = threadIdx.x; n < parts; n += blockDim.x) {
+    const float4 v = row[n];
+    st = hd_merge(st, {v.x, v.y, top ? in.top[(size_t)t * parts + n] : 0, v.z, __float_as_int(v.w)});
   }
   // The list of heavy targets, an id once: every warp has it, and sums its share.
   unsigned long long todo = hd_heavy(id, wt);
@@ -755,7 +829,7 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
     const int j = __ffsll(todo) - 1;
     const int v = __shfl_sync(0xffffffffu, j < 32 ? id[0] : id[1], j & 31);
     if (!hd_ok(v >= 0 && v < V && n < HD_MAXK, 10)) break;
-    if (n % WARPS == warp) {
+    if (n % warps == warp) {
       const float d = hd_dot<QUANT, 4>(w, x + (size_t)t * ldx, H, v);
       if (lane == 0) sh_dot[n] = d;
     }
@@ -765,21 +839,52 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const HdStat p = {__shfl_xor_sync(0xffffffffu, st.mx, o), __shfl_xor_sync(0xffffffffu, st.sum, o),
-                      __shfl_xor_sync(0xffffffffu, st.arg, o)};
+                      __shfl_xor_sync(0xffffffffu, st.arg, o), __shfl_xor_sync(0xffffffffu, st.best, o),
+                      __shfl_xor_sync(0xffffffffu, st.at, o)};
     st = (lane & o) ? hd_merge(p, st) : hd_merge(st, p);
   }
   if (lane == 0) sh[warp] = st;
   __syncthreads();
-  if (warp) return;
   st = sh[0];
+  for (int i = 1; i < warps; ++i) st = hd_merge(st, sh[i]);
+  // The same decision in every thread.
+  bool near = in.maxima ? st.sum <= 4.f && st.best > 0.f : st.best > 0.f && 4.f * st.best >= st.sum;
+  if (near) {
+    float known = 0.f;
+    for (todo = heavy; todo;) {
+      const int j = __ffsll(todo) - 1;
+      const int v = __shfl_sync(0xffffffffu, j < 32 ? id[0] : id[1], j & 31);
+      const float was = __shfl_sync(0xffffffffu, j < 32 ? z[0] : z[1], j & 31);
+      if ((unsigned)v - (unsigned)st.at < 32u) known += hd_ex2((was - st.mx) * HD_LOG2E);
+      todo &= ~hd_same(id, v);
+    }
+    near = known < 0.875f * st.best;
+  }
+  if (near) {
+    constexpr int N = 4;
+    for (int i = warp * N; i < 32; i += warps * N) {
+      float d[N];
+      hd_dots<QUANT, N>(w, x + (size_t)t * ldx, H, hd_ok(st.at >= 0, 13) ? st.at + i : V, V, d);
 #pragma unroll
-  for (int i = 1; i < WARPS; ++i) st = hd_merge(st, sh[i]);
+      for (int r = 0; r < N; ++r)
+        if (lane == 0) sh_near[i + r] = d[r];
+    }
+    __syncthreads();
+  }
+  if (warp) return;
+  if (near) {
+    st.sum += warp_sum(hd_ex2((sh_near[lane] - st.mx) * HD_LOG2E)) - st.best;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (id[i] >= 0 && (unsigned)id[i] - (unsigned)st.at < 32u) z[i] = sh_near[id[i] - st.at];
+  }
   todo = heavy;
   for (n = 0; todo; ++n) {
     const int j = __ffsll(todo) - 1;
     const int v = __shfl_sync(0xffffffffu, j < 32 ? id[0] : id[1], j & 31);
     const float was = __shfl_sync(0xffffffffu, j < 32 ? z[0] : z[1], j & 31), now = sh_dot[n];
-    st.sum += hd_ex2((now - st.mx) * HD_LOG2E) - hd_ex2((was - st.mx) * HD_LOG2E);
+    if (!near || (unsigned)v - (unsigned)st.at >= 32u)
+      st.sum += hd_ex2((now - st.mx) * HD_LOG2E) - hd_ex2((was - st.mx) * HD_LOG2E);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       if (id[i] == v) z[i] = now;  // every place of the list that names it
@@ -1079,7 +1184,8 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
   w.piece = hd_piece(T, H, V, quant, grad, dw);
   if (!grad) {
     w.out.parts = few ? hq_parts(V) : w.nt;
-    w.out.part = c.take<float2>((size_t)T * w.out.parts);
+    w.out.maxima = !few;
+    w.out.part = c.take<float4>((size_t)T * w.out.parts);
     if (top) w.out.top = c.take<int>((size_t)T * w.out.parts);
     w.out.ztgt = c.take<float>((size_t)T * K);
     if (few) {
@@ -1305,7 +1411,7 @@ extern "C" int lg_head_loss(const void* x, long long ldx, int T, int H, const vo
     }
   }
   const auto join = quant ? hd_join_kernel<true> : hd_join_kernel<false>;
-  join<<<T, HJ_THREADS, 0, st>>>(k.out, xb, ldx, H, head, ids, weights, K, V, loss, lse, top);
+  join<<<T, hj_threads(few), 0, st>>>(k.out, xb, ldx, H, head, ids, weights, K, V, loss, lse, top);
   LG_LAUNCH_CHECK("head_join");
   return LG_OK;
 }

@@ -71,13 +71,15 @@ struct HdHead {
   long long ld;
 };
 
-// Where the parts of a loss go before they are joined: per token `parts` pairs (maximum, sum of
-// exponentials from it), the ids of the maxima (or NULL), and the targets' logits.
+// Where the parts of a loss go before they are joined: per token `parts` times (maximum or another reference, sum of
+// exponentials from it, the share of that sum which the heaviest 32 ids have, the first of these), the ids of the
+// maxima (or NULL), and the targets' logits.
 struct HdParts {
-  float2* part;  // [T, parts]
+  float4* part;  // [T, parts]
   int* top;      // [T, parts]
   float* ztgt;   // [T, K]
   int parts;
+  bool maxima;  // the references are the maxima
 };
 
 // The first wait of a source file's kernels that ran out: kernel << 8 | code of the wait (lg_head_status).

@@ -111,7 +111,9 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   float* sm_sum = sm_m + 4 * 32 * NT;
   int* sm_top = reinterpret_cast<int*>(sm_sum + 4 * 32 * NT);
   float* sm_ref = reinterpret_cast<float*>(sm_top + 4 * 32 * NT);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm_ref + 4 * 32 * NT);
+  float* sm_best = sm_ref + 4 * 32 * NT;
+  int* sm_at = reinterpret_cast<int*>(sm_best + 4 * 32 * NT);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm_at + 4 * 32 * NT);
   uint64_t *w_full = bars, *w_empty = bars + 8, *full = bars + 16, *empty = bars + 24;
   uint64_t *acc_full = bars + 32, *acc_empty = bars + 34;
   uint64_t* done = bars + 36;
@@ -363,12 +365,16 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
     float mx[NT], sum[NT];  // of token c * 32 + lane: the reference (its maximum so far, or that of some tile), the sum
     int top[NT];
     float* ref = sm_ref + q * 32 * NT;  // -reference * log2(e) of each token; -inf past T: their columns hold anything
+    float* best = sm_best + q * 32 * NT;  // the largest sum of one block's exponentials, and the block
+    int* best_at = sm_at + q * 32 * NT;
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
       mx[c] = -INFINITY;
       sum[c] = 0.f;
       top[c] = 0x7fffffff;
       ref[c * 32 + lane] = -INFINITY;
+      best[c * 32 + lane] = 0.f;
+      best_at[c * 32 + lane] = 0;
     }
     bool ok = true;
     for (int i = 0; i < tiles && ok; ++i) {
@@ -437,7 +443,9 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
               if (cm > mx[c]) top[c] = id0 + arg;
             }
             if (cm > mx[c]) {
-              sum[c] *= hd_ex2((mx[c] - cm) * HD_LOG2E);  // mx = -inf: sum is 0 (or NaN)
+              const float down = hd_ex2((mx[c] - cm) * HD_LOG2E);  // mx = -inf: sum is 0 (or NaN)
+              sum[c] *= down;
+              best[c * 32 + lane] *= down;
               mx[c] = cm;
             }
             if (live) ref[c * 32 + lane] = mx[c] == -INFINITY ? 0.f : -mx[c] * HD_LOG2E;
@@ -446,7 +454,12 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
           }
 #pragma unroll
           for (int b = 0; b < 32; ++b) v[b] = hd_ex2(v[b]);
-          sum[c] += hq_across(v, [](float x, float y) { return x + y; });
+          const float block = hq_across(v, [](float x, float y) { return x + y; });
+          sum[c] += block;
+          if (block > best[c * 32 + lane]) {
+            best[c * 32 + lane] = block;
+            best_at[c * 32 + lane] = id0;
+          }
         }
       }
       tc_fence_before();
@@ -473,22 +486,31 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
   // The four warps' parts, in their order.
   if (threadIdx.x < a.T) {
     const int t = threadIdx.x;
-    float mx = -INFINITY, sum = 0.f;
-    int top = 0x7fffffff;
+    float mx = -INFINITY, sum = 0.f, best = 0.f;
+    int top = 0x7fffffff, at = 0;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float m = sm_m[q * 32 * NT + t], s = sm_sum[q * 32 * NT + t];
       const int p = sm_top[q * 32 * NT + t];
+      float b = sm_best[q * 32 * NT + t];
       if (m > mx) {
-        sum = sum * hd_ex2((mx - m) * HD_LOG2E) + s;
+        const float down = hd_ex2((mx - m) * HD_LOG2E);
+        sum = sum * down + s;
+        best *= down;
         mx = m;
         top = p;
       } else {
-        sum += m == -INFINITY ? s : s * hd_ex2((m - mx) * HD_LOG2E);
+        const float down = m == -INFINITY ? 1.f : hd_ex2((m - mx) * HD_LOG2E);
+        sum += s * down;
+        b *= down;
         if (m == mx && p < top) top = p;
       }
+      if (b > best) {
+        best = b;
+        at = sm_at[q * 32 * NT + t];
+      }
     }
-    if (hd_ok(blockIdx.x < a.out.parts, 23)) a.out.part[(size_t)t * a.out.parts + blockIdx.x] = make_float2(mx, sum);
+    if (hd_ok(blockIdx.x < a.out.parts, 23)) a.out.part[(size_t)t * a.out.parts + blockIdx.x] = make_float4(mx, sum, best, __int_as_float(at));
     if (a.out.top) a.out.top[(size_t)t * a.out.parts + blockIdx.x] = top;
   }
 }
@@ -520,7 +542,7 @@ static size_t hq_layout(int T, int H, HqArgs* a) {
   a->N = (T + 15) / 16 * 16;
   a->kb = H / 64;
   const int slots = NT == 4 ? HQ_SLOTS<4> : HQ_SLOTS<1>;
-  const size_t fixed = 1024 + (size_t)16 * 32 * NT * 4 + 38 * 8 + 32 + (size_t)2 * slots * a->N * 128;
+  const size_t fixed = 1024 + (size_t)24 * 32 * NT * 4 + 38 * 8 + 32 + (size_t)2 * slots * a->N * 128;
   for (a->ws = 8; a->ws > 4 && fixed + (size_t)a->ws * HQ_W_BYTES > HQ_SMEM_MAX; a->ws -= 2) {
   }
   return fixed + (size_t)a->ws * HQ_W_BYTES;
