@@ -784,9 +784,9 @@ __device__ __forceinline__ HdStat hd_merge(const HdStat& a, const HdStat& b) {
 // products make is 1e-5 too small, more than all other errors together (loss off by 1.5e-6 in the 2-norm
 // against 64 bits, 3e-7 with an fp32 product). The logits of targets with an eighth or more of the token's
 // weight, eight at most, are therefore summed again here, in fp32 rounded to nearest, and take their first
-// value's place in lse too. A warp sums one target's; all work side by side. So are, for lse's sake, the
-// 32 ids around a logit that has a fourth of the softmax or more, unless a target among them is nearly all of it: lse of
-// a token without a target was off by up to 2.3e-6 of itself.
+// value's place in lse too. A warp sums one target's; all work side by side. So are, for lse's
+// sake, the 32 ids around a logit that has a fourth of the softmax or more, unless a target among them is nearly all of
+// it: lse of a token without a target was off by up to 2.3e-6 of itself.
 template <bool QUANT>
 __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const __nv_bfloat16* __restrict__ x,
                                                              long long ldx, int H, HdHead w,

@@ -510,7 +510,8 @@ __global__ void __launch_bounds__(HQ_THREADS, 1)
         at = sm_at[q * 32 * NT + t];
       }
     }
-    if (hd_ok(blockIdx.x < a.out.parts, 23)) a.out.part[(size_t)t * a.out.parts + blockIdx.x] = make_float4(mx, sum, best, __int_as_float(at));
+    if (hd_ok(blockIdx.x < a.out.parts, 23))
+      a.out.part[(size_t)t * a.out.parts + blockIdx.x] = make_float4(mx, sum, best, __int_as_float(at));
     if (a.out.top) a.out.top[(size_t)t * a.out.parts + blockIdx.x] = top;
   }
 }
