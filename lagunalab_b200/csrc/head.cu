@@ -884,17 +884,19 @@ __global__ void __launch_bounds__(HJ_THREADS) hd_join_kernel(HdParts in, const _
     const int v = __shfl_sync(0xffffffffu, j < 32 ? id[0] : id[1], j & 31);
     const float was = __shfl_sync(0xffffffffu, j < 32 ? z[0] : z[1], j & 31), now = sh_dot[n];
     if (!near || (unsigned)v - (unsigned)st.at >= 32u)
-      st.sum += hd_ex2((now - st.mx) * HD_LOG2E) - hd_ex2((was - st.mx) * HD_LOG2E);
+      st.sum += hd_ex2((now - st.mx) * HD_LOG2E) - hd_ex2(fmaf(was, HD_LOG2E, -st.mx * HD_LOG2E));
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       if (id[i] == v) z[i] = now;  // every place of the list that names it
     todo &= ~hd_same(id, v);
   }
-  const float lse = st.mx + logf(st.sum);
+  // Neither loss nor what is taken off above has the roundings of large logits: the loss does not go through lse, and a
+  // term of the sum is taken off as it was put on (its argument's rounding is 2^-24 of the logit).
+  const float log_sum = logf(st.sum), lse = st.mx + log_sum;
   float l = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    if (id[i] >= 0) l += wt[i] * (lse - z[i]);
+    if (id[i] >= 0) l += wt[i] * ((st.mx - z[i]) + log_sum);
   l = warp_sum(l);
   bad = __any_sync(0xffffffffu, bad);
   if (lane == 0) {
