@@ -684,7 +684,8 @@ int lg_head_loss(const void* x, long long ldx, int T, int H, const void* w, long
  *   weights' sum,  dx = dz w (bf16 [T, H]),  dw = dz^T x (bf16 [V, H]).
  * dx or dw may be NULL (not both); a 4-bit head has no dw. A token without a target adds nothing to dw
  * and gives a row of zeros in dx, whatever its row of x holds; an id >= V counts as left out. dz is
- * rounded to bf16 for the tensor cores (2^-8 relative at most) without the factor max |g weights|, sums are fp32.
+ * rounded to bf16 for the tensor cores (2^-8 relative at most, with up to 64 tokens 2^-18) without the factor
+ * max |g weights|, sums are fp32.
  * A target that carries an eighth or more of its token's weight has its logit from the same fp32 sum as in lse:
  * its S p - w is then off by lse's own rounding at most, also where it is nearly 0.
  * The workspace holds up to 512 MB of dz (256 ids a token at least: more from 2^20 tokens on), up to 512 MB of a 4-bit

@@ -19,6 +19,8 @@
 // dx and dW are multiplied by c before they are rounded, once, at the end. So the usual g (1/n for every token)
 // and weight leave S exp(z - lse) - 1, whose -1 is exact; as -g it was off by up to 2^-8, in all tokens by the
 // same, and dx and dW with it. The other errors are independent: sums over the vocabulary or the tokens average them.
+// Up to 64 tokens average little (errors up to 1.8 times those of the results' own rounding), and their products cost
+// the reading of W: dz is then kept in two rows a token, its rounding and what that left (hd_rest).
 // z is the tensor cores' sum, which is cut after each step, but for targets that carry an eighth or more of their
 // token's weight: loss and gradient take both their logits from one fp32 sum (hd_dot), since a target's S p - w of
 // nearly 0 has all of z's error, and lse's with the other sign: what is left of it is lse's own rounding. For lse
@@ -80,7 +82,8 @@ struct HdArgs {
   // not HD_LOSS: bf16 [M, width], HD_XGRAD and parts of HD_WGRAD: fp32 [splits, M, width]
   void* tile_out;
   int width;
-  int add;  // HD_XGRAD: 0 for the first piece
+  int add;   // HD_XGRAD: 0 for the first piece
+  int rest;  // HD_PROB: rows from a token's dz to what its rounding left; 0: that is not kept
 };
 
 // K > 1: what a token's weights are multiplied with, and its g divided by, by its largest weight. g / c is at most
@@ -187,10 +190,11 @@ __device__ __forceinline__ HdRow hd_row(const HdArgs& a, const HdUnit& u, int t)
 // a row each, a tile of dW took 8,500 cycles and dx's addition 16 us of 66; stored by TMA, a box waits for
 // 2,000 to 5,000 cycles behind the loads that are queued there.
 //
-// This thread's 128 bytes of a box: rows y ... of the output's `rows`, from its column x (of a.width) on.
+// This thread's 128 bytes of a box: rows y ... of the product, `down` further in the output, from its column x (of
+// a.width) on.
 template <int KIND>
 __device__ __forceinline__ void hd_box(const HdArgs& a, uint8_t* box, const uint32_t (&r)[32], int x, int y,
-                                       int split) {
+                                       int split, int down = 0) {
   constexpr int PER = KIND == HD_XGRAD ? 4 : 8;  // elements in 16 bytes
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -213,7 +217,7 @@ __device__ __forceinline__ void hd_box(const HdArgs& a, uint8_t* box, const uint
       else
         *reinterpret_cast<uint4*>(out) = v;
     } else {
-      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.tile_out) + (size_t)(y + row) * a.width + col) = v;
+      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.tile_out) + (size_t)(down + y + row) * a.width + col) = v;
     }
   }
   __syncwarp();  // the box is free, and a tcgen05.ld of the whole warp may follow
@@ -301,44 +305,53 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, const HdUnit& u, in
     const float scale = KIND == HD_WGRAD ? *a.scale : 1.f;
 #pragma unroll 1
     for (int c = begin; c < begin + COLS && n0 + c < a.width; c += 64) {
-      uint32_t r[32];
+      const HdRow start = row;
+#pragma unroll 1
+      for (int left = 0; left <= (KIND == HD_PROB && a.rest ? 1 : 0); ++left) {
+        if (KIND == HD_PROB) row = start;
+        uint32_t r[32];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) {
+          __syncwarp();
+          if (ok) tmem_ld32_wait(taddr + c + 32 * h, v);
+          if (KIND == HD_PROB) {
+            const int id0 = a.v0 + n0 + c + 32 * h;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = ok ? row.gs * hd_ex2(fmaf(v[i], HD_LOG2E, row.off)) : nan;
+            // K > 1: of the tile's ids in order, those of the other half of the columns only pass by
+            while (a.K > 1 ? row.next >= 0 && row.next < id0 + 32 : (unsigned)row.next - (unsigned)id0 < 32u) {
+              if (a.K == 1) {
+                hd_target(v, row.next - id0, row.gs, row.gs, row.again);
+                break;
+              }
+              if (row.next >= id0) hd_target(v, row.next - id0, row.gg * row.w, row.gs, row.again);
+              const size_t at = (size_t)t * a.K + ++row.p;
+              row.next = -1;
+              if (row.p < row.p1) {
+                row.next = a.ids[at];
+                row.w = a.weights[at];
+                row.again = a.again[at];
+              }
+            }
+            if (!row.counts) {  // a token without a target: nothing of it, whatever its row holds
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = 0.f;
+            }
+          }
+          if (KIND == HD_WGRAD) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= scale;
+          }
+          if (KIND == HD_PROB && left) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] -= __bfloat162float(__float2bfloat16_rn(v[i]));
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) r[16 * h + i] = hd_pack(v[2 * i], v[2 * i + 1]);
+        }
         __syncwarp();
-        if (ok) tmem_ld32_wait(taddr + c + 32 * h, v);
-        if (KIND == HD_PROB) {
-          const int id0 = a.v0 + n0 + c + 32 * h;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = ok ? row.gs * hd_ex2(fmaf(v[i], HD_LOG2E, row.off)) : nan;
-          // K > 1: of the tile's ids in order, those of the other half of the columns only pass by
-          while (a.K > 1 ? row.next >= 0 && row.next < id0 + 32 : (unsigned)row.next - (unsigned)id0 < 32u) {
-            if (a.K == 1) {
-              hd_target(v, row.next - id0, row.gs, row.gs, row.again);
-              break;
-            }
-            if (row.next >= id0) hd_target(v, row.next - id0, row.gg * row.w, row.gs, row.again);
-            const size_t at = (size_t)t * a.K + ++row.p;
-            row.next = -1;
-            if (row.p < row.p1) {
-              row.next = a.ids[at];
-              row.w = a.weights[at];
-              row.again = a.again[at];
-            }
-          }
-          if (!row.counts) {  // a token without a target: nothing of it, whatever its row holds
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.f;
-          }
-        }
-        if (KIND == HD_WGRAD) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] *= scale;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) r[16 * h + i] = hd_pack(v[2 * i], v[2 * i + 1]);
+        hd_box<KIND>(a, box, r, n0 + c, y, 0, left * a.rest);
       }
-      __syncwarp();
-      hd_box<KIND>(a, box, r, n0 + c, y, 0);
     }
   }
 }
@@ -989,9 +1002,9 @@ __device__ __forceinline__ void hd_again(const HdScale& a, int block) {
 }
 
 // Blocks [0, a.blocks()): as HdScale says. The others, for dW: x with the rows of tokens without a target at 0, so
-// that dW has nothing of them (0 * NaN is NaN).
+// that dW has nothing of them (0 * NaN is NaN); `rest` rows further once more, for the second rows of dz.
 __global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int H,
-                                                      const HdScale a, __nv_bfloat16* __restrict__ out) {
+                                                      const HdScale a, int rest, __nv_bfloat16* __restrict__ out) {
   const int first = a.blocks();
   if ((int)blockIdx.x < first) {
     if (blockIdx.x == 0)
@@ -1008,6 +1021,7 @@ __global__ void __launch_bounds__(256) hd_rows_kernel(const __nv_bfloat16* __res
     if (!hd_ok(t >= 0 && t < a.T && c + 8 <= H, 12)) continue;
     if (hd_counts(a, t)) v = *reinterpret_cast<const uint4*>(x + (size_t)t * ldx + c);
     *reinterpret_cast<uint4*>(out + (size_t)t * H + c) = v;
+    if (rest) *reinterpret_cast<uint4*>(out + (size_t)(rest + t) * H + c) = v;
   }
 }
 
@@ -1076,6 +1090,10 @@ constexpr long long HD_DZ_BYTES = 512LL << 20;
 // few tokens: the launches cost more (37 tokens, dx of 100,352 ids: 388 us with 32 MB, 276 with 64, 234 with 256, 229
 // with 512).
 constexpr long long HD_WQ_BYTES = 512LL << 20;
+
+// Rows of dz that hold what the rounding of T tokens' rows left. Up to 64 tokens: both are one tile of rows of dx's
+// product (100,352 ids of 2,048: dx of 37 tokens 155 us instead of 145, of 128 tokens it would be 176 instead of 157).
+static int hd_rest(int T) { return T <= HD_BM / 2 ? T : 0; }
 
 static int hd_cg(int rows) { return rows > HD_BM ? 2 : 1; }
 static long long hd_rounds(long long units, int cg) {
@@ -1183,7 +1201,7 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
   HdWork w = {};
   Carver c(base);
   w.nt = (V + HD_BN - 1) / HD_BN;
-  w.piece = hd_piece(T, H, V, quant, grad, dw);
+  w.piece = hd_piece(grad ? T + hd_rest(T) : T, H, V, quant, grad, dw);
   if (!grad) {
     w.out.parts = few ? hq_parts(V) : w.nt;
     w.out.maxima = !few;
@@ -1208,15 +1226,16 @@ static HdWork hd_carve(void* base, int T, int H, int V, int K, bool quant, bool 
   if (grad) {
     w.scale = c.take<float>(1);
     w.again = c.take<float>((size_t)T * K);
-    w.dz = c.take<__nv_bfloat16>((size_t)T * w.piece);
+    const int rows = T + hd_rest(T);
+    w.dz = c.take<__nv_bfloat16>((size_t)rows * w.piece);
     if (dw) {
-      w.xz = c.take<__nv_bfloat16>((size_t)T * H);
-      w.wsplits = hd_wsplits(T, H, std::min(w.piece, V));
+      w.xz = c.take<__nv_bfloat16>((size_t)rows * H);
+      w.wsplits = hd_wsplits(rows, H, std::min(w.piece, V));
       if (w.wsplits > 1) w.dw = c.take<float>((size_t)w.wsplits * std::min(w.piece, V) * H);
     }
     if (dx) {
-      w.splits = hd_splits(T, H, std::min(w.piece, V));
-      w.dx = c.take<float>((size_t)w.splits * T * H);
+      w.splits = hd_splits(rows, H, std::min(w.piece, V));
+      w.dx = c.take<float>((size_t)w.splits * rows * H);
     }
   }
   w.bytes = align_up(c.used, 256);
@@ -1444,9 +1463,10 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
                          static_cast<const __nv_bfloat16*>(x), ldx, H, K, head, lse, k.again};
   if (!quant) {
     hd_rows_kernel<<<scale.blocks() + (dw ? hd_blocks((long long)T * (H / 8)) : 0), 256, 0, st>>>(
-        static_cast<const __nv_bfloat16*>(x), ldx, H, scale, k.xz);
+        static_cast<const __nv_bfloat16*>(x), ldx, H, scale, hd_rest(T), k.xz);
     LG_LAUNCH_CHECK("head_rows");
   }
+  const int rest = hd_rest(T), rows = T + rest;
   for (int v0 = 0; v0 < V; v0 += k.piece) {
     const int n = std::min(k.piece, V - v0);
     HD_TRY(hd_weights(w, w_scales, w_biases, H, v0, n, k, v0 == 0 ? scale : HdScale{}, st));
@@ -1464,10 +1484,12 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
     const int ldz = (n + 63) / 64 * 64;
     a.tile_out = k.dz;
     a.width = ldz;
+    a.rest = rest;
     HD_TRY(hd_launch<HD_PROB>({x, H, T, ldx}, mw, a, st));
-    const HdOperand mz = {k.dz, n, T, ldz};
+    const HdOperand mz = {k.dz, n, rows, ldz};
     if (dx) {
       HdArgs b = a;
+      b.M = rows;
       b.N = H;
       b.kblocks = (n + HD_BK - 1) / HD_BK;
       b.splits = std::min(k.splits, b.kblocks);
@@ -1480,18 +1502,18 @@ extern "C" int lg_head_loss_grad(const void* x, long long ldx, int T, int H, con
       HdArgs b = a;
       b.M = n;
       b.N = H;
-      b.kblocks = (T + HD_BK - 1) / HD_BK;
+      b.kblocks = (rows + HD_BK - 1) / HD_BK;
       b.splits = k.wsplits;
-      __nv_bfloat16* rows = static_cast<__nv_bfloat16*>(dw) + (size_t)v0 * H;
-      b.tile_out = k.wsplits > 1 ? static_cast<void*>(k.dw) : rows;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(dw) + (size_t)v0 * H;
+      b.tile_out = k.wsplits > 1 ? static_cast<void*>(k.dw) : out;
       b.width = H;
-      HD_TRY(hd_launch<HD_WGRAD>(mz, {k.xz, H, T, H}, b, st));
-      if (k.wsplits > 1) HD_TRY(hd_join_parts(k.dw, k.wsplits, (long long)n * H, k.scale, rows, st));
+      HD_TRY(hd_launch<HD_WGRAD>(mz, {k.xz, H, rows, H}, b, st));
+      if (k.wsplits > 1) HD_TRY(hd_join_parts(k.dw, k.wsplits, (long long)n * H, k.scale, out, st));
     }
   }
   if (dx) {
     // The last piece may have fewer parts than the first; later parts then kept the earlier sums.
-    const int parts = std::min(k.splits, (std::min(k.piece, V) + HD_BK - 1) / HD_BK);
+    const int parts = std::min(k.splits, (std::min(k.piece, V) + HD_BK - 1) / HD_BK) * (rest ? 2 : 1);
     HD_TRY(hd_join_parts(k.dx, parts, (long long)T * H, k.scale, dx, st));
   }
   return LG_OK;

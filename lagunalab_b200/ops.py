@@ -1024,8 +1024,8 @@ def head_loss_grad(x, head, ids, lse, g, weights=None, dx=True, dw=True):
     the logits' gradient (256 ids a token at least: more from 2^20 tokens on) and of a 4-bit head's weights, and
     fp32 parts of dx (up to eight, or 20 MB). Ids that are negative or >= V are left out; tokens
     without any other give a row of zeros in dx and nothing to dw, whatever their rows of x hold. The
-    logits' gradient, without the factor that all tokens share, is rounded to bf16 for the tensor cores;
-    sums are fp32, results rounded once."""
+    logits' gradient, without the factor that all tokens share, is rounded to bf16 for the tensor cores (with up to
+    64 tokens, what that leaves is kept as well); sums are fp32, results rounded once."""
     index, sizes, args, keep = _head_args("head_loss_grad", x, head, ids, weights)
     T, H, V, _, bits = sizes
     if not (dx or dw):
